@@ -1,0 +1,197 @@
+"""Key/value cache in 4 bits for requests of unequal lengths: pages of 64 slots that a stack of free ones gives out on the GPU, keys and values rounded
+by groups of a head's dimensions as they are appended, and softmax attention that reads the codes.
+
+A serving step, per layer after the first two lines:
+
+    cache = PagedCache4(n_layer, n_head, head_size, pages=..., requests=..., max_length=...)
+    plan = cache.plan(rows, counts, tokens)            # which slots the step's tokens get: request rows[i] brings counts[i] of the `tokens` rows
+    q = cache.append(layer, plan, q, k, v, rope=table) # rows [tokens, heads, head_size]; turns queries and keys where a table is given
+    y = cache.attend(layer, plan, q)                   # every token over its request's keys at and before its position
+    cache.truncate(rows, lengths)                      # afterwards: drafts that were rejected; length 0 ends a request
+
+Nothing looks at lengths on the host, so that a captured step serves requests of any lengths.  A group of values x is held as
+
+    lo = min(x),  s = T((max(x) - lo) * (1/15)),  code = min(max(rint((x - lo) / s), 0), 15) in fp32,       standing for code * s + lo
+
+with s and lo in the cache's type T: the smallest value is exact, and the error of the others is half of s at most, and s/15 2^-8 (bf16) or 2^-11 (fp16) of
+the group's range more at its upper end, where the rounding of s may leave 15 s short of it.
+"""
+from __future__ import annotations
+
+from typing import Optional, Sequence, Tuple, Union
+
+import torch
+
+from . import _native as N
+
+Whole = Union[torch.Tensor, Sequence[int]]
+
+REASONS = {1: "there are not enough free pages", 2: "it would be longer than it may be, or brings more tokens than the plan's max_count",
+           3: "there is no such request, or an earlier sequence names it, or its count is negative", 4: "its tokens lie behind the step's rows"}
+
+
+class CachePlan:
+    """A step's place in the cache, as int32 tensors on the GPU: ``starts [B + 1]`` first row of every sequence, ``ends [B]`` tokens held after the step (0:
+    refused), ``status [B]`` (0, or why a sequence got nothing: ``REASONS``), ``positions [T]`` and ``slots [T]`` (page * 64 + place in it) of the
+    tokens, -1 for those of refused sequences and behind the last one."""
+
+    def __init__(self, cache: "PagedCache4", B: int, T: int, max_count: int):
+        self.cache, self.B, self.T, self.max_count, self.step = cache, B, T, max_count, cache._step
+        self.data = torch.empty(4 * B + 1 + 3 * T, dtype=torch.int32, device=cache.device)
+        self.starts, self.ends, self.status, self.request, self.positions, self.slots, self.sequence = self.data.split([B + 1, B, B, B, T, T, T])
+
+    def check(self) -> None:
+        """Raise if a sequence was refused.  Waits for the GPU."""
+        for i, s in enumerate(self.status.tolist()):
+            if s:
+                raise RuntimeError(f"sequence {i} of the step was refused: {REASONS[s]}")
+
+
+class PagedCache4:
+    PAGE = 64
+
+    def __init__(self, n_layer: int, n_head: int, head_size: int, *, n_kv_head: Optional[int] = None, pages: int, requests: int, max_length: int,
+                 group: int = 64, dtype: torch.dtype = torch.bfloat16, device="cuda"):
+        """``pages`` of 64 slots for up to ``requests`` requests of up to ``max_length`` tokens; heads of 32, 64 or 128, codes by ``group``s of 32, 64 or 128
+        of their dimensions.  ``n_kv_head`` key/value heads serve ``n_head`` query heads, neighbours the same one."""
+        n_kv_head = n_head if n_kv_head is None else n_kv_head
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise RuntimeError(f"the paged cache lives on CUDA (sm_100a) only, not on {device}")
+        if dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError(f"a paged cache of {dtype} (torch.bfloat16 or torch.float16)")
+        page_bytes = N.call_ret("ll_kv4_page_bytes", head_size, group)
+        if page_bytes == 0:
+            raise ValueError(f"heads of {head_size} in groups of {group}: 32, 64 or 128 each, and no group larger than a head")
+        if n_layer < 1 or n_kv_head < 1 or n_head % n_kv_head != 0 or n_head < 1:
+            raise ValueError(f"{n_layer} layers of {n_head} heads over {n_kv_head}")
+        if min(pages, requests, max_length) < 1 or pages * self.PAGE > 2**31 - 1:
+            raise ValueError(f"{pages} pages of {self.PAGE} slots for {requests} requests of up to {max_length} tokens")
+        self.device = torch.device("cuda", torch.cuda.current_device() if device.index is None else device.index)
+        self.n_layer, self.n_head, self.n_kv_head, self.head_size, self.group, self.dtype = n_layer, n_head, n_kv_head, head_size, group, dtype
+        self.pages, self.requests, self.max_length, self.width = pages, requests, max_length, -(-max_length // self.PAGE)
+        i32 = dict(dtype=torch.int32, device=self.device)
+        self.blocks = torch.zeros((n_layer, pages, n_kv_head, page_bytes), dtype=torch.uint8, device=self.device)
+        self.table = torch.full((requests, self.width), -1, **i32)
+        self.lengths = torch.zeros(requests, **i32)
+        self.free = torch.arange(pages - 1, -1, -1, **i32)
+        self.n_free = torch.full((1,), pages, **i32)
+        self._stamp = torch.zeros(requests, **i32)
+        self._pool = [N.ptr(t) for t in (self.table, self.lengths, self.free, self.n_free, self._stamp)] + [requests, self.width, pages, max_length]
+        self._layers = [N.ptr_at(self.blocks, i * self.blocks.stride(0)) for i in range(n_layer)]
+        self._code = N.dtype_code(dtype)
+        self._step = 0
+
+    # ------------------------------------------------------------------ pages and slots
+    def _whole(self, name: str, x: Whole) -> torch.Tensor:
+        if not isinstance(x, torch.Tensor):
+            x = torch.tensor(list(x), dtype=torch.int32, device=self.device)
+        if x.dim() != 1 or x.dtype != torch.int32 or x.device != self.device:
+            raise RuntimeError(f"{name}: int32 numbers on {self.device}, one for each sequence, not {x.dtype} {tuple(x.shape)} on {x.device}")
+        return x.contiguous()
+
+    def plan(self, rows: Whole, counts: Whole, tokens: int, *, max_count: Optional[int] = None) -> CachePlan:
+        """Give the step's ``tokens`` rows their slots: the next ``counts[i]`` of them are sequence i's, the continuation of request ``rows[i]``.  A sequence
+        may bring nothing; one that cannot be served is refused whole (``CachePlan.status``), its tokens get no slot and come out of ``append`` and
+        ``attend`` as no numbers.  ``max_count``: the most that a sequence brings (``tokens`` unless said); it goes into the choice of kernels.
+        Plans of earlier steps end with this one."""
+        rows, counts = self._whole("rows", rows), self._whole("counts", counts)
+        if rows.shape != counts.shape or rows.numel() == 0:
+            raise RuntimeError(f"{rows.numel()} requests and {counts.numel()} counts")
+        max_count = tokens if max_count is None else max_count
+        if not 0 <= max_count or not 0 <= tokens < 2**31 // max(1, self.n_head):
+            raise RuntimeError(f"a step of {tokens} tokens, {max_count} at most of a sequence")
+        with torch.cuda.device(self.device):
+            self._step += 1
+            plan = CachePlan(self, rows.numel(), tokens, min(max_count, tokens))
+            N.call("ll_kv4_plan", N.ptr(rows), N.ptr(counts), plan.B, tokens, plan.max_count, *self._pool, N.ptr(plan.data), N.stream())
+        return plan
+
+    def truncate(self, rows: Whole, lengths: Whole) -> None:
+        """Cut request ``rows[i]`` to its first ``lengths[i]`` tokens (0 ends it); pages that it no longer needs are free again.  Requests that are not longer
+        stay as they are."""
+        rows, lengths = self._whole("rows", rows), self._whole("lengths", lengths)
+        if rows.shape != lengths.shape or rows.numel() == 0:
+            raise RuntimeError(f"{rows.numel()} requests and {lengths.numel()} lengths")
+        with torch.cuda.device(self.device):
+            self._step += 1
+            N.call("ll_kv4_truncate", N.ptr(rows), N.ptr(lengths), rows.numel(), *self._pool, N.stream())
+
+    def reset(self) -> None:
+        """All requests end, and pages are given out as in the beginning."""
+        self._step += 1
+        self.table.fill_(-1)
+        self.lengths.zero_()
+        torch.arange(self.pages - 1, -1, -1, out=self.free)
+        self.n_free.fill_(self.pages)
+
+    # ------------------------------------------------------------------ a layer
+    def _check(self, layer: int, plan: CachePlan) -> None:
+        if not 0 <= layer < self.n_layer:
+            raise RuntimeError(f"layer {layer} of {self.n_layer}")
+        if plan.cache is not self or plan.step != self._step:
+            raise RuntimeError("the plan is another cache's, or of a step before this cache's last plan or truncation")
+
+    def _rows(self, name: str, x: torch.Tensor, T: int, heads: int) -> torch.Tensor:
+        """Rows as the kernels take them: the heads of a token one after the other, tokens at any distance, 16-byte boundaries."""
+        if x.shape != (T, heads, self.head_size) or x.dtype != self.dtype or x.device != self.device:
+            raise RuntimeError(f"{name}: {x.dtype} {tuple(x.shape)} on {x.device}, and the cache takes {self.dtype} {(T, heads, self.head_size)} on {self.device}")
+        if torch.is_grad_enabled() and x.requires_grad:
+            raise RuntimeError(f"{name}: the 4-bit cache has no gradient")
+        if x.stride(2) != 1 or (heads > 1 and x.stride(1) != self.head_size) or (T > 1 and (x.stride(0) % 8 != 0 or x.stride(0) < heads * self.head_size)) or x.data_ptr() % 16 != 0:
+            x = x.clone(memory_format=torch.contiguous_format)
+        return x
+
+    def append(self, layer: int, plan: CachePlan, q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, rope: Optional[torch.Tensor] = None):
+        """Round the step's keys and values ``[tokens, n_kv_head, head_size]`` into their slots.  With ``rope`` (fp32 ``[positions, head_size / 2, 2]``, as
+        ``build_rope_cache``'s) keys are turned before, and queries ``[tokens, n_head, head_size]`` as well; returns the queries."""
+        self._check(layer, plan)
+        T = plan.T
+        k, v = self._rows("k", k, T, self.n_kv_head), self._rows("v", v, T, self.n_kv_head)
+        out = q
+        if rope is not None:
+            if q is None:
+                raise RuntimeError("queries have to be turned with their keys")
+            q = self._rows("q", q, T, self.n_head)
+            if rope.dtype != torch.float32 or rope.dim() != 3 or rope.shape[1:] != (self.head_size // 2, 2) or not rope.is_contiguous() \
+                    or rope.device != self.device or rope.data_ptr() % 16 != 0:
+                raise RuntimeError(f"rope: {rope.dtype} {tuple(rope.shape)} on {rope.device}, and the cache takes dense float32 [positions, {self.head_size // 2}, 2]")
+            if rope.shape[0] < self.max_length:
+                raise RuntimeError(f"rope: {rope.shape[0]} positions, and requests may have {self.max_length}")
+            out = torch.empty((T, self.n_head, self.head_size), dtype=self.dtype, device=self.device)
+        if T == 0:
+            return out
+        with torch.cuda.device(self.device):
+            N.call("ll_kv4_append", N.ptr(q) if rope is not None else None, q.stride(0) if rope is not None else 0, N.ptr(k), k.stride(0), N.ptr(v), v.stride(0),
+                   N.ptr(rope), N.ptr(plan.positions), N.ptr(plan.slots), N.ptr(out) if rope is not None else None, self._layers[layer], self._code, T,
+                   self.n_head, self.n_kv_head, self.head_size, self.group, N.stream())
+        return out
+
+    def read(self, layer: int, slots: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+        """What the cache holds at ``slots`` (a plan's, or any): keys and values ``[n, n_kv_head, head_size]``, no numbers for slots that there are not."""
+        if not 0 <= layer < self.n_layer:
+            raise RuntimeError(f"layer {layer} of {self.n_layer}")
+        slots = self._whole("slots", slots)
+        k, v = torch.empty((2, slots.numel(), self.n_kv_head, self.head_size), dtype=self.dtype, device=self.device).unbind(0)
+        if slots.numel():
+            with torch.cuda.device(self.device):
+                N.call("ll_kv4_read", self._layers[layer], N.ptr(slots), N.ptr(k), N.ptr(v), self._code, slots.numel(), self.n_kv_head, self.head_size, self.group,
+                       self.pages, N.stream())
+        return k, v
+
+    def attend(self, layer: int, plan: CachePlan, q: torch.Tensor, scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Softmax attention of the step's queries ``[tokens, n_head, head_size]`` over what their requests hold up to their positions; the tokens' own keys
+        have to be appended before.  ``scale`` of the scores: 1 / sqrt(head_size) unless given.  Rows of ``out`` behind the last token stay as they are."""
+        self._check(layer, plan)
+        T = plan.T
+        q = self._rows("q", q, T, self.n_head)
+        if out is None:
+            out = torch.empty((T, self.n_head, self.head_size), dtype=self.dtype, device=self.device)
+        elif out.shape != q.shape or out.dtype != self.dtype or out.device != self.device or not out.is_contiguous() or out.data_ptr() % 16 != 0:
+            raise RuntimeError(f"out: dense {self.dtype} {tuple(q.shape)} on {self.device}, not {out.dtype} {tuple(out.shape)} on {out.device}")
+        if T == 0:
+            return out
+        with torch.cuda.device(self.device):
+            N.call("ll_kv4_attn", N.ptr(q), q.stride(0), self._layers[layer], N.ptr(self.table), N.ptr(plan.data), N.ptr(out), self._code, plan.B, T, self.n_head,
+                   self.n_kv_head, self.head_size, self.group, self.width, self.pages, self.head_size ** -0.5 if scale is None else float(scale), N.stream())
+        return out

@@ -1,0 +1,93 @@
+"""What the paged 4-bit cache refuses before anything reaches a GPU, and the host's restatement that the GPU tests compare with."""
+import random
+
+import pytest
+import torch
+
+from lit_llama import _native as N
+from lit_llama.paged_cache import PagedCache4
+from tests.util_paged import PAGE, Pool, held_as
+
+ONE = dict(pages=4, requests=2, max_length=100)
+
+
+@pytest.mark.parametrize("args, kind, error", [
+    ((1, 4, 64), dict(ONE, device="cpu"), RuntimeError),
+    ((1, 4, 64), dict(ONE, dtype=torch.float32), ValueError),
+    ((1, 4, 48), ONE, ValueError),
+    ((1, 4, 256), ONE, ValueError),
+    ((1, 4, 64), dict(ONE, group=128), ValueError),
+    ((1, 4, 64), dict(ONE, group=16), ValueError),
+    ((1, 4, 64), dict(ONE, n_kv_head=3), ValueError),
+    ((0, 4, 64), ONE, ValueError),
+    ((1, 4, 64), dict(ONE, pages=0), ValueError),
+    ((1, 4, 64), dict(ONE, requests=0), ValueError),
+    ((1, 4, 64), dict(ONE, max_length=0), ValueError),
+    ((1, 4, 64), dict(ONE, pages=1 << 25), ValueError),
+])
+def test_refused_shapes(args, kind, error):
+    with pytest.raises(error):
+        PagedCache4(*args, **kind)
+
+
+A = 1 << 12      # an address that no launch reads
+
+
+@pytest.mark.parametrize("name, args", [
+    ("ll_kv4_plan", (0, A, 1, 1, 1, A, A, A, A, A, 1, 1, 1, 64, A, 0)),
+    ("ll_kv4_plan", (A, A, 0, 1, 1, A, A, A, A, A, 1, 1, 1, 64, A, 0)),
+    ("ll_kv4_plan", (A, A, 1, -1, 1, A, A, A, A, A, 1, 1, 1, 64, A, 0)),
+    ("ll_kv4_plan", (A, A, 1, 1, 1, A, A, A, A, A, 1, 1, 1, 65, A, 0)),           # a table too narrow for the longest request
+    ("ll_kv4_truncate", (A, 0, 1, A, A, A, A, A, 1, 1, 1, 64, 0)),
+    ("ll_kv4_append", (0, 0, A, 64, A, 64, 0, A, A, 0, A, 0, 1, 1, 1, 64, 64, 0)),     # fp32
+    ("ll_kv4_append", (0, 0, A, 64, A, 64, 0, A, A, 0, A, 1, 1, 1, 1, 64, 48, 0)),     # groups of 48
+    ("ll_kv4_append", (0, 0, A + 2, 64, A, 64, 0, A, A, 0, A, 1, 1, 1, 1, 64, 64, 0)),   # keys off a 16-byte boundary
+    ("ll_kv4_append", (0, 0, A, 65, A, 64, 0, A, A, 0, A, 1, 1, 1, 1, 64, 64, 0)),
+    ("ll_kv4_append", (0, 0, A, 64, A, 64, A, A, A, A, A, 1, 1, 1, 1, 64, 64, 0)),     # a table and no queries
+    ("ll_kv4_read", (A, A, A, A, 1, 0, 1, 64, 64, 1, 0)),
+    ("ll_kv4_attn", (A, 64, A, A, A, A, 1, 1, 1, 3, 2, 64, 64, 1, 1, 1.0, 0)),         # three heads over two
+    ("ll_kv4_attn", (A, 64, A, A, A, A, 0, 1, 1, 2, 2, 64, 64, 1, 1, 1.0, 0)),         # fp32
+    ("ll_kv4_attn", (A, 60, A, A, A, A, 1, 1, 1, 2, 2, 64, 64, 1, 1, 1.0, 0)),
+])
+def test_refused_calls(name, args):
+    with pytest.raises(RuntimeError, match="kv4"):
+        N.call(name, *args)
+
+
+def test_page_bytes():
+    """A slot of a head: D / 2 bytes of key codes and as many of value codes, and four bytes a group of either."""
+    for D in (32, 64, 128):
+        for group in (32, 64, 128):
+            want = PAGE * (D + 8 * (D // group)) if group <= D else 0
+            assert N.call_ret("ll_kv4_page_bytes", D, group) == want
+    assert N.call_ret("ll_kv4_page_bytes", 96, 32) == 0
+
+
+def test_truncation_undoes_a_plan():
+    rng = random.Random(1)
+    pool = Pool(20, 60, 500)
+    for _ in range(50):
+        rows = rng.sample(range(20), 12)
+        before = ([list(t) for t in pool.table], list(pool.lengths), list(pool.free))
+        counts = [rng.choice([0, 1, 1, rng.randrange(200)]) for _ in rows]
+        first = pool.plan(rows, counts, sum(counts), 500)
+        pool.truncate(rows, [before[1][r] for r in rows])
+        assert before == (pool.table, pool.lengths, pool.free)
+        assert pool.plan(rows, counts, sum(counts), 500) == first
+        ended = rng.sample(range(20), 9)
+        pool.truncate(ended, [0] * 9)
+
+
+def test_rounding_is_half_a_step_at_most():
+    """Half a step, and at the upper end what 15 steps fall short of the range by (the scale is rounded, by half a place at most)."""
+    torch.manual_seed(0)
+    for dtype in (torch.bfloat16, torch.float16):
+        x = torch.randn(50, 3, 128).to(dtype)
+        for group in (32, 64, 128):
+            g = x.double().unflatten(-1, (-1, group))
+            span = g.amax(-1, keepdim=True) - g.amin(-1, keepdim=True)
+            off = (held_as(x, group) - x.double()).unflatten(-1, (-1, group)).abs()
+            half = torch.finfo(dtype).eps / 2
+            assert bool((off <= span / 15 * (1 + half) / 2 * (1 + 1e-6) + span * half).all())
+            low = held_as(x, group).unflatten(-1, (-1, group)).amin(-1)
+            assert torch.equal(low, g.amin(-1))
