@@ -1,9 +1,10 @@
 // Layout of the paged key/value cache in 4 bits (paged_kv4.cu writes it, paged_attn.cu reads it).
 //
-// A page holds 64 slots.  Of every page each key/value head has one run of bytes, so that a block that walks a head's keys copies a page at once:
-//   key codes    [64 slots][D / 2 bytes]       4 chunks (t) of W = D / 32 words a slot
-//   value codes  [32 pairs of slots][D bytes]  8 chunks (g) of W words a pair
-//   key parameters, then value parameters: [64 slots][D / group][scale, lowest value], in the cache's type
+// A page holds 64 slots.  Of every page each key/value head has one run of bytes: four slices of 16 slots, so that a warp that walks a head's keys
+// copies its slice of a page at once.  A slice:
+//   key codes    [16 slots][D / 2 bytes]      4 chunks (t) of W = D / 32 words a slot
+//   value codes  [8 pairs of slots][D bytes]  8 chunks (g) of W words a pair
+//   key parameters, then value parameters: [16 slots][D / group][scale, lowest value], in the cache's type
 // The codes lie as the operands of a 16 x 16 product want them (mma.sync m16n8k16, A by rows): one load gives a lane the words of all its tiles, and a
 // word's codes become pairs of numbers by masks alone:
 //   keys:   rows are slots.  Word i of chunk t holds the dimensions 32 i + 16 (n >> 1) + 4 t + 2 (n & 1) + e, the code of nibble n, half e at bit 16 e + 4 n
@@ -16,12 +17,13 @@
 namespace llb {
 namespace {
 
-constexpr int KV4_PAGE = 64;
+constexpr int KV4_PAGE = 64, KV4_SLICE = 16;
 
-__host__ __device__ constexpr int kv4_v_codes(int D) { return KV4_PAGE * D / 2; }
-__host__ __device__ constexpr int kv4_k_params(int D) { return KV4_PAGE * D; }
-__host__ __device__ constexpr int kv4_v_params(int D, int groups) { return KV4_PAGE * D + KV4_PAGE * groups * 4; }
-__host__ __device__ constexpr int kv4_bytes(int D, int groups) { return KV4_PAGE * D + 2 * KV4_PAGE * groups * 4; }
+__host__ __device__ constexpr int kv4_v_codes(int D) { return KV4_SLICE * D / 2; }
+__host__ __device__ constexpr int kv4_k_params(int D) { return KV4_SLICE * D; }
+__host__ __device__ constexpr int kv4_v_params(int D, int groups) { return KV4_SLICE * (D + 4 * groups); }
+__host__ __device__ constexpr int kv4_slice_bytes(int D, int groups) { return KV4_SLICE * (D + 8 * groups); }
+__host__ __device__ constexpr int kv4_bytes(int D, int groups) { return KV4_PAGE / KV4_SLICE * kv4_slice_bytes(D, groups); }
 
 // where dimension d of a slot's key lies: word within the slot, bit within the word
 __device__ __forceinline__ int kv4_k_word(int D, int d) { return ((d & 15) >> 2) * (D / 32) + (d >> 5); }

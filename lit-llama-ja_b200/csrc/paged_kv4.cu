@@ -256,8 +256,8 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(Kv4Rows in, const float
   uint32_t code[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) code[e] = s > 0.f ? (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[e], lo), s)), 0.f), 15.f) : 0u;
-  uint8_t* blk = blocks + ((size_t)(slot / KV4_PAGE) * G + head) * kv4_bytes(D, NG);
-  const int at = slot % KV4_PAGE;
+  uint8_t* blk = blocks + ((size_t)(slot / KV4_PAGE) * G + head) * kv4_bytes(D, NG) + slot % KV4_PAGE / KV4_SLICE * kv4_slice_bytes(D, NG);
+  const int at = slot % KV4_SLICE;
   if (live && lane % GL == 0)
     reinterpret_cast<uint32_t*>(blk + (is_k ? kv4_k_params(D) : kv4_v_params(D, NG)))[at * NG + lane / GL] = params;
   if (is_k) {
@@ -290,8 +290,8 @@ __global__ void __launch_bounds__(D) kv4_read_kernel(const uint8_t* __restrict__
   const int t = blockIdx.x, head = blockIdx.y, d = threadIdx.x, slot = slots[t];
   float k = NAN, v = NAN;
   if (slot >= 0 && slot < pages * KV4_PAGE) {
-    const uint8_t* blk = blocks + ((size_t)(slot / KV4_PAGE) * G + head) * kv4_bytes(D, NG);
-    const int at = slot % KV4_PAGE, g = d / (D / NG);
+    const uint8_t* blk = blocks + ((size_t)(slot / KV4_PAGE) * G + head) * kv4_bytes(D, NG) + slot % KV4_PAGE / KV4_SLICE * kv4_slice_bytes(D, NG);
+    const int at = slot % KV4_SLICE, g = d / (D / NG);
     const uint32_t kw = reinterpret_cast<const uint32_t*>(blk)[at * (D / 8) + kv4_k_word(D, d)];
     const uint32_t vw = reinterpret_cast<const uint32_t*>(blk + kv4_v_codes(D))[(at / 2) * (D / 4) + kv4_v_word(D, d)];
     const float2 kp = bits_pair<T>(reinterpret_cast<const uint32_t*>(blk + kv4_k_params(D))[at * NG + g]);

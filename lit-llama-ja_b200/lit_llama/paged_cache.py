@@ -191,11 +191,14 @@ class PagedCache4:
             out = torch.empty((T, self.n_head, self.head_size), dtype=self.dtype, device=self.device)
         elif out.shape != q.shape or out.dtype != self.dtype or out.device != self.device or not out.is_contiguous() or out.data_ptr() % 16 != 0:
             raise RuntimeError(f"out: dense {self.dtype} {tuple(q.shape)} on {self.device}, not {out.dtype} {tuple(out.shape)} on {out.device}")
+        scale = self.head_size ** -0.5 if scale is None else float(scale)
+        if not 0 < scale < float("inf"):
+            raise RuntimeError(f"scores times {scale}: more than 0")
         if T == 0:
             return out
         with torch.cuda.device(self.device):
             shape = (plan.B, T, plan.max_count, self.n_head, self.n_kv_head, self.head_size)
             scratch = torch.empty(N.call_ret("ll_kv4_attn_scratch_bytes", *shape), dtype=torch.uint8, device=self.device)
             N.call("ll_kv4_attn", N.ptr(q), q.stride(0), self._layers[layer], N.ptr(self.table), N.ptr(plan.starts), N.ptr(plan.work), N.ptr(out), self._code, *shape,
-                   self.group, self.width, self.pages, self.head_size ** -0.5 if scale is None else float(scale), N.ptr(scratch), N.stream())
+                   self.group, self.width, self.pages, scale, N.ptr(scratch), N.stream())
         return out

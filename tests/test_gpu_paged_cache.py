@@ -334,7 +334,8 @@ def test_refusals():
     q, k = torch.zeros((3, 4, 64), dtype=BF, device=DEV), torch.zeros((3, 2, 64), dtype=BF, device=DEV)
     for call in (lambda: cache.attend(0, old, q), lambda: other.attend(0, plan, q), lambda: cache.attend(2, plan, q), lambda: cache.attend(-1, plan, q),
                  lambda: cache.attend(0, plan, q.half()), lambda: cache.attend(0, plan, q[:2]), lambda: cache.attend(0, plan, q.cpu()),
-                 lambda: cache.attend(0, plan, q[:, :2]), lambda: cache.attend(0, plan, q, out=q[:2]), lambda: cache.append(0, plan, q, q, k),
+                 lambda: cache.attend(0, plan, q[:, :2]), lambda: cache.attend(0, plan, q, scale=0.0), lambda: cache.attend(0, plan, q, scale=math.nan),
+                 lambda: cache.attend(0, plan, q, scale=-1.0), lambda: cache.attend(0, plan, q, out=q[:2]), lambda: cache.append(0, plan, q, q, k),
                  lambda: cache.append(0, plan, q, k, k.float()), lambda: cache.append(0, plan, None, k, k, rope=torch.zeros((100, 32, 2), device=DEV)),
                  lambda: cache.append(0, plan, q, k, k, rope=torch.zeros((99, 32, 2), device=DEV)),
                  lambda: cache.append(0, plan, q, k, k, rope=torch.zeros((100, 64, 2), device=DEV)),
