@@ -23,7 +23,9 @@ struct Kv4Attn {
   int* word;           // wait_word()
 };
 
-constexpr int KF_WARPS = 4, KF_THREADS = KF_WARPS * 32, KF_STAGES = 4;
+constexpr int KF_WARPS = 4, KF_THREADS = KF_WARPS * 32;
+// units of 32 keys in a warp's ring: four blocks an SM
+__host__ __device__ constexpr int kf_stages(int D, int groups) { return 4 * KF_WARPS * 3 * 2 * kv4_slice_bytes(D, groups) <= 222 * 1024 ? 3 : 2; }
 constexpr float KF_LOG2E = 1.4426950408889634f, KF_SLACK = 8.f;      // a column's scores may outgrow its reference by 2^8 before it moves
 constexpr float KF_NONE = -1e37f;                                       // the reference of a column that has seen no key
 constexpr uint32_t KF_WAIT_LIMIT = 1u << 20;
@@ -67,16 +69,17 @@ __device__ __forceinline__ bool kf_wait(uint64_t* bar, uint32_t parity, int* wor
   return false;
 }
 
-// Few queries a request: a block walks a range of one request's pages for one key head and up to 8 NB columns (a column: one query of one of the heads
-// that share the key head).  Each of its four warps takes a slice of 16 keys of every page through a ring of its own, with references of its own; they
-// join at the end.
-// Weights enter the second product as fp16 (TERMS 1), or as two such terms where the result is fp16, too.
-template <typename T, int D, int NG, int NB>
+// Few queries a request: a block walks a range of one request's pages for one key head and a tile of columns (a column: one query of one of the heads
+// that share the key head).  Warp w takes half w & 1 of every other page, 32 keys, through a ring and with references of its own; the four join at the end.
+// CPL = 1: up to four columns, each of which has two of the product's eight, so that a lane has one column's scores and weights enter the second
+// product as two terms of fp16 (what the first leaves over in the odd column); CPL = 2: eight columns, and 16 with NB = 2, whose weights are one term, or
+// two where the result is fp16.
+template <typename T, int D, int NG, int CPL, int NB>
 __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(const Kv4Attn a) {
-  constexpr int W = D / 32, KS = D / 16, COLS = 8 * NB, BYTES = kv4_bytes(D, NG), SLICE = kv4_slice_bytes(D, NG), SPG = KS / NG;
-  constexpr int TERMS = std::is_same<T, __half>::value ? 2 : 1;
+  constexpr int W = D / 32, KS = D / 16, COLS = 4 * CPL * NB, BYTES = kv4_bytes(D, NG), SLICE = kv4_slice_bytes(D, NG), SPG = KS / NG, STAGES = kf_stages(D, NG);
+  constexpr int TERMS = CPL == 2 && std::is_same<T, __half>::value ? 2 : 1;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ uint64_t s_full[KF_WARPS][KF_STAGES];
+  __shared__ uint64_t s_full[KF_WARPS][STAGES];
   __shared__ int s_fail;
   __shared__ float s_ref[KF_WARPS][COLS], s_sum[KF_WARPS][COLS];
   const int item = blockIdx.x, head = blockIdx.y;
@@ -95,55 +98,58 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
   }
   const int pos0 = a.ends[seq] - n;                                     // position of the sequence's first token
   const int last = pos0 + (col0 + cols - 1) / R;                        // position of the tile's last column: keys up to here are in sight
-  const int page0 = it.z * step, pages = min(page0 + step, last / KV4_PAGE + 1) - page0;
-  // the warp's slices: of the last page only what holds keys in sight
-  const int slices = pages <= 0 ? 0 : pages - ((page0 + pages - 1) * KV4_PAGE + 16 * warp > last ? 1 : 0);
+  const int page0 = it.z * step + (warp >> 1), page1 = min(it.z * step + step, last / KV4_PAGE + 1), half32 = 32 * (warp & 1);
+  // the warp's pages: page0, page0 + 2 ..; the last one only where its half holds keys in sight
+  const int units = page0 >= page1 ? 0 : (page1 - page0 + 1) / 2 - ((page0 + ((page1 - page0 - 1) & ~1)) * KV4_PAGE + half32 > last ? 1 : 0);
   const int32_t* table = a.table + (size_t)row * a.width + page0;
-  uint8_t* ring = smem + warp * KF_STAGES * SLICE;
+  uint8_t* ring = smem + warp * STAGES * 2 * SLICE;
   uint64_t* full = s_full[warp];
-  const uint8_t* from = a.blocks + (size_t)head * BYTES + warp * SLICE;
+  const uint8_t* from = a.blocks + (size_t)head * BYTES + (warp & 1) * 2 * SLICE;
   const size_t page_bytes = (size_t)a.G * BYTES;
 
-  int entry = lane < slices ? table[lane] : 0;                          // the table's entries of 32 pages, a lane each
+  int entry = lane < units ? table[2 * lane] : 0;                       // the table's entries of 32 pages, a lane each
   if (threadIdx.x == 0) s_fail = 0;
   if (lane == 0) {
-    for (int i = 0; i < KF_STAGES; ++i) mbar_init(&full[i], 1);
+    for (int i = 0; i < STAGES; ++i) mbar_init(&full[i], 1);
     fence_barrier_init();
   }
   __syncwarp();
 #pragma unroll
-  for (int i = 0; i < KF_STAGES; ++i) {
+  for (int i = 0; i < STAGES; ++i) {
     const int page = __shfl_sync(0xffffffffu, entry, i);
-    if (lane == 0 && i < slices) {
-      mbar_expect_tx(&full[i], SLICE);
-      bulk_load_1d(ring + i * SLICE, from + min(max(page, 0), a.pages - 1) * page_bytes, SLICE, &full[i]);
+    if (lane == 0 && i < units) {
+      mbar_expect_tx(&full[i], 2 * SLICE);
+      bulk_load_1d(ring + i * 2 * SLICE, from + min(max(page, 0), a.pages - 1) * page_bytes, 2 * SLICE, &full[i]);
     }
   }
 
   float o[NB][KS][4];
-  float ref[NB][2], sum[NB][2], sumlo[NB][NG][2];      // references in units of log2
-  uint32_t ev[NG];                                     // exponents of the values' scales so far, as powers of two's bits
+  float ref[NB][CPL], sum[NB][CPL], sumlo[NB][NG][CPL];      // references in units of log2
+  uint32_t ev[NG];                                           // exponents of the values' scales so far, as powers of two's bits
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
 #pragma unroll
     for (int r = 0; r < KS; ++r) o[b][r][0] = o[b][r][1] = o[b][r][2] = o[b][r][3] = 0.f;
-    ref[b][0] = ref[b][1] = KF_NONE;
-    sum[b][0] = sum[b][1] = 0.f;
 #pragma unroll
-    for (int g = 0; g < NG; ++g) sumlo[b][g][0] = sumlo[b][g][1] = 0.f;
+    for (int e = 0; e < CPL; ++e) {
+      ref[b][e] = KF_NONE;
+      sum[b][e] = 0.f;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) sumlo[b][g][e] = 0.f;
+    }
   }
 #pragma unroll
   for (int g = 0; g < NG; ++g) ev[g] = 1u << 23;
 
   const int t4 = lane & 3, g8 = lane >> 2;
-  // queries as the products' second operand: column g8, dimensions 16 s + 4 t4 .. + 3; the largest of a column is brought to 2^14 .. 2^15, the
-  // dimensions of odd nibbles are 16 times smaller
+  // queries as the products' second operand: the product's column g8, dimensions 16 s + 4 t4 .. + 3; the largest of a column is brought to
+  // 2^14 .. 2^15, the dimensions of odd nibbles are 16 times smaller
   uint32_t qb[NB][KS][2];
-  float kq[NB][2], qn[NB][NG][2];
+  float kq[NB][CPL], qn[NB][NG][CPL];
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
-    const int c = col0 + 8 * b + g8;
-    const bool live = 8 * b + g8 < cols;
+    const int mine = CPL == 2 ? 8 * b + g8 : g8 >> 1, c = col0 + mine;
+    const bool live = mine < cols && (CPL == 2 || (g8 & 1) == 0);
     const T* q = (const T*)a.q + (long long)(first + (live ? c / R : 0)) * a.q_row + (size_t)(head * R + (live ? c % R : 0)) * D;
     uint2 raw[KS];
     float mx = 0.f;
@@ -171,13 +177,13 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
     // 2^24 of the codes and 2^(ex - 127 - 14) of the queries, times the scores' scale in units of log2
     const float back = __uint_as_float((uint32_t)(ex - 14 + 24) << 23) * (a.scale * KF_LOG2E);
 #pragma unroll
-    for (int e = 0; e < 2; ++e) kq[b][e] = __shfl_sync(0xffffffffu, back, 4 * (2 * t4 + e));
+    for (int e = 0; e < CPL; ++e) kq[b][e] = __shfl_sync(0xffffffffu, back, 4 * (2 * t4 + e));
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       gs[g] += __shfl_xor_sync(0xffffffffu, gs[g], 1);
       gs[g] += __shfl_xor_sync(0xffffffffu, gs[g], 2);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) qn[b][g][e] = __shfl_sync(0xffffffffu, gs[g], 4 * (2 * t4 + e)) * 5.9604644775390625e-8f;      // 2^-24
+      for (int e = 0; e < CPL; ++e) qn[b][g][e] = __shfl_sync(0xffffffffu, gs[g], 4 * (2 * t4 + e)) * 5.9604644775390625e-8f;      // 2^-24
     }
   }
   const int first_pos = pos0 + col0 / R;                                // every column sees the keys up to here
@@ -185,68 +191,59 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
   bool ok = true;
   int st = 0;
   uint32_t parity = 0;
-  for (int i = 0; i < slices; ++i) {
+  for (int i = 0; i < units; ++i) {
     ok = __all_sync(0xffffffffu, kf_wait(&full[st], parity, a.word));
     if (!ok) break;
-    const uint8_t* blk = ring + st * SLICE;
-    uint32_t kw[2][W], vw[2][W], kp[2][NG], vp[2][NG];
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      lds_words<W>(kw[x], blk + (g8 + 8 * x) * (D / 2) + t4 * 4 * W);
-      lds_words<NG>(kp[x], blk + kv4_k_params(D) + (g8 + 8 * x) * NG * 4);
-      lds_words<W>(vw[x], blk + kv4_v_codes(D) + (t4 + 4 * x) * D + g8 * 4 * W);
-      lds_words<NG>(vp[x], blk + kv4_v_params(D, NG) + (g8 + 8 * x) * NG * 4);
-    }
-    // the next slice for this place of the ring
-    const int nxt = i + KF_STAGES;
-    if ((nxt & 31) == 0) entry = nxt + lane < slices ? table[nxt + lane] : 0;
-    const int page = __shfl_sync(0xffffffffu, entry, nxt & 31);
-    __syncwarp();                                                       // every lane has read the slice
-    if (lane == 0 && nxt < slices) {
-      mbar_expect_tx(&full[st], SLICE);
-      bulk_load_1d(ring + st * SLICE, from + min(max(page, 0), a.pages - 1) * page_bytes, SLICE, &full[st]);
-    }
-    if (++st == KF_STAGES) st = 0, parity ^= 1;
-    const int j = (page0 + i) * KV4_PAGE + 16 * warp + g8;              // the lane's keys: j, j + 8
+    const uint8_t* const unit = ring + st * 2 * SLICE;
+    const int j = (page0 + 2 * i) * KV4_PAGE + half32 + g8;             // the lane's keys: j, j + 8, j + 16, j + 24
     // scores, in the products' units
-    float s[NB][4];
+    float s[4][NB][CPL];
+    float2 pv[4][NG];
 #pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      float acc[NB][4];
-#pragma unroll
-      for (int b = 0; b < NB; ++b) acc[b][0] = acc[b][1] = acc[b][2] = acc[b][3] = 0.f;
-#pragma unroll
-      for (int e = 0; e < SPG; ++e) {
-        const int k = g * SPG + e;
-        const uint32_t w0 = (k & 1) ? kw[0][k >> 1] >> 8 : kw[0][k >> 1], w1 = (k & 1) ? kw[1][k >> 1] >> 8 : kw[1][k >> 1];
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-          mma_f16_16816(acc[b], w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u, qb[b][k][0], qb[b][k][1]);
-      }
-      const float2 p0 = bits_pair<T>(kp[0][g]), p1 = bits_pair<T>(kp[1][g]);
-#pragma unroll
-      for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 p = e < 2 ? p0 : p1;
-          s[b][e] = fmaf(p.x, acc[b][e], g == 0 ? p.y * qn[b][g][e & 1] : fmaf(p.y, qn[b][g][e & 1], s[b][e]));
-        }
-    }
-    float2 pv[2][NG];
-#pragma unroll
-    for (int x = 0; x < 2; ++x)
-#pragma unroll
-      for (int g = 0; g < NG; ++g) pv[x][g] = bits_pair<T>(vp[x][g]);
-    // which keys a column sees: all of them but at the end of its walk, where a slot behind the last key may hold anything
-    const bool masked = j - g8 + 15 > first_pos;
-    if (masked) {
+    for (int h = 0; h < 2; ++h) {
+      const uint8_t* const blk = unit + h * SLICE;
+      uint32_t kw[2][W], kp[2][NG], vp[2][NG];
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
+        lds_words<W>(kw[x], blk + (g8 + 8 * x) * (D / 2) + t4 * 4 * W);
+        lds_words<NG>(kp[x], blk + kv4_k_params(D) + (g8 + 8 * x) * NG * 4);
+        lds_words<NG>(vp[x], blk + kv4_v_params(D, NG) + (g8 + 8 * x) * NG * 4);
+      }
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        float acc[NB][4];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) acc[b][0] = acc[b][1] = acc[b][2] = acc[b][3] = 0.f;
+#pragma unroll
+        for (int e = 0; e < SPG; ++e) {
+          const int k = g * SPG + e;
+          const uint32_t w0 = (k & 1) ? kw[0][k >> 1] >> 8 : kw[0][k >> 1], w1 = (k & 1) ? kw[1][k >> 1] >> 8 : kw[1][k >> 1];
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+            mma_f16_16816(acc[b], w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u, qb[b][k][0], qb[b][k][1]);
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const float2 p = bits_pair<T>(kp[x][g]);
+          pv[2 * h + x][g] = bits_pair<T>(vp[x][g]);
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int e = 0; e < CPL; ++e)
+              s[2 * h + x][b][e] = fmaf(p.x, acc[b][2 * x + e], g == 0 ? p.y * qn[b][g][e] : fmaf(p.y, qn[b][g][e], s[2 * h + x][b][e]));
+        }
+      }
+    }
+    // which keys a column sees: all of them but at the end of its walk, where a slot behind the last key may hold anything
+    const bool masked = j - g8 + 31 > first_pos;
+    if (masked) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-            if (j + 8 * x > pos0 + min(col0 + 8 * b + 2 * t4 + e, col0 + cols - 1) / R) s[b][2 * x + e] = -INFINITY;
+          for (int e = 0; e < CPL; ++e)
+            if (j + 8 * x > pos0 + min(col0 + 8 * b + CPL * t4 + e, col0 + cols - 1) / R) s[x][b][e] = -INFINITY;
         if (j + 8 * x > last)
 #pragma unroll
           for (int g = 0; g < NG; ++g) pv[x][g] = make_float2(0.f, 0.f);
@@ -257,30 +254,36 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) grow |= fmaxf(s[b][e], s[b][e + 2]) * kq[b][e] > ref[b][e] + KF_SLACK;
+      for (int e = 0; e < CPL; ++e)
+        grow |= fmaxf(fmaxf(s[0][b][e], s[1][b][e]), fmaxf(s[2][b][e], s[3][b][e])) * kq[b][e] > ref[b][e] + KF_SLACK;
 #pragma unroll
-    for (int g = 0; g < NG; ++g) grow |= fmaxf(pv[0][g].x, pv[1][g].x) > 2.f * __uint_as_float(ev[g]);
+    for (int g = 0; g < NG; ++g) grow |= fmaxf(fmaxf(pv[0][g].x, pv[1][g].x), fmaxf(pv[2][g].x, pv[3][g].x)) > 2.f * __uint_as_float(ev[g]);
     if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-      for (int b = 0; b < NB; ++b)
+      for (int b = 0; b < NB; ++b) {
+        float f[2] = {1.f, 1.f};
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float m = fmaxf(s[b][e], s[b][e + 2]) * kq[b][e];
+        for (int e = 0; e < CPL; ++e) {
+          float m = fmaxf(fmaxf(s[0][b][e], s[1][b][e]), fmaxf(s[2][b][e], s[3][b][e])) * kq[b][e];
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
           m = fmaxf(m, ref[b][e]);
-          const float f = kf_exp2(ref[b][e] - m);
+          f[e] = kf_exp2(ref[b][e] - m);
           ref[b][e] = m;
-          sum[b][e] *= f;
+          sum[b][e] *= f[e];
 #pragma unroll
-          for (int g = 0; g < NG; ++g) sumlo[b][g][e] *= f;
-#pragma unroll
-          for (int r = 0; r < KS; ++r) o[b][r][e] *= f, o[b][r][e + 2] *= f;
+          for (int g = 0; g < NG; ++g) sumlo[b][g][e] *= f[e];
         }
+        if (CPL == 1) f[1] = f[0];
+#pragma unroll
+        for (int r = 0; r < KS; ++r) o[b][r][0] *= f[0], o[b][r][1] *= f[1], o[b][r][2] *= f[0], o[b][r][3] *= f[1];
+      }
 #pragma unroll
       for (int g = 0; g < NG; ++g) {      // (scales are not negative: their bits rise with them; infinite ones and those that are none are passed over)
-        const uint32_t e0 = __float_as_uint(pv[0][g].x), e1 = __float_as_uint(pv[1][g].x);
-        const uint32_t big = __reduce_max_sync(0xffffffffu, max(e0 < 0x7f800000u ? e0 : 0u, e1 < 0x7f800000u ? e1 : 0u)) & 0x7f800000u;
+        uint32_t big = 0;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) big = max(big, __float_as_uint(pv[x][g].x) < 0x7f800000u ? __float_as_uint(pv[x][g].x) : 0u);
+        big = __reduce_max_sync(0xffffffffu, big) & 0x7f800000u;
         if (big > ev[g]) {
           const float f = __uint_as_float(max((int)ev[g] - (int)big + (127 << 23), 0));
           ev[g] = big;
@@ -295,53 +298,77 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
     }
     // weights
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
+    for (int x = 0; x < 4; ++x)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[b][e] = kf_exp2(fmaf(s[b][e], kq[b][e & 1], -ref[b][e & 1]));
-        sum[b][e & 1] += s[b][e];
-      }
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int e = 0; e < CPL; ++e) {
+          s[x][b][e] = kf_exp2(fmaf(s[x][b][e], kq[b][e], -ref[b][e]));
+          sum[b][e] += s[x][b][e];
+        }
     // y += (p s) c, p lo: by groups, the scales brought under 4 by a power of two that only grows
 #pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      const float inv = __uint_as_float((254u << 23) - ev[g]);
-      const float s0 = pv[0][g].x * inv, s1 = pv[1][g].x * inv;
-      uint32_t bw[NB][TERMS][2];
+    for (int h = 0; h < 2; ++h) {
+      uint32_t vw[2][W];
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        float w[4] = {s[b][0] * s0, s[b][1] * s0, s[b][2] * s1, s[b][3] * s1};
-        if (masked) {                                                   // (a value that is no number, behind a column: no trace of it)
-          float l[4] = {s[b][0] * pv[0][g].y, s[b][1] * pv[0][g].y, s[b][2] * pv[1][g].y, s[b][3] * pv[1][g].y};
+      for (int x = 0; x < 2; ++x) lds_words<W>(vw[x], unit + h * SLICE + kv4_v_codes(D) + (t4 + 4 * x) * D + g8 * 4 * W);
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (s[b][e] == 0.f) w[e] = 0.f, l[e] = 0.f;
-          sumlo[b][g][0] += l[0] + l[2];
-          sumlo[b][g][1] += l[1] + l[3];
-        } else {
-          sumlo[b][g][0] = fmaf(s[b][0], pv[0][g].y, fmaf(s[b][2], pv[1][g].y, sumlo[b][g][0]));
-          sumlo[b][g][1] = fmaf(s[b][1], pv[0][g].y, fmaf(s[b][3], pv[1][g].y, sumlo[b][g][1]));
-        }
+      for (int g = 0; g < NG; ++g) {
+        const float inv = __uint_as_float((254u << 23) - ev[g]);
+        uint32_t bw[NB][TERMS][2];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          const uint32_t h = half_bits(w[2 * x], w[2 * x + 1]);
-          bw[b][0][x] = movmatrix(h);
-          if (TERMS == 2) {
-            const float2 f = bits_pair<__half>(h);
-            bw[b][TERMS - 1][x] = movmatrix(half_bits(w[2 * x] - f.x, w[2 * x + 1] - f.y));
+          const float2 p = pv[2 * h + x][g];
+          const float sc = p.x * inv;
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {
+            float w[2] = {0.f, 0.f};
+#pragma unroll
+            for (int e = 0; e < CPL; ++e) {
+              const float pe = s[2 * h + x][b][e];
+              w[e] = pe * sc;
+              if (masked) {                                             // (a value that is no number, behind a column: no trace of it)
+                if (pe == 0.f) w[e] = 0.f;
+                else sumlo[b][g][e] = fmaf(pe, p.y, sumlo[b][g][e]);
+              } else {
+                sumlo[b][g][e] = fmaf(pe, p.y, sumlo[b][g][e]);
+              }
+            }
+            if (CPL == 1) {
+              w[1] = w[0] - __half2float(__float2half_rn(w[0]));
+              bw[b][0][x] = movmatrix(half_bits(w[0], w[1]));
+            } else {
+              const uint32_t hi = half_bits(w[0], w[1]);
+              bw[b][0][x] = movmatrix(hi);
+              if (TERMS == 2) {
+                const float2 f = bits_pair<__half>(hi);
+                bw[b][TERMS - 1][x] = movmatrix(half_bits(w[0] - f.x, w[1] - f.y));
+              }
+            }
           }
         }
-      }
 #pragma unroll
-      for (int e = 0; e < SPG; ++e) {
-        const int r = g * SPG + e;
-        const uint32_t w0 = (r & 1) ? vw[0][r >> 1] >> 8 : vw[0][r >> 1], w1 = (r & 1) ? vw[1][r >> 1] >> 8 : vw[1][r >> 1];
+        for (int e = 0; e < SPG; ++e) {
+          const int r = g * SPG + e;
+          const uint32_t w0 = (r & 1) ? vw[0][r >> 1] >> 8 : vw[0][r >> 1], w1 = (r & 1) ? vw[1][r >> 1] >> 8 : vw[1][r >> 1];
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
+          for (int b = 0; b < NB; ++b)
 #pragma unroll
-          for (int x = 0; x < TERMS; ++x)
-            mma_f16_16816(o[b][r], w0 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x000f000fu, w1 & 0x00f000f0u, bw[b][x][0], bw[b][x][1]);
+            for (int x = 0; x < TERMS; ++x)
+              mma_f16_16816(o[b][r], w0 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x000f000fu, w1 & 0x00f000f0u, bw[b][x][0], bw[b][x][1]);
+        }
       }
     }
+    // the next 32 keys for this place of the ring
+    const int nxt = i + STAGES;
+    if ((nxt & 31) == 0) entry = nxt + lane < units ? table[2 * (nxt + lane)] : 0;
+    const int page = __shfl_sync(0xffffffffu, entry, nxt & 31);
+    __syncwarp();                                                       // every lane has read the unit
+    if (lane == 0 && nxt < units) {
+      mbar_expect_tx(&full[st], 2 * SLICE);
+      bulk_load_1d(ring + st * 2 * SLICE, from + min(max(page, 0), a.pages - 1) * page_bytes, 2 * SLICE, &full[st]);
+    }
+    if (++st == STAGES) st = 0, parity ^= 1;
   }
   if (!ok) {
     s_fail = 1;
@@ -351,7 +378,7 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
-    for (int e = 0; e < 2; ++e)
+    for (int e = 0; e < CPL; ++e)
 #pragma unroll
       for (int d = 4; d < 32; d <<= 1) {
         sum[b][e] += __shfl_xor_sync(0xffffffffu, sum[b][e], d);
@@ -362,8 +389,8 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) s_ref[warp][8 * b + 2 * t4 + e] = ref[b][e], s_sum[warp][8 * b + 2 * t4 + e] = sum[b][e];
-  __syncthreads();                      // every slice has been read: the rings hold the warps' sums now
+      for (int e = 0; e < CPL; ++e) s_ref[warp][8 * b + CPL * t4 + e] = ref[b][e], s_sum[warp][8 * b + CPL * t4 + e] = sum[b][e];
+  __syncthreads();                      // every unit has been read: the rings hold the warps' sums now
   if (s_fail) return;
   pdl_launch_dependents();
   float* so = reinterpret_cast<float*>(smem);                           // [warp][column][D + 4]
@@ -374,9 +401,11 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
     for (int r = 0; r < KS; ++r) {
       const float up = __uint_as_float(ev[r / SPG]);
 #pragma unroll
-      for (int e = 0; e < 4; ++e)                                       // (codes were 2^-24 and, of odd nibbles, 2^-20 of themselves)
-        so[(warp * COLS + 8 * b + 2 * t4 + (e & 1)) * LD + 16 * r + 8 * (e >> 1) + g8] =
-            fmaf(o[b][r][e] * (e < 2 ? 16777216.f : 1048576.f), up, sumlo[b][r / SPG][e & 1]);
+      for (int e = 0; e < 2 * CPL; ++e) {                               // (codes were 2^-24 and, of odd nibbles, 2^-20 of themselves)
+        const float v = CPL == 2 ? o[b][r][e] : o[b][r][2 * e] + o[b][r][2 * e + 1];
+        so[(warp * COLS + 8 * b + CPL * t4 + (CPL == 2 ? e & 1 : 0)) * LD + 16 * r + 8 * (e / CPL) + g8] =
+            fmaf(v * (e < CPL ? 16777216.f : 1048576.f), up, sumlo[b][r / SPG][CPL == 2 ? e & 1 : 0]);
+      }
     }
   __syncthreads();
   // the four warps' parts; the block's are stored as they are, or as the result where there is no other part
@@ -407,9 +436,9 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
 
 // Joins the parts of a request's walk: a block a column, a warp every KJ-th part.
 constexpr int KJ = 8;
-template <typename T, int D, int NB>
+template <typename T, int D, int COLS>
 __global__ void __launch_bounds__(KJ * 32) kv4_join_kernel(const Kv4Attn a) {
-  constexpr int COLS = 8 * NB, E = D / 32;
+  constexpr int E = D / 32;
   __shared__ float s_m[KJ], s_l[KJ], s_o[KJ][D];
   pdl_wait();
   const int item = blockIdx.x, head = blockIdx.y, c = blockIdx.z;
@@ -517,7 +546,10 @@ __global__ void __launch_bounds__(KW_THREADS) kv4_work_kernel(const int32_t* __r
 
 // How many items a step's division has at most.
 static int kf_parts(int G) { return ((sm_count() > 0 ? sm_count() : 148) * 4 + G - 1) / G; }
-static int kf_cols(int max_count, int R) { return (long long)max_count * R <= 8 ? 8 : 16; }
+static int kf_cols(int max_count, int R) {
+  const long long c = (long long)max_count * R;
+  return c <= 4 ? 4 : c <= 8 ? 8 : 16;
+}
 static long long kf_items(int B, int T, int max_count, int H, int G) {
   const int R = H / G, cols = kf_cols(max_count, R);
   const long long walks = (long long)T * R / cols + B;
@@ -558,26 +590,30 @@ int ll_kv4_attn(const void* q, long long q_row, const void* blocks, const int32_
   const int R = H / G, cols = kf_cols(max_count, R), items = (int)kf_items(B, T, max_count, H, G);
   const Kv4Attn a{q, q_row, (const uint8_t*)blocks, table, plan, plan + B + 1, plan + 3 * (size_t)B + 1, work, y, (float*)scratch, H, G, width, pages, B, items, scale, wait_word()};
   cudaStream_t st = (cudaStream_t)stream;
-#define FEW(TT, DD, NG, NB)                                                                                                                   \
+#define FEW(TT, DD, NG, CPL, NB)                                                                                                              \
   {                                                                                                                                           \
-    constexpr int ring = KF_STAGES * kv4_bytes(DD, NG), join = KF_WARPS * 8 * NB * (DD + 4) * 4, smem = ring > join ? ring : join;            \
+    constexpr int COLS = 4 * CPL * NB, ring = KF_WARPS * kf_stages(DD, NG) * 2 * kv4_slice_bytes(DD, NG), join = KF_WARPS * COLS * (DD + 4) * 4; \
+    constexpr int smem = ring > join ? ring : join;                                                                                           \
     static PerDevice set;                                                                                                                     \
     if (!set) {                                                                                                                               \
-      LL_CUDA(cudaFuncSetAttribute(kv4_few_kernel<TT, DD, NG, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));                       \
-      prefer_max_smem(kv4_few_kernel<TT, DD, NG, NB>);                                                                                        \
+      LL_CUDA(cudaFuncSetAttribute(kv4_few_kernel<TT, DD, NG, CPL, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));                  \
+      prefer_max_smem(kv4_few_kernel<TT, DD, NG, CPL, NB>);                                                                                   \
       set.mark();                                                                                                                             \
     }                                                                                                                                         \
-    kv4_few_kernel<TT, DD, NG, NB><<<dim3(items, G), KF_THREADS, smem, st>>>(a);                                                              \
+    kv4_few_kernel<TT, DD, NG, CPL, NB><<<dim3(items, G), KF_THREADS, smem, st>>>(a);                                                         \
     LL_LAUNCH_OK("kv4_few_kernel");                                                                                                           \
-    LL_CUDA(launch(kv4_join_kernel<TT, DD, NB>, dim3(items, G, (unsigned)min((long long)cols, (long long)max_count * R)), dim3(KJ * 32), 0, st, true, a));                                      \
+    LL_CUDA(launch(kv4_join_kernel<TT, DD, COLS>, dim3(items, G, (unsigned)min((long long)cols, (long long)max_count * R)), dim3(KJ * 32), 0, st, true, a)); \
   }
-#define ATTN(DD, NG)                                                   \
-  if (dtype == LL_BF16 && cols == 8) FEW(__nv_bfloat16, DD, NG, 1)     \
-  else if (dtype == LL_BF16) FEW(__nv_bfloat16, DD, NG, 2)             \
-  else if (cols == 8) FEW(__half, DD, NG, 1)                           \
-  else FEW(__half, DD, NG, 2)
+#define FEW_COLS(TT, DD, NG)              \
+  if (cols == 4) FEW(TT, DD, NG, 1, 1)    \
+  else if (cols == 8) FEW(TT, DD, NG, 2, 1) \
+  else FEW(TT, DD, NG, 2, 2)
+#define ATTN(DD, NG)                                      \
+  if (dtype == LL_BF16) { FEW_COLS(__nv_bfloat16, DD, NG) } \
+  else { FEW_COLS(__half, DD, NG) }
   KV4_SHAPES(head_size, group, ATTN)
 #undef ATTN
+#undef FEW_COLS
 #undef FEW
   LL_LAUNCH_OK("kv4_join_kernel");
   return LL_OK;
