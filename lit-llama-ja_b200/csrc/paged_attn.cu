@@ -15,13 +15,30 @@ struct Kv4Attn {
   const void* q;
   long long q_row;
   const uint8_t* blocks;
-  const int32_t *table, *starts, *ends, *request, *work;
+  const int32_t *table, *work;
   void* y;
   float* part;         // [items][G][COLS] of D sums, then [items][G][COLS] of (reference, sum of weights)
-  int H, G, width, pages, B, max_items;
+  int H, G, width, pages, max_items;
   float scale;
   int* word;           // wait_word()
 };
+
+// One part of a walk: a range of one request's pages for one tile of columns.  ll_kv4_work makes them, the largest first.
+struct __align__(16) Kv4Item {
+  int row, first, count, pos0;         // request (-1: its tokens are refused), first row and number of its tokens, position of the first one
+  int tile, page0, page1;              // tile of columns; pages of the part
+  int parts;                           // parts of the walk
+  int part, base;                      // which of them this is; index of the walk's first part among all parts
+  int pad[2];
+};
+static_assert(sizeof(Kv4Item) == 48, "three loads of 16 bytes");
+__device__ __forceinline__ Kv4Item load_item(const int32_t* work, int i) {
+  Kv4Item it;
+  const int4* p = reinterpret_cast<const int4*>(work) + 1 + 3 * (size_t)i;
+  const int4 a = p[0], b = p[1], c = p[2];
+  it.row = a.x, it.first = a.y, it.count = a.z, it.pos0 = a.w, it.tile = b.x, it.page0 = b.y, it.page1 = b.z, it.parts = b.w, it.part = c.x, it.base = c.y;
+  return it;
+}
 
 constexpr int KF_WARPS = 4, KF_THREADS = KF_WARPS * 32;
 // units of 32 keys in a warp's ring: four blocks an SM
@@ -82,12 +99,12 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
   __shared__ uint64_t s_full[KF_WARPS][STAGES];
   __shared__ int s_fail;
   __shared__ float s_ref[KF_WARPS][COLS], s_sum[KF_WARPS][COLS];
-  const int item = blockIdx.x, head = blockIdx.y;
+  const int item = blockIdx.x / a.G, head = blockIdx.x - item * a.G;
   if (item >= a.work[0]) return;
-  const int4 it = reinterpret_cast<const int4*>(a.work)[1 + item];      // sequence, tile of columns, part, parts
-  const int step = a.work[1], warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, R = a.H / a.G;
-  const int seq = it.x, first = a.starts[seq], n = a.starts[seq + 1] - first, row = a.request[seq];
-  const int col0 = it.y * COLS, cols = min(COLS, n * R - col0);
+  const Kv4Item it = load_item(a.work, item);
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, R = a.H / a.G;
+  const int first = it.first, n = it.count, row = it.row;
+  const int col0 = it.tile * COLS, cols = min(COLS, n * R - col0);
   T* y = (T*)a.y;
   if (row < 0) {                        // a refused sequence's tokens are no numbers
     for (int e = threadIdx.x; e < cols * D; e += KF_THREADS) {
@@ -96,9 +113,9 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
     }
     return;
   }
-  const int pos0 = a.ends[seq] - n;                                     // position of the sequence's first token
+  const int pos0 = it.pos0;
   const int last = pos0 + (col0 + cols - 1) / R;                        // position of the tile's last column: keys up to here are in sight
-  const int page0 = it.z * step + (warp >> 1), page1 = min(it.z * step + step, last / KV4_PAGE + 1), half32 = 32 * (warp & 1);
+  const int page0 = it.page0 + (warp >> 1), page1 = min(it.page1, last / KV4_PAGE + 1), half32 = 32 * (warp & 1);
   // the warp's pages: page0, page0 + 2 ..; the last one only where its half holds keys in sight
   const int units = page0 >= page1 ? 0 : (page1 - page0 + 1) / 2 - ((page0 + ((page1 - page0 - 1) & ~1)) * KV4_PAGE + half32 > last ? 1 : 0);
   const int32_t* table = a.table + (size_t)row * a.width + page0;
@@ -422,12 +439,12 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
       l = fmaf(s_sum[w][c], f, l);
       v[0] = fmaf(u.x, f, v[0]), v[1] = fmaf(u.y, f, v[1]), v[2] = fmaf(u.z, f, v[2]), v[3] = fmaf(u.w, f, v[3]);
     }
-    if (it.w == 1) {
+    if (it.parts == 1) {
       const int cc = col0 + c;
       const uint2 out = make_uint2(pair_bits<T>(v[0] / l, v[1] / l), pair_bits<T>(v[2] / l, v[3] / l));
       *reinterpret_cast<uint2*>(y + ((size_t)(first + cc / R) * a.H + head * R + cc % R) * D + d) = out;
     } else {
-      const size_t at = ((size_t)item * a.G + head) * COLS + c;
+      const size_t at = ((size_t)(it.base + it.part) * a.G + head) * COLS + c;
       *reinterpret_cast<float4*>(a.part + at * D + d) = make_float4(v[0], v[1], v[2], v[3]);
       if (d == 0) *reinterpret_cast<float2*>(a.part + (size_t)a.max_items * a.G * COLS * D + at * 2) = make_float2(m, l);
     }
@@ -441,13 +458,12 @@ __global__ void __launch_bounds__(KJ * 32) kv4_join_kernel(const Kv4Attn a) {
   constexpr int E = D / 32;
   __shared__ float s_m[KJ], s_l[KJ], s_o[KJ][D];
   pdl_wait();
-  const int item = blockIdx.x, head = blockIdx.y, c = blockIdx.z;
+  const int item = blockIdx.x / a.G, head = blockIdx.x - item * a.G, c = blockIdx.y;
   const int32_t* work = after_wait(a.work);
   if (item >= work[0]) return;
-  const int4 it = reinterpret_cast<const int4*>(work)[1 + item];
-  if (it.z != 0 || it.w == 1) return;
-  const int seq = it.x, first = a.starts[seq], n = a.starts[seq + 1] - first, R = a.H / a.G, col = it.y * COLS + c;
-  if (a.request[seq] < 0 || col >= n * R) return;
+  const Kv4Item it = load_item(work, item);
+  const int R = a.H / a.G, first = it.first, col = it.tile * COLS + c;
+  if (it.part != 0 || it.parts == 1 || it.row < 0 || col >= it.count * R) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const float* part = after_wait(a.part);
   const float2* ml = reinterpret_cast<const float2*>(part + (size_t)a.max_items * a.G * COLS * D);
@@ -455,8 +471,8 @@ __global__ void __launch_bounds__(KJ * 32) kv4_join_kernel(const Kv4Attn a) {
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.f;
 #pragma unroll 4
-  for (int k = warp; k < it.w; k += KJ) {
-    const size_t at = ((size_t)(item + k) * a.G + head) * COLS + c;
+  for (int k = warp; k < it.parts; k += KJ) {
+    const size_t at = ((size_t)(it.base + k) * a.G + head) * COLS + c;
     const float2 u = ml[at];
     const float mn = fmaxf(m, u.x), f = kf_exp2(m - mn), w = kf_exp2(u.x - mn);
     m = mn;
@@ -493,52 +509,68 @@ __device__ __forceinline__ int block_sum(int v, int* s_warp) {
   return __reduce_add_sync(0xffffffffu, s_warp[threadIdx.x & 31]);
 }
 
-// Parts of `step` pages at most, step the smallest with which a step's walks are cut no more than `parts` times.
+// Parts of `step` pages at most, step the smallest with which a step's walks are cut no more than `cuts` times.  Parts of a size stand together, the
+// largest first: blocks take them in that order, and the short ones fill the end.
+constexpr int KW_SIZES = 512;           // sizes told apart (larger ones by their 1 / KW_SIZES of the largest)
 __global__ void __launch_bounds__(KW_THREADS) kv4_work_kernel(const int32_t* __restrict__ starts, const int32_t* __restrict__ ends,
-                                                             const int32_t* __restrict__ request, int B, int R, int cols, int least, int longest, int parts,
-                                                             int max_items, int32_t* __restrict__ work) {
-  __shared__ int s_warp[32];
-  auto walks = [&](int i) { return ((starts[i + 1] - starts[i]) * R + cols - 1) / cols; };
+                                                             const int32_t* __restrict__ request, int B, int R, int cols, int longest, int cuts, int max_items,
+                                                             int32_t* __restrict__ work) {
+  __shared__ int s_warp[32], s_size[KW_SIZES];
+  auto tokens = [&](int i) { return starts[i + 1] - starts[i]; };
+  auto walks = [&](int i) { return (tokens(i) * R + cols - 1) / cols; };
   auto pages = [&](int i) { return request[i] >= 0 ? max(1, (ends[i] + KV4_PAGE - 1) / KV4_PAGE) : 1; };
   auto total = [&](int step) {
     int v = 0;
     for (int i = threadIdx.x; i < B; i += KW_THREADS) v += walks(i) * ((pages(i) + step - 1) / step);
     return block_sum(v, s_warp);
   };
-  const int most = parts + total(longest);
-  int lo = least, hi = max(least, longest);
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
+  const int most = cuts + total(longest);
+  int step = 1, hi = max(1, longest);
+  while (step < hi) {
+    const int mid = (step + hi) >> 1;
     if (total(mid) <= most) hi = mid;
-    else lo = mid + 1;
+    else step = mid + 1;
   }
-  // a warp a sequence: its place among the items is the sum before it, taken 1024 sequences at a time
-  int base = 0;
-  for (int i0 = 0; i0 < B; i0 += KW_THREADS) {
-    const int i = i0 + threadIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int w = i < B ? walks(i) : 0, k = i < B ? (pages(i) + lo - 1) / lo : 0;
-    int incl = w * k;
+  // a walk's pages in equal parts; the places of the sizes, counted and summed from the largest down
+  auto bucket = [&](int size) { return KW_SIZES - 1 - (int)((long long)(min(size, step) - 1) * KW_SIZES / step); };
+  for (int x = threadIdx.x; x < KW_SIZES; x += KW_THREADS) s_size[x] = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < B; i += KW_THREADS) {
+    const int w = walks(i), p = pages(i), k = (p + step - 1) / step, each = (p + k - 1) / k;
+    if (w > 0) atomicAdd(&s_size[bucket(each)], w * k);
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    int before = 0;
+    for (int x0 = 0; x0 < KW_SIZES; x0 += 32) {
+      const int v = s_size[x0 + threadIdx.x];
+      int incl = v;
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, incl, d);
-      if (lane >= d) incl += u;
+      for (int d = 1; d < 32; d <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, incl, d);
+        if ((int)threadIdx.x >= d) incl += u;
+      }
+      s_size[x0 + threadIdx.x] = before + incl - v;
+      before += __shfl_sync(0xffffffffu, incl, 31);
     }
-    __syncthreads();
-    if (lane == 31) s_warp[warp] = incl;
-    __syncthreads();
-    int before = base;
-    for (int x = 0; x < warp; ++x) before += s_warp[x];
-    const int mine = before + incl - w * k;
-    for (int x = 0; x < 32; ++x) base += s_warp[x];
-    for (int l = 0; l < 32; ++l) {
-      const int at = __shfl_sync(0xffffffffu, mine, l), n = __shfl_sync(0xffffffffu, w * k, l), kk = __shfl_sync(0xffffffffu, k, l), seq = i0 + 32 * warp + l;
-      for (int e = lane; e < n; e += 32)
-        if (at + e < max_items) reinterpret_cast<int4*>(work)[1 + at + e] = make_int4(seq, e / kk, e % kk, kk);
-    }
+    if (threadIdx.x == 0) work[0] = min(before, max_items);
   }
-  if (threadIdx.x == 0) {
-    work[0] = min(base, max_items);
-    work[1] = lo;
+  __syncthreads();
+  // (which of the sequences with parts of one size comes first is left to chance, and of no consequence: every part has its own place for its sums)
+  const int lane = threadIdx.x & 31;
+  for (int i = threadIdx.x >> 5; i < B; i += KW_THREADS / 32) {
+    const int w = walks(i), p = pages(i), k = (p + step - 1) / step, each = (p + k - 1) / k, n = tokens(i), row = request[i], pos0 = ends[i] - n;
+    if (w == 0) continue;
+    int at = 0;
+    if (lane == 0) at = atomicAdd(&s_size[bucket(each)], w * k);
+    at = __shfl_sync(0xffffffffu, at, 0);
+    for (int e = lane; e < w * k && at + e < max_items; e += 32) {
+      int4* o = reinterpret_cast<int4*>(work) + 1 + 3 * (size_t)(at + e);
+      const int tile = e / k, part = e - tile * k;
+      o[0] = make_int4(row, starts[i], n, pos0);
+      o[1] = make_int4(tile, part * each, (part + 1) * each, k);
+      o[2] = make_int4(part, at + tile * k, 0, 0);
+    }
   }
 }
 
@@ -563,12 +595,12 @@ using namespace llb;
 
 extern "C" {
 
-size_t ll_kv4_work_ints(int B, int T, int max_count, int H, int G) { return 4 + 4 * (size_t)kf_items(B, T, max_count, H, G); }
+size_t ll_kv4_work_ints(int B, int T, int max_count, int H, int G) { return 4 + sizeof(Kv4Item) / 4 * (size_t)kf_items(B, T, max_count, H, G); }
 
 int ll_kv4_work(const int32_t* plan, int B, int T, int max_count, int H, int G, int max_length, int32_t* work, ll_stream stream) {
   LL_CHECK_ARG(plan && work && B > 0 && T >= 0 && max_count >= 0 && G > 0 && H > 0 && H % G == 0 && max_length > 0, "kv4_work: %d sequences of %d tokens, %d heads over %d",
                B, T, H, G);
-  kv4_work_kernel<<<1, KW_THREADS, 0, (cudaStream_t)stream>>>(plan, plan + B + 1, plan + 3 * (size_t)B + 1, B, H / G, kf_cols(max_count, H / G), 1,
+  kv4_work_kernel<<<1, KW_THREADS, 0, (cudaStream_t)stream>>>(plan, plan + B + 1, plan + 3 * (size_t)B + 1, B, H / G, kf_cols(max_count, H / G),
                                                               (max_length + KV4_PAGE - 1) / KV4_PAGE, kf_parts(G), (int)kf_items(B, T, max_count, H, G), work);
   LL_LAUNCH_OK("kv4_work_kernel");
   return LL_OK;
@@ -587,8 +619,10 @@ int ll_kv4_attn(const void* q, long long q_row, const void* blocks, const int32_
   LL_CHECK_ARG(scale > 0.f, "kv4_attn: scores times %g (more than 0)", scale);
   LL_CHECK_ARG((((uintptr_t)q | (uintptr_t)y | (uintptr_t)blocks | (uintptr_t)scratch | (uintptr_t)work) & 15) == 0 && q_row % 8 == 0,
                "kv4_attn: rows have to start on 16-byte boundaries");
-  const int R = H / G, cols = kf_cols(max_count, R), items = (int)kf_items(B, T, max_count, H, G);
-  const Kv4Attn a{q, q_row, (const uint8_t*)blocks, table, plan, plan + B + 1, plan + 3 * (size_t)B + 1, work, y, (float*)scratch, H, G, width, pages, B, items, scale, wait_word()};
+  const int R = H / G, cols = kf_cols(max_count, R);
+  const long long items = kf_items(B, T, max_count, H, G);
+  LL_CHECK_ARG(items * G < 0x7fffffffll, "kv4_attn: %d sequences of %d tokens, %d heads", B, T, H);
+  const Kv4Attn a{q, q_row, (const uint8_t*)blocks, table, work, y, (float*)scratch, H, G, width, pages, (int)items, scale, wait_word()};
   cudaStream_t st = (cudaStream_t)stream;
 #define FEW(TT, DD, NG, CPL, NB)                                                                                                              \
   {                                                                                                                                           \
@@ -600,9 +634,9 @@ int ll_kv4_attn(const void* q, long long q_row, const void* blocks, const int32_
       prefer_max_smem(kv4_few_kernel<TT, DD, NG, CPL, NB>);                                                                                   \
       set.mark();                                                                                                                             \
     }                                                                                                                                         \
-    kv4_few_kernel<TT, DD, NG, CPL, NB><<<dim3(items, G), KF_THREADS, smem, st>>>(a);                                                         \
+    kv4_few_kernel<TT, DD, NG, CPL, NB><<<(unsigned)(items * G), KF_THREADS, smem, st>>>(a);                                                         \
     LL_LAUNCH_OK("kv4_few_kernel");                                                                                                           \
-    LL_CUDA(launch(kv4_join_kernel<TT, DD, COLS>, dim3(items, G, (unsigned)min((long long)cols, (long long)max_count * R)), dim3(KJ * 32), 0, st, true, a)); \
+    LL_CUDA(launch(kv4_join_kernel<TT, DD, COLS>, dim3((unsigned)(items * G), (unsigned)min((long long)cols, (long long)max_count * R)), dim3(KJ * 32), 0, st, true, a)); \
   }
 #define FEW_COLS(TT, DD, NG)              \
   if (cols == 4) FEW(TT, DD, NG, 1, 1)    \
