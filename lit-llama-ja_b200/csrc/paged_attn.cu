@@ -509,11 +509,12 @@ __device__ __forceinline__ int block_sum(int v, int* s_warp) {
   return __reduce_add_sync(0xffffffffu, s_warp[threadIdx.x & 31]);
 }
 
-// Parts of `step` pages at most, step the smallest with which a step's walks are cut no more than `cuts` times.  Parts of a size stand together, the
-// largest first: blocks take them in that order, and the short ones fill the end.
+// Parts of `step` pages at most, step the smallest with which a step's walks make no more than `parts` parts, as many as there are places for blocks, or
+// where the walks are more than half of that are cut no more than `parts` times.  Parts of a size stand together, the largest first: blocks take them in
+// that order, and the short ones fill the end.
 constexpr int KW_SIZES = 512;           // sizes told apart (larger ones by their 1 / KW_SIZES of the largest)
 __global__ void __launch_bounds__(KW_THREADS) kv4_work_kernel(const int32_t* __restrict__ starts, const int32_t* __restrict__ ends,
-                                                             const int32_t* __restrict__ request, int B, int R, int cols, int longest, int cuts, int max_items,
+                                                             const int32_t* __restrict__ request, int B, int R, int cols, int longest, int parts, int max_items,
                                                              int32_t* __restrict__ work) {
   __shared__ int s_warp[32], s_size[KW_SIZES];
   auto tokens = [&](int i) { return starts[i + 1] - starts[i]; };
@@ -524,7 +525,7 @@ __global__ void __launch_bounds__(KW_THREADS) kv4_work_kernel(const int32_t* __r
     for (int i = threadIdx.x; i < B; i += KW_THREADS) v += walks(i) * ((pages(i) + step - 1) / step);
     return block_sum(v, s_warp);
   };
-  const int most = cuts + total(longest);
+  const int all = total(longest), most = 2 * all > parts ? all + parts : parts;
   int step = 1, hi = max(1, longest);
   while (step < hi) {
     const int mid = (step + hi) >> 1;
@@ -577,7 +578,10 @@ __global__ void __launch_bounds__(KW_THREADS) kv4_work_kernel(const int32_t* __r
 }  // namespace
 
 // How many items a step's division has at most.
-static int kf_parts(int G) { return ((sm_count() > 0 ? sm_count() : 148) * 4 + G - 1) / G; }
+static int kf_parts(int G) {
+  const int places = (sm_count() > 0 ? sm_count() : 148) * 4;
+  return places > G ? places / G : 1;
+}
 static int kf_cols(int max_count, int R) {
   const long long c = (long long)max_count * R;
   return c <= 4 ? 4 : c <= 8 ? 8 : 16;
