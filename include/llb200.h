@@ -863,13 +863,13 @@ LL_API int ll_kv4_append(const void* q, long long q_row, const void* k, long lon
 /* The values that slots stand for, k, v [n][G][D]; no numbers for a slot that there is not. */
 LL_API int ll_kv4_read(const void* blocks, const int32_t* slots, void* k, void* v, int dtype, int n, int G, int head_size, int group, int pages, ll_stream stream);
 /* Softmax attention of the plan's tokens: q rows of H heads, y [T][H][D]; a token sees its request's keys at and before its position.  Tokens of refused
- * sequences are no numbers, rows behind the last token are left as they are.  plan: ll_kv4_plan's out, of sequences that bring up to max_count tokens;
- * work: ll_kv4_work's division of the step's walks over keys, the same for every layer, ll_kv4_work_ints numbers on a 16-byte boundary. */
-LL_API size_t ll_kv4_work_ints(int B, int T, int max_count, int H, int G);
-LL_API int ll_kv4_work(const int32_t* plan, int B, int T, int max_count, int H, int G, int max_length, int32_t* work, ll_stream stream);
+ * sequences are no numbers, rows behind the last token are left as they are.  work: ll_kv4_work's division of the step's walks over keys, made from
+ * ll_kv4_plan's out (plan) for sequences that bring up to max_count tokens, the same for every layer; ll_kv4_work_ints numbers on a 16-byte boundary. */
+LL_API size_t ll_kv4_work_ints(int B, int T, int max_count, int H, int G, int head_size);
+LL_API int ll_kv4_work(const int32_t* plan, int B, int T, int max_count, int H, int G, int head_size, int max_length, int32_t* work, ll_stream stream);
 LL_API size_t ll_kv4_attn_scratch_bytes(int B, int T, int max_count, int H, int G, int head_size);
-LL_API int ll_kv4_attn(const void* q, long long q_row, const void* blocks, const int32_t* table, const int32_t* plan, const int32_t* work, void* y, int dtype,
-                       int B, int T, int max_count, int H, int G, int head_size, int group, int width, int pages, float scale, void* scratch,
+LL_API int ll_kv4_attn(const void* q, long long q_row, const void* blocks, const int32_t* table, const int32_t* work, void* y, int dtype, int B, int T,
+                       int max_count, int H, int G, int head_size, int group, int width, int pages, float scale, void* scratch,
                        ll_stream stream);
 
 #ifdef __cplusplus

@@ -46,6 +46,18 @@ template <typename T> __device__ __forceinline__ uint32_t pair_bits(float a, flo
 }
 template <typename T> __device__ __forceinline__ float2 bits_pair(uint32_t u) { return to_float2(*reinterpret_cast<const typename pair_of<T>::type*>(&u)); }
 
+template <int W> __device__ __forceinline__ void lds_words(uint32_t (&w)[W], const uint8_t* p) {
+  if constexpr (W == 4) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+  } else if constexpr (W == 2) {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    w[0] = u.x, w[1] = u.y;
+  } else {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
+}
+
 // head sizes and groups that there are kernels for
 inline bool kv4_shape_ok(int D, int group) { return (D == 32 || D == 64 || D == 128) && (group == 32 || group == 64 || group == 128) && group <= D; }
 

@@ -4,47 +4,18 @@
 // With K = s c + lo and V alike, by groups of a head's dimensions (c: codes),
 //   q.k_j = sum_g s_jg (q.c_j)_g + lo_jg (sum of q)_g           y = sum_j p_j v_j = sum_j (p_j s_jg) c_j + sum_j p_j lo_jg
 // so that the products run over codes, which a mask turns into numbers of fp16 (subnormal ones, exactly), and scales meet 16 keys at a time.
+#include <climits>
 #include <type_traits>
 
-#include "kv4.cuh"
+#include "paged_work.cuh"
 
 namespace llb {
 namespace {
-
-struct Kv4Attn {
-  const void* q;
-  long long q_row;
-  const uint8_t* blocks;
-  const int32_t *table, *work;
-  void* y;
-  float* part;         // [items][G][COLS] of D sums, then [items][G][COLS] of (reference, sum of weights)
-  int H, G, width, pages, max_items;
-  float scale;
-  int* word;           // wait_word()
-};
-
-// One part of a walk: a range of one request's pages for one tile of columns.  ll_kv4_work makes them, the largest first.
-struct __align__(16) Kv4Item {
-  int row, first, count, pos0;         // request (-1: its tokens are refused), first row and number of its tokens, position of the first one
-  int tile, page0, page1;              // tile of columns; pages of the part
-  int parts;                           // parts of the walk
-  int part, base;                      // which of them this is; index of the walk's first part among all parts
-  int pad[2];
-};
-static_assert(sizeof(Kv4Item) == 48, "three loads of 16 bytes");
-__device__ __forceinline__ Kv4Item load_item(const int32_t* work, int i) {
-  Kv4Item it;
-  const int4* p = reinterpret_cast<const int4*>(work) + 1 + 3 * (size_t)i;
-  const int4 a = p[0], b = p[1], c = p[2];
-  it.row = a.x, it.first = a.y, it.count = a.z, it.pos0 = a.w, it.tile = b.x, it.page0 = b.y, it.page1 = b.z, it.parts = b.w, it.part = c.x, it.base = c.y;
-  return it;
-}
 
 constexpr int KF_WARPS = 4, KF_THREADS = KF_WARPS * 32;
 // units of 32 keys in a warp's ring: four blocks an SM
 __host__ __device__ constexpr int kf_stages(int D, int groups) { return 4 * KF_WARPS * 3 * 2 * kv4_slice_bytes(D, groups) <= 222 * 1024 ? 3 : 2; }
 constexpr float KF_LOG2E = 1.4426950408889634f, KF_SLACK = 8.f;      // a column's scores may outgrow its reference by 2^8 before it moves
-constexpr float KF_NONE = -1e37f;                                       // the reference of a column that has seen no key
 constexpr uint32_t KF_WAIT_LIMIT = 1u << 20;
 
 __device__ __forceinline__ float kf_exp2(float x) {
@@ -63,17 +34,6 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t v) {
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
-}
-template <int W> __device__ __forceinline__ void lds_words(uint32_t (&w)[W], const uint8_t* p) {
-  if constexpr (W == 4) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
-  } else if constexpr (W == 2) {
-    const uint2 u = *reinterpret_cast<const uint2*>(p);
-    w[0] = u.x, w[1] = u.y;
-  } else {
-    w[0] = *reinterpret_cast<const uint32_t*>(p);
-  }
 }
 __device__ __forceinline__ uint32_t half_bits(float a, float b) { return pair_bits<__half>(a, b); }
 
@@ -149,7 +109,7 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
     for (int r = 0; r < KS; ++r) o[b][r][0] = o[b][r][1] = o[b][r][2] = o[b][r][3] = 0.f;
 #pragma unroll
     for (int e = 0; e < CPL; ++e) {
-      ref[b][e] = KF_NONE;
+      ref[b][e] = KV4_NONE;
       sum[b][e] = 0.f;
 #pragma unroll
       for (int g = 0; g < NG; ++g) sumlo[b][g][e] = 0.f;
@@ -467,13 +427,14 @@ __global__ void __launch_bounds__(KJ * 32) kv4_join_kernel(const Kv4Attn a) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const float* part = after_wait(a.part);
   const float2* ml = reinterpret_cast<const float2*>(part + (size_t)a.max_items * a.G * COLS * D);
-  float m = KF_NONE, l = 0.f, o[E];
+  float m = KV4_NONE, l = 0.f, o[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.f;
 #pragma unroll 4
   for (int k = warp; k < it.parts; k += KJ) {
     const size_t at = ((size_t)(it.base + k) * a.G + head) * COLS + c;
     const float2 u = ml[at];
+    if (u.y == 0.f) continue;                  // (a part that holds no key of the column's)
     const float mn = fmaxf(m, u.x), f = kf_exp2(m - mn), w = kf_exp2(u.x - mn);
     m = mn;
     l = fmaf(l, f, u.y * w);
@@ -498,6 +459,42 @@ __global__ void __launch_bounds__(KJ * 32) kv4_join_kernel(const Kv4Attn a) {
   dt<T>::st((T*)a.y, ((size_t)(first + col / R) * a.H + head * R + col % R) * D + d, num / den);
 }
 
+// The same for the tcgen05 kernel's tiles: a warp a column, a block every KJ-th of 32.
+template <typename T, int D>
+__global__ void __launch_bounds__(KJ * 32) kv4_join_many_kernel(const Kv4Attn a) {
+  constexpr int E = D / 32;
+  pdl_wait();
+  const int item = blockIdx.x / a.G, head = blockIdx.x - item * a.G;
+  const int32_t* work = after_wait(a.work);
+  if (item >= work[0]) return;
+  const Kv4Item it = load_item(work, item);
+  if (it.part != 0 || it.parts == 1 || it.row < 0) return;
+  const int R = a.H / a.G, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const float* part = after_wait(a.part);
+  const float2* ml = reinterpret_cast<const float2*>(part + (size_t)a.max_items * a.G * KV4_MANY * D);
+  for (int c = 32 * blockIdx.y + warp; c < 32 * (blockIdx.y + 1); c += KJ) {
+    const int col = it.tile * KV4_MANY + c;
+    if (col >= it.count * R) return;
+    float m = KV4_NONE, l = 0.f, o[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = 0.f;
+#pragma unroll 2
+    for (int k = 0; k < it.parts; ++k) {
+      const size_t at = ((size_t)(it.base + k) * a.G + head) * KV4_MANY + c;
+      const float2 u = ml[at];
+      if (u.y == 0.f) continue;                // (a part that holds no key of the column's)
+      const float mn = fmaxf(m, u.x), f = kf_exp2(m - mn), w = kf_exp2(u.x - mn);
+      m = mn;
+      l = fmaf(l, f, u.y * w);
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = fmaf(o[e], f, part[at * D + lane + 32 * e] * w);
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      dt<T>::st((T*)a.y, ((size_t)(it.first + col / R) * a.H + head * R + col % R) * D + lane + 32 * e, o[e] / l);
+  }
+}
+
 // ------------------------------------------------------------------ the division of a step's walks
 constexpr int KW_THREADS = 1024;
 
@@ -512,33 +509,55 @@ __device__ __forceinline__ int block_sum(int v, int* s_warp) {
 // Parts of `step` pages at most, step the smallest with which a step's walks make no more than `parts` parts, as many as there are places for blocks, or
 // where the walks are more than half of that are cut no more than `parts` times.  Parts of a size stand together, the largest first: blocks take them in
 // that order, and the short ones fill the end.
+// MANY false: the sequences of up to `few` columns, a thread each, whose tiles count as long as the last one; true: the others, a warp each.
 constexpr int KW_SIZES = 512;           // sizes told apart (larger ones by their 1 / KW_SIZES of the largest)
+template <bool MANY>
 __global__ void __launch_bounds__(KW_THREADS) kv4_work_kernel(const int32_t* __restrict__ starts, const int32_t* __restrict__ ends,
-                                                             const int32_t* __restrict__ request, int B, int R, int cols, int longest, int parts, int max_items,
-                                                             int32_t* __restrict__ work) {
+                                                             const int32_t* __restrict__ request, int B, int R, int few, int cols, int longest, int parts,
+                                                             int max_items, int32_t* __restrict__ work) {
   __shared__ int s_warp[32], s_size[KW_SIZES];
+  const int lane = threadIdx.x & 31, first = MANY ? threadIdx.x >> 5 : threadIdx.x, by = MANY ? KW_THREADS / 32 : KW_THREADS;
   auto tokens = [&](int i) { return starts[i + 1] - starts[i]; };
-  auto walks = [&](int i) { return (tokens(i) * R + cols - 1) / cols; };
-  auto pages = [&](int i) { return request[i] >= 0 ? max(1, (ends[i] + KV4_PAGE - 1) / KV4_PAGE) : 1; };
+  auto tiles = [&](int i) {
+    const long long c = (long long)tokens(i) * R;
+    return (c > few) == MANY ? (int)((c + cols - 1) / cols) : 0;
+  };
+  // pages that a tile's last column sees
+  auto pages = [&](int i, int tile) {
+    if (request[i] < 0) return 1;
+    const int n = tokens(i);
+    return (ends[i] - n + (MANY ? (int)min((long long)n - 1, ((long long)(tile + 1) * cols - 1) / R) : n - 1)) / KV4_PAGE + 1;
+  };
   auto total = [&](int step) {
     int v = 0;
-    for (int i = threadIdx.x; i < B; i += KW_THREADS) v += walks(i) * ((pages(i) + step - 1) / step);
+    for (int i = first; i < B; i += by) {
+      const int w = tiles(i);
+      if (MANY)
+        for (int t = lane; t < w; t += 32) v += (pages(i, t) + step - 1) / step;
+      else if (w > 0)
+        v += w * ((pages(i, 0) + step - 1) / step);
+    }
     return block_sum(v, s_warp);
   };
-  const int all = total(longest), most = 2 * all > parts ? all + parts : parts;
+  const int all = total(max(1, longest)), most = 2 * (long long)all > parts ? all + parts : parts;
   int step = 1, hi = max(1, longest);
+  if (all >= 4ll * parts) step = hi;    // (walks for several rounds even out by themselves)
   while (step < hi) {
     const int mid = (step + hi) >> 1;
     if (total(mid) <= most) hi = mid;
     else step = mid + 1;
   }
   // a walk's pages in equal parts; the places of the sizes, counted and summed from the largest down
+  auto cut = [&](int p) { return (p + step - 1) / step; };
   auto bucket = [&](int size) { return KW_SIZES - 1 - (int)((long long)(min(size, step) - 1) * KW_SIZES / step); };
   for (int x = threadIdx.x; x < KW_SIZES; x += KW_THREADS) s_size[x] = 0;
   __syncthreads();
-  for (int i = threadIdx.x; i < B; i += KW_THREADS) {
-    const int w = walks(i), p = pages(i), k = (p + step - 1) / step, each = (p + k - 1) / k;
-    if (w > 0) atomicAdd(&s_size[bucket(each)], w * k);
+  for (int i = first; i < B; i += by) {
+    const int w = tiles(i);
+    for (int t = MANY ? lane : 0; t < (MANY ? w : min(w, 1)); t += 32) {
+      const int p = pages(i, t), k = cut(p);
+      atomicAdd(&s_size[bucket((p + k - 1) / k)], MANY ? k : w * k);
+    }
   }
   __syncthreads();
   if (threadIdx.x < 32) {
@@ -549,7 +568,7 @@ __global__ void __launch_bounds__(KW_THREADS) kv4_work_kernel(const int32_t* __r
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
         const int u = __shfl_up_sync(0xffffffffu, incl, d);
-        if ((int)threadIdx.x >= d) incl += u;
+        if (lane >= d) incl += u;
       }
       s_size[x0 + threadIdx.x] = before + incl - v;
       before += __shfl_sync(0xffffffffu, incl, 31);
@@ -557,41 +576,56 @@ __global__ void __launch_bounds__(KW_THREADS) kv4_work_kernel(const int32_t* __r
     if (threadIdx.x == 0) work[0] = min(before, max_items);
   }
   __syncthreads();
-  // (which of the sequences with parts of one size comes first is left to chance, and of no consequence: every part has its own place for its sums)
-  const int lane = threadIdx.x & 31;
+  // (which of the parts of one size comes first is left to chance, and of no consequence: every part has its own place for its sums)
   for (int i = threadIdx.x >> 5; i < B; i += KW_THREADS / 32) {
-    const int w = walks(i), p = pages(i), k = (p + step - 1) / step, each = (p + k - 1) / k, n = tokens(i), row = request[i], pos0 = ends[i] - n;
+    const int w = tiles(i), n = tokens(i), row = request[i], pos0 = ends[i] - n;
     if (w == 0) continue;
-    int at = 0;
-    if (lane == 0) at = atomicAdd(&s_size[bucket(each)], w * k);
-    at = __shfl_sync(0xffffffffu, at, 0);
-    for (int e = lane; e < w * k && at + e < max_items; e += 32) {
-      int4* o = reinterpret_cast<int4*>(work) + 1 + 3 * (size_t)(at + e);
-      const int tile = e / k, part = e - tile * k;
+    auto store = [&](int at, int tile, int part, int each, int k, int base) {
+      if (at >= max_items) return;
+      int4* o = reinterpret_cast<int4*>(work) + 1 + 3 * (size_t)at;
       o[0] = make_int4(row, starts[i], n, pos0);
       o[1] = make_int4(tile, part * each, (part + 1) * each, k);
-      o[2] = make_int4(part, at + tile * k, 0, 0);
+      o[2] = make_int4(part, base, 0, 0);
+    };
+    if (MANY) {
+      for (int t = lane; t < w; t += 32) {
+        const int p = pages(i, t), k = cut(p), each = (p + k - 1) / k, at = atomicAdd(&s_size[bucket(each)], k);
+        for (int e = 0; e < k; ++e) store(at + e, t, e, each, k, at);
+      }
+    } else {
+      const int p = pages(i, 0), k = cut(p), each = (p + k - 1) / k;
+      int at = 0;
+      if (lane == 0) at = atomicAdd(&s_size[bucket(each)], w * k);
+      at = __shfl_sync(0xffffffffu, at, 0);
+      for (int e = lane; e < w * k; e += 32) store(at + e, e / k, e % k, each, k, at + e / k * k);
     }
   }
 }
 
 }  // namespace
 
-// How many items a step's division has at most.
-static int kf_parts(int G) {
-  const int places = (sm_count() > 0 ? sm_count() : 148) * 4;
-  return places > G ? places / G : 1;
-}
-static int kf_cols(int max_count, int R) {
-  const long long c = (long long)max_count * R;
-  return c <= 4 ? 4 : c <= 8 ? 8 : 16;
-}
-static long long kf_items(int B, int T, int max_count, int H, int G) {
-  const int R = H / G, cols = kf_cols(max_count, R);
-  const long long walks = (long long)T * R / cols + B;
-  const int parts = kf_parts(G);
-  return walks + parts;
-}
+// A step's two lists: sequences of few columns and, where one may bring more, of many.  Sizes as the host knows them.
+struct Kv4Lists {
+  int R, cols, few, few_parts, many_parts;
+  long long few_items, many_items;      // at most
+  bool many;
+  Kv4Lists(int B, int T, int max_count, int H, int G, int head_size) {
+    R = H / G;
+    many = kv4_many(max_count, R, head_size);
+    const long long c = (long long)max_count * R;
+    cols = many ? 8 : c <= 4 ? 4 : c <= 8 ? 8 : 16;
+    few = many ? KV4_FEW_MOST : INT_MAX;
+    few_parts = max(1, 4 * kv4_sms() / G);
+    many_parts = max(1, kv4_sms() / G);
+    const long long each = many ? (KV4_FEW_MOST + cols - 1) / cols : T, seqs = min(B, max(T, 1));
+    few_items = min((long long)T * R / cols + seqs, seqs * each) + few_parts;
+    many_items = many ? (long long)T * R / KV4_MANY + min((long long)seqs, (long long)T * R / KV4_FEW_MOST) + many_parts : 0;
+  }
+  size_t few_ints() const { return 4 + sizeof(Kv4Item) / 4 * (size_t)few_items; }
+  size_t ints() const { return few_ints() + (many ? 4 + sizeof(Kv4Item) / 4 * (size_t)many_items : 0); }
+  size_t few_floats(int G, int D) const { return ((size_t)few_items * G * cols * (D + 2) + 3) / 4 * 4; }
+  size_t floats(int G, int D) const { return few_floats(G, D) + (size_t)many_items * G * KV4_MANY * (D + 2); }
+};
 
 }  // namespace llb
 
@@ -599,34 +633,57 @@ using namespace llb;
 
 extern "C" {
 
-size_t ll_kv4_work_ints(int B, int T, int max_count, int H, int G) { return 4 + sizeof(Kv4Item) / 4 * (size_t)kf_items(B, T, max_count, H, G); }
+size_t ll_kv4_work_ints(int B, int T, int max_count, int H, int G, int head_size) { return Kv4Lists(B, T, max_count, H, G, head_size).ints(); }
 
-int ll_kv4_work(const int32_t* plan, int B, int T, int max_count, int H, int G, int max_length, int32_t* work, ll_stream stream) {
+int ll_kv4_work(const int32_t* plan, int B, int T, int max_count, int H, int G, int head_size, int max_length, int32_t* work, ll_stream stream) {
   LL_CHECK_ARG(plan && work && B > 0 && T >= 0 && max_count >= 0 && G > 0 && H > 0 && H % G == 0 && max_length > 0, "kv4_work: %d sequences of %d tokens, %d heads over %d",
                B, T, H, G);
-  kv4_work_kernel<<<1, KW_THREADS, 0, (cudaStream_t)stream>>>(plan, plan + B + 1, plan + 3 * (size_t)B + 1, B, H / G, kf_cols(max_count, H / G),
-                                                              (max_length + KV4_PAGE - 1) / KV4_PAGE, kf_parts(G), (int)kf_items(B, T, max_count, H, G), work);
+  const Kv4Lists l(B, T, max_count, H, G, head_size);
+  const int32_t *ends = plan + B + 1, *request = plan + 3 * (size_t)B + 1;
+  const int longest = (max_length + KV4_PAGE - 1) / KV4_PAGE;
+  LL_CHECK_ARG(l.few_items * G < 0x7fffffffll && l.many_items * G < 0x7fffffffll, "kv4_work: %d sequences of %d tokens, %d heads", B, T, H);
+  kv4_work_kernel<false><<<1, KW_THREADS, 0, (cudaStream_t)stream>>>(plan, ends, request, B, l.R, l.few, l.cols, longest, l.few_parts, (int)l.few_items, work);
   LL_LAUNCH_OK("kv4_work_kernel");
+  if (l.many) {
+    kv4_work_kernel<true><<<1, KW_THREADS, 0, (cudaStream_t)stream>>>(plan, ends, request, B, l.R, l.few, KV4_MANY, longest, l.many_parts, (int)l.many_items,
+                                                                      work + l.few_ints());
+    LL_LAUNCH_OK("kv4_work_kernel");
+  }
   return LL_OK;
 }
 
 size_t ll_kv4_attn_scratch_bytes(int B, int T, int max_count, int H, int G, int head_size) {
-  return sizeof(float) * (size_t)kf_items(B, T, max_count, H, G) * G * kf_cols(max_count, H / G) * (head_size + 2);
+  return sizeof(float) * Kv4Lists(B, T, max_count, H, G, head_size).floats(G, head_size);
 }
 
-int ll_kv4_attn(const void* q, long long q_row, const void* blocks, const int32_t* table, const int32_t* plan, const int32_t* work, void* y, int dtype, int B, int T,
+int ll_kv4_attn(const void* q, long long q_row, const void* blocks, const int32_t* table, const int32_t* work, void* y, int dtype, int B, int T,
                 int max_count, int H, int G, int head_size, int group, int width, int pages, float scale, void* scratch, ll_stream stream) {
   LL_CHECK_ARG(kv4_shape_ok(head_size, group), "kv4_attn: heads of %d in groups of %d (32, 64 or 128 each)", head_size, group);
   LL_CHECK_ARG(dtype == LL_BF16 || dtype == LL_F16, "kv4_attn: type %d (bf16 or fp16)", dtype);
-  LL_CHECK_ARG(q && blocks && table && plan && work && y && scratch && B > 0 && T > 0 && max_count >= 0 && G > 0 && G <= 65535 && H > 0 && H % G == 0 && width > 0 && pages > 0,
+  LL_CHECK_ARG(q && blocks && table && work && y && scratch && B > 0 && T > 0 && max_count >= 0 && G > 0 && G <= 65535 && H > 0 && H % G == 0 && width > 0 && pages > 0,
                "kv4_attn: %d tokens of %d heads, %d cached", T, H, G);
   LL_CHECK_ARG(scale > 0.f, "kv4_attn: scores times %g (more than 0)", scale);
   LL_CHECK_ARG((((uintptr_t)q | (uintptr_t)y | (uintptr_t)blocks | (uintptr_t)scratch | (uintptr_t)work) & 15) == 0 && q_row % 8 == 0,
                "kv4_attn: rows have to start on 16-byte boundaries");
-  const int R = H / G, cols = kf_cols(max_count, R);
-  const long long items = kf_items(B, T, max_count, H, G);
-  LL_CHECK_ARG(items * G < 0x7fffffffll, "kv4_attn: %d sequences of %d tokens, %d heads", B, T, H);
+  const Kv4Lists l(B, T, max_count, H, G, head_size);
+  LL_CHECK_ARG(l.few_items * G < 0x7fffffffll && l.many_items * G < 0x7fffffffll, "kv4_attn: %d sequences of %d tokens, %d heads", B, T, H);
+  const int R = l.R, cols = l.cols;
+  const long long items = l.few_items;
   const Kv4Attn a{q, q_row, (const uint8_t*)blocks, table, work, y, (float*)scratch, H, G, width, pages, (int)items, scale, wait_word()};
+  if (l.many) {
+    Kv4Attn m = a;
+    m.work = work + l.few_ints();
+    m.part = (float*)scratch + l.few_floats(G, head_size);
+    m.max_items = (int)l.many_items;
+    if (int r = kv4_prompt_launch(m, dtype, head_size, group, (cudaStream_t)stream)) return r;
+#define JOIN_MANY(TT, DD) LL_CUDA(launch(kv4_join_many_kernel<TT, DD>, dim3((unsigned)(l.many_items * G), KV4_MANY / 32), dim3(KJ * 32), 0, (cudaStream_t)stream, true, m));
+    if (dtype == LL_BF16 && head_size == 64) { JOIN_MANY(__nv_bfloat16, 64) }
+    else if (dtype == LL_BF16) { JOIN_MANY(__nv_bfloat16, 128) }
+    else if (head_size == 64) { JOIN_MANY(__half, 64) }
+    else { JOIN_MANY(__half, 128) }
+#undef JOIN_MANY
+    LL_LAUNCH_OK("kv4_join_many_kernel");
+  }
   cudaStream_t st = (cudaStream_t)stream;
 #define FEW(TT, DD, NG, CPL, NB)                                                                                                              \
   {                                                                                                                                           \

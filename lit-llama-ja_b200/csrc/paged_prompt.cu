@@ -1,0 +1,505 @@
+// Attention of prompts over the paged 4-bit cache on tcgen05: S = Q K^T and O += P V with fp32 accumulators in tensor memory.
+//
+// A block owns two tiles of 128 columns (queries of the heads that share a key head) of one request and walks a range of its pages of 64 keys:
+//   warps 0-7, 8-15 : softmax of tile 0 / tile 1, two threads a row with 32 of its 64 scores each; before, they bring the queries as fp16
+//   warps 16, 17    : one thread each issues the MMAs of a tile: the scores of the next page first, then P V of this one
+//   warps 18-21     : a slice of 16 keys each: codes by bulk copies into a ring, from there as fp16 numbers into the operands
+// All operands are fp16, whatever the cache's type: its 11 bits hold a query exactly (a row under a power of two of its own) and a key or value
+// c s + lo rounded once, where bf16 would lose three bits more.  Slices are brought into range by powers of two 2^e, e a multiple of 16 (so that
+// e is the same, mostly 0, for all of them): scores are multiplied back by 2^e; weights by 2^(e - E), E the largest so far, to which O is rescaled.
+// A word's codes become pairs by masks: 1024 + c under exponent bits, from which one operation takes the 1024 (of odd nibbles, 1024 + 16 c, 64 + c), and
+// one more multiplies and adds.  Keys' pairs run along the dimensions, values' along the keys: values stand with the keys in a row, so that both
+// operands are K-major.
+// Values that are no numbers are zeros in the operand, the first position of such a group is kept and rows that see it end as no numbers: 0 * NaN would
+// reach rows that do not.
+// Every wait is bounded; one that runs out records a code, all roles stop, copies in flight are waited for, tensor memory is freed.
+#include "attn_tc.cuh"
+#include "paged_work.cuh"
+
+namespace llb {
+namespace {
+
+constexpr int KP_ROWS = 128, KP_SOFTMAX = 16, KP_DEQUANT = 4, KP_THREADS = (KP_SOFTMAX + 2 + KP_DEQUANT) * 32;
+constexpr int KP_QBOX = KP_ROWS * 128, KP_KBOX = KV4_PAGE * 128;      // 64 numbers of 16 bits a row
+constexpr int KP_RING = 3, KP_STAGES = 3, KP_EXPS = 8;               // copies in flight a slice; pages of K and of V; pages whose exponents are kept
+
+template <int D, int NG>
+struct KpShape {
+  static constexpr int NB = D / 64, SLICE = kv4_slice_bytes(D, NG);
+  static constexpr int Q = 2 * NB * KP_QBOX, K = NB * KP_KBOX, V = D * 128;
+  static constexpr int RING = KP_DEQUANT * KP_RING * SLICE;
+  static constexpr int SMEM = 1024 + Q + KP_STAGES * (K + V) + RING + 512 + 4 * KP_ROWS * 4 + KP_EXPS * 4 * 8;
+};
+
+__device__ __forceinline__ bool kp_wait(uint64_t* bar, uint32_t parity, volatile int* fail, int* word, int code) {
+  if (mbar_try_wait(bar, parity)) return true;
+  for (uint32_t i = 0; i < AT_WAIT_LIMIT; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 255u) == 255u && *fail) return false;
+  }
+  *fail = 1;
+  wait_ran_out(word, 710 + code);
+  return false;
+}
+
+__host__ __device__ constexpr uint32_t instr_desc_f16(int M, int N) { return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24); }
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }      // -126 <= e <= 127
+
+// A slice's power of two: the multiple of 16 that brings numbers of up to `largest` (bits of a float) under 2^10.
+__device__ __forceinline__ int slice_exponent(uint32_t largest) {
+  const int fl = (int)(largest >> 23) - 127;
+  return max(-112, min(112, ((fl + 6) >> 4) << 4));
+}
+// the larger of |lo| and |lo + 15 s|, bits of a float; 0 for a group that is no number
+__device__ __forceinline__ uint32_t group_reach(float2 p) {
+  const uint32_t b = __float_as_uint(fmaxf(fabsf(p.y), fabsf(fmaf(15.f, p.x, p.y))));
+  return b < 0x7f800000u ? b : 0u;
+}
+__device__ __forceinline__ __half2 as_half2(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
+__device__ __forceinline__ uint32_t as_u32(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
+// the pairs of nibble n of a word, as c s + lo
+template <int N>
+__device__ __forceinline__ uint32_t word_pair(uint32_t w, __half2 s, __half2 lo) {
+  const uint32_t u = N >= 2 ? w >> 8 : w;
+  const __half2 c = (N & 1) ? __hfma2(as_half2((u & 0x00f000f0u) | 0x64006400u), __half2half2(__ushort_as_half(0x2c00)), __half2half2(__ushort_as_half(0xd400)))
+                            : __hadd2(as_half2((u & 0x000f000fu) | 0x64006400u), __half2half2(__ushort_as_half(0xe400)));      // (1/16, -64; -1024)
+  return as_u32(__hfma2(c, s, lo));
+}
+
+template <typename T, int D, int NG>
+__global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn a) {
+  using Shape = KpShape<D, NG>;
+  constexpr int NB = Shape::NB, SLICE = Shape::SLICE, W = D / 32, BYTES = kv4_bytes(D, NG);
+  constexpr uint32_t TM_S = 0, TM_O = 256;            // per tile: two score buffers of 64 columns; 128 accumulator columns
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const int item = blockIdx.x / a.G, head = blockIdx.x - item * a.G;
+  if (item >= a.work[0]) return;
+  const Kv4Item it = load_item(a.work, item);
+  const int R = a.H / a.G, cols_all = it.count * R, col0 = it.tile * KV4_MANY, cols = min(KV4_MANY, cols_all - col0);
+  T* const y = (T*)a.y;
+  if (it.row < 0) {                     // a refused sequence's tokens are no numbers
+    for (int e = threadIdx.x; e < cols * D; e += KP_THREADS) {
+      const int c = col0 + e / D;
+      dt<T>::st(y, ((size_t)(it.first + c / R) * a.H + head * R + c % R) * D + e % D, NAN);
+    }
+    return;
+  }
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem) + 1023) & ~(uintptr_t)1023);
+  uint8_t* sq = base;                                 // [2 tiles][NB][128][64]
+  uint8_t* sk = sq + Shape::Q;                        // [stage][NB][64 keys][64]
+  uint8_t* sv = sk + KP_STAGES * Shape::K;            // [stage][D][64 keys]
+  uint8_t* ring = sv + KP_STAGES * Shape::V;          // [slice][stage]
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(ring + Shape::RING);
+  uint64_t* k_full = q_full + 1;
+  uint64_t* k_empty = k_full + KP_STAGES;
+  uint64_t* v_full = k_empty + KP_STAGES;
+  uint64_t* v_empty = v_full + KP_STAGES;
+  uint64_t* s_full = v_empty + KP_STAGES;             // [tile][buffer] scores are there
+  uint64_t* p_full = s_full + 4;                      // [tile][buffer] weights are there
+  uint64_t* o_full = p_full + 4;                      // [tile][buffer] P V is done
+  uint64_t* r_full = o_full + 4;                      // [slice][stage]
+  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(r_full + KP_DEQUANT * KP_RING);
+  int* s_fail = reinterpret_cast<int*>(tmem_ptr + 1);
+  int* s_none = s_fail + 1;                           // [4] per group the first position whose value is no number
+  float* s_x = reinterpret_cast<float*>(ring + Shape::RING + 512);      // [tile][half][row]: what the two threads of a row tell one another
+  int* s_ek = reinterpret_cast<int*>(s_x + 4 * KP_ROWS);                // [page & 7][slice] exponents of keys and values
+  int* s_ev = s_ek + KP_EXPS * 4;
+
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  // what every role walks: pages page0 .. page1; per tile the last page that one of its rows sees
+  const int last = it.pos0 + (col0 + cols - 1) / R, page0 = it.page0;
+  const int hi1 = cols > KP_ROWS ? min(it.page1, last / KV4_PAGE + 1) - 1 : -1;
+  const int hi0 = min(it.page1, (it.pos0 + (col0 + min(cols, KP_ROWS) - 1) / R) / KV4_PAGE + 1) - 1;
+  const int page_last = max(hi0, hi1);
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, KP_SOFTMAX);
+    for (int i = 0; i < KP_STAGES; ++i) mbar_init(&k_full[i], KP_DEQUANT), mbar_init(&k_empty[i], 2), mbar_init(&v_full[i], KP_DEQUANT), mbar_init(&v_empty[i], 2);
+    for (int i = 0; i < 4; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], KP_SOFTMAX / 2), mbar_init(&o_full[i], 1), s_none[i] = INT_MAX;
+    for (int i = 0; i < KP_DEQUANT * KP_RING; ++i) mbar_init(&r_full[i], 1);
+    *s_fail = 0;
+    fence_barrier_init();
+  }
+  if (warp == KP_SOFTMAX) tmem_alloc(tmem_ptr, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_ptr, 0);
+
+  if (warp >= KP_SOFTMAX + 2) {
+    // ===================== codes into operands =====================
+    const int sl = warp - KP_SOFTMAX - 2, t4 = lane & 3, g8 = lane >> 2;
+    const int32_t* table = a.table + (size_t)it.row * a.width + page0;
+    const uint8_t* from = a.blocks + (size_t)head * BYTES + sl * SLICE;
+    const size_t page_bytes = (size_t)a.G * BYTES;
+    const int units = page_last - page0 + 1;
+    uint8_t* mine = ring + sl * KP_RING * SLICE;
+    uint64_t* full = r_full + sl * KP_RING;
+    int entry = lane < units ? table[lane] : 0;
+#pragma unroll
+    for (int i = 0; i < KP_RING; ++i) {
+      const int page = __shfl_sync(0xffffffffu, entry, i);
+      if (lane == 0 && i < units) {
+        mbar_expect_tx(&full[i], SLICE);
+        bulk_load_1d(mine + i * SLICE, from + min(max(page, 0), a.pages - 1) * page_bytes, SLICE, &full[i]);
+      }
+    }
+    bool ok = true;
+    for (int n = 0; n < units; ++n) {
+      const int st = n % KP_RING, ks = n % KP_STAGES;
+      ok = __all_sync(0xffffffffu, kp_wait(&full[st], (n / KP_RING) & 1, s_fail, a.word, 1));
+      if (!ok) break;
+      const uint8_t* blk = mine + st * SLICE;
+      uint32_t kw[2][W], vw[2][W];
+      float2 kp[2][NG], vp[2][2][NG];                 // keys g8 + 8 x; values of slots 2 (t4 + 4 x) + e
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        uint32_t u[NG];
+        lds_words<W>(kw[x], blk + (g8 + 8 * x) * (D / 2) + t4 * 4 * W);
+        lds_words<W>(vw[x], blk + kv4_v_codes(D) + (t4 + 4 * x) * D + g8 * 4 * W);
+        lds_words<NG>(u, blk + kv4_k_params(D) + (g8 + 8 * x) * NG * 4);
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {                // (a slot behind the last key may hold anything)
+          kp[x][g] = bits_pair<T>(u[g]);
+          if ((page0 + n) * KV4_PAGE + KV4_SLICE * sl + g8 + 8 * x > last) kp[x][g] = make_float2(0.f, 0.f);
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          lds_words<NG>(u, blk + kv4_v_params(D, NG) + (2 * (t4 + 4 * x) + e) * NG * 4);
+          const int pos = (page0 + n) * KV4_PAGE + KV4_SLICE * sl + 2 * (t4 + 4 * x) + e;
+#pragma unroll
+          for (int g = 0; g < NG; ++g) {
+            vp[x][e][g] = bits_pair<T>(u[g]);
+            if (pos > last) vp[x][e][g] = make_float2(0.f, 0.f);
+            if (isnan(vp[x][e][g].y)) {
+              atomicMin(&s_none[g], pos);
+              vp[x][e][g] = make_float2(0.f, 0.f);
+            }
+          }
+        }
+      }
+      const int nxt = n + KP_RING;
+      if ((nxt & 31) == 0) entry = nxt + lane < units ? table[nxt + lane] : 0;
+      const int page = __shfl_sync(0xffffffffu, entry, nxt & 31);
+      __syncwarp();                                   // every lane has read the slice
+      if (lane == 0 && nxt < units) {
+        mbar_expect_tx(&full[st], SLICE);
+        bulk_load_1d(mine + st * SLICE, from + min(max(page, 0), a.pages - 1) * page_bytes, SLICE, &full[st]);
+      }
+      uint32_t rk = 0, rv = 0;
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int g = 0; g < NG; ++g) rk = max(rk, group_reach(kp[x][g])), rv = max(rv, max(group_reach(vp[x][0][g]), group_reach(vp[x][1][g])));
+      const int ek = slice_exponent(__reduce_max_sync(0xffffffffu, rk)), ev = slice_exponent(__reduce_max_sync(0xffffffffu, rv));
+      const float fk = pow2(-ek), fv = pow2(-ev);
+      // keys: row = slot, 8 bytes of four dimensions at a time
+      ok = __all_sync(0xffffffffu, kp_wait(&k_empty[ks], ((n / KP_STAGES) & 1) ^ 1, s_fail, a.word, 2));
+      if (!ok) break;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int r = KV4_SLICE * sl + g8 + 8 * x;
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+          const float2 p = kp[x][i * NG / W];
+          const __half2 s = __float2half2_rn(p.x * fk), lo = __float2half2_rn(p.y * fk);
+          uint8_t* row = sk + ks * Shape::K + (i >> 1) * KP_KBOX + r * 128;
+          const int c = 4 * (i & 1) + (t4 >> 1), b = 8 * (t4 & 1);      // 16-byte piece of dimensions 32 i + 4 t4 in the row, 8 bytes in it
+          *reinterpret_cast<uint2*>(row + ((c ^ (r & 7)) << 4) + b) = make_uint2(word_pair<0>(kw[x][i], s, lo), word_pair<1>(kw[x][i], s, lo));
+          *reinterpret_cast<uint2*>(row + (((c + 2) ^ (r & 7)) << 4) + b) = make_uint2(word_pair<2>(kw[x][i], s, lo), word_pair<3>(kw[x][i], s, lo));
+        }
+      }
+      if (lane == 0) s_ek[(n & (KP_EXPS - 1)) * 4 + sl] = ek, s_ev[(n & (KP_EXPS - 1)) * 4 + sl] = ev;
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&k_full[ks]);
+      // values: row = dimension, a pair of slots at a time
+      ok = __all_sync(0xffffffffu, kp_wait(&v_empty[ks], ((n / KP_STAGES) & 1) ^ 1, s_fail, a.word, 3));
+      if (!ok) break;
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+          const float2 p0 = vp[x][0][i * NG / W], p1 = vp[x][1][i * NG / W];
+          const __half2 s = __floats2half2_rn(p0.x * fv, p1.x * fv), lo = __floats2half2_rn(p0.y * fv, p1.y * fv);
+          uint8_t* at = sv + ks * Shape::V + (32 * i + g8) * 128 + (((2 * sl + x) ^ g8) << 4) + 4 * t4;
+          *reinterpret_cast<uint32_t*>(at) = word_pair<0>(vw[x][i], s, lo);
+          *reinterpret_cast<uint32_t*>(at + 8 * 128) = word_pair<1>(vw[x][i], s, lo);
+          *reinterpret_cast<uint32_t*>(at + 16 * 128) = word_pair<2>(vw[x][i], s, lo);
+          *reinterpret_cast<uint32_t*>(at + 24 * 128) = word_pair<3>(vw[x][i], s, lo);
+        }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&v_full[ks]);
+    }
+    if (!ok && lane == 0) let_issued_work_end();
+    __syncwarp();
+  } else if (warp >= KP_SOFTMAX) {
+    // ===================== MMA issuers, one thread per tile =====================
+    if (elect_one()) {
+      constexpr uint32_t idesc_s = instr_desc_f16(KP_ROWS, KV4_PAGE), idesc_o = instr_desc_f16(KP_ROWS, D);
+      const int i = warp - KP_SOFTMAX, myhi = i == 0 ? hi0 : hi1;
+      const uint32_t tm_s = tmem + TM_S + 128u * i, tm_o = tmem + TM_O + 128u * i;
+      const uint64_t qdesc = smem_desc_sw128(smem_u32(sq + i * NB * KP_QBOX));
+      const uint64_t kdesc0 = smem_desc_sw128(smem_u32(sk)), vdesc0 = smem_desc_sw128(smem_u32(sv));
+      const int units = page_last - page0 + 1;
+      auto scores = [&](int n) {
+        const int ks = n % KP_STAGES;
+        if (!kp_wait(&k_full[ks], (n / KP_STAGES) & 1, s_fail, a.word, 4)) return false;
+        tc_fence_after();
+        if (page0 + n <= myhi) {
+          const uint32_t d = tm_s + 64u * (n & 1);
+          const uint64_t kdesc = kdesc0 + (uint64_t)(ks * (Shape::K >> 4));
+#pragma unroll
+          for (int c = 0; c < NB; ++c)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              umma_bf16(d, qdesc + (uint64_t)(c * (KP_QBOX >> 4) + 2 * k), kdesc + (uint64_t)(c * (KP_KBOX >> 4) + 2 * k), idesc_s, (c | k) != 0 ? 1u : 0u);
+          umma_commit(&s_full[2 * i + (n & 1)]);
+          umma_commit(&k_empty[ks]);
+        } else {
+          mbar_arrive(&k_empty[ks]);
+        }
+        return true;
+      };
+      bool ok = kp_wait(q_full, 0, s_fail, a.word, 5);
+      if (ok && units > 0) ok = scores(0);
+      for (int n = 0; ok && n < units; ++n) {
+        if (n + 1 < units && !(ok = scores(n + 1))) break;
+        const int vs = n % KP_STAGES;
+        if (!(ok = kp_wait(&v_full[vs], (n / KP_STAGES) & 1, s_fail, a.word, 6))) break;
+        if (page0 + n <= myhi) {
+          const uint32_t buf = n & 1;
+          if (!(ok = kp_wait(&p_full[2 * i + (int)buf], (n >> 1) & 1u, s_fail, a.word, 7))) break;
+          tc_fence_after();
+          const uint64_t vdesc = vdesc0 + (uint64_t)(vs * (Shape::V >> 4));
+#pragma unroll
+          for (int k = 0; k < KV4_PAGE / UMMA_K; ++k)      // 16 keys: 8 columns of packed weights
+            umma_ts(tm_o, tm_s + 64u * buf + 32u * (k >> 1) + 8u * (k & 1), vdesc + (uint64_t)(2 * k), idesc_o, (n | k) != 0 ? 1u : 0u);
+          umma_commit(&o_full[2 * i + (int)buf]);
+          umma_commit(&v_empty[vs]);
+        } else {
+          mbar_arrive(&v_empty[vs]);
+        }
+      }
+      if (!ok) let_issued_work_end();
+    }
+    __syncwarp();
+  } else {
+    // ===================== queries, softmax, then the epilogue =====================
+    const int tile = warp >> 3, half = (warp >> 2) & 1, row = (int)(threadIdx.x & (KP_ROWS - 1));
+    const int c = col0 + tile * KP_ROWS + row, myhi = tile == 0 ? hi0 : hi1;
+    const bool live = tile * KP_ROWS + row < cols;
+    const int qp = it.pos0 + (live ? c : col0) / R;                     // position of the row's query
+    const size_t out_row = (size_t)(it.first + (live ? c : col0) / R) * a.H + head * R + (live ? c : col0) % R;
+    float* const own = s_x + (tile * 2 + half) * KP_ROWS + row;
+    const float* const other = s_x + (tile * 2 + (half ^ 1)) * KP_ROWS + row;
+    const int bar = 1 + tile * 4 + (warp & 3);
+    float mul;                                                          // what a raw score is multiplied by, to units of log2
+    {
+      constexpr int P = D / 16;                                         // 16-byte pieces of half a row
+      const T* q = (const T*)a.q + (long long)(it.first + (live ? c : col0) / R) * a.q_row + (size_t)(head * R + (live ? c : col0) % R) * D + half * (D / 2);
+      uint4 u[P];
+      float mx = 0.f;
+#pragma unroll
+      for (int e = 0; e < P; ++e) {
+        u[e] = live ? reinterpret_cast<const uint4*>(q)[e] : make_uint4(0u, 0u, 0u, 0u);
+        const uint32_t w[4] = {u[e].x, u[e].y, u[e].z, u[e].w};
+#pragma unroll
+        for (int z = 0; z < 4; ++z) {
+          const float2 f = bits_pair<T>(w[z]);
+          mx = fmaxf(mx, fmaxf(fabsf(f.x), fabsf(f.y)));
+        }
+      }
+      *own = mx;
+      at_any(bar, false);
+      mx = fmaxf(mx, *other);
+      at_any(bar, false);
+      const int ex = min(max((int)(__float_as_uint(mx) >> 23), 15), 240);
+      const float up = pow2(127 + 14 - ex);                             // the row's largest comes to 2^14 .. 2^15
+      mul = pow2(ex - 127 - 14) * (a.scale * AT_LOG2E);
+      uint8_t* to = sq + (tile * NB + (NB == 2 ? half : 0)) * KP_QBOX + row * 128;
+#pragma unroll
+      for (int e = 0; e < P; ++e) {
+        const uint32_t w[4] = {u[e].x, u[e].y, u[e].z, u[e].w};
+        uint32_t h[4];
+#pragma unroll
+        for (int z = 0; z < 4; ++z) {
+          const float2 f = bits_pair<T>(w[z]);
+          h[z] = pair_bits<__half>(f.x * up, f.y * up);
+        }
+        const int piece = (NB == 2 ? 0 : half * P) + e;
+        *reinterpret_cast<uint4*>(to + ((piece ^ (row & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+    }
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t ts0 = tmem + lanes + TM_S + 128u * tile, to = tmem + lanes + TM_O + 128u * tile;
+    float ref = -INFINITY, sum = 0.f;
+    int ebase = -128;                                                   // the power of two that O stands under
+    bool ok = true;
+    const int count = max(0, myhi - page0 + 1);
+    for (int n = 0; n < count; ++n) {
+      const uint32_t ts = ts0 + 64u * (n & 1);
+      ok = kp_wait(&s_full[2 * tile + (n & 1)], (n >> 1) & 1, s_fail, a.word, 8);
+      __syncwarp();
+      tc_fence_after();
+      uint32_t sr[32];
+      tmem_ld32_async(ts + 32u * half, sr);
+      const int* ek = s_ek + (n & (KP_EXPS - 1)) * 4 + 2 * half;
+      const int4 ev = *reinterpret_cast<const int4*>(s_ev + (n & (KP_EXPS - 1)) * 4);
+      const int emax = max(max(ev.x, ev.y), max(ev.z, ev.w)), ev0 = half ? ev.z : ev.x, ev1 = half ? ev.w : ev.y;
+      const float mul0 = mul * pow2(ek[0]), mul1 = mul * pow2(ek[1]);   // of the two slices
+      tmem_wait_ld();
+      tie32(sr);
+      const int cmax = qp - ((page0 + n) * KV4_PAGE + 32 * half);       // the row's last visible column of these 32
+      const bool masked = __any_sync(0xffffffffu, cmax < 31);
+      if (masked) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+          if (e > cmax) sr[e] = __float_as_uint(-INFINITY);
+      }
+      float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int e = 0; e < 32; e += 2) m4[e >> 3] = at_max3(m4[e >> 3], __uint_as_float(sr[e]), __uint_as_float(sr[e + 1]));
+      float mx = fmaxf(fmaxf(m4[0], m4[1]) * mul0, fmaxf(m4[2], m4[3]) * mul1);
+      __syncwarp();      // the stores to tensor memory below are the whole warp's: lanes part above this line and not between it and them
+      // (one barrier of the rows' two warps per page: does any row's reference have to move, or the exponent, has any wait run out?)
+      if (at_any(bar, !ok || mx > ref + AT_SLACK || (ref == -INFINITY && mx > -INFINITY) || emax > ebase)) {
+        *own = mx;
+        ok = !at_any(bar, !ok);
+        if (!ok) break;
+        const float nref = fmaxf(ref, fmaxf(mx, *other));
+        const int nbase = max(ebase, emax);
+        const float g = ref == -INFINITY ? 0.f : at_exp2(ref - nref), f = g * pow2(max(ebase - nbase, -126));
+        ref = nref;
+        ebase = nbase;
+        sum *= g;
+        if (n > 0) ok = kp_wait(&o_full[2 * tile + ((n - 1) & 1)], ((n - 1) >> 1) & 1, s_fail, a.word, 9);
+        __syncwarp();
+        tc_fence_after();
+        if (at_any(bar, !ok)) {                                         // (also: both threads of a row have read the other's)
+          ok = false;
+          break;
+        }
+        if (n > 0) {                                                    // what the pages before have added up
+#pragma unroll 1
+          for (int z = 32 * half; z < D; z += 64) {
+            uint32_t o[32];
+            tmem_ld32_async(to + (uint32_t)z, o);
+            tmem_wait_ld();
+            tie32(o);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            tmem_st16(to + (uint32_t)z, o);
+            tmem_st16(to + (uint32_t)z + 16u, o + 16);
+          }
+        }
+      }
+      const float sub = ref == -INFINITY ? 0.f : -ref;
+      uint32_t ph[16];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {                                     // the two slices
+        const float mm = x ? mul1 : mul0, shift = sub + (float)((x ? ev1 : ev0) - ebase);
+        const f2 m2 = f2_of(mm, mm), s2 = f2_of(shift, shift);
+        f2 part = f2_of(0.f, 0.f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float a0, a1;
+          f2_split(f2_fma(f2_of(__uint_as_float(sr[16 * x + 2 * e]), __uint_as_float(sr[16 * x + 2 * e + 1])), m2, s2), a0, a1);
+          ph[8 * x + e] = pair_bits<__half>(at_exp2(a0), at_exp2(a1));
+          const float2 p = bits_pair<__half>(ph[8 * x + e]);            // the sum is of the weights as the product sees them
+          part = f2_add(part, f2_of(p.x, p.y));
+        }
+        float p0, p1;
+        f2_split(part, p0, p1);
+        sum = fmaf(p0 + p1, pow2(min(ebase - (x ? ev1 : ev0), 126)), sum);
+      }
+      // the weights go over the thread's own scores
+      tmem_st16(ts + 32u * half, ph);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[2 * tile + (n & 1)]);
+    }
+    if (ok && count > 0) ok = kp_wait(&o_full[2 * tile + ((count - 1) & 1)], ((count - 1) >> 1) & 1, s_fail, a.word, 10);
+    __syncwarp();
+    tc_fence_after();
+    *own = sum;
+    if (!at_any(bar, !ok)) {
+      const float den = half == 0 ? sum + *other : *other + sum;        // the halves' sums in the order of the keys
+      const size_t part_at = ((size_t)(it.base + it.part) * a.G + head) * KV4_MANY + tile * KP_ROWS + row;
+      const bool whole = it.parts == 1;
+      if (!whole && live && half == 0)
+        *reinterpret_cast<float2*>(a.part + (size_t)a.max_items * a.G * KV4_MANY * D + part_at * 2) = make_float2(ref == -INFINITY ? KV4_NONE : ref, den);
+      const float fin = pow2(max(min(ebase, 126), -126)) / (whole ? den : 1.f);
+      if (count > 0) {
+#pragma unroll
+        for (int z = 32 * half; z < D; z += 64) {
+          uint32_t o[32];
+          tmem_ld32_async(to + (uint32_t)z, o);
+          tmem_wait_ld();
+          tie32(o);
+          const float f = s_none[z * NG / D] <= qp ? NAN : fin;         // (a value that is none, at a position that the row sees)
+          if (live) {
+            if (whole) {
+              T* dst = y + out_row * D + z;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                uint32_t w[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[j] = pair_bits<T>(__uint_as_float(o[8 * e + 2 * j]) * f, __uint_as_float(o[8 * e + 2 * j + 1]) * f);
+                *reinterpret_cast<uint4*>(dst + 8 * e) = make_uint4(w[0], w[1], w[2], w[3]);
+              }
+            } else {
+              float* dst = a.part + part_at * D + z;
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                *reinterpret_cast<float4*>(dst + 4 * e) = make_float4(__uint_as_float(o[4 * e]) * f, __uint_as_float(o[4 * e + 1]) * f,
+                                                                      __uint_as_float(o[4 * e + 2]) * f, __uint_as_float(o[4 * e + 3]) * f);
+            }
+          }
+          __syncwarp();
+        }
+      }
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (warp == KP_SOFTMAX) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <typename T, int D, int NG>
+int prompt_launch(const Kv4Attn& a, cudaStream_t st) {
+  constexpr int smem = KpShape<D, NG>::SMEM;
+  static_assert(smem <= 227 * 1024, "shared memory of a block");
+  static PerDevice set;
+  if (!set) {
+    LL_CUDA(cudaFuncSetAttribute(kv4_prompt_kernel<T, D, NG>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    set.mark();
+  }
+  kv4_prompt_kernel<T, D, NG><<<(unsigned)(a.max_items * a.G), KP_THREADS, smem, st>>>(a);
+  LL_LAUNCH_OK("kv4_prompt_kernel");
+  return LL_OK;
+}
+
+}  // namespace
+
+int kv4_prompt_launch(const Kv4Attn& a, int dtype, int head_size, int group, cudaStream_t st) {
+#define PROMPT(DD, NG)                                            \
+  if (head_size == DD && group == DD / NG) {                      \
+    if (dtype == LL_BF16) return prompt_launch<__nv_bfloat16, DD, NG>(a, st); \
+    return prompt_launch<__half, DD, NG>(a, st);                  \
+  }
+  PROMPT(64, 1) PROMPT(64, 2) PROMPT(128, 1) PROMPT(128, 2) PROMPT(128, 4)
+#undef PROMPT
+  set_error("kv4_attn: no prompt kernel for heads of %d in groups of %d", head_size, group);
+  return LL_ERR_UNSUPPORTED;
+}
+
+}  // namespace llb

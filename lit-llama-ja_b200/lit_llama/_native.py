@@ -125,10 +125,10 @@ EXPORTS = {
     "ll_kv4_truncate": ([vp, vp, i32, vp, vp, vp, vp, vp, i32, i32, i32, i32, vp], C.c_int),
     "ll_kv4_append": ([vp, i64, vp, i64, vp, i64, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp], C.c_int),
     "ll_kv4_read": ([vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp], C.c_int),
-    "ll_kv4_work_ints": ([i32, i32, i32, i32, i32], sz_t),
-    "ll_kv4_work": ([vp, i32, i32, i32, i32, i32, i32, vp, vp], C.c_int),
+    "ll_kv4_work_ints": ([i32, i32, i32, i32, i32, i32], sz_t),
+    "ll_kv4_work": ([vp, i32, i32, i32, i32, i32, i32, i32, vp, vp], C.c_int),
     "ll_kv4_attn_scratch_bytes": ([i32, i32, i32, i32, i32, i32], sz_t),
-    "ll_kv4_attn": ([vp, i64, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, i32, i32, i32, C.c_float, vp, vp], C.c_int),
+    "ll_kv4_attn": ([vp, i64, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, i32, i32, i32, C.c_float, vp, vp], C.c_int),
     "ll_embed_ssq": ([vp, vp, vp, vp, i32, i32, vp], C.c_int),
     "ll_rope_kv_append": ([vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp], C.c_int),
     "ll_decode_attn": ([vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp, vp, i32, vp], C.c_int),

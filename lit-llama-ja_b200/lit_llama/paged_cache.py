@@ -37,7 +37,7 @@ class CachePlan:
 
     def __init__(self, cache: "PagedCache4", B: int, T: int, max_count: int):
         self.cache, self.B, self.T, self.max_count, self.step = cache, B, T, max_count, cache._step
-        work = N.call_ret("ll_kv4_work_ints", B, T, max_count, cache.n_head, cache.n_kv_head)
+        work = N.call_ret("ll_kv4_work_ints", B, T, max_count, cache.n_head, cache.n_kv_head, cache.head_size)
         data = torch.empty(work + 4 * B + 1 + 3 * T, dtype=torch.int32, device=cache.device)
         self.work, self.starts, self.ends, self.status, self.request, self.positions, self.slots, self.sequence = data.split([work, B + 1, B, B, B, T, T, T])
 
@@ -106,7 +106,7 @@ class PagedCache4:
             self._step += 1
             plan = CachePlan(self, rows.numel(), tokens, min(max_count, tokens))
             N.call("ll_kv4_plan", N.ptr(rows), N.ptr(counts), plan.B, tokens, plan.max_count, *self._pool, N.ptr(plan.starts), N.stream())
-            N.call("ll_kv4_work", N.ptr(plan.starts), plan.B, tokens, plan.max_count, self.n_head, self.n_kv_head, self.max_length, N.ptr(plan.work), N.stream())
+            N.call("ll_kv4_work", N.ptr(plan.starts), plan.B, tokens, plan.max_count, self.n_head, self.n_kv_head, self.head_size, self.max_length, N.ptr(plan.work), N.stream())
         return plan
 
     def truncate(self, rows: Whole, lengths: Whole) -> None:
@@ -199,6 +199,6 @@ class PagedCache4:
         with torch.cuda.device(self.device):
             shape = (plan.B, T, plan.max_count, self.n_head, self.n_kv_head, self.head_size)
             scratch = torch.empty(N.call_ret("ll_kv4_attn_scratch_bytes", *shape), dtype=torch.uint8, device=self.device)
-            N.call("ll_kv4_attn", N.ptr(q), q.stride(0), self._layers[layer], N.ptr(self.table), N.ptr(plan.starts), N.ptr(plan.work), N.ptr(out), self._code, *shape,
+            N.call("ll_kv4_attn", N.ptr(q), q.stride(0), self._layers[layer], N.ptr(self.table), N.ptr(plan.work), N.ptr(out), self._code, *shape,
                    self.group, self.width, self.pages, scale, N.ptr(scratch), N.stream())
         return out

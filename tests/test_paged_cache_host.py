@@ -45,9 +45,9 @@ A = 1 << 12      # an address that no launch reads
     ("ll_kv4_append", (0, 0, A, 65, A, 64, 0, A, A, 0, A, 1, 1, 1, 1, 64, 64, 0)),
     ("ll_kv4_append", (0, 0, A, 64, A, 64, A, A, A, A, A, 1, 1, 1, 1, 64, 64, 0)),     # a table and no queries
     ("ll_kv4_read", (A, A, A, A, 1, 0, 1, 64, 64, 1, 0)),
-    ("ll_kv4_attn", (A, 64, A, A, A, A, A, 1, 1, 1, 1, 3, 2, 64, 64, 1, 1, 1.0, A, 0)),         # three heads over two
-    ("ll_kv4_attn", (A, 64, A, A, A, A, A, 0, 1, 1, 1, 2, 2, 64, 64, 1, 1, 1.0, A, 0)),         # fp32
-    ("ll_kv4_attn", (A, 60, A, A, A, A, A, 1, 1, 1, 1, 2, 2, 64, 64, 1, 1, 1.0, A, 0)),
+    ("ll_kv4_attn", (A, 64, A, A, A, A, 1, 1, 1, 1, 3, 2, 64, 64, 1, 1, 1.0, A, 0)),         # three heads over two
+    ("ll_kv4_attn", (A, 64, A, A, A, A, 0, 1, 1, 1, 2, 2, 64, 64, 1, 1, 1.0, A, 0)),         # fp32
+    ("ll_kv4_attn", (A, 60, A, A, A, A, 1, 1, 1, 1, 2, 2, 64, 64, 1, 1, 1.0, A, 0)),
 ])
 def test_refused_calls(name, args):
     with pytest.raises(RuntimeError, match="kv4"):
