@@ -836,41 +836,47 @@ LL_API int ll_softmax_layer(const void* x, const void* w_in, int n_in, const voi
                             int chunk, int ring, int splits, int form, void* out, void* scratch, ll_stream stream);
 
 /* ---------------------------------------------------------------------------------------
- * Key/value cache in 4 bits, in pages of 64 slots that requests of unequal lengths share (csrc/paged_kv4.cu, csrc/paged_attn.cu).
+ * Key/value cache in 4 bits, in pages of 64 slots that requests of unequal lengths share (csrc/paged_kv4.cu, csrc/paged_attn.cu,
+ * csrc/paged_prompt.cu).
  * A group of values x (32, 64 or 128 dimensions of a head of 32, 64 or 128; bf16 or fp16, the type T of queries and parameters too) is held as codes of
  * 4 bits, a scale s and its smallest value lo:  s = T((max(x) - lo) * (1/15)), code = min(max(rint((x - lo) / s), 0), 15) in fp32 (0 where s is 0); it stands
- * for code * s + lo.  A group with a number that is infinite or none stands for no numbers.
- *   blocks [pages][G heads][ll_kv4_page_bytes]: codes and parameters of one layer (layout: csrc/kv4.cuh)
- *   table [requests][width]: page of 64 slots, or -1;  lengths [requests]: tokens held;  free [pages]: stack of pages, the last of n_free[0] is next;
- *   stamp [requests]: scratch of plan and truncate.  One step at a time plans, truncates and appends on a pool.
- * ll_kv4_plan: sequence i of a step brings counts[i] tokens (the next ones of the step's T rows) for request rows[i]; pages are given out in the order of
- * the sequences.  Status: 0 done; 1 the pages did not suffice (nor for any later sequence that needs one); 2 longer than max_length, or more than
+ * for code * s + lo.  A group with a number that is infinite or none stands for no numbers. */
+typedef struct ll_kv4_cache {  /* on the host; its pointers on the device */
+  int32_t* table;              /* [requests][width] page of 64 slots, or -1 */
+  int32_t* lengths;            /* [requests] tokens held */
+  int32_t* free_pages;         /* [pages] a stack: the last of n_free[0] is given out next */
+  int32_t* n_free;             /* [1] */
+  int32_t* stamp;              /* [requests] scratch of plan and truncate */
+  int32_t requests, width, pages, max_length;
+  int32_t heads, kv_heads, head_size, group, dtype;
+} ll_kv4_cache;
+/* Bytes of one head's part of a page; a layer's blocks are [pages][kv_heads][ll_kv4_page_bytes] (layout: csrc/kv4.cuh).  0: no such shape. */
+LL_API size_t ll_kv4_page_bytes(int head_size, int group);
+/* Sequence i of a step brings counts[i] tokens (the next ones of the step's T rows) for request rows[i]; pages are given out in the order of the
+ * sequences.  Status: 0 done; 1 the pages did not suffice (nor for any later sequence that needs one); 2 longer than max_length, or more than
  * max_count tokens; 3 no such request, or one that an earlier sequence names, or a negative count; 4 tokens behind row T.  A sequence that is refused
  * gets nothing.  out: starts [B + 1] (up to T), ends [B] (tokens held after the step; 0 refused), status [B], request [B] (-1: refused, or no
- * tokens), positions [T], slots [T] (page * 64 + place; -1: refused, or behind the last token), sequence [T].
- * ll_kv4_truncate: request rows[i] keeps its first keep[i] tokens (a request named twice: the first; keep < 0 or at least the length: nothing to do);
- * the pages behind go back so that the next plan gives them out in the same order. */
-LL_API size_t ll_kv4_page_bytes(int head_size, int group);
-LL_API int ll_kv4_plan(const int32_t* rows, const int32_t* counts, int B, int T, int max_count, int32_t* table, int32_t* lengths, int32_t* free_pages,
-                       int32_t* n_free, int32_t* stamp, int requests, int width, int pages, int max_length, int32_t* out, ll_stream stream);
-LL_API int ll_kv4_truncate(const int32_t* rows, const int32_t* keep, int B, int32_t* table, int32_t* lengths, int32_t* free_pages, int32_t* n_free,
-                           int32_t* stamp, int requests, int width, int pages, int max_length, ll_stream stream);
-/* Rounds k and v [T] rows of G heads into their slots.  rope (fp32 [positions][D/2][2] of cos, sin; pairs of neighbours) or null: keys are turned before
- * and queries, H heads, into q_out [T][H][D].  Distances of rows in numbers.  A token without a slot writes nothing, and its queries are no numbers. */
-LL_API int ll_kv4_append(const void* q, long long q_row, const void* k, long long k_row, const void* v, long long v_row, const float* rope,
-                         const int32_t* positions, const int32_t* slots, void* q_out, void* blocks, int dtype, int T, int H, int G, int head_size, int group,
-                         ll_stream stream);
-/* The values that slots stand for, k, v [n][G][D]; no numbers for a slot that there is not. */
-LL_API int ll_kv4_read(const void* blocks, const int32_t* slots, void* k, void* v, int dtype, int n, int G, int head_size, int group, int pages, ll_stream stream);
-/* Softmax attention of the plan's tokens: q rows of H heads, y [T][H][D]; a token sees its request's keys at and before its position.  Tokens of refused
- * sequences are no numbers, rows behind the last token are left as they are.  work: ll_kv4_work's division of the step's walks over keys, made from
- * ll_kv4_plan's out (plan) for sequences that bring up to max_count tokens, the same for every layer; ll_kv4_work_ints numbers on a 16-byte boundary. */
-LL_API size_t ll_kv4_work_ints(int B, int T, int max_count, int H, int G, int head_size);
-LL_API int ll_kv4_work(const int32_t* plan, int B, int T, int max_count, int H, int G, int head_size, int max_length, int32_t* work, ll_stream stream);
-LL_API size_t ll_kv4_attn_scratch_bytes(int B, int T, int max_count, int H, int G, int head_size);
-LL_API int ll_kv4_attn(const void* q, long long q_row, const void* blocks, const int32_t* table, const int32_t* work, void* y, int dtype, int B, int T,
-                       int max_count, int H, int G, int head_size, int group, int width, int pages, float scale, void* scratch,
+ * tokens), positions [T], slots [T] (page * 64 + place; -1: refused, or behind the last token).  work: the division of the step's attention among blocks,
+ * the same for every layer; ll_kv4_work_ints numbers on a 16-byte boundary.  One step at a time plans, truncates and appends on a cache. */
+LL_API size_t ll_kv4_work_ints(const ll_kv4_cache* cache, int B, int T, int max_count);
+LL_API int ll_kv4_plan(const ll_kv4_cache* cache, const int32_t* rows, const int32_t* counts, int B, int T, int max_count, int32_t* out, int32_t* work,
                        ll_stream stream);
+/* Request rows[i] keeps its first keep[i] tokens (a request named twice: the first; keep < 0 or at least the length: nothing to do); the pages behind go
+ * back so that the next plan gives them out in the same order. */
+LL_API int ll_kv4_truncate(const ll_kv4_cache* cache, const int32_t* rows, const int32_t* keep, int B, ll_stream stream);
+/* Rounds k and v, T rows of kv_heads, into their slots of a layer's blocks.  rope (fp32 [positions][D/2][2] of cos, sin; pairs of neighbours) or null:
+ * keys are turned before, and queries into q_out [T][heads][D].  Distances of rows in numbers.  A token without a slot writes nothing, and its queries are
+ * no numbers. */
+LL_API int ll_kv4_append(const ll_kv4_cache* cache, void* blocks, const void* q, long long q_row, const void* k, long long k_row, const void* v,
+                         long long v_row, const float* rope, const int32_t* positions, const int32_t* slots, void* q_out, int T, ll_stream stream);
+/* The values that n slots stand for, k, v [n][kv_heads][D]; no numbers for a slot that there is not. */
+LL_API int ll_kv4_read(const ll_kv4_cache* cache, const void* blocks, const int32_t* slots, void* k, void* v, int n, ll_stream stream);
+/* Softmax attention of a plan's tokens: q rows of the heads, y [T][heads][D]; a token sees its request's keys at and before its position.  Tokens of
+ * refused sequences are no numbers, rows behind the last token are left as they are.  B, T, max_count: the plan's.  Of up to 32 queries of a key
+ * head a sequence's walk is by mma.sync, of more by tcgen05, whose operands are fp16. */
+LL_API size_t ll_kv4_attn_scratch_bytes(const ll_kv4_cache* cache, int B, int T, int max_count);
+LL_API int ll_kv4_attn(const ll_kv4_cache* cache, const void* blocks, const void* q, long long q_row, const int32_t* work, void* y, int B, int T,
+                       int max_count, float scale, void* scratch, ll_stream stream);
 
 #ifdef __cplusplus
 }

@@ -495,181 +495,34 @@ __global__ void __launch_bounds__(KJ * 32) kv4_join_many_kernel(const Kv4Attn a)
   }
 }
 
-// ------------------------------------------------------------------ the division of a step's walks
-constexpr int KW_THREADS = 1024;
-
-__device__ __forceinline__ int block_sum(int v, int* s_warp) {
-  v = __reduce_add_sync(0xffffffffu, v);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) s_warp[threadIdx.x >> 5] = v;
-  __syncthreads();
-  return __reduce_add_sync(0xffffffffu, s_warp[threadIdx.x & 31]);
-}
-
-// Parts of `step` pages at most, step the smallest with which a step's walks make no more than `parts` parts, as many as there are places for blocks, or
-// where the walks are more than half of that are cut no more than `parts` times.  Parts of a size stand together, the largest first: blocks take them in
-// that order, and the short ones fill the end.
-// MANY false: the sequences of up to `few` columns, a thread each, whose tiles count as long as the last one; true: the others, a warp each.
-constexpr int KW_SIZES = 512;           // sizes told apart (larger ones by their 1 / KW_SIZES of the largest)
-template <bool MANY>
-__global__ void __launch_bounds__(KW_THREADS) kv4_work_kernel(const int32_t* __restrict__ starts, const int32_t* __restrict__ ends,
-                                                             const int32_t* __restrict__ request, int B, int R, int few, int cols, int longest, int parts,
-                                                             int max_items, int32_t* __restrict__ work) {
-  __shared__ int s_warp[32], s_size[KW_SIZES];
-  const int lane = threadIdx.x & 31, first = MANY ? threadIdx.x >> 5 : threadIdx.x, by = MANY ? KW_THREADS / 32 : KW_THREADS;
-  auto tokens = [&](int i) { return starts[i + 1] - starts[i]; };
-  auto tiles = [&](int i) {
-    const long long c = (long long)tokens(i) * R;
-    return (c > few) == MANY ? (int)((c + cols - 1) / cols) : 0;
-  };
-  // pages that a tile's last column sees
-  auto pages = [&](int i, int tile) {
-    if (request[i] < 0) return 1;
-    const int n = tokens(i);
-    return (ends[i] - n + (MANY ? (int)min((long long)n - 1, ((long long)(tile + 1) * cols - 1) / R) : n - 1)) / KV4_PAGE + 1;
-  };
-  auto total = [&](int step) {
-    int v = 0;
-    for (int i = first; i < B; i += by) {
-      const int w = tiles(i);
-      if (MANY)
-        for (int t = lane; t < w; t += 32) v += (pages(i, t) + step - 1) / step;
-      else if (w > 0)
-        v += w * ((pages(i, 0) + step - 1) / step);
-    }
-    return block_sum(v, s_warp);
-  };
-  const int all = total(max(1, longest)), most = 2 * (long long)all > parts ? all + parts : parts;
-  int step = 1, hi = max(1, longest);
-  if (all >= 4ll * parts) step = hi;    // (walks for several rounds even out by themselves)
-  while (step < hi) {
-    const int mid = (step + hi) >> 1;
-    if (total(mid) <= most) hi = mid;
-    else step = mid + 1;
-  }
-  // a walk's pages in equal parts; the places of the sizes, counted and summed from the largest down
-  auto cut = [&](int p) { return (p + step - 1) / step; };
-  auto bucket = [&](int size) { return KW_SIZES - 1 - (int)((long long)(min(size, step) - 1) * KW_SIZES / step); };
-  for (int x = threadIdx.x; x < KW_SIZES; x += KW_THREADS) s_size[x] = 0;
-  __syncthreads();
-  for (int i = first; i < B; i += by) {
-    const int w = tiles(i);
-    for (int t = MANY ? lane : 0; t < (MANY ? w : min(w, 1)); t += 32) {
-      const int p = pages(i, t), k = cut(p);
-      atomicAdd(&s_size[bucket((p + k - 1) / k)], MANY ? k : w * k);
-    }
-  }
-  __syncthreads();
-  if (threadIdx.x < 32) {
-    int before = 0;
-    for (int x0 = 0; x0 < KW_SIZES; x0 += 32) {
-      const int v = s_size[x0 + threadIdx.x];
-      int incl = v;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, incl, d);
-        if (lane >= d) incl += u;
-      }
-      s_size[x0 + threadIdx.x] = before + incl - v;
-      before += __shfl_sync(0xffffffffu, incl, 31);
-    }
-    if (threadIdx.x == 0) work[0] = min(before, max_items);
-  }
-  __syncthreads();
-  // (which of the parts of one size comes first is left to chance, and of no consequence: every part has its own place for its sums)
-  for (int i = threadIdx.x >> 5; i < B; i += KW_THREADS / 32) {
-    const int w = tiles(i), n = tokens(i), row = request[i], pos0 = ends[i] - n;
-    if (w == 0) continue;
-    auto store = [&](int at, int tile, int part, int each, int k, int base) {
-      if (at >= max_items) return;
-      int4* o = reinterpret_cast<int4*>(work) + 1 + 3 * (size_t)at;
-      o[0] = make_int4(row, starts[i], n, pos0);
-      o[1] = make_int4(tile, part * each, (part + 1) * each, k);
-      o[2] = make_int4(part, base, 0, 0);
-    };
-    if (MANY) {
-      for (int t = lane; t < w; t += 32) {
-        const int p = pages(i, t), k = cut(p), each = (p + k - 1) / k, at = atomicAdd(&s_size[bucket(each)], k);
-        for (int e = 0; e < k; ++e) store(at + e, t, e, each, k, at);
-      }
-    } else {
-      const int p = pages(i, 0), k = cut(p), each = (p + k - 1) / k;
-      int at = 0;
-      if (lane == 0) at = atomicAdd(&s_size[bucket(each)], w * k);
-      at = __shfl_sync(0xffffffffu, at, 0);
-      for (int e = lane; e < w * k; e += 32) store(at + e, e / k, e % k, each, k, at + e / k * k);
-    }
-  }
-}
-
 }  // namespace
-
-// A step's two lists: sequences of few columns and, where one may bring more, of many.  Sizes as the host knows them.
-struct Kv4Lists {
-  int R, cols, few, few_parts, many_parts;
-  long long few_items, many_items;      // at most
-  bool many;
-  Kv4Lists(int B, int T, int max_count, int H, int G, int head_size) {
-    R = H / G;
-    many = kv4_many(max_count, R, head_size);
-    const long long c = (long long)max_count * R;
-    cols = many ? 8 : c <= 4 ? 4 : c <= 8 ? 8 : 16;
-    few = many ? KV4_FEW_MOST : INT_MAX;
-    few_parts = max(1, 4 * kv4_sms() / G);
-    many_parts = max(1, kv4_sms() / G);
-    const long long each = many ? (KV4_FEW_MOST + cols - 1) / cols : T, seqs = min(B, max(T, 1));
-    few_items = min((long long)T * R / cols + seqs, seqs * each) + few_parts;
-    many_items = many ? (long long)T * R / KV4_MANY + min((long long)seqs, (long long)T * R / KV4_FEW_MOST) + many_parts : 0;
-  }
-  size_t few_ints() const { return 4 + sizeof(Kv4Item) / 4 * (size_t)few_items; }
-  size_t ints() const { return few_ints() + (many ? 4 + sizeof(Kv4Item) / 4 * (size_t)many_items : 0); }
-  size_t few_floats(int G, int D) const { return ((size_t)few_items * G * cols * (D + 2) + 3) / 4 * 4; }
-  size_t floats(int G, int D) const { return few_floats(G, D) + (size_t)many_items * G * KV4_MANY * (D + 2); }
-};
-
 }  // namespace llb
 
 using namespace llb;
 
 extern "C" {
 
-size_t ll_kv4_work_ints(int B, int T, int max_count, int H, int G, int head_size) { return Kv4Lists(B, T, max_count, H, G, head_size).ints(); }
-
-int ll_kv4_work(const int32_t* plan, int B, int T, int max_count, int H, int G, int head_size, int max_length, int32_t* work, ll_stream stream) {
-  LL_CHECK_ARG(plan && work && B > 0 && T >= 0 && max_count >= 0 && G > 0 && H > 0 && H % G == 0 && max_length > 0, "kv4_work: %d sequences of %d tokens, %d heads over %d",
-               B, T, H, G);
-  const Kv4Lists l(B, T, max_count, H, G, head_size);
-  const int32_t *ends = plan + B + 1, *request = plan + 3 * (size_t)B + 1;
-  const int longest = (max_length + KV4_PAGE - 1) / KV4_PAGE;
-  LL_CHECK_ARG(l.few_items * G < 0x7fffffffll && l.many_items * G < 0x7fffffffll, "kv4_work: %d sequences of %d tokens, %d heads", B, T, H);
-  kv4_work_kernel<false><<<1, KW_THREADS, 0, (cudaStream_t)stream>>>(plan, ends, request, B, l.R, l.few, l.cols, longest, l.few_parts, (int)l.few_items, work);
-  LL_LAUNCH_OK("kv4_work_kernel");
-  if (l.many) {
-    kv4_work_kernel<true><<<1, KW_THREADS, 0, (cudaStream_t)stream>>>(plan, ends, request, B, l.R, l.few, KV4_MANY, longest, l.many_parts, (int)l.many_items,
-                                                                      work + l.few_ints());
-    LL_LAUNCH_OK("kv4_work_kernel");
-  }
-  return LL_OK;
+size_t ll_kv4_attn_scratch_bytes(const ll_kv4_cache* cache, int B, int T, int max_count) {
+  return sizeof(float) * Kv4Lists(B, T, max_count, cache->heads, cache->kv_heads, cache->head_size, cache->max_length).floats(cache->kv_heads, cache->head_size);
 }
 
-size_t ll_kv4_attn_scratch_bytes(int B, int T, int max_count, int H, int G, int head_size) {
-  return sizeof(float) * Kv4Lists(B, T, max_count, H, G, head_size).floats(G, head_size);
-}
-
-int ll_kv4_attn(const void* q, long long q_row, const void* blocks, const int32_t* table, const int32_t* work, void* y, int dtype, int B, int T,
-                int max_count, int H, int G, int head_size, int group, int width, int pages, float scale, void* scratch, ll_stream stream) {
+int ll_kv4_attn(const ll_kv4_cache* cache, const void* blocks, const void* q, long long q_row, const int32_t* work, void* y, int B, int T, int max_count,
+                float scale, void* scratch, ll_stream stream) {
+  LL_CHECK_ARG(cache != nullptr, "kv4_attn: no cache");
+  const int dtype = cache->dtype, H = cache->heads, G = cache->kv_heads, head_size = cache->head_size, group = cache->group;
   LL_CHECK_ARG(kv4_shape_ok(head_size, group), "kv4_attn: heads of %d in groups of %d (32, 64 or 128 each)", head_size, group);
   LL_CHECK_ARG(dtype == LL_BF16 || dtype == LL_F16, "kv4_attn: type %d (bf16 or fp16)", dtype);
-  LL_CHECK_ARG(q && blocks && table && work && y && scratch && B > 0 && T > 0 && max_count >= 0 && G > 0 && G <= 65535 && H > 0 && H % G == 0 && width > 0 && pages > 0,
+  LL_CHECK_ARG(q && blocks && cache->table && work && y && scratch && B > 0 && T > 0 && max_count >= 0 && G > 0 && G <= 65535 && H > 0 && H % G == 0 && cache->width > 0 &&
+                   cache->pages > 0 && cache->max_length > 0 && (long long)T * H <= INT_MAX,
                "kv4_attn: %d tokens of %d heads, %d cached", T, H, G);
   LL_CHECK_ARG(scale > 0.f, "kv4_attn: scores times %g (more than 0)", scale);
   LL_CHECK_ARG((((uintptr_t)q | (uintptr_t)y | (uintptr_t)blocks | (uintptr_t)scratch | (uintptr_t)work) & 15) == 0 && q_row % 8 == 0,
                "kv4_attn: rows have to start on 16-byte boundaries");
-  const Kv4Lists l(B, T, max_count, H, G, head_size);
-  LL_CHECK_ARG(l.few_items * G < 0x7fffffffll && l.many_items * G < 0x7fffffffll, "kv4_attn: %d sequences of %d tokens, %d heads", B, T, H);
+  const Kv4Lists l(B, T, max_count, H, G, head_size, cache->max_length);
+  LL_CHECK_ARG(l.few_items * G <= INT_MAX && l.many_items * G <= INT_MAX, "kv4_attn: %d sequences of %d tokens, %d heads", B, T, H);
   const int R = l.R, cols = l.cols;
   const long long items = l.few_items;
-  const Kv4Attn a{q, q_row, (const uint8_t*)blocks, table, work, y, (float*)scratch, H, G, width, pages, (int)items, scale, wait_word()};
+  const Kv4Attn a{q, q_row, (const uint8_t*)blocks, cache->table, work, y, (float*)scratch, H, G, cache->width, cache->pages, (int)items, scale, wait_word()};
   if (l.many) {
     Kv4Attn m = a;
     m.work = work + l.few_ints();
@@ -697,7 +550,7 @@ int ll_kv4_attn(const void* q, long long q_row, const void* blocks, const int32_
     }                                                                                                                                         \
     kv4_few_kernel<TT, DD, NG, CPL, NB><<<(unsigned)(items * G), KF_THREADS, smem, st>>>(a);                                                         \
     LL_LAUNCH_OK("kv4_few_kernel");                                                                                                           \
-    LL_CUDA(launch(kv4_join_kernel<TT, DD, COLS>, dim3((unsigned)(items * G), (unsigned)min((long long)cols, (long long)max_count * R)), dim3(KJ * 32), 0, st, true, a)); \
+    if (l.few_cut) LL_CUDA(launch(kv4_join_kernel<TT, DD, COLS>, dim3((unsigned)(items * G), (unsigned)min((long long)cols, (long long)max_count * R)), dim3(KJ * 32), 0, st, true, a)); \
   }
 #define FEW_COLS(TT, DD, NG)              \
   if (cols == 4) FEW(TT, DD, NG, 1, 1)    \

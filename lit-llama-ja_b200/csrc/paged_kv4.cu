@@ -2,7 +2,7 @@
 // their slots.  Layout: kv4.cuh; the attention that reads it: paged_attn.cu.
 #include <climits>
 
-#include "kv4.cuh"
+#include "paged_work.cuh"
 
 namespace llb {
 namespace {
@@ -25,10 +25,9 @@ struct Kv4Plan {
   int32_t* request;    // [B] the request, or -1 where a sequence is refused
   int32_t* positions;  // [T]
   int32_t* slots;      // [T]
-  int32_t* sequence;   // [T]
 };
 
-constexpr int PLAN_THREADS = 1024;
+constexpr int PLAN_THREADS = 1024, PLAN_HELD = 1024;      // threads at most; sequences whose numbers the block holds
 
 // Sum over the threads before this one; `total` of all of them.  Every thread of the block calls.
 template <typename V>
@@ -43,18 +42,14 @@ __device__ __forceinline__ V block_before(V v, V* s_warp, V& total) {
   __syncthreads();                     // (the sums of a scan before this one have been read)
   if (lane == 31) s_warp[warp] = incl;
   __syncthreads();
-  if (warp == 0) {
-    V w = lane < PLAN_THREADS / 32 ? s_warp[lane] : V(0);
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const V u = __shfl_up_sync(0xffffffffu, w, d);
-      if (lane >= d) w += u;
-    }
-    s_warp[lane] = w;
+  V before = V(0);
+  total = V(0);
+  for (int w = 0; w < (int)(blockDim.x >> 5); ++w) {
+    const V u = s_warp[w];
+    if (w < warp) before += u;
+    total += u;
   }
-  __syncthreads();
-  total = s_warp[31];
-  return (warp > 0 ? s_warp[warp - 1] : V(0)) + incl - v;
+  return before + incl - v;
 }
 
 __device__ __forceinline__ int pages_of(int tokens) { return (tokens + KV4_PAGE - 1) / KV4_PAGE; }
@@ -69,26 +64,184 @@ __device__ __forceinline__ void claim_requests(const int32_t* rows, const int32_
   __syncthreads();
 }
 
-// Pages of a step: prefix sums over the sequences in one block.
-__global__ void __launch_bounds__(PLAN_THREADS) kv4_plan_kernel(const int32_t* __restrict__ rows, const int32_t* __restrict__ counts, int B, int T,
-                                                               int max_count, Kv4Pool c, Kv4Plan p) {
+// What the sequences of a step came to: in shared memory where there is room, else where the plan keeps it.
+struct PlanView {
+  const int32_t *starts, *ends, *request;
+  int B;
+};
+
+// First sequence that ends behind token t (B: none).
+__device__ __forceinline__ int sequence_of(const PlanView& v, int t) {
+  int lo = 0, hi = v.B;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (v.starts[mid + 1] > t) hi = mid;
+    else lo = mid + 1;
+  }
+  return lo;
+}
+// position and slot of token t
+__device__ __forceinline__ void place_token(const PlanView& v, const Kv4Pool& c, const Kv4Plan& p, int t) {
+  const int i = sequence_of(v, t);
+  int pos = -1, slot = -1, row;
+  if (i < v.B && (row = v.request[i]) >= 0) {
+    pos = v.ends[i] - (v.starts[i + 1] - t);
+    slot = c.table[(size_t)row * c.width + pos / KV4_PAGE] * KV4_PAGE + pos % KV4_PAGE;
+  }
+  p.positions[t] = pos;
+  p.slots[t] = slot;
+}
+
+// ---- the division of a step's attention
+struct PlanWork {
+  int R, few, cols, longest, least;    // columns a token, most columns of the few, columns of a tile; most pages of a request, fewest of a part
+  int parts, max_items;                // places for blocks, items there is room for
+  int32_t* work;
+};
+constexpr int PW_SIZES = 512;          // sizes of parts told apart (larger ones by their 1 / PW_SIZES of the largest)
+
+// Parts of `step` pages at most, step the smallest with which a step's walks make no more than `parts` parts, as many as there are places for blocks, or
+// where the walks are more than half of that are cut no more than `parts` times.  Parts of a size stand together, the largest first: blocks take them in
+// that order, and the short ones fill the end.
+// MANY false: the sequences of up to `few` columns, whose tiles count as long as the last one; true: the others.
+template <bool MANY>
+__device__ __forceinline__ void divide_work(const PlanView& v, const PlanWork& d, int* s_count, int* s_size) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  auto tokens = [&](int i) { return v.starts[i + 1] - v.starts[i]; };
+  auto tiles = [&](int i) {
+    const long long c = (long long)tokens(i) * d.R;
+    return (c > d.few) == MANY ? (int)((c + d.cols - 1) / d.cols) : 0;
+  };
+  // pages that a tile's last column sees
+  auto pages = [&](int i, int tile) {
+    if (v.request[i] < 0) return 1;
+    const int n = tokens(i);
+    return (v.ends[i] - n + (MANY ? (int)min((long long)n - 1, ((long long)(tile + 1) * d.cols - 1) / d.R) : n - 1)) / KV4_PAGE + 1;
+  };
+  // parts of all walks, by one warp
+  auto total = [&](int step) {
+    int sum = 0;
+    if (MANY) {
+      for (int i = 0; i < v.B; ++i) {
+        const int w = tiles(i);
+        for (int t = lane; t < w; t += 32) sum += (pages(i, t) + step - 1) / step;
+      }
+    } else {
+      for (int i = lane; i < v.B; i += 32) {
+        const int w = tiles(i);
+        if (w > 0) sum += w * ((pages(i, 0) + step - 1) / step);
+      }
+    }
+    return __reduce_add_sync(0xffffffffu, sum);
+  };
+  // every warp looks at one of the steps between; the smallest that will do is in (lo, hi]
+  int lo = min(d.least, d.longest) - 1, hi = d.longest;
+  __syncthreads();
+  if (warp == 0) {
+    const int all = total(hi);
+    if (lane == 0) s_count[0] = all;
+  }
+  __syncthreads();
+  const int all = s_count[0], most = 2ll * all > d.parts ? all + d.parts : d.parts;
+  if (all >= 4ll * d.parts) lo = hi - 1;      // (walks for several rounds even out by themselves)
+  while (hi - lo > 1) {
+    const int each = (hi - lo + warps) / (warps + 1), mine = lo + each * (warp + 1);
+    __syncthreads();
+    if (mine < hi) {
+      const int parts = total(mine);
+      if (lane == 0) s_count[warp] = parts;
+    }
+    __syncthreads();
+    int best = hi;
+    for (int w = warps - 1; w >= 0; --w)
+      if (lo + each * (w + 1) < hi && s_count[w] <= most) best = lo + each * (w + 1);
+    int below = lo;
+    for (int w = 0; w < warps; ++w)
+      if (lo + each * (w + 1) < best) below = lo + each * (w + 1);
+    lo = below, hi = best;
+  }
+  const int step = hi;
+  // a walk's pages in equal parts; the places of the sizes, counted and summed from the largest down
+  auto cut = [&](int p) { return (p + step - 1) / step; };
+  auto bucket = [&](int size) { return PW_SIZES - 1 - (int)((long long)(min(size, step) - 1) * PW_SIZES / step); };
+  for (int x = threadIdx.x; x < PW_SIZES; x += blockDim.x) s_size[x] = 0;
+  __syncthreads();
+  for (int i = MANY ? warp : threadIdx.x; i < v.B; i += MANY ? warps : blockDim.x) {
+    const int w = tiles(i);
+    for (int t = MANY ? lane : 0; t < (MANY ? w : min(w, 1)); t += 32) {
+      const int p = pages(i, t), k = cut(p);
+      atomicAdd(&s_size[bucket((p + k - 1) / k)], MANY ? k : w * k);
+    }
+  }
+  __syncthreads();
+  if (warp == 0) {
+    int mine[PW_SIZES / 32], sum = 0;
+#pragma unroll
+    for (int x = 0; x < PW_SIZES / 32; ++x) mine[x] = s_size[lane * (PW_SIZES / 32) + x], sum += mine[x];
+    int incl = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += u;
+    }
+    if (lane == 31) d.work[0] = min(incl, d.max_items);
+    int before = incl - sum;
+#pragma unroll
+    for (int x = 0; x < PW_SIZES / 32; ++x) {
+      s_size[lane * (PW_SIZES / 32) + x] = before;
+      before += mine[x];
+    }
+  }
+  __syncthreads();
+  // (which of the parts of one size comes first is left to chance, and of no consequence: every part has its own place for its sums)
+  for (int i = warp; i < v.B; i += warps) {
+    const int w = tiles(i);
+    if (w == 0) continue;
+    const int n = tokens(i), row = v.request[i], pos0 = v.ends[i] - n, first = v.starts[i];
+    auto store = [&](int at, int tile, int part, int each, int k, int base) {
+      if (at >= d.max_items) return;
+      int4* o = reinterpret_cast<int4*>(d.work) + 1 + 3 * (size_t)at;
+      o[0] = make_int4(row, first, n, pos0);
+      o[1] = make_int4(tile, part * each, (part + 1) * each, k);
+      o[2] = make_int4(part, base, 0, 0);
+    };
+    if (MANY) {
+      for (int t = lane; t < w; t += 32) {
+        const int p = pages(i, t), k = cut(p), each = (p + k - 1) / k, at = atomicAdd(&s_size[bucket(each)], k);
+        for (int e = 0; e < k; ++e) store(at + e, t, e, each, k, at);
+      }
+    } else {
+      const int p = pages(i, 0), k = cut(p), each = (p + k - 1) / k;
+      int at = 0;
+      if (lane == 0) at = atomicAdd(&s_size[bucket(each)], w * k);
+      at = __shfl_sync(0xffffffffu, at, 0);
+      for (int e = lane; e < w * k; e += 32) store(at + e, e / k, e % k, each, k, at + e / k * k);
+    }
+  }
+}
+
+// A step's pages, slots (of up to `here` tokens) and division, by one block: prefix sums over the sequences.
+__global__ void __launch_bounds__(PLAN_THREADS) kv4_plan_kernel(const int32_t* __restrict__ rows, const int32_t* __restrict__ counts, int B, int T, int here,
+                                                               int max_count, Kv4Pool c, Kv4Plan p, PlanWork few, PlanWork many) {
   __shared__ long long s_sum[32];
-  __shared__ int s_need[32];
+  __shared__ int s_need[32], s_size[PW_SIZES];
   __shared__ int s_row[PLAN_THREADS], s_first[PLAN_THREADS], s_pages[PLAN_THREADS], s_used[PLAN_THREADS];
-  const int n_free = min(max(*c.n_free, 0), c.pages);
+  __shared__ int s_starts[PLAN_HELD + 1], s_ends[PLAN_HELD], s_request[PLAN_HELD];
+  const int n_free = min(max(*c.n_free, 0), c.pages), nt = blockDim.x, lane = threadIdx.x & 31;
+  const bool held = B <= PLAN_HELD;
   claim_requests(rows, counts, false, B, c);
   long long tokens = 0, wanted = 0;      // of the sequences before this round
   int given = 0;
-  for (int i0 = 0; i0 < B; i0 += PLAN_THREADS) {
+  for (int i0 = 0; i0 < B; i0 += nt) {
     const int i = i0 + threadIdx.x;
     const int row = i < B ? rows[i] : -1, count = i < B ? counts[i] : 0, n = max(count, 0);
     const bool named = row >= 0 && row < c.requests;
-    const int old = named ? c.lengths[row] : 0;
+    const int old = named ? c.lengths[row] : 0, claim = named && n > 0 ? c.stamp[row] : i;
     long long total;
     const long long first = tokens + block_before<long long>(n, s_sum, total);
     tokens += total;
     int status = KV4_OK;
-    if (count < 0 || (n > 0 && (!named || c.stamp[row] != i))) status = KV4_BAD_ROW;
+    if (count < 0 || (n > 0 && (!named || claim != i))) status = KV4_BAD_ROW;
     else if (first + n > T) status = KV4_BEHIND;
     else if (n > max_count || (long long)old + n > c.max_length) status = KV4_TOO_LONG;
     const int page0 = pages_of(old), need = status == KV4_OK && n > 0 ? pages_of(old + n) - page0 : 0;
@@ -104,44 +257,43 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv4_plan_kernel(const int32_t* _
     s_pages[threadIdx.x] = ok ? need : 0;
     s_used[threadIdx.x] = (int)min(before, (long long)n_free);
     if (i < B) {
+      const int end = (int)min(first + n, (long long)T), request = ok && n > 0 ? row : -1;
       if (i == 0) p.starts[0] = 0;
-      p.starts[i + 1] = (int)min(first + n, (long long)T);
+      p.starts[i + 1] = end;
       p.status[i] = status;
-      p.request[i] = ok && n > 0 ? row : -1;
+      p.request[i] = request;
+      if (held) {
+        if (i == 0) s_starts[0] = 0;
+        s_starts[i + 1] = end;
+        s_request[i] = request;
+      }
       if (ok && n > 0) c.lengths[row] = old + n;
     }
     __syncthreads();
     // the new entries of the table, a warp a sequence
-    const int lane = threadIdx.x & 31;
-    for (int j = threadIdx.x >> 5; j < min(PLAN_THREADS, B - i0); j += PLAN_THREADS / 32)
+    for (int j = threadIdx.x >> 5; j < min(nt, B - i0); j += nt >> 5)
       for (int k = lane; k < s_pages[j]; k += 32) c.table[(size_t)s_row[j] * c.width + s_first[j] + k] = c.free[n_free - 1 - s_used[j] - k];
     __syncthreads();
   }
   if (threadIdx.x == 0) *c.n_free = n_free - given;
-  for (int i = threadIdx.x; i < B; i += PLAN_THREADS) {      // (when all lengths are the step's: an idle sequence may name another one's request)
+  for (int i = threadIdx.x; i < B; i += nt) {      // (when all lengths are the step's: an idle sequence may name another one's request)
     const int row = rows[i];
-    p.ends[i] = p.status[i] == KV4_OK && row >= 0 && row < c.requests ? c.lengths[row] : 0;
+    const int end = p.status[i] == KV4_OK && row >= 0 && row < c.requests ? c.lengths[row] : 0;
+    p.ends[i] = end;
+    if (held) s_ends[i] = end;
   }
+  __syncthreads();
+  const PlanView v{held ? s_starts : p.starts, held ? s_ends : p.ends, held ? s_request : p.request, B};
+  for (int t = threadIdx.x; t < min(T, here); t += nt) place_token(v, c, p, t);
+  divide_work<false>(v, few, s_need, s_size);
+  if (many.work != nullptr) divide_work<true>(v, many, s_need, s_size);
 }
 
-// Positions and slots of a step's tokens.
-__global__ void __launch_bounds__(256) kv4_tokens_kernel(int B, int T, Kv4Pool c, Kv4Plan p) {
-  const int t = blockIdx.x * blockDim.x + threadIdx.x;
-  if (t >= T) return;
-  int lo = 0, hi = B;                  // the first sequence that ends behind t
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (p.starts[mid + 1] > t) hi = mid;
-    else lo = mid + 1;
-  }
-  int pos = -1, slot = -1, row;
-  if (lo < B && (row = p.request[lo]) >= 0) {
-    pos = p.ends[lo] - (p.starts[lo + 1] - t);
-    slot = c.table[(size_t)row * c.width + pos / KV4_PAGE] * KV4_PAGE + pos % KV4_PAGE;
-  }
-  p.positions[t] = pos;
-  p.slots[t] = slot;
-  p.sequence[t] = lo < B ? lo : -1;
+// Positions and slots of a step's tokens from `here` on.
+__global__ void __launch_bounds__(256) kv4_tokens_kernel(int B, int T, int here, Kv4Pool c, Kv4Plan p) {
+  pdl_wait();
+  const int t = here + blockIdx.x * blockDim.x + threadIdx.x;
+  if (t < T) place_token(PlanView{after_wait(p.starts), after_wait(p.ends), after_wait(p.request), B}, c, p, t);
 }
 
 // The way back: requests are cut to `keep` tokens, the pages behind go to the stack in the order that a plan would take them in again.
@@ -151,7 +303,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv4_truncate_kernel(const int32_
   const int n_free = min(max(*c.n_free, 0), c.pages);
   claim_requests(rows, keep, true, B, c);
   int total = 0;                        // the pages of all sequences have to be known before the first goes back
-  for (int i0 = 0; i0 < B; i0 += PLAN_THREADS) {
+  for (int i0 = 0; i0 < B; i0 += blockDim.x) {
     const int i = i0 + threadIdx.x, row = i < B ? rows[i] : -1;
     int n = 0, all;
     if (row >= 0 && row < c.requests && c.stamp[row] == i && keep[i] >= 0 && keep[i] < c.lengths[row]) n = pages_of(c.lengths[row]) - pages_of(keep[i]);
@@ -159,7 +311,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv4_truncate_kernel(const int32_
     total += all;
   }
   int done = 0;
-  for (int i0 = 0; i0 < B; i0 += PLAN_THREADS) {
+  for (int i0 = 0; i0 < B; i0 += blockDim.x) {
     const int i = i0 + threadIdx.x, row = i < B ? rows[i] : -1;
     int n = 0, first = 0, all;
     const bool cut = row >= 0 && row < c.requests && c.stamp[row] == i && keep[i] >= 0 && keep[i] < c.lengths[row];
@@ -173,7 +325,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv4_truncate_kernel(const int32_
     __syncthreads();
     if (cut) c.lengths[row] = keep[i];
     const int lane = threadIdx.x & 31;
-    for (int j = threadIdx.x >> 5; j < min(PLAN_THREADS, B - i0); j += PLAN_THREADS / 32)
+    for (int j = threadIdx.x >> 5; j < min((int)blockDim.x, B - i0); j += blockDim.x >> 5)
       for (int k = lane; k < s_pages[j]; k += 32) {
         int32_t* e = c.table + (size_t)s_row[j] * c.width + s_first[j] + k;
         const int at = n_free + total - 1 - s_used[j] - k;
@@ -193,120 +345,168 @@ struct Kv4Rows {
   long long q_row, k_row, v_row;       // distances of a token's rows, in numbers; heads follow one another
 };
 
-// One warp a vector of a token: a query to turn, a key to turn and round, a value to round.  E numbers a lane.
+// the smaller of two pairs; not a number where one of two is not
+__device__ __forceinline__ __nv_bfloat162 min_pair(__nv_bfloat162 a, __nv_bfloat162 b) { return __hmin2_nan(a, b); }
+__device__ __forceinline__ __half2 min_pair(__half2 a, __half2 b) { return __hmin2_nan(a, b); }
+template <typename T> __device__ __forceinline__ uint32_t min_bits(uint32_t a, uint32_t b) {
+  typedef typename pair_of<T>::type P;
+  const P r = min_pair(*reinterpret_cast<const P*>(&a), *reinterpret_cast<const P*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// A vector (a head of a token's queries, keys or values) takes D / 8 lanes of eight numbers each, a warp the same head of 32 / (D / 8) tokens one after
+// the other.  Bound by its instructions, not by memory: so the smallest and largest are found in pairs ({x, -x}: one minimum for both), a code comes from
+// a product with 1 / s, and only where that lies so near to the middle of two codes that its error could matter (1e-4; its error is below 4e-6) from the quotient.
 template <typename T, int D, int NG, bool TURN>
 __global__ void __launch_bounds__(256) kv4_append_kernel(Kv4Rows in, const float* __restrict__ rope, const int32_t* __restrict__ positions,
-                                                         const int32_t* __restrict__ slots, T* __restrict__ q_out, uint8_t* __restrict__ blocks, int H, int G) {
-  constexpr int E = D == 128 ? 4 : 2, LANES = D / E, GL = LANES / NG;
-  const int t = blockIdx.x, lane = threadIdx.x & 31, vec = blockIdx.y * 8 + (threadIdx.x >> 5);
+                                                         const int32_t* __restrict__ slots, T* __restrict__ q_out, uint8_t* __restrict__ blocks, int Tn, int H, int G) {
+  constexpr int LV = D / 8, TOKENS = 32 / LV, GL = LV / NG, W = D / 32;
+  const int lane = threadIdx.x & 31, l = lane % LV, t = blockIdx.x * TOKENS + lane / LV, vec = blockIdx.y * 8 + (threadIdx.x >> 5);
   const int nq = TURN ? H : 0;
   if (vec >= nq + 2 * G) return;
-  const int slot = slots[t], pos = positions[t];
+  const bool live = t < Tn;
+  const int slot = live ? slots[t] : -1, pos = live ? positions[t] : -1;
   const bool is_q = vec < nq, is_k = !is_q && vec < nq + G;
   const int head = is_q ? vec : is_k ? vec - nq : vec - nq - G;
-  if (!is_q && slot < 0) return;
   const T* row = is_q ? (const T*)in.q + t * in.q_row : is_k ? (const T*)in.k + t * in.k_row : (const T*)in.v + t * in.v_row;
-  row += head * D;
-  const bool live = lane < LANES;
-  const int d0 = lane * E;
-  float x[E];
-#pragma unroll
-  for (int e = 0; e < E; e += 2) {
-    const float2 f = live ? bits_pair<T>(*reinterpret_cast<const uint32_t*>(row + d0 + e)) : make_float2(0.f, 0.f);
-    x[e] = f.x, x[e + 1] = f.y;
-  }
+  uint4 u = live ? *reinterpret_cast<const uint4*>(row + head * D + 8 * l) : make_uint4(0u, 0u, 0u, 0u);
+  uint32_t w[4] = {u.x, u.y, u.z, u.w};
   if (TURN && (is_q || is_k)) {
-    const float* cs = rope + (size_t)max(pos, 0) * D;
+    const float4* cs = reinterpret_cast<const float4*>(rope + (size_t)max(pos, 0) * D + 8 * l);
+    const float4 c0 = __ldg(cs), c1 = __ldg(cs + 1);
+    const float c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
 #pragma unroll
-    for (int e = 0; e < E; e += 2) {
-      const float2 f = live ? *reinterpret_cast<const float2*>(cs + d0 + e) : make_float2(0.f, 0.f);
-      const float a = __fsub_rn(__fmul_rn(x[e], f.x), __fmul_rn(x[e + 1], f.y)), b = __fadd_rn(__fmul_rn(x[e + 1], f.x), __fmul_rn(x[e], f.y));
-      x[e] = a, x[e + 1] = b;
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = bits_pair<T>(w[j]);
+      w[j] = pair_bits<T>(__fsub_rn(__fmul_rn(f.x, c[2 * j]), __fmul_rn(f.y, c[2 * j + 1])), __fadd_rn(__fmul_rn(f.y, c[2 * j]), __fmul_rn(f.x, c[2 * j + 1])));
     }
   }
   if (is_q) {
     if (live) {
-      T* o = q_out + ((size_t)t * H + head) * D + d0;
-#pragma unroll
-      for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(o + e) = pos < 0 ? pair_bits<T>(NAN, NAN) : pair_bits<T>(x[e], x[e + 1]);
+      if (pos < 0) w[0] = w[1] = w[2] = w[3] = pair_bits<T>(NAN, NAN);
+      *reinterpret_cast<uint4*>(q_out + ((size_t)t * H + head) * D + 8 * l) = make_uint4(w[0], w[1], w[2], w[3]);
     }
     return;
   }
-  // the numbers as the cache's type has them, their smallest and largest by groups of GL lanes
-  float lo = INFINITY, hi = -INFINITY;
+  // smallest and largest of a group: {lo, -hi}
+  uint32_t low = min_bits<T>(min_bits<T>(w[0], w[1]), min_bits<T>(w[2], w[3]));
+  uint32_t high = min_bits<T>(min_bits<T>(w[0] ^ 0x80008000u, w[1] ^ 0x80008000u), min_bits<T>(w[2] ^ 0x80008000u, w[3] ^ 0x80008000u));
+  low = min_bits<T>(__byte_perm(low, high, 0x5410), __byte_perm(low, high, 0x7632));
 #pragma unroll
-  for (int e = 0; e < E; e += 2) {
-    const float2 f = bits_pair<T>(pair_bits<T>(x[e], x[e + 1]));
-    x[e] = f.x, x[e + 1] = f.y;
-    lo = fminf(lo, fminf(f.x, f.y));
-    hi = fmaxf(hi, fmaxf(f.x, f.y));
-    if (!(fabsf(f.x) < INFINITY) || !(fabsf(f.y) < INFINITY)) lo = -INFINITY, hi = INFINITY;
-  }
-#pragma unroll
-  for (int o = GL / 2; o > 0; o >>= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-  }
+  for (int o = GL / 2; o > 0; o >>= 1) low = min_bits<T>(low, __shfl_xor_sync(0xffffffffu, low, o));
+  const float2 ends = bits_pair<T>(low);
+  const float lo = ends.x, hi = -ends.y;
   uint32_t params = pair_bits<T>(__fmul_rn(__fsub_rn(hi, lo), (float)(1.0 / 15.0)), lo);
   float s = bits_pair<T>(params).x;
   if (!(s < INFINITY)) {               // a group with a number that is none, or infinite, or too wide: it stands for no numbers
     params = pair_bits<T>(NAN, NAN);
     s = 0.f;
   }
-  uint32_t code[E];
+  constexpr float ROUND = 12582912.f;                                   // 1.5 2^23: its sum with a small number has that rounded in the low bits
+  constexpr uint32_t BITS = 0x4b400000u;
+  const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
+  uint32_t code[8];
+  float far = 0.f;
 #pragma unroll
-  for (int e = 0; e < E; ++e) code[e] = s > 0.f ? (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[e], lo), s)), 0.f), 15.f) : 0u;
-  uint8_t* blk = blocks + ((size_t)(slot / KV4_PAGE) * G + head) * kv4_bytes(D, NG) + slot % KV4_PAGE / KV4_SLICE * kv4_slice_bytes(D, NG);
-  const int at = slot % KV4_SLICE;
-  if (live && lane % GL == 0)
-    reinterpret_cast<uint32_t*>(blk + (is_k ? kv4_k_params(D) : kv4_v_params(D, NG)))[at * NG + lane / GL] = params;
+  for (int j = 0; j < 4; ++j) {
+    const float2 f = bits_pair<T>(w[j]);
+    const float a = fminf(__fmul_rn(__fsub_rn(f.x, lo), inv), 15.f), b = fminf(__fmul_rn(__fsub_rn(f.y, lo), inv), 15.f);
+    const float x = __fadd_rn(a, ROUND), y = __fadd_rn(b, ROUND);
+    far = fmaxf(far, fmaxf(fabsf(a - (x - ROUND)), fabsf(b - (y - ROUND))));
+    code[2 * j] = __float_as_uint(x), code[2 * j + 1] = __float_as_uint(y);
+  }
+  if (!(far < 0.4999f) || !(inv < INFINITY)) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = bits_pair<T>(w[j]);
+      code[2 * j] = __float_as_uint(__fadd_rn(s > 0.f ? fminf(__fdiv_rn(__fsub_rn(f.x, lo), s), 15.f) : 0.f, ROUND));
+      code[2 * j + 1] = __float_as_uint(__fadd_rn(s > 0.f ? fminf(__fdiv_rn(__fsub_rn(f.y, lo), s), 15.f) : 0.f, ROUND));
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) code[j] -= BITS;
+  uint8_t* blk = blocks + ((size_t)(max(slot, 0) / KV4_PAGE) * G + head) * kv4_bytes(D, NG) + max(slot, 0) % KV4_PAGE / KV4_SLICE * kv4_slice_bytes(D, NG);
+  const int at = max(slot, 0) % KV4_SLICE;
+  if (slot >= 0 && l % GL == 0) reinterpret_cast<uint32_t*>(blk + (is_k ? kv4_k_params(D) : kv4_v_params(D, NG)))[at * NG + l / GL] = params;
   if (is_k) {
-    // a word's codes lie in the lanes that differ in the nibble number
-    uint32_t w = 0;
-#pragma unroll
-    for (int e = 0; e < E; ++e) w |= code[e] << kv4_k_bit(d0 + e);
-    if (E == 2) w |= __shfl_xor_sync(0xffffffffu, w, 1);
-    w |= __shfl_xor_sync(0xffffffffu, w, E == 4 ? 4 : 8);
-    if (live && (lane & (E == 4 ? 4 : 9)) == 0) reinterpret_cast<uint32_t*>(blk)[at * (D / 8) + kv4_k_word(D, d0)] = w;
+    // the lane's dimensions 8 l .. are four codes each of two chunks; the other codes of either word lie two lanes on
+    uint32_t a = code[0] | code[1] << 16 | code[2] << 4 | code[3] << 20, b = code[4] | code[5] << 16 | code[6] << 4 | code[7] << 20;
+    const bool up = (l & 2) != 0;
+    const uint32_t other = __shfl_xor_sync(0xffffffffu, up ? a : b, 2);
+    const uint32_t word = up ? other | b << 8 : a | other << 8;
+    if (slot >= 0) reinterpret_cast<uint32_t*>(blk)[at * (D / 8) + (2 * (l & 1) + (up ? 1 : 0)) * W + (l >> 2)] = word;
   } else {
-    // 16 bits of a word: nibbles 0 - 3 of one slot
-    unsigned long long w = 0;
+    // the lane has nibble l & 3 of the eight chunks; by halves between four lanes each comes to have all four nibbles of two chunks
+    const int n4 = 4 * (l & 3);
+    uint32_t z[4];
 #pragma unroll
-    for (int e = 0; e < E; ++e) w |= (unsigned long long)code[e] << (16 * e + kv4_v_bit(d0 + e));
-    w |= __shfl_xor_sync(0xffffffffu, w, E == 4 ? 2 : 4);
-    w |= __shfl_xor_sync(0xffffffffu, w, E == 4 ? 4 : 8);
-    const int e = E == 4 ? (lane >> 1) & 3 : (lane >> 2) & 3;      // which of the chunks this lane stores
-    if (live && e < E) {
-      const int d = d0 % 8 + e + 32 * (d0 / 32);                   // nibble 0's dimension
-      reinterpret_cast<uint16_t*>(blk + kv4_v_codes(D))[2 * ((at / 2) * (D / 4) + kv4_v_word(D, d)) + (at & 1)] = (uint16_t)(w >> (16 * e));
+    for (int j = 0; j < 4; ++j) z[j] = (code[2 * j] | code[2 * j + 1] << 16) << n4;
+    const bool odd = (l & 1) != 0, up = (l & 2) != 0;
+    uint32_t x0 = __shfl_xor_sync(0xffffffffu, odd ? z[0] : z[2], 1), x1 = __shfl_xor_sync(0xffffffffu, odd ? z[1] : z[3], 1);
+    x0 |= odd ? z[2] : z[0];
+    x1 |= odd ? z[3] : z[1];
+    uint32_t x = __shfl_xor_sync(0xffffffffu, up ? x0 : x1, 2) | (up ? x1 : x0);
+    const int g = 4 * (l & 1) + (l & 2);                                // x: chunk g, and chunk g + 1 in the high half
+    // the two slots of a pair, where two tokens of the warp have them, are stored together: a chunk each
+    const uint32_t theirs = __shfl_xor_sync(0xffffffffu, x, LV);
+    const int slot2 = __shfl_xor_sync(0xffffffffu, slot, LV);
+    uint8_t* to = blk + kv4_v_codes(D) + (at / 2) * D + (l >> 2) * 4;
+    if (slot >= 0 && slot2 == (slot ^ 1)) {
+      const bool second = (slot & 1) != 0;
+      const uint32_t word = second ? __byte_perm(theirs, x, 0x7632) : __byte_perm(x, theirs, 0x5410);
+      *reinterpret_cast<uint32_t*>(to + (g + (second ? 1 : 0)) * 4 * W) = word;
+    } else if (slot >= 0) {
+      *reinterpret_cast<uint16_t*>(to + g * 4 * W + 2 * (at & 1)) = (uint16_t)x;
+      *reinterpret_cast<uint16_t*>(to + (g + 1) * 4 * W + 2 * (at & 1)) = (uint16_t)(x >> 16);
     }
   }
 }
 
-// The values that slots stand for.
+// The values that slots stand for: a warp a slot and head.
 template <typename T, int D, int NG>
-__global__ void __launch_bounds__(D) kv4_read_kernel(const uint8_t* __restrict__ blocks, const int32_t* __restrict__ slots, T* __restrict__ k_out,
-                                                     T* __restrict__ v_out, int G, int pages) {
-  const int t = blockIdx.x, head = blockIdx.y, d = threadIdx.x, slot = slots[t];
-  float k = NAN, v = NAN;
-  if (slot >= 0 && slot < pages * KV4_PAGE) {
-    const uint8_t* blk = blocks + ((size_t)(slot / KV4_PAGE) * G + head) * kv4_bytes(D, NG) + slot % KV4_PAGE / KV4_SLICE * kv4_slice_bytes(D, NG);
-    const int at = slot % KV4_SLICE, g = d / (D / NG);
-    const uint32_t kw = reinterpret_cast<const uint32_t*>(blk)[at * (D / 8) + kv4_k_word(D, d)];
-    const uint32_t vw = reinterpret_cast<const uint32_t*>(blk + kv4_v_codes(D))[(at / 2) * (D / 4) + kv4_v_word(D, d)];
-    const float2 kp = bits_pair<T>(reinterpret_cast<const uint32_t*>(blk + kv4_k_params(D))[at * NG + g]);
-    const float2 vp = bits_pair<T>(reinterpret_cast<const uint32_t*>(blk + kv4_v_params(D, NG))[at * NG + g]);
-    k = __fadd_rn(__fmul_rn((float)((kw >> kv4_k_bit(d)) & 15u), kp.x), kp.y);
-    v = __fadd_rn(__fmul_rn((float)((vw >> (16 * (at & 1) + kv4_v_bit(d))) & 15u), vp.x), vp.y);
+__global__ void __launch_bounds__(256) kv4_read_kernel(const uint8_t* __restrict__ blocks, const int32_t* __restrict__ slots, T* __restrict__ k_out,
+                                                       T* __restrict__ v_out, int n, int G, int pages) {
+  constexpr int W = D / 32;
+  const int lane = threadIdx.x & 31;
+  const long long vec = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (vec >= (long long)n * G) return;
+  const int t = (int)(vec / G), head = (int)(vec - (long long)t * G), slot = slots[t];
+  const bool there = slot >= 0 && slot < pages * KV4_PAGE;
+  const uint8_t* blk = blocks + ((size_t)((there ? slot : 0) / KV4_PAGE) * G + head) * kv4_bytes(D, NG) + (there ? slot : 0) % KV4_PAGE / KV4_SLICE * kv4_slice_bytes(D, NG);
+  const int at = (there ? slot : 0) % KV4_SLICE;
+  T* ko = k_out + vec * D;
+  T* vo = v_out + vec * D;
+  auto value = [&](uint32_t c, float2 p) { return there ? __fadd_rn(__fmul_rn((float)c, p.x), p.y) : NAN; };
+  if (lane < 4 * W) {                  // keys: word i of chunk c, eight dimensions
+    const int c = lane / W, i = lane % W;
+    const uint32_t w = reinterpret_cast<const uint32_t*>(blk)[at * (D / 8) + lane];
+    const float2 p = bits_pair<T>(reinterpret_cast<const uint32_t*>(blk + kv4_k_params(D))[at * NG + i * NG / W]);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      *reinterpret_cast<uint2*>(ko + 32 * i + 16 * h + 4 * c) =
+          make_uint2(pair_bits<T>(value(w >> (8 * h) & 15u, p), value(w >> (8 * h + 16) & 15u, p)),
+                     pair_bits<T>(value(w >> (8 * h + 4) & 15u, p), value(w >> (8 * h + 20) & 15u, p)));
   }
-  const size_t o = ((size_t)t * G + head) * D + d;
-  dt<T>::st(k_out, o, k);
-  dt<T>::st(v_out, o, v);
+  if (lane < 8 * W) {                  // values: a slot's half of word i of chunk g, four dimensions
+    const int i = lane >> 3, g = lane & 7;
+    const uint32_t w = reinterpret_cast<const uint16_t*>(blk + kv4_v_codes(D))[(at / 2) * (D / 2) + (g * W + i) * 2 + (at & 1)];
+    const float2 p = bits_pair<T>(reinterpret_cast<const uint32_t*>(blk + kv4_v_params(D, NG))[at * NG + i * NG / W]);
+#pragma unroll
+    for (int m = 0; m < 4; ++m) dt<T>::st(vo, 32 * i + 8 * m + g, value(w >> (4 * m) & 15u, p));
+  }
 }
 
-bool pool_ok(const Kv4Pool& c) {
-  return c.table && c.lengths && c.free && c.n_free && c.stamp && c.requests > 0 && c.width > 0 && c.pages > 0 && c.pages <= INT_MAX / KV4_PAGE &&
-         c.max_length > 0 && (c.max_length - 1) / KV4_PAGE < c.width;
+int check_cache(const ll_kv4_cache* c, const char* who) {
+  LL_CHECK_ARG(c != nullptr, "%s: no cache", who);
+  LL_CHECK_ARG(kv4_shape_ok(c->head_size, c->group), "%s: kv4 heads of %d in groups of %d (32, 64 or 128 each)", who, c->head_size, c->group);
+  LL_CHECK_ARG(c->dtype == LL_BF16 || c->dtype == LL_F16, "%s: kv4 cache of type %d (bf16 or fp16)", who, c->dtype);
+  LL_CHECK_ARG(c->table && c->lengths && c->free_pages && c->n_free && c->stamp && c->requests > 0 && c->width > 0 && c->pages > 0 && c->pages <= INT_MAX / KV4_PAGE &&
+                   c->max_length > 0 && (c->max_length - 1) / KV4_PAGE < c->width && c->kv_heads > 0 && c->kv_heads <= 65535 && c->heads > 0 && c->heads % c->kv_heads == 0,
+               "%s: kv4 cache of %d requests of up to %d tokens in %d pages, %d heads over %d", who, c->requests, c->max_length, c->pages, c->heads, c->kv_heads);
+  return LL_OK;
+}
+Kv4Pool pool_of(const ll_kv4_cache* c) {
+  return Kv4Pool{c->table, c->lengths, c->free_pages, c->n_free, c->stamp, c->requests, c->width, c->pages, c->max_length};
 }
 
 }  // namespace
@@ -318,64 +518,81 @@ extern "C" {
 
 size_t ll_kv4_page_bytes(int head_size, int group) { return kv4_shape_ok(head_size, group) ? (size_t)kv4_bytes(head_size, head_size / group) : 0; }
 
-int ll_kv4_plan(const int32_t* rows, const int32_t* counts, int B, int T, int max_count, int32_t* table, int32_t* lengths, int32_t* free_pages, int32_t* n_free,
-                int32_t* stamp, int requests, int width, int pages, int max_length, int32_t* out, ll_stream stream) {
-  const Kv4Pool c{table, lengths, free_pages, n_free, stamp, requests, width, pages, max_length};
-  LL_CHECK_ARG(rows && counts && out && B > 0 && T >= 0 && max_count >= 0 && pool_ok(c), "kv4_plan: %d sequences of %d tokens, %d requests of up to %d in %d pages",
-               B, T, requests, max_length, pages);
-  const Kv4Plan p{out, out + B + 1, out + 2 * (size_t)B + 1, out + 3 * (size_t)B + 1, out + 4 * (size_t)B + 1, out + 4 * (size_t)B + 1 + T,
-                  out + 4 * (size_t)B + 1 + 2 * (size_t)T};
+size_t ll_kv4_work_ints(const ll_kv4_cache* cache, int B, int T, int max_count) {
+  return Kv4Lists(B, T, max_count, cache->heads, cache->kv_heads, cache->head_size, cache->max_length).ints();
+}
+
+int ll_kv4_plan(const ll_kv4_cache* cache, const int32_t* rows, const int32_t* counts, int B, int T, int max_count, int32_t* out, int32_t* work,
+                ll_stream stream) {
+  if (int r = check_cache(cache, "kv4_plan")) return r;
+  LL_CHECK_ARG(rows && counts && out && work && ((uintptr_t)work & 15) == 0 && B > 0 && T >= 0 && max_count >= 0 && (long long)T * cache->heads <= INT_MAX,
+               "kv4_plan: %d sequences of %d tokens, %d at most", B, T, max_count);
+  const Kv4Pool c = pool_of(cache);
+  const Kv4Plan p{out, out + B + 1, out + 2 * (size_t)B + 1, out + 3 * (size_t)B + 1, out + 4 * (size_t)B + 1, out + 4 * (size_t)B + 1 + T};
+  const Kv4Lists l(B, T, max_count, cache->heads, cache->kv_heads, cache->head_size, cache->max_length);
+  LL_CHECK_ARG(l.few_items * cache->kv_heads <= INT_MAX && l.many_items * cache->kv_heads <= INT_MAX, "kv4_plan: %d sequences of %d tokens, %d heads", B, T, cache->heads);
+  const int longest = (cache->max_length + KV4_PAGE - 1) / KV4_PAGE;
+  const PlanWork few{l.R, l.few, l.cols, longest, l.least, l.few_parts, (int)l.few_items, work};
+  const PlanWork many{l.R, l.few, KV4_MANY, longest, 1, l.many_parts, (int)l.many_items, l.many ? work + l.few_ints() : nullptr};
+  // The block itself places the tokens of a step while that takes it a few rounds; more are placed by a grid.
+  const int threads = B <= 256 && T <= 2048 ? 256 : PLAN_THREADS, here = T <= 8 * threads ? T : 0;
   cudaStream_t st = (cudaStream_t)stream;
-  kv4_plan_kernel<<<1, PLAN_THREADS, 0, st>>>(rows, counts, B, T, max_count, c, p);
+  kv4_plan_kernel<<<1, threads, 0, st>>>(rows, counts, B, T, here, max_count, c, p, few, many);
   LL_LAUNCH_OK("kv4_plan_kernel");
-  if (T > 0) {
-    kv4_tokens_kernel<<<(T + 255) / 256, 256, 0, st>>>(B, T, c, p);
+  if (here < T) {
+    LL_CUDA(launch(kv4_tokens_kernel, dim3((T - here + 255) / 256), dim3(256), 0, st, true, B, T, here, c, p));
     LL_LAUNCH_OK("kv4_tokens_kernel");
   }
   return LL_OK;
 }
 
-int ll_kv4_truncate(const int32_t* rows, const int32_t* keep, int B, int32_t* table, int32_t* lengths, int32_t* free_pages, int32_t* n_free, int32_t* stamp,
-                    int requests, int width, int pages, int max_length, ll_stream stream) {
-  const Kv4Pool c{table, lengths, free_pages, n_free, stamp, requests, width, pages, max_length};
-  LL_CHECK_ARG(rows && keep && B > 0 && pool_ok(c), "kv4_truncate: %d sequences, %d requests of up to %d in %d pages", B, requests, max_length, pages);
-  kv4_truncate_kernel<<<1, PLAN_THREADS, 0, (cudaStream_t)stream>>>(rows, keep, B, c);
+int ll_kv4_truncate(const ll_kv4_cache* cache, const int32_t* rows, const int32_t* keep, int B, ll_stream stream) {
+  if (int r = check_cache(cache, "kv4_truncate")) return r;
+  LL_CHECK_ARG(rows && keep && B > 0, "kv4_truncate: %d sequences", B);
+  kv4_truncate_kernel<<<1, B <= 256 ? 256 : PLAN_THREADS, 0, (cudaStream_t)stream>>>(rows, keep, B, pool_of(cache));
   LL_LAUNCH_OK("kv4_truncate_kernel");
   return LL_OK;
 }
 
-int ll_kv4_append(const void* q, long long q_row, const void* k, long long k_row, const void* v, long long v_row, const float* rope, const int32_t* positions,
-                  const int32_t* slots, void* q_out, void* blocks, int dtype, int T, int H, int G, int head_size, int group, ll_stream stream) {
-  LL_CHECK_ARG(kv4_shape_ok(head_size, group), "kv4_append: heads of %d in groups of %d (32, 64 or 128 each)", head_size, group);
-  LL_CHECK_ARG(dtype == LL_BF16 || dtype == LL_F16, "kv4_append: type %d (bf16 or fp16)", dtype);
-  LL_CHECK_ARG(k && v && positions && slots && blocks && (!rope || (q && q_out)) && T > 0 && H > 0 && G > 0, "kv4_append: %d tokens of %d heads, %d cached", T, H, G);
-  const uintptr_t a = (uintptr_t)(rope ? q : nullptr) | (uintptr_t)k | (uintptr_t)v | (uintptr_t)rope | (uintptr_t)q_out | (uintptr_t)blocks;
+int ll_kv4_append(const ll_kv4_cache* cache, void* blocks, const void* q, long long q_row, const void* k, long long k_row, const void* v, long long v_row,
+                  const float* rope, const int32_t* positions, const int32_t* slots, void* q_out, int T, ll_stream stream) {
+  if (int r = check_cache(cache, "kv4_append")) return r;
+  const int H = cache->heads, G = cache->kv_heads;
+  LL_CHECK_ARG(k && v && positions && slots && blocks && (!rope || (q && q_out)) && T > 0, "kv4_append: %d tokens of %d heads, %d cached", T, H, G);
+  const uintptr_t a = (uintptr_t)(rope ? q : nullptr) | (uintptr_t)k | (uintptr_t)v | (uintptr_t)rope | (uintptr_t)(rope ? q_out : nullptr) | (uintptr_t)blocks;
   LL_CHECK_ARG((a & 15) == 0 && ((rope ? q_row : 0) | k_row | v_row) % 8 == 0, "kv4_append: rows have to start on 16-byte boundaries");
   const Kv4Rows in{q, k, v, q_row, k_row, v_row};
+  const int tokens = 256 / cache->head_size, vecs = ((rope ? H : 0) + 2 * G + 7) / 8;
+  LL_CHECK_ARG(vecs <= 65535, "kv4_append: %d heads, %d cached", H, G);
   cudaStream_t st = (cudaStream_t)stream;
-  const dim3 grid(T, ((rope ? H : 0) + 2 * G + 7) / 8);
-#define APPEND(DD, NG)                                                                                                                              \
-  if (dtype == LL_BF16 && rope) kv4_append_kernel<__nv_bfloat16, DD, NG, true><<<grid, 256, 0, st>>>(in, rope, positions, slots, (__nv_bfloat16*)q_out, (uint8_t*)blocks, H, G); \
-  else if (dtype == LL_BF16) kv4_append_kernel<__nv_bfloat16, DD, NG, false><<<grid, 256, 0, st>>>(in, rope, positions, slots, (__nv_bfloat16*)q_out, (uint8_t*)blocks, H, G);    \
-  else if (rope) kv4_append_kernel<__half, DD, NG, true><<<grid, 256, 0, st>>>(in, rope, positions, slots, (__half*)q_out, (uint8_t*)blocks, H, G);  \
-  else kv4_append_kernel<__half, DD, NG, false><<<grid, 256, 0, st>>>(in, rope, positions, slots, (__half*)q_out, (uint8_t*)blocks, H, G);
-  KV4_SHAPES(head_size, group, APPEND)
+  const dim3 grid((T + tokens - 1) / tokens, vecs);
+#define APPEND_AS(TT, DD, NG, TURN) kv4_append_kernel<TT, DD, NG, TURN><<<grid, 256, 0, st>>>(in, rope, positions, slots, (TT*)q_out, (uint8_t*)blocks, T, H, G);
+#define APPEND(DD, NG)                                                                \
+  if (cache->dtype == LL_BF16 && rope) { APPEND_AS(__nv_bfloat16, DD, NG, true) }     \
+  else if (cache->dtype == LL_BF16) { APPEND_AS(__nv_bfloat16, DD, NG, false) }       \
+  else if (rope) { APPEND_AS(__half, DD, NG, true) }                                  \
+  else { APPEND_AS(__half, DD, NG, false) }
+  KV4_SHAPES(cache->head_size, cache->group, APPEND)
 #undef APPEND
+#undef APPEND_AS
   LL_LAUNCH_OK("kv4_append_kernel");
   return LL_OK;
 }
 
-int ll_kv4_read(const void* blocks, const int32_t* slots, void* k, void* v, int dtype, int n, int G, int head_size, int group, int pages, ll_stream stream) {
-  LL_CHECK_ARG(kv4_shape_ok(head_size, group), "kv4_read: heads of %d in groups of %d (32, 64 or 128 each)", head_size, group);
-  LL_CHECK_ARG(dtype == LL_BF16 || dtype == LL_F16, "kv4_read: type %d (bf16 or fp16)", dtype);
-  LL_CHECK_ARG(blocks && slots && k && v && n > 0 && G > 0 && G <= 65535 && pages > 0, "kv4_read: %d slots of %d heads", n, G);
+int ll_kv4_read(const ll_kv4_cache* cache, const void* blocks, const int32_t* slots, void* k, void* v, int n, ll_stream stream) {
+  if (int r = check_cache(cache, "kv4_read")) return r;
+  LL_CHECK_ARG(blocks && slots && k && v && n > 0, "kv4_read: %d slots", n);
+  const long long grid = ((long long)n * cache->kv_heads + 7) / 8;
+  LL_CHECK_ARG(grid <= INT_MAX, "kv4_read: %d slots of %d heads", n, cache->kv_heads);
   cudaStream_t st = (cudaStream_t)stream;
-  const dim3 grid(n, G);
-#define READ(DD, NG)                                                                                                                                   \
-  if (dtype == LL_BF16) kv4_read_kernel<__nv_bfloat16, DD, NG><<<grid, DD, 0, st>>>((const uint8_t*)blocks, slots, (__nv_bfloat16*)k, (__nv_bfloat16*)v, G, pages); \
-  else kv4_read_kernel<__half, DD, NG><<<grid, DD, 0, st>>>((const uint8_t*)blocks, slots, (__half*)k, (__half*)v, G, pages);
-  KV4_SHAPES(head_size, group, READ)
+#define READ_AS(TT, DD, NG) \
+  kv4_read_kernel<TT, DD, NG><<<(unsigned)grid, 256, 0, st>>>((const uint8_t*)blocks, slots, (TT*)k, (TT*)v, n, cache->kv_heads, cache->pages);
+#define READ(DD, NG)                                              \
+  if (cache->dtype == LL_BF16) { READ_AS(__nv_bfloat16, DD, NG) } \
+  else { READ_AS(__half, DD, NG) }
+  KV4_SHAPES(cache->head_size, cache->group, READ)
 #undef READ
+#undef READ_AS
   LL_LAUNCH_OK("kv4_read_kernel");
   return LL_OK;
 }

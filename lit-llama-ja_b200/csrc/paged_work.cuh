@@ -1,5 +1,8 @@
 // The division of a paged step's attention among blocks: which parts of which walks there are, and where a part's sums go.
 #pragma once
+#include <algorithm>
+#include <climits>
+
 #include "kv4.cuh"
 
 namespace llb {
@@ -39,10 +42,37 @@ __device__ __forceinline__ Kv4Item load_item(const int32_t* work, int i) {
 constexpr float KV4_NONE = -1e37f;      // the reference of a column that has seen no key
 
 // Sequences that bring up to this many columns a key head go to the kernel of few columns, others to the tcgen05 kernel in tiles of KV4_MANY.
-constexpr int KV4_FEW_MOST = 32, KV4_MANY = 256;
+constexpr int KV4_FEW_MOST = 32, KV4_MANY = 256, KV4_WHOLE = 8;
 
 inline bool kv4_many(int max_count, int R, int head_size) { return head_size >= 64 && (long long)max_count * R > KV4_FEW_MOST; }
 inline int kv4_sms() { return sm_count() > 0 ? sm_count() : 148; }
+
+// A step's two lists: sequences of few columns and, where one may bring more, of many.  Sizes as the host knows them.
+struct Kv4Lists {
+  int R, cols, few, few_parts, many_parts;
+  int least;                            // pages of a part of the few, at least
+  long long few_items, many_items;      // at most
+  bool many, few_cut;
+  Kv4Lists(int B, int T, int max_count, int H, int G, int head_size, int max_length) {
+    R = H / G;
+    many = kv4_many(max_count, R, head_size);
+    const long long c = (long long)max_count * R;
+    cols = many ? 8 : c <= 4 ? 4 : c <= 8 ? 8 : 16;
+    few = many ? KV4_FEW_MOST : INT_MAX;
+    few_parts = std::max(1, 4 * kv4_sms() / G);
+    many_parts = std::max(1, kv4_sms() / G);
+    // Where no request has more than KV4_WHOLE pages, walks are not cut, and there is nothing to join.
+    least = max_length <= KV4_WHOLE * KV4_PAGE ? KV4_WHOLE : 1;
+    few_cut = least == 1;
+    const long long each = many ? (KV4_FEW_MOST + cols - 1) / cols : T, seqs = std::min(B, std::max(T, 1));
+    few_items = std::min((long long)T * R / cols + seqs, seqs * each) + few_parts;
+    many_items = many ? (long long)T * R / KV4_MANY + std::min(seqs, (long long)T * R / KV4_FEW_MOST) + many_parts : 0;
+  }
+  size_t few_ints() const { return 4 + sizeof(Kv4Item) / 4 * (size_t)few_items; }
+  size_t ints() const { return few_ints() + (many ? 4 + sizeof(Kv4Item) / 4 * (size_t)many_items : 0); }
+  size_t few_floats(int G, int D) const { return ((size_t)few_items * G * cols * (D + 2) + 3) / 4 * 4; }
+  size_t floats(int G, int D) const { return few_floats(G, D) + (size_t)many_items * G * KV4_MANY * (D + 2); }
+};
 
 }  // namespace
 int kv4_prompt_launch(const Kv4Attn& a, int dtype, int head_size, int group, cudaStream_t st);      // paged_prompt.cu

@@ -50,6 +50,12 @@ class GemvArgs(C.Structure):
     ]
 
 
+class Kv4Cache(C.Structure):
+    """struct ll_kv4_cache (include/llb200.h)."""
+    _fields_ = [(n, vp) for n in ("table", "lengths", "free_pages", "n_free", "stamp")] + [
+        (n, C.c_int32) for n in ("requests", "width", "pages", "max_length", "heads", "kv_heads", "head_size", "group", "dtype")]
+
+
 def _proto(name, argtypes, restype=C.c_int):
     """Bind one export.  A reduced build of the library (build.py --only ...) lacks the kernels of the model families it
     was not built for: their entries raise when called."""
@@ -121,14 +127,13 @@ EXPORTS = {
     "ll_causal_attn_supported": ([i32, i32], C.c_int),
     "ll_causal_attn": ([vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, C.c_float, vp], C.c_int),
     "ll_kv4_page_bytes": ([i32, i32], sz_t),
-    "ll_kv4_plan": ([vp, vp, i32, i32, i32, vp, vp, vp, vp, vp, i32, i32, i32, i32, vp, vp], C.c_int),
-    "ll_kv4_truncate": ([vp, vp, i32, vp, vp, vp, vp, vp, i32, i32, i32, i32, vp], C.c_int),
-    "ll_kv4_append": ([vp, i64, vp, i64, vp, i64, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp], C.c_int),
-    "ll_kv4_read": ([vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp], C.c_int),
-    "ll_kv4_work_ints": ([i32, i32, i32, i32, i32, i32], sz_t),
-    "ll_kv4_work": ([vp, i32, i32, i32, i32, i32, i32, i32, vp, vp], C.c_int),
-    "ll_kv4_attn_scratch_bytes": ([i32, i32, i32, i32, i32, i32], sz_t),
-    "ll_kv4_attn": ([vp, i64, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, i32, i32, i32, C.c_float, vp, vp], C.c_int),
+    "ll_kv4_work_ints": ([vp, i32, i32, i32], sz_t),
+    "ll_kv4_plan": ([vp, vp, vp, i32, i32, i32, vp, vp, vp], C.c_int),
+    "ll_kv4_truncate": ([vp, vp, vp, i32, vp], C.c_int),
+    "ll_kv4_append": ([vp, vp, vp, i64, vp, i64, vp, i64, vp, vp, vp, vp, i32, vp], C.c_int),
+    "ll_kv4_read": ([vp, vp, vp, vp, vp, i32, vp], C.c_int),
+    "ll_kv4_attn_scratch_bytes": ([vp, i32, i32, i32], sz_t),
+    "ll_kv4_attn": ([vp, vp, vp, i64, vp, vp, i32, i32, i32, C.c_float, vp, vp], C.c_int),
     "ll_embed_ssq": ([vp, vp, vp, vp, i32, i32, vp], C.c_int),
     "ll_rope_kv_append": ([vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp], C.c_int),
     "ll_decode_attn": ([vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp, vp, i32, vp], C.c_int),

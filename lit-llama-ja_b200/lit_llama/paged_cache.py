@@ -18,11 +18,15 @@ the group's range more at its upper end, where the rounding of s may leave 15 s 
 """
 from __future__ import annotations
 
+import contextlib
+import ctypes as C
 from typing import Optional, Sequence, Tuple, Union
 
 import torch
 
 from . import _native as N
+
+_NOTHING = contextlib.nullcontext()
 
 Whole = Union[torch.Tensor, Sequence[int]]
 
@@ -37,9 +41,39 @@ class CachePlan:
 
     def __init__(self, cache: "PagedCache4", B: int, T: int, max_count: int):
         self.cache, self.B, self.T, self.max_count, self.step = cache, B, T, max_count, cache._step
-        work = N.call_ret("ll_kv4_work_ints", B, T, max_count, cache.n_head, cache.n_kv_head, cache.head_size)
-        data = torch.empty(work + 4 * B + 1 + 3 * T, dtype=torch.int32, device=cache.device)
-        self.work, self.starts, self.ends, self.status, self.request, self.positions, self.slots, self.sequence = data.split([work, B + 1, B, B, B, T, T, T])
+        work, self.scratch_bytes = cache._sizes(B, T, max_count)
+        self._data = torch.empty(work + 4 * B + 1 + 2 * T, dtype=torch.int32, device=cache.device)
+        self._work = N.ptr(self._data)
+        self._out = self._work + 4 * work
+        self._positions = self._out + 4 * (4 * B + 1)
+        self._slots = self._positions + 4 * T
+
+    def _part(self, first: int, n: int) -> torch.Tensor:
+        return self._data.narrow(0, (self._out - self._work) // 4 + first, n)
+
+    @property
+    def starts(self) -> torch.Tensor:
+        return self._part(0, self.B + 1)
+
+    @property
+    def ends(self) -> torch.Tensor:
+        return self._part(self.B + 1, self.B)
+
+    @property
+    def status(self) -> torch.Tensor:
+        return self._part(2 * self.B + 1, self.B)
+
+    @property
+    def request(self) -> torch.Tensor:
+        return self._part(3 * self.B + 1, self.B)
+
+    @property
+    def positions(self) -> torch.Tensor:
+        return self._part(4 * self.B + 1, self.T)
+
+    @property
+    def slots(self) -> torch.Tensor:
+        return self._part(4 * self.B + 1 + self.T, self.T)
 
     def check(self) -> None:
         """Raise if a sequence was refused.  Waits for the GPU."""
@@ -78,16 +112,33 @@ class PagedCache4:
         self.free = torch.arange(pages - 1, -1, -1, **i32)
         self.n_free = torch.full((1,), pages, **i32)
         self._stamp = torch.zeros(requests, **i32)
-        self._pool = [N.ptr(t) for t in (self.table, self.lengths, self.free, self.n_free, self._stamp)] + [requests, self.width, pages, max_length]
-        self._layers = [N.ptr_at(self.blocks, i * self.blocks.stride(0)) for i in range(n_layer)]
         self._code = N.dtype_code(dtype)
+        self._struct = N.Kv4Cache(*(N.ptr(t) for t in (self.table, self.lengths, self.free, self.n_free, self._stamp)), requests, self.width, pages, max_length,
+                                  n_head, n_kv_head, head_size, group, self._code)
+        self._c = C.addressof(self._struct)
+        self._layers = [N.ptr_at(self.blocks, i * self.blocks.stride(0)) for i in range(n_layer)]
         self._step = 0
+        self._size_of = {}
+
+    def _sizes(self, B: int, T: int, max_count: int) -> Tuple[int, int]:
+        """Numbers of a plan's division, bytes of its attention's scratch."""
+        key = (B, T, max_count)
+        got = self._size_of.get(key)
+        if got is None:
+            if len(self._size_of) >= 256:      # (prompts come in many sizes)
+                self._size_of.clear()
+            got = self._size_of[key] = (N.call_ret("ll_kv4_work_ints", self._c, *key), N.call_ret("ll_kv4_attn_scratch_bytes", self._c, *key))
+        return got
+
+    def _here(self):
+        """The cache's device as the current one, whose current stream the kernels go to."""
+        return _NOTHING if torch.cuda.current_device() == self.device.index else torch.cuda.device(self.device)
 
     # ------------------------------------------------------------------ pages and slots
     def _whole(self, name: str, x: Whole) -> torch.Tensor:
         if not isinstance(x, torch.Tensor):
             x = torch.tensor(list(x), dtype=torch.int32, device=self.device)
-        if x.dim() != 1 or x.dtype != torch.int32 or x.device != self.device:
+        if x.dim() != 1 or x.dtype is not torch.int32 or x.get_device() != self.device.index:
             raise RuntimeError(f"{name}: int32 numbers on {self.device}, one for each sequence, not {x.dtype} {tuple(x.shape)} on {x.device}")
         return x.contiguous()
 
@@ -102,11 +153,10 @@ class PagedCache4:
         max_count = tokens if max_count is None else max_count
         if not 0 <= max_count or not 0 <= tokens < 2**31 // max(1, self.n_head):
             raise RuntimeError(f"a step of {tokens} tokens, {max_count} at most of a sequence")
-        with torch.cuda.device(self.device):
+        with self._here():
             self._step += 1
             plan = CachePlan(self, rows.numel(), tokens, min(max_count, tokens))
-            N.call("ll_kv4_plan", N.ptr(rows), N.ptr(counts), plan.B, tokens, plan.max_count, *self._pool, N.ptr(plan.starts), N.stream())
-            N.call("ll_kv4_work", N.ptr(plan.starts), plan.B, tokens, plan.max_count, self.n_head, self.n_kv_head, self.head_size, self.max_length, N.ptr(plan.work), N.stream())
+            N.call("ll_kv4_plan", self._c, N.ptr(rows), N.ptr(counts), plan.B, tokens, plan.max_count, plan._out, plan._work, N.stream())
         return plan
 
     def truncate(self, rows: Whole, lengths: Whole) -> None:
@@ -115,9 +165,9 @@ class PagedCache4:
         rows, lengths = self._whole("rows", rows), self._whole("lengths", lengths)
         if rows.shape != lengths.shape or rows.numel() == 0:
             raise RuntimeError(f"{rows.numel()} requests and {lengths.numel()} lengths")
-        with torch.cuda.device(self.device):
+        with self._here():
             self._step += 1
-            N.call("ll_kv4_truncate", N.ptr(rows), N.ptr(lengths), rows.numel(), *self._pool, N.stream())
+            N.call("ll_kv4_truncate", self._c, N.ptr(rows), N.ptr(lengths), rows.numel(), N.stream())
 
     def reset(self) -> None:
         """All requests end, and pages are given out as in the beginning."""
@@ -136,11 +186,13 @@ class PagedCache4:
 
     def _rows(self, name: str, x: torch.Tensor, T: int, heads: int) -> torch.Tensor:
         """Rows as the kernels take them: the heads of a token one after the other, tokens at any distance, 16-byte boundaries."""
-        if x.shape != (T, heads, self.head_size) or x.dtype != self.dtype or x.device != self.device:
-            raise RuntimeError(f"{name}: {x.dtype} {tuple(x.shape)} on {x.device}, and the cache takes {self.dtype} {(T, heads, self.head_size)} on {self.device}")
-        if torch.is_grad_enabled() and x.requires_grad:
+        D = self.head_size
+        if x.shape != (T, heads, D) or x.dtype is not self.dtype or x.get_device() != self.device.index:
+            raise RuntimeError(f"{name}: {x.dtype} {tuple(x.shape)} on {x.device}, and the cache takes {self.dtype} {(T, heads, D)} on {self.device}")
+        if x.requires_grad and torch.is_grad_enabled():
             raise RuntimeError(f"{name}: the 4-bit cache has no gradient")
-        if x.stride(2) != 1 or (heads > 1 and x.stride(1) != self.head_size) or (T > 1 and (x.stride(0) % 8 != 0 or x.stride(0) < heads * self.head_size)) or x.data_ptr() % 16 != 0:
+        row, head, one = x.stride()
+        if one != 1 or (head != D and heads > 1) or (T > 1 and (row % 8 != 0 or row < heads * D)) or x.data_ptr() % 16 != 0:
             x = x.clone(memory_format=torch.contiguous_format)
         return x
 
@@ -163,10 +215,13 @@ class PagedCache4:
             out = torch.empty((T, self.n_head, self.head_size), dtype=self.dtype, device=self.device)
         if T == 0:
             return out
-        with torch.cuda.device(self.device):
-            N.call("ll_kv4_append", N.ptr(q) if rope is not None else None, q.stride(0) if rope is not None else 0, N.ptr(k), k.stride(0), N.ptr(v), v.stride(0),
-                   N.ptr(rope), N.ptr(plan.positions), N.ptr(plan.slots), N.ptr(out) if rope is not None else None, self._layers[layer], self._code, T,
-                   self.n_head, self.n_kv_head, self.head_size, self.group, N.stream())
+        with self._here():
+            if rope is None:
+                N.call("ll_kv4_append", self._c, self._layers[layer], None, 0, N.ptr(k), k.stride(0), N.ptr(v), v.stride(0), None, plan._positions, plan._slots, None, T,
+                       N.stream())
+            else:
+                N.call("ll_kv4_append", self._c, self._layers[layer], N.ptr(q), q.stride(0), N.ptr(k), k.stride(0), N.ptr(v), v.stride(0), N.ptr(rope), plan._positions,
+                       plan._slots, N.ptr(out), T, N.stream())
         return out
 
     def read(self, layer: int, slots: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -176,9 +231,8 @@ class PagedCache4:
         slots = self._whole("slots", slots)
         k, v = torch.empty((2, slots.numel(), self.n_kv_head, self.head_size), dtype=self.dtype, device=self.device).unbind(0)
         if slots.numel():
-            with torch.cuda.device(self.device):
-                N.call("ll_kv4_read", self._layers[layer], N.ptr(slots), N.ptr(k), N.ptr(v), self._code, slots.numel(), self.n_kv_head, self.head_size, self.group,
-                       self.pages, N.stream())
+            with self._here():
+                N.call("ll_kv4_read", self._c, self._layers[layer], N.ptr(slots), N.ptr(k), N.ptr(v), slots.numel(), N.stream())
         return k, v
 
     def attend(self, layer: int, plan: CachePlan, q: torch.Tensor, scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -196,9 +250,7 @@ class PagedCache4:
             raise RuntimeError(f"scores times {scale}: more than 0")
         if T == 0:
             return out
-        with torch.cuda.device(self.device):
-            shape = (plan.B, T, plan.max_count, self.n_head, self.n_kv_head, self.head_size)
-            scratch = torch.empty(N.call_ret("ll_kv4_attn_scratch_bytes", *shape), dtype=torch.uint8, device=self.device)
-            N.call("ll_kv4_attn", N.ptr(q), q.stride(0), self._layers[layer], N.ptr(self.table), N.ptr(plan.work), N.ptr(out), self._code, *shape,
-                   self.group, self.width, self.pages, scale, N.ptr(scratch), N.stream())
+        with self._here():
+            scratch = torch.empty(plan.scratch_bytes, dtype=torch.uint8, device=self.device)
+            N.call("ll_kv4_attn", self._c, self._layers[layer], N.ptr(q), q.stride(0), plan._work, N.ptr(out), plan.B, T, plan.max_count, scale, N.ptr(scratch), N.stream())
         return out

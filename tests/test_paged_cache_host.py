@@ -1,4 +1,5 @@
 """What the paged 4-bit cache refuses before anything reaches a GPU, and the host's restatement that the GPU tests compare with."""
+import ctypes
 import random
 
 import pytest
@@ -33,25 +34,56 @@ def test_refused_shapes(args, kind, error):
 A = 1 << 12      # an address that no launch reads
 
 
-@pytest.mark.parametrize("name, args", [
-    ("ll_kv4_plan", (0, A, 1, 1, 1, A, A, A, A, A, 1, 1, 1, 64, A, 0)),
-    ("ll_kv4_plan", (A, A, 0, 1, 1, A, A, A, A, A, 1, 1, 1, 64, A, 0)),
-    ("ll_kv4_plan", (A, A, 1, -1, 1, A, A, A, A, A, 1, 1, 1, 64, A, 0)),
-    ("ll_kv4_plan", (A, A, 1, 1, 1, A, A, A, A, A, 1, 1, 1, 65, A, 0)),           # a table too narrow for the longest request
-    ("ll_kv4_truncate", (A, 0, 1, A, A, A, A, A, 1, 1, 1, 64, 0)),
-    ("ll_kv4_append", (0, 0, A, 64, A, 64, 0, A, A, 0, A, 0, 1, 1, 1, 64, 64, 0)),     # fp32
-    ("ll_kv4_append", (0, 0, A, 64, A, 64, 0, A, A, 0, A, 1, 1, 1, 1, 64, 48, 0)),     # groups of 48
-    ("ll_kv4_append", (0, 0, A + 2, 64, A, 64, 0, A, A, 0, A, 1, 1, 1, 1, 64, 64, 0)),   # keys off a 16-byte boundary
-    ("ll_kv4_append", (0, 0, A, 65, A, 64, 0, A, A, 0, A, 1, 1, 1, 1, 64, 64, 0)),
-    ("ll_kv4_append", (0, 0, A, 64, A, 64, A, A, A, A, A, 1, 1, 1, 1, 64, 64, 0)),     # a table and no queries
-    ("ll_kv4_read", (A, A, A, A, 1, 0, 1, 64, 64, 1, 0)),
-    ("ll_kv4_attn", (A, 64, A, A, A, A, 1, 1, 1, 1, 3, 2, 64, 64, 1, 1, 1.0, A, 0)),         # three heads over two
-    ("ll_kv4_attn", (A, 64, A, A, A, A, 0, 1, 1, 1, 2, 2, 64, 64, 1, 1, 1.0, A, 0)),         # fp32
-    ("ll_kv4_attn", (A, 60, A, A, A, A, 1, 1, 1, 1, 2, 2, 64, 64, 1, 1, 1.0, A, 0)),
+def _struct(**other):
+    kind = dict(table=A, lengths=A, free_pages=A, n_free=A, stamp=A, requests=1, width=1, pages=1, max_length=64, heads=2, kv_heads=2, head_size=64, group=64, dtype=1)
+    kind.update(other)
+    return N.Kv4Cache(*(kind[n] for n, _ in N.Kv4Cache._fields_))
+
+
+PLAN, APPEND, READ, ATTN = (A, A, 1, 1, 1, A, A, 0), (A, 0, 0, A, 64, A, 64, 0, A, A, 0, 1, 0), (A, A, A, A, 1, 0), (A, A, 64, A, A, 1, 1, 1, 1.0, A, 0)
+
+
+def _with(args, **at):
+    return tuple(at.get(f"a{i}", a) for i, a in enumerate(args))
+
+
+@pytest.mark.parametrize("name, cache, args", [
+    ("ll_kv4_plan", {}, _with(PLAN, a0=0)),
+    ("ll_kv4_plan", {}, _with(PLAN, a2=0)),
+    ("ll_kv4_plan", {}, _with(PLAN, a3=-1)),
+    ("ll_kv4_plan", {}, _with(PLAN, a6=A + 4)),
+    ("ll_kv4_plan", {}, _with(PLAN, a3=1 << 30)),
+    ("ll_kv4_plan", dict(max_length=65), PLAN),                   # a table too narrow for the longest request
+    ("ll_kv4_plan", dict(pages=1 << 25), PLAN),
+    ("ll_kv4_plan", dict(table=0), PLAN),
+    ("ll_kv4_truncate", {}, (A, 0, 1, 0)),
+    ("ll_kv4_truncate", dict(requests=0), (A, A, 1, 0)),
+    ("ll_kv4_append", dict(dtype=0), APPEND),
+    ("ll_kv4_append", dict(group=48), APPEND),
+    ("ll_kv4_append", dict(group=128), APPEND),
+    ("ll_kv4_append", {}, _with(APPEND, a3=A + 2)),               # keys off a 16-byte boundary
+    ("ll_kv4_append", {}, _with(APPEND, a4=65)),
+    ("ll_kv4_append", {}, _with(APPEND, a7=A, a10=A)),            # a table and no queries
+    ("ll_kv4_append", {}, _with(APPEND, a11=0)),
+    ("ll_kv4_read", {}, _with(READ, a4=0)),
+    ("ll_kv4_attn", dict(heads=3), ATTN),                         # three heads over two
+    ("ll_kv4_attn", dict(dtype=0), ATTN),
+    ("ll_kv4_attn", dict(head_size=96), ATTN),
+    ("ll_kv4_attn", {}, _with(ATTN, a2=60)),
+    ("ll_kv4_attn", {}, _with(ATTN, a8=0.0)),
+    ("ll_kv4_attn", {}, _with(ATTN, a8=float("nan"))),
+    ("ll_kv4_attn", {}, _with(ATTN, a9=0)),
 ])
-def test_refused_calls(name, args):
+def test_refused_calls(name, cache, args):
+    c = _struct(**cache)
     with pytest.raises(RuntimeError, match="kv4"):
-        N.call(name, *args)
+        N.call(name, ctypes.addressof(c), *args)
+
+
+def test_no_cache():
+    for name, args in (("ll_kv4_plan", PLAN), ("ll_kv4_truncate", (A, A, 1, 0)), ("ll_kv4_append", APPEND), ("ll_kv4_read", READ), ("ll_kv4_attn", ATTN)):
+        with pytest.raises(RuntimeError, match="no cache"):
+            N.call(name, None, *args)
 
 
 def test_page_bytes():
