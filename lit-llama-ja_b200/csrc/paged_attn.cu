@@ -35,6 +35,9 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t v) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
+// column -> token and head, without a division where a key head serves one head
+__device__ __forceinline__ int column_token(int c, int R) { return R == 1 ? c : c / R; }
+__device__ __forceinline__ int column_head(int c, int R) { return R == 1 ? 0 : c % R; }
 __device__ __forceinline__ uint32_t half_bits(float a, float b) { return pair_bits<__half>(a, b); }
 
 // One warp's wait for its copy: bounded; one that runs out leaves a code for the host.
@@ -48,13 +51,14 @@ __device__ __forceinline__ bool kf_wait(uint64_t* bar, uint32_t parity, int* wor
 
 // Few queries a request: a block walks a range of one request's pages for one key head and a tile of columns (a column: one query of one of the heads
 // that share the key head).  Warp w takes half w & 1 of every other page, 32 keys, through a ring and with references of its own; the four join at the end.
-// CPL = 1: up to four columns, each of which has two of the product's eight, so that a lane has one column's scores and weights enter the second
-// product as two terms of fp16 (what the first leaves over in the odd column); CPL = 2: eight columns, and 16 with NB = 2, whose weights are one term, or
-// two where the result is fp16.
+// CPL = 1: up to four columns, each of which has two of the product's eight, so that a lane has one column's scores; CPL = 2: eight columns, and 16 with
+// NB = 2.  Weights enter the second product as fp16, half a place (2^-11) of which a bf16 result does not show; where the result is fp16 as two terms, with
+// CPL = 1 the second one in the odd column.
 template <typename T, int D, int NG, int CPL, int NB>
 __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(const Kv4Attn a) {
   constexpr int W = D / 32, KS = D / 16, COLS = 4 * CPL * NB, BYTES = kv4_bytes(D, NG), SLICE = kv4_slice_bytes(D, NG), SPG = KS / NG, STAGES = kf_stages(D, NG);
-  constexpr int TERMS = CPL == 2 && std::is_same<T, __half>::value ? 2 : 1;
+  constexpr bool FINE = std::is_same<T, __half>::value;                  // the result keeps 11 bits
+  constexpr int TERMS = CPL == 2 && FINE ? 2 : 1;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t s_full[KF_WARPS][STAGES];
   __shared__ int s_fail;
@@ -69,12 +73,12 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
   if (row < 0) {                        // a refused sequence's tokens are no numbers
     for (int e = threadIdx.x; e < cols * D; e += KF_THREADS) {
       const int c = col0 + e / D;
-      dt<T>::st(y, ((size_t)(first + c / R) * a.H + head * R + c % R) * D + e % D, NAN);
+      dt<T>::st(y, ((size_t)(first + column_token(c, R)) * a.H + head * R + column_head(c, R)) * D + e % D, NAN);
     }
     return;
   }
   const int pos0 = it.pos0;
-  const int last = pos0 + (col0 + cols - 1) / R;                        // position of the tile's last column: keys up to here are in sight
+  const int last = pos0 + column_token(col0 + cols - 1, R);                    // position of the tile's last column: keys up to here are in sight
   const int page0 = it.page0 + (warp >> 1), page1 = min(it.page1, last / KV4_PAGE + 1), half32 = 32 * (warp & 1);
   // the warp's pages: page0, page0 + 2 ..; the last one only where its half holds keys in sight
   const int units = page0 >= page1 ? 0 : (page1 - page0 + 1) / 2 - ((page0 + ((page1 - page0 - 1) & ~1)) * KV4_PAGE + half32 > last ? 1 : 0);
@@ -127,17 +131,18 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
   for (int b = 0; b < NB; ++b) {
     const int mine = CPL == 2 ? 8 * b + g8 : g8 >> 1, c = col0 + mine;
     const bool live = mine < cols && (CPL == 2 || (g8 & 1) == 0);
-    const T* q = (const T*)a.q + (long long)(first + (live ? c / R : 0)) * a.q_row + (size_t)(head * R + (live ? c % R : 0)) * D;
+    const T* q = (const T*)a.q + (long long)(first + (live ? column_token(c, R) : 0)) * a.q_row + (size_t)(head * R + (live ? column_head(c, R) : 0)) * D;
     uint2 raw[KS];
-    float mx = 0.f;
+    uint32_t big = 0;                                                   // sizes of numbers rise with their bits
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       raw[s] = live ? *reinterpret_cast<const uint2*>(q + 16 * s + 4 * t4) : make_uint2(0u, 0u);
-      const float2 u = bits_pair<T>(raw[s].x), v = bits_pair<T>(raw[s].y);
-      mx = fmaxf(fmaxf(mx, fmaxf(fabsf(u.x), fabsf(u.y))), fmaxf(fabsf(v.x), fabsf(v.y)));
+      big = __vmaxu2(__vmaxu2(big, raw[s].x & 0x7fff7fffu), raw[s].y & 0x7fff7fffu);
     }
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+    big = __vmaxu2(big, __shfl_xor_sync(0xffffffffu, big, 1));
+    big = __vmaxu2(big, __shfl_xor_sync(0xffffffffu, big, 2));
+    const float2 mx2 = bits_pair<T>(big);
+    const float mx = fmaxf(mx2.x, mx2.y);
     const int ex = min(max((int)(__float_as_uint(mx) >> 23), 15), 240);            // biased exponent of the largest
     const float up = __uint_as_float((uint32_t)(127 + 14 + 127 - ex) << 23);       // 2^(14 - (ex - 127))
     float gs[NG];
@@ -148,8 +153,7 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
       const float2 u = bits_pair<T>(raw[s].x), v = bits_pair<T>(raw[s].y);
       qb[b][s][0] = half_bits(u.x * up, u.y * up);
       qb[b][s][1] = half_bits(v.x * (up * 0.0625f), v.y * (up * 0.0625f));
-      const float2 x = bits_pair<__half>(qb[b][s][0]), z = bits_pair<__half>(qb[b][s][1]);
-      gs[s / SPG] += (x.x + x.y) + 16.f * (z.x + z.y);
+      gs[s / SPG] += (u.x + u.y) + (v.x + v.y);
     }
     // 2^24 of the codes and 2^(ex - 127 - 14) of the queries, times the scores' scale in units of log2
     const float back = __uint_as_float((uint32_t)(ex - 14 + 24) << 23) * (a.scale * KF_LOG2E);
@@ -160,10 +164,10 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
       gs[g] += __shfl_xor_sync(0xffffffffu, gs[g], 1);
       gs[g] += __shfl_xor_sync(0xffffffffu, gs[g], 2);
 #pragma unroll
-      for (int e = 0; e < CPL; ++e) qn[b][g][e] = __shfl_sync(0xffffffffu, gs[g], 4 * (2 * t4 + e)) * 5.9604644775390625e-8f;      // 2^-24
+      for (int e = 0; e < CPL; ++e) qn[b][g][e] = __shfl_sync(0xffffffffu, gs[g] * (up * 5.9604644775390625e-8f), 4 * (2 * t4 + e));      // (2^-24)
     }
   }
-  const int first_pos = pos0 + col0 / R;                                // every column sees the keys up to here
+  const int first_pos = pos0 + column_token(col0, R);                              // every column sees the keys up to here
 
   bool ok = true;
   int st = 0;
@@ -212,19 +216,22 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
       }
     }
     // which keys a column sees: all of them but at the end of its walk, where a slot behind the last key may hold anything
-    const bool masked = j - g8 + 31 > first_pos;
-    if (masked) {
+    bool none = false;
+    if (j - g8 + 31 > first_pos) {
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
           for (int e = 0; e < CPL; ++e)
-            if (j + 8 * x > pos0 + min(col0 + 8 * b + CPL * t4 + e, col0 + cols - 1) / R) s[x][b][e] = -INFINITY;
-        if (j + 8 * x > last)
+            if (j + 8 * x > pos0 + column_token(min(col0 + 8 * b + CPL * t4 + e, col0 + cols - 1), R)) s[x][b][e] = -INFINITY;
 #pragma unroll
-          for (int g = 0; g < NG; ++g) pv[x][g] = make_float2(0.f, 0.f);
+        for (int g = 0; g < NG; ++g) {
+          if (j + 8 * x > last) pv[x][g] = make_float2(0.f, 0.f);
+          none |= isnan(pv[x][g].y);
+        }
       }
+      none = __any_sync(0xffffffffu, none);                             // (a value that is none, maybe behind a column: 0 * NaN)
     }
     // do references or exponents have to move?
     bool grow = false;
@@ -283,59 +290,67 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
           s[x][b][e] = kf_exp2(fmaf(s[x][b][e], kq[b][e], -ref[b][e]));
           sum[b][e] += s[x][b][e];
         }
-    // y += (p s) c, p lo: by groups, the scales brought under 4 by a power of two that only grows
+    // y += (p s) c, p lo: by groups, the scales brought under 4 by a power of two that only grows.  Of a word's nibbles 0 and 1 (2 and 3) the rows of
+    // the second tile half take both as they stand, c + 16 c': the end takes c from it.  Where the result is fp16, whose 11 bits show what sums of codes
+    // lose, the sums stand around code 8: one more product takes 8 of every code, and lo gets 8 s.
+    auto add_values = [&](auto careful) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint32_t vw[2][W];
+      for (int h = 0; h < 2; ++h) {
+        uint32_t vw[2][W];
 #pragma unroll
-      for (int x = 0; x < 2; ++x) lds_words<W>(vw[x], unit + h * SLICE + kv4_v_codes(D) + (t4 + 4 * x) * D + g8 * 4 * W);
+        for (int x = 0; x < 2; ++x) lds_words<W>(vw[x], unit + h * SLICE + kv4_v_codes(D) + (t4 + 4 * x) * D + g8 * 4 * W);
 #pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        const float inv = __uint_as_float((254u << 23) - ev[g]);
-        uint32_t bw[NB][TERMS][2];
+        for (int g = 0; g < NG; ++g) {
+          const float inv = __uint_as_float((254u << 23) - ev[g]);
+          uint32_t bw[NB][TERMS][2];
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const float2 p = pv[2 * h + x][g];
-          const float sc = p.x * inv;
+          for (int x = 0; x < 2; ++x) {
+            const float2 p = pv[2 * h + x][g];
+            const float sc = p.x * inv, lo = FINE ? fmaf(8.f, p.x, p.y) : p.y;
 #pragma unroll
-          for (int b = 0; b < NB; ++b) {
-            float w[2] = {0.f, 0.f};
+            for (int b = 0; b < NB; ++b) {
+              float w[2] = {0.f, 0.f};
 #pragma unroll
-            for (int e = 0; e < CPL; ++e) {
-              const float pe = s[2 * h + x][b][e];
-              w[e] = pe * sc;
-              if (masked) {                                             // (a value that is no number, behind a column: no trace of it)
-                if (pe == 0.f) w[e] = 0.f;
-                else sumlo[b][g][e] = fmaf(pe, p.y, sumlo[b][g][e]);
-              } else {
-                sumlo[b][g][e] = fmaf(pe, p.y, sumlo[b][g][e]);
+              for (int e = 0; e < CPL; ++e) {
+                const float pe = s[2 * h + x][b][e];
+                w[e] = pe * sc;
+                if (careful.value && pe == 0.f) w[e] = 0.f;
+                else sumlo[b][g][e] = fmaf(pe, lo, sumlo[b][g][e]);
               }
-            }
-            if (CPL == 1) {
-              w[1] = w[0] - __half2float(__float2half_rn(w[0]));
-              bw[b][0][x] = movmatrix(half_bits(w[0], w[1]));
-            } else {
-              const uint32_t hi = half_bits(w[0], w[1]);
-              bw[b][0][x] = movmatrix(hi);
-              if (TERMS == 2) {
-                const float2 f = bits_pair<__half>(hi);
-                bw[b][TERMS - 1][x] = movmatrix(half_bits(w[0] - f.x, w[1] - f.y));
+              if (CPL == 1) {
+                if (FINE) {                                             // the odd column: what 11 bits leave over
+                  const float hi = __uint_as_float(__float_as_uint(w[0]) & 0xffffe000u);
+                  w[1] = w[0] - hi;
+                  w[0] = hi;
+                }
+                bw[b][0][x] = movmatrix(half_bits(w[0], w[1]));
+              } else {
+                const uint32_t hi = half_bits(w[0], w[1]);
+                bw[b][0][x] = movmatrix(hi);
+                if (TERMS == 2) {
+                  const float2 f = bits_pair<__half>(hi);
+                  bw[b][TERMS - 1][x] = movmatrix(half_bits(w[0] - f.x, w[1] - f.y));
+                }
               }
             }
           }
-        }
 #pragma unroll
-        for (int e = 0; e < SPG; ++e) {
-          const int r = g * SPG + e;
-          const uint32_t w0 = (r & 1) ? vw[0][r >> 1] >> 8 : vw[0][r >> 1], w1 = (r & 1) ? vw[1][r >> 1] >> 8 : vw[1][r >> 1];
+          for (int e = 0; e < SPG; ++e) {
+            const int r = g * SPG + e;
+            const uint32_t w0 = (r & 1) ? __byte_perm(vw[0][r >> 1], 0u, 0x4341) : vw[0][r >> 1] & 0x00ff00ffu;
+            const uint32_t w1 = (r & 1) ? __byte_perm(vw[1][r >> 1], 0u, 0x4341) : vw[1][r >> 1] & 0x00ff00ffu;
 #pragma unroll
-          for (int b = 0; b < NB; ++b)
+            for (int b = 0; b < NB; ++b) {
 #pragma unroll
-            for (int x = 0; x < TERMS; ++x)
-              mma_f16_16816(o[b][r], w0 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x000f000fu, w1 & 0x00f000f0u, bw[b][x][0], bw[b][x][1]);
+              for (int x = 0; x < TERMS; ++x) mma_f16_16816(o[b][r], w0 & 0x000f000fu, w0, w1 & 0x000f000fu, w1, bw[b][x][0], bw[b][x][1]);
+              if (FINE) mma_f16_16816(o[b][r], 0x80088008u, 0x80888088u, 0x80088008u, 0x80888088u, bw[b][0][0], bw[b][0][1]);
+            }
+          }
         }
       }
-    }
+    };
+    if (none) add_values(std::true_type());
+    else add_values(std::false_type());
     // the next 32 keys for this place of the ring
     const int nxt = i + STAGES;
     if ((nxt & 31) == 0) entry = nxt + lane < units ? table[2 * (nxt + lane)] : 0;
@@ -378,10 +393,11 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
     for (int r = 0; r < KS; ++r) {
       const float up = __uint_as_float(ev[r / SPG]);
 #pragma unroll
-      for (int e = 0; e < 2 * CPL; ++e) {                               // (codes were 2^-24 and, of odd nibbles, 2^-20 of themselves)
-        const float v = CPL == 2 ? o[b][r][e] : o[b][r][2 * e] + o[b][r][2 * e + 1];
-        so[(warp * COLS + 8 * b + CPL * t4 + (CPL == 2 ? e & 1 : 0)) * LD + 16 * r + 8 * (e / CPL) + g8] =
-            fmaf(v * (e < CPL ? 16777216.f : 1048576.f), up, sumlo[b][r / SPG][CPL == 2 ? e & 1 : 0]);
+      for (int e = 0; e < CPL; ++e) {                                   // (codes were 2^-24 of themselves)
+        const float c = CPL == 2 ? o[b][r][e] : o[b][r][0] + o[b][r][1], both = CPL == 2 ? o[b][r][2 + e] : o[b][r][2] + o[b][r][3];
+        float* const at = so + (warp * COLS + 8 * b + CPL * t4 + e) * LD + 16 * r + g8;
+        at[0] = fmaf(c * 16777216.f, up, sumlo[b][r / SPG][e]);
+        at[8] = fmaf((both - c) * 1048576.f, up, sumlo[b][r / SPG][e]);
       }
     }
   __syncthreads();
@@ -402,7 +418,7 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
     if (it.parts == 1) {
       const int cc = col0 + c;
       const uint2 out = make_uint2(pair_bits<T>(v[0] / l, v[1] / l), pair_bits<T>(v[2] / l, v[3] / l));
-      *reinterpret_cast<uint2*>(y + ((size_t)(first + cc / R) * a.H + head * R + cc % R) * D + d) = out;
+      *reinterpret_cast<uint2*>(y + ((size_t)(first + column_token(cc, R)) * a.H + head * R + column_head(cc, R)) * D + d) = out;
     } else {
       const size_t at = ((size_t)(it.base + it.part) * a.G + head) * COLS + c;
       *reinterpret_cast<float4*>(a.part + at * D + d) = make_float4(v[0], v[1], v[2], v[3]);
@@ -503,7 +519,7 @@ using namespace llb;
 extern "C" {
 
 size_t ll_kv4_attn_scratch_bytes(const ll_kv4_cache* cache, int B, int T, int max_count) {
-  return sizeof(float) * Kv4Lists(B, T, max_count, cache->heads, cache->kv_heads, cache->head_size, cache->max_length).floats(cache->kv_heads, cache->head_size);
+  return sizeof(float) * Kv4Lists(B, T, max_count, cache->heads, cache->kv_heads, cache->max_length).floats(cache->kv_heads, cache->head_size);
 }
 
 int ll_kv4_attn(const ll_kv4_cache* cache, const void* blocks, const void* q, long long q_row, const int32_t* work, void* y, int B, int T, int max_count,
@@ -518,7 +534,7 @@ int ll_kv4_attn(const ll_kv4_cache* cache, const void* blocks, const void* q, lo
   LL_CHECK_ARG(scale > 0.f, "kv4_attn: scores times %g (more than 0)", scale);
   LL_CHECK_ARG((((uintptr_t)q | (uintptr_t)y | (uintptr_t)blocks | (uintptr_t)scratch | (uintptr_t)work) & 15) == 0 && q_row % 8 == 0,
                "kv4_attn: rows have to start on 16-byte boundaries");
-  const Kv4Lists l(B, T, max_count, H, G, head_size, cache->max_length);
+  const Kv4Lists l(B, T, max_count, H, G, cache->max_length);
   LL_CHECK_ARG(l.few_items * G <= INT_MAX && l.many_items * G <= INT_MAX, "kv4_attn: %d sequences of %d tokens, %d heads", B, T, H);
   const int R = l.R, cols = l.cols;
   const long long items = l.few_items;
@@ -530,8 +546,10 @@ int ll_kv4_attn(const ll_kv4_cache* cache, const void* blocks, const void* q, lo
     m.max_items = (int)l.many_items;
     if (int r = kv4_prompt_launch(m, dtype, head_size, group, (cudaStream_t)stream)) return r;
 #define JOIN_MANY(TT, DD) LL_CUDA(launch(kv4_join_many_kernel<TT, DD>, dim3((unsigned)(l.many_items * G), KV4_MANY / 32), dim3(KJ * 32), 0, (cudaStream_t)stream, true, m));
-    if (dtype == LL_BF16 && head_size == 64) { JOIN_MANY(__nv_bfloat16, 64) }
+    if (dtype == LL_BF16 && head_size == 32) { JOIN_MANY(__nv_bfloat16, 32) }
+    else if (dtype == LL_BF16 && head_size == 64) { JOIN_MANY(__nv_bfloat16, 64) }
     else if (dtype == LL_BF16) { JOIN_MANY(__nv_bfloat16, 128) }
+    else if (head_size == 32) { JOIN_MANY(__half, 32) }
     else if (head_size == 64) { JOIN_MANY(__half, 64) }
     else { JOIN_MANY(__half, 128) }
 #undef JOIN_MANY

@@ -98,7 +98,7 @@ struct PlanWork {
   int parts, max_items;                // places for blocks, items there is room for
   int32_t* work;
 };
-constexpr int PW_SIZES = 512;          // sizes of parts told apart (larger ones by their 1 / PW_SIZES of the largest)
+constexpr int PW_SIZES = 512;          // sizes of parts told apart (where there are more, by twos, fours and so on)
 
 // Parts of `step` pages at most, step the smallest with which a step's walks make no more than `parts` parts, as many as there are places for blocks, or
 // where the walks are more than half of that are cut no more than `parts` times.  Parts of a size stand together, the largest first: blocks take them in
@@ -109,19 +109,21 @@ __device__ __forceinline__ void divide_work(const PlanView& v, const PlanWork& d
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   auto tokens = [&](int i) { return v.starts[i + 1] - v.starts[i]; };
   auto tiles = [&](int i) {
-    const long long c = (long long)tokens(i) * d.R;
-    return (c > d.few) == MANY ? (int)((c + d.cols - 1) / d.cols) : 0;
+    const uint32_t c = (uint32_t)tokens(i) * (uint32_t)d.R;          // (tokens times heads fit 31 bits)
+    return (c > (uint32_t)d.few) == MANY ? (int)((c + (uint32_t)d.cols - 1) / (uint32_t)d.cols) : 0;
   };
   // pages that a tile's last column sees
   auto pages = [&](int i, int tile) {
     if (v.request[i] < 0) return 1;
     const int n = tokens(i);
-    return (v.ends[i] - n + (MANY ? (int)min((long long)n - 1, ((long long)(tile + 1) * d.cols - 1) / d.R) : n - 1)) / KV4_PAGE + 1;
+    return (v.ends[i] - n + (MANY ? min(n - 1, (int)(((uint32_t)(tile + 1) * (uint32_t)d.cols - 1) / (uint32_t)d.R)) : n - 1)) / KV4_PAGE + 1;
   };
   // parts of all walks, by one warp
   auto total = [&](int step) {
     int sum = 0;
-    if (MANY) {
+    if (MANY && step >= d.longest) {
+      for (int i = lane; i < v.B; i += 32) sum += tiles(i);
+    } else if (MANY) {
       for (int i = 0; i < v.B; ++i) {
         const int w = tiles(i);
         for (int t = lane; t < w; t += 32) sum += (pages(i, t) + step - 1) / step;
@@ -163,7 +165,9 @@ __device__ __forceinline__ void divide_work(const PlanView& v, const PlanWork& d
   const int step = hi;
   // a walk's pages in equal parts; the places of the sizes, counted and summed from the largest down
   auto cut = [&](int p) { return (p + step - 1) / step; };
-  auto bucket = [&](int size) { return PW_SIZES - 1 - (int)((long long)(min(size, step) - 1) * PW_SIZES / step); };
+  int shift = 0;
+  while ((step - 1) >> shift >= PW_SIZES) ++shift;
+  auto bucket = [&](int size) { return PW_SIZES - 1 - ((min(size, step) - 1) >> shift); };
   for (int x = threadIdx.x; x < PW_SIZES; x += blockDim.x) s_size[x] = 0;
   __syncthreads();
   for (int i = MANY ? warp : threadIdx.x; i < v.B; i += MANY ? warps : blockDim.x) {
@@ -519,7 +523,7 @@ extern "C" {
 size_t ll_kv4_page_bytes(int head_size, int group) { return kv4_shape_ok(head_size, group) ? (size_t)kv4_bytes(head_size, head_size / group) : 0; }
 
 size_t ll_kv4_work_ints(const ll_kv4_cache* cache, int B, int T, int max_count) {
-  return Kv4Lists(B, T, max_count, cache->heads, cache->kv_heads, cache->head_size, cache->max_length).ints();
+  return Kv4Lists(B, T, max_count, cache->heads, cache->kv_heads, cache->max_length).ints();
 }
 
 int ll_kv4_plan(const ll_kv4_cache* cache, const int32_t* rows, const int32_t* counts, int B, int T, int max_count, int32_t* out, int32_t* work,
@@ -529,7 +533,7 @@ int ll_kv4_plan(const ll_kv4_cache* cache, const int32_t* rows, const int32_t* c
                "kv4_plan: %d sequences of %d tokens, %d at most", B, T, max_count);
   const Kv4Pool c = pool_of(cache);
   const Kv4Plan p{out, out + B + 1, out + 2 * (size_t)B + 1, out + 3 * (size_t)B + 1, out + 4 * (size_t)B + 1, out + 4 * (size_t)B + 1 + T};
-  const Kv4Lists l(B, T, max_count, cache->heads, cache->kv_heads, cache->head_size, cache->max_length);
+  const Kv4Lists l(B, T, max_count, cache->heads, cache->kv_heads, cache->max_length);
   LL_CHECK_ARG(l.few_items * cache->kv_heads <= INT_MAX && l.many_items * cache->kv_heads <= INT_MAX, "kv4_plan: %d sequences of %d tokens, %d heads", B, T, cache->heads);
   const int longest = (cache->max_length + KV4_PAGE - 1) / KV4_PAGE;
   const PlanWork few{l.R, l.few, l.cols, longest, l.least, l.few_parts, (int)l.few_items, work};

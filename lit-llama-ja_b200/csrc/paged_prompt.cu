@@ -13,6 +13,8 @@
 // Values that are no numbers are zeros in the operand, the first position of such a group is kept and rows that see it end as no numbers: 0 * NaN would
 // reach rows that do not.
 // Every wait is bounded; one that runs out records a code, all roles stop, copies in flight are waited for, tensor memory is freed.
+#include <type_traits>
+
 #include "attn_tc.cuh"
 #include "paged_work.cuh"
 
@@ -25,10 +27,10 @@ constexpr int KP_RING = 3, KP_STAGES = 3, KP_EXPS = 8;               // copies i
 
 template <int D, int NG>
 struct KpShape {
-  static constexpr int NB = D / 64, SLICE = kv4_slice_bytes(D, NG);
+  static constexpr int NB = (D + 63) / 64, SLICE = kv4_slice_bytes(D, NG);
   static constexpr int Q = 2 * NB * KP_QBOX, K = NB * KP_KBOX, V = D * 128;
   static constexpr int RING = KP_DEQUANT * KP_RING * SLICE;
-  static constexpr int SMEM = 1024 + Q + KP_STAGES * (K + V) + RING + 512 + 4 * KP_ROWS * 4 + KP_EXPS * 4 * 8;
+  static constexpr int SMEM = 1024 + Q + KP_STAGES * (K + V) + RING + 512 + 4 * KP_ROWS * 4 + KP_EXPS * 4 * 2;
 };
 
 __device__ __forceinline__ bool kp_wait(uint64_t* bar, uint32_t parity, volatile int* fail, int* word, int code) {
@@ -45,15 +47,12 @@ __device__ __forceinline__ bool kp_wait(uint64_t* bar, uint32_t parity, volatile
 __host__ __device__ constexpr uint32_t instr_desc_f16(int M, int N) { return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24); }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }      // -126 <= e <= 127
 
-// A slice's power of two: the multiple of 16 that brings numbers of up to `largest` (bits of a float) under 2^10.
+// A slice's power of two, from the lanes' largest scale (low half) and lowest value: the multiple of 16 that brings |lo| + 15 s under 2^11.
+template <typename T>
 __device__ __forceinline__ int slice_exponent(uint32_t largest) {
-  const int fl = (int)(largest >> 23) - 127;
+  const float2 p = bits_pair<T>(largest);
+  const int fl = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(p.y, 16.f * p.x))) >> 23) - 127;
   return max(-112, min(112, ((fl + 6) >> 4) << 4));
-}
-// the larger of |lo| and |lo + 15 s|, bits of a float; 0 for a group that is no number
-__device__ __forceinline__ uint32_t group_reach(float2 p) {
-  const uint32_t b = __float_as_uint(fmaxf(fabsf(p.y), fabsf(fmaf(15.f, p.x, p.y))));
-  return b < 0x7f800000u ? b : 0u;
 }
 __device__ __forceinline__ __half2 as_half2(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
 __device__ __forceinline__ uint32_t as_u32(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
@@ -102,8 +101,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
   int* s_fail = reinterpret_cast<int*>(tmem_ptr + 1);
   int* s_none = s_fail + 1;                           // [4] per group the first position whose value is no number
   float* s_x = reinterpret_cast<float*>(ring + Shape::RING + 512);      // [tile][half][row]: what the two threads of a row tell one another
-  int* s_ek = reinterpret_cast<int*>(s_x + 4 * KP_ROWS);                // [page & 7][slice] exponents of keys and values
-  int* s_ev = s_ek + KP_EXPS * 4;
+  signed char* s_ek = reinterpret_cast<signed char*>(s_x + 4 * KP_ROWS);      // [page & 7][slice] exponents of keys and values
+  signed char* s_ev = s_ek + KP_EXPS * 4;
 
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   // what every role walks: pages page0 .. page1; per tile the last page that one of its rows sees
@@ -151,32 +150,52 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
       if (!ok) break;
       const uint8_t* blk = mine + st * SLICE;
       uint32_t kw[2][W], vw[2][W];
-      float2 kp[2][NG], vp[2][2][NG];                 // keys g8 + 8 x; values of slots 2 (t4 + 4 x) + e
+      uint32_t kp[2][NG], vp[2][2][NG];               // parameters of keys g8 + 8 x and of the values of slots 2 (t4 + 4 x) + e
+      uint32_t bk = 0, bv = 0;                        // sizes rise with their bits: the largest scale, and the largest lowest value
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        uint32_t u[NG];
         lds_words<W>(kw[x], blk + (g8 + 8 * x) * (D / 2) + t4 * 4 * W);
         lds_words<W>(vw[x], blk + kv4_v_codes(D) + (t4 + 4 * x) * D + g8 * 4 * W);
-        lds_words<NG>(u, blk + kv4_k_params(D) + (g8 + 8 * x) * NG * 4);
+        lds_words<NG>(kp[x], blk + kv4_k_params(D) + (g8 + 8 * x) * NG * 4);
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {                // (a slot behind the last key may hold anything)
-          kp[x][g] = bits_pair<T>(u[g]);
-          if ((page0 + n) * KV4_PAGE + KV4_SLICE * sl + g8 + 8 * x > last) kp[x][g] = make_float2(0.f, 0.f);
-        }
+        for (int e = 0; e < 2; ++e) lds_words<NG>(vp[x][e], blk + kv4_v_params(D, NG) + (2 * (t4 + 4 * x) + e) * NG * 4);
+      }
+      const int pos = (page0 + n) * KV4_PAGE + KV4_SLICE * sl;
+      if (pos + KV4_SLICE - 1 > last) {               // (a slot behind the last key may hold anything)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          lds_words<NG>(u, blk + kv4_v_params(D, NG) + (2 * (t4 + 4 * x) + e) * NG * 4);
-          const int pos = (page0 + n) * KV4_PAGE + KV4_SLICE * sl + 2 * (t4 + 4 * x) + e;
+        for (int x = 0; x < 2; ++x)
 #pragma unroll
           for (int g = 0; g < NG; ++g) {
-            vp[x][e][g] = bits_pair<T>(u[g]);
-            if (pos > last) vp[x][e][g] = make_float2(0.f, 0.f);
-            if (isnan(vp[x][e][g].y)) {
-              atomicMin(&s_none[g], pos);
-              vp[x][e][g] = make_float2(0.f, 0.f);
+            if (pos + g8 + 8 * x > last) kp[x][g] = 0u;
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              if (pos + 2 * (t4 + 4 * x) + e > last) vp[x][e][g] = 0u;
+          }
+      }
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          bk = __vmaxu2(bk, kp[x][g] & 0x7fff7fffu);
+          bv = __vmaxu2(__vmaxu2(bv, vp[x][0][g] & 0x7fff7fffu), vp[x][1][g] & 0x7fff7fffu);
+        }
+      constexpr uint32_t NUMBERS = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;      // (a group that is no number is so in both)
+      if (__any_sync(0xffffffffu, (bk >> 16) >= NUMBERS || (bv >> 16) >= NUMBERS)) {
+        bk = bv = 0u;
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int g = 0; g < NG; ++g) {
+            if ((kp[x][g] & 0x7fffu) < NUMBERS) bk = __vmaxu2(bk, kp[x][g] & 0x7fff7fffu);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              if ((vp[x][e][g] & 0x7fffu) >= NUMBERS) {
+                atomicMin(&s_none[g], pos + 2 * (t4 + 4 * x) + e);
+                vp[x][e][g] = 0u;
+              }
+              bv = __vmaxu2(bv, vp[x][e][g] & 0x7fff7fffu);
             }
           }
-        }
       }
       const int nxt = n + KP_RING;
       if ((nxt & 31) == 0) entry = nxt + lane < units ? table[nxt + lane] : 0;
@@ -186,12 +205,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
         mbar_expect_tx(&full[st], SLICE);
         bulk_load_1d(mine + st * SLICE, from + min(max(page, 0), a.pages - 1) * page_bytes, SLICE, &full[st]);
       }
-      uint32_t rk = 0, rv = 0;
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int g = 0; g < NG; ++g) rk = max(rk, group_reach(kp[x][g])), rv = max(rv, max(group_reach(vp[x][0][g]), group_reach(vp[x][1][g])));
-      const int ek = slice_exponent(__reduce_max_sync(0xffffffffu, rk)), ev = slice_exponent(__reduce_max_sync(0xffffffffu, rv));
+      const int ek = slice_exponent<T>(bk), ev = slice_exponent<T>(bv);
       const float fk = pow2(-ek), fv = pow2(-ev);
       // keys: row = slot, 8 bytes of four dimensions at a time
       ok = __all_sync(0xffffffffu, kp_wait(&k_empty[ks], ((n / KP_STAGES) & 1) ^ 1, s_fail, a.word, 2));
@@ -201,7 +215,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
         const int r = KV4_SLICE * sl + g8 + 8 * x;
 #pragma unroll
         for (int i = 0; i < W; ++i) {
-          const float2 p = kp[x][i * NG / W];
+          const float2 p = bits_pair<T>(kp[x][i * NG / W]);
           const __half2 s = __float2half2_rn(p.x * fk), lo = __float2half2_rn(p.y * fk);
           uint8_t* row = sk + ks * Shape::K + (i >> 1) * KP_KBOX + r * 128;
           const int c = 4 * (i & 1) + (t4 >> 1), b = 8 * (t4 & 1);      // 16-byte piece of dimensions 32 i + 4 t4 in the row, 8 bytes in it
@@ -209,7 +223,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
           *reinterpret_cast<uint2*>(row + (((c + 2) ^ (r & 7)) << 4) + b) = make_uint2(word_pair<2>(kw[x][i], s, lo), word_pair<3>(kw[x][i], s, lo));
         }
       }
-      if (lane == 0) s_ek[(n & (KP_EXPS - 1)) * 4 + sl] = ek, s_ev[(n & (KP_EXPS - 1)) * 4 + sl] = ev;
+      if (lane == 0) s_ek[(n & (KP_EXPS - 1)) * 4 + sl] = (signed char)ek, s_ev[(n & (KP_EXPS - 1)) * 4 + sl] = (signed char)ev;
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(&k_full[ks]);
@@ -220,7 +234,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
       for (int x = 0; x < 2; ++x)
 #pragma unroll
         for (int i = 0; i < W; ++i) {
-          const float2 p0 = vp[x][0][i * NG / W], p1 = vp[x][1][i * NG / W];
+          const float2 p0 = bits_pair<T>(vp[x][0][i * NG / W]), p1 = bits_pair<T>(vp[x][1][i * NG / W]);
           const __half2 s = __floats2half2_rn(p0.x * fv, p1.x * fv), lo = __floats2half2_rn(p0.y * fv, p1.y * fv);
           uint8_t* at = sv + ks * Shape::V + (32 * i + g8) * 128 + (((2 * sl + x) ^ g8) << 4) + 4 * t4;
           *reinterpret_cast<uint32_t*>(at) = word_pair<0>(vw[x][i], s, lo);
@@ -253,7 +267,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
 #pragma unroll
           for (int c = 0; c < NB; ++c)
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
+            for (int k = 0; k < (D < 64 ? D / 16 : 4); ++k)
               umma_bf16(d, qdesc + (uint64_t)(c * (KP_QBOX >> 4) + 2 * k), kdesc + (uint64_t)(c * (KP_KBOX >> 4) + 2 * k), idesc_s, (c | k) != 0 ? 1u : 0u);
           umma_commit(&s_full[2 * i + (n & 1)]);
           umma_commit(&k_empty[ks]);
@@ -348,10 +362,15 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
       tc_fence_after();
       uint32_t sr[32];
       tmem_ld32_async(ts + 32u * half, sr);
-      const int* ek = s_ek + (n & (KP_EXPS - 1)) * 4 + 2 * half;
-      const int4 ev = *reinterpret_cast<const int4*>(s_ev + (n & (KP_EXPS - 1)) * 4);
-      const int emax = max(max(ev.x, ev.y), max(ev.z, ev.w)), ev0 = half ? ev.z : ev.x, ev1 = half ? ev.w : ev.y;
-      const float mul0 = mul * pow2(ek[0]), mul1 = mul * pow2(ek[1]);   // of the two slices
+      // (exponents that are all 0, as they mostly are, cost two loads and a comparison)
+      const uint32_t eks = reinterpret_cast<const uint32_t*>(s_ek)[n & (KP_EXPS - 1)], evs = reinterpret_cast<const uint32_t*>(s_ev)[n & (KP_EXPS - 1)];
+      float mul0 = mul, mul1 = mul;                                     // of the thread's two slices
+      int emax = 0, ev0 = 0, ev1 = 0;
+      if ((eks | evs) != 0u) {
+        mul0 *= pow2((int)(signed char)(eks >> (16 * half))), mul1 *= pow2((int)(signed char)(eks >> (16 * half + 8)));
+        ev0 = (int)(signed char)(evs >> (16 * half)), ev1 = (int)(signed char)(evs >> (16 * half + 8));
+        emax = max(max((int)(signed char)evs, (int)(signed char)(evs >> 8)), max((int)(signed char)(evs >> 16), (int)(signed char)(evs >> 24)));
+      }
       tmem_wait_ld();
       tie32(sr);
       const int cmax = qp - ((page0 + n) * KV4_PAGE + 32 * half);       // the row's last visible column of these 32
@@ -402,20 +421,23 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
       uint32_t ph[16];
 #pragma unroll
       for (int x = 0; x < 2; ++x) {                                     // the two slices
-        const float mm = x ? mul1 : mul0, shift = sub + (float)((x ? ev1 : ev0) - ebase);
-        const f2 m2 = f2_of(mm, mm), s2 = f2_of(shift, shift);
-        f2 part = f2_of(0.f, 0.f);
+        const float mm = x ? mul1 : mul0;
+        const f2 m2 = f2_of(mm, mm), s2 = f2_of(sub, sub);
+        const int down = (x ? ev1 : ev0) - ebase;                         // (0 or less, the same for the warp)
+        const float f = pow2(max(down, -126));
+        f2 part[2] = {f2_of(0.f, 0.f), f2_of(0.f, 0.f)};
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           float a0, a1;
           f2_split(f2_fma(f2_of(__uint_as_float(sr[16 * x + 2 * e]), __uint_as_float(sr[16 * x + 2 * e + 1])), m2, s2), a0, a1);
-          ph[8 * x + e] = pair_bits<__half>(at_exp2(a0), at_exp2(a1));
-          const float2 p = bits_pair<__half>(ph[8 * x + e]);            // the sum is of the weights as the product sees them
-          part = f2_add(part, f2_of(p.x, p.y));
+          float p0 = at_exp2(a0), p1 = at_exp2(a1);
+          part[e & 1] = f2_add(part[e & 1], f2_of(p0, p1));
+          if (down != 0) p0 *= f, p1 *= f;
+          ph[8 * x + e] = pair_bits<__half>(p0, p1);
         }
         float p0, p1;
-        f2_split(part, p0, p1);
-        sum = fmaf(p0 + p1, pow2(min(ebase - (x ? ev1 : ev0), 126)), sum);
+        f2_split(f2_add(part[0], part[1]), p0, p1);
+        sum += p0 + p1;
       }
       // the weights go over the thread's own scores
       tmem_st16(ts + 32u * half, ph);
@@ -496,7 +518,7 @@ int kv4_prompt_launch(const Kv4Attn& a, int dtype, int head_size, int group, cud
     if (dtype == LL_BF16) return prompt_launch<__nv_bfloat16, DD, NG>(a, st); \
     return prompt_launch<__half, DD, NG>(a, st);                  \
   }
-  PROMPT(64, 1) PROMPT(64, 2) PROMPT(128, 1) PROMPT(128, 2) PROMPT(128, 4)
+  PROMPT(32, 1) PROMPT(64, 1) PROMPT(64, 2) PROMPT(128, 1) PROMPT(128, 2) PROMPT(128, 4)
 #undef PROMPT
   set_error("kv4_attn: no prompt kernel for heads of %d in groups of %d", head_size, group);
   return LL_ERR_UNSUPPORTED;

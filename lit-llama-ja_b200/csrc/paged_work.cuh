@@ -44,7 +44,7 @@ constexpr float KV4_NONE = -1e37f;      // the reference of a column that has se
 // Sequences that bring up to this many columns a key head go to the kernel of few columns, others to the tcgen05 kernel in tiles of KV4_MANY.
 constexpr int KV4_FEW_MOST = 32, KV4_MANY = 256, KV4_WHOLE = 8;
 
-inline bool kv4_many(int max_count, int R, int head_size) { return head_size >= 64 && (long long)max_count * R > KV4_FEW_MOST; }
+inline bool kv4_many(int max_count, int R) { return (long long)max_count * R > KV4_FEW_MOST; }
 inline int kv4_sms() { return sm_count() > 0 ? sm_count() : 148; }
 
 // A step's two lists: sequences of few columns and, where one may bring more, of many.  Sizes as the host knows them.
@@ -53,9 +53,9 @@ struct Kv4Lists {
   int least;                            // pages of a part of the few, at least
   long long few_items, many_items;      // at most
   bool many, few_cut;
-  Kv4Lists(int B, int T, int max_count, int H, int G, int head_size, int max_length) {
+  Kv4Lists(int B, int T, int max_count, int H, int G, int max_length) {
     R = H / G;
-    many = kv4_many(max_count, R, head_size);
+    many = kv4_many(max_count, R);
     const long long c = (long long)max_count * R;
     cols = many ? 8 : c <= 4 ? 4 : c <= 8 ? 8 : 16;
     few = many ? KV4_FEW_MOST : INT_MAX;

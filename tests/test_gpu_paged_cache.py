@@ -442,3 +442,24 @@ def test_the_same_bits_every_time():
         cache, plan, q, _, _ = _filled(held, counts, 8, 2, 128, 64, BF)
         first = cache.attend(0, plan, q.to(DEV))
         assert all(torch.equal(cache.attend(0, plan, q.to(DEV)), first) for _ in range(20))
+
+
+@pytest.mark.parametrize("counts", [[1], [8], [150]])
+@torch.no_grad()
+def test_slices_of_unequal_size(counts):
+    """Values that are zeros for the keys of some slices and pages, 2^40 apart for others; keys 2^30 apart, under scores that stay small."""
+    held, H, D, dtype = [330], 2, 64, BF
+    torch.manual_seed(4)
+    L = held[0] + counts[0]
+    k, v = torch.randn(L, H, D), torch.randn(L, H, D) + 1.0
+    v[:, 0, :] *= torch.tensor([0.0, 1.0, 2.0 ** 20, 2.0 ** -20])[(torch.arange(L) // 16) % 4][:, None]
+    v[64:128] = 0.0
+    v[128:200] *= 2.0 ** 25
+    k[:, 1, :] *= torch.tensor([1.0, 2.0 ** -30, 0.0, 0.25])[(torch.arange(L) // 16) % 4][:, None]
+    k, v, q = k.to(dtype), v.to(dtype), torch.randn(counts[0], H, D).to(dtype)
+    cache = _cache(1, H, D, group=32, dtype=dtype, pages=9, requests=1, max_length=600)
+    plan = cache.plan([0], [L], L)
+    cache.append(0, plan, None, k.to(DEV), v.to(DEV))
+    cache.truncate([0], held)
+    plan = cache.plan([0], counts, counts[0], max_count=counts[0])
+    _near(cache.attend(0, plan, q.to(DEV)), q, held_as(k, 32), held_as(v, 32), held, counts, dtype, D ** -0.5)
