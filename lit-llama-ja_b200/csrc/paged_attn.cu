@@ -35,9 +35,6 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t v) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
-// column -> token and head, without a division where a key head serves one head
-__device__ __forceinline__ int column_token(int c, int R) { return R == 1 ? c : c / R; }
-__device__ __forceinline__ int column_head(int c, int R) { return R == 1 ? 0 : c % R; }
 __device__ __forceinline__ uint32_t half_bits(float a, float b) { return pair_bits<__half>(a, b); }
 
 // One warp's wait for its copy: bounded; one that runs out leaves a code for the host.
@@ -422,7 +419,7 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
     } else {
       const size_t at = ((size_t)(it.base + it.part) * a.G + head) * COLS + c;
       *reinterpret_cast<float4*>(a.part + at * D + d) = make_float4(v[0], v[1], v[2], v[3]);
-      if (d == 0) *reinterpret_cast<float2*>(a.part + (size_t)a.max_items * a.G * COLS * D + at * 2) = make_float2(m, l);
+      if (d == 0) *reinterpret_cast<float2*>(a.part + (size_t)a.kept * a.G * COLS * D + at * 2) = make_float2(m, l);
     }
   }
 }
@@ -442,7 +439,7 @@ __global__ void __launch_bounds__(KJ * 32) kv4_join_kernel(const Kv4Attn a) {
   if (it.part != 0 || it.parts == 1 || it.row < 0 || col >= it.count * R) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const float* part = after_wait(a.part);
-  const float2* ml = reinterpret_cast<const float2*>(part + (size_t)a.max_items * a.G * COLS * D);
+  const float2* ml = reinterpret_cast<const float2*>(part + (size_t)a.kept * a.G * COLS * D);
   float m = KV4_NONE, l = 0.f, o[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.f;
@@ -487,7 +484,7 @@ __global__ void __launch_bounds__(KJ * 32) kv4_join_many_kernel(const Kv4Attn a)
   if (it.part != 0 || it.parts == 1 || it.row < 0) return;
   const int R = a.H / a.G, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const float* part = after_wait(a.part);
-  const float2* ml = reinterpret_cast<const float2*>(part + (size_t)a.max_items * a.G * KV4_MANY * D);
+  const float2* ml = reinterpret_cast<const float2*>(part + (size_t)a.kept * a.G * KV4_MANY * D);
   for (int c = 32 * blockIdx.y + warp; c < 32 * (blockIdx.y + 1); c += KJ) {
     const int col = it.tile * KV4_MANY + c;
     if (col >= it.count * R) return;
@@ -538,12 +535,13 @@ int ll_kv4_attn(const ll_kv4_cache* cache, const void* blocks, const void* q, lo
   LL_CHECK_ARG(l.few_items * G <= INT_MAX && l.many_items * G <= INT_MAX, "kv4_attn: %d sequences of %d tokens, %d heads", B, T, H);
   const int R = l.R, cols = l.cols;
   const long long items = l.few_items;
-  const Kv4Attn a{q, q_row, (const uint8_t*)blocks, cache->table, work, y, (float*)scratch, H, G, cache->width, cache->pages, (int)items, scale, wait_word()};
+  const Kv4Attn a{q, q_row, (const uint8_t*)blocks, cache->table, work, y, (float*)scratch, H, G, cache->width, cache->pages, (int)items, l.few_kept(), scale, wait_word()};
   if (l.many) {
     Kv4Attn m = a;
     m.work = work + l.few_ints();
     m.part = (float*)scratch + l.few_floats(G, head_size);
-    m.max_items = (int)l.many_items;
+    m.items = (int)l.many_items;
+    m.kept = l.many_kept();
     if (int r = kv4_prompt_launch(m, dtype, head_size, group, (cudaStream_t)stream)) return r;
 #define JOIN_MANY(TT, DD) LL_CUDA(launch(kv4_join_many_kernel<TT, DD>, dim3((unsigned)(l.many_items * G), KV4_MANY / 32), dim3(KJ * 32), 0, (cudaStream_t)stream, true, m));
     if (dtype == LL_BF16 && head_size == 32) { JOIN_MANY(__nv_bfloat16, 32) }

@@ -94,15 +94,19 @@ __device__ __forceinline__ void place_token(const PlanView& v, const Kv4Pool& c,
 
 // ---- the division of a step's attention
 struct PlanWork {
-  int R, few, cols, longest, least;    // columns a token, most columns of the few, columns of a tile; most pages of a request, fewest of a part
-  int parts, max_items;                // places for blocks, items there is room for
+  int R, few, cols, longest;           // columns a token, most columns of the few, columns of a tile; most pages of a request
+  int parts, max_items;                // places for blocks (a key head), items there is room for
+  float fixed, joined;                 // what a part costs beside its pages, and what parts that have to be joined cost the step, in pages
+  bool cut;                            // whether walks may be cut
   int32_t* work;
 };
 constexpr int PW_SIZES = 512;          // sizes of parts told apart (where there are more, by twos, fours and so on)
+constexpr int PW_TRIES = 48;
 
-// Parts of `step` pages at most, step the smallest with which a step's walks make no more than `parts` parts, as many as there are places for blocks, or
-// where the walks are more than half of that are cut no more than `parts` times.  Parts of a size stand together, the largest first: blocks take them in
-// that order, and the short ones fill the end.
+// Parts of `step` pages at most, every walk in equal ones.  Parts of a size stand together, the largest first: blocks take them in that order, and the
+// short ones fill the end.  step is the one of PW_TRIES that leaves the step the shortest, by what such an order comes to: the load a place, and
+// of the round that is not full the time of the shortest parts, but no less than the longest part.  Walks for several rounds even out by
+// themselves and stay whole.
 // MANY false: the sequences of up to `few` columns, whose tiles count as long as the last one; true: the others.
 template <bool MANY>
 __device__ __forceinline__ void divide_work(const PlanView& v, const PlanWork& d, int* s_count, int* s_size) {
@@ -118,51 +122,66 @@ __device__ __forceinline__ void divide_work(const PlanView& v, const PlanWork& d
     const int n = tokens(i);
     return (v.ends[i] - n + (MANY ? min(n - 1, (int)(((uint32_t)(tile + 1) * (uint32_t)d.cols - 1) / (uint32_t)d.R)) : n - 1)) / KV4_PAGE + 1;
   };
-  // parts of all walks, by one warp
-  auto total = [&](int step) {
-    int sum = 0;
-    if (MANY && step >= d.longest) {
-      for (int i = lane; i < v.B; i += 32) sum += tiles(i);
-    } else if (MANY) {
-      for (int i = 0; i < v.B; ++i) {
-        const int w = tiles(i);
-        for (int t = lane; t < w; t += 32) sum += (pages(i, t) + step - 1) / step;
-      }
-    } else {
-      for (int i = lane; i < v.B; i += 32) {
-        const int w = tiles(i);
-        if (w > 0) sum += w * ((pages(i, 0) + step - 1) / step);
-      }
-    }
-    return __reduce_add_sync(0xffffffffu, sum);
-  };
-  // every warp looks at one of the steps between; the smallest that will do is in (lo, hi]
-  int lo = min(d.least, d.longest) - 1, hi = d.longest;
+  // walks, by one warp
   __syncthreads();
   if (warp == 0) {
-    const int all = total(hi);
-    if (lane == 0) s_count[0] = all;
+    int n = 0;
+    for (int i = lane; i < v.B; i += 32) n += tiles(i);
+    n = __reduce_add_sync(0xffffffffu, n);
+    if (lane == 0) s_count[0] = n;
   }
   __syncthreads();
-  const int all = s_count[0], most = 2ll * all > d.parts ? all + d.parts : d.parts;
-  if (all >= 4ll * d.parts) lo = hi - 1;      // (walks for several rounds even out by themselves)
-  while (hi - lo > 1) {
-    const int each = (hi - lo + warps) / (warps + 1), mine = lo + each * (warp + 1);
-    __syncthreads();
-    if (mine < hi) {
-      const int parts = total(mine);
-      if (lane == 0) s_count[warp] = parts;
+  const int walks = s_count[0];
+  if (walks == 0) {
+    if (threadIdx.x == 0) d.work[0] = 0;
+    return;
+  }
+  int step = d.longest;
+  if (d.cut && walks < KV4_ROUNDS * d.parts) {
+    // how long the step takes with parts of `step` pages at most, by one warp
+    auto length = [&](int step) {
+      int n = 0, sum = 0, most = 0, least = INT_MAX;
+      auto add = [&](int w, int p) {
+        const int k = (p + step - 1) / step, each = (p + k - 1) / k;
+        n += w * k, sum += w * p, most = max(most, each), least = min(least, each);
+      };
+      for (int i0 = 0; i0 < v.B; i0 += 32) {
+        const int w = i0 + lane < v.B ? tiles(i0 + lane) : 0;
+        if (MANY) {
+          for (uint32_t with = __ballot_sync(0xffffffffu, w > 0); with != 0u; with &= with - 1) {
+            const int l = __ffs(with) - 1, all = __shfl_sync(0xffffffffu, w, l);
+            for (int t = lane; t < all; t += 32) add(1, pages(i0 + l, t));
+          }
+        } else if (w > 0) {
+          add(w, pages(i0 + lane, 0));
+        }
+      }
+      n = __reduce_add_sync(0xffffffffu, n), sum = __reduce_add_sync(0xffffffffu, sum);
+      most = __reduce_max_sync(0xffffffffu, most), least = __reduce_min_sync(0xffffffffu, least);
+      const int rounds = (n + d.parts - 1) / d.parts;
+      const float load = (sum + n * d.fixed) / d.parts + (rounds - (float)n / d.parts) * (least + d.fixed);
+      return n > walks + KV4_CUTS * d.parts ? 1e30f : fmaxf(load, most + d.fixed) + (n > walks ? d.joined : 0.f);
+    };
+    // the longest walk in 1, 2 .. 24, then 30, 36, 42, 48, 60 .. parts
+    auto tried = [&](int k) {
+      const int c = k < 24 ? k + 1 : 6 * (4 + ((k - 24) & 3)) << ((k - 24) >> 2);
+      return max(1, (d.longest + c - 1) / c);
+    };
+    float best = 1e30f;
+    int mine = 0;
+    for (int k = warp; k < PW_TRIES; k += warps) {
+      const float f = length(tried(k));
+      if (f < best) best = f, mine = k;
     }
     __syncthreads();
-    int best = hi;
-    for (int w = warps - 1; w >= 0; --w)
-      if (lo + each * (w + 1) < hi && s_count[w] <= most) best = lo + each * (w + 1);
-    int below = lo;
-    for (int w = 0; w < warps; ++w)
-      if (lo + each * (w + 1) < best) below = lo + each * (w + 1);
-    lo = below, hi = best;
+    if (lane == 0) s_count[warp] = __float_as_int(best), s_size[warp] = mine;      // (not negative: the bits rise with it)
+    __syncthreads();
+    int at = 0;
+    for (int w = 1; w < warps; ++w)
+      if (s_count[w] < s_count[at] || (s_count[w] == s_count[at] && s_size[w] < s_size[at])) at = w;
+    step = tried(s_size[at]);
+    __syncthreads();
   }
-  const int step = hi;
   // a walk's pages in equal parts; the places of the sizes, counted and summed from the largest down
   auto cut = [&](int p) { return (p + step - 1) / step; };
   int shift = 0;
@@ -536,8 +555,9 @@ int ll_kv4_plan(const ll_kv4_cache* cache, const int32_t* rows, const int32_t* c
   const Kv4Lists l(B, T, max_count, cache->heads, cache->kv_heads, cache->max_length);
   LL_CHECK_ARG(l.few_items * cache->kv_heads <= INT_MAX && l.many_items * cache->kv_heads <= INT_MAX, "kv4_plan: %d sequences of %d tokens, %d heads", B, T, cache->heads);
   const int longest = (cache->max_length + KV4_PAGE - 1) / KV4_PAGE;
-  const PlanWork few{l.R, l.few, l.cols, longest, l.least, l.few_parts, (int)l.few_items, work};
-  const PlanWork many{l.R, l.few, KV4_MANY, longest, 1, l.many_parts, (int)l.many_items, l.many ? work + l.few_ints() : nullptr};
+  // (pages take a block of the few 0.8 us, of the many 1.4; a part's start and end 2 and 3, parts that are joined 3 and 8 more)
+  const PlanWork few{l.R, l.few, l.cols, longest, l.few_parts, (int)l.few_items, 2.5f, 3.5f, l.few_cut, work};
+  const PlanWork many{l.R, l.few, KV4_MANY, longest, l.many_parts, (int)l.many_items, 2.f, 5.5f, true, l.many ? work + l.few_ints() : nullptr};
   // The block itself places the tokens of a step while that takes it a few rounds; more are placed by a grid.
   const int threads = B <= 256 && T <= 2048 ? 256 : PLAN_THREADS, here = T <= 8 * threads ? T : 0;
   cudaStream_t st = (cudaStream_t)stream;

@@ -30,7 +30,7 @@ struct KpShape {
   static constexpr int NB = (D + 63) / 64, SLICE = kv4_slice_bytes(D, NG);
   static constexpr int Q = 2 * NB * KP_QBOX, K = NB * KP_KBOX, V = D * 128;
   static constexpr int RING = KP_DEQUANT * KP_RING * SLICE;
-  static constexpr int SMEM = 1024 + Q + KP_STAGES * (K + V) + RING + 512 + 4 * KP_ROWS * 4 + KP_EXPS * 4 * 2;
+  static constexpr int SMEM = 1024 + Q + KP_STAGES * (K + V) + RING + 512 + 6 * KP_ROWS * 4 + KP_EXPS * 4 * 2;
 };
 
 __device__ __forceinline__ bool kp_wait(uint64_t* bar, uint32_t parity, volatile int* fail, int* word, int code) {
@@ -101,21 +101,46 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
   int* s_fail = reinterpret_cast<int*>(tmem_ptr + 1);
   int* s_none = s_fail + 1;                           // [4] per group the first position whose value is no number
   float* s_x = reinterpret_cast<float*>(ring + Shape::RING + 512);      // [tile][half][row]: what the two threads of a row tell one another
-  signed char* s_ek = reinterpret_cast<signed char*>(s_x + 4 * KP_ROWS);      // [page & 7][slice] exponents of keys and values
+  float* s_mul = s_x + 4 * KP_ROWS;                   // [2 tiles][row] what a row's raw scores are multiplied by
+  signed char* s_ek = reinterpret_cast<signed char*>(s_mul + 2 * KP_ROWS);      // [page & 7][slice] exponents of keys and values
   signed char* s_ev = s_ek + KP_EXPS * 4;
 
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   // what every role walks: pages page0 .. page1; per tile the last page that one of its rows sees
-  const int last = it.pos0 + (col0 + cols - 1) / R, page0 = it.page0;
+  const int last = it.pos0 + column_token(col0 + cols - 1, R), page0 = it.page0;
   const int hi1 = cols > KP_ROWS ? min(it.page1, last / KV4_PAGE + 1) - 1 : -1;
-  const int hi0 = min(it.page1, (it.pos0 + (col0 + min(cols, KP_ROWS) - 1) / R) / KV4_PAGE + 1) - 1;
+  const int hi0 = min(it.page1, (it.pos0 + column_token(col0 + min(cols, KP_ROWS) - 1, R)) / KV4_PAGE + 1) - 1;
   const int page_last = max(hi0, hi1);
 
+  const int units = page_last - page0 + 1;
+  // codes into operands: the first copies are on their way before the block meets
+  const int sl = warp - KP_SOFTMAX - 2;
+  const int32_t* table = a.table + (size_t)it.row * a.width + page0;
+  const uint8_t* from = a.blocks + (size_t)head * BYTES + sl * SLICE;
+  const size_t page_bytes = (size_t)a.G * BYTES;
+  uint8_t* mine = ring + sl * KP_RING * SLICE;
+  uint64_t* full = r_full + sl * KP_RING;
+  int entry = 0;
+  if (sl >= 0) {
+    entry = lane < units ? table[lane] : 0;
+    if (lane == 0) {
+      for (int i = 0; i < KP_RING; ++i) mbar_init(&full[i], 1);
+      fence_barrier_init();
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < KP_RING; ++i) {
+      const int page = __shfl_sync(0xffffffffu, entry, i);
+      if (lane == 0 && i < units) {
+        mbar_expect_tx(&full[i], SLICE);
+        bulk_load_1d(mine + i * SLICE, from + min(max(page, 0), a.pages - 1) * page_bytes, SLICE, &full[i]);
+      }
+    }
+  }
   if (threadIdx.x == 0) {
     mbar_init(q_full, KP_SOFTMAX);
     for (int i = 0; i < KP_STAGES; ++i) mbar_init(&k_full[i], KP_DEQUANT), mbar_init(&k_empty[i], 2), mbar_init(&v_full[i], KP_DEQUANT), mbar_init(&v_empty[i], 2);
     for (int i = 0; i < 4; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], KP_SOFTMAX / 2), mbar_init(&o_full[i], 1), s_none[i] = INT_MAX;
-    for (int i = 0; i < KP_DEQUANT * KP_RING; ++i) mbar_init(&r_full[i], 1);
     *s_fail = 0;
     fence_barrier_init();
   }
@@ -127,22 +152,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
 
   if (warp >= KP_SOFTMAX + 2) {
     // ===================== codes into operands =====================
-    const int sl = warp - KP_SOFTMAX - 2, t4 = lane & 3, g8 = lane >> 2;
-    const int32_t* table = a.table + (size_t)it.row * a.width + page0;
-    const uint8_t* from = a.blocks + (size_t)head * BYTES + sl * SLICE;
-    const size_t page_bytes = (size_t)a.G * BYTES;
-    const int units = page_last - page0 + 1;
-    uint8_t* mine = ring + sl * KP_RING * SLICE;
-    uint64_t* full = r_full + sl * KP_RING;
-    int entry = lane < units ? table[lane] : 0;
-#pragma unroll
-    for (int i = 0; i < KP_RING; ++i) {
-      const int page = __shfl_sync(0xffffffffu, entry, i);
-      if (lane == 0 && i < units) {
-        mbar_expect_tx(&full[i], SLICE);
-        bulk_load_1d(mine + i * SLICE, from + min(max(page, 0), a.pages - 1) * page_bytes, SLICE, &full[i]);
-      }
-    }
+    const int t4 = lane & 3, g8 = lane >> 2;
     bool ok = true;
     for (int n = 0; n < units; ++n) {
       const int st = n % KP_RING, ks = n % KP_STAGES;
@@ -256,7 +266,6 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
       const uint32_t tm_s = tmem + TM_S + 128u * i, tm_o = tmem + TM_O + 128u * i;
       const uint64_t qdesc = smem_desc_sw128(smem_u32(sq + i * NB * KP_QBOX));
       const uint64_t kdesc0 = smem_desc_sw128(smem_u32(sk)), vdesc0 = smem_desc_sw128(smem_u32(sv));
-      const int units = page_last - page0 + 1;
       auto scores = [&](int n) {
         const int ks = n % KP_STAGES;
         if (!kp_wait(&k_full[ks], (n / KP_STAGES) & 1, s_fail, a.word, 4)) return false;
@@ -304,51 +313,48 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
     const int tile = warp >> 3, half = (warp >> 2) & 1, row = (int)(threadIdx.x & (KP_ROWS - 1));
     const int c = col0 + tile * KP_ROWS + row, myhi = tile == 0 ? hi0 : hi1;
     const bool live = tile * KP_ROWS + row < cols;
-    const int qp = it.pos0 + (live ? c : col0) / R;                     // position of the row's query
-    const size_t out_row = (size_t)(it.first + (live ? c : col0) / R) * a.H + head * R + (live ? c : col0) % R;
+    const int qt = column_token(live ? c : col0, R), qp = it.pos0 + qt;                // the row's token and its position
+    const size_t out_row = (size_t)(it.first + qt) * a.H + head * R + column_head(live ? c : col0, R);
     float* const own = s_x + (tile * 2 + half) * KP_ROWS + row;
     const float* const other = s_x + (tile * 2 + (half ^ 1)) * KP_ROWS + row;
     const int bar = 1 + tile * 4 + (warp & 3);
-    float mul;                                                          // what a raw score is multiplied by, to units of log2
     {
-      constexpr int P = D / 16;                                         // 16-byte pieces of half a row
-      const T* q = (const T*)a.q + (long long)(it.first + (live ? c : col0) / R) * a.q_row + (size_t)(head * R + (live ? c : col0) % R) * D + half * (D / 2);
-      uint4 u[P];
-      float mx = 0.f;
+      // whole rows by neighbouring lanes (a row a thread took 32 lines a load, 8000 clocks of a block): 16 rows a warp
+      constexpr int LV = D / 8, RPI = 32 / LV, N = 16 / RPI;            // lanes a row, rows a load, loads
+      const int l = lane % LV;
+      uint4 u[N];
 #pragma unroll
-      for (int e = 0; e < P; ++e) {
-        u[e] = live ? reinterpret_cast<const uint4*>(q)[e] : make_uint4(0u, 0u, 0u, 0u);
-        const uint32_t w[4] = {u[e].x, u[e].y, u[e].z, u[e].w};
-#pragma unroll
-        for (int z = 0; z < 4; ++z) {
-          const float2 f = bits_pair<T>(w[z]);
-          mx = fmaxf(mx, fmaxf(fabsf(f.x), fabsf(f.y)));
-        }
+      for (int i = 0; i < N; ++i) {
+        const int r = 16 * warp + i * RPI + lane / LV, cc = col0 + r;
+        u[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (r < cols) u[i] = *reinterpret_cast<const uint4*>((const T*)a.q + (long long)(it.first + column_token(cc, R)) * a.q_row + (size_t)(head * R + column_head(cc, R)) * D + 8 * l);
       }
-      *own = mx;
-      at_any(bar, false);
-      mx = fmaxf(mx, *other);
-      at_any(bar, false);
-      const int ex = min(max((int)(__float_as_uint(mx) >> 23), 15), 240);
-      const float up = pow2(127 + 14 - ex);                             // the row's largest comes to 2^14 .. 2^15
-      mul = pow2(ex - 127 - 14) * (a.scale * AT_LOG2E);
-      uint8_t* to = sq + (tile * NB + (NB == 2 ? half : 0)) * KP_QBOX + row * 128;
 #pragma unroll
-      for (int e = 0; e < P; ++e) {
-        const uint32_t w[4] = {u[e].x, u[e].y, u[e].z, u[e].w};
+      for (int i = 0; i < N; ++i) {
+        const int r = 16 * warp + i * RPI + lane / LV;
+        const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+        uint32_t big = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+#pragma unroll
+        for (int o = LV / 2; o > 0; o >>= 1) big = __vmaxu2(big, __shfl_xor_sync(0xffffffffu, big, o));
+        const float2 m2 = bits_pair<T>(big);
+        const int ex = min(max((int)(__float_as_uint(fmaxf(m2.x, m2.y)) >> 23), 15), 240);
+        const float up = pow2(127 + 14 - ex);                           // the row's largest comes to 2^14 .. 2^15
+        if (l == 0) s_mul[r] = pow2(ex - 127 - 14) * (a.scale * AT_LOG2E);
         uint32_t h[4];
 #pragma unroll
         for (int z = 0; z < 4; ++z) {
           const float2 f = bits_pair<T>(w[z]);
           h[z] = pair_bits<__half>(f.x * up, f.y * up);
         }
-        const int piece = (NB == 2 ? 0 : half * P) + e;
-        *reinterpret_cast<uint4*>(to + ((piece ^ (row & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+        const int tr = r & (KP_ROWS - 1);
+        *reinterpret_cast<uint4*>(sq + ((r >> 7) * NB + (l >> 3)) * KP_QBOX + tr * 128 + (((l & 7) ^ (tr & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
       }
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full);
+      asm volatile("barrier.cta.sync 9, 512;" ::: "memory");
     }
+    const float mul = s_mul[tile * KP_ROWS + row];                      // what a raw score is multiplied by, to units of log2
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t ts0 = tmem + lanes + TM_S + 128u * tile, to = tmem + lanes + TM_O + 128u * tile;
     float ref = -INFINITY, sum = 0.f;
@@ -419,26 +425,30 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
       }
       const float sub = ref == -INFINITY ? 0.f : -ref;
       uint32_t ph[16];
+      f2 part[2] = {f2_of(0.f, 0.f), f2_of(0.f, 0.f)};
+      if ((eks | evs) == 0u && ebase == 0) {                            // (as mostly)
+        const f2 m2 = f2_of(mul, mul), s2 = f2_of(sub, sub);
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {                                     // the two slices
-        const float mm = x ? mul1 : mul0;
-        const f2 m2 = f2_of(mm, mm), s2 = f2_of(sub, sub);
-        const int down = (x ? ev1 : ev0) - ebase;                         // (0 or less, the same for the warp)
-        const float f = pow2(max(down, -126));
-        f2 part[2] = {f2_of(0.f, 0.f), f2_of(0.f, 0.f)};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
+        for (int e = 0; e < 16; ++e) {
           float a0, a1;
-          f2_split(f2_fma(f2_of(__uint_as_float(sr[16 * x + 2 * e]), __uint_as_float(sr[16 * x + 2 * e + 1])), m2, s2), a0, a1);
-          float p0 = at_exp2(a0), p1 = at_exp2(a1);
+          f2_split(f2_fma(f2_of(__uint_as_float(sr[2 * e]), __uint_as_float(sr[2 * e + 1])), m2, s2), a0, a1);
+          const float p0 = at_exp2(a0), p1 = at_exp2(a1);
           part[e & 1] = f2_add(part[e & 1], f2_of(p0, p1));
-          if (down != 0) p0 *= f, p1 *= f;
-          ph[8 * x + e] = pair_bits<__half>(p0, p1);
+          ph[e] = pair_bits<__half>(p0, p1);
         }
-        float p0, p1;
-        f2_split(f2_add(part[0], part[1]), p0, p1);
-        sum += p0 + p1;
+      } else {
+        const float f0 = pow2(max(ev0 - ebase, -126)), f1 = pow2(max(ev1 - ebase, -126));
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float mm = e < 8 ? mul0 : mul1, f = e < 8 ? f0 : f1;
+          const float p0 = at_exp2(fmaf(__uint_as_float(sr[2 * e]), mm, sub)), p1 = at_exp2(fmaf(__uint_as_float(sr[2 * e + 1]), mm, sub));
+          part[e & 1] = f2_add(part[e & 1], f2_of(p0, p1));
+          ph[e] = pair_bits<__half>(p0 * f, p1 * f);
+        }
       }
+      float p0, p1;
+      f2_split(f2_add(part[0], part[1]), p0, p1);
+      sum += p0 + p1;
       // the weights go over the thread's own scores
       tmem_st16(ts + 32u * half, ph);
       tmem_wait_st();
@@ -455,7 +465,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
       const size_t part_at = ((size_t)(it.base + it.part) * a.G + head) * KV4_MANY + tile * KP_ROWS + row;
       const bool whole = it.parts == 1;
       if (!whole && live && half == 0)
-        *reinterpret_cast<float2*>(a.part + (size_t)a.max_items * a.G * KV4_MANY * D + part_at * 2) = make_float2(ref == -INFINITY ? KV4_NONE : ref, den);
+        *reinterpret_cast<float2*>(a.part + (size_t)a.kept * a.G * KV4_MANY * D + part_at * 2) = make_float2(ref == -INFINITY ? KV4_NONE : ref, den);
       const float fin = pow2(max(min(ebase, 126), -126)) / (whole ? den : 1.f);
       if (count > 0) {
 #pragma unroll
@@ -505,7 +515,7 @@ int prompt_launch(const Kv4Attn& a, cudaStream_t st) {
     LL_CUDA(cudaFuncSetAttribute(kv4_prompt_kernel<T, D, NG>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     set.mark();
   }
-  kv4_prompt_kernel<T, D, NG><<<(unsigned)(a.max_items * a.G), KP_THREADS, smem, st>>>(a);
+  kv4_prompt_kernel<T, D, NG><<<(unsigned)(a.items * a.G), KP_THREADS, smem, st>>>(a);
   LL_LAUNCH_OK("kv4_prompt_kernel");
   return LL_OK;
 }

@@ -13,8 +13,8 @@ struct Kv4Attn {
   const uint8_t* blocks;
   const int32_t *table, *work;
   void* y;
-  float* part;         // [items][G][columns] of D sums, then [items][G][columns] of (reference, sum of weights)
-  int H, G, width, pages, max_items;
+  float* part;         // [kept][G][columns] of D sums, then [kept][G][columns] of (reference, sum of weights)
+  int H, G, width, pages, items, kept;      // items a grid has, parts whose sums there is room for
   float scale;
   int* word;           // wait_word()
 };
@@ -39,10 +39,16 @@ __device__ __forceinline__ Kv4Item load_item(const int32_t* work, int i) {
   return it;
 }
 
+// column -> token and head, without a division where a key head serves one head
+__device__ __forceinline__ int column_token(int c, int R) { return R == 1 ? c : c / R; }
+__device__ __forceinline__ int column_head(int c, int R) { return R == 1 ? 0 : c % R; }
+
 constexpr float KV4_NONE = -1e37f;      // the reference of a column that has seen no key
 
 // Sequences that bring up to this many columns a key head go to the kernel of few columns, others to the tcgen05 kernel in tiles of KV4_MANY.
 constexpr int KV4_FEW_MOST = 32, KV4_MANY = 256, KV4_WHOLE = 8;
+// Walks for KV4_ROUNDS rounds of blocks stay whole; fewer are cut into at most KV4_CUTS rounds more of parts.
+constexpr int KV4_ROUNDS = 3, KV4_CUTS = 2;
 
 inline bool kv4_many(int max_count, int R) { return (long long)max_count * R > KV4_FEW_MOST; }
 inline int kv4_sms() { return sm_count() > 0 ? sm_count() : 148; }
@@ -50,7 +56,6 @@ inline int kv4_sms() { return sm_count() > 0 ? sm_count() : 148; }
 // A step's two lists: sequences of few columns and, where one may bring more, of many.  Sizes as the host knows them.
 struct Kv4Lists {
   int R, cols, few, few_parts, many_parts;
-  int least;                            // pages of a part of the few, at least
   long long few_items, many_items;      // at most
   bool many, few_cut;
   Kv4Lists(int B, int T, int max_count, int H, int G, int max_length) {
@@ -62,16 +67,18 @@ struct Kv4Lists {
     few_parts = std::max(1, 4 * kv4_sms() / G);
     many_parts = std::max(1, kv4_sms() / G);
     // Where no request has more than KV4_WHOLE pages, walks are not cut, and there is nothing to join.
-    least = max_length <= KV4_WHOLE * KV4_PAGE ? KV4_WHOLE : 1;
-    few_cut = least == 1;
+    few_cut = max_length > KV4_WHOLE * KV4_PAGE;
     const long long each = many ? (KV4_FEW_MOST + cols - 1) / cols : T, seqs = std::min(B, std::max(T, 1));
-    few_items = std::min((long long)T * R / cols + seqs, seqs * each) + few_parts;
-    many_items = many ? (long long)T * R / KV4_MANY + std::min(seqs, (long long)T * R / KV4_FEW_MOST) + many_parts : 0;
+    few_items = std::min((long long)T * R / cols + seqs, seqs * each) + KV4_CUTS * few_parts;
+    many_items = many ? (long long)T * R / KV4_MANY + std::min(seqs, (long long)T * R / KV4_FEW_MOST) + KV4_CUTS * many_parts : 0;
   }
   size_t few_ints() const { return 4 + sizeof(Kv4Item) / 4 * (size_t)few_items; }
   size_t ints() const { return few_ints() + (many ? 4 + sizeof(Kv4Item) / 4 * (size_t)many_items : 0); }
-  size_t few_floats(int G, int D) const { return ((size_t)few_items * G * cols * (D + 2) + 3) / 4 * 4; }
-  size_t floats(int G, int D) const { return few_floats(G, D) + (size_t)many_items * G * KV4_MANY * (D + 2); }
+  // sums are kept of parts that have to be joined, and none are where there are walks for KV4_ROUNDS rounds
+  int few_kept() const { return (int)std::min(few_items, (long long)(KV4_ROUNDS + KV4_CUTS) * few_parts); }
+  int many_kept() const { return (int)std::min(many_items, (long long)(KV4_ROUNDS + KV4_CUTS) * many_parts); }
+  size_t few_floats(int G, int D) const { return ((size_t)few_kept() * G * cols * (D + 2) + 3) / 4 * 4; }
+  size_t floats(int G, int D) const { return few_floats(G, D) + (size_t)many_kept() * G * KV4_MANY * (D + 2); }
 };
 
 }  // namespace
