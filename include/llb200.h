@@ -46,7 +46,7 @@ typedef void* ll_stream; /* cudaStream_t */
 LL_API const char* ll_last_error(void);
 /* The waits inside the tcgen05 kernels and the chunked delta rule are bounded; a kernel whose wait runs out skips its stores and leaves a
  * code in host memory (100 + prompt attention's, 200 + int4 rows', 300 + llm.int8's, 400 + grouped experts', 500 + delta rule's,
- * 600 + dense products', 700 + paged attention's).
+ * 600 + dense products', 800 + paged attention's).
  * The next launch through this library fails with LL_ERR_WAIT, or this call does, which looks without launching: after a synchronisation
  * it speaks for everything before it.  Either clears the code.  ll_wait_report leaves a code as a kernel does. */
 LL_API int ll_wait_check(void);

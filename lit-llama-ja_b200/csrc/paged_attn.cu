@@ -42,7 +42,7 @@ __device__ __forceinline__ bool kf_wait(uint64_t* bar, uint32_t parity, int* wor
   if (mbar_try_wait(bar, parity)) return true;
   for (uint32_t i = 0; i < KF_WAIT_LIMIT; ++i)
     if (mbar_try_wait(bar, parity)) return true;
-  wait_ran_out(word, 701);
+  wait_ran_out(word, 801);
   return false;
 }
 

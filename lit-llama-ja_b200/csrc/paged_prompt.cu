@@ -2,8 +2,9 @@
 //
 // A block owns two tiles of 128 columns (queries of the heads that share a key head) of one request and walks a range of its pages of 64 keys:
 //   warps 0-7, 8-15 : softmax of tile 0 / tile 1, two threads a row with 32 of its 64 scores each; before, they bring the queries as fp16
-//   warps 16, 17    : one thread each issues the MMAs of a tile: the scores of the next page first, then P V of this one
-//   warps 18-21     : a slice of 16 keys each: codes by bulk copies into a ring, from there as fp16 numbers into the operands
+//   warps 16, 17    : one thread each issues the MMAs of a tile: the scores of the next page first, then P V of this one (18, 19: nothing)
+//   warps 20-27     : two sets that take the pages in turn, a warp a slice of 16 keys: codes by bulk copies into a ring, from there as fp16 numbers into
+//                     the operands.  (A page takes a warp 2600 clocks, the softmax less: with one set it is what a page takes.)
 // All operands are fp16, whatever the cache's type: its 11 bits hold a query exactly (a row under a power of two of its own) and a key or value
 // c s + lo rounded once, where bf16 would lose three bits more.  Slices are brought into range by powers of two 2^e, e a multiple of 16 (so that
 // e is the same, mostly 0, for all of them): scores are multiplied back by 2^e; weights by 2^(e - E), E the largest so far, to which O is rescaled.
@@ -21,9 +22,13 @@
 namespace llb {
 namespace {
 
-constexpr int KP_ROWS = 128, KP_SOFTMAX = 16, KP_DEQUANT = 4, KP_THREADS = (KP_SOFTMAX + 2 + KP_DEQUANT) * 32;
+// Warps: softmax, MMA issuers (two of four), two sets of four that bring codes into operands, a page each in turn.
+constexpr int KP_ROWS = 128, KP_SOFTMAX = 16, KP_FIRST = KP_SOFTMAX + 4, KP_SETS = 2, KP_DEQUANT = 4 * KP_SETS, KP_THREADS = (KP_FIRST + KP_DEQUANT) * 32;
+// registers a thread: 72 at the launch; the softmax takes what the others leave
+constexpr int KP_REGS = 72, KP_REGS_SOFTMAX = 88, KP_REGS_MMA = 40, KP_REGS_DEQUANT = 56;
+static_assert(KP_THREADS * KP_REGS <= 65536 && KP_SOFTMAX * KP_REGS_SOFTMAX + 4 * KP_REGS_MMA + KP_DEQUANT * KP_REGS_DEQUANT <= KP_THREADS / 32 * KP_REGS, "registers");
 constexpr int KP_QBOX = KP_ROWS * 128, KP_KBOX = KV4_PAGE * 128;      // 64 numbers of 16 bits a row
-constexpr int KP_RING = 3, KP_STAGES = 3, KP_EXPS = 8;               // copies in flight a slice; pages of K and of V; pages whose exponents are kept
+constexpr int KP_RING = 2, KP_STAGES = 3, KP_EXPS = 8;               // copies in flight a slice of a set; pages of K and of V; pages whose exponents are kept
 
 template <int D, int NG>
 struct KpShape {
@@ -40,7 +45,7 @@ __device__ __forceinline__ bool kp_wait(uint64_t* bar, uint32_t parity, volatile
     if ((i & 255u) == 255u && *fail) return false;
   }
   *fail = 1;
-  wait_ran_out(word, 710 + code);
+  wait_ran_out(word, 810 + code);
   return false;
 }
 
@@ -114,15 +119,16 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
 
   const int units = page_last - page0 + 1;
   // codes into operands: the first copies are on their way before the block meets
-  const int sl = warp - KP_SOFTMAX - 2;
-  const int32_t* table = a.table + (size_t)it.row * a.width + page0;
+  const int dq = warp - KP_FIRST, sl = dq & 3, set = dq >> 2;         // (the slice and the set of a warp of theirs)
+  const int turns = (units - set + KP_SETS - 1) / KP_SETS;             // pages set, set + KP_SETS ..
+  const int32_t* table = a.table + (size_t)it.row * a.width + page0 + set;
   const uint8_t* from = a.blocks + (size_t)head * BYTES + sl * SLICE;
   const size_t page_bytes = (size_t)a.G * BYTES;
-  uint8_t* mine = ring + sl * KP_RING * SLICE;
-  uint64_t* full = r_full + sl * KP_RING;
+  uint8_t* mine = ring + dq * KP_RING * SLICE;
+  uint64_t* full = r_full + dq * KP_RING;
   int entry = 0;
-  if (sl >= 0) {
-    entry = lane < units ? table[lane] : 0;
+  if (dq >= 0) {
+    entry = lane < turns ? table[KP_SETS * lane] : 0;
     if (lane == 0) {
       for (int i = 0; i < KP_RING; ++i) mbar_init(&full[i], 1);
       fence_barrier_init();
@@ -131,7 +137,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
 #pragma unroll
     for (int i = 0; i < KP_RING; ++i) {
       const int page = __shfl_sync(0xffffffffu, entry, i);
-      if (lane == 0 && i < units) {
+      if (lane == 0 && i < turns) {
         mbar_expect_tx(&full[i], SLICE);
         bulk_load_1d(mine + i * SLICE, from + min(max(page, 0), a.pages - 1) * page_bytes, SLICE, &full[i]);
       }
@@ -139,7 +145,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
   }
   if (threadIdx.x == 0) {
     mbar_init(q_full, KP_SOFTMAX);
-    for (int i = 0; i < KP_STAGES; ++i) mbar_init(&k_full[i], KP_DEQUANT), mbar_init(&k_empty[i], 2), mbar_init(&v_full[i], KP_DEQUANT), mbar_init(&v_empty[i], 2);
+    for (int i = 0; i < KP_STAGES; ++i) mbar_init(&k_full[i], 4), mbar_init(&k_empty[i], 2), mbar_init(&v_full[i], 4), mbar_init(&v_empty[i], 2);
     for (int i = 0; i < 4; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], KP_SOFTMAX / 2), mbar_init(&o_full[i], 1), s_none[i] = INT_MAX;
     *s_fail = 0;
     fence_barrier_init();
@@ -150,13 +156,14 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_ptr, 0);
 
-  if (warp >= KP_SOFTMAX + 2) {
+  if (warp >= KP_FIRST) {
     // ===================== codes into operands =====================
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(KP_REGS_DEQUANT));
     const int t4 = lane & 3, g8 = lane >> 2;
     bool ok = true;
-    for (int n = 0; n < units; ++n) {
-      const int st = n % KP_RING, ks = n % KP_STAGES;
-      ok = __all_sync(0xffffffffu, kp_wait(&full[st], (n / KP_RING) & 1, s_fail, a.word, 1));
+    for (int turn = 0; turn < turns; ++turn) {
+      const int n = KP_SETS * turn + set, st = turn % KP_RING, ks = n % KP_STAGES;
+      ok = __all_sync(0xffffffffu, kp_wait(&full[st], (turn / KP_RING) & 1, s_fail, a.word, 1));
       if (!ok) break;
       const uint8_t* blk = mine + st * SLICE;
       uint32_t kw[2][W], vw[2][W];
@@ -207,11 +214,11 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
             }
           }
       }
-      const int nxt = n + KP_RING;
-      if ((nxt & 31) == 0) entry = nxt + lane < units ? table[nxt + lane] : 0;
+      const int nxt = turn + KP_RING;
+      if ((nxt & 31) == 0) entry = nxt + lane < turns ? table[KP_SETS * (nxt + lane)] : 0;
       const int page = __shfl_sync(0xffffffffu, entry, nxt & 31);
       __syncwarp();                                   // every lane has read the slice
-      if (lane == 0 && nxt < units) {
+      if (lane == 0 && nxt < turns) {
         mbar_expect_tx(&full[st], SLICE);
         bulk_load_1d(mine + st * SLICE, from + min(max(page, 0), a.pages - 1) * page_bytes, SLICE, &full[st]);
       }
@@ -260,7 +267,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
     __syncwarp();
   } else if (warp >= KP_SOFTMAX) {
     // ===================== MMA issuers, one thread per tile =====================
-    if (elect_one()) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(KP_REGS_MMA));
+    if (warp < KP_SOFTMAX + 2 && elect_one()) {
       constexpr uint32_t idesc_s = instr_desc_f16(KP_ROWS, KV4_PAGE), idesc_o = instr_desc_f16(KP_ROWS, D);
       const int i = warp - KP_SOFTMAX, myhi = i == 0 ? hi0 : hi1;
       const uint32_t tm_s = tmem + TM_S + 128u * i, tm_o = tmem + TM_O + 128u * i;
@@ -310,6 +318,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
     __syncwarp();
   } else {
     // ===================== queries, softmax, then the epilogue =====================
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(KP_REGS_SOFTMAX));
     const int tile = warp >> 3, half = (warp >> 2) & 1, row = (int)(threadIdx.x & (KP_ROWS - 1));
     const int c = col0 + tile * KP_ROWS + row, myhi = tile == 0 ? hi0 : hi1;
     const bool live = tile * KP_ROWS + row < cols;
@@ -329,24 +338,41 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
         u[i] = make_uint4(0u, 0u, 0u, 0u);
         if (r < cols) u[i] = *reinterpret_cast<const uint4*>((const T*)a.q + (long long)(it.first + column_token(cc, R)) * a.q_row + (size_t)(head * R + column_head(cc, R)) * D + 8 * l);
       }
+      // rows as they stand, where every piece of eight numbers has one of 2^-4 .. 2^14, or only zeros: small ones lose 2^-25 then; else under a
+      // power of two a row, its largest comes to 2^14 .. 2^15
+      constexpr uint32_t SMALL = std::is_same<T, __half>::value ? 0x2c00u : 0x3d80u, LARGE = std::is_same<T, __half>::value ? 0x7400u : 0x4680u;
+      uint32_t bigs[N];
+      bool odd = false;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const int r = 16 * warp + i * RPI + lane / LV;
-        const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
-        uint32_t big = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+        const uint32_t m = __vmaxu2(__vmaxu2(u[i].x & 0x7fff7fffu, u[i].y & 0x7fff7fffu), __vmaxu2(u[i].z & 0x7fff7fffu, u[i].w & 0x7fff7fffu));
+        bigs[i] = max(m & 0xffffu, m >> 16);
+        odd |= bigs[i] != 0u && (bigs[i] < SMALL || bigs[i] >= LARGE);
+      }
+      odd = __any_sync(0xffffffffu, odd);
 #pragma unroll
-        for (int o = LV / 2; o > 0; o >>= 1) big = __vmaxu2(big, __shfl_xor_sync(0xffffffffu, big, o));
-        const float2 m2 = bits_pair<T>(big);
-        const int ex = min(max((int)(__float_as_uint(fmaxf(m2.x, m2.y)) >> 23), 15), 240);
-        const float up = pow2(127 + 14 - ex);                           // the row's largest comes to 2^14 .. 2^15
-        if (l == 0) s_mul[r] = pow2(ex - 127 - 14) * (a.scale * AT_LOG2E);
+      for (int i = 0; i < N; ++i) {
+        const int r = 16 * warp + i * RPI + lane / LV, tr = r & (KP_ROWS - 1);
+        const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+        float up = 1.f, down = 1.f;
+        if (odd) {
+          uint32_t big = bigs[i];
+#pragma unroll
+          for (int o = LV / 2; o > 0; o >>= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
+          const int ex = min(max((int)(__float_as_uint(bits_pair<T>(big).x) >> 23), 15), 240);
+          up = pow2(127 + 14 - ex), down = pow2(ex - 127 - 14);
+        }
+        if (l == 0) s_mul[r] = down * (a.scale * AT_LOG2E);
         uint32_t h[4];
 #pragma unroll
         for (int z = 0; z < 4; ++z) {
-          const float2 f = bits_pair<T>(w[z]);
-          h[z] = pair_bits<__half>(f.x * up, f.y * up);
+          if (std::is_same<T, __half>::value && !odd) {
+            h[z] = w[z];
+          } else {
+            const float2 f = bits_pair<T>(w[z]);
+            h[z] = odd ? pair_bits<__half>(f.x * up, f.y * up) : pair_bits<__half>(f.x, f.y);
+          }
         }
-        const int tr = r & (KP_ROWS - 1);
         *reinterpret_cast<uint4*>(sq + ((r >> 7) * NB + (l >> 3)) * KP_QBOX + tr * 128 + (((l & 7) ^ (tr & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
       }
       fence_proxy_async();

@@ -39,9 +39,9 @@ __device__ __forceinline__ Kv4Item load_item(const int32_t* work, int i) {
   return it;
 }
 
-// column -> token and head, without a division where a key head serves one head
-__device__ __forceinline__ int column_token(int c, int R) { return R == 1 ? c : c / R; }
-__device__ __forceinline__ int column_head(int c, int R) { return R == 1 ? 0 : c % R; }
+// column -> token and head: a shift where the heads of a key head are 1, 2, 4 .., else a division
+__device__ __forceinline__ int column_token(int c, int R) { return (R & (R - 1)) == 0 ? c >> (31 - __clz(R)) : c / R; }
+__device__ __forceinline__ int column_head(int c, int R) { return (R & (R - 1)) == 0 ? c & (R - 1) : c % R; }
 
 constexpr float KV4_NONE = -1e37f;      // the reference of a column that has seen no key
 
