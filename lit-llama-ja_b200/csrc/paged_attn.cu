@@ -4,6 +4,7 @@
 // With K = s c + lo and V alike, by groups of a head's dimensions (c: codes),
 //   q.k_j = sum_g s_jg (q.c_j)_g + lo_jg (sum of q)_g           y = sum_j p_j v_j = sum_j (p_j s_jg) c_j + sum_j p_j lo_jg
 // so that the products run over codes, which a mask turns into numbers of fp16 (subnormal ones, exactly), and scales meet 16 keys at a time.
+#include <algorithm>
 #include <climits>
 #include <type_traits>
 
@@ -60,6 +61,9 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
   __shared__ uint64_t s_full[KF_WARPS][STAGES];
   __shared__ int s_fail;
   __shared__ float s_ref[KF_WARPS][COLS], s_sum[KF_WARPS][COLS];
+  // (launched when the last blocks of the prompts' kernel of the same call run: what is read here was there before that one.  The last block ends after
+  // it, so that what waits for this kernel waits for both.)
+  if (blockIdx.x == gridDim.x - 1) pdl_wait();
   const int item = blockIdx.x / a.G, head = blockIdx.x - item * a.G;
   if (item >= a.work[0]) return;
   const Kv4Item it = load_item(a.work, item);
@@ -424,87 +428,83 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
   }
 }
 
-// Joins the parts of a request's walk: a block a column, a warp every KJ-th part.
+// Joins the parts of walks.  Of the few columns a block has one at a time, a warp every KJ-th part (a long walk is in hundreds of parts); of the
+// tcgen05 kernel's tiles a warp has one (these are in a few).
 constexpr int KJ = 8;
-template <typename T, int D, int COLS>
-__global__ void __launch_bounds__(KJ * 32) kv4_join_kernel(const Kv4Attn a) {
-  constexpr int E = D / 32;
-  __shared__ float s_m[KJ], s_l[KJ], s_o[KJ][D];
-  pdl_wait();
-  const int item = blockIdx.x / a.G, head = blockIdx.x - item * a.G, c = blockIdx.y;
-  const int32_t* work = after_wait(a.work);
-  if (item >= work[0]) return;
-  const Kv4Item it = load_item(work, item);
-  const int R = a.H / a.G, first = it.first, col = it.tile * COLS + c;
-  if (it.part != 0 || it.parts == 1 || it.row < 0 || col >= it.count * R) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const float* part = after_wait(a.part);
-  const float2* ml = reinterpret_cast<const float2*>(part + (size_t)a.kept * a.G * COLS * D);
-  float m = KV4_NONE, l = 0.f, o[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) o[e] = 0.f;
-#pragma unroll 4
-  for (int k = warp; k < it.parts; k += KJ) {
-    const size_t at = ((size_t)(it.base + k) * a.G + head) * COLS + c;
-    const float2 u = ml[at];
-    if (u.y == 0.f) continue;                  // (a part that holds no key of the column's)
+template <int D>
+struct KjSum {
+  float m = KV4_NONE, l = 0.f, o[D / 32] = {};
+  __device__ __forceinline__ void add(float2 u, const float* part, int lane) {      // u: reference and sum of weights
+    if (u.y == 0.f) return;                    // (a part that holds no key of the column's)
     const float mn = fmaxf(m, u.x), f = kf_exp2(m - mn), w = kf_exp2(u.x - mn);
     m = mn;
     l = fmaf(l, f, u.y * w);
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = fmaf(o[e], f, part[at * D + lane * E + e] * w);
+    for (int e = 0; e < D / 32; ++e) o[e] = fmaf(o[e], f, part[lane + 32 * e] * w);
   }
-  if (lane == 0) s_m[warp] = m, s_l[warp] = l;
-#pragma unroll
-  for (int e = 0; e < E; ++e) s_o[warp][lane * E + e] = o[e];
-  __syncthreads();
-  const int d = threadIdx.x;
-  if (d >= D) return;
-  float mm = s_m[0], num = 0.f, den = 0.f;
-#pragma unroll
-  for (int w = 1; w < KJ; ++w) mm = fmaxf(mm, s_m[w]);
-#pragma unroll
-  for (int w = 0; w < KJ; ++w) {
-    const float f = kf_exp2(s_m[w] - mm);
-    num = fmaf(s_o[w][d], f, num);
-    den = fmaf(s_l[w], f, den);
-  }
-  dt<T>::st((T*)a.y, ((size_t)(first + col / R) * a.H + head * R + col % R) * D + d, num / den);
-}
-
-// The same for the tcgen05 kernel's tiles: a warp a column, a block every KJ-th of 32.
-template <typename T, int D>
-__global__ void __launch_bounds__(KJ * 32) kv4_join_many_kernel(const Kv4Attn a) {
-  constexpr int E = D / 32;
+};
+template <typename T, int D, int COLS>
+__global__ void __launch_bounds__(KJ * 32) kv4_join_kernel(const Kv4Attn few, const Kv4Attn many) {
+  __shared__ float s_m[KJ], s_l[KJ], s_o[KJ][D];
   pdl_wait();
-  const int item = blockIdx.x / a.G, head = blockIdx.x - item * a.G;
-  const int32_t* work = after_wait(a.work);
-  if (item >= work[0]) return;
-  const Kv4Item it = load_item(work, item);
-  if (it.part != 0 || it.parts == 1 || it.row < 0) return;
-  const int R = a.H / a.G, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const float* part = after_wait(a.part);
-  const float2* ml = reinterpret_cast<const float2*>(part + (size_t)a.kept * a.G * KV4_MANY * D);
-  for (int c = 32 * blockIdx.y + warp; c < 32 * (blockIdx.y + 1); c += KJ) {
-    const int col = it.tile * KV4_MANY + c;
-    if (col >= it.count * R) return;
-    float m = KV4_NONE, l = 0.f, o[E];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = few.G, R = few.H / few.G;
+  T* const y = (T*)few.y;
+  if (few.items > 0) {
+    const int32_t* work = after_wait(few.work);
+    const float* part = after_wait(few.part);
+    const float2* ml = reinterpret_cast<const float2*>(part + (size_t)few.kept * G * COLS * D);
+    const int units = work[1] * G * few.cols;
+    for (int u = blockIdx.x; u < units; u += gridDim.x) {
+      const int j = u / (G * few.cols), head = u / few.cols % G, c = u % few.cols;
+      const int4 a = joins_of(work, few.items)[2 * j], b = joins_of(work, few.items)[2 * j + 1];
+      const int first = a.x, col = a.z * COLS + c, parts = a.w;
+      if (col >= a.y * R) continue;
+      KjSum<D> s;
+#pragma unroll 4
+      for (int k = warp; k < parts; k += KJ) {
+        const size_t at = ((size_t)(b.x + k) * G + head) * COLS + c;
+        s.add(ml[at], part + at * D, lane);
+      }
+      __syncthreads();                         // (the unit before this one has been read)
+      if (lane == 0) s_m[warp] = s.m, s_l[warp] = s.l;
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = 0.f;
-#pragma unroll 2
-    for (int k = 0; k < it.parts; ++k) {
-      const size_t at = ((size_t)(it.base + k) * a.G + head) * KV4_MANY + c;
-      const float2 u = ml[at];
-      if (u.y == 0.f) continue;                // (a part that holds no key of the column's)
-      const float mn = fmaxf(m, u.x), f = kf_exp2(m - mn), w = kf_exp2(u.x - mn);
-      m = mn;
-      l = fmaf(l, f, u.y * w);
+      for (int e = 0; e < D / 32; ++e) s_o[warp][lane + 32 * e] = s.o[e];
+      __syncthreads();
+      const int d = threadIdx.x;
+      if (d < D) {
+        float m = s_m[0], num = 0.f, den = 0.f;
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = fmaf(o[e], f, part[at * D + lane + 32 * e] * w);
+        for (int w = 1; w < KJ; ++w) m = fmaxf(m, s_m[w]);
+#pragma unroll
+        for (int w = 0; w < KJ; ++w) {
+          const float f = kf_exp2(s_m[w] - m);
+          num = fmaf(s_o[w][d], f, num);
+          den = fmaf(s_l[w], f, den);
+        }
+        dt<T>::st(y, ((size_t)(first + column_token(col, R)) * few.H + head * R + column_head(col, R)) * D + d, num / den);
+      }
     }
+  }
+  if (many.items > 0) {
+    const int32_t* work = after_wait(many.work);
+    const float* part = after_wait(many.part);
+    const float2* ml = reinterpret_cast<const float2*>(part + (size_t)many.kept * G * KV4_MANY * D);
+    const int units = work[1] * G * (KV4_MANY / KJ);
+    for (int u = blockIdx.x; u < units; u += gridDim.x) {
+      const int j = u / (G * (KV4_MANY / KJ)), head = u / (KV4_MANY / KJ) % G, c = u % (KV4_MANY / KJ) * KJ + warp;
+      const int4 a = joins_of(work, many.items)[2 * j], b = joins_of(work, many.items)[2 * j + 1];
+      const int first = a.x, col = a.z * KV4_MANY + c, parts = a.w;
+      if (col >= a.y * R) continue;
+      KjSum<D> s;
+#pragma unroll 2
+      for (int k = 0; k < parts; ++k) {
+        const size_t at = ((size_t)(b.x + k) * G + head) * KV4_MANY + c;
+        s.add(ml[at], part + at * D, lane);
+      }
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-      dt<T>::st((T*)a.y, ((size_t)(it.first + col / R) * a.H + head * R + col % R) * D + lane + 32 * e, o[e] / l);
+      for (int e = 0; e < D / 32; ++e)
+        dt<T>::st(y, ((size_t)(first + column_token(col, R)) * few.H + head * R + column_head(col, R)) * D + lane + 32 * e, s.o[e] / s.l);
+    }
   }
 }
 
@@ -533,27 +533,22 @@ int ll_kv4_attn(const ll_kv4_cache* cache, const void* blocks, const void* q, lo
                "kv4_attn: rows have to start on 16-byte boundaries");
   const Kv4Lists l(B, T, max_count, H, G, cache->max_length);
   LL_CHECK_ARG(l.few_items * G <= INT_MAX && l.many_items * G <= INT_MAX, "kv4_attn: %d sequences of %d tokens, %d heads", B, T, H);
-  const int R = l.R, cols = l.cols;
-  const long long items = l.few_items;
-  const Kv4Attn a{q, q_row, (const uint8_t*)blocks, cache->table, work, y, (float*)scratch, H, G, cache->width, cache->pages, (int)items, l.few_kept(), scale, wait_word()};
+  const int R = l.R, cols = l.cols, used = (int)std::min((long long)cols, (long long)max_count * R);
+  const Kv4Attn a{q, q_row, (const uint8_t*)blocks, cache->table, work, y, (float*)scratch, H, G, cache->width, cache->pages, (int)l.few_items, l.few_kept(), used, scale,
+                  wait_word()};
+  Kv4Attn m = a;
+  m.items = 0;
+  cudaStream_t st = (cudaStream_t)stream;
   if (l.many) {
-    Kv4Attn m = a;
     m.work = work + l.few_ints();
     m.part = (float*)scratch + l.few_floats(G, head_size);
     m.items = (int)l.many_items;
     m.kept = l.many_kept();
-    if (int r = kv4_prompt_launch(m, dtype, head_size, group, (cudaStream_t)stream)) return r;
-#define JOIN_MANY(TT, DD) LL_CUDA(launch(kv4_join_many_kernel<TT, DD>, dim3((unsigned)(l.many_items * G), KV4_MANY / 32), dim3(KJ * 32), 0, (cudaStream_t)stream, true, m));
-    if (dtype == LL_BF16 && head_size == 32) { JOIN_MANY(__nv_bfloat16, 32) }
-    else if (dtype == LL_BF16 && head_size == 64) { JOIN_MANY(__nv_bfloat16, 64) }
-    else if (dtype == LL_BF16) { JOIN_MANY(__nv_bfloat16, 128) }
-    else if (head_size == 32) { JOIN_MANY(__half, 32) }
-    else if (head_size == 64) { JOIN_MANY(__half, 64) }
-    else { JOIN_MANY(__half, 128) }
-#undef JOIN_MANY
-    LL_LAUNCH_OK("kv4_join_many_kernel");
+    if (int r = kv4_prompt_launch(m, dtype, head_size, group, st)) return r;
   }
-  cudaStream_t st = (cudaStream_t)stream;
+  // The sequences of few columns fill the end of the prompts' kernel, which lets them in when it has begun.  The join waits for both (kv4_few_kernel's last block).
+  const bool joined = l.few_cut || l.many;
+  const unsigned join_blocks = (unsigned)std::min<long long>(4ll * kv4_sms(), (long long)l.few_joins() * G * used + (l.many ? (long long)l.many_joins() * G * (KV4_MANY / KJ) : 0));
 #define FEW(TT, DD, NG, CPL, NB)                                                                                                              \
   {                                                                                                                                           \
     constexpr int COLS = 4 * CPL * NB, ring = KF_WARPS * kf_stages(DD, NG) * 2 * kv4_slice_bytes(DD, NG), join = KF_WARPS * COLS * (DD + 4) * 4; \
@@ -564,9 +559,9 @@ int ll_kv4_attn(const ll_kv4_cache* cache, const void* blocks, const void* q, lo
       prefer_max_smem(kv4_few_kernel<TT, DD, NG, CPL, NB>);                                                                                   \
       set.mark();                                                                                                                             \
     }                                                                                                                                         \
-    kv4_few_kernel<TT, DD, NG, CPL, NB><<<(unsigned)(items * G), KF_THREADS, smem, st>>>(a);                                                         \
+    LL_CUDA(launch(kv4_few_kernel<TT, DD, NG, CPL, NB>, dim3((unsigned)(l.few_items * G)), dim3(KF_THREADS), smem, st, l.many, a));           \
     LL_LAUNCH_OK("kv4_few_kernel");                                                                                                           \
-    if (l.few_cut) LL_CUDA(launch(kv4_join_kernel<TT, DD, COLS>, dim3((unsigned)(items * G), (unsigned)min((long long)cols, (long long)max_count * R)), dim3(KJ * 32), 0, st, true, a)); \
+    if (joined) LL_CUDA(launch(kv4_join_kernel<TT, DD, COLS>, dim3(join_blocks), dim3(KJ * 32), 0, st, true, a, m));                          \
   }
 #define FEW_COLS(TT, DD, NG)              \
   if (cols == 4) FEW(TT, DD, NG, 1, 1)    \

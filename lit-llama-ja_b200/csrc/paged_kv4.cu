@@ -95,7 +95,7 @@ __device__ __forceinline__ void place_token(const PlanView& v, const Kv4Pool& c,
 // ---- the division of a step's attention
 struct PlanWork {
   int R, few, cols, longest;           // columns a token, most columns of the few, columns of a tile; most pages of a request
-  int parts, max_items;                // places for blocks (a key head), items there is room for
+  int parts, max_items, max_joins;     // places for blocks (a key head), items and joins there is room for
   float fixed, joined;                 // what a part costs beside its pages, and what parts that have to be joined cost the step, in pages
   bool cut;                            // whether walks may be cut
   int32_t* work;
@@ -133,7 +133,7 @@ __device__ __forceinline__ void divide_work(const PlanView& v, const PlanWork& d
   __syncthreads();
   const int walks = s_count[0];
   if (walks == 0) {
-    if (threadIdx.x == 0) d.work[0] = 0;
+    if (threadIdx.x == 0) d.work[0] = d.work[1] = 0;
     return;
   }
   int step = d.longest;
@@ -188,6 +188,7 @@ __device__ __forceinline__ void divide_work(const PlanView& v, const PlanWork& d
   while ((step - 1) >> shift >= PW_SIZES) ++shift;
   auto bucket = [&](int size) { return PW_SIZES - 1 - ((min(size, step) - 1) >> shift); };
   for (int x = threadIdx.x; x < PW_SIZES; x += blockDim.x) s_size[x] = 0;
+  if (threadIdx.x == 0) s_count[0] = 0;
   __syncthreads();
   for (int i = MANY ? warp : threadIdx.x; i < v.B; i += MANY ? warps : blockDim.x) {
     const int w = tiles(i);
@@ -228,10 +229,18 @@ __device__ __forceinline__ void divide_work(const PlanView& v, const PlanWork& d
       o[1] = make_int4(tile, part * each, (part + 1) * each, k);
       o[2] = make_int4(part, base, 0, 0);
     };
+    auto join = [&](int tile, int k, int base) {
+      const int j = atomicAdd(&s_count[0], 1);
+      if (j >= d.max_joins) return;
+      int4* o = const_cast<int4*>(joins_of(d.work, d.max_items)) + 2 * (size_t)j;
+      o[0] = make_int4(first, n, tile, k);
+      o[1] = make_int4(base, 0, 0, 0);
+    };
     if (MANY) {
       for (int t = lane; t < w; t += 32) {
         const int p = pages(i, t), k = cut(p), each = (p + k - 1) / k, at = atomicAdd(&s_size[bucket(each)], k);
         for (int e = 0; e < k; ++e) store(at + e, t, e, each, k, at);
+        if (k > 1) join(t, k, at);
       }
     } else {
       const int p = pages(i, 0), k = cut(p), each = (p + k - 1) / k;
@@ -239,8 +248,12 @@ __device__ __forceinline__ void divide_work(const PlanView& v, const PlanWork& d
       if (lane == 0) at = atomicAdd(&s_size[bucket(each)], w * k);
       at = __shfl_sync(0xffffffffu, at, 0);
       for (int e = lane; e < w * k; e += 32) store(at + e, e / k, e % k, each, k, at + e / k * k);
+      if (k > 1)
+        for (int t = lane; t < w; t += 32) join(t, k, at + t * k);
     }
   }
+  __syncthreads();
+  if (threadIdx.x == 0) d.work[1] = min(s_count[0], d.max_joins);
 }
 
 // A step's pages, slots (of up to `here` tokens) and division, by one block: prefix sums over the sequences.
@@ -556,8 +569,8 @@ int ll_kv4_plan(const ll_kv4_cache* cache, const int32_t* rows, const int32_t* c
   LL_CHECK_ARG(l.few_items * cache->kv_heads <= INT_MAX && l.many_items * cache->kv_heads <= INT_MAX, "kv4_plan: %d sequences of %d tokens, %d heads", B, T, cache->heads);
   const int longest = (cache->max_length + KV4_PAGE - 1) / KV4_PAGE;
   // (pages take a block of the few 0.8 us, of the many 1.4; a part's start and end 2 and 3, parts that are joined 3 and 8 more)
-  const PlanWork few{l.R, l.few, l.cols, longest, l.few_parts, (int)l.few_items, 2.5f, 3.5f, l.few_cut, work};
-  const PlanWork many{l.R, l.few, KV4_MANY, longest, l.many_parts, (int)l.many_items, 2.f, 5.5f, true, l.many ? work + l.few_ints() : nullptr};
+  const PlanWork few{l.R, l.few, l.cols, longest, l.few_parts, (int)l.few_items, l.few_joins(), 2.5f, 3.5f, l.few_cut, work};
+  const PlanWork many{l.R, l.few, KV4_MANY, longest, l.many_parts, (int)l.many_items, l.many_joins(), 2.f, 5.5f, true, l.many ? work + l.few_ints() : nullptr};
   // The block itself places the tokens of a step while that takes it a few rounds; more are placed by a grid.
   const int threads = B <= 256 && T <= 2048 ? 256 : PLAN_THREADS, here = T <= 8 * threads ? T : 0;
   cudaStream_t st = (cudaStream_t)stream;

@@ -155,6 +155,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_ptr, 0);
+  // (Not before the block has its tensor memory: a kernel let in that fits beside it could take that first, and then waits for this one's end.)
+  pdl_launch_dependents();
 
   if (warp >= KP_FIRST) {
     // ===================== codes into operands =====================

@@ -14,13 +14,15 @@ struct Kv4Attn {
   const int32_t *table, *work;
   void* y;
   float* part;         // [kept][G][columns] of D sums, then [kept][G][columns] of (reference, sum of weights)
-  int H, G, width, pages, items, kept;      // items a grid has, parts whose sums there is room for
+  int H, G, width, pages;
+  int items, kept, cols;      // items there is room for, parts whose sums there is room for, columns of a tile that may be in use
   float scale;
   int* word;           // wait_word()
 };
 
 namespace {
 
+// A list of parts of walks: four numbers (parts, walks that are in more than one part), the parts, then those walks.
 // One part of a walk: a range of one request's pages for one tile of columns (a column: one query of one of the heads that share a key head, the
 // heads of a token next to one another).  The largest parts come first.
 struct __align__(16) Kv4Item {
@@ -38,6 +40,12 @@ __device__ __forceinline__ Kv4Item load_item(const int32_t* work, int i) {
   it.row = a.x, it.first = a.y, it.count = a.z, it.pos0 = a.w, it.tile = b.x, it.page0 = b.y, it.page1 = b.z, it.parts = b.w, it.part = c.x, it.base = c.y;
   return it;
 }
+// A walk whose parts have to be joined.
+struct __align__(16) Kv4Join {
+  int first, count, tile, parts;       // first row and number of the request's tokens, tile of columns, parts
+  int base, pad[3];                    // index of the first part
+};
+__host__ __device__ __forceinline__ const int4* joins_of(const int32_t* work, int max_items) { return reinterpret_cast<const int4*>(work) + 1 + 3 * (size_t)max_items; }
 
 // column -> token and head: a shift where the heads of a key head are 1, 2, 4 .., else a division
 __device__ __forceinline__ int column_token(int c, int R) { return (R & (R - 1)) == 0 ? c >> (31 - __clz(R)) : c / R; }
@@ -72,8 +80,11 @@ struct Kv4Lists {
     few_items = std::min((long long)T * R / cols + seqs, seqs * each) + KV4_CUTS * few_parts;
     many_items = many ? (long long)T * R / KV4_MANY + std::min(seqs, (long long)T * R / KV4_FEW_MOST) + KV4_CUTS * many_parts : 0;
   }
-  size_t few_ints() const { return 4 + sizeof(Kv4Item) / 4 * (size_t)few_items; }
-  size_t ints() const { return few_ints() + (many ? 4 + sizeof(Kv4Item) / 4 * (size_t)many_items : 0); }
+  // walks in more than one part: every one has a part more than it would have whole
+  int few_joins() const { return KV4_CUTS * few_parts; }
+  int many_joins() const { return KV4_CUTS * many_parts; }
+  size_t few_ints() const { return 4 + sizeof(Kv4Item) / 4 * (size_t)few_items + sizeof(Kv4Join) / 4 * (size_t)few_joins(); }
+  size_t ints() const { return few_ints() + (many ? 4 + sizeof(Kv4Item) / 4 * (size_t)many_items + sizeof(Kv4Join) / 4 * (size_t)many_joins() : 0); }
   // sums are kept of parts that have to be joined, and none are where there are walks for KV4_ROUNDS rounds
   int few_kept() const { return (int)std::min(few_items, (long long)(KV4_ROUNDS + KV4_CUTS) * few_parts); }
   int many_kept() const { return (int)std::min(many_items, (long long)(KV4_ROUNDS + KV4_CUTS) * many_parts); }
