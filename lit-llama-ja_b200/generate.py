@@ -9,7 +9,7 @@ from __future__ import annotations
 import sys
 import time
 from pathlib import Path
-from typing import Optional
+from typing import List, Optional, Sequence
 
 import torch
 
@@ -17,6 +17,7 @@ sys.path.insert(0, str(Path(__file__).parent.resolve()))
 
 from lit_llama import LLaMA, HFTokenizer, Tokenizer  # noqa: E402
 from lit_llama._native import check_waits  # noqa: E402
+from lit_llama.stepping import graph_capture  # noqa: E402
 from lit_llama.utils import EmptyInitOnDevice, lazy_load, llama_model_lookup  # noqa: E402
 
 
@@ -99,6 +100,65 @@ def generate(
     return _sample_loop(model, idx, logits, max_new_tokens, max_seq_length, temperature, top_k, eos_id)
 
 
+def _draw(logits: torch.Tensor, temperature: float, top_k: Optional[int]) -> torch.Tensor:
+    """ref: generate.py:66-75, a row a sequence."""
+    logits = logits / temperature
+    if top_k is not None:
+        kth = torch.topk(logits, min(top_k, logits.size(-1))).values[:, -1:]
+        logits = torch.where(logits < kth, -float("Inf"), logits)
+    return torch.multinomial(torch.nn.functional.softmax(logits, dim=-1), num_samples=1)[:, 0]
+
+
+@torch.no_grad()
+def generate_batch(model: LLaMA, prompts: Sequence[torch.Tensor], max_new_tokens: int, *, temperature: float = 1.0, top_k: Optional[int] = None,
+                   eos_id: Optional[int] = None, group: Optional[int] = None) -> List[torch.Tensor]:
+    """``generate`` for prompts of unequal lengths at once, over a key/value cache in 4 bits (``lit_llama/paged_cache.py``): the prompts as one step, then a
+    token a sequence and step, replayed as one CUDA graph.  A sequence ends before its first ``eos_id``."""
+    if not prompts or max_new_tokens < 1 or any(p.dim() != 1 or p.numel() == 0 for p in prompts):
+        raise ValueError(f"{len(prompts)} prompts, {max_new_tokens} tokens to come: one of either at least, and no prompt empty")
+    lengths = [p.numel() for p in prompts]
+    if max(lengths) + max_new_tokens > model.config.block_size + 1:
+        raise ValueError(f"{max(lengths)} + {max_new_tokens} tokens, block size is only {model.config.block_size}")
+    dev, B = prompts[0].device, len(prompts)
+    held = [n + max_new_tokens - 1 for n in lengths]               # (the last token drawn is not fed)
+    cache = model.paged_cache(pages=sum(-(-n // 64) for n in held), requests=B, max_length=max(held), group=group)
+    rows = torch.arange(B, dtype=torch.int32, device=dev)
+    plan = cache.plan(rows, lengths, sum(lengths), max_count=max(lengths))
+    logits = model.forward_paged(torch.cat(list(prompts)), cache, plan)
+    new = torch.empty((B, max_new_tokens), dtype=prompts[0].dtype, device=dev)
+    live = torch.ones(B, dtype=torch.int32, device=dev)             # tokens that each sequence brings to a step
+    packed = torch.zeros(B + 1, dtype=prompts[0].dtype, device=dev)  # theirs, one after the other; the last place takes the others'
+    graph = out = None
+    done = torch.full((B,), max_new_tokens, dtype=torch.int64, device=dev)
+    for i in range(max_new_tokens):
+        if i > 0:
+            packed.scatter_(0, torch.where(live > 0, live.cumsum(0) - 1, B), token)
+
+            def step():
+                return model.forward_paged(packed[:B], cache, cache.plan(rows, live, B, max_count=1))
+
+            if graph is not None:
+                graph.replay()
+                logits = out
+            else:
+                logits = step()                                     # (the first one eagerly: workspaces, weight streams, kernel attributes)
+                if i == 1 and max_new_tokens > 3:
+                    torch.cuda.synchronize()
+                    graph = torch.cuda.CUDAGraph()
+                    with graph_capture(graph):
+                        out = step()
+        token = _draw(logits, temperature, top_k).to(new.dtype)     # (of a sequence that has ended some other one's row, and of no consequence)
+        new[:, i] = token
+        if eos_id is not None:
+            ended = (token == eos_id) & (live > 0)
+            done = torch.where(ended, i, done)
+            live.mul_((~ended).int())
+            if not bool(live.any()):
+                break
+    check_waits()
+    return [torch.cat([p, new[b, :n]]) for b, (p, n) in enumerate(zip(prompts, done.tolist()))]
+
+
 def load_model(checkpoint_path: Path, quantize: Optional[str], device: torch.device, dtype: torch.dtype) -> LLaMA:
     """ref: generate.py:124-136 (lazy_load + quantization ctx + load_state_dict).  GPTQ checkpoints go through the
     streaming loader (disk -> pinned -> HBM, the GEMV stream of every layer built under the read); llm.int8 quantizes a
@@ -132,10 +192,13 @@ def main(
     quantize: Optional[str] = None,
     prompt_ids: Optional[str] = None,
     dtype: Optional[str] = None,
+    kv_cache: Optional[str] = None,
 ) -> None:
     """ref: generate.py:92-155 - same flags and output.  ``checkpoint_path`` may also be a model folder (config.json +
     model.safetensors, any registered architecture); ``prompt_ids`` ("5,17,3") feeds token ids directly and prints ids,
-    for models that come without a tokenizer."""
+    for models that come without a tokenizer.  ``kv_cache`` "int4": all samples as one batch over a key/value cache in 4 bits."""
+    if kv_cache not in (None, "int4"):
+        raise ValueError(f"kv_cache {kv_cache!r}: None or 'int4'")
     checkpoint_path, tokenizer_path = Path(checkpoint_path), Path(tokenizer_path)
     assert checkpoint_path.exists(), checkpoint_path
     assert prompt_ids is not None or tokenizer_path.is_file(), tokenizer_path
@@ -159,6 +222,19 @@ def main(
     prompt_length = encoded.size(0)
 
     torch.manual_seed(1234)
+    if kv_cache is not None:
+        if not isinstance(model, LLaMA):
+            raise ValueError(f"the 4-bit key/value cache serves LLaMA models, not {type(model).__name__}")
+        torch.cuda.synchronize()
+        t0 = time.perf_counter()
+        ys = generate_batch(model, [encoded] * num_samples, max_new_tokens, temperature=temperature, top_k=top_k)
+        torch.cuda.synchronize()
+        t = time.perf_counter() - t0
+        for y in ys:
+            print(tokenizer.decode(y) if tokenizer is not None else ",".join(str(int(t)) for t in y))
+        n_new = sum(y.size(0) - prompt_length for y in ys)
+        print(f"Time for inference: {t:.02f} sec total, {n_new / t:.02f} tokens/sec", file=sys.stderr)
+        num_samples = 0
     for i in range(num_samples):
         torch.cuda.synchronize()
         t0 = time.perf_counter()
@@ -187,7 +263,8 @@ if __name__ == "__main__":
     ap.add_argument("--quantize", default=None, choices=[None, "llm.int8", "gptq.int4", "gptq.int8"])
     ap.add_argument("--prompt_ids", default=None, help="comma-separated token ids instead of --prompt (no tokenizer needed)")
     ap.add_argument("--dtype", default=None, choices=[None, "bfloat16", "float32"])
+    ap.add_argument("--kv_cache", default=None, choices=[None, "int4"], help="int4: all samples as one batch over a key/value cache in 4 bits")
     a = ap.parse_args()
     main(a.prompt, num_samples=a.num_samples, max_new_tokens=a.max_new_tokens, top_k=a.top_k,
          temperature=a.temperature, checkpoint_path=a.checkpoint_path, tokenizer_path=a.tokenizer_path,
-         quantize=a.quantize, prompt_ids=a.prompt_ids, dtype=a.dtype)
+         quantize=a.quantize, prompt_ids=a.prompt_ids, dtype=a.dtype, kv_cache=a.kv_cache)

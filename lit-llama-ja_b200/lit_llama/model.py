@@ -22,6 +22,7 @@ import torch.nn as nn
 from torch.nn import functional as F
 
 from . import _native as N
+from .paged_cache import CachePlan, PagedCache4
 from .quantization import gated_pair, is_plain
 from .stepping import graph_capture
 from .utils import find_multiple
@@ -410,6 +411,49 @@ class LLaMA(nn.Module):
             for i, block in enumerate(self.transformer.h):
                 x, self.kv_caches[i] = block(x, step, self.kv_caches[i])
         return x
+
+    # ------------------------------------------------------------------ requests of unequal lengths over the 4-bit cache
+    def paged_cache(self, *, pages: int, requests: int, max_length: Optional[int] = None, group: Optional[int] = None) -> PagedCache4:
+        """A 4-bit cache of this model's layers and heads: ``pages`` of 64 slots for up to ``requests`` requests of up to ``max_length`` tokens (the block
+        size unless given)."""
+        w, hs = self.transformer.wte.weight, self.config.head_size
+        max_length = self.config.block_size if max_length is None else max_length
+        if max_length > self.config.block_size:
+            raise ValueError(f"requests of up to {max_length} tokens, block size is only {self.config.block_size}")
+        return PagedCache4(len(self.transformer.h), self.transformer.h[0].attn.n_head, hs, pages=pages, requests=requests, max_length=max_length,
+                           group=min(64, hs) if group is None else group, dtype=w.dtype, device=w.device)
+
+    @torch.no_grad()
+    def forward_paged(self, tokens: torch.Tensor, cache: PagedCache4, plan: CachePlan, all_rows: bool = False) -> torch.Tensor:
+        """One step of requests of unequal lengths: ``tokens`` in the order of the plan's sequences.  Returns the logits ``[sequences, vocab]`` of every
+        sequence's last token (of one that brings none, or was refused, numbers without a meaning), or with ``all_rows`` ``[tokens, vocab]``.  Nothing
+        here looks at lengths on the host: a captured step (with its ``cache.plan``) serves any."""
+        N.require_cuda(tokens)
+        if tokens.shape != (plan.T,) or tokens.dtype not in (torch.int32, torch.int64):
+            raise RuntimeError(f"tokens of shape {tuple(tokens.shape)} in {tokens.dtype}, and the plan is of {plan.T}")
+        blocks = self.transformer.h
+        attn = blocks[0].attn
+        if any(type(b) is not Block or type(b.attn) is not CausalSelfAttention for b in blocks):
+            raise RuntimeError("the paged cache serves LLaMA's own blocks, not those of a model that extends them")
+        if (cache.n_layer, cache.n_head, cache.n_kv_head, cache.head_size) != (len(blocks), attn.n_head, attn.n_head, attn.head_size):
+            raise RuntimeError(f"a cache of {cache.n_layer} layers of {cache.n_head} heads of {cache.head_size} for a model of {len(blocks)} of {attn.n_head} of {attn.head_size}")
+        if cache.max_length > self.config.block_size:
+            raise RuntimeError(f"a cache for requests of up to {cache.max_length} tokens, block size is only {self.config.block_size}")
+        T, nh, hs = plan.T, attn.n_head, attn.head_size
+        if T == 0:
+            return torch.zeros((0 if all_rows else plan.B, self.config.padded_vocab_size), dtype=cache.dtype, device=tokens.device)
+        self._ensure_caches(tokens)
+        x = self.transformer.wte(tokens)[None]
+        y = torch.zeros((T, nh, hs), dtype=cache.dtype, device=tokens.device)        # (rows behind the last token stay zeros)
+        for i, block in enumerate(blocks):
+            q, k, v = block.attn.c_attn(block.rms_1(x)).view(T, 3, nh, hs).unbind(1)
+            q = cache.append(i, plan, q, k, v, rope=self._rope_f32)
+            cache.attend(i, plan, q, out=y)
+            x, h = _residual_norm(x, block.attn.c_proj(y.view(1, T, nh * hs)), block.rms_2)
+            x = _residual(x, block.mlp(h))
+        if not all_rows:
+            x = x.index_select(1, (plan.starts[1:] - 1).clamp(min=0))
+        return self.lm_head(self.transformer.ln_f(x))[0]
 
     def _kv_from_pool(self, shape, dtype, dev):
         """Zeroed KV tensors of this shape - the SAME tensors after every reset_cache(), so that captured step graphs

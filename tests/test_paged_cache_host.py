@@ -123,3 +123,20 @@ def test_rounding_is_half_a_step_at_most():
             assert bool((off <= span / 15 * (1 + half) / 2 * (1 + 1e-6) + span * half).all())
             low = held_as(x, group).unflatten(-1, (-1, group)).amin(-1)
             assert torch.equal(low, g.amin(-1))
+
+
+def test_generate_batch_refuses(monkeypatch):
+    import sys
+    from pathlib import Path
+    from types import SimpleNamespace
+
+    sys.path.insert(0, str(Path(__file__).parent.parent / "lit-llama-ja_b200"))
+    import generate
+
+    model = SimpleNamespace(config=SimpleNamespace(block_size=64))
+    one = torch.zeros(5, dtype=torch.int64)
+    for prompts, new in (([], 3), ([one], 0), ([one, one[:0]], 3), ([one[None]], 3), ([one], 61), ([one, torch.zeros(60, dtype=torch.int64)], 6)):
+        with pytest.raises(ValueError):
+            generate.generate_batch(model, prompts, new)
+    with pytest.raises(ValueError, match="kv_cache"):
+        generate.main(kv_cache="int8")
