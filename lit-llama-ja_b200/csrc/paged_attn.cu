@@ -41,6 +41,7 @@ __device__ __forceinline__ uint32_t half_bits(float a, float b) { return pair_bi
 // One warp's wait for its copy: bounded; one that runs out leaves a code for the host.
 __device__ __forceinline__ bool kf_wait(uint64_t* bar, uint32_t parity, int* word) {
   if (mbar_try_wait(bar, parity)) return true;
+#pragma unroll 1
   for (uint32_t i = 0; i < KF_WAIT_LIMIT; ++i)
     if (mbar_try_wait(bar, parity)) return true;
   wait_ran_out(word, 801);
@@ -72,6 +73,7 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
   const int col0 = it.tile * COLS, cols = min(COLS, n * R - col0);
   T* y = (T*)a.y;
   if (row < 0) {                        // a refused sequence's tokens are no numbers
+#pragma unroll 1
     for (int e = threadIdx.x; e < cols * D; e += KF_THREADS) {
       const int c = col0 + e / D;
       dt<T>::st(y, ((size_t)(first + column_token(c, R)) * a.H + head * R + column_head(c, R)) * D + e % D, NAN);
@@ -173,6 +175,7 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
   bool ok = true;
   int st = 0;
   uint32_t parity = 0;
+#pragma unroll 1
   for (int i = 0; i < units; ++i) {
     ok = __all_sync(0xffffffffu, kf_wait(&full[st], parity, a.word));
     if (!ok) break;
@@ -365,7 +368,7 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
   }
   if (!ok) {
     s_fail = 1;
-    for (int w = 0; w < 2048; ++w) __nanosleep(512);                    // copies that were asked for end before the block does
+    kv4_let_end();                                                      // copies that were asked for end before the block does
   }
   // a column's sums over the lanes that share it
 #pragma unroll
@@ -403,6 +406,7 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
     }
   __syncthreads();
   // the four warps' parts; the block's are stored as they are, or as the result where there is no other part
+#pragma unroll 1
   for (int x = threadIdx.x; x < cols * (D / 4); x += KF_THREADS) {
     const int c = x / (D / 4), d = x % (D / 4) * 4;
     float m = s_ref[0][c];

@@ -54,14 +54,32 @@ __device__ __forceinline__ V block_before(V v, V* s_warp, V& total) {
 
 __device__ __forceinline__ int pages_of(int tokens) { return (tokens + KV4_PAGE - 1) / KV4_PAGE; }
 
-// The first sequence that names a request has it: an ordered claim, so that a request named twice is the same one's in every run.
+// The first sequence that names a request has it, so that a request named twice is the same one's in every run.  Up to PLAN_NEAR sequences look
+// through the names before theirs in shared memory; more leave an ordered claim with the request.
+constexpr int PLAN_NEAR = 256;
 __device__ __forceinline__ void claim_requests(const int32_t* rows, const int32_t* wants, bool any_want, int B, const Kv4Pool& c) {
+  if (B <= PLAN_NEAR) return;
   for (int i = threadIdx.x; i < B; i += blockDim.x)
     if ((any_want || wants[i] > 0) && rows[i] >= 0 && rows[i] < c.requests) c.stamp[rows[i]] = INT_MAX;
   __syncthreads();
   for (int i = threadIdx.x; i < B; i += blockDim.x)
     if ((any_want || wants[i] > 0) && rows[i] >= 0 && rows[i] < c.requests) atomicMin(&c.stamp[rows[i]], i);
   __syncthreads();
+}
+// Whether sequence i's claim on `row` holds (`claims`: it has one).  Every thread of the block calls.
+__device__ __forceinline__ bool claimed(int i, int row, bool claims, int B, const Kv4Pool& c, int* s_name) {
+  if (B > PLAN_NEAR) return claims && c.stamp[row] == i;
+  if (i < PLAN_NEAR) s_name[i] = claims ? row : -1;
+  __syncthreads();
+  bool first = claims;
+  if (claims) {
+    const int4* names = reinterpret_cast<const int4*>(s_name);
+    for (int j = 0; 4 * j < i; ++j) {
+      const int4 n = names[j];
+      first &= !(n.x == row && 4 * j < i) && !(n.y == row && 4 * j + 1 < i) && !(n.z == row && 4 * j + 2 < i) && !(n.w == row && 4 * j + 3 < i);
+    }
+  }
+  return first;
 }
 
 // What the sequences of a step came to: in shared memory where there is room, else where the plan keeps it.
@@ -170,6 +188,7 @@ __device__ __forceinline__ void divide_work(const PlanView& v, const PlanWork& d
     float best = 1e30f;
     int mine = 0;
     for (int k = warp; k < PW_TRIES; k += warps) {
+      if (k > 0 && tried(k) == tried(k - 1)) continue;
       const float f = length(tried(k));
       if (f < best) best = f, mine = k;
     }
@@ -218,38 +237,48 @@ __device__ __forceinline__ void divide_work(const PlanView& v, const PlanWork& d
   }
   __syncthreads();
   // (which of the parts of one size comes first is left to chance, and of no consequence: every part has its own place for its sums)
-  for (int i = warp; i < v.B; i += warps) {
-    const int w = tiles(i);
-    if (w == 0) continue;
-    const int n = tokens(i), row = v.request[i], pos0 = v.ends[i] - n, first = v.starts[i];
-    auto store = [&](int at, int tile, int part, int each, int k, int base) {
-      if (at >= d.max_items) return;
-      int4* o = reinterpret_cast<int4*>(d.work) + 1 + 3 * (size_t)at;
-      o[0] = make_int4(row, first, n, pos0);
-      o[1] = make_int4(tile, part * each, (part + 1) * each, k);
-      o[2] = make_int4(part, base, 0, 0);
-    };
-    auto join = [&](int tile, int k, int base) {
-      const int j = atomicAdd(&s_count[0], 1);
-      if (j >= d.max_joins) return;
-      int4* o = const_cast<int4*>(joins_of(d.work, d.max_items)) + 2 * (size_t)j;
-      o[0] = make_int4(first, n, tile, k);
-      o[1] = make_int4(base, 0, 0, 0);
-    };
-    if (MANY) {
+  auto store = [&](int i, int at, int tile, int part, int each, int k, int base) {
+    if (at >= d.max_items) return;
+    const int n = tokens(i);
+    int4* o = reinterpret_cast<int4*>(d.work) + 1 + 3 * (size_t)at;
+    o[0] = make_int4(v.request[i], v.starts[i], n, v.ends[i] - n);
+    o[1] = make_int4(tile, part * each, (part + 1) * each, k);
+    o[2] = make_int4(part, base, 0, 0);
+  };
+  auto join = [&](int i, int tile, int k, int base) {
+    const int j = atomicAdd(&s_count[0], 1);
+    if (j >= d.max_joins) return;
+    int4* o = const_cast<int4*>(joins_of(d.work, d.max_items)) + 2 * (size_t)j;
+    o[0] = make_int4(v.starts[i], tokens(i), tile, k);
+    o[1] = make_int4(base, 0, 0, 0);
+  };
+  if (MANY) {
+    for (int i = warp; i < v.B; i += warps) {
+      const int w = tiles(i);
       for (int t = lane; t < w; t += 32) {
         const int p = pages(i, t), k = cut(p), each = (p + k - 1) / k, at = atomicAdd(&s_size[bucket(each)], k);
-        for (int e = 0; e < k; ++e) store(at + e, t, e, each, k, at);
-        if (k > 1) join(t, k, at);
+        for (int e = 0; e < k; ++e) store(i, at + e, t, e, each, k, at);
+        if (k > 1) join(i, t, k, at);
       }
-    } else {
-      const int p = pages(i, 0), k = cut(p), each = (p + k - 1) / k;
-      int at = 0;
-      if (lane == 0) at = atomicAdd(&s_size[bucket(each)], w * k);
-      at = __shfl_sync(0xffffffffu, at, 0);
-      for (int e = lane; e < w * k; e += 32) store(at + e, e / k, e % k, each, k, at + e / k * k);
-      if (k > 1)
-        for (int t = lane; t < w; t += 32) join(t, k, at + t * k);
+    }
+  } else {      // a thread a sequence; its warp helps where there are more than four parts
+    for (int i0 = 32 * warp; i0 < v.B; i0 += 32 * warps) {
+      const int i = i0 + lane, w = i < v.B ? tiles(i) : 0;
+      int k = 0, each = 1, at = 0;
+      if (w > 0) {
+        const int p = pages(i, 0);
+        k = cut(p), each = (p + k - 1) / k;
+        at = atomicAdd(&s_size[bucket(each)], w * k);
+        if (w * k <= 4)
+          for (int e = 0; e < w * k; ++e) store(i, at + e, e / k, e % k, each, k, at + e / k * k);
+        if (k > 1)
+          for (int t = 0; t < w; ++t) join(i, t, k, at + t * k);
+      }
+      for (uint32_t more = __ballot_sync(0xffffffffu, w * k > 4); more != 0u; more &= more - 1) {
+        const int l = __ffs(more) - 1, ww = __shfl_sync(0xffffffffu, w, l), kk = __shfl_sync(0xffffffffu, k, l), ee = __shfl_sync(0xffffffffu, each, l),
+                  aa = __shfl_sync(0xffffffffu, at, l);
+        for (int e = lane; e < ww * kk; e += 32) store(i0 + l, aa + e, e / kk, e % kk, ee, kk, aa + e / kk * kk);
+      }
     }
   }
   __syncthreads();
@@ -263,6 +292,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv4_plan_kernel(const int32_t* _
   __shared__ int s_need[32], s_size[PW_SIZES];
   __shared__ int s_row[PLAN_THREADS], s_first[PLAN_THREADS], s_pages[PLAN_THREADS], s_used[PLAN_THREADS];
   __shared__ int s_starts[PLAN_HELD + 1], s_ends[PLAN_HELD], s_request[PLAN_HELD];
+  __shared__ __align__(16) int s_name[PLAN_NEAR];
   const int n_free = min(max(*c.n_free, 0), c.pages), nt = blockDim.x, lane = threadIdx.x & 31;
   const bool held = B <= PLAN_HELD;
   claim_requests(rows, counts, false, B, c);
@@ -272,12 +302,13 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv4_plan_kernel(const int32_t* _
     const int i = i0 + threadIdx.x;
     const int row = i < B ? rows[i] : -1, count = i < B ? counts[i] : 0, n = max(count, 0);
     const bool named = row >= 0 && row < c.requests;
-    const int old = named ? c.lengths[row] : 0, claim = named && n > 0 ? c.stamp[row] : i;
+    const int old = named ? c.lengths[row] : 0;
+    const bool mine = claimed(i, row, named && n > 0, B, c, s_name);
     long long total;
     const long long first = tokens + block_before<long long>(n, s_sum, total);
     tokens += total;
     int status = KV4_OK;
-    if (count < 0 || (n > 0 && (!named || claim != i))) status = KV4_BAD_ROW;
+    if (count < 0 || (n > 0 && !mine)) status = KV4_BAD_ROW;
     else if (first + n > T) status = KV4_BEHIND;
     else if (n > max_count || (long long)old + n > c.max_length) status = KV4_TOO_LONG;
     const int page0 = pages_of(old), need = status == KV4_OK && n > 0 ? pages_of(old + n) - page0 : 0;
@@ -303,7 +334,14 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv4_plan_kernel(const int32_t* _
         s_starts[i + 1] = end;
         s_request[i] = request;
       }
-      if (ok && n > 0) c.lengths[row] = old + n;
+      if (ok && n > 0) {
+        c.lengths[row] = old + n;
+        p.ends[i] = old + n;
+        if (held) s_ends[i] = old + n;
+      } else if (!ok) {
+        p.ends[i] = 0;
+        if (held) s_ends[i] = 0;
+      }
     }
     __syncthreads();
     // the new entries of the table, a warp a sequence
@@ -313,8 +351,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv4_plan_kernel(const int32_t* _
   }
   if (threadIdx.x == 0) *c.n_free = n_free - given;
   for (int i = threadIdx.x; i < B; i += nt) {      // (when all lengths are the step's: an idle sequence may name another one's request)
-    const int row = rows[i];
-    const int end = p.status[i] == KV4_OK && row >= 0 && row < c.requests ? c.lengths[row] : 0;
+    if (counts[i] != 0 || p.status[i] != KV4_OK) continue;
+    const int row = rows[i], end = row >= 0 && row < c.requests ? c.lengths[row] : 0;
     p.ends[i] = end;
     if (held) s_ends[i] = end;
   }
@@ -336,39 +374,37 @@ __global__ void __launch_bounds__(256) kv4_tokens_kernel(int B, int T, int here,
 __global__ void __launch_bounds__(PLAN_THREADS) kv4_truncate_kernel(const int32_t* __restrict__ rows, const int32_t* __restrict__ keep, int B, Kv4Pool c) {
   __shared__ int s_sum[32];
   __shared__ int s_row[PLAN_THREADS], s_first[PLAN_THREADS], s_pages[PLAN_THREADS], s_used[PLAN_THREADS];
-  const int n_free = min(max(*c.n_free, 0), c.pages);
+  __shared__ __align__(16) int s_name[PLAN_NEAR];
+  const int n_free = min(max(*c.n_free, 0), c.pages), nt = blockDim.x, lane = threadIdx.x & 31;
   claim_requests(rows, keep, true, B, c);
-  int total = 0;                        // the pages of all sequences have to be known before the first goes back
-  for (int i0 = 0; i0 < B; i0 += blockDim.x) {
-    const int i = i0 + threadIdx.x, row = i < B ? rows[i] : -1;
-    int n = 0, all;
-    if (row >= 0 && row < c.requests && c.stamp[row] == i && keep[i] >= 0 && keep[i] < c.lengths[row]) n = pages_of(c.lengths[row]) - pages_of(keep[i]);
-    block_before<int>(n, s_sum, all);
-    total += all;
-  }
-  int done = 0;
-  for (int i0 = 0; i0 < B; i0 += blockDim.x) {
-    const int i = i0 + threadIdx.x, row = i < B ? rows[i] : -1;
-    int n = 0, first = 0, all;
-    const bool cut = row >= 0 && row < c.requests && c.stamp[row] == i && keep[i] >= 0 && keep[i] < c.lengths[row];
-    if (cut) first = pages_of(keep[i]), n = pages_of(c.lengths[row]) - first;
-    const int before = done + block_before<int>(n, s_sum, all);
-    done += all;
-    s_row[threadIdx.x] = row;
-    s_first[threadIdx.x] = first;
-    s_pages[threadIdx.x] = n;
-    s_used[threadIdx.x] = before;
-    __syncthreads();
-    if (cut) c.lengths[row] = keep[i];
-    const int lane = threadIdx.x & 31;
-    for (int j = threadIdx.x >> 5; j < min((int)blockDim.x, B - i0); j += blockDim.x >> 5)
-      for (int k = lane; k < s_pages[j]; k += 32) {
-        int32_t* e = c.table + (size_t)s_row[j] * c.width + s_first[j] + k;
-        const int at = n_free + total - 1 - s_used[j] - k;
-        if (at < c.pages) c.free[at] = *e;
-        *e = -1;
-      }
-    __syncthreads();
+  int total = 0, done = 0;              // the pages of all sequences have to be known before the first goes back
+  for (int round = B > nt ? 0 : 1; round < 2; ++round) {
+    for (int i0 = 0; i0 < B; i0 += nt) {
+      const int i = i0 + threadIdx.x, row = i < B ? rows[i] : -1, to = i < B ? keep[i] : -1;
+      const bool named = row >= 0 && row < c.requests;
+      const int old = named ? c.lengths[row] : 0;
+      const bool cut = claimed(i, row, named, B, c, s_name) && to >= 0 && to < old;
+      const int first = cut ? pages_of(to) : 0, n = cut ? pages_of(old) - first : 0;
+      int all;
+      const int before = done + block_before<int>(n, s_sum, all);
+      if (round == 0 || B <= nt) total += all;
+      if (round == 0) continue;
+      done += all;
+      s_row[threadIdx.x] = row;
+      s_first[threadIdx.x] = first;
+      s_pages[threadIdx.x] = n;
+      s_used[threadIdx.x] = before;
+      __syncthreads();
+      if (cut) c.lengths[row] = to;
+      for (int j = threadIdx.x >> 5; j < min(nt, B - i0); j += nt >> 5)
+        for (int k = lane; k < s_pages[j]; k += 32) {
+          int32_t* e = c.table + (size_t)s_row[j] * c.width + s_first[j] + k;
+          const int at = n_free + total - 1 - s_used[j] - k;
+          if (at < c.pages) c.free[at] = *e;
+          *e = -1;
+        }
+      __syncthreads();
+    }
   }
   if (threadIdx.x == 0) *c.n_free = min(n_free + total, c.pages);
 }

@@ -38,17 +38,23 @@ struct KpShape {
   static constexpr int SMEM = 1024 + Q + KP_STAGES * (K + V) + RING + 512 + 6 * KP_ROWS * 4 + KP_EXPS * 4 * 2;
 };
 
-__device__ __forceinline__ bool kp_wait(uint64_t* bar, uint32_t parity, volatile int* fail, int* word, int code) {
-  if (mbar_try_wait(bar, parity)) return true;
-  for (uint32_t i = 0; i < AT_WAIT_LIMIT; ++i) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if ((i & 255u) == 255u && *fail) return false;
-  }
+__device__ __forceinline__ void kp_ran_out(volatile int* fail, int* word, int code) {
   *fail = 1;
   wait_ran_out(word, 810 + code);
-  return false;
 }
-
+// A wait that ends: on its phase, when another role has given up, or after the limit.
+__device__ __forceinline__ bool kp_wait(uint64_t* bar, uint32_t parity, volatile int* fail, int* word, int code) {
+#pragma unroll 1
+  for (uint32_t i = 0; !mbar_try_wait(bar, parity); ++i) {
+    if ((i & 255u) != 255u) continue;
+    if (*fail) return false;
+    if (i >= AT_WAIT_LIMIT) {
+      kp_ran_out(fail, word, code);
+      return false;
+    }
+  }
+  return true;
+}
 __host__ __device__ constexpr uint32_t instr_desc_f16(int M, int N) { return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24); }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }      // -126 <= e <= 127
 
@@ -82,6 +88,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
   const int R = a.H / a.G, cols_all = it.count * R, col0 = it.tile * KV4_MANY, cols = min(KV4_MANY, cols_all - col0);
   T* const y = (T*)a.y;
   if (it.row < 0) {                     // a refused sequence's tokens are no numbers
+#pragma unroll 1
     for (int e = threadIdx.x; e < cols * D; e += KP_THREADS) {
       const int c = col0 + e / D;
       dt<T>::st(y, ((size_t)(it.first + c / R) * a.H + head * R + c % R) * D + e % D, NAN);
@@ -163,6 +170,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(KP_REGS_DEQUANT));
     const int t4 = lane & 3, g8 = lane >> 2;
     bool ok = true;
+#pragma unroll 1
     for (int turn = 0; turn < turns; ++turn) {
       const int n = KP_SETS * turn + set, st = turn % KP_RING, ks = n % KP_STAGES;
       ok = __all_sync(0xffffffffu, kp_wait(&full[st], (turn / KP_RING) & 1, s_fail, a.word, 1));
@@ -265,7 +273,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
       __syncwarp();
       if (lane == 0) mbar_arrive(&v_full[ks]);
     }
-    if (!ok && lane == 0) let_issued_work_end();
+    if (!ok && lane == 0) kv4_let_end();
     __syncwarp();
   } else if (warp >= KP_SOFTMAX) {
     // ===================== MMA issuers, one thread per tile =====================
@@ -297,6 +305,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
       };
       bool ok = kp_wait(q_full, 0, s_fail, a.word, 5);
       if (ok && units > 0) ok = scores(0);
+#pragma unroll 1
       for (int n = 0; ok && n < units; ++n) {
         if (n + 1 < units && !(ok = scores(n + 1))) break;
         const int vs = n % KP_STAGES;
@@ -315,7 +324,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
           mbar_arrive(&v_empty[vs]);
         }
       }
-      if (!ok) let_issued_work_end();
+      if (!ok) kv4_let_end();
     }
     __syncwarp();
   } else {
@@ -389,6 +398,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
     int ebase = -128;                                                   // the power of two that O stands under
     bool ok = true;
     const int count = max(0, myhi - page0 + 1);
+#pragma unroll 1
     for (int n = 0; n < count; ++n) {
       const uint32_t ts = ts0 + 64u * (n & 1);
       ok = kp_wait(&s_full[2 * tile + (n & 1)], (n >> 1) & 1, s_fail, a.word, 8);

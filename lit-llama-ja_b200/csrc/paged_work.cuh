@@ -47,6 +47,11 @@ struct __align__(16) Kv4Join {
 };
 __host__ __device__ __forceinline__ const int4* joins_of(const int32_t* work, int max_items) { return reinterpret_cast<const int4*>(work) + 1 + 3 * (size_t)max_items; }
 
+// For a role that gives up: copies and products that it has issued end (a millisecond and more) before the block lets go of its memory.
+__device__ __forceinline__ void kv4_let_end() {
+  for (const long long from = clock64(); clock64() - from < 2000000;) __nanosleep(512);
+}
+
 // column -> token and head: a shift where the heads of a key head are 1, 2, 4 .., else a division
 __device__ __forceinline__ int column_token(int c, int R) { return (R & (R - 1)) == 0 ? c >> (31 - __clz(R)) : c / R; }
 __device__ __forceinline__ int column_head(int c, int R) { return (R & (R - 1)) == 0 ? c & (R - 1) : c % R; }
