@@ -66,8 +66,8 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
   // it, so that what waits for this kernel waits for both.)
   if (blockIdx.x == gridDim.x - 1) pdl_wait();
   const int item = blockIdx.x / a.G, head = blockIdx.x - item * a.G;
+  const Kv4Item it = load_item(a.work, item);                           // (there is room for it: asked for together with the number of parts)
   if (item >= a.work[0]) return;
-  const Kv4Item it = load_item(a.work, item);
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, R = a.H / a.G;
   const int first = it.first, n = it.count, row = it.row;
   const int col0 = it.tile * COLS, cols = min(COLS, n * R - col0);

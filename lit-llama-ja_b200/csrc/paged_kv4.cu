@@ -42,14 +42,15 @@ __device__ __forceinline__ V block_before(V v, V* s_warp, V& total) {
   __syncthreads();                     // (the sums of a scan before this one have been read)
   if (lane == 31) s_warp[warp] = incl;
   __syncthreads();
-  V before = V(0);
-  total = V(0);
-  for (int w = 0; w < (int)(blockDim.x >> 5); ++w) {
-    const V u = s_warp[w];
-    if (w < warp) before += u;
-    total += u;
+  V sums = lane < (int)(blockDim.x >> 5) ? s_warp[lane] : V(0);       // (every warp sums the warps' sums for itself)
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const V u = __shfl_up_sync(0xffffffffu, sums, d);
+    if (lane >= d) sums += u;
   }
-  return before + incl - v;
+  total = __shfl_sync(0xffffffffu, sums, 31);
+  const V before = __shfl_sync(0xffffffffu, sums, warp > 0 ? warp - 1 : 0);
+  return (warp > 0 ? before : V(0)) + incl - v;
 }
 
 __device__ __forceinline__ int pages_of(int tokens) { return (tokens + KV4_PAGE - 1) / KV4_PAGE; }
@@ -127,7 +128,7 @@ constexpr int PW_TRIES = 48;
 // themselves and stay whole.
 // MANY false: the sequences of up to `few` columns, whose tiles count as long as the last one; true: the others.
 template <bool MANY>
-__device__ __forceinline__ void divide_work(const PlanView& v, const PlanWork& d, int* s_count, int* s_size) {
+__device__ __forceinline__ void divide_work(const PlanView& v, const PlanWork& d, int* s_count, int* s_size, int2* s_walk) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   auto tokens = [&](int i) { return v.starts[i + 1] - v.starts[i]; };
   auto tiles = [&](int i) {
@@ -140,16 +141,23 @@ __device__ __forceinline__ void divide_work(const PlanView& v, const PlanWork& d
     const int n = tokens(i);
     return (v.ends[i] - n + (MANY ? min(n - 1, (int)(((uint32_t)(tile + 1) * (uint32_t)d.cols - 1) / (uint32_t)d.R)) : n - 1)) / KV4_PAGE + 1;
   };
-  // walks, by one warp
+  // tiles of the sequences, and pages of their last one, where the block can hold them; all walks
+  const bool held = v.B <= PLAN_HELD;
   __syncthreads();
-  if (warp == 0) {
-    int n = 0;
-    for (int i = lane; i < v.B; i += 32) n += tiles(i);
-    n = __reduce_add_sync(0xffffffffu, n);
-    if (lane == 0) s_count[0] = n;
+  if (threadIdx.x == 0) s_count[0] = 0;
+  __syncthreads();
+  for (int i0 = 0; i0 < v.B; i0 += blockDim.x) {
+    const int i = i0 + threadIdx.x, w = i < v.B ? tiles(i) : 0, n = __reduce_add_sync(0xffffffffu, w);
+    if (held && i < v.B) s_walk[i] = make_int2(w, w > 0 ? pages(i, w - 1) : 0);
+    if (lane == 0 && n > 0) atomicAdd(&s_count[0], n);
   }
   __syncthreads();
   const int walks = s_count[0];
+  auto walk_of = [&](int i) {
+    if (held) return s_walk[i];
+    const int w = tiles(i);
+    return make_int2(w, w > 0 ? pages(i, w - 1) : 0);
+  };
   if (walks == 0) {
     if (threadIdx.x == 0) d.work[0] = d.work[1] = 0;
     return;
@@ -164,14 +172,15 @@ __device__ __forceinline__ void divide_work(const PlanView& v, const PlanWork& d
         n += w * k, sum += w * p, most = max(most, each), least = min(least, each);
       };
       for (int i0 = 0; i0 < v.B; i0 += 32) {
-        const int w = i0 + lane < v.B ? tiles(i0 + lane) : 0;
+        const int2 wp = i0 + lane < v.B ? walk_of(i0 + lane) : make_int2(0, 0);
+        const int w = wp.x;
         if (MANY) {
           for (uint32_t with = __ballot_sync(0xffffffffu, w > 0); with != 0u; with &= with - 1) {
             const int l = __ffs(with) - 1, all = __shfl_sync(0xffffffffu, w, l);
             for (int t = lane; t < all; t += 32) add(1, pages(i0 + l, t));
           }
         } else if (w > 0) {
-          add(w, pages(i0 + lane, 0));
+          add(w, wp.y);
         }
       }
       n = __reduce_add_sync(0xffffffffu, n), sum = __reduce_add_sync(0xffffffffu, sum);
@@ -210,9 +219,10 @@ __device__ __forceinline__ void divide_work(const PlanView& v, const PlanWork& d
   if (threadIdx.x == 0) s_count[0] = 0;
   __syncthreads();
   for (int i = MANY ? warp : threadIdx.x; i < v.B; i += MANY ? warps : blockDim.x) {
-    const int w = tiles(i);
+    const int2 wp = walk_of(i);
+    const int w = wp.x;
     for (int t = MANY ? lane : 0; t < (MANY ? w : min(w, 1)); t += 32) {
-      const int p = pages(i, t), k = cut(p);
+      const int p = MANY ? pages(i, t) : wp.y, k = cut(p);
       atomicAdd(&s_size[bucket((p + k - 1) / k)], MANY ? k : w * k);
     }
   }
@@ -254,7 +264,7 @@ __device__ __forceinline__ void divide_work(const PlanView& v, const PlanWork& d
   };
   if (MANY) {
     for (int i = warp; i < v.B; i += warps) {
-      const int w = tiles(i);
+      const int w = walk_of(i).x;
       for (int t = lane; t < w; t += 32) {
         const int p = pages(i, t), k = cut(p), each = (p + k - 1) / k, at = atomicAdd(&s_size[bucket(each)], k);
         for (int e = 0; e < k; ++e) store(i, at + e, t, e, each, k, at);
@@ -262,11 +272,15 @@ __device__ __forceinline__ void divide_work(const PlanView& v, const PlanWork& d
       }
     }
   } else {      // a thread a sequence; its warp helps where there are more than four parts
-    for (int i0 = 32 * warp; i0 < v.B; i0 += 32 * warps) {
-      const int i = i0 + lane, w = i < v.B ? tiles(i) : 0;
+    // (sequences are dealt out, so that every warp has some)
+    const int per = min(32, (v.B + warps - 1) / warps);
+    for (int i0 = per * warp; i0 < v.B; i0 += per * warps) {
+      const int i = i0 + lane;
+      const int2 wp = lane < per && i < v.B ? walk_of(i) : make_int2(0, 0);
+      const int w = wp.x;
       int k = 0, each = 1, at = 0;
       if (w > 0) {
-        const int p = pages(i, 0);
+        const int p = wp.y;
         k = cut(p), each = (p + k - 1) / k;
         at = atomicAdd(&s_size[bucket(each)], w * k);
         if (w * k <= 4)
@@ -293,6 +307,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv4_plan_kernel(const int32_t* _
   __shared__ int s_row[PLAN_THREADS], s_first[PLAN_THREADS], s_pages[PLAN_THREADS], s_used[PLAN_THREADS];
   __shared__ int s_starts[PLAN_HELD + 1], s_ends[PLAN_HELD], s_request[PLAN_HELD];
   __shared__ __align__(16) int s_name[PLAN_NEAR];
+  __shared__ int2 s_walk[PLAN_HELD];
   const int n_free = min(max(*c.n_free, 0), c.pages), nt = blockDim.x, lane = threadIdx.x & 31;
   const bool held = B <= PLAN_HELD;
   claim_requests(rows, counts, false, B, c);
@@ -359,8 +374,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv4_plan_kernel(const int32_t* _
   __syncthreads();
   const PlanView v{held ? s_starts : p.starts, held ? s_ends : p.ends, held ? s_request : p.request, B};
   for (int t = threadIdx.x; t < min(T, here); t += nt) place_token(v, c, p, t);
-  divide_work<false>(v, few, s_need, s_size);
-  if (many.work != nullptr) divide_work<true>(v, many, s_need, s_size);
+  divide_work<false>(v, few, s_need, s_size, s_walk);
+  if (many.work != nullptr) divide_work<true>(v, many, s_need, s_size, s_walk);
 }
 
 // Positions and slots of a step's tokens from `here` on.
@@ -608,7 +623,7 @@ int ll_kv4_plan(const ll_kv4_cache* cache, const int32_t* rows, const int32_t* c
   const PlanWork few{l.R, l.few, l.cols, longest, l.few_parts, (int)l.few_items, l.few_joins(), 2.5f, 3.5f, l.few_cut, work};
   const PlanWork many{l.R, l.few, KV4_MANY, longest, l.many_parts, (int)l.many_items, l.many_joins(), 2.f, 5.5f, true, l.many ? work + l.few_ints() : nullptr};
   // The block itself places the tokens of a step while that takes it a few rounds; more are placed by a grid.
-  const int threads = B <= 256 && T <= 2048 ? 256 : PLAN_THREADS, here = T <= 8 * threads ? T : 0;
+  const int threads = B <= 16 && T <= 2048 ? 256 : B <= 256 && T <= 4096 ? 512 : PLAN_THREADS, here = T <= 8 * threads ? T : 0;
   cudaStream_t st = (cudaStream_t)stream;
   kv4_plan_kernel<<<1, threads, 0, st>>>(rows, counts, B, T, here, max_count, c, p, few, many);
   LL_LAUNCH_OK("kv4_plan_kernel");
@@ -622,7 +637,7 @@ int ll_kv4_plan(const ll_kv4_cache* cache, const int32_t* rows, const int32_t* c
 int ll_kv4_truncate(const ll_kv4_cache* cache, const int32_t* rows, const int32_t* keep, int B, ll_stream stream) {
   if (int r = check_cache(cache, "kv4_truncate")) return r;
   LL_CHECK_ARG(rows && keep && B > 0, "kv4_truncate: %d sequences", B);
-  kv4_truncate_kernel<<<1, B <= 256 ? 256 : PLAN_THREADS, 0, (cudaStream_t)stream>>>(rows, keep, B, pool_of(cache));
+  kv4_truncate_kernel<<<1, B <= 32 ? 256 : PLAN_THREADS, 0, (cudaStream_t)stream>>>(rows, keep, B, pool_of(cache));
   LL_LAUNCH_OK("kv4_truncate_kernel");
   return LL_OK;
 }

@@ -83,8 +83,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
   constexpr uint32_t TM_S = 0, TM_O = 256;            // per tile: two score buffers of 64 columns; 128 accumulator columns
   extern __shared__ __align__(1024) uint8_t smem[];
   const int item = blockIdx.x / a.G, head = blockIdx.x - item * a.G;
+  const Kv4Item it = load_item(a.work, item);                           // (there is room for it: asked for together with the number of parts)
   if (item >= a.work[0]) return;
-  const Kv4Item it = load_item(a.work, item);
   const int R = a.H / a.G, cols_all = it.count * R, col0 = it.tile * KV4_MANY, cols = min(KV4_MANY, cols_all - col0);
   T* const y = (T*)a.y;
   if (it.row < 0) {                     // a refused sequence's tokens are no numbers
