@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
   }
 
   float o[NB][KS][4];
-  float ref[NB][CPL], sum[NB][CPL], sumlo[NB][NG][CPL];      // references in units of log2
+  float ref[NB][CPL], sum[NB][CPL], sumlo[NB][NG][CPL];      // references in the products' units
   uint32_t ev[NG];                                           // exponents of the values' scales so far, as powers of two's bits
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
       gs[s / SPG] += (u.x + u.y) + (v.x + v.y);
     }
     // 2^24 of the codes and 2^(ex - 127 - 14) of the queries, times the scores' scale in units of log2
-    const float back = __uint_as_float((uint32_t)(ex - 14 + 24) << 23) * (a.scale * KF_LOG2E);
+    const float back = fmaxf(__uint_as_float((uint32_t)(ex - 14 + 24) << 23) * (a.scale * KF_LOG2E), 1.2e-38f);      // (not 0: masked scores are -inf)
 #pragma unroll
     for (int e = 0; e < CPL; ++e) kq[b][e] = __shfl_sync(0xffffffffu, back, 4 * (2 * t4 + e));
 #pragma unroll
@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
     for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int e = 0; e < CPL; ++e)
-        grow |= fmaxf(fmaxf(s[0][b][e], s[1][b][e]), fmaxf(s[2][b][e], s[3][b][e])) * kq[b][e] > ref[b][e] + KF_SLACK;
+        grow |= (fmaxf(fmaxf(s[0][b][e], s[1][b][e]), fmaxf(s[2][b][e], s[3][b][e])) - ref[b][e]) * kq[b][e] > KF_SLACK;
 #pragma unroll
     for (int g = 0; g < NG; ++g) grow |= fmaxf(fmaxf(pv[0][g].x, pv[1][g].x), fmaxf(pv[2][g].x, pv[3][g].x)) > 2.f * __uint_as_float(ev[g]);
     if (__any_sync(0xffffffffu, grow)) {
@@ -252,11 +252,11 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
         float f[2] = {1.f, 1.f};
 #pragma unroll
         for (int e = 0; e < CPL; ++e) {
-          float m = fmaxf(fmaxf(s[0][b][e], s[1][b][e]), fmaxf(s[2][b][e], s[3][b][e])) * kq[b][e];
+          float m = fmaxf(fmaxf(s[0][b][e], s[1][b][e]), fmaxf(s[2][b][e], s[3][b][e]));
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
           m = fmaxf(m, ref[b][e]);
-          f[e] = kf_exp2(ref[b][e] - m);
+          f[e] = kf_exp2((ref[b][e] - m) * kq[b][e]);
           ref[b][e] = m;
           sum[b][e] *= f[e];
 #pragma unroll
@@ -284,14 +284,14 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
         }
       }
     }
-    // weights
+    // weights (the difference first: of scores past 2^27 a product and a rounded one of the same numbers are too far apart)
 #pragma unroll
     for (int x = 0; x < 4; ++x)
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int e = 0; e < CPL; ++e) {
-          s[x][b][e] = kf_exp2(fmaf(s[x][b][e], kq[b][e], -ref[b][e]));
+          s[x][b][e] = kf_exp2((s[x][b][e] - ref[b][e]) * kq[b][e]);
           sum[b][e] += s[x][b][e];
         }
     // y += (p s) c, p lo: by groups, the scales brought under 4 by a power of two that only grows.  Of a word's nibbles 0 and 1 (2 and 3) the rows of
@@ -385,7 +385,7 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
-      for (int e = 0; e < CPL; ++e) s_ref[warp][8 * b + CPL * t4 + e] = ref[b][e], s_sum[warp][8 * b + CPL * t4 + e] = sum[b][e];
+      for (int e = 0; e < CPL; ++e) s_ref[warp][8 * b + CPL * t4 + e] = ref[b][e] == KV4_NONE ? KV4_NONE : ref[b][e] * kq[b][e], s_sum[warp][8 * b + CPL * t4 + e] = sum[b][e];
   __syncthreads();                      // every unit has been read: the rings hold the warps' sums now
   if (s_fail) return;
   pdl_launch_dependents();

@@ -588,7 +588,7 @@ int check_cache(const ll_kv4_cache* c, const char* who) {
   LL_CHECK_ARG(kv4_shape_ok(c->head_size, c->group), "%s: kv4 heads of %d in groups of %d (32, 64 or 128 each)", who, c->head_size, c->group);
   LL_CHECK_ARG(c->dtype == LL_BF16 || c->dtype == LL_F16, "%s: kv4 cache of type %d (bf16 or fp16)", who, c->dtype);
   LL_CHECK_ARG(c->table && c->lengths && c->free_pages && c->n_free && c->stamp && c->requests > 0 && c->width > 0 && c->pages > 0 && c->pages <= INT_MAX / KV4_PAGE &&
-                   c->max_length > 0 && (c->max_length - 1) / KV4_PAGE < c->width && c->kv_heads > 0 && c->kv_heads <= 65535 && c->heads > 0 && c->heads % c->kv_heads == 0,
+                   c->max_length > 0 && c->max_length <= (1 << 30) && (c->max_length - 1) / KV4_PAGE < c->width && c->kv_heads > 0 && c->kv_heads <= 65535 && c->heads > 0 && c->heads % c->kv_heads == 0,
                "%s: kv4 cache of %d requests of up to %d tokens in %d pages, %d heads over %d", who, c->requests, c->max_length, c->pages, c->heads, c->kv_heads);
   return LL_OK;
 }

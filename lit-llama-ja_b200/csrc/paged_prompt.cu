@@ -63,7 +63,7 @@ template <typename T>
 __device__ __forceinline__ int slice_exponent(uint32_t largest) {
   const float2 p = bits_pair<T>(largest);
   const int fl = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(p.y, 16.f * p.x))) >> 23) - 127;
-  return max(-112, min(112, ((fl + 6) >> 4) << 4));
+  return fl < -126 ? 0 : max(-112, min(112, ((fl + 6) >> 4) << 4));      // (zeros alone, as behind the last key: any will do)
 }
 __device__ __forceinline__ __half2 as_half2(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
 __device__ __forceinline__ uint32_t as_u32(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
           const int ex = min(max((int)(__float_as_uint(bits_pair<T>(big).x) >> 23), 15), 240);
           up = pow2(127 + 14 - ex), down = pow2(ex - 127 - 14);
         }
-        if (l == 0) s_mul[r] = down * (a.scale * AT_LOG2E);
+        if (l == 0) s_mul[r] = fmaxf(down * (a.scale * AT_LOG2E), 1.2e-38f);      // (not 0: masked scores are -inf)
         uint32_t h[4];
 #pragma unroll
         for (int z = 0; z < 4; ++z) {
@@ -397,6 +397,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
     float ref = -INFINITY, sum = 0.f;
     int ebase = -128;                                                   // the power of two that O stands under
     bool ok = true;
+    bool far = false;                                                   // a reference past 2^24: a product and a rounded one of the same numbers differ
     const int count = max(0, myhi - page0 + 1);
 #pragma unroll 1
     for (int n = 0; n < count; ++n) {
@@ -438,6 +439,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
         const int nbase = max(ebase, emax);
         const float g = ref == -INFINITY ? 0.f : at_exp2(ref - nref), f = g * pow2(max(ebase - nbase, -126));
         ref = nref;
+        far = __any_sync(0xffffffffu, fabsf(ref) > 16777216.f && ref != -INFINITY);
         ebase = nbase;
         sum *= g;
         if (n > 0) ok = kp_wait(&o_full[2 * tile + ((n - 1) & 1)], ((n - 1) >> 1) & 1, s_fail, a.word, 9);
@@ -464,7 +466,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
       const float sub = ref == -INFINITY ? 0.f : -ref;
       uint32_t ph[16];
       f2 part[2] = {f2_of(0.f, 0.f), f2_of(0.f, 0.f)};
-      if ((eks | evs) == 0u && ebase == 0) {                            // (as mostly)
+      if ((eks | evs) == 0u && ebase == 0 && !far) {                    // (as mostly)
         const f2 m2 = f2_of(mul, mul), s2 = f2_of(sub, sub);
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
@@ -479,7 +481,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const float mm = e < 8 ? mul0 : mul1, f = e < 8 ? f0 : f1;
-          const float p0 = at_exp2(fmaf(__uint_as_float(sr[2 * e]), mm, sub)), p1 = at_exp2(fmaf(__uint_as_float(sr[2 * e + 1]), mm, sub));
+          const float s0 = __uint_as_float(sr[2 * e]), s1 = __uint_as_float(sr[2 * e + 1]);      // (-inf: masked, whatever mm may have come to)
+          const float p0 = s0 == -INFINITY ? 0.f : at_exp2(__fadd_rn(__fmul_rn(s0, mm), sub)), p1 = s1 == -INFINITY ? 0.f : at_exp2(__fadd_rn(__fmul_rn(s1, mm), sub));
           part[e & 1] = f2_add(part[e & 1], f2_of(p0, p1));
           ph[e] = pair_bits<__half>(p0 * f, p1 * f);
         }

@@ -81,8 +81,10 @@ struct Kv4Lists {
     many_parts = std::max(1, kv4_sms() / G);
     // Where no request has more than KV4_WHOLE pages, walks are not cut, and there is nothing to join.
     few_cut = max_length > KV4_WHOLE * KV4_PAGE;
-    const long long each = many ? (KV4_FEW_MOST + cols - 1) / cols : T, seqs = std::min(B, std::max(T, 1));
-    few_items = std::min((long long)T * R / cols + seqs, seqs * each) + KV4_CUTS * few_parts;
+    // tiles: of n columns n / cols, and one more a sequence that is not a whole number of them; sequences of the few have KV4_FEW_MOST columns at most
+    // where the others go to the many (and refused ones, whose tokens count here too, may have any)
+    const long long seqs = std::min(B, std::max(T, 1)), tiles = (long long)T * R / cols + seqs;
+    few_items = (many ? std::min(tiles, seqs * ((KV4_FEW_MOST + cols - 1) / cols)) : tiles) + KV4_CUTS * few_parts;
     many_items = many ? (long long)T * R / KV4_MANY + std::min(seqs, (long long)T * R / KV4_FEW_MOST) + KV4_CUTS * many_parts : 0;
   }
   // walks in more than one part: every one has a part more than it would have whole

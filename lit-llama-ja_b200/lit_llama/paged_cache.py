@@ -100,7 +100,7 @@ class PagedCache4:
             raise ValueError(f"heads of {head_size} in groups of {group}: 32, 64 or 128 each, and no group larger than a head")
         if n_layer < 1 or n_kv_head < 1 or n_head % n_kv_head != 0 or n_head < 1:
             raise ValueError(f"{n_layer} layers of {n_head} heads over {n_kv_head}")
-        if min(pages, requests, max_length) < 1 or pages * self.PAGE > 2**31 - 1:
+        if min(pages, requests, max_length) < 1 or pages * self.PAGE > 2**31 - 1 or max_length > 2**30:
             raise ValueError(f"{pages} pages of {self.PAGE} slots for {requests} requests of up to {max_length} tokens")
         self.device = torch.device("cuda", torch.cuda.current_device() if device.index is None else device.index)
         self.n_layer, self.n_head, self.n_kv_head, self.head_size, self.group, self.dtype = n_layer, n_head, n_kv_head, head_size, group, dtype

@@ -463,3 +463,78 @@ def test_slices_of_unequal_size(counts):
     cache.truncate([0], held)
     plan = cache.plan([0], counts, counts[0], max_count=counts[0])
     _near(cache.attend(0, plan, q.to(DEV)), q, held_as(k, 32), held_as(v, 32), held, counts, dtype, D ** -0.5)
+
+
+@pytest.mark.parametrize("held, counts, H, G", [
+    ([1500], [1], 32, 1),                       # one token of as many columns as the few may have
+    ([700, 5], [1, 1], 40, 1),                  # more of them: tcgen05 for single tokens
+    ([200, 0, 64], [1, 7, 100], 9, 3),          # heads of a key head that are no power of two
+    ([30, 600], [11, 1], 9, 3),
+    ([4000], [40], 4, 4),                       # few queries over a long past: walks in many parts
+    ([2000, 1], [300, 1], 8, 8),
+])
+@torch.no_grad()
+def test_columns_of_any_number(held, counts, H, G):
+    cache, plan, q, k, v = _filled(held, counts, H, G, 64, 32, BF, seed=6)
+    _near(cache.attend(0, plan, q.to(DEV)), q, k, v, held, counts, BF, 0.125)
+
+
+@pytest.mark.parametrize("n, new", [(1500, 1), (300, 2), (300, 40)])
+@torch.no_grad()
+def test_many_sequences(n, new):
+    """More sequences than the planning block holds, or than look through the names before theirs."""
+    rng = random.Random(n)
+    held, counts = [rng.randrange(0, 90) for _ in range(n)], [rng.choice([0, 1, new]) for _ in range(n)]
+    cache, plan, q, k, v = _filled(held, counts, 2, 1, 32, 32, BF, seed=7)
+    _near(cache.attend(0, plan, q.to(DEV)), q, k, v, held, counts, BF, 32 ** -0.5)
+
+
+@torch.no_grad()
+def test_sequences_that_bring_more_than_was_said():
+    """Tokens of a sequence that is refused for its count come out as no numbers, however many they are."""
+    cache, plan, q, k, v = _filled([10, 20, 400], [1, 90, 1], 32, 1, 64, 32, BF)
+    rows = plan.request.tolist()
+    for most in (1, 2):
+        cache.truncate(rows, [10, 20, 400])
+        plan = cache.plan(rows, [1, 90, 1], 92, max_count=most)
+        assert plan.status.tolist() == [0, 2, 0]
+        y = cache.attend(0, plan, q.to(DEV))
+        assert y[1:91].isnan().all()
+        _near(y[:1], q[:1], k[:11], v[:11], [10], [1], BF, 0.125)
+
+
+@pytest.mark.parametrize("count", [1, 6, 90])
+@torch.no_grad()
+def test_queries_that_are_no_numbers(count):
+    """Such a query's output is none, the others' are as ever; large and small queries keep their 8 bits."""
+    cache, plan, q, k, v = _filled([150], [count], 4, 2, 64, 32, BF, loud=False)
+    q[count - 1, 3, 5] = math.inf
+    q[0, 1] *= 2.0 ** 40
+    q[0, 2] *= 2.0 ** -40
+    q[0, 0, 7] = math.nan
+    y = cache.attend(0, plan, q.to(DEV)).cpu()
+    assert y[count - 1, 3].isnan().all() and y[0, 0].isnan().all()
+    want = attention(q[:1, 2:3], k[:151, 1:], v[:151, 1:], 150, 0.125)[0]
+    assert float((y[0, 2].double() - want[0, 0]).abs().max()) <= 2.0 ** -6
+    # scores 2^40 apart: the largest key's value alone
+    s = (q[0, 1].double() * k[:151, 0]).sum(-1)
+    assert float((y[0, 1].double() - v[int(s.argmax()), 0]).abs().max()) <= 2.0 ** -7 * float(v.abs().max())
+    if count > 1:
+        rest = y.clone()
+        rest[count - 1, 3] = 0
+        rest[0, 0] = 0
+        assert not rest.isnan().any()
+
+
+@pytest.mark.parametrize("scale", [0.125, 1e-30])
+@pytest.mark.parametrize("count", [1, 5, 100])
+@torch.no_grad()
+def test_queries_of_zeros_and_scales_of_nearly_nothing(count, scale):
+    """All keys in sight weigh the same: the mean of their values."""
+    cache, plan, q, k, v = _filled([70], [count], 2, 2, 64, 64, BF, loud=False)
+    q[0] = 0
+    y = cache.attend(0, plan, q.to(DEV), scale=scale).double().cpu()
+    rows = range(1) if scale > 1e-20 else range(count)
+    for r in rows:
+        want = v[:71 + r].mean(0)
+        assert float((y[r] - want).abs().max()) <= 2.0 ** -8 * float(want.abs().max()) + 2.0 ** -11 * float(v.abs().max())

@@ -25,6 +25,7 @@ ONE = dict(pages=4, requests=2, max_length=100)
     ((1, 4, 64), dict(ONE, requests=0), ValueError),
     ((1, 4, 64), dict(ONE, max_length=0), ValueError),
     ((1, 4, 64), dict(ONE, pages=1 << 25), ValueError),
+    ((1, 4, 64), dict(ONE, max_length=(1 << 30) + 1), ValueError),
 ])
 def test_refused_shapes(args, kind, error):
     with pytest.raises(error):
@@ -55,6 +56,7 @@ def _with(args, **at):
     ("ll_kv4_plan", {}, _with(PLAN, a3=1 << 30)),
     ("ll_kv4_plan", dict(max_length=65), PLAN),                   # a table too narrow for the longest request
     ("ll_kv4_plan", dict(pages=1 << 25), PLAN),
+    ("ll_kv4_plan", dict(max_length=(1 << 30) + 64, width=1 << 25), PLAN),
     ("ll_kv4_plan", dict(table=0), PLAN),
     ("ll_kv4_truncate", {}, (A, 0, 1, 0)),
     ("ll_kv4_truncate", dict(requests=0), (A, A, 1, 0)),
