@@ -1,5 +1,8 @@
 // The paged key/value cache in 4 bits: which pages and slots a step's tokens get, how they give them back, and the rounding of keys and values into
-// their slots.  Layout: kv4.cuh; the attention that reads it: paged_attn.cu.
+// their slots.  Layout: kv4.cuh; the attention that reads it: paged_attn.cu, paged_prompt.cu.
+//
+// A plan is a chain of dependent loads, sums and stores of one block: 64 requests 11 us, with the division of the step's attention (4 of them), 200 prompts of
+// 182 000 tokens 36 and 5 for the tokens' grid.  It is made once a step and serves all layers.
 #include <climits>
 
 #include "paged_work.cuh"
