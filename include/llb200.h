@@ -857,7 +857,7 @@ LL_API size_t ll_kv4_page_bytes(int head_size, int group);
  * max_count tokens; 3 no such request, or one that an earlier sequence names, or a negative count; 4 tokens behind row T.  A sequence that is refused
  * gets nothing.  out: starts [B + 1] (up to T), ends [B] (tokens held after the step; 0 refused), status [B], request [B] (-1: refused, or no
  * tokens), positions [T], slots [T] (page * 64 + place; -1: refused, or behind the last token).  work: the division of the step's attention among blocks,
- * the same for every layer; ll_kv4_work_ints numbers on a 16-byte boundary.  One step at a time plans, truncates and appends on a cache. */
+ * the same for every layer; ll_kv4_work_ints numbers (0: no such step) on a 16-byte boundary.  One step at a time plans, truncates and appends on a cache. */
 LL_API size_t ll_kv4_work_ints(const ll_kv4_cache* cache, int B, int T, int max_count);
 LL_API int ll_kv4_plan(const ll_kv4_cache* cache, const int32_t* rows, const int32_t* counts, int B, int T, int max_count, int32_t* out, int32_t* work,
                        ll_stream stream);

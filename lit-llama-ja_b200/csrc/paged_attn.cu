@@ -526,6 +526,7 @@ using namespace llb;
 extern "C" {
 
 size_t ll_kv4_attn_scratch_bytes(const ll_kv4_cache* cache, int B, int T, int max_count) {
+  if (!kv4_step_ok(cache, B, T, max_count)) return 0;
   return sizeof(float) * Kv4Lists(B, T, max_count, cache->heads, cache->kv_heads, cache->max_length).floats(cache->kv_heads, cache->head_size);
 }
 

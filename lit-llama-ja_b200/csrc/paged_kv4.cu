@@ -609,6 +609,7 @@ extern "C" {
 size_t ll_kv4_page_bytes(int head_size, int group) { return kv4_shape_ok(head_size, group) ? (size_t)kv4_bytes(head_size, head_size / group) : 0; }
 
 size_t ll_kv4_work_ints(const ll_kv4_cache* cache, int B, int T, int max_count) {
+  if (!kv4_step_ok(cache, B, T, max_count)) return 0;
   return Kv4Lists(B, T, max_count, cache->heads, cache->kv_heads, cache->max_length).ints();
 }
 

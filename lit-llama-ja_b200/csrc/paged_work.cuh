@@ -70,6 +70,12 @@ constexpr int KV4_ROUNDS = 3, KV4_CUTS = 2;
 inline bool kv4_many(int max_count, int R) { return (long long)max_count * R > KV4_FEW_MOST; }
 inline int kv4_sms() { return sm_count() > 0 ? sm_count() : 148; }
 
+// whether a step's lists have a size
+inline bool kv4_step_ok(const ll_kv4_cache* c, int B, int T, int max_count) {
+  return c != nullptr && c->kv_heads > 0 && c->heads > 0 && c->heads % c->kv_heads == 0 && c->max_length > 0 && B > 0 && T >= 0 && max_count >= 0 &&
+         (long long)T * c->heads <= INT_MAX;
+}
+
 // A step's two lists: sequences of few columns and, where one may bring more, of many.  Sizes as the host knows them.
 struct Kv4Lists {
   int R, cols, few, few_parts, many_parts;

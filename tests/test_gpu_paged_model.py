@@ -110,6 +110,25 @@ def test_generate_batch(quantize):
 
 
 @torch.no_grad()
+def test_generate_batch_of_int4_weights(golden):
+    """Weights in 4 bits too: rows of a step through the modules that single tokens, batches and prompts take."""
+    from generate import generate_batch
+    from tests.test_gpu_model import build_q_model
+
+    m = build_q_model(golden["model_tiny"], "rtn32bf16.", BF)
+    prompts = [torch.randint(0, 100, (n,), device=DEV) for n in (20, 1, 33)]
+    out = generate_batch(m, prompts, 8, top_k=1)
+    assert [len(o) for o in out] == [len(p) + 8 for p in prompts]
+    cache = m.paged_cache(pages=6, requests=3)
+    n = [len(o) - 1 for o in out]
+    logits = m.forward_paged(torch.cat([o[:-1] for o in out]), cache, cache.plan(range(3), n, sum(n)), all_rows=True).float()
+    slack = 4 * 2.0 ** -8 * float(logits.abs().max())
+    for part, o, p in zip(logits.split(n), out, prompts):
+        part = part[len(p) - 1:]
+        assert bool((part.gather(1, o[len(p):, None])[:, 0] >= part.max(1).values - slack).all())
+
+
+@torch.no_grad()
 def test_generate_batch_ends_at_eos():
     """Sequences that meet the end token stop before it and no longer change; the others go on."""
     from generate import generate_batch

@@ -82,6 +82,17 @@ def test_refused_calls(name, cache, args):
         N.call(name, ctypes.addressof(c), *args)
 
 
+def test_sizes_of_steps_that_are_none():
+    """No division by the heads that are not there, no sizes of nothing."""
+    for name in ("ll_kv4_work_ints", "ll_kv4_attn_scratch_bytes"):
+        assert N.call_ret(name, ctypes.addressof(_struct()), 2, 5, 5) > 0
+        assert N.call_ret(name, None, 1, 1, 1) == 0
+        for other in (dict(kv_heads=0), dict(heads=0), dict(heads=3), dict(kv_heads=-1), dict(max_length=0)):
+            assert N.call_ret(name, ctypes.addressof(_struct(**other)), 1, 1, 1) == 0
+        for step in ((0, 1, 1), (1, -1, 1), (1, 1, -1), (1, 1 << 30, 1)):
+            assert N.call_ret(name, ctypes.addressof(_struct()), *step) == 0
+
+
 def test_no_cache():
     for name, args in (("ll_kv4_plan", PLAN), ("ll_kv4_truncate", (A, A, 1, 0)), ("ll_kv4_append", APPEND), ("ll_kv4_read", READ), ("ll_kv4_attn", ATTN)):
         with pytest.raises(RuntimeError, match="no cache"):
