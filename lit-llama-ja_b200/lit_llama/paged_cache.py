@@ -27,6 +27,7 @@ import torch
 from . import _native as N
 
 _NOTHING = contextlib.nullcontext()
+_current_device = N._current_device or torch.cuda.current_device
 
 Whole = Union[torch.Tensor, Sequence[int]]
 
@@ -42,14 +43,15 @@ class CachePlan:
     def __init__(self, cache: "PagedCache4", B: int, T: int, max_count: int):
         self.cache, self.B, self.T, self.max_count, self.step = cache, B, T, max_count, cache._step
         work, self.scratch_bytes = cache._sizes(B, T, max_count)
-        self._data = torch.empty(work + 4 * B + 1 + 2 * T, dtype=torch.int32, device=cache.device)
+        self._data, self._first = cache.lengths.new_empty(work + 4 * B + 1 + 2 * T), work
         self._work = N.ptr(self._data)
         self._out = self._work + 4 * work
         self._positions = self._out + 4 * (4 * B + 1)
         self._slots = self._positions + 4 * T
 
     def _part(self, first: int, n: int) -> torch.Tensor:
-        return self._data.narrow(0, (self._out - self._work) // 4 + first, n)
+        first += self._first
+        return self._data[first:first + n]
 
     @property
     def starts(self) -> torch.Tensor:
@@ -103,6 +105,7 @@ class PagedCache4:
         if min(pages, requests, max_length) < 1 or pages * self.PAGE > 2**31 - 1 or max_length > 2**30:
             raise ValueError(f"{pages} pages of {self.PAGE} slots for {requests} requests of up to {max_length} tokens")
         self.device = torch.device("cuda", torch.cuda.current_device() if device.index is None else device.index)
+        self._index = self.device.index
         self.n_layer, self.n_head, self.n_kv_head, self.head_size, self.group, self.dtype = n_layer, n_head, n_kv_head, head_size, group, dtype
         self.pages, self.requests, self.max_length, self.width = pages, requests, max_length, -(-max_length // self.PAGE)
         i32 = dict(dtype=torch.int32, device=self.device)
@@ -132,13 +135,13 @@ class PagedCache4:
 
     def _here(self):
         """The cache's device as the current one, whose current stream the kernels go to."""
-        return _NOTHING if torch.cuda.current_device() == self.device.index else torch.cuda.device(self.device)
+        return _NOTHING if _current_device() == self._index else torch.cuda.device(self.device)
 
     # ------------------------------------------------------------------ pages and slots
     def _whole(self, name: str, x: Whole) -> torch.Tensor:
         if not isinstance(x, torch.Tensor):
             x = torch.tensor(list(x), dtype=torch.int32, device=self.device)
-        if x.dim() != 1 or x.dtype is not torch.int32 or x.get_device() != self.device.index:
+        if x.dim() != 1 or x.dtype is not torch.int32 or x.get_device() != self._index:
             raise RuntimeError(f"{name}: int32 numbers on {self.device}, one for each sequence, not {x.dtype} {tuple(x.shape)} on {x.device}")
         return x.contiguous()
 
@@ -187,7 +190,7 @@ class PagedCache4:
     def _rows(self, name: str, x: torch.Tensor, T: int, heads: int) -> torch.Tensor:
         """Rows as the kernels take them: the heads of a token one after the other, tokens at any distance, 16-byte boundaries."""
         D = self.head_size
-        if x.shape != (T, heads, D) or x.dtype is not self.dtype or x.get_device() != self.device.index:
+        if x.shape != (T, heads, D) or x.dtype is not self.dtype or x.get_device() != self._index:
             raise RuntimeError(f"{name}: {x.dtype} {tuple(x.shape)} on {x.device}, and the cache takes {self.dtype} {(T, heads, D)} on {self.device}")
         if x.requires_grad and torch.is_grad_enabled():
             raise RuntimeError(f"{name}: the 4-bit cache has no gradient")
@@ -207,12 +210,12 @@ class PagedCache4:
             if q is None:
                 raise RuntimeError("queries have to be turned with their keys")
             q = self._rows("q", q, T, self.n_head)
-            if rope.dtype != torch.float32 or rope.dim() != 3 or rope.shape[1:] != (self.head_size // 2, 2) or not rope.is_contiguous() \
-                    or rope.device != self.device or rope.data_ptr() % 16 != 0:
+            if rope.dtype is not torch.float32 or rope.dim() != 3 or rope.shape != (rope.shape[0], self.head_size // 2, 2) or not rope.is_contiguous() \
+                    or rope.get_device() != self._index or rope.data_ptr() % 16 != 0:
                 raise RuntimeError(f"rope: {rope.dtype} {tuple(rope.shape)} on {rope.device}, and the cache takes dense float32 [positions, {self.head_size // 2}, 2]")
             if rope.shape[0] < self.max_length:
                 raise RuntimeError(f"rope: {rope.shape[0]} positions, and requests may have {self.max_length}")
-            out = torch.empty((T, self.n_head, self.head_size), dtype=self.dtype, device=self.device)
+            out = q.new_empty(T, self.n_head, self.head_size)
         if T == 0:
             return out
         with self._here():
@@ -229,10 +232,11 @@ class PagedCache4:
         if not 0 <= layer < self.n_layer:
             raise RuntimeError(f"layer {layer} of {self.n_layer}")
         slots = self._whole("slots", slots)
-        k, v = torch.empty((2, slots.numel(), self.n_kv_head, self.head_size), dtype=self.dtype, device=self.device).unbind(0)
-        if slots.numel():
+        n = slots.numel()
+        k, v = (torch.empty((n, self.n_kv_head, self.head_size), dtype=self.dtype, device=self.device) for _ in range(2))
+        if n:
             with self._here():
-                N.call("ll_kv4_read", self._c, self._layers[layer], N.ptr(slots), N.ptr(k), N.ptr(v), slots.numel(), N.stream())
+                N.call("ll_kv4_read", self._c, self._layers[layer], N.ptr(slots), N.ptr(k), N.ptr(v), n, N.stream())
         return k, v
 
     def attend(self, layer: int, plan: CachePlan, q: torch.Tensor, scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -242,7 +246,7 @@ class PagedCache4:
         T = plan.T
         q = self._rows("q", q, T, self.n_head)
         if out is None:
-            out = torch.empty((T, self.n_head, self.head_size), dtype=self.dtype, device=self.device)
+            out = q.new_empty(T, self.n_head, self.head_size)
         elif out.shape != q.shape or out.dtype != self.dtype or out.device != self.device or not out.is_contiguous() or out.data_ptr() % 16 != 0:
             raise RuntimeError(f"out: dense {self.dtype} {tuple(q.shape)} on {self.device}, not {out.dtype} {tuple(out.shape)} on {out.device}")
         scale = self.head_size ** -0.5 if scale is None else float(scale)
@@ -251,6 +255,6 @@ class PagedCache4:
         if T == 0:
             return out
         with self._here():
-            scratch = torch.empty(plan.scratch_bytes, dtype=torch.uint8, device=self.device)
+            scratch = self.blocks.new_empty(plan.scratch_bytes)
             N.call("ll_kv4_attn", self._c, self._layers[layer], N.ptr(q), q.stride(0), plan._work, N.ptr(out), plan.B, T, plan.max_count, scale, N.ptr(scratch), N.stream())
         return out
