@@ -447,36 +447,48 @@ template <typename T> __device__ __forceinline__ uint32_t min_bits(uint32_t a, u
 // A vector (a head of a token's queries, keys or values) takes D / 8 lanes of eight numbers each, a warp the same head of 32 / (D / 8) tokens one after
 // the other.  Bound by its instructions, not by memory: so the smallest and largest are found in pairs ({x, -x}: one minimum for both), a code comes from
 // a product with 1 / s, and only where that lies so near to the middle of two codes that its error could matter (1e-4; its error is below 4e-6) from the quotient.
+constexpr int APPEND_HEADS = 4;
 template <typename T, int D, int NG, bool TURN>
 __global__ void __launch_bounds__(256) kv4_append_kernel(Kv4Rows in, const float* __restrict__ rope, const int32_t* __restrict__ positions,
                                                          const int32_t* __restrict__ slots, T* __restrict__ q_out, uint8_t* __restrict__ blocks, int Tn, int H, int G) {
   constexpr int LV = D / 8, TOKENS = 32 / LV, GL = LV / NG, W = D / 32;
-  const int lane = threadIdx.x & 31, l = lane % LV, t = blockIdx.x * TOKENS + lane / LV, vec = blockIdx.y * 8 + (threadIdx.x >> 5);
-  const int nq = TURN ? H : 0;
-  if (vec >= nq + 2 * G) return;
-  const bool live = t < Tn;
-  const int slot = live ? slots[t] : -1, pos = live ? positions[t] : -1;
-  const bool is_q = vec < nq, is_k = !is_q && vec < nq + G;
-  const int head = is_q ? vec : is_k ? vec - nq : vec - nq - G;
-  const T* row = is_q ? (const T*)in.q + t * in.q_row : is_k ? (const T*)in.k + t * in.k_row : (const T*)in.v + t * in.v_row;
-  uint4 u = live ? *reinterpret_cast<const uint4*>(row + head * D + 8 * l) : make_uint4(0u, 0u, 0u, 0u);
-  uint32_t w[4] = {u.x, u.y, u.z, u.w};
-  if (TURN && (is_q || is_k)) {
+  const int lane = threadIdx.x & 31, l = lane % LV, t = blockIdx.x * TOKENS + lane / LV, unit = blockIdx.y * 8 + (threadIdx.x >> 5);
+  const int turned = TURN ? (H + APPEND_HEADS - 1) / APPEND_HEADS : 0, vec = unit - turned;
+  if (vec >= 2 * G) return;
+  const bool live = t < Tn, is_q = vec < 0, is_k = vec < G;
+  const int pos = live ? positions[t] : -1, slot = live && !is_q ? slots[t] : -1;
+  float c[8];
+  if (TURN && is_k) {
     const float4* cs = reinterpret_cast<const float4*>(rope + (size_t)max(pos, 0) * D + 8 * l);
     const float4 c0 = __ldg(cs), c1 = __ldg(cs + 1);
-    const float c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 f = bits_pair<T>(w[j]);
-      w[j] = pair_bits<T>(__fsub_rn(__fmul_rn(f.x, c[2 * j]), __fmul_rn(f.y, c[2 * j + 1])), __fadd_rn(__fmul_rn(f.y, c[2 * j]), __fmul_rn(f.x, c[2 * j + 1])));
-    }
+    c[0] = c0.x, c[1] = c0.y, c[2] = c0.z, c[3] = c0.w, c[4] = c1.x, c[5] = c1.y, c[6] = c1.z, c[7] = c1.w;
   }
-  if (is_q) {
-    if (live) {
-      if (pos < 0) w[0] = w[1] = w[2] = w[3] = pair_bits<T>(NAN, NAN);
-      *reinterpret_cast<uint4*>(q_out + ((size_t)t * H + head) * D + 8 * l) = make_uint4(w[0], w[1], w[2], w[3]);
+  auto turn = [&](uint32_t x, int j) {
+    const float2 f = bits_pair<T>(x);
+    return pair_bits<T>(__fsub_rn(__fmul_rn(f.x, c[2 * j]), __fmul_rn(f.y, c[2 * j + 1])), __fadd_rn(__fmul_rn(f.y, c[2 * j]), __fmul_rn(f.x, c[2 * j + 1])));
+  };
+  if (TURN && is_q) {
+    const int h0 = unit * APPEND_HEADS;
+    const T* row = (const T*)in.q + t * in.q_row + h0 * D + 8 * l;
+    T* to = q_out + ((size_t)t * H + h0) * D + 8 * l;
+    uint4 u[APPEND_HEADS];
+#pragma unroll
+    for (int h = 0; h < APPEND_HEADS; ++h) u[h] = live && h0 + h < H ? *reinterpret_cast<const uint4*>(row + h * D) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+    for (int h = 0; h < APPEND_HEADS; ++h) {
+      uint4 x = make_uint4(turn(u[h].x, 0), turn(u[h].y, 1), turn(u[h].z, 2), turn(u[h].w, 3));
+      if (pos < 0) x.x = x.y = x.z = x.w = pair_bits<T>(NAN, NAN);
+      if (live && h0 + h < H) *reinterpret_cast<uint4*>(to + h * D) = x;
     }
     return;
+  }
+  const int head = is_k ? vec : vec - G;
+  const T* row = (is_k ? (const T*)in.k + t * in.k_row : (const T*)in.v + t * in.v_row) + head * D + 8 * l;
+  const uint4 u = live ? *reinterpret_cast<const uint4*>(row) : make_uint4(0u, 0u, 0u, 0u);
+  uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  if (TURN && is_k) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = turn(w[j], j);
   }
   // smallest and largest of a group: {lo, -hi}
   uint32_t low = min_bits<T>(min_bits<T>(w[0], w[1]), min_bits<T>(w[2], w[3]));
@@ -552,37 +564,69 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(Kv4Rows in, const float
   }
 }
 
-// The values that slots stand for: a warp a slot and head.
+// The values that slots stand for: a warp a head of read_slots(D) slots, keys by a word (eight numbers) a lane, values by four numbers a lane that lie
+// side by side, whose codes are in four chunks: loads of two bytes (from L1) and a store of eight, instead of a load and four stores of two.
+constexpr int read_slots(int D) { return 512 / D; }
+// a code as a number: integers are converted at an eighth of an addition's rate
+__device__ __forceinline__ float code_value(uint32_t code, float2 p) {
+  return __fadd_rn(__fmul_rn(__uint_as_float(0x4b000000u | (code & 15u)) - 8388608.f, p.x), p.y);
+}
 template <typename T, int D, int NG>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const uint8_t* __restrict__ blocks, const int32_t* __restrict__ slots, T* __restrict__ k_out,
                                                        T* __restrict__ v_out, int n, int G, int pages) {
-  constexpr int W = D / 32;
+  constexpr int W = D / 32, LK = 4 * W, LV = 8 * W, SLOTS = read_slots(D), KR = SLOTS * LK / 32, VR = SLOTS * LV / 32;
   const int lane = threadIdx.x & 31;
-  const long long vec = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (vec >= (long long)n * G) return;
-  const int t = (int)(vec / G), head = (int)(vec - (long long)t * G), slot = slots[t];
-  const bool there = slot >= 0 && slot < pages * KV4_PAGE;
-  const uint8_t* blk = blocks + ((size_t)((there ? slot : 0) / KV4_PAGE) * G + head) * kv4_bytes(D, NG) + (there ? slot : 0) % KV4_PAGE / KV4_SLICE * kv4_slice_bytes(D, NG);
-  const int at = (there ? slot : 0) % KV4_SLICE;
-  T* ko = k_out + vec * D;
-  T* vo = v_out + vec * D;
-  auto value = [&](uint32_t c, float2 p) { return there ? __fadd_rn(__fmul_rn((float)c, p.x), p.y) : NAN; };
-  if (lane < 4 * W) {                  // keys: word i of chunk c, eight dimensions
-    const int c = lane / W, i = lane % W;
-    const uint32_t w = reinterpret_cast<const uint32_t*>(blk)[at * (D / 8) + lane];
-    const float2 p = bits_pair<T>(reinterpret_cast<const uint32_t*>(blk + kv4_k_params(D))[at * NG + i * NG / W]);
+  const long long vec = (long long)blockIdx.x * 8 + (threadIdx.x >> 5), t0 = vec / G * SLOTS;
+  if (t0 >= n) return;
+  const int head = (int)(vec % G), mine = lane < SLOTS && t0 + lane < n ? slots[t0 + lane] : -1;
+  uint32_t kw[KR], vw[VR];
+  float2 kp[KR], vp[VR];
+  auto slice = [&](int slot) {
+    return blocks + ((size_t)(slot / KV4_PAGE) * G + head) * kv4_bytes(D, NG) + slot % KV4_PAGE / KV4_SLICE * kv4_slice_bytes(D, NG);
+  };
+  auto params = [&](const uint8_t* at, bool there) { return there ? bits_pair<T>(*reinterpret_cast<const uint32_t*>(at)) : make_float2(NAN, NAN); };
+  const int kl = lane % LK, ki = kl % W, kc = kl / W;              // keys: word ki of chunk kc, eight dimensions
+  const int vl = lane % LV, vi = vl >> 3, vg = 4 * (vl & 1), vm = (vl >> 1) & 3;      // values: nibble vm of word vi of chunks vg .. vg + 3
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-      *reinterpret_cast<uint2*>(ko + 32 * i + 16 * h + 4 * c) =
-          make_uint2(pair_bits<T>(value(w >> (8 * h) & 15u, p), value(w >> (8 * h + 16) & 15u, p)),
-                     pair_bits<T>(value(w >> (8 * h + 4) & 15u, p), value(w >> (8 * h + 20) & 15u, p)));
+  for (int r = 0; r < KR; ++r) {
+    int slot = __shfl_sync(0xffffffffu, mine, r * (32 / LK) + lane / LK);
+    const bool there = slot >= 0 && slot < pages * KV4_PAGE;
+    slot = there ? slot : 0;
+    const uint8_t* s = slice(slot);
+    kw[r] = reinterpret_cast<const uint32_t*>(s)[slot % KV4_SLICE * (D / 8) + kl];
+    kp[r] = params(s + kv4_k_params(D) + 4 * (slot % KV4_SLICE * NG + ki * NG / W), there);
   }
-  if (lane < 8 * W) {                  // values: a slot's half of word i of chunk g, four dimensions
-    const int i = lane >> 3, g = lane & 7;
-    const uint32_t w = reinterpret_cast<const uint16_t*>(blk + kv4_v_codes(D))[(at / 2) * (D / 2) + (g * W + i) * 2 + (at & 1)];
-    const float2 p = bits_pair<T>(reinterpret_cast<const uint32_t*>(blk + kv4_v_params(D, NG))[at * NG + i * NG / W]);
 #pragma unroll
-    for (int m = 0; m < 4; ++m) dt<T>::st(vo, 32 * i + 8 * m + g, value(w >> (4 * m) & 15u, p));
+  for (int r = 0; r < VR; ++r) {
+    int slot = __shfl_sync(0xffffffffu, mine, r * (32 / LV) + lane / LV);
+    const bool there = slot >= 0 && slot < pages * KV4_PAGE;
+    slot = there ? slot : 0;
+    const uint8_t* s = slice(slot);
+    const int at = slot % KV4_SLICE;
+    const uint16_t* c = reinterpret_cast<const uint16_t*>(s + kv4_v_codes(D)) + (at / 2) * (D / 2) + (vg * W + vi) * 2 + (at & 1);
+    vw[r] = 0;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) vw[r] |= ((uint32_t)c[2 * g * W] >> (4 * vm) & 15u) << (8 * g);
+    vp[r] = params(s + kv4_v_params(D, NG) + 4 * (at * NG + vi * NG / W), there);
+  }
+#pragma unroll
+  for (int r = 0; r < KR; ++r) {
+    const long long t = t0 + r * (32 / LK) + lane / LK;
+    if (t >= n) continue;
+    T* to = k_out + (t * G + head) * D + 32 * ki + 4 * kc;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t w = kw[r] >> (8 * h);
+      *reinterpret_cast<uint2*>(to + 16 * h) = make_uint2(pair_bits<T>(code_value(w, kp[r]), code_value(w >> 16, kp[r])),
+                                                          pair_bits<T>(code_value(w >> 4, kp[r]), code_value(w >> 20, kp[r])));
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < VR; ++r) {
+    const long long t = t0 + r * (32 / LV) + lane / LV;
+    if (t >= n) continue;
+    *reinterpret_cast<uint2*>(v_out + (t * G + head) * D + 4 * vl) = make_uint2(pair_bits<T>(code_value(vw[r], vp[r]), code_value(vw[r] >> 8, vp[r])),
+                                                                               pair_bits<T>(code_value(vw[r] >> 16, vp[r]), code_value(vw[r] >> 24, vp[r])));
   }
 }
 
@@ -654,7 +698,7 @@ int ll_kv4_append(const ll_kv4_cache* cache, void* blocks, const void* q, long l
   const uintptr_t a = (uintptr_t)(rope ? q : nullptr) | (uintptr_t)k | (uintptr_t)v | (uintptr_t)rope | (uintptr_t)(rope ? q_out : nullptr) | (uintptr_t)blocks;
   LL_CHECK_ARG((a & 15) == 0 && ((rope ? q_row : 0) | k_row | v_row) % 8 == 0, "kv4_append: rows have to start on 16-byte boundaries");
   const Kv4Rows in{q, k, v, q_row, k_row, v_row};
-  const int tokens = 256 / cache->head_size, vecs = ((rope ? H : 0) + 2 * G + 7) / 8;
+  const int tokens = 256 / cache->head_size, vecs = ((rope ? (H + APPEND_HEADS - 1) / APPEND_HEADS : 0) + 2 * G + 7) / 8;
   LL_CHECK_ARG(vecs <= 65535, "kv4_append: %d heads, %d cached", H, G);
   cudaStream_t st = (cudaStream_t)stream;
   const dim3 grid((T + tokens - 1) / tokens, vecs);
@@ -674,7 +718,8 @@ int ll_kv4_append(const ll_kv4_cache* cache, void* blocks, const void* q, long l
 int ll_kv4_read(const ll_kv4_cache* cache, const void* blocks, const int32_t* slots, void* k, void* v, int n, ll_stream stream) {
   if (int r = check_cache(cache, "kv4_read")) return r;
   LL_CHECK_ARG(blocks && slots && k && v && n > 0, "kv4_read: %d slots", n);
-  const long long grid = ((long long)n * cache->kv_heads + 7) / 8;
+  const int at_once = read_slots(cache->head_size);
+  const long long grid = (((long long)n + at_once - 1) / at_once * cache->kv_heads + 7) / 8;
   LL_CHECK_ARG(grid <= INT_MAX, "kv4_read: %d slots of %d heads", n, cache->kv_heads);
   cudaStream_t st = (cudaStream_t)stream;
 #define READ_AS(TT, DD, NG) \
