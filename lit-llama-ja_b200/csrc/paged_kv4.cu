@@ -444,9 +444,12 @@ template <typename T> __device__ __forceinline__ uint32_t min_bits(uint32_t a, u
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// A vector (a head of a token's queries, keys or values) takes D / 8 lanes of eight numbers each, a warp the same head of 32 / (D / 8) tokens one after
-// the other.  Bound by its instructions, not by memory: so the smallest and largest are found in pairs ({x, -x}: one minimum for both), a code comes from
-// a product with 1 / s, and only where that lies so near to the middle of two codes that its error could matter (1e-4; its error is below 4e-6) from the quotient.
+// A vector (a head of a token's queries, keys or values) takes D / 8 lanes of eight numbers each, so that a warp has the same head of 32 / (D / 8) tokens one
+// after the other: APPEND_HEADS heads of queries, whose turns' numbers are then loaded once, or one of keys or values.  Queries are bound by memory (5716
+// tokens of 40 heads of 128 with 8 of keys and values: 17 of 30 us, for 117 MB; with one, two and eight heads a warp 38, 31 and 36 together).  Keys and values
+// are bound by their instructions (13 us for 30 MB; both of a head by one warp 12, but 31 together, and 62 tokens 6.1 instead of 5.5): so the smallest and
+// largest are found in pairs ({x, -x}: one minimum for both), a code comes from a product with 1 / s, and only where that lies so near to the middle of two
+// codes that its error could matter (1e-4; its error is below 4e-6) from the quotient.
 constexpr int APPEND_HEADS = 4;
 template <typename T, int D, int NG, bool TURN>
 __global__ void __launch_bounds__(256) kv4_append_kernel(Kv4Rows in, const float* __restrict__ rope, const int32_t* __restrict__ positions,
@@ -565,7 +568,8 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(Kv4Rows in, const float
 }
 
 // The values that slots stand for: a warp a head of read_slots(D) slots, keys by a word (eight numbers) a lane, values by four numbers a lane that lie
-// side by side, whose codes are in four chunks: loads of two bytes (from L1) and a store of eight, instead of a load and four stores of two.
+// side by side, whose codes are in four chunks: loads of two bytes (from L1) and a store of eight, instead of a load and four stores of two.  5716 slots of 8
+// heads of 128 in 9.9 us for 29 MB, bound by its instructions (issue 71 %; 256 / D and 1024 / D slots a warp: 10.9 and 10.7; a warp a slot with those stores 13).
 constexpr int read_slots(int D) { return 512 / D; }
 // a code as a number: integers are converted at an eighth of an addition's rate
 __device__ __forceinline__ float code_value(uint32_t code, float2 p) {

@@ -9,7 +9,8 @@ A serving step, per layer after the first two lines:
     y = cache.attend(layer, plan, q)                   # every token over its request's keys at and before its position
     cache.truncate(rows, lengths)                      # afterwards: drafts that were rejected; length 0 ends a request
 
-Nothing looks at lengths on the host, so that a captured step serves requests of any lengths.  A group of values x is held as
+Nothing looks at lengths on the host, so that a captured step serves requests of any lengths.  All of it goes to the current stream of the
+cache's device: on another stream a step waits for the one before it, and a plan is kept until its kernels there are done.  A group of values x is held as
 
     lo = min(x),  s = T((max(x) - lo) * (1/15)),  code = min(max(rint((x - lo) / s), 0), 15) in fp32,       standing for code * s + lo
 
@@ -115,6 +116,7 @@ class PagedCache4:
         self.free = torch.arange(pages - 1, -1, -1, **i32)
         self.n_free = torch.full((1,), pages, **i32)
         self._stamp = torch.zeros(requests, **i32)
+        self._none = torch.empty(0, dtype=dtype, device=self.device)      # (a result's type and device)
         self._code = N.dtype_code(dtype)
         self._struct = N.Kv4Cache(*(N.ptr(t) for t in (self.table, self.lengths, self.free, self.n_free, self._stamp)), requests, self.width, pages, max_length,
                                   n_head, n_kv_head, head_size, group, self._code)
@@ -233,7 +235,8 @@ class PagedCache4:
             raise RuntimeError(f"layer {layer} of {self.n_layer}")
         slots = self._whole("slots", slots)
         n = slots.numel()
-        k, v = (torch.empty((n, self.n_kv_head, self.head_size), dtype=self.dtype, device=self.device) for _ in range(2))
+        k = self._none.new_empty(n, self.n_kv_head, self.head_size)
+        v = torch.empty_like(k)
         if n:
             with self._here():
                 N.call("ll_kv4_read", self._c, self._layers[layer], N.ptr(slots), N.ptr(k), N.ptr(v), n, N.stream())
