@@ -156,6 +156,7 @@ __device__ __forceinline__ void divide_work(const PlanView& v, const PlanWork& d
   }
   __syncthreads();
   const int walks = s_count[0];
+  __syncthreads();                     // (the word counts the joins next: every warp has read the walks)
   auto walk_of = [&](int i) {
     if (held) return s_walk[i];
     const int w = tiles(i);
