@@ -189,29 +189,31 @@ class PagedCache4:
         if plan.cache is not self or plan.step != self._step:
             raise RuntimeError("the plan is another cache's, or of a step before this cache's last plan or truncation")
 
-    def _rows(self, name: str, x: torch.Tensor, T: int, heads: int) -> torch.Tensor:
-        """Rows as the kernels take them: the heads of a token one after the other, tokens at any distance, 16-byte boundaries."""
+    def _rows(self, name: str, x: torch.Tensor, T: int, heads: int) -> Tuple[torch.Tensor, int]:
+        """Rows as the kernels take them, and their distance: the heads of a token one after the other, tokens at any distance, 16-byte boundaries."""
         D = self.head_size
         if x.shape != (T, heads, D) or x.dtype is not self.dtype or x.get_device() != self._index:
             raise RuntimeError(f"{name}: {x.dtype} {tuple(x.shape)} on {x.device}, and the cache takes {self.dtype} {(T, heads, D)} on {self.device}")
         if x.requires_grad and torch.is_grad_enabled():
             raise RuntimeError(f"{name}: the 4-bit cache has no gradient")
         row, head, one = x.stride()
-        if one != 1 or (head != D and heads > 1) or (T > 1 and (row % 8 != 0 or row < heads * D)) or x.data_ptr() % 16 != 0:
-            x = x.clone(memory_format=torch.contiguous_format)
-        return x
+        if T < 2:                        # (one row's distance to a next one may be any)
+            row = heads * D
+        if one != 1 or (head != D and heads > 1) or row % 8 != 0 or row < heads * D or x.data_ptr() % 16 != 0:
+            return x.clone(memory_format=torch.contiguous_format), heads * D
+        return x, row
 
     def append(self, layer: int, plan: CachePlan, q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, rope: Optional[torch.Tensor] = None):
         """Round the step's keys and values ``[tokens, n_kv_head, head_size]`` into their slots.  With ``rope`` (fp32 ``[positions, head_size / 2, 2]``, as
         ``build_rope_cache``'s) keys are turned before, and queries ``[tokens, n_head, head_size]`` as well; returns the queries."""
         self._check(layer, plan)
         T = plan.T
-        k, v = self._rows("k", k, T, self.n_kv_head), self._rows("v", v, T, self.n_kv_head)
+        (k, k_row), (v, v_row) = self._rows("k", k, T, self.n_kv_head), self._rows("v", v, T, self.n_kv_head)
         out = q
         if rope is not None:
             if q is None:
                 raise RuntimeError("queries have to be turned with their keys")
-            q = self._rows("q", q, T, self.n_head)
+            q, q_row = self._rows("q", q, T, self.n_head)
             if rope.dtype is not torch.float32 or rope.dim() != 3 or rope.shape != (rope.shape[0], self.head_size // 2, 2) or not rope.is_contiguous() \
                     or rope.get_device() != self._index or rope.data_ptr() % 16 != 0:
                 raise RuntimeError(f"rope: {rope.dtype} {tuple(rope.shape)} on {rope.device}, and the cache takes dense float32 [positions, {self.head_size // 2}, 2]")
@@ -222,10 +224,10 @@ class PagedCache4:
             return out
         with self._here():
             if rope is None:
-                N.call("ll_kv4_append", self._c, self._layers[layer], None, 0, N.ptr(k), k.stride(0), N.ptr(v), v.stride(0), None, plan._positions, plan._slots, None, T,
+                N.call("ll_kv4_append", self._c, self._layers[layer], None, 0, N.ptr(k), k_row, N.ptr(v), v_row, None, plan._positions, plan._slots, None, T,
                        N.stream())
             else:
-                N.call("ll_kv4_append", self._c, self._layers[layer], N.ptr(q), q.stride(0), N.ptr(k), k.stride(0), N.ptr(v), v.stride(0), N.ptr(rope), plan._positions,
+                N.call("ll_kv4_append", self._c, self._layers[layer], N.ptr(q), q_row, N.ptr(k), k_row, N.ptr(v), v_row, N.ptr(rope), plan._positions,
                        plan._slots, N.ptr(out), T, N.stream())
         return out
 
@@ -247,7 +249,7 @@ class PagedCache4:
         have to be appended before.  ``scale`` of the scores: 1 / sqrt(head_size) unless given.  Rows of ``out`` behind the last token stay as they are."""
         self._check(layer, plan)
         T = plan.T
-        q = self._rows("q", q, T, self.n_head)
+        q, q_row = self._rows("q", q, T, self.n_head)
         if out is None:
             out = q.new_empty(T, self.n_head, self.head_size)
         elif out.shape != q.shape or out.dtype != self.dtype or out.device != self.device or not out.is_contiguous() or out.data_ptr() % 16 != 0:
@@ -259,5 +261,5 @@ class PagedCache4:
             return out
         with self._here():
             scratch = self.blocks.new_empty(plan.scratch_bytes)
-            N.call("ll_kv4_attn", self._c, self._layers[layer], N.ptr(q), q.stride(0), plan._work, N.ptr(out), plan.B, T, plan.max_count, scale, N.ptr(scratch), N.stream())
+            N.call("ll_kv4_attn", self._c, self._layers[layer], N.ptr(q), q_row, plan._work, N.ptr(out), plan.B, T, plan.max_count, scale, N.ptr(scratch), N.stream())
         return out

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from tests.test_gpu_paged_cache import BF, DEV, _cache
+from tests.test_gpu_paged_cache import BF, DEV, _cache, _filled, _near
 
 pytestmark = pytest.mark.gpu
 
@@ -27,3 +27,26 @@ def test_every_walk_is_in_the_division(B, new):
         assert int(plan._data[0]) == B * -(-2 * new // cols)
         assert bool((out == 0.0).all())
         cache.truncate(rows, held)
+
+
+@pytest.mark.parametrize("held, counts, H, G", [([70, 3], [1, 1], 4, 2), ([900], [1], 8, 8), ([5], [1], 40, 1)])
+@torch.no_grad()
+def test_single_tokens_of_any_stride(held, counts, H, G):
+    """Rows of one or two tokens at any distance: the same result as dense ones, from ``append`` and from ``attend``."""
+    cache, plan, q, k, v = _filled(held, counts, H, G, 64, 64, BF)
+    want = cache.attend(0, plan, q.to(DEV))
+    _near(want, q, k, v, held, counts, BF, 0.125)
+    rope = torch.rand(cache.max_length, 32, 2, device=DEV)
+    new = [torch.randn(len(counts), g, 64, device=DEV).to(BF) for g in (H, G, G)]
+    turned = cache.append(0, plan, *new, rope=rope)
+    kept = cache.read(0, plan.slots)
+    makes = [lambda x, pad=pad: torch.cat([x.flatten(1), x.flatten(1)[:, :pad]], 1)[:, :x.shape[1] * 64].unflatten(1, (-1, 64)) for pad in (1, 3, 8, 60)]
+    makes.append(lambda x: x.as_strided(x.shape, (1, 64, 1)) if x.shape[0] == 1 else x)
+    for make in makes:
+        cache.append(0, plan, None, torch.zeros_like(new[1]), torch.zeros_like(new[2]))
+        assert torch.equal(cache.append(0, plan, *(make(x) for x in new), rope=rope), turned)
+        assert all(torch.equal(a, b) for a, b in zip(cache.read(0, plan.slots), kept))
+    at = [sum(held[:i + 1]) + sum(counts[:i]) for i in range(len(held))]
+    cache.append(0, plan, None, *(x[at].to(DEV) for x in cache.brought))
+    for make in makes:
+        assert torch.equal(cache.attend(0, plan, make(q.to(DEV))), want)
