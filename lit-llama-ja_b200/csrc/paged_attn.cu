@@ -558,8 +558,9 @@ int ll_kv4_attn(const ll_kv4_cache* cache, const void* blocks, const void* q, lo
     if (int r = kv4_prompt_launch(m, dtype, head_size, group, st)) return r;
   }
   // The sequences of few columns fill the end of the prompts' kernel, which lets them in when it has begun.  The join waits for both (kv4_few_kernel's last block).
-  const bool joined = l.few_cut || l.many;
-  const unsigned join_blocks = (unsigned)std::min<long long>(4ll * kv4_sms(), (long long)l.few_joins() * G * used + (l.many ? (long long)l.many_joins() * G * (KV4_MANY / KJ) : 0));
+  // (None where walks are not cut, or where no sequence may bring a token: then all that bring some are refused.)
+  const unsigned join_blocks =
+      l.few_cut || l.many ? (unsigned)std::min<long long>(4ll * kv4_sms(), (long long)l.few_joins() * G * used + (l.many ? (long long)l.many_joins() * G * (KV4_MANY / KJ) : 0)) : 0;
 #define FEW(TT, DD, NG, CPL, NB)                                                                                                              \
   {                                                                                                                                           \
     constexpr int COLS = 4 * CPL * NB, ring = KF_WARPS * kf_stages(DD, NG) * 2 * kv4_slice_bytes(DD, NG), join = KF_WARPS * COLS * (DD + 4) * 4; \
@@ -572,7 +573,7 @@ int ll_kv4_attn(const ll_kv4_cache* cache, const void* blocks, const void* q, lo
     }                                                                                                                                         \
     LL_CUDA(launch(kv4_few_kernel<TT, DD, NG, CPL, NB>, dim3((unsigned)(l.few_items * G)), dim3(KF_THREADS), smem, st, l.many, a));           \
     LL_LAUNCH_OK("kv4_few_kernel");                                                                                                           \
-    if (joined) LL_CUDA(launch(kv4_join_kernel<TT, DD, COLS>, dim3(join_blocks), dim3(KJ * 32), 0, st, true, a, m));                          \
+    if (join_blocks > 0) LL_CUDA(launch(kv4_join_kernel<TT, DD, COLS>, dim3(join_blocks), dim3(KJ * 32), 0, st, true, a, m));                          \
   }
 #define FEW_COLS(TT, DD, NG)              \
   if (cols == 4) FEW(TT, DD, NG, 1, 1)    \

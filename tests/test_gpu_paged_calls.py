@@ -50,3 +50,16 @@ def test_single_tokens_of_any_stride(held, counts, H, G):
     cache.append(0, plan, None, *(x[at].to(DEV) for x in cache.brought))
     for make in makes:
         assert torch.equal(cache.attend(0, plan, make(q.to(DEV))), want)
+
+
+@pytest.mark.parametrize("max_length", [400, 2000])
+@torch.no_grad()
+def test_a_step_whose_sequences_may_bring_nothing(max_length):
+    """``max_count`` 0: every sequence that brings tokens is refused, its tokens come out as no numbers, and rows behind the last one are left alone."""
+    for H, G in ((2, 2), (40, 1)):
+        cache = _cache(1, H, 64, n_kv_head=G, pages=12, requests=3, max_length=max_length)
+        plan = cache.plan([0, 1, 2], [2, 0, 1], 5, max_count=0)
+        assert plan.status.tolist() == [2, 0, 2] and cache.lengths.tolist() == [0, 0, 0]
+        q, out = torch.randn(5, H, 64, device=DEV).to(BF), torch.full((5, H, 64), 7.0, dtype=BF, device=DEV)
+        y = cache.attend(0, plan, q, out=out)
+        assert bool(y[:3].isnan().all()) and bool((y[3:] == 7.0).all())
