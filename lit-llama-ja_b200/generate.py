@@ -155,8 +155,9 @@ def generate_batch(model: LLaMA, prompts: Sequence[torch.Tensor], max_new_tokens
             live.mul_((~ended).int())
             if not bool(live.any()):
                 break
+    ends = done.tolist()                                            # (waits for the last step: then the check speaks for all of them)
     check_waits()
-    return [torch.cat([p, new[b, :n]]) for b, (p, n) in enumerate(zip(prompts, done.tolist()))]
+    return [torch.cat([p, new[b, :n]]) for b, (p, n) in enumerate(zip(prompts, ends))]
 
 
 def load_model(checkpoint_path: Path, quantize: Optional[str], device: torch.device, dtype: torch.dtype) -> LLaMA:

@@ -1,4 +1,7 @@
 """Calls of the paged 4-bit cache at the ends of what it allows."""
+import sys
+from pathlib import Path
+
 import pytest
 import torch
 
@@ -63,3 +66,23 @@ def test_a_step_whose_sequences_may_bring_nothing(max_length):
         q, out = torch.randn(5, H, 64, device=DEV).to(BF), torch.full((5, H, 64), 7.0, dtype=BF, device=DEV)
         y = cache.attend(0, plan, q, out=out)
         assert bool(y[:3].isnan().all()) and bool((y[3:] == 7.0).all())
+
+
+@torch.no_grad()
+def test_a_batch_is_checked_when_it_is_done(monkeypatch):
+    """generate_batch looks whether a bounded wait ran out after the last step has come to its end, not while it is under way."""
+    sys.path.insert(0, str(Path(__file__).parent.parent / "lit-llama-ja_b200"))
+    import generate
+    from tests.test_gpu_paged_model import _model
+
+    m, done, draw = _model(64), [], generate._draw
+
+    def slow(*a):
+        torch.cuda._sleep(20_000_000)                          # some ten milliseconds
+        return draw(*a)
+
+    monkeypatch.setattr(generate, "_draw", slow)
+    monkeypatch.setattr(generate, "check_waits", lambda: done.append(torch.cuda.current_stream().query()))
+    prompts = [torch.randint(0, 100, (n,), device=DEV) for n in (12, 3)]
+    generate.generate_batch(m, prompts, 6, top_k=1)
+    assert done == [True]
