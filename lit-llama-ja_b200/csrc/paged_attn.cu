@@ -64,6 +64,7 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
   constexpr int W = D / 32, KS = D / 16, COLS = 4 * CPL * NB, BYTES = kv4_bytes(D, NG), SLICE = kv4_slice_bytes(D, NG), SPG = KS / NG, STAGES = kf_stages(D, NG);
   constexpr bool FINE = std::is_same<T, __half>::value;                  // the result keeps 11 bits
   constexpr int TERMS = CPL == 2 && FINE ? 2 : 1;
+  constexpr bool MIDDLE = FINE && TERMS == 1;                            // the sums stand around the middle code
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t s_full[KF_WARPS][STAGES];
   __shared__ int s_fail;
@@ -301,8 +302,9 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
           sum[b][e] += s[x][b][e];
         }
     // y += (p s) c, p lo: by groups, the scales brought under 4 by a power of two that only grows.  Of a word's nibbles 0 and 1 (2 and 3) the rows of
-    // the second tile half take both as they stand, c + 16 c': the end takes c from it.  Where the result is fp16, whose 11 bits show what sums of codes
-    // lose, the sums stand around code 8: one more product takes 8 of every code, and lo gets 8 s.
+    // the second tile half take both as they stand, c + 16 c': the end takes c from it.  Where the result is fp16 and both of a
+    // weight's terms are columns of one product (CPL = 1), the sums stand around code 8: one more product takes 8 of every code, and lo gets 8 s.  Two
+    // terms in two products have their 22 bits without that.
     auto add_values = [&](auto careful) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -316,7 +318,7 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             const float2 p = pv[2 * h + x][g];
-            const float sc = p.x * inv, lo = FINE ? fmaf(8.f, p.x, p.y) : p.y;
+            const float sc = p.x * inv, lo = MIDDLE ? fmaf(8.f, p.x, p.y) : p.y;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
               float w[2] = {0.f, 0.f};
@@ -353,7 +355,7 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
             for (int b = 0; b < NB; ++b) {
 #pragma unroll
               for (int x = 0; x < TERMS; ++x) mma_f16_16816(o[b][r], w0 & 0x000f000fu, w0, w1 & 0x000f000fu, w1, bw[b][x][0], bw[b][x][1]);
-              if (FINE) mma_f16_16816(o[b][r], 0x80088008u, 0x80888088u, 0x80088008u, 0x80888088u, bw[b][0][0], bw[b][0][1]);
+              if (MIDDLE) mma_f16_16816(o[b][r], 0x80088008u, 0x80888088u, 0x80088008u, 0x80888088u, bw[b][0][0], bw[b][0][1]);
             }
           }
         }
