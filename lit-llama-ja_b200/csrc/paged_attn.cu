@@ -67,7 +67,6 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
   constexpr bool MIDDLE = FINE && TERMS == 1;                            // the sums stand around the middle code
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t s_full[KF_WARPS][STAGES];
-  __shared__ int s_fail;
   __shared__ float s_ref[KF_WARPS][COLS], s_sum[KF_WARPS][COLS];
   // (launched when the last blocks of the prompts' kernel of the same call run: what is read here was there before that one.  The last block ends after
   // it, so that what waits for this kernel waits for both.)
@@ -99,7 +98,6 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
   const size_t page_bytes = (size_t)a.G * BYTES;
 
   int entry = lane < units ? table[2 * lane] : 0;                       // the table's entries of 32 pages, a lane each
-  if (threadIdx.x == 0) s_fail = 0;
   if (lane == 0) {
     for (int i = 0; i < STAGES; ++i) mbar_init(&full[i], 1);
     fence_barrier_init();
@@ -374,10 +372,7 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
     }
     if (++st == STAGES) st = 0, parity ^= 1;
   }
-  if (!ok) {
-    s_fail = 1;
-    kv4_let_end();                                                      // copies that were asked for end before the block does
-  }
+  if (!ok) kv4_let_end();                                               // copies that were asked for end before the block does
   // a column's sums over the lanes that share it
 #pragma unroll
   for (int b = 0; b < NB; ++b)
@@ -394,8 +389,7 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
     for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int e = 0; e < CPL; ++e) s_ref[warp][8 * b + CPL * t4 + e] = ref[b][e] == KV4_NONE ? KV4_NONE : ref[b][e] * kq[b][e], s_sum[warp][8 * b + CPL * t4 + e] = sum[b][e];
-  __syncthreads();                      // every unit has been read: the rings hold the warps' sums now
-  if (s_fail) return;
+  if (__syncthreads_or(!ok)) return;    // every unit has been read: the rings hold the warps' sums now
   pdl_launch_dependents();
   float* so = reinterpret_cast<float*>(smem);                           // [warp][column][D + 4]
   constexpr int LD = D + 4;
