@@ -163,8 +163,9 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
       qb[b][s][1] = half_bits(v.x * (up * 0.0625f), v.y * (up * 0.0625f));
       gs[s / SPG] += (u.x + u.y) + (v.x + v.y);
     }
-    // 2^24 of the codes and 2^(ex - 127 - 14) of the queries, times the scores' scale in units of log2
-    const float back = fmaxf(__uint_as_float((uint32_t)(ex - 14 + 24) << 23) * (a.scale * KF_LOG2E), 1.2e-38f);      // (not 0: masked scores are -inf)
+    // 2^24 of the codes and 2^(ex - 127 - 14) of the queries, times the scores' scale in units of log2.  (Less than 1e-36 is what queries of nearly nothing
+    // come to under a scale of nearly nothing: scores of 0 either way.)
+    const float back = fmaxf(__uint_as_float((uint32_t)(ex - 14 + 24) << 23) * (a.scale * KF_LOG2E), 1e-36f);      // (masked scores are -inf, and a first one is more than KF_SLACK from KV4_NONE)
 #pragma unroll
     for (int e = 0; e < CPL; ++e) kq[b][e] = __shfl_sync(0xffffffffu, back, 4 * (2 * t4 + e));
 #pragma unroll

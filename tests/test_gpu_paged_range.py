@@ -3,10 +3,25 @@ trace in what the other keys give."""
 import pytest
 import torch
 
-from tests.test_gpu_paged_cache import DEV, HF, _cache
+from tests.test_gpu_paged_cache import BF, DEV, HF, PAGE, _cache
 from tests.util_paged import held_as
 
 pytestmark = pytest.mark.gpu
+
+
+def _attended(q, k, v, held, group, scale=None, n_kv_head=None, **plan):
+    """One request's last tokens over all of its keys: what the kernels give, and what the cache holds."""
+    L, G, D = k.shape
+    cache = _cache(1, q.shape[1], D, n_kv_head=G, group=group, dtype=k.dtype, pages=-(-L // PAGE) + 2, requests=1, max_length=max(L, 1000))
+    cache.free.copy_(torch.randperm(cache.pages))
+    cache.blocks.fill_(255)
+    whole = cache.plan([0], [L], L)
+    whole.check()
+    cache.append(0, whole, None, k.to(DEV), v.to(DEV))
+    cache.truncate([0], [held])
+    step = cache.plan([0], [L - held], L - held, max_count=L - held)
+    step.check()
+    return cache.attend(0, step, q.to(DEV), scale=scale).double().cpu(), held_as(k, group), held_as(v, group)
 
 
 @pytest.mark.parametrize("counts, R", [([1], 1), ([4], 1), ([1], 8), ([5], 1), ([8], 1), ([16], 1), ([16], 2), ([1, 60], 1), ([1, 60], 6)])
@@ -35,3 +50,16 @@ def test_fp16_results_keep_their_bits(counts, R, D, group):
     span = want.unflatten(-1, (-1, group)).amax(-1) - want.unflatten(-1, (-1, group)).amin(-1)
     tol = want.abs() * 2.0 ** -11 + span.repeat_interleave(group, -1) * 2.0 ** -17 + 2.0 ** -25
     assert bool(((got - want).abs() <= tol).all()), float(((got - want).abs() / tol).max())
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@torch.no_grad()
+def test_a_query_of_zeros_beside_others_under_a_tiny_scale(dtype):
+    """Its keys weigh the same, also those that a warp walks for it alone: the 65th, on a page that the other token does not see."""
+    torch.manual_seed(19)
+    D = 64
+    k, v, q = torch.randn(65, 1, D), torch.zeros(65, 1, D), torch.randn(2, 1, D)
+    v[64] = 65.0
+    q[1] = 0
+    got, K, V = _attended(q.to(dtype), k.to(dtype), v.to(dtype), 63, 64, scale=1e-7)
+    assert float(got[0].abs().max()) <= 0.0 and float((got[1] - 1.0).abs().max()) <= 2.0 ** -8
