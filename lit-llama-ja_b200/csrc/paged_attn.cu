@@ -23,6 +23,8 @@ constexpr int KF_WARPS = 4, KF_THREADS = KF_WARPS * 32;
 // units of 32 keys in a warp's ring: four blocks an SM
 __host__ __device__ constexpr int kf_stages(int D, int groups) { return 4 * KF_WARPS * 3 * 2 * kv4_slice_bytes(D, groups) <= 222 * 1024 ? 3 : 2; }
 constexpr float KF_LOG2E = 1.4426950408889634f, KF_SLACK = 8.f;      // a column's scores may outgrow its reference by 2^8 before it moves
+// Weights are at most 2^KF_SLACK, and scales at most KF_SCALES of what a column's sums stand under unless the unit is looked at: 2^15 in fp16.
+constexpr float KF_SCALES = 128.f, KF_LEAST = 1.17549435082228751e-38f;      // (2^-126)
 constexpr uint32_t KF_WAIT_LIMIT = 1u << 20;
 
 __device__ __forceinline__ float kf_exp2(float x) {
@@ -30,6 +32,9 @@ __device__ __forceinline__ float kf_exp2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
+// the power of two at or under x, and one over it (2^-126 <= x <= 2^126)
+__device__ __forceinline__ float pow2_of(float x) { return __uint_as_float(__float_as_uint(x) & 0x7f800000u); }
+__device__ __forceinline__ float one_over_pow2(float x) { return __uint_as_float((254u << 23) - (__float_as_uint(x) & 0x7f800000u)); }
 // D(16x8, f32) += A(16x16, f16, by rows) * B(16x8, f16, by columns)
 __device__ __forceinline__ void mma_f16_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -114,7 +119,9 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
 
   float o[NB][KS][4];
   float ref[NB][CPL], sum[NB][CPL], sumlo[NB][NG][CPL];      // references in the products' units
-  uint32_t ev[NG];                                           // exponents of the values' scales so far, as powers of two's bits
+  // About the largest product of a weight and a scale so far, whose power of two a column's sums over codes stand under: neither a scale that the column does
+  // not weigh nor one that it does not see costs the others their bits.
+  float most[NB][NG][CPL];
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
 #pragma unroll
@@ -124,11 +131,9 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
       ref[b][e] = KV4_NONE;
       sum[b][e] = 0.f;
 #pragma unroll
-      for (int g = 0; g < NG; ++g) sumlo[b][g][e] = 0.f;
+      for (int g = 0; g < NG; ++g) sumlo[b][g][e] = 0.f, most[b][g][e] = KF_LEAST;
     }
   }
-#pragma unroll
-  for (int g = 0; g < NG; ++g) ev[g] = 1u << 23;
 
   const int t4 = lane & 3, g8 = lane >> 2;
   // queries as the products' second operand: the product's column g8, dimensions 16 s + 4 t4 .. + 3; the largest of a column is brought to
@@ -226,7 +231,7 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
       }
     }
     // which keys a column sees: all of them but at the end of its walk, where a slot behind the last key may hold anything
-    bool none = false;
+    bool none = false;                                                  // whether the unit's values have to be looked at one by one
     if (j - g8 + 31 > first_pos) {
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
@@ -243,52 +248,54 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
       }
       none = __any_sync(0xffffffffu, none);                             // (a value that is none, maybe behind a column: 0 * NaN)
     }
-    // do references or exponents have to move?
+    // do references have to move, or what the sums stand under?
     bool grow = false;
+    float top[NG];                                                      // the largest scale of the lane's keys
+#pragma unroll
+    for (int g = 0; g < NG; ++g) top[g] = fmaxf(fmaxf(pv[0][g].x, pv[1][g].x), fmaxf(pv[2][g].x, pv[3][g].x));
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
-      for (int e = 0; e < CPL; ++e)
+      for (int e = 0; e < CPL; ++e) {
         grow |= (fmaxf(fmaxf(s[0][b][e], s[1][b][e]), fmaxf(s[2][b][e], s[3][b][e])) - ref[b][e]) * kq[b][e] > KF_SLACK;
 #pragma unroll
-    for (int g = 0; g < NG; ++g) grow |= fmaxf(fmaxf(pv[0][g].x, pv[1][g].x), fmaxf(pv[2][g].x, pv[3][g].x)) > 2.f * __uint_as_float(ev[g]);
+        for (int g = 0; g < NG; ++g) grow |= top[g] * one_over_pow2(most[b][g][e]) > KF_SCALES;
+      }
     if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        float f[2] = {1.f, 1.f};
+      for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int e = 0; e < CPL; ++e) {
           float m = fmaxf(fmaxf(s[0][b][e], s[1][b][e]), fmaxf(s[2][b][e], s[3][b][e]));
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
           m = fmaxf(m, ref[b][e]);
-          f[e] = kf_exp2((ref[b][e] - m) * kq[b][e]);
+          const float fe = kf_exp2((ref[b][e] - m) * kq[b][e]);
           ref[b][e] = m;
-          sum[b][e] *= f[e];
+          sum[b][e] *= fe;
 #pragma unroll
-          for (int g = 0; g < NG; ++g) sumlo[b][g][e] *= f[e];
+          for (int g = 0; g < NG; ++g) {
+            sumlo[b][g][e] *= fe;
+            // the largest product of the 32 keys (one that is none is passed over: such a group's results are none whatever they stand under) and the
+            // largest scale: what a column's lanes agree on.  Up to four times the largest product, where the scales are within bounds then.
+            float now = 0.f, scale = top[g];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) now = fmaxf(now, kf_exp2((s[x][b][e] - m) * kq[b][e]) * pv[x][g].x);
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, d)), scale = fmaxf(scale, __shfl_xor_sync(0xffffffffu, scale, d));
+            now = fmaxf(most[b][g][e] * fe, fmaxf(now, fminf(4.f * now, scale * (1.f / KF_SCALES))));
+            now = fminf(fmaxf(now, KF_LEAST), 1.f / KF_LEAST);
+            const float f = fe * pow2_of(most[b][g][e]) * one_over_pow2(now);
+            most[b][g][e] = now;
+            none |= scale * one_over_pow2(now) > KF_SCALES;
+#pragma unroll
+            for (int r = 0; r < SPG; ++r) {
+              o[b][g * SPG + r][e] *= f, o[b][g * SPG + r][2 + e] *= f;
+              if (CPL == 1) o[b][g * SPG + r][1] *= f, o[b][g * SPG + r][3] *= f;
+            }
+          }
         }
-        if (CPL == 1) f[1] = f[0];
-#pragma unroll
-        for (int r = 0; r < KS; ++r) o[b][r][0] *= f[0], o[b][r][1] *= f[1], o[b][r][2] *= f[0], o[b][r][3] *= f[1];
-      }
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {      // (scales are not negative: their bits rise with them; infinite ones and those that are none are passed over)
-        uint32_t big = 0;
-#pragma unroll
-        for (int x = 0; x < 4; ++x) big = max(big, __float_as_uint(pv[x][g].x) < 0x7f800000u ? __float_as_uint(pv[x][g].x) : 0u);
-        big = __reduce_max_sync(0xffffffffu, big) & 0x7f800000u;
-        if (big > ev[g]) {
-          const float f = __uint_as_float(max((int)ev[g] - (int)big + (127 << 23), 0));
-          ev[g] = big;
-#pragma unroll
-          for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int r = 0; r < SPG; ++r)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) o[b][g * SPG + r][e] *= f;
-        }
-      }
+      none = __any_sync(0xffffffffu, none);                             // (a scale that a column does not weigh: its product is taken before it is brought under E)
     }
     // weights (the difference first: of scores past 2^27 a product and a rounded one of the same numbers are too far apart)
 #pragma unroll
@@ -300,7 +307,7 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
           s[x][b][e] = kf_exp2((s[x][b][e] - ref[b][e]) * kq[b][e]);
           sum[b][e] += s[x][b][e];
         }
-    // y += (p s) c, p lo: by groups, the scales brought under 4 by a power of two that only grows.  Of a word's nibbles 0 and 1 (2 and 3) the rows of
+    // y += (p s) c, p lo: by groups, p s under what the column's sums stand under, and so under 2^15.  Of a word's nibbles 0 and 1 (2 and 3) the rows of
     // the second tile half take both as they stand, c + 16 c': the end takes c from it.  Where the result is fp16 and both of a
     // weight's terms are columns of one product (CPL = 1), the sums stand around code 8: one more product takes 8 of every code, and lo gets 8 s.  Two
     // terms in two products have their 22 bits without that.
@@ -312,19 +319,18 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
         for (int x = 0; x < 2; ++x) lds_words<W>(vw[x], unit + h * SLICE + kv4_v_codes(D) + (t4 + 4 * x) * D + g8 * 4 * W);
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-          const float inv = __uint_as_float((254u << 23) - ev[g]);
           uint32_t bw[NB][TERMS][2];
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             const float2 p = pv[2 * h + x][g];
-            const float sc = p.x * inv, lo = MIDDLE ? fmaf(8.f, p.x, p.y) : p.y;
+            const float lo = MIDDLE ? fmaf(8.f, p.x, p.y) : p.y;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
               float w[2] = {0.f, 0.f};
 #pragma unroll
               for (int e = 0; e < CPL; ++e) {
                 const float pe = s[2 * h + x][b][e];
-                w[e] = pe * sc;
+                w[e] = careful.value ? pe * p.x * one_over_pow2(most[b][g][e]) : pe * (p.x * one_over_pow2(most[b][g][e]));
                 if (careful.value && pe == 0.f) w[e] = 0.f;
                 else sumlo[b][g][e] = fmaf(pe, lo, sumlo[b][g][e]);
               }
@@ -398,9 +404,9 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
   for (int b = 0; b < NB; ++b)
 #pragma unroll
     for (int r = 0; r < KS; ++r) {
-      const float up = __uint_as_float(ev[r / SPG]);
 #pragma unroll
       for (int e = 0; e < CPL; ++e) {                                   // (codes were 2^-24 of themselves)
+        const float up = pow2_of(most[b][r / SPG][e]);
         const float c = CPL == 2 ? o[b][r][e] : o[b][r][0] + o[b][r][1], both = CPL == 2 ? o[b][r][2 + e] : o[b][r][2] + o[b][r][3];
         float* const at = so + (warp * COLS + 8 * b + CPL * t4 + e) * LD + 16 * r + g8;
         at[0] = fmaf(c * 16777216.f, up, sumlo[b][r / SPG][e]);

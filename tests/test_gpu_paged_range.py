@@ -1,10 +1,12 @@
 """Attention over the paged 4-bit cache where numbers are of very unequal size: keys and values behind a query, or in sight and without weight, leave no
 trace in what the other keys give."""
+import math
+
 import pytest
 import torch
 
 from tests.test_gpu_paged_cache import BF, DEV, HF, PAGE, _cache
-from tests.util_paged import held_as
+from tests.util_paged import attention, held_as
 
 pytestmark = pytest.mark.gpu
 
@@ -22,6 +24,142 @@ def _attended(q, k, v, held, group, scale=None, n_kv_head=None, **plan):
     step = cache.plan([0], [L - held], L - held, max_count=L - held)
     step.check()
     return cache.attend(0, step, q.to(DEV), scale=scale).double().cpu(), held_as(k, group), held_as(v, group)
+
+
+def _check(got, q, K, V, held, group, dtype, scale):
+    """A weight and its sum are off by half a place of fp16 each (2^-11), a value too (2^-11, and up to twice that of its group's largest where it is a subnormal
+    number), a score by 2^-11 of sum |q| |k| (keys in 11 bits) and 2^-18 for sums in fp32 and the exponential, which moves a weight by twice that; a weight may come to
+    nothing below 2^-23 of the largest product of a weight and a group's range, once a key.  Errors of a weight meet codes, so that a group's largest value
+    counts for all of its dimensions.  The result is rounded once."""
+    top = V.abs().unflatten(-1, (-1, group)).amax(-1, keepdim=True).expand(*V.shape[:2], -1, group).flatten(-2)
+    y, _, mag = attention(q, K, V, held, scale)
+    size = attention(q, K, top, held, scale)[0]
+    half = torch.finfo(dtype).eps / 2
+    tol = y.abs() * half + size * (4 * 2.0 ** -11 + 2 * mag * (2.0 ** -11 + 2.0 ** -18) + K.shape[0] * 2.0 ** -22) + 1e-30
+    off = (got - y).abs()
+    assert bool((off <= tol).all()), float((off / tol).nan_to_num(math.inf).max())
+
+
+def _columns(count, D=128, G=2, R=1, L=300, dtype=BF, spread=0.1):
+    """Keys, values and queries of a request of ``L`` tokens, the last ``count`` of them the step's."""
+    k, v, q = torch.randn(L, G, D), torch.randn(L, G, D) + 0.5, torch.randn(count, G * R, D) * spread
+    return k.to(dtype), v.to(dtype), q.to(dtype)
+
+
+FORMS = [(2, 1, BF, 64), (2, 1, HF, 64), (7, 1, BF, 32), (7, 1, HF, 128), (15, 2, BF, 64)]
+
+
+@pytest.mark.parametrize("count, R, dtype, group", FORMS)
+@pytest.mark.parametrize("size", [1500.0, 30000.0, 1e9, 1e30])
+@torch.no_grad()
+def test_a_later_value_leaves_earlier_rows_alone(count, R, dtype, group, size):
+    """One number of the last token's value is large: the rows before it do not see it."""
+    if size > torch.finfo(dtype).max:
+        return
+    torch.manual_seed(11)
+    k, v, q = _columns(count, R=R, dtype=dtype)
+    held = k.shape[0] - count
+    v[-1, :, 3] = size
+    got, K, V = _attended(q, k, v, held, group)
+    _check(got[:-1], q[:-1], K[:-1], V[:-1], held, group, dtype, 128 ** -0.5)
+
+
+@pytest.mark.parametrize("count, R, dtype, group", FORMS)
+@pytest.mark.parametrize("size", [30000.0, 1e9, 1e30])
+@torch.no_grad()
+def test_a_later_key_leaves_earlier_rows_alone(count, R, dtype, group, size):
+    if size > torch.finfo(dtype).max:
+        return
+    torch.manual_seed(12)
+    k, v, q = _columns(count, R=R, dtype=dtype)
+    held = k.shape[0] - count
+    k[-1, :, 3] = -size
+    got, K, V = _attended(q, k, v, held, group)
+    _check(got[:-1], q[:-1], K[:-1], V[:-1], held, group, dtype, 128 ** -0.5)
+
+
+@pytest.mark.parametrize("count, R, dtype, group", [(1, 1, BF, 64), (1, 1, HF, 32)] + FORMS)
+@pytest.mark.parametrize("size", [1500.0, 30000.0, 1e9])
+@pytest.mark.parametrize("at", [0, 40, 200])
+@torch.no_grad()
+def test_a_value_in_sight_without_weight(count, R, dtype, group, size, at):
+    """A key that no query weighs (2^-80 and less) has a large value; the others share the weight."""
+    if size > torch.finfo(dtype).max:
+        return
+    torch.manual_seed(13)
+    k, v, q = _columns(count, R=R, dtype=dtype)
+    held = k.shape[0] - count
+    q[..., 0], k[..., 0] = 8.0, 0.0
+    k[at, :, 0] = -80.0                                       # scores of -640 / sqrt(128)
+    v[at, :, 3] = size
+    got, K, V = _attended(q, k, v, held, group)
+    first = max(0, at - held)
+    _check(got, q, K, V, held, group, dtype, 128 ** -0.5)
+    assert first == 0 or torch.isfinite(got).all()
+
+
+@pytest.mark.parametrize("count, R, group", [(2, 1, 64), (3, 1, 32), (9, 1, 64), (15, 2, 64)])
+@pytest.mark.parametrize("large", [1100.0, 1e9])
+@pytest.mark.parametrize("hidden", [False, True])
+@torch.no_grad()
+def test_many_small_weights_beside_a_first_token(count, R, group, large, hidden):
+    """The first token has nearly all of the weight and a small value, so that the result is that of the others, at 2^-11 each; one value, in sight without
+    weight or behind the query, is large."""
+    torch.manual_seed(14)
+    L = 190
+    k, v, q = _columns(count, R=R, L=L)
+    held = L - count
+    q[..., 0], k[..., 0] = 8.0, 0.0
+    k[0, :, 0] = 11 * math.log(2.0) * math.sqrt(128) / 8.0
+    v[0] *= 2.0 ** -10
+    v[-1 if hidden else 5, :, 5] = large
+    if not hidden:
+        k[5, :, 0] = -80.0
+    got, K, V = _attended(q, k, v, held, group)
+    n = count - 1 if hidden else count
+    _check(got[:n], q[:n], K[:held + n], V[:held + n], held, group, BF, 128 ** -0.5)
+
+
+@pytest.mark.parametrize("count, R, group", [(1, 1, 32), (4, 1, 32), (9, 1, 64), (16, 2, 32)])
+@torch.no_grad()
+def test_groups_of_very_unequal_size(count, R, group):
+    """Groups of one token's values 2^40 apart, keys' alike: each group's result to its own size."""
+    torch.manual_seed(15)
+    k, v, q = _columns(count, R=R, L=330)
+    v[..., :group] *= 2.0 ** 20
+    v[..., group:] *= 2.0 ** -20
+    k[..., :group] *= 2.0 ** -20
+    got, K, V = _attended(q, k, v, 330 - count, group)
+    _check(got, q, K, V, 330 - count, group, BF, 128 ** -0.5)
+
+
+@pytest.mark.parametrize("count, R, group", [(1, 1, 64), (6, 1, 32), (16, 2, 64)])
+@pytest.mark.parametrize("power", [-60, -20, -9, 0, 9, 20, 60])
+@torch.no_grad()
+def test_values_of_any_size(count, R, group, power):
+    """All values under a power of two, and the queries' scores with them where the keys are: the same result under it."""
+    torch.manual_seed(16)
+    k, v, q = _columns(count, R=R, L=330)
+    v, k, q = v * 2.0 ** power, k * 2.0 ** -(power // 3), q * 2.0 ** (power // 3)
+    got, K, V = _attended(q, k, v, 330 - count, group)
+    _check(got, q, K, V, 330 - count, group, BF, 128 ** -0.5)
+
+
+@pytest.mark.parametrize("grow", [1, 40])
+@pytest.mark.parametrize("count, R, dtype", [(1, 1, BF), (1, 1, HF), (6, 1, BF), (16, 2, HF)])
+@torch.no_grad()
+def test_scores_that_rise_over_values_that_fall(count, R, dtype, grow):
+    """Scores that rise along the keys, so that references move again and again, over values that get smaller (grow 1: larger): what counts is the
+    product of weight and value."""
+    torch.manual_seed(17)
+    L = 700
+    k, v, q = _columns(count, R=R, L=L, dtype=dtype)
+    ramp = torch.arange(L) / L
+    q[..., 0] = 8.0
+    k[..., 0] = (30.0 * ramp)[:, None]
+    v = (v.float() * 2.0 ** ((10 if grow == 1 else -10) * ramp)[:, None, None]).to(dtype)
+    got, K, V = _attended(q, k, v, L - count, 64)
+    _check(got, q, K, V, L - count, 64, dtype, 128 ** -0.5)
 
 
 @pytest.mark.parametrize("counts, R", [([1], 1), ([4], 1), ([1], 8), ([5], 1), ([8], 1), ([16], 1), ([16], 2), ([1, 60], 1), ([1, 60], 6)])
