@@ -49,6 +49,8 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t v) {
 }
 __device__ __forceinline__ uint32_t half_bits(float a, float b) { return pair_bits<__half>(a, b); }
 
+__device__ __forceinline__ void mbar_inval(uint64_t* bar) { asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory"); }
+
 // One warp's wait for its copy: bounded; one that runs out leaves a code for the host.
 __device__ __forceinline__ bool kf_wait(uint64_t* bar, uint32_t parity, int* word) {
   if (mbar_try_wait(bar, parity)) return true;
@@ -64,33 +66,27 @@ __device__ __forceinline__ bool kf_wait(uint64_t* bar, uint32_t parity, int* wor
 // CPL = 1: up to four columns, each of which has two of the product's eight, so that a lane has one column's scores and not those of columns that are
 // not there (drafts of four tokens, 12 requests of up to 3000 keys, 40 heads: 35 us, with eight columns 39); CPL = 2: eight columns, and 16 with NB = 2.  Weights enter the second product as fp16, half a place (2^-11) of which a bf16 result does not show; where the result is fp16 as two terms, with
 // CPL = 1 the second one in the odd column.
+template <int COLS, int STAGES>
+struct KfShared {
+  uint64_t full[KF_WARPS][STAGES];
+  float ref[KF_WARPS][COLS], sum[KF_WARPS][COLS];
+};
+// Where a part's sums go: [parts there is room for][G][stride] of D sums, then of (reference, sum of weights), from column `at` of a walk's.
+struct KfPart {
+  float* part;
+  int kept, stride, at;
+};
+// Columns col0 .. of an item's walk.  False where a wait ran out; every thread of the block calls.
 template <typename T, int D, int NG, int CPL, int NB>
-__global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(const Kv4Attn a) {
+__device__ __forceinline__ bool few_walk(const Kv4Attn& a, const Kv4Item& it, int head, int col0, const KfPart to, uint8_t* smem,
+                                         KfShared<4 * CPL * NB, kf_stages(D, NG)>& sh) {
   constexpr int W = D / 32, KS = D / 16, COLS = 4 * CPL * NB, BYTES = kv4_bytes(D, NG), SLICE = kv4_slice_bytes(D, NG), SPG = KS / NG, STAGES = kf_stages(D, NG);
   constexpr bool FINE = std::is_same<T, __half>::value;                  // the result keeps 11 bits
   constexpr int TERMS = CPL == 2 && FINE ? 2 : 1;
   constexpr bool MIDDLE = FINE && TERMS == 1;                            // the sums stand around the middle code
-  extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ uint64_t s_full[KF_WARPS][STAGES];
-  __shared__ float s_ref[KF_WARPS][COLS], s_sum[KF_WARPS][COLS];
-  // (launched when the last blocks of the prompts' kernel of the same call run: what is read here was there before that one.  The last block ends after
-  // it, so that what waits for this kernel waits for both.)
-  if (blockIdx.x == gridDim.x - 1) pdl_wait();
-  const int item = blockIdx.x / a.G, head = blockIdx.x - item * a.G;
-  const Kv4Item it = load_item(a.work, item);                           // (there is room for it: asked for together with the number of parts)
-  if (item >= a.work[0]) return;
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, R = a.H / a.G;
-  const int first = it.first, n = it.count, row = it.row;
-  const int col0 = it.tile * COLS, cols = min(COLS, n * R - col0);
+  const int first = it.first, n = it.count, row = it.row, cols = min(COLS, n * R - col0);
   T* y = (T*)a.y;
-  if (row < 0) {                        // a refused sequence's tokens are no numbers
-#pragma unroll 1
-    for (int e = threadIdx.x; e < cols * D; e += KF_THREADS) {
-      const int c = col0 + e / D;
-      dt<T>::st(y, ((size_t)(first + column_token(c, R)) * a.H + head * R + column_head(c, R)) * D + e % D, NAN);
-    }
-    return;
-  }
   const int pos0 = it.pos0;
   const int last = pos0 + column_token(col0 + cols - 1, R);                    // position of the tile's last column: keys up to here are in sight
   const int page0 = it.page0 + (warp >> 1), page1 = min(it.page1, last / KV4_PAGE + 1), half32 = 32 * (warp & 1);
@@ -98,7 +94,7 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
   const int units = page0 >= page1 ? 0 : (page1 - page0 + 1) / 2 - ((page0 + ((page1 - page0 - 1) & ~1)) * KV4_PAGE + half32 > last ? 1 : 0);
   const int32_t* table = a.table + (size_t)row * a.width + page0;
   uint8_t* ring = smem + warp * STAGES * 2 * SLICE;
-  uint64_t* full = s_full[warp];
+  uint64_t* full = sh.full[warp];
   const uint8_t* from = a.blocks + (size_t)head * BYTES + (warp & 1) * 2 * SLICE;
   const size_t page_bytes = (size_t)a.G * BYTES;
 
@@ -395,8 +391,8 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
-      for (int e = 0; e < CPL; ++e) s_ref[warp][8 * b + CPL * t4 + e] = ref[b][e] == KV4_NONE ? KV4_NONE : ref[b][e] * kq[b][e], s_sum[warp][8 * b + CPL * t4 + e] = sum[b][e];
-  if (__syncthreads_or(!ok)) return;    // every unit has been read: the rings hold the warps' sums now
+      for (int e = 0; e < CPL; ++e) sh.ref[warp][8 * b + CPL * t4 + e] = ref[b][e] == KV4_NONE ? KV4_NONE : ref[b][e] * kq[b][e], sh.sum[warp][8 * b + CPL * t4 + e] = sum[b][e];
+  if (__syncthreads_or(!ok)) return false;    // every unit has been read: the rings hold the warps' sums now
   pdl_launch_dependents();
   float* so = reinterpret_cast<float*>(smem);                           // [warp][column][D + 4]
   constexpr int LD = D + 4;
@@ -418,15 +414,15 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
 #pragma unroll 1
   for (int x = threadIdx.x; x < cols * (D / 4); x += KF_THREADS) {
     const int c = x / (D / 4), d = x % (D / 4) * 4;
-    float m = s_ref[0][c];
+    float m = sh.ref[0][c];
 #pragma unroll
-    for (int w = 1; w < KF_WARPS; ++w) m = fmaxf(m, s_ref[w][c]);
+    for (int w = 1; w < KF_WARPS; ++w) m = fmaxf(m, sh.ref[w][c]);
     float l = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < KF_WARPS; ++w) {
-      const float f = kf_exp2(s_ref[w][c] - m);
+      const float f = kf_exp2(sh.ref[w][c] - m);
       const float4 u = *reinterpret_cast<const float4*>(so + (w * COLS + c) * LD + d);
-      l = fmaf(s_sum[w][c], f, l);
+      l = fmaf(sh.sum[w][c], f, l);
       v[0] = fmaf(u.x, f, v[0]), v[1] = fmaf(u.y, f, v[1]), v[2] = fmaf(u.z, f, v[2]), v[3] = fmaf(u.w, f, v[3]);
     }
     if (it.parts == 1) {
@@ -434,11 +430,76 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
       const uint2 out = make_uint2(pair_bits<T>(v[0] / l, v[1] / l), pair_bits<T>(v[2] / l, v[3] / l));
       *reinterpret_cast<uint2*>(y + ((size_t)(first + column_token(cc, R)) * a.H + head * R + column_head(cc, R)) * D + d) = out;
     } else {
-      const size_t at = ((size_t)(it.base + it.part) * a.G + head) * COLS + c;
-      *reinterpret_cast<float4*>(a.part + at * D + d) = make_float4(v[0], v[1], v[2], v[3]);
-      if (d == 0) *reinterpret_cast<float2*>(a.part + (size_t)a.kept * a.G * COLS * D + at * 2) = make_float2(m, l);
+      const size_t at = ((size_t)(it.base + it.part) * a.G + head) * to.stride + to.at + c;
+      *reinterpret_cast<float4*>(to.part + at * D + d) = make_float4(v[0], v[1], v[2], v[3]);
+      if (d == 0) *reinterpret_cast<float2*>(to.part + (size_t)to.kept * a.G * to.stride * D + at * 2) = make_float2(m, l);
     }
   }
+  return true;
+}
+
+// A block an item and key head of the list `a`; beside a list `m` of the many there are blocks more, which go through the tiles that kv4_prompt_kernel has left (groups
+// that fp16 numbers do not hold), eight columns at a time.
+template <typename T, int D, int NG, int CPL, int NB>
+__global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(const Kv4Attn a, const Kv4Attn m) {
+  constexpr int COLS = 4 * CPL * NB;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ KfShared<COLS, kf_stages(D, NG)> sh;
+  // (launched when the last blocks of the prompts' kernel of the same call run: what is read here was there before that one.  The last block ends after
+  // it, so that what waits for this kernel waits for both.)
+  if (blockIdx.x == gridDim.x - 1) pdl_wait();
+  const int R = a.H / a.G, blocks = a.items * a.G;
+  if constexpr (COLS == KV4_FEW_BESIDE) {
+    if ((int)blockIdx.x >= blocks) {      // (what these read the prompts' kernel has left)
+      constexpr int SUBS = KV4_MANY / COLS;
+      __shared__ uint32_t s_left[KF_WARPS];
+      pdl_launch_dependents();
+      pdl_wait();
+      const int again = gridDim.x - blocks;
+      const int32_t* work = after_wait(m.work);
+      const int* odd = after_wait(m.odd);
+      const long long units = (long long)min(work[0], m.items) * a.G * SUBS;
+#pragma unroll 1
+      for (long long u0 = blockIdx.x - blocks; u0 < units; u0 += (long long)again * KF_THREADS) {
+        const long long mine = u0 + (long long)again * threadIdx.x;
+        const uint32_t left = __ballot_sync(0xffffffffu, mine < units && (odd[mine / SUBS] >> (mine % SUBS / (SUBS / 2)) & 1) != 0);
+        __syncthreads();
+        if ((threadIdx.x & 31) == 0) s_left[threadIdx.x >> 5] = left;
+        __syncthreads();
+#pragma unroll 1
+        for (int w = 0; w < KF_WARPS; ++w)
+#pragma unroll 1
+          for (uint32_t bits = s_left[w]; bits != 0u; bits &= bits - 1) {
+            const long long unit = u0 + (long long)again * (32 * w + __ffs(bits) - 1);
+            const int block = (int)(unit / SUBS), item = block / a.G, head = block - item * a.G, at = (int)(unit % SUBS) * COLS;
+            const Kv4Item it = load_item(work, item);
+            const int col0 = it.tile * KV4_MANY + at;
+            if (col0 >= it.count * R) continue;
+            if (!few_walk<T, D, NG, CPL, NB>(a, it, head, col0, KfPart{m.part, m.kept, KV4_MANY, at}, smem, sh)) return;
+            fence_proxy_async();                                        // (the rings' memory has been written and read by threads: copies come next)
+            __syncthreads();
+            if ((threadIdx.x & 31) == 0)
+              for (int i = 0; i < kf_stages(D, NG); ++i) mbar_inval(&sh.full[threadIdx.x >> 5][i]);
+            __syncwarp();
+          }
+      }
+      return;
+    }
+  }
+  const int item = blockIdx.x / a.G, head = blockIdx.x - item * a.G;
+  const Kv4Item it = load_item(a.work, item);                           // (there is room for it: asked for together with the number of parts)
+  if (item >= a.work[0]) return;
+  const int col0 = it.tile * COLS;
+  if (it.row < 0) {                     // a refused sequence's tokens are no numbers
+    const int cols = min(COLS, it.count * R - col0);
+#pragma unroll 1
+    for (int e = threadIdx.x; e < cols * D; e += KF_THREADS) {
+      const int c = col0 + e / D;
+      dt<T>::st((T*)a.y, ((size_t)(it.first + column_token(c, R)) * a.H + head * R + column_head(c, R)) * D + e % D, NAN);
+    }
+    return;
+  }
+  few_walk<T, D, NG, CPL, NB>(a, it, head, col0, KfPart{a.part, a.kept, COLS, 0}, smem, sh);
 }
 
 // Joins the parts of walks.  Of the few columns a block has one at a time, a warp every KJ-th part (a long walk is in hundreds of parts); of the
@@ -530,7 +591,7 @@ extern "C" {
 
 size_t ll_kv4_attn_scratch_bytes(const ll_kv4_cache* cache, int B, int T, int max_count) {
   if (!kv4_step_ok(cache, B, T, max_count)) return 0;
-  return sizeof(float) * Kv4Lists(B, T, max_count, cache->heads, cache->kv_heads, cache->max_length).floats(cache->kv_heads, cache->head_size);
+  return Kv4Lists(B, T, max_count, cache->heads, cache->kv_heads, cache->max_length).bytes(cache->kv_heads, cache->head_size);
 }
 
 int ll_kv4_attn(const ll_kv4_cache* cache, const void* blocks, const void* q, long long q_row, const int32_t* work, void* y, int B, int T, int max_count,
@@ -549,21 +610,24 @@ int ll_kv4_attn(const ll_kv4_cache* cache, const void* blocks, const void* q, lo
   LL_CHECK_ARG(l.few_items * G <= INT_MAX && l.many_items * G <= INT_MAX, "kv4_attn: %d sequences of %d tokens, %d heads", B, T, H);
   const int R = l.R, cols = l.cols, used = (int)std::min((long long)cols, (long long)max_count * R);
   const Kv4Attn a{q, q_row, (const uint8_t*)blocks, cache->table, work, y, (float*)scratch, H, G, cache->width, cache->pages, (int)l.few_items, l.few_kept(), used, scale,
-                  wait_word()};
+                  wait_word(), nullptr};
   Kv4Attn m = a;
   m.items = 0;
   cudaStream_t st = (cudaStream_t)stream;
   if (l.many) {
     m.work = work + l.few_ints();
     m.part = (float*)scratch + l.few_floats(G, head_size);
+    m.odd = (int*)(m.part + l.many_floats(G, head_size));
     m.items = (int)l.many_items;
     m.kept = l.many_kept();
     if (int r = kv4_prompt_launch(m, dtype, head_size, group, st)) return r;
   }
-  // The sequences of few columns fill the end of the prompts' kernel, which lets them in when it has begun.  The join waits for both (kv4_few_kernel's last block).
+  // The sequences of few columns fill the end of the prompts' kernel, which lets them in when it has begun.  The join waits for both (kv4_few_kernel's last blocks).
   // (None where walks are not cut, or where no sequence may bring a token: then all that bring some are refused.)
   const unsigned join_blocks =
       l.few_cut || l.many ? (unsigned)std::min<long long>(4ll * kv4_sms(), (long long)l.few_joins() * G * used + (l.many ? (long long)l.many_joins() * G * (KV4_MANY / KJ) : 0)) : 0;
+  LL_CHECK_ARG(l.few_items * G + 4ll * kv4_sms() <= INT_MAX, "kv4_attn: %d sequences of %d tokens, %d heads", B, T, H);
+  const unsigned few_blocks = (unsigned)(l.few_items * G) + (l.many ? 4u * kv4_sms() : 0u);
 #define FEW(TT, DD, NG, CPL, NB)                                                                                                              \
   {                                                                                                                                           \
     constexpr int COLS = 4 * CPL * NB, ring = KF_WARPS * kf_stages(DD, NG) * 2 * kv4_slice_bytes(DD, NG), join = KF_WARPS * COLS * (DD + 4) * 4; \
@@ -574,7 +638,7 @@ int ll_kv4_attn(const ll_kv4_cache* cache, const void* blocks, const void* q, lo
       prefer_max_smem(kv4_few_kernel<TT, DD, NG, CPL, NB>);                                                                                   \
       set.mark();                                                                                                                             \
     }                                                                                                                                         \
-    LL_CUDA(launch(kv4_few_kernel<TT, DD, NG, CPL, NB>, dim3((unsigned)(l.few_items * G)), dim3(KF_THREADS), smem, st, l.many, a));           \
+    LL_CUDA(launch(kv4_few_kernel<TT, DD, NG, CPL, NB>, dim3(few_blocks), dim3(KF_THREADS), smem, st, l.many, a, m));           \
     LL_LAUNCH_OK("kv4_few_kernel");                                                                                                           \
     if (join_blocks > 0) LL_CUDA(launch(kv4_join_kernel<TT, DD, COLS>, dim3(join_blocks), dim3(KJ * 32), 0, st, true, a, m));                          \
   }

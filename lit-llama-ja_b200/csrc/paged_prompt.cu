@@ -6,13 +6,12 @@
 //   warps 20-27     : two sets that take the pages in turn, a warp a slice of 16 keys: codes by bulk copies into a ring, from there as fp16 numbers into
 //                     the operands.  (One set took 2600 clocks a page, and with it the block; 700 tokens over 5000 keys, 32 / 8 heads: 132 -> 125 us.)
 // All operands are fp16, whatever the cache's type: its 11 bits hold a query exactly (a row under a power of two of its own) and a key or value
-// c s + lo rounded once, where bf16 would lose three bits more.  Slices are brought into range by powers of two 2^e, e a multiple of 16 (so that
-// e is the same, mostly 0, for all of them): scores are multiplied back by 2^e; weights by 2^(e - E), E the largest so far, to which O is rescaled.
+// c s + lo rounded once, where bf16 would lose three bits more.  What fp16 numbers do not hold (group_fits) is left to the walk of few columns: a tile that
+// sees such a group, or one that is no number, stores nothing and is named in `odd`.  (Powers of two by slices of keys cost the keys and values beside a large
+// one their bits, also in rows that do not see it, and 3 to 14 us of the three prompts below.)
 // A word's codes become pairs by masks: 1024 + c under exponent bits, from which one operation takes the 1024 (of odd nibbles, 1024 + 16 c, 64 + c), and
 // one more multiplies and adds.  Keys' pairs run along the dimensions, values' along the keys: values stand with the keys in a row, so that both
 // operands are K-major.
-// Values that are no numbers are zeros in the operand, the first position of such a group is kept and rows that see it end as no numbers: 0 * NaN would
-// reach rows that do not.
 // What bounds it: issue slots (63 % of them used), which the softmax and the unpacking share; the exponential unit is busy 30, the tensor pipe 29 % of the
 // time.  A prompt of 2048, 32 heads of 128, us: 92 with the queries a row a thread (8000 clocks of a block) and all walks cut, 73 with whole rows and walks
 // as they are, 64 with two sets of unpacking warps and the other sequences' kernel let in at the end, 62 with waits and loops as one turn of code;
@@ -32,14 +31,17 @@ constexpr int KP_ROWS = 128, KP_SOFTMAX = 16, KP_FIRST = KP_SOFTMAX + 4, KP_SETS
 constexpr int KP_REGS = 72, KP_REGS_SOFTMAX = 88, KP_REGS_MMA = 40, KP_REGS_DEQUANT = 56;
 static_assert(KP_THREADS * KP_REGS <= 65536 && KP_SOFTMAX * KP_REGS_SOFTMAX + 4 * KP_REGS_MMA + KP_DEQUANT * KP_REGS_DEQUANT <= KP_THREADS / 32 * KP_REGS, "registers");
 constexpr int KP_QBOX = KP_ROWS * 128, KP_KBOX = KV4_PAGE * 128;      // 64 numbers of 16 bits a row
-constexpr int KP_RING = 2, KP_STAGES = 3, KP_EXPS = 8;               // copies in flight a slice of a set; pages of K and of V; pages whose exponents are kept
+constexpr int KP_RING = 2, KP_STAGES = 3;                            // copies in flight a slice of a set; pages of K and of V
+// A row's largest weight is 2^KP_UP or more, so that a weight in fp16 comes to nothing under 2^-31 of it only, and under 2^15: its scores may outgrow the
+// reference by KP_SLACK before it moves.
+constexpr float KP_UP = 6.f, KP_SLACK = KP_UP + AT_SLACK;
 
 template <int D, int NG>
 struct KpShape {
   static constexpr int NB = (D + 63) / 64, SLICE = kv4_slice_bytes(D, NG);
   static constexpr int Q = 2 * NB * KP_QBOX, K = NB * KP_KBOX, V = D * 128;
   static constexpr int RING = KP_DEQUANT * KP_RING * SLICE;
-  static constexpr int SMEM = 1024 + Q + KP_STAGES * (K + V) + RING + 512 + 6 * KP_ROWS * 4 + KP_EXPS * 4 * 2;
+  static constexpr int SMEM = 1024 + Q + KP_STAGES * (K + V) + RING + 512 + 6 * KP_ROWS * 4;
 };
 
 __device__ __forceinline__ void kp_ran_out(volatile int* fail, int* word, int code) {
@@ -62,12 +64,16 @@ __device__ __forceinline__ bool kp_wait(uint64_t* bar, uint32_t parity, volatile
 __host__ __device__ constexpr uint32_t instr_desc_f16(int M, int N) { return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24); }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }      // -126 <= e <= 127
 
-// A slice's power of two, from the lanes' largest scale (low half) and lowest value: the multiple of 16 that brings |lo| + 15 s under 2^11.
+// Whether a group of scale s and lowest value lo (the halves of a word) keeps its bits as fp16 numbers: |c s + lo| is under 2^13, and rounding it and, from bf16,
+// s and lo costs 2^-10 of the group's largest (2^-11 of it over 2^-13; a bf16 scale from 2^-17 on is exact, and a smaller one is off by 2^-25, 15 codes 2^-21).
+// Then weights that come to nothing (2^-31 of a row's largest) take 2^-18 from a result at most.  A group that is no number does not fit, one of zeros does.
 template <typename T>
-__device__ __forceinline__ int slice_exponent(uint32_t largest) {
-  const float2 p = bits_pair<T>(largest);
-  const int fl = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(p.y, 16.f * p.x))) >> 23) - 127;
-  return fl < -126 ? 0 : max(-112, min(112, ((fl + 6) >> 4) << 4));      // (zeros alone, as behind the last key: any will do)
+__device__ __forceinline__ bool group_fits(uint32_t w) {
+  constexpr bool F = std::is_same<T, __half>::value;
+  constexpr uint32_t S_LARGE = F ? 0x5c00u : 0x4380u, LO_LARGE = F ? 0x6c00u : 0x4580u;      // 2^8, 2^12
+  constexpr uint32_t S_SMALL = F ? 0x0100u : 0x3780u, LO_SMALL = F ? 0x1400u : 0x3a80u;      // 2^-16, 2^-10
+  const uint32_t s = w & 0x7fffu, lo = (w >> 16) & 0x7fffu;
+  return s < S_LARGE && lo < LO_LARGE && (s >= S_SMALL || lo >= LO_SMALL || (s | lo) == 0u);
 }
 __device__ __forceinline__ __half2 as_half2(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
 __device__ __forceinline__ uint32_t as_u32(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
@@ -92,6 +98,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
   const int R = a.H / a.G, cols_all = it.count * R, col0 = it.tile * KV4_MANY, cols = min(KV4_MANY, cols_all - col0);
   T* const y = (T*)a.y;
   if (it.row < 0) {                     // a refused sequence's tokens are no numbers
+    if (threadIdx.x == 0) a.odd[blockIdx.x] = 0;
 #pragma unroll 1
     for (int e = threadIdx.x; e < cols * D; e += KP_THREADS) {
       const int c = col0 + e / D;
@@ -115,11 +122,9 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
   uint64_t* r_full = o_full + 4;                      // [slice][stage]
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(r_full + KP_DEQUANT * KP_RING);
   int* s_fail = reinterpret_cast<int*>(tmem_ptr + 1);
-  int* s_none = s_fail + 1;                           // [4] per group the first position whose value is no number
+  volatile int* s_odd = s_fail + 1;                   // [tile] whether the tile sees a group that fp16 numbers do not hold
   float* s_x = reinterpret_cast<float*>(ring + Shape::RING + 512);      // [tile][half][row]: what the two threads of a row tell one another
   float* s_mul = s_x + 4 * KP_ROWS;                   // [2 tiles][row] what a row's raw scores are multiplied by
-  signed char* s_ek = reinterpret_cast<signed char*>(s_mul + 2 * KP_ROWS);      // [page & 7][slice] exponents of keys and values
-  signed char* s_ev = s_ek + KP_EXPS * 4;
 
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   // what every role walks: pages page0 .. page1; per tile the last page that one of its rows sees
@@ -157,8 +162,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
   if (threadIdx.x == 0) {
     mbar_init(q_full, KP_SOFTMAX);
     for (int i = 0; i < KP_STAGES; ++i) mbar_init(&k_full[i], 4), mbar_init(&k_empty[i], 2), mbar_init(&v_full[i], 4), mbar_init(&v_empty[i], 2);
-    for (int i = 0; i < 4; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], KP_SOFTMAX / 2), mbar_init(&o_full[i], 1), s_none[i] = INT_MAX;
-    *s_fail = 0;
+    for (int i = 0; i < 4; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], KP_SOFTMAX / 2), mbar_init(&o_full[i], 1);
+    *s_fail = s_odd[0] = s_odd[1] = 0;
     fence_barrier_init();
   }
   if (warp == KP_SOFTMAX) tmem_alloc(tmem_ptr, 512);
@@ -182,7 +187,6 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
       const uint8_t* blk = mine + st * SLICE;
       uint32_t kw[2][W], vw[2][W];
       uint32_t kp[2][NG], vp[2][2][NG];               // parameters of keys g8 + 8 x and of the values of slots 2 (t4 + 4 x) + e
-      uint32_t bk = 0, bv = 0;                        // sizes rise with their bits: the largest scale, and the largest lowest value
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         lds_words<W>(kw[x], blk + (g8 + 8 * x) * (D / 2) + t4 * 4 * W);
@@ -191,7 +195,18 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
 #pragma unroll
         for (int e = 0; e < 2; ++e) lds_words<NG>(vp[x][e], blk + kv4_v_params(D, NG) + (2 * (t4 + 4 * x) + e) * NG * 4);
       }
-      const int pos = (page0 + n) * KV4_PAGE + KV4_SLICE * sl;
+      const int page_at = page0 + n, pos = page_at * KV4_PAGE + KV4_SLICE * sl;
+      {                                               // (a lane has the groups of a key or of a value)
+        uint32_t mine[NG];
+        lds_words<NG>(mine, blk + kv4_k_params(D) + lane * NG * 4);
+        bool fits = true;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) fits &= group_fits<T>(mine[g]);
+        if (!fits && pos + (lane & (KV4_SLICE - 1)) <= last) {
+          if (page_at <= hi0) s_odd[0] = 1;
+          if (page_at <= hi1) s_odd[1] = 1;
+        }
+      }
       if (pos + KV4_SLICE - 1 > last) {               // (a slot behind the last key may hold anything)
 #pragma unroll
         for (int x = 0; x < 2; ++x)
@@ -203,31 +218,6 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
               if (pos + 2 * (t4 + 4 * x) + e > last) vp[x][e][g] = 0u;
           }
       }
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          bk = __vmaxu2(bk, kp[x][g] & 0x7fff7fffu);
-          bv = __vmaxu2(__vmaxu2(bv, vp[x][0][g] & 0x7fff7fffu), vp[x][1][g] & 0x7fff7fffu);
-        }
-      constexpr uint32_t NUMBERS = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;      // (a group that is no number is so in both)
-      if (__any_sync(0xffffffffu, (bk >> 16) >= NUMBERS || (bv >> 16) >= NUMBERS)) {
-        bk = bv = 0u;
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-          for (int g = 0; g < NG; ++g) {
-            if ((kp[x][g] & 0x7fffu) < NUMBERS) bk = __vmaxu2(bk, kp[x][g] & 0x7fff7fffu);
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              if ((vp[x][e][g] & 0x7fffu) >= NUMBERS) {
-                atomicMin(&s_none[g], pos + 2 * (t4 + 4 * x) + e);
-                vp[x][e][g] = 0u;
-              }
-              bv = __vmaxu2(bv, vp[x][e][g] & 0x7fff7fffu);
-            }
-          }
-      }
       const int nxt = turn + KP_RING;
       if ((nxt & 31) == 0) entry = nxt + lane < turns ? table[KP_SETS * (nxt + lane)] : 0;
       const int page = __shfl_sync(0xffffffffu, entry, nxt & 31);
@@ -236,8 +226,6 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
         mbar_expect_tx(&full[st], SLICE);
         bulk_load_1d(mine + st * SLICE, from + min(max(page, 0), a.pages - 1) * page_bytes, SLICE, &full[st]);
       }
-      const int ek = slice_exponent<T>(bk), ev = slice_exponent<T>(bv);
-      const float fk = pow2(-ek), fv = pow2(-ev);
       // keys: row = slot, 8 bytes of four dimensions at a time
       ok = __all_sync(0xffffffffu, kp_wait(&k_empty[ks], ((n / KP_STAGES) & 1) ^ 1, s_fail, a.word, 2));
       if (!ok) break;
@@ -247,14 +235,13 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
 #pragma unroll
         for (int i = 0; i < W; ++i) {
           const float2 p = bits_pair<T>(kp[x][i * NG / W]);
-          const __half2 s = __float2half2_rn(p.x * fk), lo = __float2half2_rn(p.y * fk);
+          const __half2 s = __float2half2_rn(p.x), lo = __float2half2_rn(p.y);
           uint8_t* row = sk + ks * Shape::K + (i >> 1) * KP_KBOX + r * 128;
           const int c = 4 * (i & 1) + (t4 >> 1), b = 8 * (t4 & 1);      // 16-byte piece of dimensions 32 i + 4 t4 in the row, 8 bytes in it
           *reinterpret_cast<uint2*>(row + ((c ^ (r & 7)) << 4) + b) = make_uint2(word_pair<0>(kw[x][i], s, lo), word_pair<1>(kw[x][i], s, lo));
           *reinterpret_cast<uint2*>(row + (((c + 2) ^ (r & 7)) << 4) + b) = make_uint2(word_pair<2>(kw[x][i], s, lo), word_pair<3>(kw[x][i], s, lo));
         }
       }
-      if (lane == 0) s_ek[(n & (KP_EXPS - 1)) * 4 + sl] = (signed char)ek, s_ev[(n & (KP_EXPS - 1)) * 4 + sl] = (signed char)ev;
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(&k_full[ks]);
@@ -266,7 +253,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
 #pragma unroll
         for (int i = 0; i < W; ++i) {
           const float2 p0 = bits_pair<T>(vp[x][0][i * NG / W]), p1 = bits_pair<T>(vp[x][1][i * NG / W]);
-          const __half2 s = __floats2half2_rn(p0.x * fv, p1.x * fv), lo = __floats2half2_rn(p0.y * fv, p1.y * fv);
+          const __half2 s = __floats2half2_rn(p0.x, p1.x), lo = __floats2half2_rn(p0.y, p1.y);
           uint8_t* at = sv + ks * Shape::V + (32 * i + g8) * 128 + (((2 * sl + x) ^ g8) << 4) + 4 * t4;
           *reinterpret_cast<uint32_t*>(at) = word_pair<0>(vw[x][i], s, lo);
           *reinterpret_cast<uint32_t*>(at + 8 * 128) = word_pair<1>(vw[x][i], s, lo);
@@ -399,7 +386,6 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t ts0 = tmem + lanes + TM_S + 128u * tile, to = tmem + lanes + TM_O + 128u * tile;
     float ref = -INFINITY, sum = 0.f;
-    int ebase = -128;                                                   // the power of two that O stands under
     bool ok = true;
     bool far = false;                                                   // a reference past 2^24: a product and a rounded one of the same numbers differ
     const int count = max(0, myhi - page0 + 1);
@@ -411,15 +397,6 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
       tc_fence_after();
       uint32_t sr[32];
       tmem_ld32_async(ts + 32u * half, sr);
-      // (exponents that are all 0, as they mostly are, cost two loads and a comparison)
-      const uint32_t eks = reinterpret_cast<const uint32_t*>(s_ek)[n & (KP_EXPS - 1)], evs = reinterpret_cast<const uint32_t*>(s_ev)[n & (KP_EXPS - 1)];
-      float mul0 = mul, mul1 = mul;                                     // of the thread's two slices
-      int emax = 0, ev0 = 0, ev1 = 0;
-      if ((eks | evs) != 0u) {
-        mul0 *= pow2((int)(signed char)(eks >> (16 * half))), mul1 *= pow2((int)(signed char)(eks >> (16 * half + 8)));
-        ev0 = (int)(signed char)(evs >> (16 * half)), ev1 = (int)(signed char)(evs >> (16 * half + 8));
-        emax = max(max((int)(signed char)evs, (int)(signed char)(evs >> 8)), max((int)(signed char)(evs >> 16), (int)(signed char)(evs >> 24)));
-      }
       tmem_wait_ld();
       tie32(sr);
       const int cmax = qp - ((page0 + n) * KV4_PAGE + 32 * half);       // the row's last visible column of these 32
@@ -432,20 +409,19 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
       float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
       for (int e = 0; e < 32; e += 2) m4[e >> 3] = at_max3(m4[e >> 3], __uint_as_float(sr[e]), __uint_as_float(sr[e + 1]));
-      float mx = fmaxf(fmaxf(m4[0], m4[1]) * mul0, fmaxf(m4[2], m4[3]) * mul1);
+      const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * mul;
       __syncwarp();      // the stores to tensor memory below are the whole warp's: lanes part above this line and not between it and them
-      // (one barrier of the rows' two warps per page: does any row's reference have to move, or the exponent, has any wait run out?)
-      if (at_any(bar, !ok || mx > ref + AT_SLACK || (ref == -INFINITY && mx > -INFINITY) || emax > ebase)) {
+      // (one barrier of the rows' two warps per page: does any row's reference have to move, has any wait run out?  The difference is exact where a sum
+      // with the slack would be rounded; it is no number where a row has seen nothing.)
+      if (at_any(bar, !ok || mx - ref > KP_SLACK)) {
         *own = mx;
         ok = !at_any(bar, !ok);
         if (!ok) break;
-        const float nref = fmaxf(ref, fmaxf(mx, *other));
-        const int nbase = max(ebase, emax);
-        const float g = ref == -INFINITY ? 0.f : at_exp2(ref - nref), f = g * pow2(max(ebase - nbase, -126));
+        const float nref = fmaxf(ref, fmaxf(mx, *other) - KP_UP);
+        const float f = ref == -INFINITY ? 0.f : at_exp2(ref - nref);
         ref = nref;
         far = __any_sync(0xffffffffu, fabsf(ref) > 16777216.f && ref != -INFINITY);
-        ebase = nbase;
-        sum *= g;
+        sum *= f;
         if (n > 0) ok = kp_wait(&o_full[2 * tile + ((n - 1) & 1)], ((n - 1) >> 1) & 1, s_fail, a.word, 9);
         __syncwarp();
         tc_fence_after();
@@ -470,7 +446,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
       const float sub = ref == -INFINITY ? 0.f : -ref;
       uint32_t ph[16];
       f2 part[2] = {f2_of(0.f, 0.f), f2_of(0.f, 0.f)};
-      if ((eks | evs) == 0u && ebase == 0 && !far) {                    // (as mostly)
+      if (!far) {
         const f2 m2 = f2_of(mul, mul), s2 = f2_of(sub, sub);
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
@@ -481,14 +457,12 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
           ph[e] = pair_bits<__half>(p0, p1);
         }
       } else {
-        const float f0 = pow2(max(ev0 - ebase, -126)), f1 = pow2(max(ev1 - ebase, -126));
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float mm = e < 8 ? mul0 : mul1, f = e < 8 ? f0 : f1;
-          const float s0 = __uint_as_float(sr[2 * e]), s1 = __uint_as_float(sr[2 * e + 1]);      // (-inf: masked, whatever mm may have come to)
-          const float p0 = s0 == -INFINITY ? 0.f : at_exp2(__fadd_rn(__fmul_rn(s0, mm), sub)), p1 = s1 == -INFINITY ? 0.f : at_exp2(__fadd_rn(__fmul_rn(s1, mm), sub));
+          const float s0 = __uint_as_float(sr[2 * e]), s1 = __uint_as_float(sr[2 * e + 1]);
+          const float p0 = s0 == -INFINITY ? 0.f : at_exp2(__fadd_rn(__fmul_rn(s0, mul), sub)), p1 = s1 == -INFINITY ? 0.f : at_exp2(__fadd_rn(__fmul_rn(s1, mul), sub));
           part[e & 1] = f2_add(part[e & 1], f2_of(p0, p1));
-          ph[e] = pair_bits<__half>(p0 * f, p1 * f);
+          ph[e] = pair_bits<__half>(p0, p1);
         }
       }
       float p0, p1;
@@ -505,13 +479,14 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
     __syncwarp();
     tc_fence_after();
     *own = sum;
-    if (!at_any(bar, !ok)) {
+    // (what a tile gives that sees a group out of range counts for nothing: kv4_few_kernel has its walk)
+    if (!at_any(bar, !ok) && s_odd[tile] == 0) {
       const float den = half == 0 ? sum + *other : *other + sum;        // the halves' sums in the order of the keys
       const size_t part_at = ((size_t)(it.base + it.part) * a.G + head) * KV4_MANY + tile * KP_ROWS + row;
       const bool whole = it.parts == 1;
       if (!whole && live && half == 0)
         *reinterpret_cast<float2*>(a.part + (size_t)a.kept * a.G * KV4_MANY * D + part_at * 2) = make_float2(ref == -INFINITY ? KV4_NONE : ref, den);
-      const float fin = pow2(max(min(ebase, 126), -126)) / (whole ? den : 1.f);
+      const float f = whole ? 1.f / den : 1.f;
       if (count > 0) {
 #pragma unroll
         for (int z = 32 * half; z < D; z += 64) {
@@ -519,7 +494,6 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
           tmem_ld32_async(to + (uint32_t)z, o);
           tmem_wait_ld();
           tie32(o);
-          const float f = s_none[z * NG / D] <= qp ? NAN : fin;         // (a value that is none, at a position that the row sees)
           if (live) {
             if (whole) {
               T* dst = y + out_row * D + z;
@@ -549,6 +523,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
+  if (threadIdx.x == 0) a.odd[blockIdx.x] = s_odd[0] | s_odd[1] << 1;
 }
 
 template <typename T, int D, int NG>

@@ -18,6 +18,7 @@ struct Kv4Attn {
   int items, kept, cols;      // items there is room for, parts whose sums there is room for, columns of a tile that may be in use
   float scale;
   int* word;           // wait_word()
+  int* odd;            // [items][G] of the tcgen05 kernel: bit 0, 1: its tile 0, 1 is left to the kernel of few columns
 };
 
 namespace {
@@ -58,12 +59,13 @@ __device__ __forceinline__ int column_head(int c, int R) { return (R & (R - 1)) 
 
 constexpr float KV4_NONE = -1e37f;      // the reference of a column that has seen no key
 
-// Sequences that bring up to KV4_FEW_MOST columns a key head go to the kernel of few columns, others to the tcgen05 kernel in tiles of KV4_MANY.
+// Sequences that bring up to KV4_FEW_MOST columns a key head go to the kernel of few columns (in tiles of KV4_FEW_BESIDE beside the others), others to the
+// tcgen05 kernel in tiles of KV4_MANY.
 // us, few / tcgen05, heads of 128, 2000 keys: 32 heads over 32, one request of 16, 32, 48 tokens 15.6 / 22.7, 19.3 / 22.9, 22.9 / 23.3, eight requests 41 / 86,
 // 54 / 86, 116 / 86; 32 heads over 8, one of 8, 16, 24 tokens 15.2 / 21.5, 15.5 / 22.0, 19.0 / 22.8, eight 27 / 33, 41 / 34, 62 / 35.
 // Where no request of the cache has more than KV4_WHOLE pages, walks are not cut, and the launch that joins parts falls away (30 to 500 keys of 32 heads, whole /
 // cut: one request 3.7 - 6.1 / 4.7 - 6.3, 64 requests 13.8 - 34.8 / 14.8 - 36.1).
-constexpr int KV4_FEW_MOST = 32, KV4_MANY = 256, KV4_WHOLE = 8;
+constexpr int KV4_FEW_MOST = 32, KV4_FEW_BESIDE = 8, KV4_MANY = 256, KV4_WHOLE = 8;
 // Walks for KV4_ROUNDS rounds of blocks stay whole; fewer are cut into at most KV4_CUTS rounds more of parts.
 constexpr int KV4_ROUNDS = 3, KV4_CUTS = 2;
 
@@ -85,7 +87,7 @@ struct Kv4Lists {
     R = H / G;
     many = kv4_many(max_count, R);
     const long long c = (long long)max_count * R;
-    cols = many ? 8 : c <= 4 ? 4 : c <= 8 ? 8 : 16;
+    cols = many ? KV4_FEW_BESIDE : c <= 4 ? 4 : c <= 8 ? 8 : 16;
     few = many ? KV4_FEW_MOST : INT_MAX;
     few_parts = std::max(1, 4 * kv4_sms() / G);
     many_parts = std::max(1, kv4_sms() / G);
@@ -106,7 +108,9 @@ struct Kv4Lists {
   int few_kept() const { return (int)std::min(few_items, (long long)(KV4_ROUNDS + KV4_CUTS) * few_parts); }
   int many_kept() const { return (int)std::min(many_items, (long long)(KV4_ROUNDS + KV4_CUTS) * many_parts); }
   size_t few_floats(int G, int D) const { return ((size_t)few_kept() * G * cols * (D + 2) + 3) / 4 * 4; }
-  size_t floats(int G, int D) const { return few_floats(G, D) + (size_t)many_kept() * G * KV4_MANY * (D + 2); }
+  size_t many_floats(int G, int D) const { return (size_t)many_kept() * G * KV4_MANY * (D + 2); }
+  // sums of both lists, and a word for every block of the many
+  size_t bytes(int G, int D) const { return sizeof(float) * (few_floats(G, D) + many_floats(G, D)) + sizeof(int) * (size_t)many_items * G; }
 };
 
 }  // namespace

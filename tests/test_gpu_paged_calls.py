@@ -1,11 +1,12 @@
-"""Calls of the paged 4-bit cache at the ends of what it allows."""
+"""Calls of the paged 4-bit cache at the ends of what it allows: steps that are divided whole, single tokens of any stride, counts of nothing, results
+in place, the wait check of a batch."""
 import sys
 from pathlib import Path
 
 import pytest
 import torch
 
-from tests.test_gpu_paged_cache import BF, DEV, _cache, _filled, _near
+from tests.test_gpu_paged_cache import BF, DEV, HF, _cache, _filled, _near
 
 pytestmark = pytest.mark.gpu
 
@@ -66,6 +67,25 @@ def test_a_step_whose_sequences_may_bring_nothing(max_length):
         q, out = torch.randn(5, H, 64, device=DEV).to(BF), torch.full((5, H, 64), 7.0, dtype=BF, device=DEV)
         y = cache.attend(0, plan, q, out=out)
         assert bool(y[:3].isnan().all()) and bool((y[3:] == 7.0).all())
+
+
+@pytest.mark.parametrize("held, counts, H, G", [([70, 3], [1, 1], 4, 2), ([1900], [1], 8, 8), ([300, 5], [9, 3], 8, 2), ([300, 0], [130, 200], 8, 2), ([2000, 1], [300, 1], 8, 8)])
+@pytest.mark.parametrize("large", [False, True])
+@torch.no_grad()
+def test_results_over_their_queries(held, counts, H, G, large):
+    """``out`` may be the queries themselves."""
+    cache, plan, q, k, v = _filled(held, counts, H, G, 64, 32, BF)
+    if large:                                                 # values that a product of fp16 operands does not hold
+        k, v = (x.clone() for x in cache.brought)
+        v[0, :, 3] = 1e6
+        rows, total = plan.request.tolist(), [a + b for a, b in zip(held, counts)]
+        cache.truncate(rows, [0] * len(rows))
+        cache.append(0, cache.plan(rows, total, sum(total)), None, k.to(DEV), v.to(DEV))
+        cache.truncate(rows, held)
+        plan = cache.plan(rows, counts, sum(counts), max_count=max(counts))
+    want = cache.attend(0, plan, q.to(DEV))
+    mine = q.to(DEV)
+    assert cache.attend(0, plan, mine, out=mine) is mine and torch.equal(mine, want)
 
 
 @torch.no_grad()

@@ -46,7 +46,7 @@ def _columns(count, D=128, G=2, R=1, L=300, dtype=BF, spread=0.1):
     return k.to(dtype), v.to(dtype), q.to(dtype)
 
 
-FORMS = [(2, 1, BF, 64), (2, 1, HF, 64), (7, 1, BF, 32), (7, 1, HF, 128), (15, 2, BF, 64)]
+FORMS = [(2, 1, BF, 64), (2, 1, HF, 64), (7, 1, BF, 32), (7, 1, HF, 128), (15, 2, BF, 64), (64, 1, BF, 64), (130, 2, HF, 32), (250, 1, BF, 128), (290, 2, BF, 64)]
 
 
 @pytest.mark.parametrize("count, R, dtype, group", FORMS)
@@ -98,7 +98,7 @@ def test_a_value_in_sight_without_weight(count, R, dtype, group, size, at):
     assert first == 0 or torch.isfinite(got).all()
 
 
-@pytest.mark.parametrize("count, R, group", [(2, 1, 64), (3, 1, 32), (9, 1, 64), (15, 2, 64)])
+@pytest.mark.parametrize("count, R, group", [(2, 1, 64), (3, 1, 32), (9, 1, 64), (15, 2, 64), (40, 1, 64), (150, 1, 32), (180, 2, 64)])
 @pytest.mark.parametrize("large", [1100.0, 1e9])
 @pytest.mark.parametrize("hidden", [False, True])
 @torch.no_grad()
@@ -120,7 +120,7 @@ def test_many_small_weights_beside_a_first_token(count, R, group, large, hidden)
     _check(got[:n], q[:n], K[:held + n], V[:held + n], held, group, BF, 128 ** -0.5)
 
 
-@pytest.mark.parametrize("count, R, group", [(1, 1, 32), (4, 1, 32), (9, 1, 64), (16, 2, 32)])
+@pytest.mark.parametrize("count, R, group", [(1, 1, 32), (4, 1, 32), (9, 1, 64), (16, 2, 32), (70, 1, 32), (300, 2, 64)])
 @torch.no_grad()
 def test_groups_of_very_unequal_size(count, R, group):
     """Groups of one token's values 2^40 apart, keys' alike: each group's result to its own size."""
@@ -133,7 +133,7 @@ def test_groups_of_very_unequal_size(count, R, group):
     _check(got, q, K, V, 330 - count, group, BF, 128 ** -0.5)
 
 
-@pytest.mark.parametrize("count, R, group", [(1, 1, 64), (6, 1, 32), (16, 2, 64)])
+@pytest.mark.parametrize("count, R, group", [(1, 1, 64), (6, 1, 32), (16, 2, 64), (90, 1, 32), (300, 2, 64)])
 @pytest.mark.parametrize("power", [-60, -20, -9, 0, 9, 20, 60])
 @torch.no_grad()
 def test_values_of_any_size(count, R, group, power):
@@ -146,7 +146,7 @@ def test_values_of_any_size(count, R, group, power):
 
 
 @pytest.mark.parametrize("grow", [1, 40])
-@pytest.mark.parametrize("count, R, dtype", [(1, 1, BF), (1, 1, HF), (6, 1, BF), (16, 2, HF)])
+@pytest.mark.parametrize("count, R, dtype", [(1, 1, BF), (1, 1, HF), (6, 1, BF), (16, 2, HF), (80, 1, BF)])
 @torch.no_grad()
 def test_scores_that_rise_over_values_that_fall(count, R, dtype, grow):
     """Scores that rise along the keys, so that references move again and again, over values that get smaller (grow 1: larger): what counts is the
