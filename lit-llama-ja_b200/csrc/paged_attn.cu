@@ -438,9 +438,10 @@ __device__ __forceinline__ bool few_walk(const Kv4Attn& a, const Kv4Item& it, in
   return true;
 }
 
-// A block an item and key head of the list `a`; beside a list `m` of the many there are blocks more, which go through the tiles that kv4_prompt_kernel has left (groups
-// that fp16 numbers do not hold), eight columns at a time.
-template <typename T, int D, int NG, int CPL, int NB>
+// A block an item and key head of the list `a`.  BESIDE a list `m` of the many there are blocks more, which go through the tiles that kv4_prompt_kernel has
+// left (groups that fp16 numbers do not hold), KV4_FEW_BESIDE columns at a time.  (A kernel of its own: with that walk in it too, twelve drafts of eight tokens
+// took 37 us instead of 36.)
+template <typename T, int D, int NG, int CPL, int NB, bool BESIDE>
 __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(const Kv4Attn a, const Kv4Attn m) {
   constexpr int COLS = 4 * CPL * NB;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -449,7 +450,7 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
   // it, so that what waits for this kernel waits for both.)
   if (blockIdx.x == gridDim.x - 1) pdl_wait();
   const int R = a.H / a.G, blocks = a.items * a.G;
-  if constexpr (COLS == KV4_FEW_BESIDE) {
+  if constexpr (BESIDE) {
     if ((int)blockIdx.x >= blocks) {      // (what these read the prompts' kernel has left)
       constexpr int SUBS = KV4_MANY / COLS;
       __shared__ uint32_t s_left[KF_WARPS];
@@ -628,24 +629,26 @@ int ll_kv4_attn(const ll_kv4_cache* cache, const void* blocks, const void* q, lo
       l.few_cut || l.many ? (unsigned)std::min<long long>(4ll * kv4_sms(), (long long)l.few_joins() * G * used + (l.many ? (long long)l.many_joins() * G * (KV4_MANY / KJ) : 0)) : 0;
   LL_CHECK_ARG(l.few_items * G + 4ll * kv4_sms() <= INT_MAX, "kv4_attn: %d sequences of %d tokens, %d heads", B, T, H);
   const unsigned few_blocks = (unsigned)(l.few_items * G) + (l.many ? 4u * kv4_sms() : 0u);
-#define FEW(TT, DD, NG, CPL, NB)                                                                                                              \
+#define FEW(TT, DD, NG, CPL, NB, BESIDE)                                                                                                      \
   {                                                                                                                                           \
+    static_assert(!BESIDE || 4 * CPL * NB == KV4_FEW_BESIDE, "columns beside the many");                                                      \
     constexpr int COLS = 4 * CPL * NB, ring = KF_WARPS * kf_stages(DD, NG) * 2 * kv4_slice_bytes(DD, NG), join = KF_WARPS * COLS * (DD + 4) * 4; \
     constexpr int smem = ring > join ? ring : join;                                                                                           \
     static PerDevice set;                                                                                                                     \
     if (!set) {                                                                                                                               \
-      LL_CUDA(cudaFuncSetAttribute(kv4_few_kernel<TT, DD, NG, CPL, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));                  \
-      prefer_max_smem(kv4_few_kernel<TT, DD, NG, CPL, NB>);                                                                                   \
+      LL_CUDA(cudaFuncSetAttribute(kv4_few_kernel<TT, DD, NG, CPL, NB, BESIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));                  \
+      prefer_max_smem(kv4_few_kernel<TT, DD, NG, CPL, NB, BESIDE>);                                                                                   \
       set.mark();                                                                                                                             \
     }                                                                                                                                         \
-    LL_CUDA(launch(kv4_few_kernel<TT, DD, NG, CPL, NB>, dim3(few_blocks), dim3(KF_THREADS), smem, st, l.many, a, m));           \
+    LL_CUDA(launch(kv4_few_kernel<TT, DD, NG, CPL, NB, BESIDE>, dim3(few_blocks), dim3(KF_THREADS), smem, st, l.many, a, m));           \
     LL_LAUNCH_OK("kv4_few_kernel");                                                                                                           \
     if (join_blocks > 0) LL_CUDA(launch(kv4_join_kernel<TT, DD, COLS>, dim3(join_blocks), dim3(KJ * 32), 0, st, true, a, m));                          \
   }
-#define FEW_COLS(TT, DD, NG)              \
-  if (cols == 4) FEW(TT, DD, NG, 1, 1)    \
-  else if (cols == 8) FEW(TT, DD, NG, 2, 1) \
-  else FEW(TT, DD, NG, 2, 2)
+#define FEW_COLS(TT, DD, NG)                          \
+  if (l.many) FEW(TT, DD, NG, 2, 1, true)             \
+  else if (cols == 4) FEW(TT, DD, NG, 1, 1, false)    \
+  else if (cols == 8) FEW(TT, DD, NG, 2, 1, false)    \
+  else FEW(TT, DD, NG, 2, 2, false)
 #define ATTN(DD, NG)                                      \
   if (dtype == LL_BF16) { FEW_COLS(__nv_bfloat16, DD, NG) } \
   else { FEW_COLS(__half, DD, NG) }
