@@ -604,7 +604,7 @@ int ll_kv4_attn(const ll_kv4_cache* cache, const void* blocks, const void* q, lo
   LL_CHECK_ARG(q && blocks && cache->table && work && y && scratch && B > 0 && T > 0 && max_count >= 0 && G > 0 && G <= 65535 && H > 0 && H % G == 0 && cache->width > 0 &&
                    cache->pages > 0 && cache->max_length > 0 && (long long)T * H <= INT_MAX,
                "kv4_attn: %d tokens of %d heads, %d cached", T, H, G);
-  LL_CHECK_ARG(scale > 0.f, "kv4_attn: scores times %g (more than 0)", scale);
+  LL_CHECK_ARG(scale > 0.f && scale < INFINITY, "kv4_attn: scores times %g (more than 0, and a number of 32 bits)", scale);
   LL_CHECK_ARG((((uintptr_t)q | (uintptr_t)y | (uintptr_t)blocks | (uintptr_t)scratch | (uintptr_t)work) & 15) == 0 && q_row % 8 == 0,
                "kv4_attn: rows have to start on 16-byte boundaries");
   const Kv4Lists l(B, T, max_count, H, G, cache->max_length);
