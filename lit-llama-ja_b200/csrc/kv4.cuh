@@ -25,13 +25,6 @@ __host__ __device__ constexpr int kv4_v_params(int D, int groups) { return KV4_S
 __host__ __device__ constexpr int kv4_slice_bytes(int D, int groups) { return KV4_SLICE * (D + 8 * groups); }
 __host__ __device__ constexpr int kv4_bytes(int D, int groups) { return KV4_PAGE / KV4_SLICE * kv4_slice_bytes(D, groups); }
 
-// where dimension d of a slot's key lies: word within the slot, bit within the word
-__device__ __forceinline__ int kv4_k_word(int D, int d) { return ((d & 15) >> 2) * (D / 32) + (d >> 5); }
-__device__ __forceinline__ int kv4_k_bit(int d) { return 16 * (d & 1) + 4 * (2 * ((d >> 4) & 1) + ((d >> 1) & 1)); }
-// where dimension d of a value lies: word within the pair, bit within the slot's half of it
-__device__ __forceinline__ int kv4_v_word(int D, int d) { return (d & 7) * (D / 32) + (d >> 5); }
-__device__ __forceinline__ int kv4_v_bit(int d) { return 4 * ((d >> 3) & 3); }
-
 template <typename T> struct pair_of;
 template <> struct pair_of<__nv_bfloat16> { typedef __nv_bfloat162 type; };
 template <> struct pair_of<__half> { typedef __half2 type; };

@@ -149,8 +149,8 @@ class PagedCache4:
 
     def plan(self, rows: Whole, counts: Whole, tokens: int, *, max_count: Optional[int] = None) -> CachePlan:
         """Give the step's ``tokens`` rows their slots: the next ``counts[i]`` of them are sequence i's, the continuation of request ``rows[i]``.  A sequence
-        may bring nothing; one that cannot be served is refused whole (``CachePlan.status``), its tokens get no slot and come out of ``append`` and
-        ``attend`` as no numbers.  ``max_count``: the most that a sequence brings (``tokens`` unless said); it goes into the choice of kernels.
+        may bring nothing; one that cannot be served is refused whole (``CachePlan.status``), its tokens get no slot and come out of ``attend`` as no numbers
+        (of ``append`` too where it turns queries; else these are the caller's).  ``max_count``: the most that a sequence brings (``tokens`` unless said); it goes into the choice of kernels.
         Plans of earlier steps end with this one."""
         rows, counts = self._whole("rows", rows), self._whole("counts", counts)
         if rows.shape != counts.shape or rows.numel() == 0:
