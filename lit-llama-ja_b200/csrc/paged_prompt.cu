@@ -6,9 +6,12 @@
 //   warps 20-27     : two sets that take the pages in turn, a warp a slice of 16 keys: codes by bulk copies into a ring, from there as fp16 numbers into
 //                     the operands.  (One set took 2600 clocks a page, and with it the block; 700 tokens over 5000 keys, 32 / 8 heads: 132 -> 125 us.)
 // All operands are fp16, whatever the cache's type: its 11 bits hold a query exactly (a row under a power of two of its own) and a key or value
-// c s + lo rounded once, where bf16 would lose three bits more.  What fp16 numbers do not hold (group_fits) is left to the walk of few columns: a tile that
-// sees such a group, or one that is no number, stores nothing and is named in `odd`.  (Powers of two by slices of keys cost the keys and values beside a large
-// one their bits, also in rows that do not see it, and 3 to 14 us of the three prompts below.)
+// c s + lo rounded once, where bf16 would lose three bits more.  Where the result is fp16, whose 11 bits show that, keys are two terms (split_terms), and
+// weights too: five prompts of up to 3333, 8 heads of 64, differ from 64 bits by 0.00028 of their norm instead of 0.00064 (0.00034 with the keys' terms
+// alone), in 158 us instead of 134.  (Values as two terms instead of weights: 0.00029, 180 us.  Eight warps unpack, sixteen weigh.)
+// What fp16 numbers do not hold (group_fits) is left to the walk of few columns: a tile that sees such a group, or one that is no number, stores nothing and
+// is named in `odd`.  (Powers of two by slices of keys cost what stands beside a large number its bits, also in rows that do not see it, and 3 to 14 us of the
+// prompts here.)
 // A word's codes become pairs by masks: 1024 + c under exponent bits, from which one operation takes the 1024 (of odd nibbles, 1024 + 16 c, 64 + c), and
 // one more multiplies and adds.  Keys' pairs run along the dimensions, values' along the keys: values stand with the keys in a row, so that both
 // operands are K-major.
@@ -31,17 +34,19 @@ constexpr int KP_ROWS = 128, KP_SOFTMAX = 16, KP_FIRST = KP_SOFTMAX + 4, KP_SETS
 constexpr int KP_REGS = 72, KP_REGS_SOFTMAX = 88, KP_REGS_MMA = 40, KP_REGS_DEQUANT = 56;
 static_assert(KP_THREADS * KP_REGS <= 65536 && KP_SOFTMAX * KP_REGS_SOFTMAX + 4 * KP_REGS_MMA + KP_DEQUANT * KP_REGS_DEQUANT <= KP_THREADS / 32 * KP_REGS, "registers");
 constexpr int KP_QBOX = KP_ROWS * 128, KP_KBOX = KV4_PAGE * 128;      // 64 numbers of 16 bits a row
-constexpr int KP_RING = 2, KP_STAGES = 3;                            // copies in flight a slice of a set; pages of K and of V
+constexpr int KP_COPIES = 2;                                         // in flight a slice of a set
 // A row's largest weight is 2^KP_UP or more, so that a weight in fp16 comes to nothing under 2^-31 of it only, and under 2^15: its scores may outgrow the
 // reference by KP_SLACK before it moves.
 constexpr float KP_UP = 6.f, KP_SLACK = KP_UP + AT_SLACK;
 
-template <int D, int NG>
+// TERMS: of a key and of a weight, two where the result is fp16.  STAGES: pages of K and of V.
+template <typename T, int D, int NG>
 struct KpShape {
+  static constexpr int TERMS = std::is_same<T, __half>::value ? 2 : 1, STAGES = TERMS == 2 && D == 128 ? 2 : 3;
   static constexpr int NB = (D + 63) / 64, SLICE = kv4_slice_bytes(D, NG);
-  static constexpr int Q = 2 * NB * KP_QBOX, K = NB * KP_KBOX, V = D * 128;
-  static constexpr int RING = KP_DEQUANT * KP_RING * SLICE;
-  static constexpr int SMEM = 1024 + Q + KP_STAGES * (K + V) + RING + 512 + 6 * KP_ROWS * 4;
+  static constexpr int Q = 2 * NB * KP_QBOX, K = TERMS * NB * KP_KBOX, V = D * 128;
+  static constexpr int RING = KP_DEQUANT * KP_COPIES * SLICE, SPLIT = TERMS == 2 ? KP_DEQUANT * KV4_SLICE * NG * 16 : 0;
+  static constexpr int SMEM = 1024 + Q + STAGES * (K + V) + RING + SPLIT + 512 + 6 * KP_ROWS * 4;
 };
 
 __device__ __forceinline__ void kp_ran_out(volatile int* fail, int* word, int code) {
@@ -85,11 +90,28 @@ __device__ __forceinline__ uint32_t word_pair(uint32_t w, __half2 s, __half2 lo)
                             : __hadd2(as_half2((u & 0x000f000fu) | 0x64006400u), __half2half2(__ushort_as_half(0xe400)));      // (1/16, -64; -1024)
   return as_u32(__hfma2(c, s, lo));
 }
+// Two terms of such pairs.  With m the code next to 0, s1 the first seven bits of s and s2 the others, c s + lo = (c - m) s1 + ((c - m) s2 + (lo + m s)).  The
+// first term is exact in 11 bits; the second is under s where the group's range holds 0, so that its rounding is 2^-12 of s (of |lo| where it does not,
+// as one term's).  x: -1024 - m, y: s1, z: s2, w: lo + m s, twice each.
+__device__ __forceinline__ uint4 split_terms(uint32_t params) {
+  const float2 p = __half22float2(as_half2(params));
+  const float m = p.x > 0.f ? fminf(fmaxf(rintf(__fdividef(-p.y, p.x)), 0.f), 15.f) : 0.f;
+  const __half2 s = as_half2(__byte_perm(params, params, 0x1010)), s1 = as_half2(as_u32(s) & 0xfff0fff0u);
+  return make_uint4(as_u32(__float2half2_rn(-1024.f - m)), as_u32(s1), as_u32(__hsub2(s, s1)), as_u32(__float2half2_rn(fmaf(m, p.x, p.y))));
+}
+template <int N>
+__device__ __forceinline__ void word_terms(uint32_t w, uint4 t, uint32_t& a, uint32_t& b) {
+  const uint32_t u = N >= 2 ? w >> 8 : w;
+  const __half2 even = as_half2(t.x), odd = __hadd2(even, __half2half2(__ushort_as_half(0x6380)));      // (960)
+  const __half2 c = (N & 1) ? __hfma2(as_half2((u & 0x00f000f0u) | 0x64006400u), __half2half2(__ushort_as_half(0x2c00)), odd)
+                            : __hadd2(as_half2((u & 0x000f000fu) | 0x64006400u), even);
+  a = as_u32(__hmul2(c, as_half2(t.y))), b = as_u32(__hfma2(c, as_half2(t.z), as_half2(t.w)));
+}
 
 template <typename T, int D, int NG>
 __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn a) {
-  using Shape = KpShape<D, NG>;
-  constexpr int NB = Shape::NB, SLICE = Shape::SLICE, W = D / 32, BYTES = kv4_bytes(D, NG);
+  using Shape = KpShape<T, D, NG>;
+  constexpr int TERMS = Shape::TERMS, STAGES = Shape::STAGES, NB = Shape::NB, SLICE = Shape::SLICE, W = D / 32, BYTES = kv4_bytes(D, NG);
   constexpr uint32_t TM_S = 0, TM_O = 256;            // per tile: two score buffers of 64 columns; 128 accumulator columns
   extern __shared__ __align__(1024) uint8_t smem[];
   const int item = blockIdx.x / a.G, head = blockIdx.x - item * a.G;
@@ -109,21 +131,21 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem) + 1023) & ~(uintptr_t)1023);
   uint8_t* sq = base;                                 // [2 tiles][NB][128][64]
   uint8_t* sk = sq + Shape::Q;                        // [stage][NB][64 keys][64]
-  uint8_t* sv = sk + KP_STAGES * Shape::K;            // [stage][D][64 keys]
-  uint8_t* ring = sv + KP_STAGES * Shape::V;          // [slice][stage]
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(ring + Shape::RING);
+  uint8_t* sv = sk + STAGES * Shape::K;            // [stage][D][64 keys]
+  uint8_t* ring = sv + STAGES * Shape::V;          // [slice][stage]
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(ring + Shape::RING + Shape::SPLIT);
   uint64_t* k_full = q_full + 1;
-  uint64_t* k_empty = k_full + KP_STAGES;
-  uint64_t* v_full = k_empty + KP_STAGES;
-  uint64_t* v_empty = v_full + KP_STAGES;
-  uint64_t* s_full = v_empty + KP_STAGES;             // [tile][buffer] scores are there
+  uint64_t* k_empty = k_full + STAGES;
+  uint64_t* v_full = k_empty + STAGES;
+  uint64_t* v_empty = v_full + STAGES;
+  uint64_t* s_full = v_empty + STAGES;             // [tile][buffer] scores are there
   uint64_t* p_full = s_full + 4;                      // [tile][buffer] weights are there
   uint64_t* o_full = p_full + 4;                      // [tile][buffer] P V is done
   uint64_t* r_full = o_full + 4;                      // [slice][stage]
-  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(r_full + KP_DEQUANT * KP_RING);
+  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(r_full + KP_DEQUANT * KP_COPIES);
   int* s_fail = reinterpret_cast<int*>(tmem_ptr + 1);
   volatile int* s_odd = s_fail + 1;                   // [tile] whether the tile sees a group that fp16 numbers do not hold
-  float* s_x = reinterpret_cast<float*>(ring + Shape::RING + 512);      // [tile][half][row]: what the two threads of a row tell one another
+  float* s_x = reinterpret_cast<float*>(ring + Shape::RING + Shape::SPLIT + 512);      // [tile][half][row]: what the two threads of a row tell one another
   float* s_mul = s_x + 4 * KP_ROWS;                   // [2 tiles][row] what a row's raw scores are multiplied by
 
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
@@ -140,18 +162,19 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
   const int32_t* table = a.table + (size_t)it.row * a.width + page0 + set;
   const uint8_t* from = a.blocks + (size_t)head * BYTES + sl * SLICE;
   const size_t page_bytes = (size_t)a.G * BYTES;
-  uint8_t* mine = ring + dq * KP_RING * SLICE;
-  uint64_t* full = r_full + dq * KP_RING;
+  uint8_t* mine = ring + dq * KP_COPIES * SLICE;
+  uint64_t* full = r_full + dq * KP_COPIES;
+  uint8_t* split = ring + Shape::RING + dq * (KV4_SLICE * NG * 16);
   int entry = 0;
   if (dq >= 0) {
     entry = lane < turns ? table[KP_SETS * lane] : 0;
     if (lane == 0) {
-      for (int i = 0; i < KP_RING; ++i) mbar_init(&full[i], 1);
+      for (int i = 0; i < KP_COPIES; ++i) mbar_init(&full[i], 1);
       fence_barrier_init();
     }
     __syncwarp();
 #pragma unroll
-    for (int i = 0; i < KP_RING; ++i) {
+    for (int i = 0; i < KP_COPIES; ++i) {
       const int page = __shfl_sync(0xffffffffu, entry, i);
       if (lane == 0 && i < turns) {
         mbar_expect_tx(&full[i], SLICE);
@@ -161,7 +184,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
   }
   if (threadIdx.x == 0) {
     mbar_init(q_full, KP_SOFTMAX);
-    for (int i = 0; i < KP_STAGES; ++i) mbar_init(&k_full[i], 4), mbar_init(&k_empty[i], 2), mbar_init(&v_full[i], 4), mbar_init(&v_empty[i], 2);
+    for (int i = 0; i < STAGES; ++i) mbar_init(&k_full[i], 4), mbar_init(&k_empty[i], 2), mbar_init(&v_full[i], 4), mbar_init(&v_empty[i], 2);
     for (int i = 0; i < 4; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], KP_SOFTMAX / 2), mbar_init(&o_full[i], 1);
     *s_fail = s_odd[0] = s_odd[1] = 0;
     fence_barrier_init();
@@ -181,8 +204,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
     bool ok = true;
 #pragma unroll 1
     for (int turn = 0; turn < turns; ++turn) {
-      const int n = KP_SETS * turn + set, st = turn % KP_RING, ks = n % KP_STAGES;
-      ok = __all_sync(0xffffffffu, kp_wait(&full[st], (turn / KP_RING) & 1, s_fail, a.word, 1));
+      const int n = KP_SETS * turn + set, st = turn % KP_COPIES, ks = n % STAGES;
+      ok = __all_sync(0xffffffffu, kp_wait(&full[st], (turn / KP_COPIES) & 1, s_fail, a.word, 1));
       if (!ok) break;
       const uint8_t* blk = mine + st * SLICE;
       uint32_t kw[2][W], vw[2][W];
@@ -218,7 +241,14 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
               if (pos + 2 * (t4 + 4 * x) + e > last) vp[x][e][g] = 0u;
           }
       }
-      const int nxt = turn + KP_RING;
+      if constexpr (TERMS == 2) {                     // (a lane splits the scales of a key's groups for the four that take the key)
+#pragma unroll
+        for (int z = lane; z < KV4_SLICE * NG; z += 32) {
+          const uint32_t p = *reinterpret_cast<const uint32_t*>(blk + kv4_k_params(D) + 4 * z);
+          reinterpret_cast<uint4*>(split)[z] = split_terms(pos + z / NG <= last ? p : 0u);
+        }
+      }
+      const int nxt = turn + KP_COPIES;
       if ((nxt & 31) == 0) entry = nxt + lane < turns ? table[KP_SETS * (nxt + lane)] : 0;
       const int page = __shfl_sync(0xffffffffu, entry, nxt & 31);
       __syncwarp();                                   // every lane has read the slice
@@ -227,34 +257,49 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
         bulk_load_1d(mine + st * SLICE, from + min(max(page, 0), a.pages - 1) * page_bytes, SLICE, &full[st]);
       }
       // keys: row = slot, 8 bytes of four dimensions at a time
-      ok = __all_sync(0xffffffffu, kp_wait(&k_empty[ks], ((n / KP_STAGES) & 1) ^ 1, s_fail, a.word, 2));
+      ok = __all_sync(0xffffffffu, kp_wait(&k_empty[ks], ((n / STAGES) & 1) ^ 1, s_fail, a.word, 2));
       if (!ok) break;
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const int r = KV4_SLICE * sl + g8 + 8 * x;
 #pragma unroll
         for (int i = 0; i < W; ++i) {
-          const float2 p = bits_pair<T>(kp[x][i * NG / W]);
-          const __half2 s = __float2half2_rn(p.x), lo = __float2half2_rn(p.y);
           uint8_t* row = sk + ks * Shape::K + (i >> 1) * KP_KBOX + r * 128;
           const int c = 4 * (i & 1) + (t4 >> 1), b = 8 * (t4 & 1);      // 16-byte piece of dimensions 32 i + 4 t4 in the row, 8 bytes in it
-          *reinterpret_cast<uint2*>(row + ((c ^ (r & 7)) << 4) + b) = make_uint2(word_pair<0>(kw[x][i], s, lo), word_pair<1>(kw[x][i], s, lo));
-          *reinterpret_cast<uint2*>(row + (((c + 2) ^ (r & 7)) << 4) + b) = make_uint2(word_pair<2>(kw[x][i], s, lo), word_pair<3>(kw[x][i], s, lo));
+          uint8_t *const first = row + ((c ^ (r & 7)) << 4) + b, *const second = row + (((c + 2) ^ (r & 7)) << 4) + b;
+          if constexpr (TERMS == 2) {
+            const uint4 t = reinterpret_cast<const uint4*>(split)[(g8 + 8 * x) * NG + i * NG / W];
+            uint2 u, v;
+            word_terms<0>(kw[x][i], t, u.x, v.x), word_terms<1>(kw[x][i], t, u.y, v.y);
+            *reinterpret_cast<uint2*>(first) = u, *reinterpret_cast<uint2*>(first + NB * KP_KBOX) = v;
+            word_terms<2>(kw[x][i], t, u.x, v.x), word_terms<3>(kw[x][i], t, u.y, v.y);
+            *reinterpret_cast<uint2*>(second) = u, *reinterpret_cast<uint2*>(second + NB * KP_KBOX) = v;
+          } else {
+            const float2 p = bits_pair<T>(kp[x][i * NG / W]);
+            const __half2 s = __float2half2_rn(p.x), lo = __float2half2_rn(p.y);
+            *reinterpret_cast<uint2*>(first) = make_uint2(word_pair<0>(kw[x][i], s, lo), word_pair<1>(kw[x][i], s, lo));
+            *reinterpret_cast<uint2*>(second) = make_uint2(word_pair<2>(kw[x][i], s, lo), word_pair<3>(kw[x][i], s, lo));
+          }
         }
       }
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(&k_full[ks]);
       // values: row = dimension, a pair of slots at a time
-      ok = __all_sync(0xffffffffu, kp_wait(&v_empty[ks], ((n / KP_STAGES) & 1) ^ 1, s_fail, a.word, 3));
+      ok = __all_sync(0xffffffffu, kp_wait(&v_empty[ks], ((n / STAGES) & 1) ^ 1, s_fail, a.word, 3));
       if (!ok) break;
 #pragma unroll
       for (int x = 0; x < 2; ++x)
 #pragma unroll
         for (int i = 0; i < W; ++i) {
-          const float2 p0 = bits_pair<T>(vp[x][0][i * NG / W]), p1 = bits_pair<T>(vp[x][1][i * NG / W]);
-          const __half2 s = __floats2half2_rn(p0.x, p1.x), lo = __floats2half2_rn(p0.y, p1.y);
           uint8_t* at = sv + ks * Shape::V + (32 * i + g8) * 128 + (((2 * sl + x) ^ g8) << 4) + 4 * t4;
+          __half2 s, lo;
+          if constexpr (TERMS == 2) {
+            s = as_half2(__byte_perm(vp[x][0][i * NG / W], vp[x][1][i * NG / W], 0x5410)), lo = as_half2(__byte_perm(vp[x][0][i * NG / W], vp[x][1][i * NG / W], 0x7632));
+          } else {
+            const float2 p0 = bits_pair<T>(vp[x][0][i * NG / W]), p1 = bits_pair<T>(vp[x][1][i * NG / W]);
+            s = __floats2half2_rn(p0.x, p1.x), lo = __floats2half2_rn(p0.y, p1.y);
+          }
           *reinterpret_cast<uint32_t*>(at) = word_pair<0>(vw[x][i], s, lo);
           *reinterpret_cast<uint32_t*>(at + 8 * 128) = word_pair<1>(vw[x][i], s, lo);
           *reinterpret_cast<uint32_t*>(at + 16 * 128) = word_pair<2>(vw[x][i], s, lo);
@@ -276,17 +321,17 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
       const uint64_t qdesc = smem_desc_sw128(smem_u32(sq + i * NB * KP_QBOX));
       const uint64_t kdesc0 = smem_desc_sw128(smem_u32(sk)), vdesc0 = smem_desc_sw128(smem_u32(sv));
       auto scores = [&](int n) {
-        const int ks = n % KP_STAGES;
-        if (!kp_wait(&k_full[ks], (n / KP_STAGES) & 1, s_fail, a.word, 4)) return false;
+        const int ks = n % STAGES;
+        if (!kp_wait(&k_full[ks], (n / STAGES) & 1, s_fail, a.word, 4)) return false;
         tc_fence_after();
         if (page0 + n <= myhi) {
           const uint32_t d = tm_s + 64u * (n & 1);
           const uint64_t kdesc = kdesc0 + (uint64_t)(ks * (Shape::K >> 4));
 #pragma unroll
-          for (int c = 0; c < NB; ++c)
+          for (int c = 0; c < TERMS * NB; ++c)
 #pragma unroll
             for (int k = 0; k < (D < 64 ? D / 16 : 4); ++k)
-              umma_bf16(d, qdesc + (uint64_t)(c * (KP_QBOX >> 4) + 2 * k), kdesc + (uint64_t)(c * (KP_KBOX >> 4) + 2 * k), idesc_s, (c | k) != 0 ? 1u : 0u);
+              umma_bf16(d, qdesc + (uint64_t)(c % NB * (KP_QBOX >> 4) + 2 * k), kdesc + (uint64_t)(c * (KP_KBOX >> 4) + 2 * k), idesc_s, (c | k) != 0 ? 1u : 0u);
           umma_commit(&s_full[2 * i + (n & 1)]);
           umma_commit(&k_empty[ks]);
         } else {
@@ -299,16 +344,18 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
 #pragma unroll 1
       for (int n = 0; ok && n < units; ++n) {
         if (n + 1 < units && !(ok = scores(n + 1))) break;
-        const int vs = n % KP_STAGES;
-        if (!(ok = kp_wait(&v_full[vs], (n / KP_STAGES) & 1, s_fail, a.word, 6))) break;
+        const int vs = n % STAGES;
+        if (!(ok = kp_wait(&v_full[vs], (n / STAGES) & 1, s_fail, a.word, 6))) break;
         if (page0 + n <= myhi) {
           const uint32_t buf = n & 1;
           if (!(ok = kp_wait(&p_full[2 * i + (int)buf], (n >> 1) & 1u, s_fail, a.word, 7))) break;
           tc_fence_after();
           const uint64_t vdesc = vdesc0 + (uint64_t)(vs * (Shape::V >> 4));
 #pragma unroll
-          for (int k = 0; k < KV4_PAGE / UMMA_K; ++k)      // 16 keys: 8 columns of packed weights
-            umma_ts(tm_o, tm_s + 64u * buf + 32u * (k >> 1) + 8u * (k & 1), vdesc + (uint64_t)(2 * k), idesc_o, (n | k) != 0 ? 1u : 0u);
+          for (int k = 0; k < KV4_PAGE / UMMA_K; ++k)      // 16 keys: 8 columns of packed weights, a term
+#pragma unroll
+            for (int t = 0; t < TERMS; ++t)
+              umma_ts(tm_o, tm_s + 64u * buf + 32u * (k >> 1) + 16u * t + 8u * (k & 1), vdesc + (uint64_t)(2 * k), idesc_o, (n | k | t) != 0 ? 1u : 0u);
           umma_commit(&o_full[2 * i + (int)buf]);
           umma_commit(&v_empty[vs]);
         } else {
@@ -444,7 +491,15 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
         }
       }
       const float sub = ref == -INFINITY ? 0.f : -ref;
-      uint32_t ph[16];
+      uint32_t ph[16 * TERMS];
+      // weights as a pair, and what their 11 bits leave over
+      auto weights = [&](int e, float p0, float p1) {
+        ph[e] = pair_bits<__half>(p0, p1);
+        if constexpr (TERMS == 2) {
+          const float2 f = bits_pair<__half>(ph[e]);
+          ph[16 + e] = pair_bits<__half>(p0 - f.x, p1 - f.y);
+        }
+      };
       f2 part[2] = {f2_of(0.f, 0.f), f2_of(0.f, 0.f)};
       if (!far) {
         const f2 m2 = f2_of(mul, mul), s2 = f2_of(sub, sub);
@@ -454,7 +509,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
           f2_split(f2_fma(f2_of(__uint_as_float(sr[2 * e]), __uint_as_float(sr[2 * e + 1])), m2, s2), a0, a1);
           const float p0 = at_exp2(a0), p1 = at_exp2(a1);
           part[e & 1] = f2_add(part[e & 1], f2_of(p0, p1));
-          ph[e] = pair_bits<__half>(p0, p1);
+          weights(e, p0, p1);
         }
       } else {
 #pragma unroll
@@ -462,7 +517,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
           const float s0 = __uint_as_float(sr[2 * e]), s1 = __uint_as_float(sr[2 * e + 1]);
           const float p0 = s0 == -INFINITY ? 0.f : at_exp2(__fadd_rn(__fmul_rn(s0, mul), sub)), p1 = s1 == -INFINITY ? 0.f : at_exp2(__fadd_rn(__fmul_rn(s1, mul), sub));
           part[e & 1] = f2_add(part[e & 1], f2_of(p0, p1));
-          ph[e] = pair_bits<__half>(p0, p1);
+          weights(e, p0, p1);
         }
       }
       float p0, p1;
@@ -470,6 +525,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
       sum += p0 + p1;
       // the weights go over the thread's own scores
       tmem_st16(ts + 32u * half, ph);
+      if constexpr (TERMS == 2) tmem_st16(ts + 32u * half + 16u, ph + 16);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -528,7 +584,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Attn
 
 template <typename T, int D, int NG>
 int prompt_launch(const Kv4Attn& a, cudaStream_t st) {
-  constexpr int smem = KpShape<D, NG>::SMEM;
+  constexpr int smem = KpShape<T, D, NG>::SMEM;
   static_assert(smem <= 227 * 1024, "shared memory of a block");
   static PerDevice set;
   if (!set) {

@@ -201,3 +201,19 @@ def test_a_query_of_zeros_beside_others_under_a_tiny_scale(dtype):
     q[1] = 0
     got, K, V = _attended(q.to(dtype), k.to(dtype), v.to(dtype), 63, 64, scale=1e-7)
     assert float(got[0].abs().max()) <= 0.0 and float((got[1] - 1.0).abs().max()) <= 2.0 ** -8
+
+
+@pytest.mark.parametrize("D, group", [(32, 32), (64, 32), (64, 64), (128, 32), (128, 64), (128, 128)])
+@pytest.mark.parametrize("held, count, R", [(0, 300, 1), (500, 140, 2), (40, 30, 3)])
+@torch.no_grad()
+def test_fp16_prompts_are_as_exact_as_their_values(D, group, held, count, R):
+    """Scores that some large dimensions of the keys make: only a value's rounding to 11 bits and the result's are left to see.  Each is off by up to half a place,
+    2^-11, evenly spread: 2^-11 / sqrt(3) of it in the mean square at most; values of both signs add up as their errors do, so that the norm of both together
+    is sqrt(2 / 3) 2^-11 of the result's.  Weights and keys have 20 bits and more, sums in fp32 lose 2^-15 at most."""
+    torch.manual_seed(20)
+    G, L = 2, held + count
+    loud = torch.where(torch.arange(D) % 20 == 3, 6.0, 1.0)
+    k, v, q = (torch.randn(L, G, D) * loud).to(HF), torch.randn(L, G, D).to(HF), torch.randn(count, G * R, D).to(HF)
+    got, K, V = _attended(q, k, v, held, group)
+    want = attention(q, K, V, held, D ** -0.5)[0]
+    assert float((got - want).norm() / want.norm()) <= math.sqrt(2 / 3) * 2.0 ** -11 + 2.0 ** -15
