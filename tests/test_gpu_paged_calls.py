@@ -106,3 +106,35 @@ def test_a_batch_is_checked_when_it_is_done(monkeypatch):
     prompts = [torch.randint(0, 100, (n,), device=DEV) for n in (12, 3)]
     generate.generate_batch(m, prompts, 6, top_k=1)
     assert done == [True]
+
+
+@pytest.mark.parametrize("held, counts, H, G, dtype", [([300, 0], [130, 200], 8, 2, BF), ([2000, 1, 40], [300, 1, 0], 8, 8, HF), ([1500], [40], 16, 2, BF)])
+@torch.no_grad()
+def test_prompts_over_large_values_are_the_same_every_time(held, counts, H, G, dtype):
+    """Tiles that are left to the walk of few columns, in a captured step and beside another one: the same bits as alone."""
+    sets = []
+    for seed in (0, 1):
+        cache, plan, q, _, _ = _filled(held, counts, H, G, 128, 64, dtype, seed=seed)
+        k, v = (x.clone() for x in cache.brought)
+        v[::50, :, 3], k[7, :, 9] = 3e4, 2e4
+        rows, total = range(len(held)), [a + b for a, b in zip(held, counts)]
+        cache.reset()
+        cache.append(0, cache.plan(rows, total, sum(total)), None, k.to(DEV), v.to(DEV))
+        cache.truncate(rows, held)
+        plan = cache.plan(rows, counts, sum(counts), max_count=max(counts))
+        plan.check()
+        q = q.to(DEV)
+        want = cache.attend(0, plan, q)
+        assert bool(torch.isfinite(want).all()) and all(torch.equal(cache.attend(0, plan, q), want) for _ in range(5))
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = [cache.attend(0, plan, q) for _ in range(3)]
+        sets.append((cache, plan, q, want, g, out, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for _, _, _, _, g, _, s in sets:
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for *_, want, _, out, _ in sets:
+        assert all(torch.equal(x, want) for x in out)

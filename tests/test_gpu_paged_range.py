@@ -217,3 +217,22 @@ def test_fp16_prompts_are_as_exact_as_their_values(D, group, held, count, R):
     got, K, V = _attended(q, k, v, held, group)
     want = attention(q, K, V, held, D ** -0.5)[0]
     assert float((got - want).norm() / want.norm()) <= math.sqrt(2 / 3) * 2.0 ** -11 + 2.0 ** -15
+
+
+@pytest.mark.parametrize("D, group", [(32, 32), (64, 64), (128, 32), (128, 128)])
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("held, count, R", [(700, 1, 1), (300, 4, 1), (90, 1, 8), (200, 9, 1), (100, 16, 2)])
+@torch.no_grad()
+def test_few_columns_take_keys_as_they_are(D, group, dtype, held, count, R):
+    """Scores that large dimensions make, with nothing lost of keys and scales: 2^-18 of sum |q| |k| for sums in fp32 and the exponential, which moves a weight by
+    twice that; half a place of fp16 for a weight, which meets codes (its group's largest), and 2^-22 of that once a key; the result is rounded once."""
+    torch.manual_seed(21)
+    G, L = 2, held + count
+    loud = torch.where(torch.arange(D) % 20 == 3, 6.0, 1.0)
+    k, v, q = (torch.randn(L, G, D) * loud).to(dtype), torch.randn(L, G, D).to(dtype), torch.randn(count, G * R, D).to(dtype)
+    got, K, V = _attended(q, k, v, held, group)
+    top = V.abs().unflatten(-1, (-1, group)).amax(-1, keepdim=True).expand(L, G, -1, group).flatten(-2)
+    y, _, mag = attention(q, K, V, held, D ** -0.5)
+    size = attention(q, K, top, held, D ** -0.5)[0]
+    tol = y.abs() * torch.finfo(dtype).eps / 2 + size * (2 * 2.0 ** -11 + 2 * mag * 2.0 ** -18 + L * 2.0 ** -22)
+    assert bool(((got - y).abs() <= tol).all()), float(((got - y).abs() / tol).max())
