@@ -138,3 +138,17 @@ def test_prompts_over_large_values_are_the_same_every_time(held, counts, H, G, d
     torch.cuda.synchronize()
     for *_, want, _, out, _ in sets:
         assert all(torch.equal(x, want) for x in out)
+
+
+@torch.no_grad()
+def test_the_command_line_serves_its_samples_as_one_batch(monkeypatch, capsys, tmp_path):
+    sys.path.insert(0, str(Path(__file__).parent.parent / "lit-llama-ja_b200"))
+    import generate
+    from tests.test_gpu_paged_model import _model
+
+    (tmp_path / "x.pth").write_bytes(b"")
+    monkeypatch.setattr(generate, "load_model", lambda *a: _model(64))
+    generate.main(checkpoint_path=tmp_path / "x.pth", prompt_ids="5,17,3", num_samples=3, max_new_tokens=7, kv_cache="int4")
+    out = capsys.readouterr()
+    lines = [[int(t) for t in line.split(",")] for line in out.out.split()]
+    assert len(lines) == 3 and all(x[:3] == [5, 17, 3] and len(x) == 10 for x in lines) and "tokens/sec" in out.err
