@@ -47,6 +47,9 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t v) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
+__device__ __forceinline__ void add_pair(float& a, float& b, float x, float y) {
+  asm("{\n\t.reg .b64 p, q;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %3};\n\tadd.rn.f32x2 p, p, q;\n\tmov.b64 {%0, %1}, p;\n\t}" : "+f"(a), "+f"(b) : "f"(x), "f"(y));
+}
 __device__ __forceinline__ uint32_t half_bits(float a, float b) { return pair_bits<__half>(a, b); }
 
 __device__ __forceinline__ void mbar_inval(uint64_t* bar) { asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory"); }
@@ -83,7 +86,6 @@ __device__ __forceinline__ bool few_walk(const Kv4Attn& a, const Kv4Item& it, in
   constexpr int W = D / 32, KS = D / 16, COLS = 4 * CPL * NB, BYTES = kv4_bytes(D, NG), SLICE = kv4_slice_bytes(D, NG), SPG = KS / NG, STAGES = kf_stages(D, NG);
   constexpr bool FINE = std::is_same<T, __half>::value;                  // the result keeps 11 bits
   constexpr int TERMS = CPL == 2 && FINE ? 2 : 1;
-  constexpr bool MIDDLE = FINE && TERMS == 1;                            // the sums stand around the middle code
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, R = a.H / a.G;
   const int first = it.first, n = it.count, row = it.row, cols = min(COLS, n * R - col0);
   T* y = (T*)a.y;
@@ -304,9 +306,11 @@ __device__ __forceinline__ bool few_walk(const Kv4Attn& a, const Kv4Item& it, in
           sum[b][e] += s[x][b][e];
         }
     // y += (p s) c, p lo: by groups, p s under what the column's sums stand under, and so under 2^15.  Of a word's nibbles 0 and 1 (2 and 3) the rows of
-    // the second tile half take both as they stand, c + 16 c': the end takes c from it.  Where the result is fp16 and both of a
-    // weight's terms are columns of one product (CPL = 1), the sums stand around code 8: one more product takes 8 of every code, and lo gets 8 s.  Two
-    // terms in two products have their 22 bits without that.
+    // the second tile half take both as they stand, c + 16 c': the end takes c from it.  Where the result is fp16, the sums of
+    // 16 keys are added in fp32, and codes are four times as large: the tensor pipe cuts products off two bits below the last one of the sum that they join, and
+    // those of a subnormal number as if it were the smallest normal one.  (130 000 keys of like weights, whose values leave a 40th of a scale: 0.00021 of
+    // the norm off, as a rounded exact result is, instead of 0.00028 with the sums around code 8 in the pipe, which also took 45 us instead of 40; eight columns
+    // 0.00022 instead of 0.00066 around code 0, 60 us instead of 58.)
     auto add_values = [&](auto careful) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -319,7 +323,6 @@ __device__ __forceinline__ bool few_walk(const Kv4Attn& a, const Kv4Item& it, in
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             const float2 p = pv[2 * h + x][g];
-            const float lo = MIDDLE ? fmaf(8.f, p.x, p.y) : p.y;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
               float w[2] = {0.f, 0.f};
@@ -328,7 +331,7 @@ __device__ __forceinline__ bool few_walk(const Kv4Attn& a, const Kv4Item& it, in
                 const float pe = s[2 * h + x][b][e];
                 w[e] = careful.value ? pe * p.x * one_over_pow2(most[b][g][e]) : pe * (p.x * one_over_pow2(most[b][g][e]));
                 if (careful.value && pe == 0.f) w[e] = 0.f;
-                else sumlo[b][g][e] = fmaf(pe, lo, sumlo[b][g][e]);
+                else sumlo[b][g][e] = fmaf(pe, p.y, sumlo[b][g][e]);
               }
               if (CPL == 1) {
                 if (FINE) {                                             // the odd column: what 11 bits leave over
@@ -350,13 +353,21 @@ __device__ __forceinline__ bool few_walk(const Kv4Attn& a, const Kv4Item& it, in
 #pragma unroll
           for (int e = 0; e < SPG; ++e) {
             const int r = g * SPG + e;
-            const uint32_t w0 = (r & 1) ? __byte_perm(vw[0][r >> 1], 0u, 0x4341) : vw[0][r >> 1] & 0x00ff00ffu;
-            const uint32_t w1 = (r & 1) ? __byte_perm(vw[1][r >> 1], 0u, 0x4341) : vw[1][r >> 1] & 0x00ff00ffu;
+            auto codes = [](uint32_t w, bool upper) {
+              if (FINE) return (upper ? w >> 6 : w << 2) & 0x03fc03fcu;
+              return upper ? __byte_perm(w, 0u, 0x4341) : w & 0x00ff00ffu;
+            };
+            constexpr uint32_t LOW = FINE ? 0x003c003cu : 0x000f000fu;
+            const uint32_t w0 = codes(vw[0][r >> 1], (r & 1) != 0), w1 = codes(vw[1][r >> 1], (r & 1) != 0);
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
+              float t[4] = {0.f, 0.f, 0.f, 0.f};
+              float (&sums)[4] = FINE ? t : o[b][r];
 #pragma unroll
-              for (int x = 0; x < TERMS; ++x) mma_f16_16816(o[b][r], w0 & 0x000f000fu, w0, w1 & 0x000f000fu, w1, bw[b][x][0], bw[b][x][1]);
-              if (MIDDLE) mma_f16_16816(o[b][r], 0x80088008u, 0x80888088u, 0x80088008u, 0x80888088u, bw[b][0][0], bw[b][0][1]);
+              for (int x = 0; x < TERMS; ++x) mma_f16_16816(sums, w0 & LOW, w0, w1 & LOW, w1, bw[b][x][0], bw[b][x][1]);
+              if (FINE)
+#pragma unroll
+                for (int x = 0; x < 4; x += 2) add_pair(o[b][r][x], o[b][r][x + 1], t[x], t[x + 1]);
             }
           }
         }
@@ -401,12 +412,12 @@ __device__ __forceinline__ bool few_walk(const Kv4Attn& a, const Kv4Item& it, in
 #pragma unroll
     for (int r = 0; r < KS; ++r) {
 #pragma unroll
-      for (int e = 0; e < CPL; ++e) {                                   // (codes were 2^-24 of themselves)
+      for (int e = 0; e < CPL; ++e) {                                   // (codes were 2^-24 of themselves, or 2^-22)
         const float up = pow2_of(most[b][r / SPG][e]);
         const float c = CPL == 2 ? o[b][r][e] : o[b][r][0] + o[b][r][1], both = CPL == 2 ? o[b][r][2 + e] : o[b][r][2] + o[b][r][3];
         float* const at = so + (warp * COLS + 8 * b + CPL * t4 + e) * LD + 16 * r + g8;
-        at[0] = fmaf(c * 16777216.f, up, sumlo[b][r / SPG][e]);
-        at[8] = fmaf((both - c) * 1048576.f, up, sumlo[b][r / SPG][e]);
+        at[0] = fmaf(c * (FINE ? 4194304.f : 16777216.f), up, sumlo[b][r / SPG][e]);
+        at[8] = fmaf((both - c) * (FINE ? 262144.f : 1048576.f), up, sumlo[b][r / SPG][e]);
       }
     }
   __syncthreads();

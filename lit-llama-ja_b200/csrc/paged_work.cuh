@@ -61,8 +61,8 @@ constexpr float KV4_NONE = -1e37f;      // the reference of a column that has se
 
 // Sequences that bring up to KV4_FEW_MOST columns a key head go to the kernel of few columns (in tiles of KV4_FEW_BESIDE beside the others), others to the
 // tcgen05 kernel in tiles of KV4_MANY.
-// us, few / tcgen05, heads of 128, 2000 keys: 32 heads over 32, one request of 16, 32, 48 tokens 15.6 / 22.7, 19.3 / 22.9, 22.9 / 23.3, eight requests 41 / 86,
-// 54 / 86, 116 / 86; 32 heads over 8, one of 8, 16, 24 tokens 15.2 / 21.5, 15.5 / 22.0, 19.0 / 22.8, eight 27 / 33, 41 / 34, 62 / 35.
+// us, few / tcgen05, heads of 128, 2000 keys: 32 heads over 32, one request of 16, 32, 48 tokens 16.1 / 21.9, 19.9 / 22.3, 23.5 / 22.7, eight requests 43 / 77,
+// 57 / 77, 118 / 78; 32 heads over 8, one of 8, 16 tokens 15.8 / 22.3, 16.0 / 22.9, eight 28 / 31, 42 / 32.
 // Where no request of the cache has more than KV4_WHOLE pages, walks are not cut, and the launch that joins parts falls away (30 to 500 keys of 32 heads, whole /
 // cut: one request 3.7 - 6.1 / 4.7 - 6.3, 64 requests 13.8 - 34.8 / 14.8 - 36.1).
 constexpr int KV4_FEW_MOST = 32, KV4_FEW_BESIDE = 8, KV4_MANY = 256, KV4_WHOLE = 8;

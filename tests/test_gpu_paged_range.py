@@ -236,3 +236,16 @@ def test_few_columns_take_keys_as_they_are(D, group, dtype, held, count, R):
     size = attention(q, K, top, held, D ** -0.5)[0]
     tol = y.abs() * torch.finfo(dtype).eps / 2 + size * (2 * 2.0 ** -11 + 2 * mag * 2.0 ** -18 + L * 2.0 ** -22)
     assert bool(((got - y).abs() <= tol).all()), float(((got - y).abs() / tol).max())
+
+
+@pytest.mark.parametrize("R, D, group", [(1, 128, 32), (4, 64, 32), (8, 128, 128), (8, 64, 32), (16, 64, 64)])
+@torch.no_grad()
+def test_fp16_results_over_many_keys(R, D, group):
+    """120 000 keys of weights some 2^9 apart, whose values leave little of one another: nothing is left to see but the result's rounding, half a place, 2^-11, at most and
+    2^-11 / sqrt(3) of it in the mean square at most.  Sums in fp32 of parts that are added up in a tree lose 2^-24 of some 60 codes' worth of a value a part."""
+    torch.manual_seed(22)
+    L = 120000
+    k, v, q = torch.randn(L, 1, D).to(HF), torch.randn(L, 1, D).to(HF), (torch.randn(1, R, D) * 1.5).to(HF)
+    got, K, V = _attended(q, k, v, L - 1, group)
+    want = attention(q, K, V, L - 1, D ** -0.5)[0]
+    assert float((got - want).norm() / want.norm()) <= math.sqrt(1 / 3) * 2.0 ** -11 + 2.0 ** -15
