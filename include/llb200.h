@@ -873,7 +873,8 @@ LL_API int ll_kv4_append(const ll_kv4_cache* cache, void* blocks, const void* q,
 LL_API int ll_kv4_read(const ll_kv4_cache* cache, const void* blocks, const int32_t* slots, void* k, void* v, int n, ll_stream stream);
 /* Softmax attention of a plan's tokens: q rows of the heads, y [T][heads][D]; a token sees its request's keys at and before its position.  Tokens of
  * refused sequences are no numbers, rows behind the last token are left as they are.  B, T, max_count: the plan's.  Of up to 32 queries of a key
- * head a sequence's walk is by mma.sync, of more by tcgen05, whose operands are fp16. */
+ * head a sequence's walk is by mma.sync, of more by tcgen05, whose operands are fp16; tiles that see a group which fp16 numbers do not hold (a scale of 2^8
+ * or a lowest value of 2^12 and more, both under 2^-16 and 2^-10 unless 0, or no numbers) are by mma.sync too.  y may be q. */
 LL_API size_t ll_kv4_attn_scratch_bytes(const ll_kv4_cache* cache, int B, int T, int max_count);
 LL_API int ll_kv4_attn(const ll_kv4_cache* cache, const void* blocks, const void* q, long long q_row, const int32_t* work, void* y, int B, int T,
                        int max_count, float scale, void* scratch, ll_stream stream);

@@ -6,7 +6,7 @@
 // so that the products run over codes, which a mask turns into numbers of fp16 (subnormal ones, exactly), and scales meet 16 keys at a time.
 //
 // What bounds it: memory in a burst, 60 requests of up to 4096 keys, 32 heads of 128 in groups of 64, 579 MB in 91 us (97 % of the copy rate); in a loop,
-// where the power cap takes the SMs from 1.97 to 1.64 GHz, its instructions (109 us), of which the masks are a third.  tcgen05 would not help: the walk
+// where the power cap takes the SMs from 1.97 to 1.64 GHz, its instructions (103 to 111 us), of which the masks are a third.  tcgen05 would not help: the walk
 // needs no products faster, and a tile of 128 rows would hold one query a head.  us on the way there: a warp a key on the CUDA cores 1290; codes by
 // mma.sync, a block's warps sharing a ring 185; a ring a warp and one look at all maxima 137; 32 keys a look and four columns of two each 118; the
 // largest parts first 102; fewer masks (c + 16 c' in the second row half) and no looks behind a column but at a walk's end 94; loops as one turn of code 91.
@@ -67,8 +67,9 @@ __device__ __forceinline__ bool kf_wait(uint64_t* bar, uint32_t parity, int* wor
 // Few queries a request: a block walks a range of one request's pages for one key head and a tile of columns (a column: one query of one of the heads
 // that share the key head).  Warp w takes half w & 1 of every other page, 32 keys, through a ring and with references of its own; the four join at the end.
 // CPL = 1: up to four columns, each of which has two of the product's eight, so that a lane has one column's scores and not those of columns that are
-// not there (drafts of four tokens, 12 requests of up to 3000 keys, 40 heads: 35 us, with eight columns 39); CPL = 2: eight columns, and 16 with NB = 2.  Weights enter the second product as fp16, half a place (2^-11) of which a bf16 result does not show; where the result is fp16 as two terms, with
-// CPL = 1 the second one in the odd column.
+// not there (drafts of four tokens, 12 requests of up to 3000 keys, 40 heads: 35 us, with eight columns 39); CPL = 2: eight columns, and 16 with NB = 2.
+// Weights enter the second product as fp16, half a place (2^-11) of which a bf16 result does not show; where the result is fp16 as two terms, with CPL = 1 the
+// second one in the odd column.
 template <int COLS, int STAGES>
 struct KfShared {
   uint64_t full[KF_WARPS][STAGES];

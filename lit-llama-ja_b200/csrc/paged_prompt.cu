@@ -15,10 +15,11 @@
 // A word's codes become pairs by masks: 1024 + c under exponent bits, from which one operation takes the 1024 (of odd nibbles, 1024 + 16 c, 64 + c), and
 // one more multiplies and adds.  Keys' pairs run along the dimensions, values' along the keys: values stand with the keys in a row, so that both
 // operands are K-major.
-// What bounds it: issue slots (63 % of them used), which the softmax and the unpacking share; the exponential unit is busy 30, the tensor pipe 29 % of the
-// time.  A prompt of 2048, 32 heads of 128, us: 92 with the queries a row a thread (8000 clocks of a block) and all walks cut, 73 with whole rows and walks
-// as they are, 64 with two sets of unpacking warps and the other sequences' kernel let in at the end, 62 with waits and loops as one turn of code;
-// over the bf16 cache (csrc/attn_tc.cuh) 65.
+// What bounds it: no pipe (issue slots 62 %, exponential unit 32, tensor pipe 31) but the chain of a page's turn, some 1.4 us: scores, their maximum, the meeting
+// of a row's two threads, weights, arrivals, and the unpacking beside it; leaving either of these two out gains 8 to 15 %.  A prompt of 2048, 32 heads of 128, us:
+// 92 with the queries a row a thread (8000 clocks of a block) and all walks cut, 73 with whole rows and walks as they are, 64 with two sets of unpacking warps
+// and the other sequences' kernel let in at the end, 62 with waits and loops as one turn of code, 59 without powers of two; over the bf16 cache
+// (csrc/attn_tc.cuh) 65.  With values that are all left to the walk of few columns 328.
 // Every wait is bounded; one that runs out records a code, all roles stop, copies in flight are waited for, tensor memory is freed.
 #include <type_traits>
 

@@ -246,7 +246,8 @@ class PagedCache4:
 
     def attend(self, layer: int, plan: CachePlan, q: torch.Tensor, scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Softmax attention of the step's queries ``[tokens, n_head, head_size]`` over what their requests hold up to their positions; the tokens' own keys
-        have to be appended before.  ``scale`` of the scores: 1 / sqrt(head_size) unless given.  Rows of ``out`` behind the last token stay as they are."""
+        have to be appended before.  ``scale`` of the scores: 1 / sqrt(head_size) unless given.  Rows of ``out`` behind the last token stay as they are; it may
+        be ``q``."""
         self._check(layer, plan)
         T = plan.T
         q, q_row = self._rows("q", q, T, self.n_head)
