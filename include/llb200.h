@@ -22,7 +22,7 @@
 extern "C" {
 #endif
 
-#define LL_ABI_VERSION 20
+#define LL_ABI_VERSION 21
 
 #define LL_OK 0
 #define LL_ERR_ARG (-1)         /* bad shape / dtype / null pointer */
@@ -878,6 +878,32 @@ LL_API int ll_kv4_read(const ll_kv4_cache* cache, const void* blocks, const int3
 LL_API size_t ll_kv4_attn_scratch_bytes(const ll_kv4_cache* cache, int B, int T, int max_count);
 LL_API int ll_kv4_attn(const ll_kv4_cache* cache, const void* blocks, const void* q, long long q_row, const int32_t* work, void* y, int B, int T,
                        int max_count, float scale, void* scratch, ll_stream stream);
+/* Requests that share pages (csrc/paged_share.cu).  shared: [2][pages], zeros and then -1 before the first call: holders of a page beyond its first, and scratch.
+ * A cache whose requests share pages is cut by ll_kv4_release, never by ll_kv4_truncate.  blocks: the cache's, `layers` of [pages][kv_heads][page bytes] one
+ * after the other.  work: 5 B numbers.
+ * Fork: the empty request into[i] becomes a copy of rows[i] as it is before the call; whole pages are shared, a last one that is not full is copied.  Status: 0 done;
+ * 1 no free page for that; 3 no such request, into[i] is not empty or an earlier sequence names it.  Copies that are refused stay empty.
+ * Release: as ll_kv4_truncate, and a page goes back with its last holder.  A cut that ends inside a page which others hold copies it; status 1: no page was free before
+ * the call for that, and the request stays as it was. */
+LL_API int ll_kv4_fork(const ll_kv4_cache* cache, void* blocks, int layers, int32_t* shared, const int32_t* rows, const int32_t* into, int B, int32_t* status,
+                       int32_t* work, ll_stream stream);
+LL_API int ll_kv4_release(const ll_kv4_cache* cache, void* blocks, int layers, int32_t* shared, const int32_t* rows, const int32_t* keep, int B, int32_t* status,
+                          int32_t* work, ll_stream stream);
+
+/* ---------------------------------------------------------------------------------------
+ * What a step's logits are asked: a token a row (csrc/sample_rows.cu), and how likely given ones are (csrc/token_logprobs.cu).  logits: R rows of V numbers
+ * (fp32, bf16 or fp16), `row` numbers apart.  Settings: one a row on the device, or null and one for all.
+ * Draw.  With the row's largest logit m and a temperature T > 0, token i weighs w_i = rint(2^44 exp((l_i - m) / T)) in 64 bits (l_i = m: 2^44).  Kept are logits at least
+ * as large as the k-th largest (top_k < 1, or V and more: all), of these the largest up to the first one with which the weights reach top_p of the kept ones' (1 and
+ * more: all), of these those with w >= min_p 2^44 (min_p above 1 counts as 1); logits that are equal stay together.  The token is the first one whose running sum of kept weights exceeds
+ * min(floor(u * sum), sum - 1).  T = 0: the first of the largest logits.  -1: a logit or setting is no number, all logits are -inf, T is negative or
+ * infinite, or u is outside of 0 .. 1.  V up to 2^18. */
+LL_API int ll_sample_rows(const void* logits, int dtype, int R, int V, long long row, const float* u, const float* temperature, float temperature_all,
+                          const int32_t* top_k, int top_k_all, const float* top_p, float top_p_all, const float* min_p, float min_p_all, int64_t* tokens, ll_stream stream);
+/* out[r] = log of the softmax of logits / T at tokens[r], in fp32; no number for a token outside of 0 .. V - 1, a T that is not above 0 and finite, or a row with a
+ * logit that is no number, or without any above -inf. */
+LL_API int ll_token_logprobs(const void* logits, int dtype, int R, int V, long long row, const int64_t* tokens, const float* temperature, float temperature_all,
+                             float* out, ll_stream stream);
 
 #ifdef __cplusplus
 }

@@ -134,6 +134,10 @@ EXPORTS = {
     "ll_kv4_read": ([vp, vp, vp, vp, vp, i32, vp], C.c_int),
     "ll_kv4_attn_scratch_bytes": ([vp, i32, i32, i32], sz_t),
     "ll_kv4_attn": ([vp, vp, vp, i64, vp, vp, i32, i32, i32, C.c_float, vp, vp], C.c_int),
+    "ll_kv4_fork": ([vp, vp, i32, vp, vp, vp, i32, vp, vp, vp], C.c_int),
+    "ll_kv4_release": ([vp, vp, i32, vp, vp, vp, i32, vp, vp, vp], C.c_int),
+    "ll_sample_rows": ([vp, i32, i32, i32, i64, vp, vp, C.c_float, vp, i32, vp, C.c_float, vp, C.c_float, vp, vp], C.c_int),
+    "ll_token_logprobs": ([vp, i32, i32, i32, i64, vp, vp, C.c_float, vp, vp], C.c_int),
     "ll_embed_ssq": ([vp, vp, vp, vp, i32, i32, vp], C.c_int),
     "ll_rope_kv_append": ([vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp], C.c_int),
     "ll_decode_attn": ([vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp, vp, i32, vp], C.c_int),
@@ -249,7 +253,7 @@ EXPORTS = {
 }
 _fn = {name: _proto(name, a, r) for name, (a, r) in EXPORTS.items()}
 
-ABI_VERSION = 20
+ABI_VERSION = 21
 if _fn["ll_abi_version"]() != ABI_VERSION:
     raise ImportError("libllb200.so ABI version mismatch; rebuild with lit-llama-ja_b200/build.py")
 

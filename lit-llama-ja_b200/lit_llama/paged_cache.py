@@ -8,6 +8,7 @@ A serving step, per layer after the first two lines:
     q = cache.append(layer, plan, q, k, v, rope=table) # rows [tokens, heads, head_size]; turns queries and keys where a table is given
     y = cache.attend(layer, plan, q)                   # every token over its request's keys at and before its position
     cache.truncate(rows, lengths)                      # afterwards: drafts that were rejected; length 0 ends a request
+    cache.fork(rows, into)                             # requests into[i] become copies of rows[i], sharing their pages (PagedCache4(.., share=True))
 
 Nothing looks at lengths on the host, so that a captured step serves requests of any lengths.  All of it goes to the current stream of the
 cache's device: on another stream a step waits for the one before it, and a plan is kept until its kernels there are done.  A group of values x is held as
@@ -89,9 +90,9 @@ class PagedCache4:
     PAGE = 64
 
     def __init__(self, n_layer: int, n_head: int, head_size: int, *, n_kv_head: Optional[int] = None, pages: int, requests: int, max_length: int,
-                 group: int = 64, dtype: torch.dtype = torch.bfloat16, device="cuda"):
+                 group: int = 64, dtype: torch.dtype = torch.bfloat16, device="cuda", share: bool = False):
         """``pages`` of 64 slots for up to ``requests`` requests of up to ``max_length`` tokens; heads of 32, 64 or 128, codes by ``group``s of 32, 64 or 128
-        of their dimensions.  ``n_kv_head`` key/value heads serve ``n_head`` query heads, neighbours the same one."""
+        of their dimensions.  ``n_kv_head`` key/value heads serve ``n_head`` query heads, neighbours the same one.  ``share``: requests may be forked."""
         n_kv_head = n_head if n_kv_head is None else n_kv_head
         device = torch.device(device)
         if device.type != "cuda":
@@ -116,6 +117,11 @@ class PagedCache4:
         self.free = torch.arange(pages - 1, -1, -1, **i32)
         self.n_free = torch.full((1,), pages, **i32)
         self._stamp = torch.zeros(requests, **i32)
+        self.share = bool(share)
+        self._shared = None                                               # a page's holders beyond the first, and scratch of -1
+        if self.share:
+            self._shared = torch.zeros((2, pages), **i32)
+            self._shared[1].fill_(-1)
         self._none = torch.empty(0, dtype=dtype, device=self.device)      # (a result's type and device)
         self._code = N.dtype_code(dtype)
         self._struct = N.Kv4Cache(*(N.ptr(t) for t in (self.table, self.lengths, self.free, self.n_free, self._stamp)), requests, self.width, pages, max_length,
@@ -164,15 +170,38 @@ class PagedCache4:
             N.call("ll_kv4_plan", self._c, N.ptr(rows), N.ptr(counts), plan.B, tokens, plan.max_count, plan._out, plan._work, N.stream())
         return plan
 
-    def truncate(self, rows: Whole, lengths: Whole) -> None:
-        """Cut request ``rows[i]`` to its first ``lengths[i]`` tokens (0 ends it); pages that it no longer needs are free again.  Requests that are not longer
-        stay as they are."""
+    def truncate(self, rows: Whole, lengths: Whole) -> Optional[torch.Tensor]:
+        """Cut request ``rows[i]`` to its first ``lengths[i]`` tokens (0 ends it); pages that no request needs any longer are free again.  Requests that are not
+        longer stay as they are.  Where requests may share pages, a cut that ends inside a page which others hold takes a page for a copy of it; returned are then
+        int32 numbers, one for each sequence: 0, or 1 where no page was free for that before the call and the request stays as it was."""
         rows, lengths = self._whole("rows", rows), self._whole("lengths", lengths)
         if rows.shape != lengths.shape or rows.numel() == 0:
             raise RuntimeError(f"{rows.numel()} requests and {lengths.numel()} lengths")
         with self._here():
             self._step += 1
+            if self._shared is not None:
+                return self._share("ll_kv4_release", rows, lengths)
             N.call("ll_kv4_truncate", self._c, N.ptr(rows), N.ptr(lengths), rows.numel(), N.stream())
+
+    def fork(self, rows: Whole, into: Whole) -> torch.Tensor:
+        """Make the empty requests ``into[i]`` copies of ``rows[i]``, one request of as many as one likes: they share its whole pages, and a last page that is not full is
+        copied.  Returns int32 numbers, one for each sequence: 0; 1 where there is no free page for that; 3 where there is no such request, or ``into[i]`` is not
+        empty or named before (``REASONS``).  Copies that are refused stay empty.  Plans of earlier steps end with this one."""
+        if self._shared is None:
+            raise RuntimeError("requests of this cache do not share pages: PagedCache4(.., share=True)")
+        rows, into = self._whole("rows", rows), self._whole("into", into)
+        if rows.shape != into.shape or rows.numel() == 0:
+            raise RuntimeError(f"{rows.numel()} requests and {into.numel()} copies")
+        with self._here():
+            self._step += 1
+            return self._share("ll_kv4_fork", rows, into)
+
+    def _share(self, what: str, rows: torch.Tensor, other: torch.Tensor) -> torch.Tensor:
+        B = rows.numel()
+        out = self.lengths.new_empty(6 * B)                                # statuses, and what the call notes of its sequences
+        at = N.ptr(out)
+        N.call(what, self._c, self._layers[0], self.n_layer, N.ptr(self._shared), N.ptr(rows), N.ptr(other), B, at, at + 4 * B, N.stream())
+        return out[:B]
 
     def reset(self) -> None:
         """All requests end, and pages are given out as in the beginning."""
@@ -181,13 +210,15 @@ class PagedCache4:
         self.lengths.zero_()
         torch.arange(self.pages - 1, -1, -1, out=self.free)
         self.n_free.fill_(self.pages)
+        if self._shared is not None:
+            self._shared[0].zero_()
 
     # ------------------------------------------------------------------ a layer
     def _check(self, layer: int, plan: CachePlan) -> None:
         if not 0 <= layer < self.n_layer:
             raise RuntimeError(f"layer {layer} of {self.n_layer}")
         if plan.cache is not self or plan.step != self._step:
-            raise RuntimeError("the plan is another cache's, or of a step before this cache's last plan or truncation")
+            raise RuntimeError("the plan is another cache's, or of a step before this cache's last plan, truncation or fork")
 
     def _rows(self, name: str, x: torch.Tensor, T: int, heads: int) -> Tuple[torch.Tensor, int]:
         """Rows as the kernels take them, and their distance: the heads of a token one after the other, tokens at any distance, 16-byte boundaries."""
