@@ -121,7 +121,11 @@ def test_rows_anywhere():
             k = torch.tensor([5, 0, 9, 1, 70, 3], dtype=torch.int32, device=DEV)[:R]
             assert torch.equal(sample(view, u[:R], top_k=k, top_p=0.9), sample(dense, u[:R].contiguous(), top_k=k, top_p=0.9))
             tokens = torch.randint(0, view.shape[1], (2 * R,), device=DEV)[::2]
-            assert torch.equal(token_logprobs(view, tokens), token_logprobs(dense, tokens.contiguous()))
+            # sums of 32 bits are by vectors that begin at 16-byte boundaries: where a row begins otherwise, its terms meet in another order, and either
+            # result is within the bound of a score's error of the exact one, so that two are within twice the bound of each other
+            got, other = token_logprobs(view, tokens).double().cpu(), token_logprobs(dense, tokens.contiguous()).double().cpu()
+            exact = torch.log_softmax(dense.double().cpu(), -1).gather(1, tokens.cpu()[:, None])[:, 0]
+            assert bool(((got - other).abs() <= 2 * _score_bound(dense.cpu(), 1.0, exact)).all())
     empty = sample(wide[:0], u[:0])
     assert empty.shape == (0,) and empty.dtype is torch.int64 and token_logprobs(wide[:0], empty).shape == (0,)
 
