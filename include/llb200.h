@@ -896,7 +896,7 @@ LL_API int ll_kv4_release(const ll_kv4_cache* cache, void* blocks, int layers, i
  * Draw.  With the row's largest logit m and a temperature T > 0, token i weighs w_i = rint(2^44 exp((l_i - m) / T)) in 64 bits (l_i = m: 2^44).  Kept are logits at least
  * as large as the k-th largest (top_k < 1, or V and more: all), of these the largest up to the first one with which the weights reach top_p of the kept ones' (1 and
  * more: all), of these those with w >= min_p 2^44 (min_p above 1 counts as 1); logits that are equal stay together.  The token is the first one whose running sum of kept weights exceeds
- * min(floor(u * sum), sum - 1).  T = 0: the first of the largest logits.  -1: a logit or setting is no number, all logits are -inf, T is negative or
+ * min(floor(u * sum), sum - 1).  T under 2^-100: the first of the largest logits.  -1: a logit or setting is no number, all logits are -inf, T is negative or
  * infinite, or u is outside of 0 .. 1.  V up to 2^18. */
 LL_API int ll_sample_rows(const void* logits, int dtype, int R, int V, long long row, const float* u, const float* temperature, float temperature_all,
                           const int32_t* top_k, int top_k_all, const float* top_p, float top_p_all, const float* min_p, float min_p_all, int64_t* tokens, ll_stream stream);

@@ -2,8 +2,13 @@
 //
 // Weights are whole numbers, w = rint(2^44 exp((l - m) / T)): V of them have a sum of 62 bits, exactly, so that neither a border of top-p nor a draw depends on
 // the order of sums, and blocks may add in any order.  Both borders are values: top-k's the largest x with k logits at or above it, top-p's the largest x with
-// top_p of the kept weight there.  A border is found by counts (or weights) in 1024 equal steps below m down to where weights are 0, then by those of
-// the numbers' keys within the step that it falls into: once for 16-bit logits, up to three times for 32.
+// top_p of the kept weight there.
+//   top-k: counts in 1024 equal steps below m, down to where weights are 0.
+//   top-p: the steps' weights, in the same pass that adds up all of them: within a step they differ by 3 %, so that 13 bits of each one's part of the step's largest
+//   are enough to leave one step or two that the border can be in.
+// The few numbers of those steps are then compared with one another, on top of the exact sum of what lies above; where they are many (rows of few values), the border is
+// found by counts or exact weights of their keys, 1024 ranges at a time.  (Exact weights in all steps, two dependent additions of 32 bits in shared memory each: 301
+// rows of 100 003 numbers 738 us.)
 //
 // A cluster of blocks has a row in its shared memory, read once.
 #include <cooperative_groups.h>
@@ -17,11 +22,12 @@ namespace cg = cooperative_groups;
 
 constexpr double SR_ONE = 17592186044416.0;      // 2^44
 constexpr float SR_REACH = 31.25f;               // weights are 0 from 45 ln 2 = 31.19 temperatures below m on
-constexpr int SR_BINS = 1024;
+constexpr float SR_LEAST = 7.888609052210118e-31f;      // 2^-100: less of a temperature counts as 0
+constexpr int SR_BINS = 1024, SR_LIST = 512, SR_TABLE = 256;
 constexpr int SR_WIDE = 512, SR_NARROW = 128, SR_MOST = 8, SR_TURNS = 17;      // threads; blocks a row and vectors a thread, at most
 typedef unsigned long long u64;
 
-// Numbers in the order of their values, as whole numbers one after the other in their type; 0 and -0 are one.
+// Numbers in the order of their values, as whole numbers in the steps of their type; 0 and -0 are one.
 __device__ __forceinline__ uint32_t order_bits(float x) {
   const uint32_t b = __float_as_uint(x + 0.f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
@@ -33,6 +39,21 @@ template <typename T> __device__ __forceinline__ uint32_t order_key(float x) { r
 template <typename T> __device__ __forceinline__ float key_value(uint32_t k) {
   k <<= key_shift<T>::n;
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~(k | ((1u << key_shift<T>::n) - 1u)));
+}
+
+// rint(2^44 exp(d / T)) for d <= 0, with c = 256 / (T ln 2): by a table of 2^(j / 256) and a polynomial of degree 4 around its places (Tang, Table-driven
+// implementation of the exponential function, 1989): at most half of ln 2 / 256 from one, so that the next term is under 2^-54.  c d is off by 2^-52 of itself, times
+// exp(d / T) less than 2^-8 of a whole one.
+__device__ __forceinline__ u64 weight_of(double d, double c, const double* table) {
+  constexpr double SHIFT = 6755399441055744.0;   // 1.5 2^52: the sum's last bits are the nearest whole number
+  constexpr double L = 0.0027076061740622863;    // ln 2 / 256
+  const double shifted = fma(d, c, SHIFT);
+  const int k = __double2loint(shifted);
+  const double r = fma(d, c, SHIFT - shifted);
+  const double p = r * fma(r, fma(r, fma(r, L * L * L * L / 24, L * L * L / 6), L * L / 2), L);
+  const double at = table[k & (SR_TABLE - 1)], y = fma(at, p, at);
+  const double scaled = __hiloint2double(__double2hiint(y) + ((k >> 8) << 20) + (44 << 20), __double2loint(y));
+  return (u64)__double_as_longlong(scaled + 4503599627370496.0) & 0xfffffffffffffull;      // 2^52
 }
 
 struct SampleArgs {
@@ -48,11 +69,36 @@ struct SampleArgs {
 
 template <int THREADS>
 struct SampleShared {
-  uint32_t hist[2][2][SR_BINS];                  // two in turn: low and high halves of sums
-  u64 scan[THREADS / 32], found_base, totals[SR_MOST], segment[SR_TURNS][THREADS / 32];
-  uint32_t key[SR_MOST], warp_key[THREADS / 32], range[2];
-  int found;
+  uint32_t hist[2][2][SR_BINS];                  // two in turn: low and high halves of sums; or a block's list of numbers that a border is among
+  double exps[SR_TABLE];                         // 2^(j / 256)
+  u64 list_weight[SR_LIST];                      // all blocks' lists
+  uint32_t list_key[SR_LIST];
+  u64 scan[THREADS / 32], found_base, sums[2][SR_MOST];
+  uint32_t key[SR_MOST], warp_key[THREADS / 32], range[2], listed[2];
+  int found, last;
 };
+static_assert(SR_LIST * 12 <= 2 * SR_BINS * 4, "a list in the place of counts");
+
+// Another block's shared memory, asked for by its place in this one's.
+__device__ __forceinline__ uint32_t there(const void* p, int rank) {
+  uint32_t at;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+  return at;
+}
+__device__ __forceinline__ uint32_t remote(uint32_t at) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+  return v;
+}
+template <int BINS>
+__device__ __forceinline__ void remote_bins(uint32_t (&h)[BINS], uint32_t at) {
+  if constexpr (BINS == 2) {
+    asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(h[0]), "=r"(h[1]) : "r"(at) : "memory");
+  } else {
+#pragma unroll
+    for (int b = 0; b < BINS; ++b) h[b] = remote(at + 4 * b);
+  }
+}
 
 // Sum over the threads before this one.  Every thread of the block calls.
 template <int THREADS>
@@ -73,40 +119,43 @@ __device__ __forceinline__ u64 threads_before(u64 v, u64* s) {
 }
 
 template <typename T, int THREADS>
-__global__ void __launch_bounds__(THREADS) sample_rows_kernel(const SampleArgs a) {
-  constexpr int N = row_vec<T>::n, WARPS = THREADS / 32, BINS = SR_BINS / THREADS;
+__global__ void __launch_bounds__(THREADS, THREADS == SR_WIDE ? 2 : 8) sample_rows_kernel(const SampleArgs a) {
+  constexpr int N = row_vec<T>::n, WARPS = THREADS / 32, BINS = SR_BINS / THREADS, MOST = THREADS == SR_WIDE ? SR_MOST : 1;
   __shared__ SampleShared<THREADS> sh;
   cg::cluster_group cluster = cg::this_cluster();
   cluster.barrier_arrive();                      // (other blocks' memory is touched when all of them have begun)
   const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int r = blockIdx.x / C, t = threadIdx.x, lane = t & 31, warp = t >> 5, V = a.V;
   const T* l = (const T*)a.logits + r * a.row;
-  const float u = a.u[r], temperature = a.temperature ? a.temperature[r] : a.temperature_all, top_p = a.top_p ? a.top_p[r] : a.top_p_all,
-              min_p = a.min_p ? a.min_p[r] : a.min_p_all;
-  const int top_k = a.top_k ? a.top_k[r] : a.top_k_all;
-  const int i0 = rank * a.turns * THREADS * N - row_offset(l);      // the block's first number
-
-  // ---- the row, and its largest logit
-  extern __shared__ uint4 s_row[];               // [turns][THREADS]: a thread's own vectors
-  float top = -INFINITY;
+  const float u = a.u[r];
+  float temperature = a.temperature ? a.temperature[r] : a.temperature_all, top_p = a.top_p ? a.top_p[r] : a.top_p_all, min_p = a.min_p ? a.min_p[r] : a.min_p_all;
+  int top_k = a.top_k ? a.top_k[r] : a.top_k_all;
   bool bad = !(u >= 0.f && u <= 1.f) || !(temperature >= 0.f && temperature < INFINITY) || isnan(top_p) || isnan(min_p);
+  const bool first = temperature < SR_LEAST;     // the first one of the largest
+  if (first) temperature = 1.f, top_k = 1, top_p = 1.f, min_p = 0.f;
+
+  // ---- the row, a run of it a warp, and its largest logit
+  extern __shared__ uint4 s_row[];
+  uint4* const mine = s_row + warp * a.turns * 32 + lane;      // the thread's vectors, 32 apart
+  const int i0 = (rank * THREADS + warp * 32) * a.turns * N + lane * N - row_offset(l);      // the first one's first number
+  float top = -INFINITY;
 #pragma unroll 4
   for (int j = 0; j < a.turns; ++j) {
-    const uint4 raw = load_vector(l, i0 + (j * THREADS + t) * N, V);
-    s_row[j * THREADS + t] = raw;
+    const uint4 raw = load_vector(l, i0 + j * 32 * N, V);
+    mine[j * 32] = raw;
     float x[N];
     vec_values<T>(raw, x);
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      bad |= isnan(x[e]);
-      top = fmaxf(top, x[e]);
-    }
+    for (int e = 0; e < N; ++e) asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(x[e]));
   }
+  bad |= isnan(top);
   for (int b = t; b < 2 * 2 * SR_BINS; b += THREADS) (&sh.hist[0][0][0])[b] = 0;
+  for (int b = t; b < SR_TABLE; b += THREADS) sh.exps[b] = exp2(b * (1.0 / SR_TABLE));
+  if (t < 2) sh.listed[t] = 0;
   {
     const uint32_t k = __reduce_max_sync(0xffffffffu, order_bits(top));
     const bool any = __any_sync(0xffffffffu, bad);
-    if (lane == 0) sh.warp_key[warp] = any ? 0xffffffffu : k;      // (the key of a number that is none: above all others)
+    if (lane == 0) sh.warp_key[warp] = any ? 0xffffffffu : k;      // (above all others)
     __syncthreads();
     cluster.barrier_wait();
     if (warp == 0) {
@@ -121,200 +170,366 @@ __global__ void __launch_bounds__(THREADS) sample_rows_kernel(const SampleArgs a
     if (rank == 0 && t == 0) a.tokens[r] = -1;
     return;
   }
-  const float m = __uint_as_float(top_bits & 0x80000000u ? top_bits & 0x7fffffffu : ~top_bits);
-  const uint32_t top_key = top_bits >> key_shift<T>::n;
+  float m = __uint_as_float(top_bits & 0x80000000u ? top_bits & 0x7fffffffu : ~top_bits);
+  if (m == INFINITY) {                           // the limit: these alone, all alike
+    m = 0.f;
+    for (int j = 0; j < a.turns; ++j) {
+      float x[N];
+      vec_values<T>(mine[j * 32], x);
+      T* to = reinterpret_cast<T*>(&mine[j * 32]);
+#pragma unroll
+      for (int e = 0; e < N; ++e) dt<T>::st(to, e, x[e] == INFINITY ? 0.f : -INFINITY);
+    }
+  }
 
-  // ---- weights, and steps below m
-  const double inv = 1.0 / (double)temperature;
-  const float per_step = temperature > 0.f ? (float)SR_BINS / (SR_REACH * temperature) : INFINITY;
-  // how many steps below m; SR_BINS and more: a weight of 0.  (A temperature so large that a step has no size: one step for all.)
-  auto below = [&](float v) -> float { return v == m ? 0.f : v == -INFINITY ? (float)SR_BINS : per_step == 0.f ? 0.f : (m - v) * per_step; };
-  auto weight = [&](float v) -> u64 { return v == m ? (u64)SR_ONE : (u64)(long long)rint(exp(((double)v - (double)m) * inv) * SR_ONE); };
-  uint32_t border = 0;                           // kept are keys from here on
-
-  // ---- the largest key at or above which counts or weights reach what they have to
-  int turn = 0;
-  auto select = [&](auto weigh, auto reached) {
-    constexpr bool WEIGHTS = decltype(weigh)::value;
-    uint32_t lo = 0, hi = 0;
-    int shift = -1;                              // -1: steps below m; else steps of 2^shift keys below hi
-    u64 base = 0;
-    while (true) {
-      uint32_t(*hist)[SR_BINS] = sh.hist[turn];
+  // ---- steps below m, and weights
+  const double c64 = 369.32994026157255 / (double)temperature, m64 = m;      // 256 / ln 2
+  const float half_m = 0.5f * m, per_half = 2.f * (SR_BINS / SR_REACH) / temperature;      // (by halves: m - v may be more than a float holds)
+  const float cut = fmaxf(m - 31.5f * temperature, -3.402823466e38f);      // weights are 0 from here on; -inf is below
+  auto below = [&](float v) { return fmaf(v, -0.5f, half_m) * per_half; };
+  // The step that is nearest (a float past 2^23 has no fraction); of numbers above `cut` those of SR_BINS steps and more weigh nothing.
+  auto step_of = [&](float s) { return __float_as_int(s + 8388608.f) & 0x7fffff; };
+  auto weight = [&](float v) { return weight_of((double)v - m64, c64, sh.exps); };      // (of numbers from `cut` on)
+  float lowest = cut;                            // kept are numbers from here on
+  int turn = 0, sums = 0;
+  // the thread's vectors that have a number from `from` on in their warp
+  auto each = [&](float from, auto visit) {
 #pragma unroll 1
-      for (int j = 0; j < a.turns; ++j) {
-        float x[N];
-        vec_values<T>(s_row[j * THREADS + t], x);
+    for (int j = 0; j < a.turns; ++j) {
+      float x[N];
+      vec_values<T>(mine[j * 32], x);
+      float most = x[0];
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const float v = x[e];
-          const uint32_t key = order_key<T>(v);
-          int bin;
-          if (shift < 0) {
-            const float s = below(v);
-            bin = s < (float)SR_BINS ? (int)s : SR_BINS;
-          } else {
-            bin = key >= lo && key <= hi ? (int)((hi - key) >> shift) : SR_BINS;
-          }
-          if (bin < SR_BINS && key >= border) {
-            if (WEIGHTS) {
-              const u64 w = weight(v);
-              const uint32_t part = (uint32_t)w, old = atomicAdd(&hist[0][bin], part), up = (uint32_t)(w >> 32) + (old + part < old ? 1u : 0u);
-              if (up != 0u) atomicAdd(&hist[1][bin], up);
-            } else {
-              atomicAdd(&hist[0][bin], 1u);
-            }
-          }
-        }
-      }
-      cluster.sync();
-      // every block adds up all blocks' and finds the step
-      u64 n[BINS], mine = 0;
+      for (int e = 1; e < N; ++e) most = fmaxf(most, x[e]);
+      if (__any_sync(0xffffffffu, most >= from)) visit(x, j);
+    }
+  };
+  // a sum of all blocks' threads' numbers, behind a barrier of the cluster; `before`: of the blocks before this one
+  auto cluster_sum = [&](u64 v, u64& before) {
 #pragma unroll
-      for (int b = 0; b < BINS; ++b) n[b] = 0;
-      for (int c = 0; c < C; ++c) {
-        const uint32_t* h = cluster.map_shared_rank(&hist[0][0], c);
-#pragma unroll
-        for (int b = 0; b < BINS; ++b) n[b] += (WEIGHTS ? (u64)h[SR_BINS + BINS * t + b] << 32 : 0) + h[BINS * t + b];
-      }
-#pragma unroll
-      for (int b = 0; b < BINS; ++b) mine += n[b];
-      if (t == 0) sh.found = -1;
-      const u64 before = threads_before<THREADS>(mine, sh.scan);
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (lane == 0) sh.scan[warp] = v;
+    __syncthreads();
+    if (warp == 0) {
       u64 all = 0;
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) all += sh.scan[w];
-      u64 at = base + before;
+      if (lane < C) cluster.map_shared_rank(&sh.sums[sums][0], lane)[rank] = all;
+    }
+    cluster.sync();
+    v = 0;
+    for (int c = 0; c < C; ++c) {
+      if (c == rank) before = v;
+      v += sh.sums[sums][c];
+    }
+    sums ^= 1;                                   // (read before the next barrier, and written again behind that)
+    return v;
+  };
+  // This turn's counts of all blocks, behind a barrier of the cluster: the thread's bins, which are neighbours.
+  auto counted = [&](bool high, u64 (&n)[BINS]) {
+#pragma unroll
+    for (int b = 0; b < BINS; ++b) n[b] = 0;
+    for (int part = 0; part < (high ? 2 : 1); ++part) {
+      uint32_t h[MOST][BINS];
+#pragma unroll
+      for (int c = 0; c < MOST; ++c)
+        if (c < C) remote_bins(h[c], there(&sh.hist[turn][part][BINS * t], c));
+#pragma unroll
+      for (int c = 0; c < MOST; ++c)
+        if (c < C)
+#pragma unroll
+          for (int b = 0; b < BINS; ++b) n[b] += (u64)h[c][b] << (32 * part);
+    }
+    if (t == 0) sh.found = -1, sh.last = SR_BINS - 1, sh.range[0] = 0;
+    // (what the turn before has left has been read by every block: behind a barrier of the cluster that comes after)
+    for (int b = t; b < 2 * SR_BINS; b += THREADS) (&sh.hist[turn ^ 1][0][0])[b] = 0;
+    turn ^= 1;
+  };
+  auto bins_before = [&](const u64 (&n)[BINS]) {
+    u64 all = 0;
+#pragma unroll
+    for (int b = 0; b < BINS; ++b) all += n[b];
+    return threads_before<THREADS>(all, sh.scan);
+  };
+  // The keys of the steps first_bin .. last_bin below m: the smallest key at most so many steps below, by 32 at a time.
+  auto keys_of = [&](int first_bin, int last_bin) {
+    if (warp < 2) {
+      const int most = warp == 0 ? last_bin : first_bin - 1;
+      const uint32_t top_key = order_key<T>(m);
+      uint32_t from = order_key<T>(-INFINITY), to = top_key;             // `from` is more than `most` steps below m, `to` is not
+      while (most >= 0 && to - from > 1u) {
+        const uint32_t step = (to - from - 1u) / 33u + 1u;
+        const u64 probe = min((u64)from + (u64)(lane + 1) * step, (u64)to);
+        const float s = below(key_value<T>((uint32_t)probe));
+        const uint32_t in = __ballot_sync(0xffffffffu, s < (float)SR_BINS && step_of(s) <= most);
+        const int at = in != 0u ? __ffs(in) - 1 : 32;
+        const u64 above = (u64)from + (u64)at * step;
+        if (in != 0u) to = (uint32_t)min(above + step, (u64)to);
+        from = (uint32_t)above;
+      }
+      if (lane == 0) sh.range[warp] = most < 0 ? top_key : warp == 0 ? to : to - 1u;
+    }
+    __syncthreads();
+  };
+  // (a sum of 64 bits by halves: the one that makes the lower one run over adds to the upper one)
+  auto add_weight = [](uint32_t(*hist)[SR_BINS], uint32_t bin, u64 w) {
+    const uint32_t part = (uint32_t)w, old = atomicAdd(&hist[0][bin], part), up = (uint32_t)(w >> 32) + (old + part < old ? 1u : 0u);
+    if (up != 0u) atomicAdd(&hist[1][bin], up);
+  };
+  // The largest key of lo .. hi at or above which the counts (or weights) reach what they have to.  Counts of what lies above hi are known (`base`), weights are added up.
+  auto by_keys = [&](auto weights, uint32_t lo, uint32_t hi, u64 base, auto reached) {
+    constexpr bool WEIGHTS = decltype(weights)::value;
+    const float least = fmaxf(key_value<T>(lo), lowest), most = key_value<T>(hi);
+    for (bool begin = true;; begin = false) {
+      int shift = 0;
+      while (((hi - lo) >> shift) >= (uint32_t)SR_BINS) ++shift;
+      uint32_t(*hist)[SR_BINS] = sh.hist[turn];
+      u64 above = 0, none;
+      each(least, [&](const float (&x)[N], int) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          if (x[e] < least) continue;
+          if (x[e] > most) {
+            if (WEIGHTS && begin) above += weight(x[e]);
+            continue;
+          }
+          const uint32_t key = order_key<T>(x[e]);
+          if (key < lo || key > hi) continue;
+          const uint32_t bin = (hi - key) >> shift;
+          if (WEIGHTS) {
+            add_weight(hist, bin, weight(x[e]));
+          } else {
+            atomicAdd(&hist[0][bin], 1u);
+          }
+        }
+      });
+      if (WEIGHTS && begin) base = cluster_sum(above, none);
+      else cluster.sync();
+      u64 n[BINS];
+      counted(WEIGHTS, n);
+      u64 at = base + bins_before(n);
 #pragma unroll
       for (int b = 0; b < BINS; ++b) {
-        if (!reached(at, all, shift) && reached(at + n[b], all, shift)) sh.found = BINS * t + b, sh.found_base = at;
+        if (!reached(at) && reached(at + n[b])) sh.found = BINS * t + b, sh.found_base = at;
         at += n[b];
       }
-      // (the sums of the turn before have been read by every block: behind a barrier of the cluster that comes after)
-      for (int b = t; b < 2 * SR_BINS; b += THREADS) (&sh.hist[turn ^ 1][0][0])[b] = 0;
-      turn ^= 1;
       __syncthreads();
       const int found = sh.found;
-      if (found < 0) return;                     // (fewer than k within reach: all of them are kept)
+      if (found < 0) return lo;                  // (there is one: a border is not looked for where it cannot be)
       base = sh.found_base;
-      if (shift < 0) {
-        // the keys of the step: the smallest one at most so many steps below m, by 32 at a time
-        if (warp < 2) {
-          const int most = found - warp;
-          uint32_t from = order_key<T>(-INFINITY), to = top_key;       // above: `from` is more than `most` steps below m, `to` is not
-          while (most >= 0 && to - from > 1u) {
-            const uint32_t step = max(1u, (uint32_t)(((u64)(to - from) + 32) / 33));
-            const u64 probe = min((u64)from + (u64)(lane + 1) * step, (u64)to);
-            const float s = below(key_value<T>((uint32_t)probe));
-            const uint32_t in = __ballot_sync(0xffffffffu, s < (float)SR_BINS && (int)s <= most);
-            const int first = __ffs(in) - 1;     // (lane 31's is `to`, or the search goes on above it)
-            const uint32_t next_to = first < 0 ? to : (uint32_t)min((u64)from + (u64)(first + 1) * step, (u64)to);
-            from = first < 0 ? (uint32_t)min((u64)from + 32ull * step, (u64)to) : (uint32_t)((u64)from + (u64)first * step);
-            to = next_to;
-          }
-          if (lane == 0) sh.range[warp] = most < 0 ? top_key : warp == 0 ? to : to - 1u;
-        }
-        __syncthreads();
-        lo = sh.range[0], hi = sh.range[1];
-      } else {
-        hi -= (uint32_t)found << shift;
-        if (hi - lo >= 1u << shift) lo = hi - ((1u << shift) - 1u);
-      }
-      if (lo == hi) {
-        border = hi;
-        return;
-      }
-      shift = 0;
-      while (((hi - lo) >> shift) >= (uint32_t)SR_BINS) ++shift;
+      hi -= (uint32_t)found << shift;
+      if (hi - lo >= 1u << shift) lo = hi - ((1u << shift) - 1u);
+      if (lo == hi) return hi;
     }
   };
-  if (top_k >= 1 && top_k < V) select(std::false_type(), [&](u64 n, u64, int) { return n >= (u64)top_k; });
-  if (top_p < 1.f) {
-    double want = 0.0;
-    select(std::true_type(), [&](u64 n, u64 all, int shift) {
-      if (shift < 0) want = (double)top_p * (double)all;
-      return n > 0 && (double)n >= want;
+  // The same where SR_LIST numbers at most have keys lo .. hi: every block compares all of them.
+  auto by_list = [&](auto weights, uint32_t lo, uint32_t hi, u64 base, auto reached, int which) {
+    constexpr bool WEIGHTS = decltype(weights)::value;
+    const float least = fmaxf(key_value<T>(lo), lowest), most = key_value<T>(hi);
+    u64* const weight_here = reinterpret_cast<u64*>(&sh.hist[turn][0][0]);      // (zeros that nobody reads)
+    uint32_t* const key_here = reinterpret_cast<uint32_t*>(weight_here + SR_LIST);
+    u64 above = 0, none;
+    each(least, [&](const float (&x)[N], int) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        if (x[e] < least || (!WEIGHTS && x[e] > most)) continue;
+        const u64 w = WEIGHTS ? weight(x[e]) : 1;
+        if (x[e] > most) {
+          above += w;
+        } else {
+          const uint32_t at = atomicAdd(&sh.listed[which], 1u);
+          if (at < SR_LIST) key_here[at] = order_key<T>(x[e]), weight_here[at] = w;
+        }
+      }
     });
+    if (WEIGHTS) base = cluster_sum(above, none);
+    else cluster.sync();
+    // all lists one after the other, a warp or some a block's
+    if (t < C) sh.key[t] = min(remote(there(&sh.listed[which], t)), (uint32_t)SR_LIST);
+    // (the counts before have been read by every block; the list, until the next barrier, by others)
+    uint32_t(*hist)[SR_BINS] = sh.hist[turn ^ 1];
+    for (int b = t; b < 2 * SR_BINS; b += THREADS) hist[0][b] = 0;
+    turn ^= 1;
+    __syncthreads();
+    int n = 0;
+    for (int c = 0; c < C; ++c) {
+      const int of_c = min((int)sh.key[c], SR_LIST - n);
+      if (warp % C == c)
+        for (int i = lane + 32 * (warp / C); i < of_c; i += 32 * (WARPS / C)) {
+          const uint32_t w = there(weight_here + i, c);
+          sh.list_weight[n + i] = (u64)remote(w + 4) << 32 | remote(w);
+          sh.list_key[n + i] = remote(there(key_here + i, c));
+        }
+      n += of_c;
+    }
+    __syncthreads();
+    while (lo < hi) {
+      int shift = 0;
+      while (((hi - lo) >> shift) >= (uint32_t)SR_BINS) ++shift;
+      for (int i = t; i < n; i += THREADS)
+        if (const uint32_t key = sh.list_key[i]; key >= lo && key <= hi) add_weight(hist, (hi - key) >> shift, sh.list_weight[i]);
+      if (t == 0) sh.found = -1;
+      __syncthreads();
+      u64 here[BINS];
+#pragma unroll
+      for (int b = 0; b < BINS; ++b) {
+        uint32_t* h = &hist[0][BINS * t + b];
+        here[b] = (u64)h[SR_BINS] << 32 | h[0];
+        h[0] = h[SR_BINS] = 0;
+      }
+      u64 at = base + bins_before(here);
+#pragma unroll
+      for (int b = 0; b < BINS; ++b) {
+        if (!reached(at) && reached(at + here[b])) sh.found = BINS * t + b, sh.found_base = at;
+        at += here[b];
+      }
+      __syncthreads();
+      const int found = sh.found;
+      if (found < 0) break;                      // (there is one: a border is not looked for where it cannot be)
+      base = sh.found_base;
+      hi -= (uint32_t)found << shift;
+      if (hi - lo >= 1u << shift) lo = hi - ((1u << shift) - 1u);
+      __syncthreads();
+    }
+    return lo;
+  };
+
+  if (top_k >= 1 && top_k < V) {
+    uint32_t* hist = sh.hist[turn][0];
+    each(cut, [&](const float (&x)[N], int) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float s = below(x[e]);
+        if (s < SR_BINS - 0.5f) atomicAdd(&hist[step_of(s)], 1u);
+      }
+    });
+    cluster.sync();
+    auto reached = [&](u64 n) { return n >= (u64)top_k; };
+    u64 n[BINS];
+    counted(false, n);
+    u64 at = bins_before(n);
+#pragma unroll
+    for (int b = 0; b < BINS; ++b) {
+      if (!reached(at) && reached(at + n[b])) sh.found = BINS * t + b, sh.found_base = at, sh.range[0] = (uint32_t)n[b];
+      at += n[b];
+    }
+    __syncthreads();
+    const int found = sh.found;
+    if (found >= 0) {                            // (else all that have a weight are kept)
+      const u64 base = sh.found_base;
+      const bool few = sh.range[0] <= SR_LIST;
+      __syncthreads();
+      keys_of(found, found);
+      const uint32_t lo = sh.range[0], hi = sh.range[1];
+      const uint32_t border = lo == hi ? hi : few ? by_list(std::false_type(), lo, hi, base, reached, 0) : by_keys(std::false_type(), lo, hi, base, reached);
+      lowest = fmaxf(lowest, key_value<T>(border));
+    }
+  }
+  if (top_p < 1.f) {
+    // A step's weights as parts of its middle one, in 13 bits: each off by half of one in 8067, 2^-13.98 (a part is at least exp(-15.6 / 1024)), by 2^-17.4 with
+    // its place in the step (three roundings of a number of 1024, times 0.03), and by 2^-27 with the series: less than 2^-13 together; and a weight, rounded to a whole
+    // number, by half of one, the step's middle one too.
+    u64 all = 0, none;
+    uint32_t* hist = sh.hist[turn][0];
+    each(lowest, [&](const float (&x)[N], int) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float v = fmaxf(x[e], cut), s = below(v), at = s + 8388608.f, d = (s - (at - 8388608.f)) * (SR_REACH / SR_BINS);
+        const u64 w = weight(v);
+        if (x[e] >= lowest) {
+          all += w;
+          const float part = fmaf(fmaf(fmaf(d, -1.f / 6, 0.5f), d, -1.f) * d, 8192.f, 8192.f);
+          if (s < SR_BINS - 0.5f) atomicAdd(&hist[__float_as_int(at) & 0x7fffff], (uint32_t)(__float_as_int(part + 8388608.f) & 0x7fffff));
+        }
+      }
+    });
+    all = cluster_sum(all, none);
+    const double want = (double)top_p * (double)all;
+    u64 n[BINS];
+    uint32_t numbers[BINS];
+    counted(false, n);
+#pragma unroll
+    for (int b = 0; b < BINS; ++b) {
+      numbers[b] = (uint32_t)n[b] / 8060u + 1u;              // at most
+      n[b] = (u64)((double)n[b] * ((double)weight_of(-(BINS * t + b) * (double)(SR_REACH / SR_BINS), 369.32994026157255, sh.exps) * (1.0 / 8192)));
+    }
+    u64 at = bins_before(n);
+    constexpr double OFF = 1.0 / 8192;
+    auto may = [&](u64 x) { return ((double)x + 2 * V + 1024) * (1.0 + OFF) >= want; };
+    auto must = [&](u64 x) { return x > 0 && ((double)x - 2 * V - 1024) * (1.0 - OFF) >= want; };
+#pragma unroll
+    for (int b = 0; b < BINS; ++b) {
+      if ((BINS * t + b == 0 || !may(at)) && may(at + n[b])) sh.found = BINS * t + b;
+      if (!must(at) && must(at + n[b])) sh.last = BINS * t + b;
+      at += n[b];
+    }
+    __syncthreads();
+    const int from = max(sh.found, 0), to = sh.last;
+#pragma unroll
+    for (int b = 0; b < BINS; ++b)
+      if (BINS * t + b >= from && BINS * t + b <= to) atomicAdd(&sh.range[0], numbers[b]);
+    __syncthreads();
+    const bool few = sh.range[0] <= SR_LIST;
+    __syncthreads();
+    keys_of(from, to);
+    const uint32_t lo = sh.range[0], hi = sh.range[1];
+    auto reached = [&](u64 x) { return x > 0 && (double)x >= want; };
+    const uint32_t border = lo == hi ? hi : few ? by_list(std::true_type(), lo, hi, 0, reached, 1) : by_keys(std::true_type(), lo, hi, 0, reached);
+    lowest = fmaxf(lowest, key_value<T>(border));
   }
 
-  // ---- kept weights by runs of a warp's numbers, which follow one another in the row
-  const double least = fmin((double)min_p, 1.0) * SR_ONE;
-  // (beyond so many steps min-p keeps nothing; a step more than that comes to, for the roundings)
-  const float reach = min_p > 0.f ? fminf((float)SR_BINS, -logf(fminf(min_p, 1.f)) * ((float)SR_BINS / SR_REACH) + 1.f) : (float)SR_BINS;
+  // ---- kept weights
+  if (min_p > 0.f) {                             // the smallest number that weighs as much, by 32 at a time (every warp)
+    const u64 least = (u64)ceil((double)fminf(min_p, 1.f) * SR_ONE);
+    uint32_t from = order_key<T>(lowest) - 1u, to = order_key<T>(m);     // `from` weighs less or is not kept, `to` is
+    while (to - from > 1u) {
+      const uint32_t step = (to - from - 1u) / 33u + 1u;
+      const u64 probe = min((u64)from + (u64)(lane + 1) * step, (u64)to);
+      const uint32_t in = __ballot_sync(0xffffffffu, weight(fmaxf(key_value<T>((uint32_t)probe), cut)) >= least);
+      const int at = in != 0u ? __ffs(in) - 1 : 32;
+      const u64 above = (u64)from + (u64)at * step;
+      if (in != 0u) to = (uint32_t)min(above + step, (u64)to);
+      from = (uint32_t)above;
+    }
+    lowest = fmaxf(lowest, key_value<T>(to));
+  }
   auto kept = [&](float v) -> u64 {
-    if (order_key<T>(v) < border || !(below(v) < reach)) return 0;
-    const u64 w = weight(v);
-    return (double)w >= least ? w : 0;
+    const u64 w = weight(fmaxf(v, cut));
+    return v >= lowest ? w : 0;
   };
-  u64 total = 0;
-#pragma unroll 1
-  for (int j = 0; j < a.turns; ++j) {
-    float x[N];
-    vec_values<T>(s_row[j * THREADS + t], x);
-    u64 n = 0;
+  u64 n = 0, before = 0;
+  each(lowest, [&](const float (&x)[N], int) {
 #pragma unroll
     for (int e = 0; e < N; ++e) n += kept(x[e]);
+  });
+  const u64 total = cluster_sum(n, before);
+  const u64 target = first ? 0 : min((u64)floor((double)u * (double)total), total - 1);
+  // the warp that the target falls to goes through its run
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-    if (lane == 0) sh.segment[j][warp] = n;
-  }
-  __syncthreads();
-  if (warp == 0) {
-    for (int s = lane; s < a.turns * WARPS; s += 32) total += (&sh.segment[0][0])[s];
+  for (int w = 0; w < WARPS; ++w) before += w < warp ? sh.scan[w] : 0;
+  if (target < before || target >= before + sh.scan[warp]) return;
+  each(lowest, [&](const float (&x)[N], int j) {
+    u64 w[N], incl = 0;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    if (lane < C) cluster.map_shared_rank(sh.totals, lane)[rank] = total;
-  }
-  cluster.sync();
-  u64 before = 0;
-  total = 0;
-  for (int c = 0; c < C; ++c) {
-    if (c == rank) before = total;
-    total += sh.totals[c];
-  }
-  const u64 target = temperature == 0.f ? 0 : min((u64)floor((double)u * (double)total), total - 1);
-  if (target < before || target >= before + sh.totals[rank]) return;
-  // the run that the target falls into (every warp looks for itself), and the number in it
-  int run = -1;
-  for (int s0 = 0; s0 < a.turns * WARPS && run < 0; s0 += 32) {
-    const u64 n = s0 + lane < a.turns * WARPS ? (&sh.segment[0][0])[s0 + lane] : 0;
-    u64 incl = n;
+    for (int e = 0; e < N; ++e) w[e] = kept(x[e]), incl += w[e];
+    const u64 own = incl;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const u64 v = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += v;
     }
-    const uint32_t past = __ballot_sync(0xffffffffu, before + incl > target);
-    if (past != 0u) {
-      run = s0 + __ffs(past) - 1;
-      before += __shfl_sync(0xffffffffu, incl - n, __ffs(past) - 1);
-    } else {
-      before += __shfl_sync(0xffffffffu, incl, 31);
+    u64 at = before + incl - own;
+    if (at <= target && target < at + own) {
+      int e0 = 0;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        at += w[e];
+        if (at <= target) e0 = e + 1;
+      }
+      a.tokens[r] = i0 + j * 32 * N + e0;
     }
-  }
-  if (run < 0 || run % WARPS != warp) return;
-  const int j = run / WARPS;
-  float x[N];
-  vec_values<T>(s_row[j * THREADS + t], x);
-  u64 w[N], n = 0;
-#pragma unroll
-  for (int e = 0; e < N; ++e) w[e] = kept(x[e]), n += w[e];
-  u64 incl = n;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const u64 v = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += v;
-  }
-  u64 at = before + incl - n;
-  if (at <= target && target < at + n) {
-    int e0 = 0;
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-      at += w[e];
-      if (at <= target) e0 = e + 1;
-    }
-    a.tokens[r] = i0 + (j * THREADS + t) * N + e0;
-  }
+    before += __shfl_sync(0xffffffffu, incl, 31);
+  });
 }
 
 // Blocks a row: enough that a thread has at most 32 numbers, and more of them while there are few rows.

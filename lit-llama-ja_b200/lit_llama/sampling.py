@@ -58,7 +58,7 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature: Setting = 1.0,
     Kept are the ``top_k`` largest logits, of these the largest ones until their probabilities reach ``top_p`` of the kept ones', of these those of at
     least ``min_p`` of the largest probability; equal logits stay together, as ``generate``'s top_k keeps them.  The draw goes through the kept ones in the
     order of the vocabulary.  Weights are whole numbers of 2^-44 of the largest one, so that a draw depends on no order of sums; a token of less is not
-    drawn.  ``temperature`` 0: the largest logit (of equal ones the first).
+    drawn.  ``temperature`` 0 (under 2^-100): the largest logit (of equal ones the first).
 
     Settings are numbers or one a row on the GPU, float32 (``top_k`` int32); there a ``top_k`` below 1, a ``top_p`` of 1 and a ``min_p`` of 0 change nothing.  A row that
     allows no draw gets -1: a logit or setting that is no number, no logit above -inf, a negative temperature, a ``u`` outside of 0 to 1."""
