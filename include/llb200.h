@@ -890,6 +890,16 @@ LL_API int ll_kv4_fork(const ll_kv4_cache* cache, void* blocks, int layers, int3
 LL_API int ll_kv4_release(const ll_kv4_cache* cache, void* blocks, int layers, int32_t* shared, const int32_t* rows, const int32_t* keep, int B, int32_t* status,
                           int32_t* work, ll_stream stream);
 
+/* Plan and attention of such a cache's steps, with sizes of their own: where neighbouring sequences of a step have their first pages in common (two at least, and as many
+ * as the two before them), these pages are walked once for all of them.  Of steps of up to 32 queries of a key head a sequence, 2 to 512 sequences, in a cache for
+ * requests of more than 512 tokens; others are as ll_kv4_plan's and ll_kv4_attn's.  A plan of the one kind goes with the attention of that kind. */
+LL_API size_t ll_kv4_shared_work_ints(const ll_kv4_cache* cache, int B, int T, int max_count);
+LL_API int ll_kv4_shared_plan(const ll_kv4_cache* cache, const int32_t* rows, const int32_t* counts, int B, int T, int max_count, int32_t* out, int32_t* work,
+                              ll_stream stream);
+LL_API size_t ll_kv4_shared_attn_scratch_bytes(const ll_kv4_cache* cache, int B, int T, int max_count);
+LL_API int ll_kv4_shared_attn(const ll_kv4_cache* cache, const void* blocks, const void* q, long long q_row, const int32_t* work, void* y, int B, int T,
+                              int max_count, float scale, void* scratch, ll_stream stream);
+
 /* ---------------------------------------------------------------------------------------
  * What a step's logits are asked: a token a row (csrc/sample_rows.cu), and how likely given ones are (csrc/token_logprobs.cu).  logits: R rows of V numbers
  * (fp32, bf16 or fp16), `row` numbers apart.  Settings: one a row on the device, or null and one for all.

@@ -595,6 +595,84 @@ __global__ void __launch_bounds__(KJ * 32) kv4_join_kernel(const Kv4Attn few, co
   }
 }
 
+// Joins a sequence's parts over pages of its own with its group's over the pages that they share.  A record: first row and number of its tokens, parts of a tile of
+// its own and where they are kept; then parts of a tile of the group's, where these are kept, its first column in the group, and whether in the list of the
+// many.  A warp a column where there are up to KJ_FEW parts, else a block, a warp every KJ-th part.
+constexpr int KJ_FEW = 16;
+template <typename T, int D>
+__global__ void __launch_bounds__(KJ * 32) kv4_join_shared_kernel(const Kv4Attn few, const Kv4Attn many, const int4* __restrict__ records) {
+  constexpr int COLS = KV4_FEW_BESIDE;
+  __shared__ float s_m[KJ], s_l[KJ], s_o[KJ][D];
+  pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = few.G, R = few.H / few.G;
+  T* const y = (T*)few.y;
+  const int32_t* work = after_wait(few.work);
+  const int4* rec = after_wait(records);
+  const float *few_part = after_wait(few.part), *many_part = after_wait(many.part);
+  const float2 *few_ml = reinterpret_cast<const float2*>(few_part + (size_t)few.kept * G * COLS * D),
+               *many_ml = reinterpret_cast<const float2*>(many_part + (size_t)many.kept * G * KV4_MANY * D);
+  const int units = work[1] * G * few.cols;
+  for (int u0 = blockIdx.x * KJ; u0 < units; u0 += gridDim.x * KJ) {
+    // part k of unit u's column c: the group's first, as the keys come
+    auto walk = [&](int u, int first, int stride, KjSum<D>& s, auto emit) {
+      const int j = u / (G * few.cols), head = u / few.cols % G, c = u % few.cols;
+      const int4 a = rec[2 * j], b = rec[2 * j + 1];
+      if (c >= a.y * R) return;
+      const int gc = b.z + c;
+#pragma unroll 4
+      for (int k = first; k < b.x + a.z; k += stride) {
+        if (k >= b.x) {
+          const size_t at = ((size_t)(a.w + c / COLS * a.z + k - b.x) * G + head) * COLS + c % COLS;
+          s.add(few_ml[at], few_part + at * D, lane);
+        } else if (b.w != 0) {
+          const size_t at = ((size_t)(b.y + gc / KV4_MANY * b.x + k) * G + head) * KV4_MANY + gc % KV4_MANY;
+          s.add(many_ml[at], many_part + at * D, lane);
+        } else {
+          const size_t at = ((size_t)(b.y + gc / COLS * b.x + k) * G + head) * COLS + gc % COLS;
+          s.add(few_ml[at], few_part + at * D, lane);
+        }
+      }
+      emit((size_t)(a.x + column_token(c, R)) * few.H + head * R + column_head(c, R));
+    };
+    auto parts_of = [&](int u) {
+      const int j = u / (G * few.cols);
+      return rec[2 * j].z + rec[2 * j + 1].x;
+    };
+    if (u0 + warp < units && parts_of(u0 + warp) <= KJ_FEW) {
+      KjSum<D> s;
+      walk(u0 + warp, 0, 1, s, [&](size_t row) {
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e) dt<T>::st(y, row * D + lane + 32 * e, s.o[e] / s.l);
+      });
+    }
+    for (int i = 0; i < KJ && u0 + i < units; ++i) {
+      if (parts_of(u0 + i) <= KJ_FEW) continue;      // (the same for the whole block)
+      KjSum<D> s;
+      size_t row = 0;
+      bool there = false;
+      walk(u0 + i, warp, KJ, s, [&](size_t at) { row = at, there = true; });
+      __syncthreads();                         // (the unit before this one has been read)
+      if (lane == 0) s_m[warp] = s.m, s_l[warp] = s.l;
+#pragma unroll
+      for (int e = 0; e < D / 32; ++e) s_o[warp][lane + 32 * e] = s.o[e];
+      __syncthreads();
+      const int d = threadIdx.x;
+      if (there && d < D) {
+        float m = s_m[0], num = 0.f, den = 0.f;
+#pragma unroll
+        for (int w = 1; w < KJ; ++w) m = fmaxf(m, s_m[w]);
+#pragma unroll
+        for (int w = 0; w < KJ; ++w) {
+          const float f = kf_exp2(s_m[w] - m);
+          num = fmaf(s_o[w][d], f, num);
+          den = fmaf(s_l[w], f, den);
+        }
+        dt<T>::st(y, row * D + d, num / den);
+      }
+    }
+  }
+}
+
 }  // namespace
 }  // namespace llb
 
@@ -602,13 +680,15 @@ using namespace llb;
 
 extern "C" {
 
-size_t ll_kv4_attn_scratch_bytes(const ll_kv4_cache* cache, int B, int T, int max_count) {
+static size_t scratch_bytes(const ll_kv4_cache* cache, int B, int T, int max_count, bool share) {
   if (!kv4_step_ok(cache, B, T, max_count)) return 0;
-  return Kv4Lists(B, T, max_count, cache->heads, cache->kv_heads, cache->max_length).bytes(cache->kv_heads, cache->head_size);
+  return Kv4Lists(B, T, max_count, cache->heads, cache->kv_heads, cache->max_length, share && kv4_shares(cache, B, T, max_count)).bytes(cache->kv_heads, cache->head_size);
 }
+size_t ll_kv4_attn_scratch_bytes(const ll_kv4_cache* cache, int B, int T, int max_count) { return scratch_bytes(cache, B, T, max_count, false); }
+size_t ll_kv4_shared_attn_scratch_bytes(const ll_kv4_cache* cache, int B, int T, int max_count) { return scratch_bytes(cache, B, T, max_count, true); }
 
-int ll_kv4_attn(const ll_kv4_cache* cache, const void* blocks, const void* q, long long q_row, const int32_t* work, void* y, int B, int T, int max_count,
-                float scale, void* scratch, ll_stream stream) {
+static int attend(const ll_kv4_cache* cache, const void* blocks, const void* q, long long q_row, const int32_t* work, void* y, int B, int T, int max_count,
+                  float scale, void* scratch, ll_stream stream, bool share) {
   LL_CHECK_ARG(cache != nullptr, "kv4_attn: no cache");
   const int dtype = cache->dtype, H = cache->heads, G = cache->kv_heads, head_size = cache->head_size, group = cache->group;
   LL_CHECK_ARG(kv4_shape_ok(head_size, group), "kv4_attn: heads of %d in groups of %d (32, 64 or 128 each)", head_size, group);
@@ -619,7 +699,8 @@ int ll_kv4_attn(const ll_kv4_cache* cache, const void* blocks, const void* q, lo
   LL_CHECK_ARG(scale > 0.f && scale < INFINITY, "kv4_attn: scores times %g (more than 0, and a number of 32 bits)", scale);
   LL_CHECK_ARG((((uintptr_t)q | (uintptr_t)y | (uintptr_t)blocks | (uintptr_t)scratch | (uintptr_t)work) & 15) == 0 && q_row % 8 == 0,
                "kv4_attn: rows have to start on 16-byte boundaries");
-  const Kv4Lists l(B, T, max_count, H, G, cache->max_length);
+  share = share && kv4_shares(cache, B, T, max_count);
+  const Kv4Lists l(B, T, max_count, H, G, cache->max_length, share);
   LL_CHECK_ARG(l.few_items * G <= INT_MAX && l.many_items * G <= INT_MAX, "kv4_attn: %d sequences of %d tokens, %d heads", B, T, H);
   const int R = l.R, cols = l.cols, used = (int)std::min((long long)cols, (long long)max_count * R);
   const Kv4Attn a{q, q_row, (const uint8_t*)blocks, cache->table, work, y, (float*)scratch, H, G, cache->width, cache->pages, (int)l.few_items, l.few_kept(), used, scale,
@@ -638,9 +719,14 @@ int ll_kv4_attn(const ll_kv4_cache* cache, const void* blocks, const void* q, lo
   // The sequences of few columns fill the end of the prompts' kernel, which lets them in when it has begun.  The join waits for both (kv4_few_kernel's last blocks).
   // (None where walks are not cut, or where no sequence may bring a token: then all that bring some are refused.)
   const unsigned join_blocks =
+      share ? (unsigned)std::min<long long>(4ll * kv4_sms(), ((long long)B * G * std::min<long long>((long long)max_count * R, KV4_FEW_MOST) + KJ - 1) / KJ) :
       l.few_cut || l.many ? (unsigned)std::min<long long>(4ll * kv4_sms(), (long long)l.few_joins() * G * used + (l.many ? (long long)l.many_joins() * G * (KV4_MANY / KJ) : 0)) : 0;
   LL_CHECK_ARG(l.few_items * G + 4ll * kv4_sms() <= INT_MAX, "kv4_attn: %d sequences of %d tokens, %d heads", B, T, H);
   const unsigned few_blocks = (unsigned)(l.few_items * G) + (l.many ? 4u * kv4_sms() : 0u);
+  // (columns that a sequence may have, not a tile)
+  Kv4Attn b = a;
+  b.cols = (int)std::min<long long>((long long)max_count * R, KV4_FEW_MOST);
+  const int4* records = reinterpret_cast<const int4*>(work + l.list_ints());
 #define FEW(TT, DD, NG, CPL, NB, BESIDE)                                                                                                      \
   {                                                                                                                                           \
     static_assert(!BESIDE || 4 * CPL * NB == KV4_FEW_BESIDE, "columns beside the many");                                                      \
@@ -654,7 +740,8 @@ int ll_kv4_attn(const ll_kv4_cache* cache, const void* blocks, const void* q, lo
     }                                                                                                                                         \
     LL_CUDA(launch(kv4_few_kernel<TT, DD, NG, CPL, NB, BESIDE>, dim3(few_blocks), dim3(KF_THREADS), smem, st, l.many, a, m));           \
     LL_LAUNCH_OK("kv4_few_kernel");                                                                                                           \
-    if (join_blocks > 0) LL_CUDA(launch(kv4_join_kernel<TT, DD, COLS>, dim3(join_blocks), dim3(KJ * 32), 0, st, true, a, m));                          \
+    if (share && join_blocks > 0) LL_CUDA(launch(kv4_join_shared_kernel<TT, DD>, dim3(join_blocks), dim3(KJ * 32), 0, st, true, b, m, records));        \
+    else if (join_blocks > 0) LL_CUDA(launch(kv4_join_kernel<TT, DD, COLS>, dim3(join_blocks), dim3(KJ * 32), 0, st, true, a, m));                     \
   }
 #define FEW_COLS(TT, DD, NG)                          \
   if (l.many) FEW(TT, DD, NG, 2, 1, true)             \
@@ -670,6 +757,15 @@ int ll_kv4_attn(const ll_kv4_cache* cache, const void* blocks, const void* q, lo
 #undef FEW
   LL_LAUNCH_OK("kv4_join_kernel");
   return LL_OK;
+}
+
+int ll_kv4_attn(const ll_kv4_cache* cache, const void* blocks, const void* q, long long q_row, const int32_t* work, void* y, int B, int T, int max_count,
+                float scale, void* scratch, ll_stream stream) {
+  return attend(cache, blocks, q, q_row, work, y, B, T, max_count, scale, scratch, stream, false);
+}
+int ll_kv4_shared_attn(const ll_kv4_cache* cache, const void* blocks, const void* q, long long q_row, const int32_t* work, void* y, int B, int T, int max_count,
+                       float scale, void* scratch, ll_stream stream) {
+  return attend(cache, blocks, q, q_row, work, y, B, T, max_count, scale, scratch, stream, true);
 }
 
 }  // extern "C"

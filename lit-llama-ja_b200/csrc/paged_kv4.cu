@@ -24,8 +24,40 @@ constexpr int PLAN_HELD = 1024;      // sequences whose numbers the block holds
 
 // What the sequences of a step came to: in shared memory where there is room, else where the plan keeps it.
 struct PlanView {
+  static constexpr bool SHARED = false;
   const int32_t *starts, *ends, *request;
   int B;
+  __device__ __forceinline__ int tokens(int i) const { return starts[i + 1] - starts[i]; }
+  __device__ __forceinline__ int4 place(int i) const { return make_int4(request[i], starts[i], tokens(i), ends[i] - tokens(i)); }
+};
+
+// Walks of a step whose sequences share pages.  0 .. B - 1: the sequences, from the first page on that is theirs alone; B ..: groups of sequences that follow one
+// another, over the pages that all of them have, for all of their columns.  Of the groups those count that `most` columns lie on one side of.
+struct ShareView {
+  static constexpr bool SHARED = true;
+  PlanView v;
+  const int32_t *first_page, *group_first, *group_last;      // [v.B], [groups] first and last sequence
+  int2* note;                                                // [B] parts of a walk (of each of its tiles), and where they are kept
+  int B, R, most;
+  bool larger;
+  __device__ __forceinline__ int tokens(int i) const {
+    if (i < v.B) return larger ? 0 : v.tokens(i);
+    const int n = v.starts[group_last[i - v.B] + 1] - v.starts[group_first[i - v.B]];
+    return ((long long)n * R > most) == larger ? n : 0;
+  }
+  __device__ __forceinline__ int shared_pages(int i) const { return first_page[group_last[i - v.B]]; }
+  __device__ __forceinline__ int from(int i) const { return i < v.B ? first_page[i] : 0; }
+  __device__ __forceinline__ int pages(int i) const {
+    if (i >= v.B) return shared_pages(i);
+    return v.request[i] < 0 ? 1 : (v.ends[i] - 1) / KV4_PAGE + 1 - first_page[i];
+  }
+  __device__ __forceinline__ int4 place(int i) const {
+    if (i < v.B) return v.place(i);
+    const int g = group_first[i - v.B];                      // (behind all of these pages' keys)
+    return make_int4(v.request[g], v.starts[g], tokens(i), shared_pages(i) * KV4_PAGE);
+  }
+  // parts that say whether an item's sums are the result: those of groups and of their sequences never are
+  __device__ __forceinline__ int parts(int i, int k) const { return i >= v.B || first_page[i] > 0 ? max(k, 2) : k; }
 };
 
 // First sequence that ends behind token t (B: none).
@@ -66,19 +98,22 @@ constexpr int PW_TRIES = 48;
 // of the round that is not full the time of the shortest parts, but no less than the longest part.  Walks for several rounds even out by
 // themselves and stay whole.
 // MANY false: the sequences of up to `few` columns, whose tiles count as long as the last one; true: the others.
-template <bool MANY>
-__device__ __forceinline__ void divide_work(const PlanView& v, const PlanWork& d, int* s_count, int* s_size, int2* s_walk) {
+template <bool MANY, class View>
+__device__ __forceinline__ void divide_work(const View& v, const PlanWork& d, int* s_count, int* s_size, int2* s_walk) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  auto tokens = [&](int i) { return v.starts[i + 1] - v.starts[i]; };
+  auto tokens = [&](int i) { return v.tokens(i); };
   auto tiles = [&](int i) {
     const uint32_t c = (uint32_t)tokens(i) * (uint32_t)d.R;          // (tokens times heads fit 31 bits)
     return (c > (uint32_t)d.few) == MANY ? (int)((c + (uint32_t)d.cols - 1) / (uint32_t)d.cols) : 0;
   };
   // pages that a tile's last column sees
   auto pages = [&](int i, int tile) {
-    if (v.request[i] < 0) return 1;
+    if constexpr (View::SHARED) return v.pages(i);
+    else if (v.request[i] < 0) return 1;
+    else {
     const int n = tokens(i);
     return (v.ends[i] - n + (MANY ? min(n - 1, (int)(((uint32_t)(tile + 1) * (uint32_t)d.cols - 1) / (uint32_t)d.R)) : n - 1)) / KV4_PAGE + 1;
+    }
   };
   // tiles of the sequences, and pages of their last one, where the block can hold them; all walks
   const bool held = v.B <= PLAN_HELD;
@@ -189,17 +224,18 @@ __device__ __forceinline__ void divide_work(const PlanView& v, const PlanWork& d
   // (which of the parts of one size comes first is left to chance, and of no consequence: every part has its own place for its sums)
   auto store = [&](int i, int at, int tile, int part, int each, int k, int base) {
     if (at >= d.max_items) return;
-    const int n = tokens(i);
     int4* o = reinterpret_cast<int4*>(d.work) + 1 + 3 * (size_t)at;
-    o[0] = make_int4(v.request[i], v.starts[i], n, v.ends[i] - n);
-    o[1] = make_int4(tile, part * each, (part + 1) * each, k);
+    o[0] = v.place(i);
+    if constexpr (View::SHARED) o[1] = make_int4(tile, v.from(i) + part * each, v.from(i) + min((part + 1) * each, v.pages(i)), v.parts(i, k));
+    else o[1] = make_int4(tile, part * each, (part + 1) * each, k);
     o[2] = make_int4(part, base, 0, 0);
   };
   auto join = [&](int i, int tile, int k, int base) {
+    if constexpr (View::SHARED) return;
     const int j = atomicAdd(&s_count[0], 1);
     if (j >= d.max_joins) return;
     int4* o = const_cast<int4*>(joins_of(d.work, d.max_items)) + 2 * (size_t)j;
-    o[0] = make_int4(v.starts[i], tokens(i), tile, k);
+    o[0] = make_int4(v.place(i).y, tokens(i), tile, k);
     o[1] = make_int4(base, 0, 0, 0);
   };
   if (MANY) {
@@ -223,6 +259,7 @@ __device__ __forceinline__ void divide_work(const PlanView& v, const PlanWork& d
         const int p = wp.y;
         k = cut(p), each = (p + k - 1) / k;
         at = atomicAdd(&s_size[bucket(each)], w * k);
+        if constexpr (View::SHARED) v.note[i] = make_int2(k, at);
         if (w * k <= 4)
           for (int e = 0; e < w * k; ++e) store(i, at + e, e / k, e % k, each, k, at + e / k * k);
         if (k > 1)
@@ -314,8 +351,94 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv4_plan_kernel(const int32_t* _
   __syncthreads();
   const PlanView v{held ? s_starts : p.starts, held ? s_ends : p.ends, held ? s_request : p.request, B};
   for (int t = threadIdx.x; t < min(T, here); t += nt) place_token(v, c, p, t);
+  if (few.work == nullptr) return;                // (kv4_share_kernel divides it)
   divide_work<false>(v, few, s_need, s_size, s_walk);
   if (many.work != nullptr) divide_work<true>(v, many, s_need, s_size, s_walk);
+}
+
+// The division of a step whose sequences may share pages, by one block: neighbours that have their first pages in common, as many as the two before, are a group.
+__global__ void __launch_bounds__(PLAN_THREADS) kv4_share_kernel(Kv4Pool c, Kv4Plan p, int B, PlanWork few, PlanWork many, int32_t* records) {
+  __shared__ int s_need[32], s_size[PW_SIZES], s_groups;
+  __shared__ int s_starts[KV4_SHARE_MOST + 1], s_ends[KV4_SHARE_MOST], s_request[KV4_SHARE_MOST];
+  __shared__ int s_link[KV4_SHARE_MOST], s_page[KV4_SHARE_MOST], s_group[KV4_SHARE_MOST], s_first[KV4_SHARE_MOST / 2], s_last[KV4_SHARE_MOST / 2];
+  __shared__ int2 s_walk[PLAN_HELD], s_few[KV4_SHARE_MOST + KV4_SHARE_MOST / 2], s_many[KV4_SHARE_MOST + KV4_SHARE_MOST / 2];
+  pdl_wait();
+  const int nt = blockDim.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, R = few.R;
+  const int32_t *starts = after_wait(p.starts), *ends = after_wait(p.ends), *request = after_wait(p.request), *table = after_wait(c.table);
+  for (int i = threadIdx.x; i < B; i += nt) {
+    s_starts[i + 1] = starts[i + 1];
+    s_ends[i] = ends[i];
+    s_request[i] = request[i];
+    s_page[i] = 0;
+    s_group[i] = -1;
+  }
+  if (threadIdx.x == 0) s_starts[0] = 0, s_groups = 0;
+  __syncthreads();
+  // pages that a sequence has in common with the one before it that brings tokens: tables are alike up to where they part
+  for (int i = warp; i < B; i += nt >> 5) {
+    int link = 0;
+    if (i > 0 && s_request[i] >= 0) {
+      int j = i - 1;
+      while (j > 0 && s_starts[j + 1] == s_starts[j]) --j;
+      const int a = s_request[j], b = s_request[i];
+      if (a >= 0 && s_starts[j + 1] > s_starts[j]) {
+        int hi = min(s_ends[j] - (s_starts[j + 1] - s_starts[j]), s_ends[i] - (s_starts[i + 1] - s_starts[i])) / KV4_PAGE;      // whole, and before all of the step's tokens
+        const int32_t *ta = table + (size_t)a * c.width, *tb = table + (size_t)b * c.width;
+        while (link < hi) {                       // (the first `link` are alike, number hi is not or is of no interest)
+          const int step = (hi - link - 1) / 32 + 1, at = link + (lane + 1) * step - 1;
+          const uint32_t same = __ballot_sync(0xffffffffu, at < hi && ta[at] == tb[at]);
+          const int n = __popc(same & ~(same + 1u));      // (from the first lane on, without a gap)
+          if (n < 32) hi = min(hi, link + (n + 1) * step - 1);
+          link += n * step;
+        }
+        if (link < KV4_SHARE_LEAST) link = 0;
+      }
+    }
+    if (lane == 0) s_link[i] = link;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int before = -1, groups = 0;                 // the sequence before that brings tokens
+    bool open = false;                           // whether it is in a group
+    for (int i = 0; i < B; ++i) {
+      if (s_starts[i + 1] == s_starts[i]) continue;
+      const int link = s_request[i] >= 0 ? s_link[i] : 0;
+      if (link > 0 && (!open || link == s_page[before])) {
+        if (!open) s_first[groups++] = before, s_group[before] = groups - 1, s_page[before] = link;
+        s_group[i] = groups - 1, s_page[i] = link, s_last[groups - 1] = i, open = true;
+      } else {
+        open = false;
+      }
+      before = i;
+    }
+    s_groups = groups;
+  }
+  __syncthreads();
+  const PlanView v{s_starts, s_ends, s_request, B};
+  const int n = B + s_groups;
+  divide_work<false>(ShareView{v, s_page, s_first, s_last, s_few, n, R, KV4_FEW_MOST, false}, few, s_need, s_size, s_walk);
+  divide_work<false>(ShareView{v, s_page, s_first, s_last, s_many, n, R, KV4_FEW_MOST, true}, many, s_need, s_size, s_walk);
+  __syncthreads();
+  // what has to be joined: a sequence's parts and its group's
+  if (threadIdx.x == 0) s_need[0] = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < B; i += nt) {
+    const int count = v.tokens(i), g = s_group[i];
+    if (count == 0 || s_request[i] < 0 || (g < 0 && s_few[i].x <= 1)) continue;
+    const int at = atomicAdd(&s_need[0], 1);
+    int4* o = reinterpret_cast<int4*>(records) + 2 * (size_t)at;
+    o[0] = make_int4(s_starts[i], count, s_few[i].x, s_few[i].y);
+    if (g < 0) {
+      o[1] = make_int4(0, 0, 0, 0);
+    } else {
+      const int column = (s_starts[i] - s_starts[s_first[g]]) * R;
+      const bool large = (long long)(s_starts[s_last[g] + 1] - s_starts[s_first[g]]) * R > KV4_FEW_MOST;
+      const int2 w = large ? s_many[B + g] : s_few[B + g];
+      o[1] = make_int4(w.x, w.y, column, large ? 1 : 0);
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) few.work[1] = s_need[0];
 }
 
 // Positions and slots of a step's tokens from `here` on.
@@ -580,34 +703,51 @@ extern "C" {
 
 size_t ll_kv4_page_bytes(int head_size, int group) { return kv4_shape_ok(head_size, group) ? (size_t)kv4_bytes(head_size, head_size / group) : 0; }
 
-size_t ll_kv4_work_ints(const ll_kv4_cache* cache, int B, int T, int max_count) {
+static size_t work_ints(const ll_kv4_cache* cache, int B, int T, int max_count, bool share) {
   if (!kv4_step_ok(cache, B, T, max_count)) return 0;
-  return Kv4Lists(B, T, max_count, cache->heads, cache->kv_heads, cache->max_length).ints();
+  return Kv4Lists(B, T, max_count, cache->heads, cache->kv_heads, cache->max_length, share && kv4_shares(cache, B, T, max_count)).ints();
 }
+size_t ll_kv4_work_ints(const ll_kv4_cache* cache, int B, int T, int max_count) { return work_ints(cache, B, T, max_count, false); }
+size_t ll_kv4_shared_work_ints(const ll_kv4_cache* cache, int B, int T, int max_count) { return work_ints(cache, B, T, max_count, true); }
 
-int ll_kv4_plan(const ll_kv4_cache* cache, const int32_t* rows, const int32_t* counts, int B, int T, int max_count, int32_t* out, int32_t* work,
-                ll_stream stream) {
+static int make_plan(const ll_kv4_cache* cache, const int32_t* rows, const int32_t* counts, int B, int T, int max_count, int32_t* out, int32_t* work,
+                     ll_stream stream, bool share) {
   if (int r = check_cache(cache, "kv4_plan")) return r;
   LL_CHECK_ARG(rows && counts && out && work && ((uintptr_t)work & 15) == 0 && B > 0 && T >= 0 && max_count >= 0 && (long long)T * cache->heads <= INT_MAX,
                "kv4_plan: %d sequences of %d tokens, %d at most", B, T, max_count);
+  share = share && kv4_shares(cache, B, T, max_count);
   const Kv4Pool c = pool_of(cache);
   const Kv4Plan p{out, out + B + 1, out + 2 * (size_t)B + 1, out + 3 * (size_t)B + 1, out + 4 * (size_t)B + 1, out + 4 * (size_t)B + 1 + T};
-  const Kv4Lists l(B, T, max_count, cache->heads, cache->kv_heads, cache->max_length);
+  const Kv4Lists l(B, T, max_count, cache->heads, cache->kv_heads, cache->max_length, share);
   LL_CHECK_ARG(l.few_items * cache->kv_heads <= INT_MAX && l.many_items * cache->kv_heads <= INT_MAX, "kv4_plan: %d sequences of %d tokens, %d heads", B, T, cache->heads);
   const int longest = (cache->max_length + KV4_PAGE - 1) / KV4_PAGE;
   // (pages take a block of the few 0.8 us, of the many 1.4; a part's start and end 2 and 3, parts that are joined 3 and 8 more)
-  const PlanWork few{l.R, l.few, l.cols, longest, l.few_parts, (int)l.few_items, l.few_joins(), 2.5f, 3.5f, l.few_cut, work};
-  const PlanWork many{l.R, l.few, KV4_MANY, longest, l.many_parts, (int)l.many_items, l.many_joins(), 2.f, 5.5f, true, l.many ? work + l.few_ints() : nullptr};
+  PlanWork few{l.R, share ? INT_MAX : l.few, l.cols, longest, l.few_parts, (int)l.few_items, l.few_joins(), 2.5f, share ? 0.f : 3.5f, l.few_cut, work};
+  PlanWork many{l.R, share ? INT_MAX : l.few, KV4_MANY, longest, l.many_parts, (int)l.many_items, l.many_joins(), 2.f, share ? 0.f : 5.5f, true, l.many ? work + l.few_ints() : nullptr};
   // The block itself places the tokens of a step while that takes it a few rounds; more are placed by a grid.
   const int threads = B <= 16 && T <= 2048 ? 256 : B <= 256 && T <= 4096 ? 512 : PLAN_THREADS, here = T <= 8 * threads ? T : 0;
   cudaStream_t st = (cudaStream_t)stream;
-  kv4_plan_kernel<<<1, threads, 0, st>>>(rows, counts, B, T, here, max_count, c, p, few, many);
+  PlanWork none = few;
+  if (share) none.work = nullptr;
+  kv4_plan_kernel<<<1, threads, 0, st>>>(rows, counts, B, T, here, max_count, c, p, none, many);
   LL_LAUNCH_OK("kv4_plan_kernel");
   if (here < T) {
     LL_CUDA(launch(kv4_tokens_kernel, dim3((T - here + 255) / 256), dim3(256), 0, st, true, B, T, here, c, p));
     LL_LAUNCH_OK("kv4_tokens_kernel");
   }
+  if (share) {
+    LL_CUDA(launch(kv4_share_kernel, dim3(1), dim3(PLAN_THREADS), 0, st, here == T, c, p, B, few, many, work + l.list_ints()));
+    LL_LAUNCH_OK("kv4_share_kernel");
+  }
   return LL_OK;
+}
+int ll_kv4_plan(const ll_kv4_cache* cache, const int32_t* rows, const int32_t* counts, int B, int T, int max_count, int32_t* out, int32_t* work,
+                ll_stream stream) {
+  return make_plan(cache, rows, counts, B, T, max_count, out, work, stream, false);
+}
+int ll_kv4_shared_plan(const ll_kv4_cache* cache, const int32_t* rows, const int32_t* counts, int B, int T, int max_count, int32_t* out, int32_t* work,
+                       ll_stream stream) {
+  return make_plan(cache, rows, counts, B, T, max_count, out, work, stream, true);
 }
 
 int ll_kv4_truncate(const ll_kv4_cache* cache, const int32_t* rows, const int32_t* keep, int B, ll_stream stream) {

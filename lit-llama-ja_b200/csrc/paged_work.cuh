@@ -82,10 +82,12 @@ inline bool kv4_step_ok(const ll_kv4_cache* c, int B, int T, int max_count) {
 struct Kv4Lists {
   int R, cols, few, few_parts, many_parts;
   long long few_items, many_items;      // at most
-  bool many, few_cut;
-  Kv4Lists(int B, int T, int max_count, int H, int G, int max_length) {
+  bool many, few_cut, share;
+  int sequences;
+  // `share`: a step whose sequences may share pages (kv4_shares); its groups' walks are in both lists, and the sums of all parts are kept
+  Kv4Lists(int B, int T, int max_count, int H, int G, int max_length, bool share = false) : share(share), sequences(B) {
     R = H / G;
-    many = kv4_many(max_count, R);
+    many = share || kv4_many(max_count, R);
     const long long c = (long long)max_count * R;
     cols = many ? KV4_FEW_BESIDE : c <= 4 ? 4 : c <= 8 ? 8 : 16;
     few = many ? KV4_FEW_MOST : INT_MAX;
@@ -96,22 +98,35 @@ struct Kv4Lists {
     // tiles: of n columns n / cols, and one more a sequence that is not a whole number of them; sequences of the few have KV4_FEW_MOST columns at most
     // where the others go to the many (and refused ones, whose tokens count here too, may have any)
     const long long seqs = std::min(B, std::max(T, 1)), tiles = (long long)T * R / cols + seqs;
-    few_items = (many ? std::min(tiles, seqs * ((KV4_FEW_MOST + cols - 1) / cols)) : tiles) + KV4_CUTS * few_parts;
+    few_items = (many && !share ? std::min(tiles, seqs * ((KV4_FEW_MOST + cols - 1) / cols)) : tiles) + KV4_CUTS * few_parts;
+    if (share) few_items += tiles;      // (groups' tiles: no more columns than their sequences')
     many_items = many ? (long long)T * R / KV4_MANY + std::min(seqs, (long long)T * R / KV4_FEW_MOST) + KV4_CUTS * many_parts : 0;
   }
   // walks in more than one part: every one has a part more than it would have whole
   int few_joins() const { return KV4_CUTS * few_parts; }
   int many_joins() const { return KV4_CUTS * many_parts; }
   size_t few_ints() const { return 4 + sizeof(Kv4Item) / 4 * (size_t)few_items + sizeof(Kv4Join) / 4 * (size_t)few_joins(); }
-  size_t ints() const { return few_ints() + (many ? 4 + sizeof(Kv4Item) / 4 * (size_t)many_items + sizeof(Kv4Join) / 4 * (size_t)many_joins() : 0); }
+  size_t list_ints() const { return few_ints() + (many ? 4 + sizeof(Kv4Item) / 4 * (size_t)many_items + sizeof(Kv4Join) / 4 * (size_t)many_joins() : 0); }
+  // (where pages are shared, what has to be joined comes behind the lists, eight numbers a sequence)
+  size_t ints() const { return list_ints() + (share ? 8 * (size_t)sequences : 0); }
   // sums are kept of parts that have to be joined, and none are where there are walks for KV4_ROUNDS rounds
-  int few_kept() const { return (int)std::min(few_items, (long long)(KV4_ROUNDS + KV4_CUTS) * few_parts); }
-  int many_kept() const { return (int)std::min(many_items, (long long)(KV4_ROUNDS + KV4_CUTS) * many_parts); }
+  int few_kept() const { return share ? (int)few_items : (int)std::min(few_items, (long long)(KV4_ROUNDS + KV4_CUTS) * few_parts); }
+  int many_kept() const { return share ? (int)many_items : (int)std::min(many_items, (long long)(KV4_ROUNDS + KV4_CUTS) * many_parts); }
   size_t few_floats(int G, int D) const { return ((size_t)few_kept() * G * cols * (D + 2) + 3) / 4 * 4; }
   size_t many_floats(int G, int D) const { return (size_t)many_kept() * G * KV4_MANY * (D + 2); }
   // sums of both lists, and a word for every block of the many
   size_t bytes(int G, int D) const { return sizeof(float) * (few_floats(G, D) + many_floats(G, D)) + sizeof(int) * (size_t)many_items * G; }
 };
+
+// Whether a step of a cache whose requests share pages is divided by groups of sequences that do: steps of few columns a sequence (single tokens, drafts), of
+// requests that may be long enough to be cut, while the sums of all their parts stay below KV4_SHARE_BYTES.
+constexpr int KV4_SHARE_MOST = 512, KV4_SHARE_LEAST = 2;      // sequences at most, and pages that have to be in common
+constexpr size_t KV4_SHARE_BYTES = 512u << 20;
+inline bool kv4_shares(const ll_kv4_cache* c, int B, int T, int max_count) {
+  if (B < 2 || B > KV4_SHARE_MOST || T < 2 || kv4_many(max_count, c->heads / c->kv_heads) || c->max_length <= KV4_WHOLE * KV4_PAGE) return false;
+  const Kv4Lists l(B, T, max_count, c->heads, c->kv_heads, c->max_length, true);
+  return l.few_items * c->kv_heads <= INT_MAX / 2 && l.many_items * c->kv_heads <= INT_MAX / 2 && l.bytes(c->kv_heads, c->head_size) <= KV4_SHARE_BYTES;
+}
 
 }  // namespace
 int kv4_prompt_launch(const Kv4Attn& a, int dtype, int head_size, int group, cudaStream_t st);      // paged_prompt.cu

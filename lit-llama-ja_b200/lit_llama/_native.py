@@ -134,6 +134,10 @@ EXPORTS = {
     "ll_kv4_read": ([vp, vp, vp, vp, vp, i32, vp], C.c_int),
     "ll_kv4_attn_scratch_bytes": ([vp, i32, i32, i32], sz_t),
     "ll_kv4_attn": ([vp, vp, vp, i64, vp, vp, i32, i32, i32, C.c_float, vp, vp], C.c_int),
+    "ll_kv4_shared_work_ints": ([vp, i32, i32, i32], sz_t),
+    "ll_kv4_shared_plan": ([vp, vp, vp, i32, i32, i32, vp, vp, vp], C.c_int),
+    "ll_kv4_shared_attn_scratch_bytes": ([vp, i32, i32, i32], sz_t),
+    "ll_kv4_shared_attn": ([vp, vp, vp, i64, vp, vp, i32, i32, i32, C.c_float, vp, vp], C.c_int),
     "ll_kv4_fork": ([vp, vp, i32, vp, vp, vp, i32, vp, vp, vp], C.c_int),
     "ll_kv4_release": ([vp, vp, i32, vp, vp, vp, i32, vp, vp, vp], C.c_int),
     "ll_sample_rows": ([vp, i32, i32, i32, i64, vp, vp, C.c_float, vp, i32, vp, C.c_float, vp, C.c_float, vp, vp], C.c_int),

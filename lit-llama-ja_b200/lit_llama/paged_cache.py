@@ -128,6 +128,8 @@ class PagedCache4:
                                   n_head, n_kv_head, head_size, group, self._code)
         self._c = C.addressof(self._struct)
         self._layers = [N.ptr_at(self.blocks, i * self.blocks.stride(0)) for i in range(n_layer)]
+        # (steps of requests that share pages are divided by groups that do)
+        self._entry = {n: f"ll_kv4_{'shared_' if self.share else ''}{n}" for n in ("work_ints", "plan", "attn_scratch_bytes", "attn")}
         self._step = 0
         self._size_of = {}
 
@@ -138,7 +140,7 @@ class PagedCache4:
         if got is None:
             if len(self._size_of) >= 256:      # (prompts come in many sizes)
                 self._size_of.clear()
-            got = self._size_of[key] = (N.call_ret("ll_kv4_work_ints", self._c, *key), N.call_ret("ll_kv4_attn_scratch_bytes", self._c, *key))
+            got = self._size_of[key] = (N.call_ret(self._entry["work_ints"], self._c, *key), N.call_ret(self._entry["attn_scratch_bytes"], self._c, *key))
         return got
 
     def _here(self):
@@ -167,7 +169,7 @@ class PagedCache4:
         with self._here():
             self._step += 1
             plan = CachePlan(self, rows.numel(), tokens, min(max_count, tokens))
-            N.call("ll_kv4_plan", self._c, N.ptr(rows), N.ptr(counts), plan.B, tokens, plan.max_count, plan._out, plan._work, N.stream())
+            N.call(self._entry["plan"], self._c, N.ptr(rows), N.ptr(counts), plan.B, tokens, plan.max_count, plan._out, plan._work, N.stream())
         return plan
 
     def truncate(self, rows: Whole, lengths: Whole) -> Optional[torch.Tensor]:
@@ -293,5 +295,5 @@ class PagedCache4:
             return out
         with self._here():
             scratch = self.blocks.new_empty(plan.scratch_bytes)
-            N.call("ll_kv4_attn", self._c, self._layers[layer], N.ptr(q), q_row, plan._work, N.ptr(out), plan.B, T, plan.max_count, scale, N.ptr(scratch), N.stream())
+            N.call(self._entry["attn"], self._c, self._layers[layer], N.ptr(q), q_row, plan._work, N.ptr(out), plan.B, T, plan.max_count, scale, N.ptr(scratch), N.stream())
         return out
