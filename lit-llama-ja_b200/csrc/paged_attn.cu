@@ -80,8 +80,9 @@ struct KfPart {
   float* part;
   int kept, stride, at;
 };
-// Columns col0 .. of an item's walk.  False where a wait ran out; every thread of the block calls.
-template <typename T, int D, int NG, int CPL, int NB>
+// Columns col0 .. of an item's walk.  False where a wait ran out; every thread of the block calls, or, of a walk that one warp has (SOLO), every thread of that one,
+// which goes through all of its pages by halves.
+template <typename T, int D, int NG, int CPL, int NB, bool SOLO = false>
 __device__ __forceinline__ bool few_walk(const Kv4Attn& a, const Kv4Item& it, int head, int col0, const KfPart to, uint8_t* smem,
                                          KfShared<4 * CPL * NB, kf_stages(D, NG)>& sh) {
   constexpr int W = D / 32, KS = D / 16, COLS = 4 * CPL * NB, BYTES = kv4_bytes(D, NG), SLICE = kv4_slice_bytes(D, NG), SPG = KS / NG, STAGES = kf_stages(D, NG);
@@ -92,16 +93,22 @@ __device__ __forceinline__ bool few_walk(const Kv4Attn& a, const Kv4Item& it, in
   T* y = (T*)a.y;
   const int pos0 = it.pos0;
   const int last = pos0 + column_token(col0 + cols - 1, R);                    // position of the tile's last column: keys up to here are in sight
-  const int page0 = it.page0 + (warp >> 1), page1 = min(it.page1, last / KV4_PAGE + 1), half32 = 32 * (warp & 1);
+  const int page0 = it.page0 + (SOLO ? 0 : warp >> 1), page1 = min(it.page1, last / KV4_PAGE + 1), half32 = SOLO ? 0 : 32 * (warp & 1);
   // the warp's pages: page0, page0 + 2 ..; the last one only where its half holds keys in sight
-  const int units = page0 >= page1 ? 0 : (page1 - page0 + 1) / 2 - ((page0 + ((page1 - page0 - 1) & ~1)) * KV4_PAGE + half32 > last ? 1 : 0);
+  const int units = page0 >= page1 ? 0 : SOLO ? 2 * (page1 - page0) - ((page1 - 1) * KV4_PAGE + 32 > last ? 1 : 0) : (page1 - page0 + 1) / 2 - ((page0 + ((page1 - page0 - 1) & ~1)) * KV4_PAGE + half32 > last ? 1 : 0);
   const int32_t* table = a.table + (size_t)row * a.width + page0;
   uint8_t* ring = smem + warp * STAGES * 2 * SLICE;
   uint64_t* full = sh.full[warp];
-  const uint8_t* from = a.blocks + (size_t)head * BYTES + (warp & 1) * 2 * SLICE;
+  const uint8_t* from = a.blocks + (size_t)head * BYTES + (SOLO ? 0 : (warp & 1) * 2 * SLICE);
   const size_t page_bytes = (size_t)a.G * BYTES;
 
-  int entry = lane < units ? table[2 * lane] : 0;                       // the table's entries of 32 pages, a lane each
+  constexpr int PER = SOLO ? 2 : 1;                                     // units of a page
+  auto entry_of = [&](int i) { return i < units ? table[SOLO ? i / 2 : 2 * i] : 0; };      // of unit i's page
+  int entry = entry_of(PER * lane);                                     // the table's entries of 32 pages, a lane each
+  auto ask = [&](int page, int i, int to) {                             // unit i of the walk into a place of the ring
+    mbar_expect_tx(&full[to], 2 * SLICE);
+    bulk_load_1d(ring + to * 2 * SLICE, from + min(max(page, 0), a.pages - 1) * page_bytes + (SOLO ? (i & 1) * 2 * SLICE : 0), 2 * SLICE, &full[to]);
+  };
   if (lane == 0) {
     for (int i = 0; i < STAGES; ++i) mbar_init(&full[i], 1);
     fence_barrier_init();
@@ -109,11 +116,8 @@ __device__ __forceinline__ bool few_walk(const Kv4Attn& a, const Kv4Item& it, in
   __syncwarp();
 #pragma unroll
   for (int i = 0; i < STAGES; ++i) {
-    const int page = __shfl_sync(0xffffffffu, entry, i);
-    if (lane == 0 && i < units) {
-      mbar_expect_tx(&full[i], 2 * SLICE);
-      bulk_load_1d(ring + i * 2 * SLICE, from + min(max(page, 0), a.pages - 1) * page_bytes, 2 * SLICE, &full[i]);
-    }
+    const int page = __shfl_sync(0xffffffffu, entry, i / PER);
+    if (lane == 0 && i < units) ask(page, i, i);
   }
 
   float o[NB][KS][4];
@@ -190,7 +194,7 @@ __device__ __forceinline__ bool few_walk(const Kv4Attn& a, const Kv4Item& it, in
     ok = __all_sync(0xffffffffu, kf_wait(&full[st], parity, a.word));
     if (!ok) break;
     const uint8_t* const unit = ring + st * 2 * SLICE;
-    const int j = (page0 + 2 * i) * KV4_PAGE + half32 + g8;             // the lane's keys: j, j + 8, j + 16, j + 24
+    const int j = (SOLO ? page0 * KV4_PAGE + 32 * i : (page0 + 2 * i) * KV4_PAGE + half32) + g8;      // the lane's keys: j, j + 8, j + 16, j + 24
     // scores, in the products' units
     float s[4][NB][CPL];
     float2 pv[4][NG];
@@ -378,13 +382,10 @@ __device__ __forceinline__ bool few_walk(const Kv4Attn& a, const Kv4Item& it, in
     else add_values(std::false_type());
     // the next 32 keys for this place of the ring
     const int nxt = i + STAGES;
-    if ((nxt & 31) == 0) entry = nxt + lane < units ? table[2 * (nxt + lane)] : 0;
-    const int page = __shfl_sync(0xffffffffu, entry, nxt & 31);
+    if (nxt % (32 * PER) == 0) entry = entry_of(nxt + PER * lane);
+    const int page = __shfl_sync(0xffffffffu, entry, nxt / PER & 31);
     __syncwarp();                                                       // every lane has read the unit
-    if (lane == 0 && nxt < units) {
-      mbar_expect_tx(&full[st], 2 * SLICE);
-      bulk_load_1d(ring + st * 2 * SLICE, from + min(max(page, 0), a.pages - 1) * page_bytes, 2 * SLICE, &full[st]);
-    }
+    if (lane == 0 && nxt < units) ask(page, nxt, st);
     if (++st == STAGES) st = 0, parity ^= 1;
   }
   if (!ok) kv4_let_end();                                               // copies that were asked for end before the block does
@@ -404,10 +405,17 @@ __device__ __forceinline__ bool few_walk(const Kv4Attn& a, const Kv4Item& it, in
     for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int e = 0; e < CPL; ++e) sh.ref[warp][8 * b + CPL * t4 + e] = ref[b][e] == KV4_NONE ? KV4_NONE : ref[b][e] * kq[b][e], sh.sum[warp][8 * b + CPL * t4 + e] = sum[b][e];
-  if (__syncthreads_or(!ok)) return false;    // every unit has been read: the rings hold the warps' sums now
+  if (SOLO) {
+    __syncwarp();
+    if (!ok) return false;
+  } else if (__syncthreads_or(!ok)) {
+    return false;
+  }
+  // every unit has been read: the rings hold the warps' sums now
   pdl_launch_dependents();
-  float* so = reinterpret_cast<float*>(smem);                           // [warp][column][D + 4]
   constexpr int LD = D + 4;
+  static_assert(!SOLO || COLS * LD * 4 <= STAGES * 2 * SLICE, "a warp's sums in its ring");
+  float* so = SOLO ? reinterpret_cast<float*>(ring) - warp * COLS * LD : reinterpret_cast<float*>(smem);      // [warp][column][D + 4]
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -421,21 +429,26 @@ __device__ __forceinline__ bool few_walk(const Kv4Attn& a, const Kv4Item& it, in
         at[8] = fmaf((both - c) * (FINE ? 262144.f : 1048576.f), up, sumlo[b][r / SPG][e]);
       }
     }
-  __syncthreads();
+  if (SOLO) __syncwarp();
+  else __syncthreads();
   // the four warps' parts; the block's are stored as they are, or as the result where there is no other part
 #pragma unroll 1
-  for (int x = threadIdx.x; x < cols * (D / 4); x += KF_THREADS) {
+  for (int x = SOLO ? lane : threadIdx.x; x < cols * (D / 4); x += SOLO ? 32 : KF_THREADS) {
     const int c = x / (D / 4), d = x % (D / 4) * 4;
-    float m = sh.ref[0][c];
+    float m = sh.ref[SOLO ? warp : 0][c], l = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (SOLO) {
+      const float4 u = *reinterpret_cast<const float4*>(so + (warp * COLS + c) * LD + d);
+      l = sh.sum[warp][c], v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
+    } else {
 #pragma unroll
-    for (int w = 1; w < KF_WARPS; ++w) m = fmaxf(m, sh.ref[w][c]);
-    float l = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int w = 1; w < KF_WARPS; ++w) m = fmaxf(m, sh.ref[w][c]);
 #pragma unroll
-    for (int w = 0; w < KF_WARPS; ++w) {
-      const float f = kf_exp2(sh.ref[w][c] - m);
-      const float4 u = *reinterpret_cast<const float4*>(so + (w * COLS + c) * LD + d);
-      l = fmaf(sh.sum[w][c], f, l);
-      v[0] = fmaf(u.x, f, v[0]), v[1] = fmaf(u.y, f, v[1]), v[2] = fmaf(u.z, f, v[2]), v[3] = fmaf(u.w, f, v[3]);
+      for (int w = 0; w < KF_WARPS; ++w) {
+        const float f = kf_exp2(sh.ref[w][c] - m);
+        const float4 u = *reinterpret_cast<const float4*>(so + (w * COLS + c) * LD + d);
+        l = fmaf(sh.sum[w][c], f, l);
+        v[0] = fmaf(u.x, f, v[0]), v[1] = fmaf(u.y, f, v[1]), v[2] = fmaf(u.z, f, v[2]), v[3] = fmaf(u.w, f, v[3]);
+      }
     }
     if (it.parts == 1) {
       const int cc = col0 + c;
@@ -448,6 +461,43 @@ __device__ __forceinline__ bool few_walk(const Kv4Attn& a, const Kv4Item& it, in
     }
   }
   return true;
+}
+
+// The tiles of the list `m` that kv4_prompt_kernel has left, by `again` blocks of which this is number block0.
+template <typename T, int D, int NG, int CPL, int NB>
+__device__ __forceinline__ void left_tiles(const Kv4Attn& a, const Kv4Attn& m, int again, int block0, uint8_t* smem, KfShared<4 * CPL * NB, kf_stages(D, NG)>& sh) {
+  const int R = a.H / a.G;
+  constexpr int COLS = 4 * CPL * NB, SUBS = KV4_MANY / COLS;
+  __shared__ uint32_t s_left[KF_WARPS];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int32_t* work = after_wait(m.work);
+  const int* odd = after_wait(m.odd);
+  const long long units = (long long)min(work[0], m.items) * a.G * SUBS;
+#pragma unroll 1
+  for (long long u0 = block0; u0 < units; u0 += (long long)again * KF_THREADS) {
+    const long long mine = u0 + (long long)again * threadIdx.x;
+    const uint32_t left = __ballot_sync(0xffffffffu, mine < units && (odd[mine / SUBS] >> (mine % SUBS / (SUBS / 2)) & 1) != 0);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) s_left[threadIdx.x >> 5] = left;
+    __syncthreads();
+#pragma unroll 1
+    for (int w = 0; w < KF_WARPS; ++w)
+#pragma unroll 1
+      for (uint32_t bits = s_left[w]; bits != 0u; bits &= bits - 1) {
+        const long long unit = u0 + (long long)again * (32 * w + __ffs(bits) - 1);
+        const int block = (int)(unit / SUBS), item = block / a.G, head = block - item * a.G, at = (int)(unit % SUBS) * COLS;
+        const Kv4Item it = load_item(work, item);
+        const int col0 = it.tile * KV4_MANY + at;
+        if (col0 >= it.count * R) continue;
+        if (!few_walk<T, D, NG, CPL, NB>(a, it, head, col0, KfPart{m.part, m.kept, KV4_MANY, at}, smem, sh)) return;
+        fence_proxy_async();                                        // (the rings' memory has been written and read by threads: copies come next)
+        __syncthreads();
+        if ((threadIdx.x & 31) == 0)
+          for (int i = 0; i < kf_stages(D, NG); ++i) mbar_inval(&sh.full[threadIdx.x >> 5][i]);
+        __syncwarp();
+      }
+  }
 }
 
 // A block an item and key head of the list `a`.  BESIDE a list `m` of the many there are blocks more, which go through the tiles that kv4_prompt_kernel has
@@ -463,39 +513,8 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
   if (blockIdx.x == gridDim.x - 1) pdl_wait();
   const int R = a.H / a.G, blocks = a.items * a.G;
   if constexpr (BESIDE) {
-    if ((int)blockIdx.x >= blocks) {      // (what these read the prompts' kernel has left)
-      constexpr int SUBS = KV4_MANY / COLS;
-      __shared__ uint32_t s_left[KF_WARPS];
-      pdl_launch_dependents();
-      pdl_wait();
-      const int again = gridDim.x - blocks;
-      const int32_t* work = after_wait(m.work);
-      const int* odd = after_wait(m.odd);
-      const long long units = (long long)min(work[0], m.items) * a.G * SUBS;
-#pragma unroll 1
-      for (long long u0 = blockIdx.x - blocks; u0 < units; u0 += (long long)again * KF_THREADS) {
-        const long long mine = u0 + (long long)again * threadIdx.x;
-        const uint32_t left = __ballot_sync(0xffffffffu, mine < units && (odd[mine / SUBS] >> (mine % SUBS / (SUBS / 2)) & 1) != 0);
-        __syncthreads();
-        if ((threadIdx.x & 31) == 0) s_left[threadIdx.x >> 5] = left;
-        __syncthreads();
-#pragma unroll 1
-        for (int w = 0; w < KF_WARPS; ++w)
-#pragma unroll 1
-          for (uint32_t bits = s_left[w]; bits != 0u; bits &= bits - 1) {
-            const long long unit = u0 + (long long)again * (32 * w + __ffs(bits) - 1);
-            const int block = (int)(unit / SUBS), item = block / a.G, head = block - item * a.G, at = (int)(unit % SUBS) * COLS;
-            const Kv4Item it = load_item(work, item);
-            const int col0 = it.tile * KV4_MANY + at;
-            if (col0 >= it.count * R) continue;
-            if (!few_walk<T, D, NG, CPL, NB>(a, it, head, col0, KfPart{m.part, m.kept, KV4_MANY, at}, smem, sh)) return;
-            fence_proxy_async();                                        // (the rings' memory has been written and read by threads: copies come next)
-            __syncthreads();
-            if ((threadIdx.x & 31) == 0)
-              for (int i = 0; i < kf_stages(D, NG); ++i) mbar_inval(&sh.full[threadIdx.x >> 5][i]);
-            __syncwarp();
-          }
-      }
+    if ((int)blockIdx.x >= blocks) {
+      left_tiles<T, D, NG, CPL, NB>(a, m, gridDim.x - blocks, blockIdx.x - blocks, smem, sh);
       return;
     }
   }
@@ -513,6 +532,26 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
     return;
   }
   few_walk<T, D, NG, CPL, NB>(a, it, head, col0, KfPart{a.part, a.kept, COLS, 0}, smem, sh);
+}
+
+// The walks of a step whose sequences may share pages: a warp an item and key head of the list `a`, neighbours with neighbouring heads.  What a sequence has of its own
+// is a few pages: with a block each, four warps of a unit or two, starts, ends and the warps' meeting took most of the time (60 sequences of 1 to 200 tokens of their own, 32
+// heads: 28 us, with a warp each XX).  Blocks more go through the tiles that kv4_prompt_kernel has left.
+template <typename T, int D, int NG, int CPL>
+__global__ void __launch_bounds__(KF_THREADS, 4) kv4_solo_kernel(const Kv4Attn a, const Kv4Attn m) {
+  constexpr int COLS = 4 * CPL;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ KfShared<COLS, kf_stages(D, NG)> sh;
+  if (blockIdx.x == gridDim.x - 1) pdl_wait();      // (as in kv4_few_kernel)
+  const int blocks = (a.items * a.G + KF_WARPS - 1) / KF_WARPS;
+  if ((int)blockIdx.x >= blocks) {
+    left_tiles<T, D, NG, CPL, 1>(a, m, gridDim.x - blocks, blockIdx.x - blocks, smem, sh);
+    return;
+  }
+  const int unit = blockIdx.x * KF_WARPS + (threadIdx.x >> 5), item = unit / a.G, head = unit - item * a.G;
+  if (item >= a.items || item >= a.work[0]) return;
+  const Kv4Item it = load_item(a.work, item);
+  few_walk<T, D, NG, CPL, 1, true>(a, it, head, it.tile * COLS, KfPart{a.part, a.kept, COLS, 0}, smem, sh);
 }
 
 // Joins the parts of walks.  Of the few columns a block has one at a time, a warp every KJ-th part (a long walk is in hundreds of parts); of the
@@ -596,12 +635,11 @@ __global__ void __launch_bounds__(KJ * 32) kv4_join_kernel(const Kv4Attn few, co
 }
 
 // Joins a sequence's parts over pages of its own with its group's over the pages that they share.  A record: first row and number of its tokens, parts of a tile of
-// its own and where they are kept; then parts of a tile of the group's, where these are kept, its first column in the group, and whether in the list of the
-// many.  A warp a column where there are up to KJ_FEW parts, else a block, a warp every KJ-th part.
+// its own and where they are kept; then parts of a tile of the group's, where these are kept, its first column in the group, and 1 where in the list of the
+// many (2: the sequence is refused).  A warp a column where there are up to KJ_FEW parts, else a block, a warp every KJ-th part.
 constexpr int KJ_FEW = 16;
-template <typename T, int D>
+template <typename T, int D, int COLS>
 __global__ void __launch_bounds__(KJ * 32) kv4_join_shared_kernel(const Kv4Attn few, const Kv4Attn many, const int4* __restrict__ records) {
-  constexpr int COLS = KV4_FEW_BESIDE;
   __shared__ float s_m[KJ], s_l[KJ], s_o[KJ][D];
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = few.G, R = few.H / few.G;
@@ -618,6 +656,11 @@ __global__ void __launch_bounds__(KJ * 32) kv4_join_shared_kernel(const Kv4Attn 
       const int j = u / (G * few.cols), head = u / few.cols % G, c = u % few.cols;
       const int4 a = rec[2 * j], b = rec[2 * j + 1];
       if (c >= a.y * R) return;
+      if (b.w == 2) {                              // a refused sequence's tokens are no numbers
+        for (int x = c; x < a.y * R; x += few.cols)
+          for (int d = lane; d < D; d += 32) dt<T>::st(y, ((size_t)(a.x + column_token(x, R)) * few.H + head * R + column_head(x, R)) * D + d, NAN);
+        return;
+      }
       const int gc = b.z + c;
 #pragma unroll 4
       for (int k = first; k < b.x + a.z; k += stride) {
@@ -702,6 +745,8 @@ static int attend(const ll_kv4_cache* cache, const void* blocks, const void* q, 
   share = share && kv4_shares(cache, B, T, max_count);
   const Kv4Lists l(B, T, max_count, H, G, cache->max_length, share);
   LL_CHECK_ARG(l.few_items * G <= INT_MAX && l.many_items * G <= INT_MAX, "kv4_attn: %d sequences of %d tokens, %d heads", B, T, H);
+  // (columns that a sequence may have; all are refused where none may have one)
+  const int columns = (int)std::max(1ll, std::min<long long>((long long)max_count * l.R, KV4_FEW_MOST));
   const int R = l.R, cols = l.cols, used = (int)std::min((long long)cols, (long long)max_count * R);
   const Kv4Attn a{q, q_row, (const uint8_t*)blocks, cache->table, work, y, (float*)scratch, H, G, cache->width, cache->pages, (int)l.few_items, l.few_kept(), used, scale,
                   wait_word(), nullptr};
@@ -719,13 +764,13 @@ static int attend(const ll_kv4_cache* cache, const void* blocks, const void* q, 
   // The sequences of few columns fill the end of the prompts' kernel, which lets them in when it has begun.  The join waits for both (kv4_few_kernel's last blocks).
   // (None where walks are not cut, or where no sequence may bring a token: then all that bring some are refused.)
   const unsigned join_blocks =
-      share ? (unsigned)std::min<long long>(4ll * kv4_sms(), ((long long)B * G * std::min<long long>((long long)max_count * R, KV4_FEW_MOST) + KJ - 1) / KJ) :
+      share ? (unsigned)std::min<long long>(4ll * kv4_sms(), ((long long)B * G * columns + KJ - 1) / KJ) :
       l.few_cut || l.many ? (unsigned)std::min<long long>(4ll * kv4_sms(), (long long)l.few_joins() * G * used + (l.many ? (long long)l.many_joins() * G * (KV4_MANY / KJ) : 0)) : 0;
   LL_CHECK_ARG(l.few_items * G + 4ll * kv4_sms() <= INT_MAX, "kv4_attn: %d sequences of %d tokens, %d heads", B, T, H);
+  const unsigned solo_blocks = (unsigned)((l.few_items * G + KF_WARPS - 1) / KF_WARPS) + 4u * kv4_sms();
   const unsigned few_blocks = (unsigned)(l.few_items * G) + (l.many ? 4u * kv4_sms() : 0u);
-  // (columns that a sequence may have, not a tile)
   Kv4Attn b = a;
-  b.cols = (int)std::min<long long>((long long)max_count * R, KV4_FEW_MOST);
+  b.cols = columns;
   const int4* records = reinterpret_cast<const int4*>(work + l.list_ints());
 #define FEW(TT, DD, NG, CPL, NB, BESIDE)                                                                                                      \
   {                                                                                                                                           \
@@ -740,11 +785,26 @@ static int attend(const ll_kv4_cache* cache, const void* blocks, const void* q, 
     }                                                                                                                                         \
     LL_CUDA(launch(kv4_few_kernel<TT, DD, NG, CPL, NB, BESIDE>, dim3(few_blocks), dim3(KF_THREADS), smem, st, l.many, a, m));           \
     LL_LAUNCH_OK("kv4_few_kernel");                                                                                                           \
-    if (share && join_blocks > 0) LL_CUDA(launch(kv4_join_shared_kernel<TT, DD>, dim3(join_blocks), dim3(KJ * 32), 0, st, true, b, m, records));        \
-    else if (join_blocks > 0) LL_CUDA(launch(kv4_join_kernel<TT, DD, COLS>, dim3(join_blocks), dim3(KJ * 32), 0, st, true, a, m));                     \
+    if (join_blocks > 0) LL_CUDA(launch(kv4_join_kernel<TT, DD, COLS>, dim3(join_blocks), dim3(KJ * 32), 0, st, true, a, m));                     \
+  }
+#define SOLO(TT, DD, NG, CPL)                                                                                                                 \
+  {                                                                                                                                           \
+    constexpr int COLS = 4 * CPL, ring = KF_WARPS * kf_stages(DD, NG) * 2 * kv4_slice_bytes(DD, NG), join = KF_WARPS * COLS * (DD + 4) * 4;     \
+    constexpr int smem = ring > join ? ring : join;                                                                                           \
+    static PerDevice set;                                                                                                                     \
+    if (!set) {                                                                                                                               \
+      LL_CUDA(cudaFuncSetAttribute(kv4_solo_kernel<TT, DD, NG, CPL>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));                      \
+      prefer_max_smem(kv4_solo_kernel<TT, DD, NG, CPL>);                                                                                       \
+      set.mark();                                                                                                                             \
+    }                                                                                                                                         \
+    LL_CUDA(launch(kv4_solo_kernel<TT, DD, NG, CPL>, dim3(solo_blocks), dim3(KF_THREADS), smem, st, true, a, m));                              \
+    LL_LAUNCH_OK("kv4_solo_kernel");                                                                                                          \
+    LL_CUDA(launch(kv4_join_shared_kernel<TT, DD, COLS>, dim3(join_blocks), dim3(KJ * 32), 0, st, true, b, m, records));                       \
   }
 #define FEW_COLS(TT, DD, NG)                          \
-  if (l.many) FEW(TT, DD, NG, 2, 1, true)             \
+  if (share && cols == 4) SOLO(TT, DD, NG, 1)         \
+  else if (share) SOLO(TT, DD, NG, 2)                 \
+  else if (l.many) FEW(TT, DD, NG, 2, 1, true)             \
   else if (cols == 4) FEW(TT, DD, NG, 1, 1, false)    \
   else if (cols == 8) FEW(TT, DD, NG, 2, 1, false)    \
   else FEW(TT, DD, NG, 2, 2, false)
@@ -754,6 +814,7 @@ static int attend(const ll_kv4_cache* cache, const void* blocks, const void* q, 
   KV4_SHAPES(head_size, group, ATTN)
 #undef ATTN
 #undef FEW_COLS
+#undef SOLO
 #undef FEW
   LL_LAUNCH_OK("kv4_join_kernel");
   return LL_OK;

@@ -41,7 +41,7 @@ struct ShareView {
   int B, R, most;
   bool larger;
   __device__ __forceinline__ int tokens(int i) const {
-    if (i < v.B) return larger ? 0 : v.tokens(i);
+    if (i < v.B) return larger || v.request[i] < 0 ? 0 : v.tokens(i);      // (refused ones: kv4_join_shared_kernel)
     const int n = v.starts[group_last[i - v.B] + 1] - v.starts[group_first[i - v.B]];
     return ((long long)n * R > most) == larger ? n : 0;
   }
@@ -49,7 +49,7 @@ struct ShareView {
   __device__ __forceinline__ int from(int i) const { return i < v.B ? first_page[i] : 0; }
   __device__ __forceinline__ int pages(int i) const {
     if (i >= v.B) return shared_pages(i);
-    return v.request[i] < 0 ? 1 : (v.ends[i] - 1) / KV4_PAGE + 1 - first_page[i];
+    return (v.ends[i] - 1) / KV4_PAGE + 1 - first_page[i];
   }
   __device__ __forceinline__ int4 place(int i) const {
     if (i < v.B) return v.place(i);
@@ -89,6 +89,7 @@ struct PlanWork {
   float fixed, joined;                 // what a part costs beside its pages, and what parts that have to be joined cost the step, in pages
   bool cut;                            // whether walks may be cut
   int32_t* work;
+  int cuts = KV4_CUTS;                 // how many rounds of parts cuts may add
 };
 constexpr int PW_SIZES = 512;          // sizes of parts told apart (where there are more, by twos, fours and so on)
 constexpr int PW_TRIES = 48;
@@ -162,7 +163,7 @@ __device__ __forceinline__ void divide_work(const View& v, const PlanWork& d, in
       most = __reduce_max_sync(0xffffffffu, most), least = __reduce_min_sync(0xffffffffu, least);
       const int rounds = (n + d.parts - 1) / d.parts;
       const float load = (sum + n * d.fixed) / d.parts + (rounds - (float)n / d.parts) * (least + d.fixed);
-      return n > walks + KV4_CUTS * d.parts ? 1e30f : fmaxf(load, most + d.fixed) + (n > walks ? d.joined : 0.f);
+      return n > walks + d.cuts * d.parts ? 1e30f : fmaxf(load, most + d.fixed) + (n > walks ? d.joined : 0.f);
     };
     // the longest walk in 1, 2 .. 24, then 30, 36, 42, 48, 60 .. parts
     auto tried = [&](int k) {
@@ -424,11 +425,14 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv4_share_kernel(Kv4Pool c, Kv4P
   __syncthreads();
   for (int i = threadIdx.x; i < B; i += nt) {
     const int count = v.tokens(i), g = s_group[i];
-    if (count == 0 || s_request[i] < 0 || (g < 0 && s_few[i].x <= 1)) continue;
+    const bool refused = s_request[i] < 0;
+    if (count == 0 || (!refused && g < 0 && s_few[i].x <= 1)) continue;
     const int at = atomicAdd(&s_need[0], 1);
     int4* o = reinterpret_cast<int4*>(records) + 2 * (size_t)at;
-    o[0] = make_int4(s_starts[i], count, s_few[i].x, s_few[i].y);
-    if (g < 0) {
+    o[0] = make_int4(s_starts[i], count, refused ? 0 : s_few[i].x, s_few[i].y);
+    if (refused) {
+      o[1] = make_int4(0, 0, 0, 2);
+    } else if (g < 0) {
       o[1] = make_int4(0, 0, 0, 0);
     } else {
       const int column = (s_starts[i] - s_starts[s_first[g]]) * R;
@@ -721,12 +725,13 @@ static int make_plan(const ll_kv4_cache* cache, const int32_t* rows, const int32
   const Kv4Lists l(B, T, max_count, cache->heads, cache->kv_heads, cache->max_length, share);
   LL_CHECK_ARG(l.few_items * cache->kv_heads <= INT_MAX && l.many_items * cache->kv_heads <= INT_MAX, "kv4_plan: %d sequences of %d tokens, %d heads", B, T, cache->heads);
   const int longest = (cache->max_length + KV4_PAGE - 1) / KV4_PAGE;
-  // (pages take a block of the few 0.8 us, of the many 1.4; a part's start and end 2 and 3, parts that are joined 3 and 8 more)
+  // (pages take a block of the few 0.8 us, of the many 1.4; a part's start and end 2 and 3, parts that are joined 3 and 8 more; a warp alone 3.2 and 2)
   PlanWork few{l.R, share ? INT_MAX : l.few, l.cols, longest, l.few_parts, (int)l.few_items, l.few_joins(), 2.5f, share ? 0.f : 3.5f, l.few_cut, work};
   PlanWork many{l.R, share ? INT_MAX : l.few, KV4_MANY, longest, l.many_parts, (int)l.many_items, l.many_joins(), 2.f, share ? 0.f : 5.5f, true, l.many ? work + l.few_ints() : nullptr};
   // The block itself places the tokens of a step while that takes it a few rounds; more are placed by a grid.
   const int threads = B <= 16 && T <= 2048 ? 256 : B <= 256 && T <= 4096 ? 512 : PLAN_THREADS, here = T <= 8 * threads ? T : 0;
   cudaStream_t st = (cudaStream_t)stream;
+  if (share) few.cuts = many.cuts = KV4_SHARE_CUTS, few.fixed = 0.7f;
   PlanWork none = few;
   if (share) none.work = nullptr;
   kv4_plan_kernel<<<1, threads, 0, st>>>(rows, counts, B, T, here, max_count, c, p, none, many);

@@ -68,6 +68,7 @@ constexpr float KV4_NONE = -1e37f;      // the reference of a column that has se
 constexpr int KV4_FEW_MOST = 32, KV4_FEW_BESIDE = 8, KV4_MANY = 256, KV4_WHOLE = 8;
 // Walks for KV4_ROUNDS rounds of blocks stay whole; fewer are cut into at most KV4_CUTS rounds more of parts.
 constexpr int KV4_ROUNDS = 3, KV4_CUTS = 2;
+constexpr int KV4_SOLO = 16, KV4_SHARE_CUTS = 1;      // where pages are shared: warps of an SM that have a walk each, and rounds of them that cuts add
 
 inline bool kv4_many(int max_count, int R) { return (long long)max_count * R > KV4_FEW_MOST; }
 inline int kv4_sms() { return sm_count() > 0 ? sm_count() : 148; }
@@ -89,17 +90,18 @@ struct Kv4Lists {
     R = H / G;
     many = share || kv4_many(max_count, R);
     const long long c = (long long)max_count * R;
-    cols = many ? KV4_FEW_BESIDE : c <= 4 ? 4 : c <= 8 ? 8 : 16;
+    cols = many && !(share && c <= 4) ? KV4_FEW_BESIDE : c <= 4 ? 4 : c <= 8 ? 8 : 16;
     few = many ? KV4_FEW_MOST : INT_MAX;
-    few_parts = std::max(1, 4 * kv4_sms() / G);
+    few_parts = std::max(1, (share ? KV4_SOLO : 4) * kv4_sms() / G);      // (a warp a walk where pages are shared: its blocks have four)
     many_parts = std::max(1, kv4_sms() / G);
     // Where no request has more than KV4_WHOLE pages, walks are not cut, and there is nothing to join.
     few_cut = max_length > KV4_WHOLE * KV4_PAGE;
     // tiles: of n columns n / cols, and one more a sequence that is not a whole number of them; sequences of the few have KV4_FEW_MOST columns at most
     // where the others go to the many (and refused ones, whose tokens count here too, may have any)
     const long long seqs = std::min(B, std::max(T, 1)), tiles = (long long)T * R / cols + seqs;
-    few_items = (many && !share ? std::min(tiles, seqs * ((KV4_FEW_MOST + cols - 1) / cols)) : tiles) + KV4_CUTS * few_parts;
-    if (share) few_items += tiles;      // (groups' tiles: no more columns than their sequences')
+    few_items = (many ? std::min(tiles, seqs * ((KV4_FEW_MOST + cols - 1) / cols)) : tiles) + KV4_CUTS * few_parts;
+    // (groups have no more tiles than their sequences; of refused ones, which may have any number of columns, there are no items)
+    if (share) few_items = 2 * seqs * ((c + cols - 1) / cols) + KV4_SHARE_CUTS * few_parts;
     many_items = many ? (long long)T * R / KV4_MANY + std::min(seqs, (long long)T * R / KV4_FEW_MOST) + KV4_CUTS * many_parts : 0;
   }
   // walks in more than one part: every one has a part more than it would have whole
