@@ -536,7 +536,7 @@ __global__ void __launch_bounds__(KF_THREADS, NB == 1 ? 4 : 2) kv4_few_kernel(co
 
 // The walks of a step whose sequences may share pages: a warp an item and key head of the list `a`, neighbours with neighbouring heads.  What a sequence has of its own
 // is a few pages: with a block each, four warps of a unit or two, starts, ends and the warps' meeting took most of the time (60 sequences of 1 to 200 tokens of their own, 32
-// heads: 28 us, with a warp each XX).  Blocks more go through the tiles that kv4_prompt_kernel has left.
+// heads: 28 us, with a warp each 14).  Blocks more go through the tiles that kv4_prompt_kernel has left.
 template <typename T, int D, int NG, int CPL>
 __global__ void __launch_bounds__(KF_THREADS, 4) kv4_solo_kernel(const Kv4Attn a, const Kv4Attn m) {
   constexpr int COLS = 4 * CPL;
@@ -636,8 +636,8 @@ __global__ void __launch_bounds__(KJ * 32) kv4_join_kernel(const Kv4Attn few, co
 
 // Joins a sequence's parts over pages of its own with its group's over the pages that they share.  A record: first row and number of its tokens, parts of a tile of
 // its own and where they are kept; then parts of a tile of the group's, where these are kept, its first column in the group, and 1 where in the list of the
-// many (2: the sequence is refused).  A warp a column where there are up to KJ_FEW parts, else a block, a warp every KJ-th part.
-constexpr int KJ_FEW = 16;
+// many (2: the sequence is refused).  A warp a column where there are up to 32 parts, a lane each for their references and sums, so that all of them are asked for at
+// once (one after the other 11 us for 64 sequences of 32 heads, now 6.5); else a block, a warp every KJ-th part.
 template <typename T, int D, int COLS>
 __global__ void __launch_bounds__(KJ * 32) kv4_join_shared_kernel(const Kv4Attn few, const Kv4Attn many, const int4* __restrict__ records) {
   __shared__ float s_m[KJ], s_l[KJ], s_o[KJ][D];
@@ -651,56 +651,75 @@ __global__ void __launch_bounds__(KJ * 32) kv4_join_shared_kernel(const Kv4Attn 
                *many_ml = reinterpret_cast<const float2*>(many_part + (size_t)many.kept * G * KV4_MANY * D);
   const int units = work[1] * G * few.cols;
   for (int u0 = blockIdx.x * KJ; u0 < units; u0 += gridDim.x * KJ) {
-    // part k of unit u's column c: the group's first, as the keys come
-    auto walk = [&](int u, int first, int stride, KjSum<D>& s, auto emit) {
-      const int j = u / (G * few.cols), head = u / few.cols % G, c = u % few.cols;
-      const int4 a = rec[2 * j], b = rec[2 * j + 1];
-      if (c >= a.y * R) return;
-      if (b.w == 2) {                              // a refused sequence's tokens are no numbers
-        for (int x = c; x < a.y * R; x += few.cols)
-          for (int d = lane; d < D; d += 32) dt<T>::st(y, ((size_t)(a.x + column_token(x, R)) * few.H + head * R + column_head(x, R)) * D + d, NAN);
-        return;
-      }
-      const int gc = b.z + c;
-#pragma unroll 4
-      for (int k = first; k < b.x + a.z; k += stride) {
-        if (k >= b.x) {
-          const size_t at = ((size_t)(a.w + c / COLS * a.z + k - b.x) * G + head) * COLS + c % COLS;
-          s.add(few_ml[at], few_part + at * D, lane);
-        } else if (b.w != 0) {
-          const size_t at = ((size_t)(b.y + gc / KV4_MANY * b.x + k) * G + head) * KV4_MANY + gc % KV4_MANY;
-          s.add(many_ml[at], many_part + at * D, lane);
-        } else {
-          const size_t at = ((size_t)(b.y + gc / COLS * b.x + k) * G + head) * COLS + gc % COLS;
-          s.add(few_ml[at], few_part + at * D, lane);
-        }
-      }
-      emit((size_t)(a.x + column_token(c, R)) * few.H + head * R + column_head(c, R));
+    struct Unit {
+      int4 a, b;
+      int head, c;
     };
-    auto parts_of = [&](int u) {
+    auto unit_of = [&](int u) {
       const int j = u / (G * few.cols);
-      return rec[2 * j].z + rec[2 * j + 1].x;
+      return Unit{rec[2 * j], rec[2 * j + 1], u / few.cols % G, u % few.cols};
     };
-    if (u0 + warp < units && parts_of(u0 + warp) <= KJ_FEW) {
-      KjSum<D> s;
-      walk(u0 + warp, 0, 1, s, [&](size_t row) {
+    // where part k's sums are, the group's first, as the keys come
+    auto part_at = [&](const Unit& n, int k, bool& in_many) {
+      const int gc = n.b.z + n.c;
+      in_many = k < n.b.x && n.b.w != 0;
+      if (k >= n.b.x) return ((size_t)(n.a.w + n.c / COLS * n.a.z + k - n.b.x) * G + n.head) * COLS + n.c % COLS;
+      if (in_many) return ((size_t)(n.b.y + gc / KV4_MANY * n.b.x + k) * G + n.head) * KV4_MANY + gc % KV4_MANY;
+      return ((size_t)(n.b.y + gc / COLS * n.b.x + k) * G + n.head) * COLS + gc % COLS;
+    };
+    auto row_of = [&](const Unit& n, int c) { return (size_t)(n.a.x + column_token(c, R)) * few.H + n.head * R + column_head(c, R); };
+    bool longer = false;
+    if (u0 + warp < units) {
+      const Unit n = unit_of(u0 + warp);
+      const int parts = n.a.z + n.b.x;
+      longer = parts > 32;
+      if (n.b.w == 2) {                          // a refused sequence's tokens are no numbers
+        for (int x = n.c; x < n.a.y * R; x += few.cols)
+          for (int d = lane; d < D; d += 32) dt<T>::st(y, row_of(n, x) * D + d, NAN);
+      } else if (!longer && n.c < n.a.y * R) {
+        float2 u = make_float2(KV4_NONE, 0.f);
+        unsigned long long mine = 0;
+        if (lane < parts) {
+          bool in_many;
+          const size_t at = part_at(n, lane, in_many);
+          u = in_many ? many_ml[at] : few_ml[at];
+          mine = reinterpret_cast<unsigned long long>((in_many ? many_part : few_part) + at * D);
+        }
+        const float m = warp_max(u.y == 0.f ? KV4_NONE : u.x), w = u.y == 0.f ? 0.f : kf_exp2(u.x - m), l = warp_sum(u.y * w);
+        float o[D / 32] = {};
+#pragma unroll 8
+        for (int k = 0; k < parts; ++k) {
+          const float* part = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, mine, k));
+          const float wk = __shfl_sync(0xffffffffu, w, k);
 #pragma unroll
-        for (int e = 0; e < D / 32; ++e) dt<T>::st(y, row * D + lane + 32 * e, s.o[e] / s.l);
-      });
+          for (int e = 0; e < D / 32; ++e) {
+            const float v = part[lane + 32 * e];
+            o[e] = wk == 0.f ? o[e] : fmaf(v, wk, o[e]);      // (a part that holds no key of the column's may hold anything)
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e) dt<T>::st(y, row_of(n, n.c) * D + lane + 32 * e, o[e] / l);
+      }
     }
+    if (__syncthreads_or(longer) == 0) continue;
     for (int i = 0; i < KJ && u0 + i < units; ++i) {
-      if (parts_of(u0 + i) <= KJ_FEW) continue;      // (the same for the whole block)
+      const Unit n = unit_of(u0 + i);
+      const int parts = n.a.z + n.b.x;
+      if (parts <= 32 || n.c >= n.a.y * R) continue;      // (the same for the whole block)
       KjSum<D> s;
-      size_t row = 0;
-      bool there = false;
-      walk(u0 + i, warp, KJ, s, [&](size_t at) { row = at, there = true; });
+#pragma unroll 4
+      for (int k = warp; k < parts; k += KJ) {
+        bool in_many;
+        const size_t at = part_at(n, k, in_many);
+        s.add(in_many ? many_ml[at] : few_ml[at], (in_many ? many_part : few_part) + at * D, lane);
+      }
       __syncthreads();                         // (the unit before this one has been read)
       if (lane == 0) s_m[warp] = s.m, s_l[warp] = s.l;
 #pragma unroll
       for (int e = 0; e < D / 32; ++e) s_o[warp][lane + 32 * e] = s.o[e];
       __syncthreads();
       const int d = threadIdx.x;
-      if (there && d < D) {
+      if (d < D) {
         float m = s_m[0], num = 0.f, den = 0.f;
 #pragma unroll
         for (int w = 1; w < KJ; ++w) m = fmaxf(m, s_m[w]);
@@ -710,7 +729,7 @@ __global__ void __launch_bounds__(KJ * 32) kv4_join_shared_kernel(const Kv4Attn 
           num = fmaf(s_o[w][d], f, num);
           den = fmaf(s_l[w], f, den);
         }
-        dt<T>::st(y, row * D + d, num / den);
+        dt<T>::st(y, row_of(n, n.c) * D + d, num / den);
       }
     }
   }

@@ -417,8 +417,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv4_share_kernel(Kv4Pool c, Kv4P
   __syncthreads();
   const PlanView v{s_starts, s_ends, s_request, B};
   const int n = B + s_groups;
-  divide_work<false>(ShareView{v, s_page, s_first, s_last, s_few, n, R, KV4_FEW_MOST, false}, few, s_need, s_size, s_walk);
-  divide_work<false>(ShareView{v, s_page, s_first, s_last, s_many, n, R, KV4_FEW_MOST, true}, many, s_need, s_size, s_walk);
+  divide_work<false>(ShareView{v, s_page, s_first, s_last, s_few, n, R, KV4_SHARE_FEW, false}, few, s_need, s_size, s_walk);
+  divide_work<false>(ShareView{v, s_page, s_first, s_last, s_many, n, R, KV4_SHARE_FEW, true}, many, s_need, s_size, s_walk);
   __syncthreads();
   // what has to be joined: a sequence's parts and its group's
   if (threadIdx.x == 0) s_need[0] = 0;
@@ -436,7 +436,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv4_share_kernel(Kv4Pool c, Kv4P
       o[1] = make_int4(0, 0, 0, 0);
     } else {
       const int column = (s_starts[i] - s_starts[s_first[g]]) * R;
-      const bool large = (long long)(s_starts[s_last[g] + 1] - s_starts[s_first[g]]) * R > KV4_FEW_MOST;
+      const bool large = (long long)(s_starts[s_last[g] + 1] - s_starts[s_first[g]]) * R > KV4_SHARE_FEW;
       const int2 w = large ? s_many[B + g] : s_few[B + g];
       o[1] = make_int4(w.x, w.y, column, large ? 1 : 0);
     }

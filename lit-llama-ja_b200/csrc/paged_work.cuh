@@ -123,6 +123,7 @@ struct Kv4Lists {
 // Whether a step of a cache whose requests share pages is divided by groups of sequences that do: steps of few columns a sequence (single tokens, drafts), of
 // requests that may be long enough to be cut, while the sums of all their parts stay below KV4_SHARE_BYTES.
 constexpr int KV4_SHARE_MOST = 512, KV4_SHARE_LEAST = 2;      // sequences at most, and pages that have to be in common
+constexpr int KV4_SHARE_FEW = 32;                             // columns of groups that go to the kernel of few columns
 constexpr size_t KV4_SHARE_BYTES = 512u << 20;
 inline bool kv4_shares(const ll_kv4_cache* c, int B, int T, int max_count) {
   if (B < 2 || B > KV4_SHARE_MOST || T < 2 || kv4_many(max_count, c->heads / c->kv_heads) || c->max_length <= KV4_WHOLE * KV4_PAGE) return false;
