@@ -880,7 +880,7 @@ LL_API int ll_kv4_attn(const ll_kv4_cache* cache, const void* blocks, const void
                        int max_count, float scale, void* scratch, ll_stream stream);
 /* Requests that share pages (csrc/paged_share.cu).  shared: [2][pages], zeros and then -1 before the first call: holders of a page beyond its first, and scratch.
  * A cache whose requests share pages is cut by ll_kv4_release, never by ll_kv4_truncate.  blocks: the cache's, `layers` of [pages][kv_heads][page bytes] one
- * after the other.  work: 5 B numbers.
+ * after the other.  work: 5 B + 1 numbers.
  * Fork: the empty request into[i] becomes a copy of rows[i] as it is before the call; whole pages are shared, a last one that is not full is copied.  Status: 0 done;
  * 1 no free page for that; 3 no such request, into[i] is not empty or an earlier sequence names it.  Copies that are refused stay empty.
  * Release: as ll_kv4_truncate, and a page goes back with its last holder.  A cut that ends inside a page which others hold copies it; status 1: no page was free before

@@ -10,21 +10,58 @@
 namespace llb {
 namespace {
 
-// What a call notes of its sequences, [B] each: a page to copy and where to (-1: none), entries of the table that are given back, pages that become free
-// (then: those of the sequences before).
+// What a call notes: of its sequences, [B] each, entries of the table that are shared or given back and a number of tokens (-1: nothing to do); and its copies of pages,
+// one after the other, their number behind them.
 struct ShareWork {
-  int32_t *src, *dst, *first, *end, *freed;
-  __host__ __device__ ShareWork(int32_t* w, int B) : src(w), dst(w + B), first(w + 2 * (size_t)B), end(w + 3 * (size_t)B), freed(w + 4 * (size_t)B) {}
+  int32_t *first, *end, *tokens, *src, *dst, *copies;
+  int B;
+  __host__ __device__ ShareWork(int32_t* w, int B)
+      : first(w), end(w + B), tokens(w + 2 * (size_t)B), src(w + 3 * (size_t)B), dst(w + 4 * (size_t)B), copies(w + 5 * (size_t)B), B(B) {}
 };
 
-// Empty requests into[i] become copies of rows[i], both as they are before the call.  One block: a thread a sequence decides, a warp a sequence copies its
-// entries of the table.
-__global__ void __launch_bounds__(PLAN_THREADS) kv4_fork_kernel(const int32_t* __restrict__ rows, const int32_t* __restrict__ into, int B, Kv4Pool c,
+// The entries of a round of sequences (as many as the block has threads), one after the other: a thread has SHARE_EACH neighbours, whichever sequences these are of.
+// What bounds both kernels are dependent loads, atomics and sums of one block; with a warp a sequence, 203 sequences of 17 entries each, a fork took 11 us and a cut 27, now
+// XX and XX.
+constexpr int SHARE_EACH = 4;
+struct ShareRound {
+  int sum[32], row[PLAN_THREADS], first[PLAN_THREADS], at[PLAN_THREADS + 1];
+};
+// Threads bring their sequence's request (or -1), first entry and number of entries; returns the entries of all.
+__device__ __forceinline__ int round_entries(ShareRound& s, int row, int first, int n) {
+  int all;
+  const int before = block_before<int>(n, s.sum, all);
+  s.row[threadIdx.x] = row;
+  s.first[threadIdx.x] = first;
+  s.at[threadIdx.x] = before;
+  if (threadIdx.x == 0) s.at[blockDim.x] = all;
+  __syncthreads();
+  return all;
+}
+// Entries e0 .. e0 + SHARE_EACH - 1: their sequences in the round, and their places in the tables.
+__device__ __forceinline__ void find_entries(const ShareRound& s, int e0, int all, int (&seq)[SHARE_EACH], int (&entry)[SHARE_EACH]) {
+  int lo = 0, hi = blockDim.x;                   // the last sequence that begins at e0 or before it, and has entries
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (s.at[mid + 1] > e0) hi = mid;
+    else lo = mid + 1;
+  }
+#pragma unroll
+  for (int q = 0; q < SHARE_EACH; ++q) {
+    const int e = e0 + q;
+    if (e < all)
+      while (s.at[lo + 1] <= e) ++lo;
+    seq[q] = e < all ? lo : -1;
+    entry[q] = e < all ? s.first[lo] + e - s.at[lo] : 0;
+  }
+}
+
+// Empty requests into[i] become copies of rows[i], both as they are before the call.
+__global__ void __launch_bounds__(PLAN_THREADS) kv4_fork_kernel(const int32_t* __restrict__ rows, const int32_t* __restrict__ into, Kv4Pool c,
                                                                int32_t* __restrict__ shared, int32_t* __restrict__ status, ShareWork w) {
-  __shared__ int s_sum[32];
-  __shared__ int s_from[PLAN_THREADS], s_to[PLAN_THREADS], s_whole[PLAN_THREADS], s_new[PLAN_THREADS];
+  __shared__ ShareRound s;
+  __shared__ int s_to[PLAN_THREADS];
   __shared__ __align__(16) int s_name[PLAN_NEAR];
-  const int n_free = min(max(*c.n_free, 0), c.pages), nt = blockDim.x, lane = threadIdx.x & 31;
+  const int n_free = min(max(*c.n_free, 0), c.pages), nt = blockDim.x, B = w.B;
   claim_requests(into, into, true, B, c);
   long long wanted = 0;
   int given = 0;
@@ -34,151 +71,173 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv4_fork_kernel(const int32_t* _
     const bool mine = claimed(i, to, to >= 0 && to < c.requests, B, c, s_name) && named && c.lengths[max(to, 0)] == 0;
     const int held = mine ? c.lengths[from] : 0, whole = held / KV4_PAGE, part = held % KV4_PAGE != 0 ? 1 : 0;
     int all;
-    const long long before = wanted + block_before<int>(part, s_sum, all);
+    const long long before = wanted + block_before<int>(part, s.sum, all);
     wanted += all;
     const bool fits = part == 0 || before < n_free, ok = mine && fits, copy = ok && part != 0;
-    block_before<int>(copy ? 1 : 0, s_sum, all);
-    given += all;
-    s_from[threadIdx.x] = from;
-    s_to[threadIdx.x] = to;
-    s_whole[threadIdx.x] = ok ? whole : 0;
-    const int page = copy ? c.free[n_free - 1 - (int)before] : -1;
-    s_new[threadIdx.x] = page;
+    given += __syncthreads_count(copy);
+    if (copy) {                                  // (all that wanted a page before have one)
+      const int page = c.free[n_free - 1 - (int)before];
+      w.src[before] = c.table[(size_t)from * c.width + whole];
+      w.dst[before] = page;
+      c.table[(size_t)to * c.width + whole] = page;
+    }
     if (i < B) {
       status[i] = !mine ? KV4_BAD_ROW : fits ? KV4_OK : KV4_NO_PAGES;
-      w.src[i] = copy ? c.table[(size_t)from * c.width + whole] : -1;
-      w.dst[i] = page;
-      w.end[i] = ok ? held : 0;
+      w.tokens[i] = ok ? held : 0;
     }
-    __syncthreads();
-    for (int j = threadIdx.x >> 5; j < min(nt, B - i0); j += nt >> 5) {
-      if (s_whole[j] == 0 && s_new[j] < 0) continue;
-      const int32_t* a = c.table + (size_t)s_from[j] * c.width;
-      int32_t* b = c.table + (size_t)s_to[j] * c.width;
-      for (int k = lane; k < s_whole[j]; k += 32) {
-        const int p = a[k];
-        b[k] = p;
-        atomicAdd(&shared[p], 1);
-      }
-      if (lane == 0 && s_new[j] >= 0) b[s_whole[j]] = s_new[j];
+    s_to[threadIdx.x] = to;
+    const int entries = round_entries(s, from, 0, ok ? whole : 0);
+    for (int e0 = SHARE_EACH * threadIdx.x; e0 < entries; e0 += SHARE_EACH * nt) {
+      int seq[SHARE_EACH], entry[SHARE_EACH], page[SHARE_EACH];
+      find_entries(s, e0, entries, seq, entry);
+#pragma unroll
+      for (int q = 0; q < SHARE_EACH; ++q)
+        if (seq[q] >= 0) page[q] = c.table[(size_t)s.row[seq[q]] * c.width + entry[q]];
+#pragma unroll
+      for (int q = 0; q < SHARE_EACH; ++q)
+        if (seq[q] >= 0) {
+          c.table[(size_t)s_to[seq[q]] * c.width + entry[q]] = page[q];
+          atomicAdd(&shared[page[q]], 1);
+        }
     }
     __syncthreads();
   }
-  if (threadIdx.x == 0) *c.n_free = n_free - given;
+  if (threadIdx.x == 0) *c.n_free = n_free - given, *w.copies = given;
   for (int i = threadIdx.x; i < B; i += nt)      // (lengths change when all have been read: a request may be a copy and have one that names it)
-    if (w.end[i] > 0) c.lengths[into[i]] = w.end[i];
+    if (w.tokens[i] > 0) c.lengths[into[i]] = w.tokens[i];
 }
 
 // Requests are cut to `keep` tokens.  All decisions are taken on the pool as it is before the call: a cut inside a page that others hold needs a free page
 // for its copy, and is refused where there is none.  A page goes back to the stack when its last holder has given it back, in the order of the sequences, and
 // by the last of those that give it back in one call: whoever comes first makes no difference.
-__global__ void __launch_bounds__(PLAN_THREADS) kv4_release_kernel(const int32_t* __restrict__ rows, const int32_t* __restrict__ keep, int B, Kv4Pool c,
+__global__ void __launch_bounds__(PLAN_THREADS) kv4_release_kernel(const int32_t* __restrict__ rows, const int32_t* __restrict__ keep, Kv4Pool c,
                                                                   int32_t* __restrict__ shared, int32_t* __restrict__ status, ShareWork w) {
-  __shared__ int s_sum[32];
+  __shared__ ShareRound s;
+  __shared__ int s_freed;
   __shared__ __align__(16) int s_name[PLAN_NEAR];
-  const int n_free = min(max(*c.n_free, 0), c.pages), nt = blockDim.x, lane = threadIdx.x & 31;
+  const int n_free = min(max(*c.n_free, 0), c.pages), nt = blockDim.x, B = w.B;
   int32_t* const latest = shared + c.pages;      // the last sequence that gives a page back (-1 between calls)
   claim_requests(rows, keep, true, B, c);
-  int copies = 0;
+  if (threadIdx.x == 0) s_freed = 0;
+  int copies = 0, row = -1, first = 0, end = -1, to = -1;
   long long wanted = 0;
   for (int i0 = 0; i0 < B; i0 += nt) {
-    const int i = i0 + threadIdx.x, row = i < B ? rows[i] : -1, to = i < B ? keep[i] : -1;
+    const int i = i0 + threadIdx.x;
+    row = i < B ? rows[i] : -1, to = i < B ? keep[i] : -1;
     const bool named = row >= 0 && row < c.requests;
     const int old = named ? c.lengths[row] : 0;
     const bool cut = claimed(i, row, named, B, c, s_name) && to >= 0 && to < old;
     const int page = cut && to % KV4_PAGE != 0 ? c.table[(size_t)row * c.width + to / KV4_PAGE] : -1;
     const int part = page >= 0 && shared[page] > 0 ? 1 : 0;
     int all;
-    const long long before = wanted + block_before<int>(part, s_sum, all);
+    const long long before = wanted + block_before<int>(part, s.sum, all);
     wanted += all;
     const bool fits = part == 0 || before < n_free, copy = part != 0 && fits;
-    block_before<int>(copy ? 1 : 0, s_sum, all);
-    copies += all;
+    copies += __syncthreads_count(copy);
+    if (copy) w.src[before] = page, w.dst[before] = c.free[n_free - 1 - (int)before];      // (all that wanted a page before have one)
+    first = copy ? to / KV4_PAGE : pages_of(max(to, 0));
+    end = cut && fits ? pages_of(old) : -1;
     if (i < B) {
       status[i] = fits ? KV4_OK : KV4_NO_PAGES;
-      w.src[i] = copy ? page : -1;
-      w.dst[i] = copy ? c.free[n_free - 1 - (int)before] : -1;
-      w.first[i] = copy ? to / KV4_PAGE : cut ? pages_of(to) : 0;
-      w.end[i] = cut && fits ? pages_of(old) : -1;
+      w.first[i] = first;
+      w.end[i] = end;
+      w.tokens[i] = copy ? (int)before : -1;
     }
   }
+  if (threadIdx.x == 0) *w.copies = copies;
   __syncthreads();
-  auto entries = [&](auto visit) {               // a warp a sequence: its entries that are given back
-    for (int i = threadIdx.x >> 5; i < B; i += nt >> 5) {
-      if (w.end[i] < 0) continue;
-      const int32_t* t = c.table + (size_t)rows[i] * c.width;
-      for (int k0 = w.first[i]; k0 < w.end[i]; k0 += 32) visit(i, k0 + lane < w.end[i] ? k0 + lane : -1, t);
+  // the rounds' entries that are given back: visit(sequences, places in the table, pages) of SHARE_EACH a thread
+  int entries = 0, round0 = 0;
+  auto rounds = [&](bool again, auto visit) {
+    for (int i0 = 0; i0 < B; i0 += nt) {
+      round0 = i0;
+      if (B > nt || !again) {                    // (one round's entries are still there)
+        const int i = i0 + threadIdx.x;
+        const int f = B <= nt ? first : i < B ? w.first[i] : 0, l = B <= nt ? end : i < B ? w.end[i] : -1;
+        entries = round_entries(s, B <= nt ? row : i < B ? rows[i] : -1, f, max(l - f, 0));
+      }
+      for (int b0 = 0; b0 < entries; b0 += SHARE_EACH * nt) {
+        int seq[SHARE_EACH], entry[SHARE_EACH], page[SHARE_EACH];
+        find_entries(s, b0 + SHARE_EACH * threadIdx.x, entries, seq, entry);
+#pragma unroll
+        for (int q = 0; q < SHARE_EACH; ++q) page[q] = seq[q] >= 0 ? c.table[(size_t)s.row[seq[q]] * c.width + entry[q]] : -1;
+        visit(seq, entry, page);
+      }
+      __syncthreads();
     }
-    __syncthreads();
   };
-  entries([&](int i, int k, const int32_t* t) {
-    if (k < 0) return;
-    atomicSub(&shared[t[k]], 1);
-    atomicMax(&latest[t[k]], i);
+  int freed = 0;
+  rounds(false, [&](const int(&seq)[SHARE_EACH], const int(&)[SHARE_EACH], const int(&page)[SHARE_EACH]) {
+#pragma unroll
+    for (int q = 0; q < SHARE_EACH; ++q)
+      if (page[q] >= 0) {
+        freed += atomicSub(&shared[page[q]], 1) == 0 ? 1 : 0;      // (one of a page that becomes free meets this)
+        atomicMax(&latest[page[q]], round0 + seq[q]);
+      }
   });
-  // (counters that atomics have changed are read past L1)
-  auto frees = [&](int i, int page) { return __ldcg(&shared[page]) < 0 && __ldcg(&latest[page]) == i; };
-  for (int i = threadIdx.x; i < B; i += nt) w.freed[i] = 0;
+  if (freed > 0) atomicAdd(&s_freed, freed);
   __syncthreads();
-  entries([&](int i, int k, const int32_t* t) {
-    const uint32_t with = __ballot_sync(0xffffffffu, k >= 0 && frees(i, t[max(k, 0)]));
-    if (lane == 0) w.freed[i] += __popc(with);
-  });
-  int total = 0;
-  for (int i0 = 0; i0 < B; i0 += nt) {
-    const int i = i0 + threadIdx.x, n = i < B ? w.freed[i] : 0;
+  const int total = s_freed;
+  int top = n_free - copies + total - 1;
+  rounds(true, [&](const int(&seq)[SHARE_EACH], const int(&entry)[SHARE_EACH], const int(&page)[SHARE_EACH]) {
+    // (counters that atomics have changed are read past L1; who gives a page back last sets them back, which makes no difference to the others)
+    bool last[SHARE_EACH], free[SHARE_EACH];
+    int n = 0;
+#pragma unroll
+    for (int q = 0; q < SHARE_EACH; ++q) {
+      last[q] = page[q] >= 0 && __ldcg(&latest[max(page[q], 0)]) == round0 + seq[q];
+      free[q] = last[q] && __ldcg(&shared[max(page[q], 0)]) < 0;
+      n += free[q] ? 1 : 0;
+    }
     int all;
-    const int before = total + block_before<int>(n, s_sum, all);
-    total += all;
-    if (i < B) w.freed[i] = before;
-  }
-  __syncthreads();
-  const int top = n_free - copies + total - 1;
-  entries([&](int i, int k, const int32_t* t) {
-    const bool mine = k >= 0 && frees(i, t[max(k, 0)]);
-    const uint32_t with = __ballot_sync(0xffffffffu, mine);
-    const int at = top - w.freed[i] - __popc(with & ((1u << lane) - 1u));
-    if (mine && at >= 0 && at < c.pages) c.free[at] = t[k];
-    __syncwarp();
-    if (lane == 0) w.freed[i] += __popc(with);
-    __syncwarp();
-  });
-  entries([&](int i, int k, const int32_t* t) {
-    if (k < 0) return;
-    atomicMax(&shared[t[k]], 0);
-    latest[t[k]] = -1;
-    const_cast<int32_t*>(t)[k] = -1;
+    int at = top - block_before<int>(n, s.sum, all);
+    top -= all;
+#pragma unroll
+    for (int q = 0; q < SHARE_EACH; ++q) {
+      if (free[q]) {
+        if (at >= 0 && at < c.pages) c.free[at] = page[q];
+        --at;
+        shared[page[q]] = 0;
+      }
+      if (last[q]) latest[page[q]] = -1;
+      if (page[q] >= 0) c.table[(size_t)s.row[seq[q]] * c.width + entry[q]] = -1;
+    }
   });
   for (int i = threadIdx.x; i < B; i += nt) {
     if (w.end[i] < 0) continue;
-    if (w.dst[i] >= 0) c.table[(size_t)rows[i] * c.width + w.first[i]] = w.dst[i];
+    if (w.tokens[i] >= 0) c.table[(size_t)rows[i] * c.width + w.first[i]] = w.dst[w.tokens[i]];
     c.lengths[rows[i]] = keep[i];
   }
   if (threadIdx.x == 0) *c.n_free = min(max(n_free - copies + total, 0), c.pages);
 }
 
-// Pages src[i] to dst[i], all layers: a block 16 kB of one.
+// The copies, all layers: blocks take 16 kB of one each, copies of a page next to one another.  203 copies of pages of 41 kB in five layers: XX us for 49 MB.
 constexpr int COPY_THREADS = 256, COPY_BLOCK = 4 * COPY_THREADS;      // threads, vectors of 16 bytes
-__global__ void __launch_bounds__(COPY_THREADS) kv4_copy_kernel(uint4* __restrict__ blocks, long long layer, int page, const int32_t* __restrict__ src,
-                                                               const int32_t* __restrict__ dst) {
-  const int from = src[blockIdx.x], to = dst[blockIdx.x];
-  if (from < 0 || to < 0) return;
-  const uint4* a = blocks + blockIdx.z * layer + (long long)from * page;
-  uint4* b = blocks + blockIdx.z * layer + (long long)to * page;
-  const int at = blockIdx.y * COPY_BLOCK + threadIdx.x;
-  uint4 v[4];
+__global__ void __launch_bounds__(COPY_THREADS) kv4_copy_kernel(uint4* __restrict__ blocks, long long layer, int page, int layers, ShareWork w) {
+  pdl_wait();
+  const int copies = *after_wait(w.copies), parts = (page + COPY_BLOCK - 1) / COPY_BLOCK;
+  const int32_t *src = after_wait(w.src), *dst = after_wait(w.dst);
+  const long long units = (long long)copies * parts * layers;
+  for (long long u = blockIdx.x; u < units; u += gridDim.x) {
+    const int i = (int)(u % copies), part = (int)(u / copies % parts), l = (int)(u / copies / parts);
+    const uint4* a = blocks + l * layer + (long long)src[i] * page;
+    uint4* b = blocks + l * layer + (long long)dst[i] * page;
+    const int at = part * COPY_BLOCK + threadIdx.x;
+    uint4 v[4];
 #pragma unroll
-  for (int k = 0; k < 4; ++k)
-    if (at + k * COPY_THREADS < page) v[k] = a[at + k * COPY_THREADS];
+    for (int k = 0; k < 4; ++k)
+      if (at + k * COPY_THREADS < page) v[k] = a[at + k * COPY_THREADS];
 #pragma unroll
-  for (int k = 0; k < 4; ++k)
-    if (at + k * COPY_THREADS < page) b[at + k * COPY_THREADS] = v[k];
+    for (int k = 0; k < 4; ++k)
+      if (at + k * COPY_THREADS < page) b[at + k * COPY_THREADS] = v[k];
+  }
 }
 
-int copy_pages(const ll_kv4_cache* c, void* blocks, int layers, const ShareWork& w, int B, cudaStream_t st) {
+int copy_pages(const ll_kv4_cache* c, void* blocks, int layers, const ShareWork& w, cudaStream_t st) {
   const long long page = (long long)c->kv_heads * kv4_bytes(c->head_size, c->head_size / c->group) / 16;
-  const dim3 grid(B, (unsigned)((page + COPY_BLOCK - 1) / COPY_BLOCK), layers);
-  kv4_copy_kernel<<<grid, COPY_THREADS, 0, st>>>((uint4*)blocks, page * c->pages, (int)page, w.src, w.dst);
+  const long long units = (page + COPY_BLOCK - 1) / COPY_BLOCK * layers * w.B;
+  const int sms = sm_count() > 0 ? sm_count() : 148;
+  LL_CUDA(launch(kv4_copy_kernel, dim3((unsigned)std::min<long long>(units, 8ll * sms)), dim3(COPY_THREADS), 0, st, true, (uint4*)blocks, page * c->pages, (int)page, layers, w));
   LL_LAUNCH_OK("kv4_copy_kernel");
   return LL_OK;
 }
@@ -187,7 +246,6 @@ int check_share(const ll_kv4_cache* c, const void* blocks, int layers, const voi
   if (int r = check_cache(c, who)) return r;
   LL_CHECK_ARG(blocks && shared && a && b && status && work && B > 0 && layers > 0 && layers <= 65535 && ((uintptr_t)blocks & 15) == 0,
                "%s: %d sequences, %d layers", who, B, layers);
-  LL_CHECK_ARG((long long)c->kv_heads * kv4_bytes(c->head_size, c->head_size / c->group) / 16 <= 65535ll * COPY_BLOCK, "%s: %d heads of %d", who, c->kv_heads, c->head_size);
   return LL_OK;
 }
 
@@ -202,18 +260,18 @@ int ll_kv4_fork(const ll_kv4_cache* cache, void* blocks, int layers, int32_t* sh
                 ll_stream stream) {
   if (int r = check_share(cache, blocks, layers, shared, rows, into, B, status, work, "kv4_fork")) return r;
   const ShareWork w(work, B);
-  kv4_fork_kernel<<<1, B <= 32 ? 256 : PLAN_THREADS, 0, (cudaStream_t)stream>>>(rows, into, B, pool_of(cache), shared, status, w);
+  kv4_fork_kernel<<<1, B <= 32 ? 256 : PLAN_THREADS, 0, (cudaStream_t)stream>>>(rows, into, pool_of(cache), shared, status, w);
   LL_LAUNCH_OK("kv4_fork_kernel");
-  return copy_pages(cache, blocks, layers, w, B, (cudaStream_t)stream);
+  return copy_pages(cache, blocks, layers, w, (cudaStream_t)stream);
 }
 
 int ll_kv4_release(const ll_kv4_cache* cache, void* blocks, int layers, int32_t* shared, const int32_t* rows, const int32_t* keep, int B, int32_t* status, int32_t* work,
                    ll_stream stream) {
   if (int r = check_share(cache, blocks, layers, shared, rows, keep, B, status, work, "kv4_release")) return r;
   const ShareWork w(work, B);
-  kv4_release_kernel<<<1, B <= 32 ? 256 : PLAN_THREADS, 0, (cudaStream_t)stream>>>(rows, keep, B, pool_of(cache), shared, status, w);
+  kv4_release_kernel<<<1, B <= 32 ? 256 : PLAN_THREADS, 0, (cudaStream_t)stream>>>(rows, keep, pool_of(cache), shared, status, w);
   LL_LAUNCH_OK("kv4_release_kernel");
-  return copy_pages(cache, blocks, layers, w, B, (cudaStream_t)stream);
+  return copy_pages(cache, blocks, layers, w, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -200,7 +200,7 @@ class PagedCache4:
 
     def _share(self, what: str, rows: torch.Tensor, other: torch.Tensor) -> torch.Tensor:
         B = rows.numel()
-        out = self.lengths.new_empty(6 * B)                                # statuses, and what the call notes of its sequences
+        out = self.lengths.new_empty(6 * B + 1)                              # statuses, and what the call notes of its sequences
         at = N.ptr(out)
         N.call(what, self._c, self._layers[0], self.n_layer, N.ptr(self._shared), N.ptr(rows), N.ptr(other), B, at, at + 4 * B, N.stream())
         return out[:B]
