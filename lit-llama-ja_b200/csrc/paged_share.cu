@@ -21,7 +21,7 @@ struct ShareWork {
 
 // The entries of a round of sequences (as many as the block has threads), one after the other: a thread has SHARE_EACH neighbours, whichever sequences these are of.
 // What bounds both kernels are dependent loads, atomics and sums of one block; with a warp a sequence, 203 sequences of 17 entries each, a fork took 11 us and a cut 27, now
-// XX and XX.
+// 10 and 17.
 constexpr int SHARE_EACH = 4;
 struct ShareRound {
   int sum[32], row[PLAN_THREADS], first[PLAN_THREADS], at[PLAN_THREADS + 1];
@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv4_release_kernel(const int32_t
   if (threadIdx.x == 0) *c.n_free = min(max(n_free - copies + total, 0), c.pages);
 }
 
-// The copies, all layers: blocks take 16 kB of one each, copies of a page next to one another.  203 copies of pages of 41 kB in five layers: XX us for 49 MB.
+// The copies, all layers: blocks take 16 kB of one each, copies of a page next to one another.  203 copies of pages of 41 kB in five layers: 9 us for 43 MB.
 constexpr int COPY_THREADS = 256, COPY_BLOCK = 4 * COPY_THREADS;      // threads, vectors of 16 bytes
 __global__ void __launch_bounds__(COPY_THREADS) kv4_copy_kernel(uint4* __restrict__ blocks, long long layer, int page, int layers, ShareWork w) {
   pdl_wait();
@@ -260,7 +260,7 @@ int ll_kv4_fork(const ll_kv4_cache* cache, void* blocks, int layers, int32_t* sh
                 ll_stream stream) {
   if (int r = check_share(cache, blocks, layers, shared, rows, into, B, status, work, "kv4_fork")) return r;
   const ShareWork w(work, B);
-  kv4_fork_kernel<<<1, B <= 32 ? 256 : PLAN_THREADS, 0, (cudaStream_t)stream>>>(rows, into, pool_of(cache), shared, status, w);
+  kv4_fork_kernel<<<1, B <= 64 ? 256 : PLAN_THREADS, 0, (cudaStream_t)stream>>>(rows, into, pool_of(cache), shared, status, w);
   LL_LAUNCH_OK("kv4_fork_kernel");
   return copy_pages(cache, blocks, layers, w, (cudaStream_t)stream);
 }
@@ -269,7 +269,7 @@ int ll_kv4_release(const ll_kv4_cache* cache, void* blocks, int layers, int32_t*
                    ll_stream stream) {
   if (int r = check_share(cache, blocks, layers, shared, rows, keep, B, status, work, "kv4_release")) return r;
   const ShareWork w(work, B);
-  kv4_release_kernel<<<1, B <= 32 ? 256 : PLAN_THREADS, 0, (cudaStream_t)stream>>>(rows, keep, pool_of(cache), shared, status, w);
+  kv4_release_kernel<<<1, B <= 64 ? 256 : PLAN_THREADS, 0, (cudaStream_t)stream>>>(rows, keep, pool_of(cache), shared, status, w);
   LL_LAUNCH_OK("kv4_release_kernel");
   return copy_pages(cache, blocks, layers, w, (cudaStream_t)stream);
 }

@@ -27,6 +27,27 @@ __device__ __forceinline__ void vec_values(const uint4& r, float (&x)[8]) {
     x[2 * j] = f.x, x[2 * j + 1] = f.y;
   }
 }
+// The largest of a vector, of pairs at once; a number that is none is passed over.
+template <typename T>
+__device__ __forceinline__ float vec_max(const uint4& r) {
+  if constexpr (std::is_same<T, float>::value) {
+    return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), fmaxf(__uint_as_float(r.z), __uint_as_float(r.w)));
+  } else if constexpr (std::is_same<T, __half>::value) {
+    auto h = [](const uint32_t& u) { return *reinterpret_cast<const __half2*>(&u); };
+    const float2 f = __half22float2(__hmax2(__hmax2(h(r.x), h(r.y)), __hmax2(h(r.z), h(r.w))));
+    return fmaxf(f.x, f.y);
+  } else {
+    auto h = [](const uint32_t& u) { return *reinterpret_cast<const __nv_bfloat162*>(&u); };
+    const float2 f = __bfloat1622float2(__hmax2(__hmax2(h(r.x), h(r.y)), __hmax2(h(r.z), h(r.w))));
+    return fmaxf(f.x, f.y);
+  }
+}
+// A vector of -inf.
+template <typename T>
+__device__ __forceinline__ uint4 none_vector() {
+  constexpr uint32_t NONE = std::is_same<T, float>::value ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+  return make_uint4(NONE, NONE, NONE, NONE);
+}
 // How many numbers the row begins behind a 16-byte boundary.
 template <typename T>
 __device__ __forceinline__ int row_offset(const T* row) { return (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T)); }
