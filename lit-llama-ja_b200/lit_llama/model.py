@@ -413,15 +413,16 @@ class LLaMA(nn.Module):
         return x
 
     # ------------------------------------------------------------------ requests of unequal lengths over the 4-bit cache
-    def paged_cache(self, *, pages: int, requests: int, max_length: Optional[int] = None, group: Optional[int] = None) -> PagedCache4:
+    def paged_cache(self, *, pages: int, requests: int, max_length: Optional[int] = None, group: Optional[int] = None,
+                    share: bool = False) -> PagedCache4:
         """A 4-bit cache of this model's layers and heads: ``pages`` of 64 slots for up to ``requests`` requests of up to ``max_length`` tokens (the block
-        size unless given)."""
+        size unless given), which may be forked where ``share`` is set."""
         w, hs = self.transformer.wte.weight, self.config.head_size
         max_length = self.config.block_size if max_length is None else max_length
         if max_length > self.config.block_size:
             raise ValueError(f"requests of up to {max_length} tokens, block size is only {self.config.block_size}")
         return PagedCache4(len(self.transformer.h), self.transformer.h[0].attn.n_head, hs, pages=pages, requests=requests, max_length=max_length,
-                           group=min(64, hs) if group is None else group, dtype=w.dtype, device=w.device)
+                           group=min(64, hs) if group is None else group, dtype=w.dtype, device=w.device, share=share)
 
     @torch.no_grad()
     def forward_paged(self, tokens: torch.Tensor, cache: PagedCache4, plan: CachePlan, all_rows: bool = False) -> torch.Tensor:
