@@ -7,8 +7,12 @@
 //   top-p: the steps' weights, in the same pass that adds up all of them: within a step they differ by 3 %, so that 13 bits of each one's part of the step's largest
 //   are enough to leave one step or two that the border can be in.
 // The few numbers of those steps are then compared with one another, on top of the exact sum of what lies above; where they are many (rows of few values), the border is
-// found by counts or exact weights of their keys, 1024 ranges at a time.  (Exact weights in all steps, two dependent additions of 32 bits in shared memory each: 301
-// rows of 100 003 numbers 738 us.)
+// found by counts or exact weights of their keys, 1024 ranges at a time.
+//
+// What bounds it: 301 rows of 100 003 (fp32) under top-p and min-p 343 us, 128 without a border (copying them takes 18): the barriers of a cluster, 1 to 1.5 us each, between phases of 3
+// to 6 us of the exponentials' instructions (eleven of 64 bits each), two blocks an SM.  One row of 32 000 (bf16): 5.3 us, 8.0 under top-k, 14 under top-p.  On the way (us, 301 rows, top-p):
+// a block a row and bisection 3334; exact weights in all steps, two dependent additions of 32 bits in shared memory each, 738; steps' weights in parts, and a list of the border's
+// numbers appended by remote atomics 639, by one's own 435; the exponential by a table 343.
 //
 // A cluster of blocks has a row in its shared memory, read once.
 #include <cooperative_groups.h>
@@ -131,6 +135,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == SR_WIDE ? 2 : 8) sample_ro
   float temperature = a.temperature ? a.temperature[r] : a.temperature_all, top_p = a.top_p ? a.top_p[r] : a.top_p_all, min_p = a.min_p ? a.min_p[r] : a.min_p_all;
   int top_k = a.top_k ? a.top_k[r] : a.top_k_all;
   bool bad = !(u >= 0.f && u <= 1.f) || !(temperature >= 0.f && temperature < INFINITY) || isnan(top_p) || isnan(min_p);
+  top_p = fmaxf(top_p, 0.f);
   const bool first = temperature < SR_LEAST;     // the first one of the largest
   if (first) temperature = 1.f, top_k = 1, top_p = 1.f, min_p = 0.f;
 
@@ -240,7 +245,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == SR_WIDE ? 2 : 8) sample_ro
 #pragma unroll
           for (int b = 0; b < BINS; ++b) n[b] += (u64)h[c][b] << (32 * part);
     }
-    if (t == 0) sh.found = -1, sh.last = SR_BINS - 1, sh.range[0] = 0;
+    if (t == 0) sh.found = -1, sh.last = SR_BINS - 1, sh.range[0] = sh.range[1] = 0;
     // (what the turn before has left has been read by every block: behind a barrier of the cluster that comes after)
     for (int b = t; b < 2 * SR_BINS; b += THREADS) (&sh.hist[turn ^ 1][0][0])[b] = 0;
     turn ^= 1;
@@ -394,6 +399,139 @@ __global__ void __launch_bounds__(THREADS, THREADS == SR_WIDE ? 2 : 8) sample_ro
     return lo;
   };
 
+  // ---- Where few numbers can be kept, the first block finishes alone: those up to `last` steps below m, in the order of the row, HERE at most.  `want`: the weight that top-p
+  // has to reach, or less than 0: `top_p` of the weight that top-k leaves.  It compares all of them with one another, and no other barrier of the cluster follows.
+  // us with it / without, top-k 50 and top-k 200 with top-p 0.9: 301 rows of 100 003 (fp32) 165 / 191 and 188 / 318, 16 rows 17.1 / 18.7 and 23 / 32; bf16, one row of
+  // 32 000 (eight blocks) 9.0 / 8.0 and 13.0 / 12.4, 128 rows (two blocks) 17.1 / 14.8 and 23 / 27, 100 of 5000 (one block) 11.4 / 12.3 and 17 / 24: 16-bit numbers,
+  // whose borders are found in one go, do without it where a row has several blocks, or two and no top-p.
+  constexpr int HERE = THREADS == SR_WIDE ? SR_LIST : SR_LIST / 2, EACH = HERE / THREADS;
+  const bool alone = sizeof(T) == 4 || C == 1 || (C == 2 && top_p < 1.f);
+  auto finish_here = [&](int last, double want) {
+    float* const value_here = reinterpret_cast<float*>(&sh.hist[turn][0][0]);      // (zeros that nobody reads)
+    int* const place_here = reinterpret_cast<int*>(value_here + HERE);
+    auto in = [&](float v) { return v >= lowest && step_of(below(v)) <= last; };
+    int n = 0;
+    each(lowest, [&](const float (&x)[N], int) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) n += in(x[e]) ? 1 : 0;
+    });
+    n = __reduce_add_sync(0xffffffffu, n);
+    if (lane == 0) sh.warp_key[warp] = n;
+    __syncthreads();
+    int at = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      at += w < warp ? (int)sh.warp_key[w] : 0;
+      all += (int)sh.warp_key[w];
+    }
+    each(lowest, [&](const float (&x)[N], int j) {
+      int mine = 0;
+#pragma unroll
+      for (int e = 0; e < N; ++e) mine += in(x[e]) ? 1 : 0;
+      if (!__any_sync(0xffffffffu, mine > 0)) return;
+      int incl = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+      }
+      int to = at + incl - mine;
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (in(x[e])) {
+          if (to < HERE) value_here[to] = x[e], place_here[to] = i0 + j * 32 * N + e;
+          ++to;
+        }
+      at += __shfl_sync(0xffffffffu, incl, 31);
+    });
+    if (t == 0) sh.listed[0] = (uint32_t)all;
+    cluster.sync();
+    float v[EACH];
+    int place[EACH];
+    n = 0;
+    if (rank == 0) {
+      if (t < C) sh.key[t] = remote(there(&sh.listed[0], t));
+      __syncthreads();
+#pragma unroll
+      for (int q = 0; q < EACH; ++q) {
+        const int i = t * EACH + q;
+        int first_of = 0;
+        v[q] = -INFINITY, place[q] = -1;
+        for (int c = 0; c < C; ++c) {
+          const int of_c = (int)sh.key[c];
+          if (i >= first_of && i < first_of + of_c) {
+            v[q] = __uint_as_float(remote(there(value_here + i - first_of, c)));
+            place[q] = (int)remote(there(place_here + i - first_of, c));
+          }
+          first_of += of_c;
+        }
+        n = min(first_of, HERE);
+        sh.list_key[i] = __float_as_uint(v[q]);
+      }
+    }
+    cluster.sync();                              // (the other blocks may go)
+    if (rank > 0) return;
+    n = (n + 3) & ~3;                            // (-inf behind the last one)
+    const float4* values = reinterpret_cast<const float4*>(sh.list_key);
+    u64 w[EACH], sum = 0;
+#pragma unroll
+    for (int q = 0; q < EACH; ++q) {
+      bool keep = place[q] >= 0;
+      if (want < 0.0 && __any_sync(0xffffffffu, keep)) {                          // as large as the k-th largest: fewer than k are larger
+        int larger = 0;
+#pragma unroll 4
+        for (int j = 0; j < n / 4; ++j) {
+          const float4 o = values[j];
+          larger += (o.x > v[q] ? 1 : 0) + (o.y > v[q] ? 1 : 0) + (o.z > v[q] ? 1 : 0) + (o.w > v[q] ? 1 : 0);
+        }
+        keep = keep && larger < top_k;
+      }
+      w[q] = keep ? weight(v[q]) : 0;
+      sh.list_weight[t * EACH + q] = w[q];
+      sum += w[q];
+    }
+    auto block_before = [&](u64 x, u64& total) {
+      __syncthreads();                           // (the sums before have been read)
+      const u64 before = threads_before<THREADS>(x, sh.scan);
+      total = 0;
+#pragma unroll
+      for (int o = 0; o < WARPS; ++o) total += sh.scan[o];
+      return before;
+    };
+    u64 total;
+    block_before(sum, total);
+    if (top_p < 1.f) {                           // what is larger does not reach it
+      if (want < 0.0) want = (double)top_p * (double)total;
+      const ulonglong2* weights = reinterpret_cast<const ulonglong2*>(sh.list_weight);
+#pragma unroll
+      for (int q = 0; q < EACH; ++q) {
+        if (!__any_sync(0xffffffffu, w[q] > 0)) continue;
+        u64 larger = 0;
+#pragma unroll 2
+        for (int j = 0; j < n / 4; ++j) {
+          const float4 o = values[j];
+          const ulonglong2 a = weights[2 * j], b = weights[2 * j + 1];
+          larger += (o.x > v[q] ? a.x : 0) + (o.y > v[q] ? a.y : 0) + (o.z > v[q] ? b.x : 0) + (o.w > v[q] ? b.y : 0);
+        }
+        if (larger > 0 && (double)larger >= want) w[q] = 0;
+      }
+    }
+    const u64 least = min_p > 0.f ? (u64)ceil((double)fminf(min_p, 1.f) * SR_ONE) : 0;
+    sum = 0;
+#pragma unroll
+    for (int q = 0; q < EACH; ++q) {
+      if (w[q] < least) w[q] = 0;
+      sum += w[q];
+    }
+    u64 running = block_before(sum, total);
+    const u64 target = first ? 0 : min((u64)floor((double)u * (double)total), total - 1);
+#pragma unroll
+    for (int q = 0; q < EACH; ++q) {
+      if (running <= target && target < running + w[q]) a.tokens[r] = place[q];
+      running += w[q];
+    }
+  };
+
   if (top_k >= 1 && top_k < V) {
     uint32_t* hist = sh.hist[turn][0];
     each(cut, [&](const float (&x)[N], int) {
@@ -418,6 +556,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == SR_WIDE ? 2 : 8) sample_ro
     if (found >= 0) {                            // (else all that have a weight are kept)
       const u64 base = sh.found_base;
       const bool few = sh.range[0] <= SR_LIST;
+      if (alone && base + sh.range[0] <= HERE) return finish_here(found, -1.0);
       __syncthreads();
       keys_of(found, found);
       const uint32_t lo = sh.range[0], hi = sh.range[1];
@@ -450,7 +589,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == SR_WIDE ? 2 : 8) sample_ro
     counted(false, n);
 #pragma unroll
     for (int b = 0; b < BINS; ++b) {
-      numbers[b] = (uint32_t)n[b] / 8060u + 1u;              // at most
+      numbers[b] = ((uint32_t)n[b] + 8059u) / 8060u;         // at most
       n[b] = (u64)((double)n[b] * ((double)weight_of(-(BINS * t + b) * (double)(SR_REACH / SR_BINS), 369.32994026157255, sh.exps) * (1.0 / 8192)));
     }
     u64 at = bins_before(n);
@@ -466,10 +605,13 @@ __global__ void __launch_bounds__(THREADS, THREADS == SR_WIDE ? 2 : 8) sample_ro
     __syncthreads();
     const int from = max(sh.found, 0), to = sh.last;
 #pragma unroll
-    for (int b = 0; b < BINS; ++b)
+    for (int b = 0; b < BINS; ++b) {
       if (BINS * t + b >= from && BINS * t + b <= to) atomicAdd(&sh.range[0], numbers[b]);
+      if (BINS * t + b <= to && numbers[b] > 0) atomicAdd(&sh.range[1], numbers[b]);
+    }
     __syncthreads();
     const bool few = sh.range[0] <= SR_LIST;
+    if (alone && sh.range[1] <= HERE) return finish_here(to, want);
     __syncthreads();
     keys_of(from, to);
     const uint32_t lo = sh.range[0], hi = sh.range[1];
