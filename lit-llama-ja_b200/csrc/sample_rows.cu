@@ -73,10 +73,10 @@ struct SampleArgs {
 
 template <int THREADS>
 struct SampleShared {
-  uint32_t hist[2][2][SR_BINS];                  // two in turn: low and high halves of sums; or a block's list of numbers that a border is among
+  alignas(16) uint32_t hist[2][2][SR_BINS];      // two in turn: low and high halves of sums; or a block's list of numbers that a border is among
   double exps[SR_TABLE];                         // 2^(j / 256)
-  u64 list_weight[SR_LIST];                      // all blocks' lists
-  uint32_t list_key[SR_LIST];
+  alignas(16) u64 list_weight[SR_LIST];          // all blocks' lists
+  alignas(16) uint32_t list_key[SR_LIST];
   u64 scan[THREADS / 32], found_base, sums[2][SR_MOST];
   uint32_t key[SR_MOST], warp_key[THREADS / 32], range[2], listed[2];
   int found, last;

@@ -47,7 +47,7 @@ def _setting(name: str, x: Setting, logits: torch.Tensor, off, low, high, dtype=
         return _vector(name, x, dtype, logits), off
     if x is None:
         return None, off
-    if not low <= x <= high:                                          # (no numbers too)
+    if not low <= x <= high or (dtype is torch.int32 and x != int(x)):      # (no numbers too)
         raise ValueError(f"{name} {x}: {low} to {high}")
     return None, x
 
@@ -79,7 +79,7 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature: Setting = 1.0,
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: Setting = 1.0) -> torch.Tensor:
     """Logarithms of the probabilities that softmax(``logits [rows, vocabulary]`` / temperature) gives to ``tokens [rows]`` (int64): float32 ``[rows]``.  No number
-    for a token that is not of the vocabulary, or a row of which there is no softmax."""
+    for a token that is not of the vocabulary, or a row of which there is no softmax.  Sums are of 32 bits, by vectors of 16 bytes: a row's last bits go with where it begins."""
     logits = _rows(logits)
     t, t_all = _setting("temperature", temperature, logits, 1.0, 1.0e-30, 3.0e38)
     tokens = _vector("tokens", tokens, torch.int64, logits)

@@ -108,14 +108,25 @@ def _filled(H, G, D, group, dtype, held, copies, more, seed, order=None):
     return cache, rows, [more[i][1] for i in order], q, keys
 
 
-def _near(y, q, keys, counts, dtype, scale):
+def _held_parts(x, group):
+    """|code * scale| + |lowest value|: what a value that the cache holds is made of."""
+    g = x.float().unflatten(-1, (-1, group))
+    lo = g.min(-1, keepdim=True).values.double()
+    return ((held_as(x, group).unflatten(-1, (-1, group)) - lo).abs() + lo.abs()).flatten(-2)
+
+
+def _near(y, q, keys, counts, dtype, scale, parts=None):
     """The tolerance: half a step of the result, weights of 11 bits and values and keys of a bf16 cache's prompts rounded to 11 bits (each 2^-11 of
-    sum w |v| at most, with the scores' 2^-11 of sum |q| |k| scaled), once more for sums."""
+    sum w |v| at most, with the scores' 2^-11 of sum |q| |k| scaled), once more for sums.  ``parts``: the sums run over w s c and w lo apart, and weights
+    of 11 bits meet the first alone: where a number far below its group's others makes these c s + lo of two large terms, an error of a weight is
+    multiplied by |c s|, not by |v|, so that sum w (|c s| + |lo|) takes the place of sum w |v|."""
     at = 0
-    for (k, v), n in zip(keys, counts):
+    for i, ((k, v), n) in enumerate(zip(keys, counts)):
         if n == 0:
             continue
         want, size, mag = attention(q[at:at + n], k, v, k.shape[0] - n, scale)
+        if parts is not None:
+            size = attention(q[at:at + n], k, parts[i], k.shape[0] - n, scale)[1]
         tol = want.abs() * torch.finfo(dtype).eps / 2 + size * (3 * 2.0**-11 + mag * 2.0**-11 * 2)
         got = y[at:at + n].cpu().double()
         assert bool(((got - want).abs() <= tol).all()), float(((got - want).abs() / tol).max())
@@ -144,6 +155,47 @@ def test_attention_of_copies(held, copies, more, H, G, D, group, dtype):
     y = cache.attend(1, plan, q.to(DEV))
     _near(y, q, keys, counts, dtype, D ** -0.5)
     assert torch.equal(y, cache.attend(1, plan, q.to(DEV)))          # the same bits
+
+
+@pytest.mark.parametrize("H, G, D, group, dtype, held, copies", [(2, 1, 64, 64, BF, 20000, 3), (1, 1, 64, 64, BF, 20000, 40), (4, 1, 128, 32, HF, 9000, 20), (8, 2, 128, 128, BF, 5003, 2)],
+                         ids=str)
+def test_long_shared_prompts(H, G, D, group, dtype, held, copies):
+    """Walks of shared pages in more parts than a warp joins, of few columns and of many."""
+    more = [(1 + i % 5, 1) for i in range(copies)]
+    cache, rows, counts, q, keys = _filled(H, G, D, group, dtype, [held], [copies], more, seed=copies)
+    plan = cache.plan(rows, counts, sum(counts), max_count=1)
+    y = cache.attend(1, plan, q.to(DEV))
+    _near(y, q, keys, counts, dtype, D ** -0.5)
+    assert torch.equal(y, cache.attend(1, plan, q.to(DEV)))
+
+
+@pytest.mark.parametrize("H, G, new, dtype", [(2, 2, 1, BF), (8, 2, 1, HF), (2, 2, 3, BF)], ids=str)
+def test_shared_pages_of_large_values(H, G, new, dtype):
+    """Shared pages with numbers that fp16 operands do not hold: their tiles are left to the walk of few columns.  And values that are no numbers in a copy's own
+    page, which are its own."""
+    D, held, copies = 64, 700, 40
+    gen = torch.Generator().manual_seed(1)
+    make = lambda n: torch.randn(n, G, D, generator=gen)  # noqa: E731
+    k, v = make(held), make(held)
+    v[::50, :, 3] = 3e4
+    v[130, :, 40] = -6e4 if dtype == HF else -1e6
+    k, v = k.to(dtype), v.to(dtype)
+    cache = _cache(1, H, D, n_kv_head=G, group=64, pages=11 + 2 * copies, requests=1 + copies, max_length=held + 60, dtype=dtype)
+    cache.append(0, cache.plan([0], [held], held), None, k.to(DEV), v.to(DEV))
+    into = list(range(1, 1 + copies))
+    assert cache.fork([0] * copies, into).tolist() == [0] * copies
+    pk, pv = make(copies * new).to(dtype), make(copies * new).to(dtype)
+    pv[5 * new] = float("nan")
+    plan = cache.plan(into, [new] * copies, copies * new, max_count=new)
+    cache.append(0, plan, None, pk.to(DEV), pv.to(DEV))
+    q = torch.randn(copies * new, H, D, generator=gen).to(dtype)
+    y = cache.attend(0, plan, q.to(DEV))
+    assert bool(y[5 * new:6 * new].isnan().all()) and bool(torch.isfinite(torch.cat([y[:5 * new], y[6 * new:]])).all())
+    keys = [tuple(torch.cat([held_as(a, 64), held_as(b[i * new:(i + 1) * new], 64)]) for a, b in ((k, pk), (v, pv))) for i in range(copies)]
+    there = [i for i in range(copies) if i != 5]
+    at = torch.cat([torch.arange(i * new, (i + 1) * new) for i in there])
+    parts = [torch.cat([_held_parts(v, 64), _held_parts(pv[i * new:(i + 1) * new], 64)]) for i in there]
+    _near(y.cpu()[at], q[at], [keys[i] for i in there], [new] * len(there), dtype, D ** -0.5, parts)
 
 
 def test_copies_in_any_order():

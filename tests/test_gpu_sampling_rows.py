@@ -130,11 +130,41 @@ def test_rows_anywhere():
     assert empty.shape == (0,) and empty.dtype is torch.int64 and token_logprobs(wide[:0], empty).shape == (0,)
 
 
+def test_rows_past_32_bits():
+    """The last rows of a matrix of more than 2^32 bytes and 2^31 numbers."""
+    from lit_llama.sampling import sample, token_logprobs
+
+    R, V = 70000, 32003
+    x = torch.zeros(R, V, dtype=BF, device=DEV)
+    tail = _logits(5, V, BF, 11)
+    x[-5:] = tail.to(DEV)
+    u = torch.full((R,), 0.3, device=DEV)
+    got = sample(x, u, top_p=0.9)
+    assert got[-5:].tolist() == [drawn(r.float().numpy(), float(np.float32(0.3)), top_p=float(np.float32(0.9))) for r in tail]
+    assert got[:3].tolist() == [math.floor(float(np.float32(0.3)) * V)] * 3      # (equal logits are all kept)
+    tokens = torch.full((R,), 7, device=DEV)
+    want = torch.log_softmax(tail.double(), -1)[:, 7]
+    assert bool(((token_logprobs(x, tokens)[-5:].cpu().double() - want).abs() <= _score_bound(tail, 1.0, want)).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, FP], ids=str)
+def test_borders_among_many_alike(dtype):
+    """Borders of top-k and top-p among more equal, or nearly equal, logits than a block compares with one another; over and under what one block finishes alone."""
+    V = 60000
+    gen = torch.Generator().manual_seed(8)
+    eps = torch.finfo(dtype).eps
+    some = torch.randint(0, 3, (V,), generator=gen).float()
+    rows = [4.0 + some * 4 * eps, 4.0 + torch.rand(V, generator=gen) * 0.01, torch.where(torch.rand(V, generator=gen) < 0.02, 6.0 + some * 4 * eps, 1.0), torch.rand(V, generator=gen) * 1e-3]
+    x = torch.stack(rows).to(dtype)
+    for s in (dict(top_k=700), dict(top_k=30000), dict(top_p=0.3), dict(top_p=0.97, temperature=0.5), dict(top_k=900, top_p=0.5), dict(top_k=300, top_p=0.5, min_p=0.9)):
+        _same(x, torch.rand(len(rows), generator=gen), **s)
+
+
 def test_refusals():
     from lit_llama.sampling import sample, token_logprobs
 
     x, u = torch.zeros(3, 9, device=DEV), torch.zeros(3, device=DEV)
-    for kind in (dict(temperature=-1.0), dict(temperature=math.nan), dict(temperature=math.inf), dict(top_k=0), dict(top_k=-1), dict(top_p=-0.1), dict(top_p=1.1), dict(top_p=math.nan),
+    for kind in (dict(temperature=-1.0), dict(temperature=math.nan), dict(temperature=math.inf), dict(top_k=0), dict(top_k=-1), dict(top_k=2.5), dict(top_p=-0.1), dict(top_p=1.1), dict(top_p=math.nan),
                  dict(min_p=-0.1), dict(min_p=1.1)):
         with pytest.raises(ValueError):
             sample(x, u, **kind)
