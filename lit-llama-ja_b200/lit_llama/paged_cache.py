@@ -122,6 +122,7 @@ class PagedCache4:
         if self.share:
             self._shared = torch.zeros((2, pages), **i32)
             self._shared[1].fill_(-1)
+            self._shared_at = N.ptr(self._shared)
         self._none = torch.empty(0, dtype=dtype, device=self.device)      # (a result's type and device)
         self._code = N.dtype_code(dtype)
         self._struct = N.Kv4Cache(*(N.ptr(t) for t in (self.table, self.lengths, self.free, self.n_free, self._stamp)), requests, self.width, pages, max_length,
@@ -201,8 +202,8 @@ class PagedCache4:
     def _share(self, what: str, rows: torch.Tensor, other: torch.Tensor) -> torch.Tensor:
         B = rows.numel()
         out = self.lengths.new_empty(6 * B + 1)                              # statuses, and what the call notes of its sequences
-        at = N.ptr(out)
-        N.call(what, self._c, self._layers[0], self.n_layer, N.ptr(self._shared), N.ptr(rows), N.ptr(other), B, at, at + 4 * B, N.stream())
+        at = out.data_ptr()
+        N.call(what, self._c, self._layers[0], self.n_layer, self._shared_at, rows.data_ptr(), other.data_ptr(), B, at, at + 4 * B, N.stream())
         return out[:B]
 
     def reset(self) -> None:
