@@ -78,7 +78,7 @@ struct SampleShared {
   alignas(16) u64 list_weight[SR_LIST];          // all blocks' lists
   alignas(16) uint32_t list_key[SR_LIST];
   u64 scan[THREADS / 32], found_base, sums[2][SR_MOST];
-  uint32_t key[SR_MOST], warp_key[THREADS / 32], range[2], listed[2];
+  uint32_t key[SR_MOST], warp_key[THREADS / 32], range[2], listed[2], least_key;
   int found, last;
 };
 static_assert(SR_LIST * 12 <= 2 * SR_BINS * 4, "a list in the place of counts");
@@ -621,19 +621,23 @@ __global__ void __launch_bounds__(THREADS, THREADS == SR_WIDE ? 2 : 8) sample_ro
   }
 
   // ---- kept weights
-  if (min_p > 0.f) {                             // the smallest number that weighs as much, by 32 at a time (every warp)
-    const u64 least = (u64)ceil((double)fminf(min_p, 1.f) * SR_ONE);
-    uint32_t from = order_key<T>(lowest) - 1u, to = order_key<T>(m);     // `from` weighs less or is not kept, `to` is
-    while (to - from > 1u) {
-      const uint32_t step = (to - from - 1u) / 33u + 1u;
-      const u64 probe = min((u64)from + (u64)(lane + 1) * step, (u64)to);
-      const uint32_t in = __ballot_sync(0xffffffffu, weight(fmaxf(key_value<T>((uint32_t)probe), cut)) >= least);
-      const int at = in != 0u ? __ffs(in) - 1 : 32;
-      const u64 above = (u64)from + (u64)at * step;
-      if (in != 0u) to = (uint32_t)min(above + step, (u64)to);
-      from = (uint32_t)above;
+  if (min_p > 0.f) {                             // the smallest number that weighs as much, by 32 at a time
+    if (warp == 0) {
+      const u64 least = (u64)ceil((double)fminf(min_p, 1.f) * SR_ONE);
+      uint32_t from = order_key<T>(lowest) - 1u, to = order_key<T>(m);     // `from` weighs less or is not kept, `to` is
+      while (to - from > 1u) {
+        const uint32_t step = (to - from - 1u) / 33u + 1u;
+        const u64 probe = min((u64)from + (u64)(lane + 1) * step, (u64)to);
+        const uint32_t in = __ballot_sync(0xffffffffu, weight(fmaxf(key_value<T>((uint32_t)probe), cut)) >= least);
+        const int at = in != 0u ? __ffs(in) - 1 : 32;
+        const u64 above = (u64)from + (u64)at * step;
+        if (in != 0u) to = (uint32_t)min(above + step, (u64)to);
+        from = (uint32_t)above;
+      }
+      if (lane == 0) sh.least_key = to;
     }
-    lowest = fmaxf(lowest, key_value<T>(to));
+    __syncthreads();
+    lowest = fmaxf(lowest, key_value<T>(sh.least_key));
   }
   auto kept = [&](float v) -> u64 {
     const u64 w = weight(fmaxf(v, cut));
@@ -674,7 +678,8 @@ __global__ void __launch_bounds__(THREADS, THREADS == SR_WIDE ? 2 : 8) sample_ro
   });
 }
 
-// Blocks a row: enough that a thread has at most 32 numbers, and more of them while there are few rows.
+// Blocks a row: enough that a thread has at most 32 numbers, and more while there are fewer blocks than SMs.  us without a border and under top-p, by one / two / four / eight
+// blocks a row of 32 000 (bf16): one row 18.9, 55 / 11.6, 31 / 7.8, 22 / 6.1, 21; 64 rows 19.4, 56 / 12.1, 38 / 11.1, 39 / 15.0, 62; 128 rows 19.6, 56 / 16.4, 53 / 19.7, 64 / 24.6, 104.
 template <typename T, int THREADS>
 int launch_sample(SampleArgs a, int R, int C, cudaStream_t st) {
   constexpr int N = row_vec<T>::n;
