@@ -169,7 +169,7 @@ def test_long_shared_prompts(H, G, D, group, dtype, held, copies):
     assert torch.equal(y, cache.attend(1, plan, q.to(DEV)))
 
 
-@pytest.mark.parametrize("H, G, new, dtype", [(2, 2, 1, BF), (8, 2, 1, HF), (2, 2, 3, BF)], ids=str)
+@pytest.mark.parametrize("H, G, new, dtype", [(2, 2, 1, BF), (8, 2, 1, HF), (2, 2, 3, BF), (8, 2, 2, BF)], ids=str)
 def test_shared_pages_of_large_values(H, G, new, dtype):
     """Shared pages with numbers that fp16 operands do not hold: their tiles are left to the walk of few columns.  And values that are no numbers in a copy's own
     page, which are its own."""
