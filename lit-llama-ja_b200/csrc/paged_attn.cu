@@ -650,33 +650,31 @@ __global__ void __launch_bounds__(KJ * 32) kv4_join_shared_kernel(const Kv4Attn 
   const float2 *few_ml = reinterpret_cast<const float2*>(few_part + (size_t)few.kept * G * COLS * D),
                *many_ml = reinterpret_cast<const float2*>(many_part + (size_t)many.kept * G * KV4_MANY * D);
   const int units = work[1] * G * few.cols;
+  struct Unit {
+    int4 a, b;
+    int head, c;
+  };
+  auto unit_of = [&](int u) {
+    const int j = u / (G * few.cols);
+    return Unit{rec[2 * j], rec[2 * j + 1], u / few.cols % G, u % few.cols};
+  };
+  // where part k's sums are, the group's first, as the keys come
+  auto part_at = [&](const Unit& n, int k, bool& in_many) {
+    const int gc = n.b.z + n.c;
+    in_many = k < n.b.x && n.b.w != 0;
+    if (k >= n.b.x) return ((size_t)(n.a.w + n.c / COLS * n.a.z + k - n.b.x) * G + n.head) * COLS + n.c % COLS;
+    if (in_many) return ((size_t)(n.b.y + gc / KV4_MANY * n.b.x + k) * G + n.head) * KV4_MANY + gc % KV4_MANY;
+    return ((size_t)(n.b.y + gc / COLS * n.b.x + k) * G + n.head) * COLS + gc % COLS;
+  };
+  auto row_of = [&](const Unit& n, int c) { return (size_t)(n.a.x + column_token(c, R)) * few.H + n.head * R + column_head(c, R); };
   for (int u0 = blockIdx.x * KJ; u0 < units; u0 += gridDim.x * KJ) {
-    struct Unit {
-      int4 a, b;
-      int head, c;
-    };
-    auto unit_of = [&](int u) {
-      const int j = u / (G * few.cols);
-      return Unit{rec[2 * j], rec[2 * j + 1], u / few.cols % G, u % few.cols};
-    };
-    // where part k's sums are, the group's first, as the keys come
-    auto part_at = [&](const Unit& n, int k, bool& in_many) {
-      const int gc = n.b.z + n.c;
-      in_many = k < n.b.x && n.b.w != 0;
-      if (k >= n.b.x) return ((size_t)(n.a.w + n.c / COLS * n.a.z + k - n.b.x) * G + n.head) * COLS + n.c % COLS;
-      if (in_many) return ((size_t)(n.b.y + gc / KV4_MANY * n.b.x + k) * G + n.head) * KV4_MANY + gc % KV4_MANY;
-      return ((size_t)(n.b.y + gc / COLS * n.b.x + k) * G + n.head) * COLS + gc % COLS;
-    };
-    auto row_of = [&](const Unit& n, int c) { return (size_t)(n.a.x + column_token(c, R)) * few.H + n.head * R + column_head(c, R); };
-    bool longer = false;
     if (u0 + warp < units) {
       const Unit n = unit_of(u0 + warp);
       const int parts = n.a.z + n.b.x;
-      longer = parts > 32;
       if (n.b.w == 2) {                          // a refused sequence's tokens are no numbers
         for (int x = n.c; x < n.a.y * R; x += few.cols)
           for (int d = lane; d < D; d += 32) dt<T>::st(y, row_of(n, x) * D + d, NAN);
-      } else if (!longer && n.c < n.a.y * R) {
+      } else if (parts <= 32 && n.c < n.a.y * R) {
         float2 u = make_float2(KV4_NONE, 0.f);
         unsigned long long mine = 0;
         if (lane < parts) {
@@ -701,36 +699,36 @@ __global__ void __launch_bounds__(KJ * 32) kv4_join_shared_kernel(const Kv4Attn 
         for (int e = 0; e < D / 32; ++e) dt<T>::st(y, row_of(n, n.c) * D + lane + 32 * e, o[e] / l);
       }
     }
-    if (__syncthreads_or(longer) == 0) continue;
-    for (int i = 0; i < KJ && u0 + i < units; ++i) {
-      const Unit n = unit_of(u0 + i);
-      const int parts = n.a.z + n.b.x;
-      if (parts <= 32 || n.c >= n.a.y * R) continue;      // (the same for the whole block)
-      KjSum<D> s;
+  }
+  if (work[3] <= 32) return;
+  for (int u = blockIdx.x; u < units; u += gridDim.x) {
+    const Unit n = unit_of(u);
+    const int parts = n.a.z + n.b.x;
+    if (parts <= 32 || n.c >= n.a.y * R) continue;      // (the same for the whole block)
+    KjSum<D> s;
 #pragma unroll 4
-      for (int k = warp; k < parts; k += KJ) {
-        bool in_many;
-        const size_t at = part_at(n, k, in_many);
-        s.add(in_many ? many_ml[at] : few_ml[at], (in_many ? many_part : few_part) + at * D, lane);
+    for (int k = warp; k < parts; k += KJ) {
+      bool in_many;
+      const size_t at = part_at(n, k, in_many);
+      s.add(in_many ? many_ml[at] : few_ml[at], (in_many ? many_part : few_part) + at * D, lane);
+    }
+    __syncthreads();                         // (the unit before this one has been read)
+    if (lane == 0) s_m[warp] = s.m, s_l[warp] = s.l;
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) s_o[warp][lane + 32 * e] = s.o[e];
+    __syncthreads();
+    const int d = threadIdx.x;
+    if (d < D) {
+      float m = s_m[0], num = 0.f, den = 0.f;
+#pragma unroll
+      for (int w = 1; w < KJ; ++w) m = fmaxf(m, s_m[w]);
+#pragma unroll
+      for (int w = 0; w < KJ; ++w) {
+        const float f = kf_exp2(s_m[w] - m);
+        num = fmaf(s_o[w][d], f, num);
+        den = fmaf(s_l[w], f, den);
       }
-      __syncthreads();                         // (the unit before this one has been read)
-      if (lane == 0) s_m[warp] = s.m, s_l[warp] = s.l;
-#pragma unroll
-      for (int e = 0; e < D / 32; ++e) s_o[warp][lane + 32 * e] = s.o[e];
-      __syncthreads();
-      const int d = threadIdx.x;
-      if (d < D) {
-        float m = s_m[0], num = 0.f, den = 0.f;
-#pragma unroll
-        for (int w = 1; w < KJ; ++w) m = fmaxf(m, s_m[w]);
-#pragma unroll
-        for (int w = 0; w < KJ; ++w) {
-          const float f = kf_exp2(s_m[w] - m);
-          num = fmaf(s_o[w][d], f, num);
-          den = fmaf(s_l[w], f, den);
-        }
-        dt<T>::st(y, row_of(n, n.c) * D + d, num / den);
-      }
+      dt<T>::st(y, row_of(n, n.c) * D + d, num / den);
     }
   }
 }
@@ -783,7 +781,7 @@ static int attend(const ll_kv4_cache* cache, const void* blocks, const void* q, 
   // The sequences of few columns fill the end of the prompts' kernel, which lets them in when it has begun.  The join waits for both (kv4_few_kernel's last blocks).
   // (None where walks are not cut, or where no sequence may bring a token: then all that bring some are refused.)
   const unsigned join_blocks =
-      share ? (unsigned)std::min<long long>(4ll * kv4_sms(), ((long long)B * G * columns + KJ - 1) / KJ) :
+      share ? (unsigned)std::min<long long>(4ll * kv4_sms(), (long long)B * G * columns) :
       l.few_cut || l.many ? (unsigned)std::min<long long>(4ll * kv4_sms(), (long long)l.few_joins() * G * used + (l.many ? (long long)l.many_joins() * G * (KV4_MANY / KJ) : 0)) : 0;
   LL_CHECK_ARG(l.few_items * G + 4ll * kv4_sms() <= INT_MAX, "kv4_attn: %d sequences of %d tokens, %d heads", B, T, H);
   const unsigned solo_blocks = (unsigned)((l.few_items * G + KF_WARPS - 1) / KF_WARPS) + 4u * kv4_sms();

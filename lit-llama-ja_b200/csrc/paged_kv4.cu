@@ -421,7 +421,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv4_share_kernel(Kv4Pool c, Kv4P
   divide_work<false>(ShareView{v, s_page, s_first, s_last, s_many, n, R, KV4_SHARE_FEW, true}, many, s_need, s_size, s_walk);
   __syncthreads();
   // what has to be joined: a sequence's parts and its group's
-  if (threadIdx.x == 0) s_need[0] = 0;
+  if (threadIdx.x == 0) s_need[0] = s_need[1] = 0;
   __syncthreads();
   for (int i = threadIdx.x; i < B; i += nt) {
     const int count = v.tokens(i), g = s_group[i];
@@ -434,15 +434,17 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv4_share_kernel(Kv4Pool c, Kv4P
       o[1] = make_int4(0, 0, 0, 2);
     } else if (g < 0) {
       o[1] = make_int4(0, 0, 0, 0);
+      atomicMax(&s_need[1], s_few[i].x);
     } else {
       const int column = (s_starts[i] - s_starts[s_first[g]]) * R;
       const bool large = (long long)(s_starts[s_last[g] + 1] - s_starts[s_first[g]]) * R > KV4_SHARE_FEW;
       const int2 w = large ? s_many[B + g] : s_few[B + g];
       o[1] = make_int4(w.x, w.y, column, large ? 1 : 0);
+      atomicMax(&s_need[1], s_few[i].x + w.x);
     }
   }
   __syncthreads();
-  if (threadIdx.x == 0) few.work[1] = s_need[0];
+  if (threadIdx.x == 0) few.work[1] = s_need[0], few.work[3] = s_need[1];
 }
 
 // Positions and slots of a step's tokens from `here` on.

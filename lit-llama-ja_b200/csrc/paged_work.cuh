@@ -23,7 +23,8 @@ struct Kv4Attn {
 
 namespace {
 
-// A list of parts of walks: four numbers (parts, walks that are in more than one part), the parts, then those walks.
+// A list of parts of walks: four numbers (parts, walks that are in more than one part; where pages are shared, records of what has to be joined, nothing, and the most parts
+// of one), the parts, then those walks.
 // One part of a walk: a range of one request's pages for one tile of columns (a column: one query of one of the heads that share a key head, the
 // heads of a token next to one another).  The largest parts come first.
 struct __align__(16) Kv4Item {
