@@ -104,22 +104,33 @@ __device__ __forceinline__ void remote_bins(uint32_t (&h)[BINS], uint32_t at) {
   }
 }
 
-// Sum over the threads before this one.  Every thread of the block calls.
+// Of the warps' sums those before this warp's, and all.
+template <int WARPS>
+__device__ __forceinline__ u64 warps_before(const u64* s, u64& all) {
+  const int lane = threadIdx.x & 31;
+  const u64 x = lane < WARPS ? s[lane] : 0;
+  u64 incl = x;
+#pragma unroll
+  for (int o = 1; o < WARPS; o <<= 1) {
+    const u64 n = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += n;
+  }
+  all = __shfl_sync(0xffffffffu, incl, WARPS - 1);
+  return __shfl_sync(0xffffffffu, incl - x, threadIdx.x >> 5);
+}
+// Sum over the threads before this one, and over all.  Every thread of the block calls.
 template <int THREADS>
-__device__ __forceinline__ u64 threads_before(u64 v, u64* s) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+__device__ __forceinline__ u64 threads_before(u64 v, u64* s, u64& all) {
+  const int lane = threadIdx.x & 31;
   u64 incl = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const u64 n = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += n;
   }
-  if (lane == 31) s[warp] = incl;
+  if (lane == 31) s[threadIdx.x >> 5] = incl;
   __syncthreads();
-  u64 before = 0;
-#pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) before += w < warp ? s[w] : 0;
-  return before + incl - v;
+  return warps_before<THREADS / 32>(s, all) + incl - v;
 }
 
 template <typename T, int THREADS>
@@ -216,9 +227,8 @@ __global__ void __launch_bounds__(THREADS, THREADS == SR_WIDE ? 2 : 8) sample_ro
     if (lane == 0) sh.scan[warp] = v;
     __syncthreads();
     if (warp == 0) {
-      u64 all = 0;
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) all += sh.scan[w];
+      u64 all;
+      warps_before<WARPS>(sh.scan, all);
       if (lane < C) cluster.map_shared_rank(&sh.sums[sums][0], lane)[rank] = all;
     }
     cluster.sync();
@@ -254,7 +264,8 @@ __global__ void __launch_bounds__(THREADS, THREADS == SR_WIDE ? 2 : 8) sample_ro
     u64 all = 0;
 #pragma unroll
     for (int b = 0; b < BINS; ++b) all += n[b];
-    return threads_before<THREADS>(all, sh.scan);
+    u64 total;
+    return threads_before<THREADS>(all, sh.scan, total);
   };
   // The keys of the steps first_bin .. last_bin below m: the smallest key at most so many steps below, by 32 at a time.
   auto keys_of = [&](int first_bin, int last_bin) {
@@ -492,11 +503,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == SR_WIDE ? 2 : 8) sample_ro
     }
     auto block_before = [&](u64 x, u64& total) {
       __syncthreads();                           // (the sums before have been read)
-      const u64 before = threads_before<THREADS>(x, sh.scan);
-      total = 0;
-#pragma unroll
-      for (int o = 0; o < WARPS; ++o) total += sh.scan[o];
-      return before;
+      return threads_before<THREADS>(x, sh.scan, total);
     };
     u64 total;
     block_before(sum, total);
@@ -651,8 +658,8 @@ __global__ void __launch_bounds__(THREADS, THREADS == SR_WIDE ? 2 : 8) sample_ro
   const u64 total = cluster_sum(n, before);
   const u64 target = first ? 0 : min((u64)floor((double)u * (double)total), total - 1);
   // the warp that the target falls to goes through its run
-#pragma unroll
-  for (int w = 0; w < WARPS; ++w) before += w < warp ? sh.scan[w] : 0;
+  u64 in_block;
+  before += warps_before<WARPS>(sh.scan, in_block);
   if (target < before || target >= before + sh.scan[warp]) return;
   each(lowest, [&](const float (&x)[N], int j) {
     u64 w[N], incl = 0;
