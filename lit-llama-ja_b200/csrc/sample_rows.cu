@@ -9,10 +9,11 @@
 // The few numbers of those steps are then compared with one another, on top of the exact sum of what lies above; where they are many (rows of few values), the border is
 // found by counts or exact weights of their keys, 1024 ranges at a time.
 //
-// What bounds it: 301 rows of 100 003 (fp32) under top-p and min-p 343 us, 128 without a border (copying them takes 18): the barriers of a cluster, 1 to 1.5 us each, between phases of 3
-// to 6 us of the exponentials' instructions (eleven of 64 bits each), two blocks an SM.  One row of 32 000 (bf16): 5.3 us, 8.0 under top-k, 14 under top-p.  On the way (us, 301 rows, top-p):
-// a block a row and bisection 3334; exact weights in all steps, two dependent additions of 32 bits in shared memory each, 738; steps' weights in parts, and a list of the border's
-// numbers appended by remote atomics 639, by one's own 435; the exponential by a table 343.
+// What bounds it: 301 rows of 100 003 (fp32) under top-p and min-p 325 us, 125 without a border (copying them takes 18): instructions (54 % of the issue slots) and the barriers of
+// a cluster, 1 to 1.5 us each, between phases of 3 to 6 us of exponentials (eleven instructions of 64 bits each), two blocks an SM.  One row of 32 000 (bf16): 5.2 us, 7.9 under top-k,
+// 14 under top-p.  On the way (us, 301 rows, top-p and min-p): a block a row and bisection 3334; exact weights in all steps, two dependent additions of 32 bits in shared memory each, 738;
+// steps' weights in parts, and a list of the border's numbers by remote atomics 639, by one's own 435; the exponential by a table, one block that finishes alone and
+// sums by lanes 325.
 //
 // A cluster of blocks has a row in its shared memory, read once.
 #include <cooperative_groups.h>
@@ -165,7 +166,8 @@ __global__ void __launch_bounds__(THREADS, THREADS == SR_WIDE ? 2 : 8) sample_ro
     for (int e = 0; e < N; ++e) asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(x[e]));
   }
   bad |= isnan(top);
-  for (int b = t; b < 2 * 2 * SR_BINS; b += THREADS) (&sh.hist[0][0][0])[b] = 0;
+  if ((top_k >= 1 && top_k < V) || top_p < 1.f)      // (the first turn's counts; what comes after them is set to none on the way)
+    for (int b = t; b < SR_BINS; b += THREADS) sh.hist[0][0][b] = 0;
   for (int b = t; b < SR_TABLE; b += THREADS) sh.exps[b] = exp2(b * (1.0 / SR_TABLE));
   if (t < 2) sh.listed[t] = 0;
   {
