@@ -78,11 +78,11 @@ struct SampleShared {
   double exps[SR_TABLE];                         // 2^(j / 256)
   alignas(16) u64 list_weight[SR_LIST];          // all blocks' lists
   alignas(16) uint32_t list_key[SR_LIST];
-  u64 scan[THREADS / 32], found_base, sums[2][SR_MOST];
+  u64 scan[THREADS / 32], found_base, sums[2][SR_MOST], kept[SR_MOST];
   uint32_t key[SR_MOST], warp_key[THREADS / 32], range[2], listed[2], least_key;
   int found, last;
 };
-static_assert(SR_LIST * 12 <= 2 * SR_BINS * 4, "a list in the place of counts");
+static_assert(SR_LIST * 16 <= 2 * SR_BINS * 4, "a list in the place of counts");
 
 // Another block's shared memory, asked for by its place in this one's.
 __device__ __forceinline__ uint32_t there(const void* p, int rank) {
@@ -341,11 +341,14 @@ __global__ void __launch_bounds__(THREADS, THREADS == SR_WIDE ? 2 : 8) sample_ro
     }
   };
   // The same where SR_LIST numbers at most have keys lo .. hi: every block compares all of them.
+  int listed = 0;
+  u64 warp_above = 0;                            // of the warp's numbers what lies above hi
   auto by_list = [&](auto weights, uint32_t lo, uint32_t hi, u64 base, auto reached, int which) {
     constexpr bool WEIGHTS = decltype(weights)::value;
     const float least = fmaxf(key_value<T>(lo), lowest), most = key_value<T>(hi);
     u64* const weight_here = reinterpret_cast<u64*>(&sh.hist[turn][0][0]);      // (zeros that nobody reads)
     uint32_t* const key_here = reinterpret_cast<uint32_t*>(weight_here + SR_LIST);
+    uint32_t* const warp_here = key_here + SR_LIST;
     u64 above = 0, none;
     each(least, [&](const float (&x)[N], int) {
 #pragma unroll
@@ -356,11 +359,11 @@ __global__ void __launch_bounds__(THREADS, THREADS == SR_WIDE ? 2 : 8) sample_ro
           above += w;
         } else {
           const uint32_t at = atomicAdd(&sh.listed[which], 1u);
-          if (at < SR_LIST) key_here[at] = order_key<T>(x[e]), weight_here[at] = w;
+          if (at < SR_LIST) key_here[at] = order_key<T>(x[e]), weight_here[at] = w, warp_here[at] = warp;
         }
       }
     });
-    if (WEIGHTS) base = cluster_sum(above, none);
+    if (WEIGHTS) base = cluster_sum(above, none), warp_above = sh.scan[warp];
     else cluster.sync();
     // all lists one after the other, a warp or some a block's
     if (t < C) sh.key[t] = min(remote(there(&sh.listed[which], t)), (uint32_t)SR_LIST);
@@ -381,6 +384,8 @@ __global__ void __launch_bounds__(THREADS, THREADS == SR_WIDE ? 2 : 8) sample_ro
       n += of_c;
     }
     __syncthreads();
+    if (WEIGHTS) cluster.barrier_arrive();       // (the lists have been read; the wait stands where the kept weights are added up)
+    listed = n;
     while (lo < hi) {
       int shift = 0;
       while (((hi - lo) >> shift) >= (uint32_t)SR_BINS) ++shift;
@@ -573,6 +578,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == SR_WIDE ? 2 : 8) sample_ro
       lowest = fmaxf(lowest, key_value<T>(border));
     }
   }
+  float settled = -INFINITY;                     // numbers above it and those of a list are all that is kept
   if (top_p < 1.f) {
     // A step's weights as parts of its middle one, in 13 bits: each off by half of one in 8067, 2^-13.98 (a part is at least exp(-15.6 / 1024)), by 2^-17.4 with
     // its place in the step (three roundings of a number of 1024, times 0.03), and by 2^-27 with the series: less than 2^-13 together; and a weight, rounded to a whole
@@ -625,6 +631,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == SR_WIDE ? 2 : 8) sample_ro
     keys_of(from, to);
     const uint32_t lo = sh.range[0], hi = sh.range[1];
     auto reached = [&](u64 x) { return x > 0 && (double)x >= want; };
+    if (lo != hi && few) settled = key_value<T>(hi);
     const uint32_t border = lo == hi ? hi : few ? by_list(std::true_type(), lo, hi, 0, reached, 1) : by_keys(std::true_type(), lo, hi, 0, reached);
     lowest = fmaxf(lowest, key_value<T>(border));
   }
@@ -652,12 +659,36 @@ __global__ void __launch_bounds__(THREADS, THREADS == SR_WIDE ? 2 : 8) sample_ro
     const u64 w = weight(fmaxf(v, cut));
     return v >= lowest ? w : 0;
   };
-  u64 n = 0, before = 0;
-  each(lowest, [&](const float (&x)[N], int) {
+  u64 before = 0, total = 0;
+  if (settled > -INFINITY) cluster.barrier_wait();
+  if (lowest <= settled) {                       // top-p's list and what lies above it: sums of warps and blocks without another look at the row
+    const uint32_t from = order_key<T>(lowest);
+    const u64* const weight_here = reinterpret_cast<const u64*>(&sh.hist[turn ^ 1][0][0]);
+    const uint32_t *const key_here = reinterpret_cast<const uint32_t*>(weight_here + SR_LIST), *const warp_here = key_here + SR_LIST;
+    if (lane == 0) sh.scan[warp] = warp_above;
+    if (t < C) sh.kept[t] = sh.sums[sums ^ 1][t];
+    __syncthreads();
+    for (int i = t; i < min((int)sh.listed[1], SR_LIST); i += THREADS)
+      if (key_here[i] >= from) atomicAdd(&sh.scan[warp_here[i]], weight_here[i]);
+    for (int i = t; i < listed; i += THREADS) {
+      if (sh.list_key[i] < from) continue;
+      int c = 0;
+      for (int end = (int)sh.key[0]; i >= end; end += (int)sh.key[c]) ++c;
+      atomicAdd(&sh.kept[c], sh.list_weight[i]);
+    }
+    __syncthreads();
+    for (int c = 0; c < C; ++c) {
+      if (c == rank) before = total;
+      total += sh.kept[c];
+    }
+  } else {
+    u64 n = 0;
+    each(lowest, [&](const float (&x)[N], int) {
 #pragma unroll
-    for (int e = 0; e < N; ++e) n += kept(x[e]);
-  });
-  const u64 total = cluster_sum(n, before);
+      for (int e = 0; e < N; ++e) n += kept(x[e]);
+    });
+    total = cluster_sum(n, before);
+  }
   const u64 target = first ? 0 : min((u64)floor((double)u * (double)total), total - 1);
   // the warp that the target falls to goes through its run
   u64 in_block;

@@ -160,6 +160,16 @@ def test_borders_among_many_alike(dtype):
         _same(x, torch.rand(len(rows), generator=gen), **s)
 
 
+@pytest.mark.parametrize("dtype", [BF, HF, FP], ids=str)
+@pytest.mark.parametrize("R, V", [(6, 60000), (3, 150001), (40, 9000)])
+def test_top_p_beside_min_p(R, V, dtype):
+    """Borders of min-p below, among and above the numbers that top-p's falls into; one draw from each part of a row."""
+    for i, (p, m, t, k) in enumerate([(0.9, 1e-4, 1.0, 0), (0.9, 0.004, 1.0, 0), (0.9, 0.02, 1.0, 0), (0.95, 0.3, 1.0, 0), (0.99, 1e-3, 1.5, 0), (0.7, 0.01, 0.8, 5000), (0.999, 1e-6, 2.0, 0)]):
+        x = _logits(R, V, dtype, 50 + i)
+        u = torch.arange(R).float().add(0.5).div(R)
+        _same(x, u, top_p=p, min_p=m, temperature=t, top_k=k if k else None)
+
+
 def test_refusals():
     from lit_llama.sampling import sample, token_logprobs
 
