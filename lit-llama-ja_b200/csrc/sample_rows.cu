@@ -9,11 +9,11 @@
 // The few numbers of those steps are then compared with one another, on top of the exact sum of what lies above; where they are many (rows of few values), the border is
 // found by counts or exact weights of their keys, 1024 ranges at a time.
 //
-// What bounds it: 301 rows of 100 003 (fp32) under top-p and min-p 325 us, 125 without a border (copying them takes 18): instructions (54 % of the issue slots) and the barriers of
-// a cluster, 1 to 1.5 us each, between phases of 3 to 6 us of exponentials (eleven instructions of 64 bits each), two blocks an SM.  One row of 32 000 (bf16): 5.2 us, 7.9 under top-k,
-// 14 under top-p.  On the way (us, 301 rows, top-p and min-p): a block a row and bisection 3334; exact weights in all steps, two dependent additions of 32 bits in shared memory each, 738;
-// steps' weights in parts, and a list of the border's numbers by remote atomics 639, by one's own 435; the exponential by a table, one block that finishes alone and
-// sums by lanes 325.
+// What bounds it: 301 rows of 100 003 (fp32) under top-p and min-p 253 us, under top-p alone 317, 125 without a border (copying them takes 18): instructions (half of the issue slots)
+// and the barriers of a cluster, 1 to 1.5 us each, between phases of 3 to 6 us of exponentials (ten instructions of 64 bits each), two blocks an SM.  One row of 32 000 (bf16): 5.2 us,
+// 7.9 under top-k, 14 under top-p.  On the way (us, 301 rows, top-p and min-p): a block a row and bisection 3334; exact weights in all steps, two dependent additions of 32 bits in shared
+// memory each, 738; steps' weights in parts, and a list of the border's numbers by remote atomics 639, by one's own 435; the exponential by a table, one block that
+// finishes alone and sums by lanes 325; top-p's border not looked for where min-p's is above it 253.
 //
 // A cluster of blocks has a row in its shared memory, read once.
 #include <cooperative_groups.h>
@@ -578,7 +578,27 @@ __global__ void __launch_bounds__(THREADS, THREADS == SR_WIDE ? 2 : 8) sample_ro
       lowest = fmaxf(lowest, key_value<T>(border));
     }
   }
-  float settled = -INFINITY;                     // numbers above it and those of a list are all that is kept
+  // The smallest number that min-p keeps, by 32 at a time (-inf: all).
+  auto least_of = [&]() {
+    if (!(min_p > 0.f)) return -INFINITY;
+    if (warp == 0) {
+      const u64 least = (u64)ceil((double)fminf(min_p, 1.f) * SR_ONE);
+      uint32_t from = order_key<T>(lowest) - 1u, to = order_key<T>(m);     // `from` weighs less or is not kept, `to` is
+      while (to - from > 1u) {
+        const uint32_t step = (to - from - 1u) / 33u + 1u;
+        const u64 probe = min((u64)from + (u64)(lane + 1) * step, (u64)to);
+        const uint32_t in = __ballot_sync(0xffffffffu, weight(fmaxf(key_value<T>((uint32_t)probe), cut)) >= least);
+        const int at = in != 0u ? __ffs(in) - 1 : 32;
+        const u64 above = (u64)from + (u64)at * step;
+        if (in != 0u) to = (uint32_t)min(above + step, (u64)to);
+        from = (uint32_t)above;
+      }
+      if (lane == 0) sh.least_key = to;
+    }
+    __syncthreads();
+    return key_value<T>(sh.least_key);
+  };
+  float settled = -INFINITY, least_kept = -INFINITY;      // numbers above `settled` and those of a list are all that is kept
   if (top_p < 1.f) {
     // A step's weights as parts of its middle one, in 13 bits: each off by half of one in 8067, 2^-13.98 (a part is at least exp(-15.6 / 1024)), by 2^-17.4 with
     // its place in the step (three roundings of a number of 1024, times 0.03), and by 2^-27 with the series: less than 2^-13 together; and a weight, rounded to a whole
@@ -631,30 +651,18 @@ __global__ void __launch_bounds__(THREADS, THREADS == SR_WIDE ? 2 : 8) sample_ro
     keys_of(from, to);
     const uint32_t lo = sh.range[0], hi = sh.range[1];
     auto reached = [&](u64 x) { return x > 0 && (double)x >= want; };
-    if (lo != hi && few) settled = key_value<T>(hi);
-    const uint32_t border = lo == hi ? hi : few ? by_list(std::true_type(), lo, hi, 0, reached, 1) : by_keys(std::true_type(), lo, hi, 0, reached);
-    lowest = fmaxf(lowest, key_value<T>(border));
+    least_kept = least_of();
+    if (least_kept <= key_value<T>(hi)) {        // (else min-p keeps less than top-p)
+      if (lo != hi && few) settled = key_value<T>(hi);
+      const uint32_t border = lo == hi ? hi : few ? by_list(std::true_type(), lo, hi, 0, reached, 1) : by_keys(std::true_type(), lo, hi, 0, reached);
+      lowest = fmaxf(lowest, key_value<T>(border));
+    }
+  } else {
+    least_kept = least_of();
   }
+  lowest = fmaxf(lowest, least_kept);
 
   // ---- kept weights
-  if (min_p > 0.f) {                             // the smallest number that weighs as much, by 32 at a time
-    if (warp == 0) {
-      const u64 least = (u64)ceil((double)fminf(min_p, 1.f) * SR_ONE);
-      uint32_t from = order_key<T>(lowest) - 1u, to = order_key<T>(m);     // `from` weighs less or is not kept, `to` is
-      while (to - from > 1u) {
-        const uint32_t step = (to - from - 1u) / 33u + 1u;
-        const u64 probe = min((u64)from + (u64)(lane + 1) * step, (u64)to);
-        const uint32_t in = __ballot_sync(0xffffffffu, weight(fmaxf(key_value<T>((uint32_t)probe), cut)) >= least);
-        const int at = in != 0u ? __ffs(in) - 1 : 32;
-        const u64 above = (u64)from + (u64)at * step;
-        if (in != 0u) to = (uint32_t)min(above + step, (u64)to);
-        from = (uint32_t)above;
-      }
-      if (lane == 0) sh.least_key = to;
-    }
-    __syncthreads();
-    lowest = fmaxf(lowest, key_value<T>(sh.least_key));
-  }
   auto kept = [&](float v) -> u64 {
     const u64 w = weight(fmaxf(v, cut));
     return v >= lowest ? w : 0;
