@@ -903,7 +903,8 @@ LL_API int ll_kv4_shared_attn(const ll_kv4_cache* cache, const void* blocks, con
 /* ---------------------------------------------------------------------------------------
  * What a step's logits are asked: a token a row (csrc/sample_rows.cu), and how likely given ones are (csrc/token_logprobs.cu).  logits: R rows of V numbers
  * (fp32, bf16 or fp16), `row` numbers apart.  Settings: one a row on the device, or null and one for all.
- * Draw.  With the row's largest logit m and a temperature T > 0, token i weighs w_i = rint(2^44 exp((l_i - m) / T)) in 64 bits (l_i = m: 2^44).  Kept are logits at least
+ * Draw.  With the row's largest logit m and a temperature T > 0, token i weighs w_i = rint(2^44 exp((l_i - m) / T)) in 64 bits (l_i = m: 2^44; where what is rounded lies within
+ * 2^-6 of a half, the whole number on either side of it).  Kept are logits at least
  * as large as the k-th largest (top_k < 1, or V and more: all), of these the largest up to the first one with which the weights reach top_p of the kept ones' (1 and
  * more: all), of these those with w >= min_p 2^44 (min_p above 1 counts as 1); logits that are equal stay together.  The token is the first one whose running sum of kept weights exceeds
  * min(floor(u * sum), sum - 1).  T under 2^-100: the first of the largest logits.  -1: a logit or setting is no number, all logits are -inf, T is negative or

@@ -26,6 +26,7 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr double SR_ONE = 17592186044416.0;      // 2^44
+constexpr double SR_PER = 256 * 1.4426950408889634;      // 256 / ln 2
 constexpr float SR_REACH = 31.25f;               // weights are 0 from 45 ln 2 = 31.19 temperatures below m on
 constexpr float SR_LEAST = 7.888609052210118e-31f;      // 2^-100: less of a temperature counts as 0
 constexpr int SR_BINS = 1024, SR_LIST = 512, SR_TABLE = 256;
@@ -46,9 +47,10 @@ template <typename T> __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~(k | ((1u << key_shift<T>::n) - 1u)));
 }
 
-// rint(2^44 exp(d / T)) for d <= 0, with c = 256 / (T ln 2): by a table of 2^(j / 256) and a polynomial of degree 4 around its places (Tang, Table-driven
-// implementation of the exponential function, 1989): at most half of ln 2 / 256 from one, so that the next term is under 2^-54.  c d is off by 2^-52 of itself, times
-// exp(d / T) less than 2^-8 of a whole one.
+// rint(2^44 exp(d / T)) for d <= 0, with c = SR_PER / T: by a table of 2^(j / 256) and a polynomial of degree 4 around its places (Tang, Table-driven
+// implementation of the exponential function, 1989): at most half of ln 2 / 256 from one, so that the next term is under 2^-54 of a weight.  Before it is rounded a weight is off by
+// less than 2^-6 of a whole one: by 2^-52 of |d / T| of itself with c (x exp(-x) is 0.37 at most), 2^-52 with the table and 2^-53 with the last product.  So one in some thousand weights is the
+// whole number beside the nearest one.
 __device__ __forceinline__ u64 weight_of(double d, double c, const double* table) {
   constexpr double SHIFT = 6755399441055744.0;   // 1.5 2^52: the sum's last bits are the nearest whole number
   constexpr double L = 0.0027076061740622863;    // ln 2 / 256
@@ -201,7 +203,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == SR_WIDE ? 2 : 8) sample_ro
   }
 
   // ---- steps below m, and weights
-  const double c64 = 369.32994026157255 / (double)temperature, m64 = m;      // 256 / ln 2
+  const double c64 = SR_PER / (double)temperature, m64 = m;
   const float half_m = 0.5f * m, per_half = 2.f * (SR_BINS / SR_REACH) / temperature;      // (by halves: m - v may be more than a float holds)
   const float cut = fmaxf(m - 31.5f * temperature, -3.402823466e38f);      // weights are 0 from here on; -inf is below
   auto below = [&](float v) { return fmaf(v, -0.5f, half_m) * per_half; };
@@ -625,7 +627,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == SR_WIDE ? 2 : 8) sample_ro
 #pragma unroll
     for (int b = 0; b < BINS; ++b) {
       numbers[b] = ((uint32_t)n[b] + 8059u) / 8060u;         // at most
-      n[b] = (u64)((double)n[b] * ((double)weight_of(-(BINS * t + b) * (double)(SR_REACH / SR_BINS), 369.32994026157255, sh.exps) * (1.0 / 8192)));
+      n[b] = (u64)((double)n[b] * ((double)weight_of(-(BINS * t + b) * (double)(SR_REACH / SR_BINS), SR_PER, sh.exps) * (1.0 / 8192)));
     }
     u64 at = bins_before(n);
     constexpr double OFF = 1.0 / 8192;
