@@ -23,12 +23,18 @@ __device__ __forceinline__ float exp2_fast(float x) {
 __device__ __forceinline__ void add2(float2& a, float2 b) {
   asm("{\n\t.reg .b64 p, q;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %3};\n\tadd.rn.f32x2 p, p, q;\n\tmov.b64 {%0, %1}, p;\n\t}" : "+f"(a.x), "+f"(a.y) : "f"(b.x), "f"(b.y));
 }
+// (a - b) / (T ln 2).  FAR, for temperatures above 1e36: as (a / 4 - b / 4) (4 / (T ln 2)), since differences may be more than a number of 32 bits holds (their quarters are exact, and rounded
+// once; the factor stays a normal number).  Under lower temperatures such differences come to less than -100, of which no exponential is left.
+constexpr float LP_FAR = 1e36f;
+template <bool FAR>
+__device__ __forceinline__ float scaled(float a, float b, float c) { return (FAR ? fmaf(a, 0.25f, b * -0.25f) : a - b) * c; }
 // exp((l - m) / T) over some logits: the largest one, how many equal it, the others' sum.
 struct RowSum {
   float m, ones, sum;
+  template <bool FAR>
   __device__ __forceinline__ void under(float top, float c) {      // top >= m
     if (top == m) return;
-    const float f = exp2_fast((m - top) * c);
+    const float f = exp2_fast(scaled<FAR>(m, top, c));
     sum = (sum + ones) * f;
     ones = 0.f;
     m = top;
@@ -58,18 +64,10 @@ __device__ __forceinline__ float2 sub_mul2(float2 x, float m, float c) {
       : "=f"(r.x), "=f"(r.y) : "f"(x.x), "f"(x.y), "f"(-m), "f"(c));
   return r;
 }
-template <typename T, int THREADS>
-__global__ void __launch_bounds__(256, lp_blocks<T>) token_logprobs_kernel(const LogprobArgs a) {
-  constexpr int LP_BATCH = lp_batch<T>, N = row_vec<T>::n, ROWS = THREADS == LP_NARROW ? 8 : 1;
-  const int C = ROWS > 1 ? 1 : a.split, rank = ROWS > 1 ? 0 : (int)blockIdx.x % C;
-  const int r = (int)blockIdx.x / C * ROWS + (ROWS > 1 ? threadIdx.x >> 5 : 0), t = ROWS > 1 ? threadIdx.x & 31 : threadIdx.x, V = a.V;
-  if (r >= a.R) return;
-  const T* l = (const T*)a.logits + r * a.row;
-  const float temperature = a.temperature ? a.temperature[r] : a.temperature_all;
-  const float c = (float)(1.4426950408889634 / (double)temperature);
-  const int64_t token = a.tokens[r];
-  const bool there = token >= 0 && token < V;
-  const float mine = there ? dt<T>::ld(l, token) : 0.f;
+// The row's largest logit, how many equal it and the others' sum, of the thread's numbers (a warp has one largest).
+template <typename T, int THREADS, bool FAR>
+__device__ __forceinline__ RowSum row_sum(const T* l, int V, int t, int rank, int C, float c) {
+  constexpr int LP_BATCH = lp_batch<T>, N = row_vec<T>::n;
   RowSum s{-INFINITY, 0.f, 0.f};
 #pragma unroll 1
   for (int at = rank * LP_BATCH * THREADS * N - row_offset(l); at < V; at += C * LP_BATCH * THREADS * N) {      // (all lanes go as often)
@@ -81,17 +79,17 @@ __global__ void __launch_bounds__(256, lp_blocks<T>) token_logprobs_kernel(const
     float top = s.m;
 #pragma unroll
     for (int b = 0; b < LP_BATCH; ++b) top = fmaxf(top, vec_max<T>(raw[b]));
-    s.under(warp_max(top), c);
+    s.template under<FAR>(warp_max(top), c);
 #pragma unroll
     for (int b = 0; b < LP_BATCH; ++b) {
       float x[N];
       vec_values<T>(raw[b], x);
-      if (__any_sync(0xffffffffu, vec_max<T>(raw[b]) == s.m)) {
+      if (FAR || __any_sync(0xffffffffu, vec_max<T>(raw[b]) == s.m)) {
         float part = 0.f;
 #pragma unroll
         for (int e = 0; e < N; ++e) {
           if (x[e] == s.m) s.ones += 1.f;
-          else part += exp2_fast((x[e] - s.m) * c);
+          else part += exp2_fast(scaled<FAR>(x[e], s.m, c));
         }
         s.sum += part;
       } else {
@@ -105,14 +103,32 @@ __global__ void __launch_bounds__(256, lp_blocks<T>) token_logprobs_kernel(const
       }
     }
   }
-  s.ones = warp_sum(s.ones), s.sum = warp_sum(s.sum);      // (a warp has one largest logit)
+  return s;
+}
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(256, lp_blocks<T>) token_logprobs_kernel(const LogprobArgs a) {
+  constexpr int ROWS = THREADS == LP_NARROW ? 8 : 1;
+  const int C = ROWS > 1 ? 1 : a.split, rank = ROWS > 1 ? 0 : (int)blockIdx.x % C;
+  const int r = (int)blockIdx.x / C * ROWS + (ROWS > 1 ? threadIdx.x >> 5 : 0), t = ROWS > 1 ? threadIdx.x & 31 : threadIdx.x, V = a.V;
+  if (r >= a.R) return;
+  const T* l = (const T*)a.logits + r * a.row;
+  const float temperature = a.temperature ? a.temperature[r] : a.temperature_all;
+  const bool far = temperature > LP_FAR;
+  const float c = (float)(1.4426950408889634 / (double)temperature * (far ? 4.0 : 1.0));
+  const int64_t token = a.tokens[r];
+  const bool there = token >= 0 && token < V;
+  const float mine = there ? dt<T>::ld(l, token) : 0.f;
+  RowSum s = far ? row_sum<T, THREADS, true>(l, V, t, rank, C, c) : row_sum<T, THREADS, false>(l, V, t, rank, C, c);
+  s.ones = warp_sum(s.ones), s.sum = warp_sum(s.sum);
   if constexpr (ROWS == 1) {
     __shared__ float s_part[3][THREADS / 32];
     if ((t & 31) == 0) s_part[0][t >> 5] = s.m, s_part[1][t >> 5] = s.ones, s_part[2][t >> 5] = s.sum;
     __syncthreads();
     auto join = [&](const float(*part)[THREADS / 32], int n) {      // by one warp
       s = t < n ? RowSum{part[0][t], part[1][t], part[2][t]} : RowSum{-INFINITY, 0.f, 0.f};
-      s.under(warp_max(s.m), c);
+      const float top = warp_max(s.m);
+      if (far) s.template under<true>(top, c);
+      else s.template under<false>(top, c);
       s.ones = warp_sum(s.ones), s.sum = warp_sum(s.sum);
     };
     if (t < 32) join(s_part, THREADS / 32);
