@@ -29,15 +29,39 @@ constexpr float LP_FAR = 1e36f;
 template <bool FAR>
 __device__ __forceinline__ float scaled(float a, float b, float c) { return (FAR ? fmaf(a, 0.25f, b * -0.25f) : a - b) * c; }
 // exp((l - m) / T) over some logits: the largest one, how many equal it, the others' sum.
+// Sum: of 64 bits for 32-bit numbers of a block's rows, of which a thread has up to 65 batches; of 32 for the others (17 of 16-bit numbers, 6 where a warp has a row).  With 32 for
+// all, a slowly rising row, whose every batch has a new largest logit, took the error of a factor and some additions a batch (2^18 numbers that rise by up to 30: 2.6e-6 off, now 0.8e-6);
+// with 64 for all, 2048 rows of 32 000 (bf16) took 31.8 us instead of 30.8.
+template <typename Sum>
 struct RowSum {
-  float m, ones, sum;
+  float m, ones;
+  Sum sum;
   template <bool FAR>
   __device__ __forceinline__ void under(float top, float c) {      // top >= m
     if (top == m) return;
-    const float f = exp2_fast(scaled<FAR>(m, top, c));
-    sum = (sum + ones) * f;
+    const float y = scaled<FAR>(m, top, c);
+    sum += (Sum)ones;
+    if (sizeof(Sum) == 8 && y > -1.f) {          // by the factor's difference from 1: many small steps are off by as much as one large one
+      float p = 1.0178086e-7f;                   // (2^y - 1) / y: ln 2^k / k! from k = 9 down; the next term is under 2^-26
+      p = fmaf(p, y, 1.3215487e-6f);
+      p = fmaf(p, y, 1.5252734e-5f);
+      p = fmaf(p, y, 1.5403530e-4f);
+      p = fmaf(p, y, 1.3333558e-3f);
+      p = fmaf(p, y, 9.6181291e-3f);
+      p = fmaf(p, y, 5.5504109e-2f);
+      p = fmaf(p, y, 2.4022651e-1f);
+      p = fmaf(p, y, 6.9314718e-1f);
+      sum = fma(sum, (Sum)(p * y), sum);
+    } else {
+      sum *= (Sum)exp2_fast(y);
+    }
     ones = 0.f;
     m = top;
+  }
+  __device__ __forceinline__ void add_lanes() {      // of one largest logit
+    ones = warp_sum(ones);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   }
 };
 
@@ -57,6 +81,7 @@ constexpr int LP_WIDE = 256, LP_NARROW = 32, LP_MOST = 8;      // LP_MOST: block
 // four 63 us, 2048 of 32 000 with four and six 30.5).
 template <typename T> constexpr int lp_batch = sizeof(T) == 4 ? 4 : 8;
 template <typename T> constexpr int lp_blocks = sizeof(T) == 4 ? 6 : 4;
+template <typename T, int THREADS> using lp_sum = RowSum<typename std::conditional<sizeof(T) == 4 && THREADS == LP_WIDE, double, float>::type>;
 // a - b and a * b of pairs, one instruction each
 __device__ __forceinline__ float2 sub_mul2(float2 x, float m, float c) {
   float2 r;
@@ -66,9 +91,9 @@ __device__ __forceinline__ float2 sub_mul2(float2 x, float m, float c) {
 }
 // The row's largest logit, how many equal it and the others' sum, of the thread's numbers (a warp has one largest).
 template <typename T, int THREADS, bool FAR>
-__device__ __forceinline__ RowSum row_sum(const T* l, int V, int t, int rank, int C, float c) {
+__device__ __forceinline__ lp_sum<T, THREADS> row_sum(const T* l, int V, int t, int rank, int C, float c) {
   constexpr int LP_BATCH = lp_batch<T>, N = row_vec<T>::n;
-  RowSum s{-INFINITY, 0.f, 0.f};
+  lp_sum<T, THREADS> s{-INFINITY, 0.f, 0};
 #pragma unroll 1
   for (int at = rank * LP_BATCH * THREADS * N - row_offset(l); at < V; at += C * LP_BATCH * THREADS * N) {      // (all lanes go as often)
     const int i0 = at + t * N;
@@ -80,28 +105,34 @@ __device__ __forceinline__ RowSum row_sum(const T* l, int V, int t, int rank, in
 #pragma unroll
     for (int b = 0; b < LP_BATCH; ++b) top = fmaxf(top, vec_max<T>(raw[b]));
     s.template under<FAR>(warp_max(top), c);
+    float sum = 0.f;
 #pragma unroll
     for (int b = 0; b < LP_BATCH; ++b) {
       float x[N];
       vec_values<T>(raw[b], x);
+      float2 w[N / 2];
       if (FAR || __any_sync(0xffffffffu, vec_max<T>(raw[b]) == s.m)) {
-        float part = 0.f;
+        auto one = [&](float v) {
+          if (v != s.m) return exp2_fast(scaled<FAR>(v, s.m, c));
+          s.ones += 1.f;
+          return 0.f;
+        };
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-          if (x[e] == s.m) s.ones += 1.f;
-          else part += exp2_fast(scaled<FAR>(x[e], s.m, c));
-        }
-        s.sum += part;
+        for (int e = 0; e < N; e += 2) w[e / 2] = make_float2(one(x[e]), one(x[e + 1]));
       } else {
-        float2 part = make_float2(0.f, 0.f);
 #pragma unroll
         for (int e = 0; e < N; e += 2) {
           const float2 d = sub_mul2(make_float2(x[e], x[e + 1]), s.m, c);
-          add2(part, make_float2(exp2_fast(d.x), exp2_fast(d.y)));
+          w[e / 2] = make_float2(exp2_fast(d.x), exp2_fast(d.y));
         }
-        s.sum += part.x + part.y;
       }
+#pragma unroll
+      for (int n = N / 4; n > 0; n /= 2)         // (by halves: three additions a number at most)
+#pragma unroll
+        for (int e = 0; e < n; ++e) add2(w[e], w[e + n]);
+      sum += w[0].x + w[0].y;
     }
+    s.sum += sum;
   }
   return s;
 }
@@ -118,28 +149,25 @@ __global__ void __launch_bounds__(256, lp_blocks<T>) token_logprobs_kernel(const
   const int64_t token = a.tokens[r];
   const bool there = token >= 0 && token < V;
   const float mine = there ? dt<T>::ld(l, token) : 0.f;
-  RowSum s = far ? row_sum<T, THREADS, true>(l, V, t, rank, C, c) : row_sum<T, THREADS, false>(l, V, t, rank, C, c);
-  s.ones = warp_sum(s.ones), s.sum = warp_sum(s.sum);
+  lp_sum<T, THREADS> s = far ? row_sum<T, THREADS, true>(l, V, t, rank, C, c) : row_sum<T, THREADS, false>(l, V, t, rank, C, c);
+  s.add_lanes();
   if constexpr (ROWS == 1) {
-    __shared__ float s_part[3][THREADS / 32];
-    if ((t & 31) == 0) s_part[0][t >> 5] = s.m, s_part[1][t >> 5] = s.ones, s_part[2][t >> 5] = s.sum;
+    __shared__ lp_sum<T, THREADS> s_part[THREADS / 32];
+    if ((t & 31) == 0) s_part[t >> 5] = s;
     __syncthreads();
-    auto join = [&](const float(*part)[THREADS / 32], int n) {      // by one warp
-      s = t < n ? RowSum{part[0][t], part[1][t], part[2][t]} : RowSum{-INFINITY, 0.f, 0.f};
+    auto join = [&](const lp_sum<T, THREADS>* part, int n) {      // by one warp
+      s = t < n ? part[t] : lp_sum<T, THREADS>{-INFINITY, 0.f, 0};
       const float top = warp_max(s.m);
       if (far) s.template under<true>(top, c);
       else s.template under<false>(top, c);
-      s.ones = warp_sum(s.ones), s.sum = warp_sum(s.sum);
+      s.add_lanes();
     };
     if (t < 32) join(s_part, THREADS / 32);
     if (C > 1) {
-      __shared__ float s_all[3][THREADS / 32];
+      __shared__ lp_sum<T, THREADS> s_all[LP_MOST];
       cg::cluster_group cluster = cg::this_cluster();
       cluster.sync();                            // (the first block has begun)
-      if (t == 0) {
-        float(*all)[THREADS / 32] = cluster.map_shared_rank(s_all, 0);
-        all[0][rank] = s.m, all[1][rank] = s.ones, all[2][rank] = s.sum;
-      }
+      if (t == 0) cluster.map_shared_rank(s_all, 0)[rank] = s;
       cluster.sync();
       if (rank > 0) return;
       if (t < 32) join(s_all, C);
@@ -154,7 +182,7 @@ __global__ void __launch_bounds__(256, lp_blocks<T>) token_logprobs_kernel(const
 
 // A warp a row where a lane has up to eight vectors, or 20 while there are four rows an SM; else a block, and several while their blocks fit the SMs.  us, a warp / a
 // block: bf16, 4000 rows of 1500 6.1 / 27, 300 of 1500 3.8 / 5.0, 2000 of 5000 8.2 / 14.9, 100 of 5000 6.4 / 3.7, 2000 of 16 000 18.1 / 16.0; fp32, 4000 of 1500 6.6 / 13.2, 1000 of
-// 5000 10.1 / 7.2.  One row of 200 000 (fp32) by one block 32.8, by eight 7.5.
+// 5000 10.1 / 7.8.  One row of 200 000 (fp32) by one block 32.8, by eight 7.7.
 template <typename T>
 int launch_logprobs(LogprobArgs a, cudaStream_t st) {
   const int sms = sm_count() > 0 ? sm_count() : 148;

@@ -84,7 +84,8 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature: Setting = 1.0,
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: Setting = 1.0) -> torch.Tensor:
     """Logarithms of the probabilities that softmax(``logits [rows, vocabulary]`` / temperature) gives to ``tokens [rows]`` (int64): float32 ``[rows]``.  No number
-    for a token that is not of the vocabulary, or a row of which there is no softmax.  Sums are of 32 bits, by vectors of 16 bytes: a row's last bits go with where it begins."""
+    for a token that is not of the vocabulary, or a row of which there is no softmax.  Batches of vectors of 16 bytes are added up in 32 bits,
+    and these in 64 for 32-bit rows that are not short: a row's last bits go with where it begins."""
     logits, code, R, V, device = _rows(logits)
     t, t_all = _setting("temperature", temperature, R, device, 1.0, 1.0e-30, 3.0e38)
     tokens = _vector("tokens", tokens, torch.int64, R, device)
