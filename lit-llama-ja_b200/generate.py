@@ -139,7 +139,7 @@ def generate_batch(model: LLaMA, prompts: Sequence[torch.Tensor], max_new_tokens
     token a sequence and step, replayed as one CUDA graph.  A sequence ends before its first ``eos_id``.
 
     ``samples`` answers to every prompt, one after the other: a prompt is stepped once, and its answers share its pages.  Where ``top_p`` or ``min_p`` is given, or a setting
-    is a tensor (one number a sequence, on the GPU), tokens are drawn by ``lit_llama.sampling.sample``.  Returns the sequences; with ``logprobs`` also a tensor of each
+    is a vector (one number a sequence, on the GPU), tokens are drawn by ``lit_llama.sampling.sample``.  Returns the sequences; with ``logprobs`` also a tensor of each
     one's new tokens' log-probabilities, as the model gives them (temperature 1, all tokens)."""
     if not prompts or max_new_tokens < 1 or samples < 1 or any(p.dim() != 1 or p.numel() == 0 for p in prompts):
         raise ValueError(f"{len(prompts)} prompts, {samples} answers to each, {max_new_tokens} tokens to come: one of each at least, and no prompt empty")
@@ -158,7 +158,7 @@ def generate_batch(model: LLaMA, prompts: Sequence[torch.Tensor], max_new_tokens
         cache.fork(copies[:, :1].expand(-1, samples - 1).reshape(-1), copies[:, 1:].reshape(-1))
         logits = logits.repeat_interleave(samples, 0)
         prompts = [p for p in prompts for _ in range(samples)]
-    drawn = top_p is not None or min_p is not None or any(isinstance(s, torch.Tensor) for s in (temperature, top_k))
+    drawn = top_p is not None or min_p is not None or any(isinstance(s, torch.Tensor) and s.dim() == 1 for s in (temperature, top_k))
     none = torch.zeros(B, dtype=torch.bool, device=dev)
     new = torch.empty((B, max_new_tokens), dtype=prompts[0].dtype, device=dev)
     scores = torch.empty((B, max_new_tokens), dtype=torch.float32, device=dev) if logprobs else None
