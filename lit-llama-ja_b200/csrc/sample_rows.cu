@@ -728,8 +728,8 @@ __global__ void __launch_bounds__(THREADS, THREADS == SR_WIDE ? 2 : 8) sample_ro
   });
 }
 
-// Blocks a row: enough that a thread has at most 32 numbers, and more while there are fewer blocks than SMs.  us without a border and under top-p, by one / two / four / eight
-// blocks a row of 32 000 (bf16): one row 18.9, 55 / 11.6, 31 / 7.8, 22 / 6.1, 21; 64 rows 19.4, 56 / 12.1, 38 / 11.1, 39 / 15.0, 62; 128 rows 19.6, 56 / 16.4, 53 / 19.7, 64 / 24.6, 104.
+// Blocks a row: enough that a thread has at most 32 numbers (eight at most: 68 in rows of 2^18), and more while there are fewer blocks than SMs.  us without a border and under top-p, by
+// one / two / four / eight blocks a row of 32 000 (bf16): one row 14.0, 34 / 9.0, 22 / 6.6, 17 / 5.3, 14; 64 rows 14.6, 40 / 9.6, 26 / 8.8, 23 / 12.7, 36; 128 rows 14.7, 41 / 13.2, 35 / 17.0, 45 / 24.5, 69.
 template <typename T, int THREADS>
 int launch_sample(SampleArgs a, int R, int C, cudaStream_t st) {
   constexpr int N = row_vec<T>::n;

@@ -138,7 +138,8 @@ def generate_batch(model: LLaMA, prompts: Sequence[torch.Tensor], max_new_tokens
     """``generate`` for prompts of unequal lengths at once, over a key/value cache in 4 bits (``lit_llama/paged_cache.py``): the prompts as one step, then a
     token a sequence and step, replayed as one CUDA graph.  A sequence ends before its first ``eos_id``.
 
-    ``samples`` answers to every prompt, one after the other: a prompt is stepped once, and its answers share its pages.  Where ``top_p`` or ``min_p`` is given, or a setting
+    ``samples`` answers to every prompt, one after the other: a prompt is stepped once, and its answers share its pages.  (Answers to prompts of fewer than 128 tokens have no two whole pages to
+    walk together; where sequences may have more than 512 tokens, steps then take some percent longer than those of as many prompts.)  Where ``top_p`` or ``min_p`` is given, or a setting
     is a vector (one number a sequence, on the GPU), tokens are drawn by ``lit_llama.sampling.sample``.  Returns the sequences; with ``logprobs`` also a tensor of each
     one's new tokens' log-probabilities, as the model gives them (temperature 1, all tokens)."""
     if not prompts or max_new_tokens < 1 or samples < 1 or any(p.dim() != 1 or p.numel() == 0 for p in prompts):

@@ -93,7 +93,9 @@ class PagedCache4:
                  group: int = 64, dtype: torch.dtype = torch.bfloat16, device="cuda", share: bool = False):
         """``pages`` of 64 slots for up to ``requests`` requests of up to ``max_length`` tokens; heads of 32, 64 or 128, codes by ``group``s of 32, 64 or 128
         of their dimensions.  ``n_kv_head`` key/value heads serve ``n_head`` query heads, neighbours the same one.  ``share``: requests may be forked, and steps
-        walk pages that neighbouring sequences share once (steps whose requests share none are up to a third slower than without it)."""
+        walk pages that neighbouring sequences share once.  Steps whose requests share none are slower than without it (attention 1.1 to 1.75 times, a plan of 8, 64 and 512
+        sequences 9, 7 and 11 us -> 14, 21 and 69), and fp16 results over pages that more than 32 queries of a key head share are a little less exact (values of 11 bits meet the
+        weights: 0.00027 of the norm off where a walk of one's own is 0.00021; of bf16 both are the rounding of the results)."""
         n_kv_head = n_head if n_kv_head is None else n_kv_head
         device = torch.device(device)
         if device.type != "cuda":
