@@ -28,6 +28,7 @@ namespace cg = cooperative_groups;
 constexpr double SR_ONE = 17592186044416.0;      // 2^44
 constexpr double SR_PER = 256 * 1.4426950408889634;      // 256 / ln 2
 constexpr float SR_REACH = 31.25f;               // weights are 0 from 45 ln 2 = 31.19 temperatures below m on
+constexpr float SR_STEP0 = 8388608.f;            // 2^23
 constexpr float SR_LEAST = 7.888609052210118e-31f;      // 2^-100: less of a temperature counts as 0
 constexpr int SR_BINS = 1024, SR_LIST = 512, SR_TABLE = 256;
 constexpr int SR_WIDE = 512, SR_NARROW = 128, SR_MOST = 8, SR_TURNS = 17;      // threads; blocks a row and vectors a thread, at most
@@ -206,9 +207,12 @@ __global__ void __launch_bounds__(THREADS, THREADS == SR_WIDE ? 2 : 8) sample_ro
   const double c64 = SR_PER / (double)temperature, m64 = m;
   const float half_m = 0.5f * m, per_half = 2.f * (SR_BINS / SR_REACH) / temperature;      // (by halves: m - v may be more than a float holds)
   const float cut = fmaxf(m - 31.5f * temperature, -3.402823466e38f);      // weights are 0 from here on; -inf is below
-  auto below = [&](float v) { return fmaf(v, -0.5f, half_m) * per_half; };
-  // The step that is nearest (a float past 2^23 has no fraction); of numbers above `cut` those of SR_BINS steps and more weigh nothing.
-  auto step_of = [&](float s) { return __float_as_int(s + 8388608.f) & 0x7fffff; };
+  auto below = [&](float v) { return __fmaf_rn(v, -0.5f, half_m); };
+  // SR_STEP0 and the step that is nearest (a float past 2^23 has no fraction): one rounding of the same product wherever a number's step is asked for, which the compiler may not put together
+  // in another way (with a product rounded by itself in one place and not in another, a number between two steps was counted in one and looked for in the other).  It rises as v falls.  Of numbers
+  // above `cut` those of SR_BINS steps and more weigh nothing.
+  auto step_at = [&](float v) { return __fmaf_rn(below(v), per_half, SR_STEP0); };
+  auto step_of = [&](float at) { return __float_as_int(at) & 0x7fffff; };
   auto weight = [&](float v) { return weight_of((double)v - m64, c64, sh.exps); };      // (of numbers from `cut` on)
   float lowest = cut;                            // kept are numbers from here on
   int turn = 0, sums = 0;
@@ -280,8 +284,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == SR_WIDE ? 2 : 8) sample_ro
       while (most >= 0 && to - from > 1u) {
         const uint32_t step = (to - from - 1u) / 33u + 1u;
         const u64 probe = min((u64)from + (u64)(lane + 1) * step, (u64)to);
-        const float s = below(key_value<T>((uint32_t)probe));
-        const uint32_t in = __ballot_sync(0xffffffffu, s < (float)SR_BINS && step_of(s) <= most);
+        const uint32_t in = __ballot_sync(0xffffffffu, step_at(key_value<T>((uint32_t)probe)) <= SR_STEP0 + most);
         const int at = in != 0u ? __ffs(in) - 1 : 32;
         const u64 above = (u64)from + (u64)at * step;
         if (in != 0u) to = (uint32_t)min(above + step, (u64)to);
@@ -429,7 +432,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == SR_WIDE ? 2 : 8) sample_ro
   auto finish_here = [&](int last, double want) {
     float* const value_here = reinterpret_cast<float*>(&sh.hist[turn][0][0]);      // (zeros that nobody reads)
     int* const place_here = reinterpret_cast<int*>(value_here + HERE);
-    auto in = [&](float v) { return v >= lowest && step_of(below(v)) <= last; };
+    auto in = [&](float v) { return v >= lowest && step_at(v) <= SR_STEP0 + last; };
     int n = 0;
     each(lowest, [&](const float (&x)[N], int) {
 #pragma unroll
@@ -553,8 +556,8 @@ __global__ void __launch_bounds__(THREADS, THREADS == SR_WIDE ? 2 : 8) sample_ro
     each(cut, [&](const float (&x)[N], int) {
 #pragma unroll
       for (int e = 0; e < N; ++e) {
-        const float s = below(x[e]);
-        if (s < SR_BINS - 0.5f) atomicAdd(&hist[step_of(s)], 1u);
+        const float at = step_at(x[e]);
+        if (at < SR_STEP0 + SR_BINS) atomicAdd(&hist[step_of(at)], 1u);
       }
     });
     cluster.sync();
@@ -603,19 +606,19 @@ __global__ void __launch_bounds__(THREADS, THREADS == SR_WIDE ? 2 : 8) sample_ro
   float settled = -INFINITY, least_kept = -INFINITY;      // numbers above `settled` and those of a list are all that is kept
   if (top_p < 1.f) {
     // A step's weights as parts of its middle one, in 13 bits: each off by half of one in 8067, 2^-13.98 (a part is at least exp(-15.6 / 1024)), by 2^-17.4 with
-    // its place in the step (three roundings of a number of 1024, times 0.03), and by 2^-27 with the series: less than 2^-13 together; and a weight, rounded to a whole
+    // its place in the step (two roundings of a number of 1024 and one of what is left, times 0.03), and by 2^-27 with the series: less than 2^-13 together; and a weight, rounded to a whole
     // number, by half of one, the step's middle one too.
     u64 all = 0, none;
     uint32_t* hist = sh.hist[turn][0];
     each(lowest, [&](const float (&x)[N], int) {
 #pragma unroll
       for (int e = 0; e < N; ++e) {
-        const float v = fmaxf(x[e], cut), s = below(v), at = s + 8388608.f, d = (s - (at - 8388608.f)) * (SR_REACH / SR_BINS);
+        const float v = fmaxf(x[e], cut), at = step_at(v), d = __fmaf_rn(below(v), per_half, SR_STEP0 - at) * (SR_REACH / SR_BINS);
         const u64 w = weight(v);
         if (x[e] >= lowest) {
           all += w;
           const float part = fmaf(fmaf(fmaf(d, -1.f / 6, 0.5f), d, -1.f) * d, 8192.f, 8192.f);
-          if (s < SR_BINS - 0.5f) atomicAdd(&hist[__float_as_int(at) & 0x7fffff], (uint32_t)(__float_as_int(part + 8388608.f) & 0x7fffff));
+          if (at < SR_STEP0 + SR_BINS) atomicAdd(&hist[step_of(at)], (uint32_t)(__float_as_int(part + 8388608.f) & 0x7fffff));
         }
       }
     });
