@@ -9,11 +9,12 @@
 // The few numbers of those steps are then compared with one another, on top of the exact sum of what lies above; where they are many (rows of few values), the border is
 // found by counts or exact weights of their keys, 1024 ranges at a time.
 //
-// What bounds it: 301 rows of 100 003 (fp32) under top-p and min-p 253 us, under top-p alone 317, 125 without a border (copying them takes 18): instructions (half of the issue slots)
+// What bounds it: 301 rows of 100 003 (fp32) under top-p and min-p 250 us, under top-p alone 310, 125 without a border (copying them takes 18): instructions (half of the issue slots)
 // and the barriers of a cluster, 1 to 1.5 us each, between phases of 3 to 6 us of exponentials (ten instructions of 64 bits each), two blocks an SM.  One row of 32 000 (bf16): 5.2 us,
 // 7.9 under top-k, 14 under top-p.  On the way (us, 301 rows, top-p and min-p): a block a row and bisection 3334; exact weights in all steps, two dependent additions of 32 bits in shared
 // memory each, 738; steps' weights in parts, and a list of the border's numbers by remote atomics 639, by one's own 435; the exponential by a table, one block that
-// finishes alone and sums by lanes 325; top-p's border not looked for where min-p's is above it 253.
+// finishes alone and sums by lanes 325; top-p's border not looked for where min-p's is above it 253; a number's step by one
+// product 250.
 //
 // A cluster of blocks has a row in its shared memory, read once.
 #include <cooperative_groups.h>
@@ -424,8 +425,8 @@ __global__ void __launch_bounds__(THREADS, THREADS == SR_WIDE ? 2 : 8) sample_ro
 
   // ---- Where few numbers can be kept, the first block finishes alone: those up to `last` steps below m, in the order of the row, HERE at most.  `want`: the weight that top-p
   // has to reach, or less than 0: `top_p` of the weight that top-k leaves.  It compares all of them with one another, and no other barrier of the cluster follows.
-  // us with it / without, top-k 50 and top-k 200 with top-p 0.9: 301 rows of 100 003 (fp32) 165 / 191 and 188 / 318, 16 rows 17.1 / 18.7 and 23 / 32; bf16, one row of
-  // 32 000 (eight blocks) 9.0 / 8.0 and 13.0 / 12.4, 128 rows (two blocks) 17.1 / 14.8 and 23 / 27, 100 of 5000 (one block) 11.4 / 12.3 and 17 / 24: 16-bit numbers,
+  // us with it / without, top-k 50 and top-k 200 with top-p 0.9: 301 rows of 100 003 (fp32) 154 / 179 and 172 / 292, 16 rows 15.4 / 17.6 and 21 / 30; bf16, one row of
+  // 32 000 (eight blocks) 9.0 / 8.0 and 13.0 / 12.6, 128 rows (two blocks) 17.1 / 14.2 and 21 / 26, 100 of 5000 (one block) 11.2 / 11.2 and 16 / 22: 16-bit numbers,
   // whose borders are found in one go, do without it where a row has several blocks, or two and no top-p.
   constexpr int HERE = THREADS == SR_WIDE ? SR_LIST : SR_LIST / 2, EACH = HERE / THREADS;
   const bool alone = sizeof(T) == 4 || C == 1 || (C == 2 && top_p < 1.f);
